@@ -537,6 +537,7 @@ FMLM_DEV bool resolve_work(const fmlm_attn_params& p, const int4* units, int u, 
       m.vbase = (int64_t)b * v_sb + (int64_t)h * v_sh;
     }
   }
+  if (p.flags & FMLM_FLAG_CTX_ONLY) m.n = 0;
   return true;
 }
 
@@ -2879,6 +2880,7 @@ static int check_params(const fmlm_attn_params& p) {
     if (sn < 0 || sn >= kMaxRowStride) return FMLM_E_ARG;
   if (!p.q || !p.o || !p.k || (!(p.flags & FMLM_FLAG_MLA) && !p.v)) return FMLM_E_ARG;
   if ((p.flags & FMLM_FLAG_CAUSAL_SEQ) && !p.cu_seqlens_q) return FMLM_E_ARG;
+  if ((p.flags & FMLM_FLAG_CTX_ONLY) && (p.flags & (FMLM_FLAG_CAUSAL_SEQ | FMLM_FLAG_PREFILL))) return FMLM_E_ARG;
   if (!(p.flags & FMLM_FLAG_PREFILL)) {
     const bool has_ctx = p.cu_seqlens_kv || p.ctx_len > 0;
     if (has_ctx && !p.cu_seqlens_kv && p.ctx_len > 0 && !p.k_ctx) return FMLM_E_ARG;

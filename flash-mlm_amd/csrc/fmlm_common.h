@@ -107,7 +107,7 @@ FMLM_DEV SeqInfo seq_info(const fmlm_attn_params& p, int b) {
     ctx_range(p, ctx_batch_of(p, b), c0, c1);
     s.ctx = max(c1 - c0, 0);
   }
-  s.mainlen = ((p.flags & FMLM_FLAG_CAUSAL_SEQ) && cu) ? s.q0 + L : L;
+  s.mainlen = (p.flags & FMLM_FLAG_CTX_ONLY) ? 0 : ((p.flags & FMLM_FLAG_CAUSAL_SEQ) && cu) ? s.q0 + L : L;
   return s;
 }
 

@@ -1,0 +1,312 @@
+// Filling a paged context: block table and slots of a step's new tokens, and their rows'
+// copy into the pages.
+//
+// Block table.  With old_b tokens cached and new_b to store, request b lacks need_b =
+// ceil((old_b + new_b) / 64) - ceil(old_b / 64) pages and takes them from the free list
+// behind those of the requests before it, so one prefix sum over the requests gives every
+// page, and every token's slot follows from its request's entry of that sum.  The work is a
+// few bytes per token and table entry: what it costs is the launches and the latency of
+// its dependent loads.
+//
+// Append.  A copy of rows; the slot of a token is read once and used for several heads.
+#include "fmlm_common.h"
+
+#include <algorithm>
+
+namespace fmlm {
+
+typedef fmlm_block_table_params BtParams;
+constexpr int kBtThreads = 1024;
+constexpr int kBtFillThreads = 256;
+
+FMLM_DEV int64_t bt_index(const void* a, bool i64, int64_t i) {
+  return i64 ? ((const int64_t*)a)[i] : (int64_t)((const int32_t*)a)[i];
+}
+FMLM_DEV int pages_of(int n) { return (n + FMLM_PAGE_ROWS - 1) / FMLM_PAGE_ROWS; }
+
+// workspace: per request its old length (clamped), the place of its first new page in the
+// free list, the tokens it may store and, with keep, per token its rank among the kept
+struct BtSpace {
+  int32_t *old, *base, *count, *rank;
+};
+__host__ __device__ inline BtSpace bt_space(const BtParams& p) {
+  BtSpace s;
+  s.old = (int32_t*)p.workspace;
+  s.base = s.old + p.B;
+  s.count = s.base + p.B;
+  s.rank = s.count + p.B;
+  return s;
+}
+
+// inclusive sums over the workgroup's threads of two values at once; s holds NT / 64 pairs
+template <int NT>
+FMLM_DEV int2 block_scan(int2 v, int2* s) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int x = __shfl_up(v.x, off), y = __shfl_up(v.y, off);
+    if (lane >= off) {
+      v.x += x;
+      v.y += y;
+    }
+  }
+  if (lane == 63) s[wave] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) {
+    v.x += s[w].x;
+    v.y += s[w].y;
+  }
+  __syncthreads();
+  return v;
+}
+
+// ranks of the kept tokens of sequence b, and their number, by one wave: 64 tokens a step
+FMLM_DEV void bt_rank(const BtParams& p, const BtSpace& w, int b) {
+  const int lane = threadIdx.x & 63;
+  const int c0 = p.cu_seqlens[b], c1 = min(p.cu_seqlens[b + 1], p.T);
+  int n = 0;
+  for (int t = c0; t < c1; t += 64) {
+    const bool k = t + lane < c1 && p.keep[t + lane];
+    const uint64_t m = __builtin_amdgcn_ballot_w64(k);
+    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+    if (t + lane < c1) w.rank[t + lane] = k ? n + before : -1;
+    n += __popcll(m);
+  }
+  if (lane == 0) w.count[b] = n;
+}
+
+// the requests' prefix sums, by one workgroup of kBtThreads threads
+FMLM_DEV void bt_scan(const BtParams& p, const BtSpace& w) {
+  __shared__ int2 part[kBtThreads / 64];
+  __shared__ int2 total;
+  __shared__ int sum[4];  // as summary
+  if (threadIdx.x < 4) sum[threadIdx.x] = 0;
+  __syncthreads();
+  const int cap_in = p.table_in ? min(p.in_pages, p.max_pages) * FMLM_PAGE_ROWS : 0;
+  const int cap_out = p.max_pages * FMLM_PAGE_ROWS;
+  int taken = 0, stored = 0, lacking = 0, bad = 0;  // of this thread's requests
+  int2 carry = make_int2(0, 0);                     // pages, context rows of the requests before
+  for (int b0 = 0; b0 < p.B; b0 += kBtThreads) {
+    const int b = b0 + threadIdx.x;
+    int old = 0, cnt = 0, need = 0, have = 0;
+    if (b < p.B) {
+      const int64_t raw = bt_index(p.old_lens, p.flags & FMLM_BT_OLD_I64, b);
+      old = (int)(raw < 0 ? 0 : raw > cap_in ? cap_in : raw);
+      const int c0 = p.cu_seqlens[b], c1 = min(p.cu_seqlens[b + 1], p.T);
+      cnt = p.keep ? w.count[b] : max(c1 - c0, 0);
+      const bool over = raw != old || cnt > cap_out - old;
+      bad += over;
+      cnt = min(cnt, cap_out - old);
+      have = pages_of(old);
+      need = pages_of(old + cnt) - have;
+    }
+    // the free list: what a request lacks in it, its later tokens cannot be stored in
+    int2 v = block_scan<kBtThreads>(make_int2(need, 0), part);
+    const int base = carry.x + v.x - need;
+    const int got = max(0, min(need, p.n_free - base));
+    if (got < need) cnt = max(0, min(cnt, (have + got) * FMLM_PAGE_ROWS - old));
+    int2 r = block_scan<kBtThreads>(make_int2(0, b < p.B ? old + cnt : 0), part);
+    if (b < p.B) {
+      w.old[b] = old;
+      w.base[b] = base;
+      w.count[b] = cnt;
+      p.new_lens[b] = old + cnt;
+      p.cu_kv[b + 1] = carry.y + r.y;
+      taken += got;
+      lacking += need - got;
+      stored += cnt;
+    }
+    if (threadIdx.x == kBtThreads - 1) total = make_int2(v.x, r.y);
+    __syncthreads();
+    carry.x += total.x;
+    carry.y += total.y;
+    __syncthreads();
+  }
+  atomicAdd(&sum[0], taken);
+  atomicAdd(&sum[1], lacking);
+  atomicAdd(&sum[2], bad);
+  atomicAdd(&sum[3], stored);
+  if (threadIdx.x == 0) p.cu_kv[0] = 0;
+  __syncthreads();
+  if (threadIdx.x < 4) p.summary[threadIdx.x] = sum[threadIdx.x];
+}
+
+// page i of request b, or -1
+FMLM_DEV int bt_page(const BtParams& p, const BtSpace& w, int b, int i) {
+  const int old = w.old[b], have = pages_of(old), all = pages_of(old + w.count[b]);
+  if (i < have) return (int)bt_index(p.table_in, p.flags & FMLM_BT_TABLE_I64, (int64_t)b * p.in_pages + i);
+  if (i >= all) return -1;
+  return (int)bt_index(p.free_pages, p.flags & FMLM_BT_FREE_I64, w.base[b] + i - have);
+}
+
+// table entries and tokens from `first` on, every `step`-th
+FMLM_DEV void bt_fill(const BtParams& p, const BtSpace& w, int64_t first, int64_t step) {
+  const int64_t entries = (int64_t)p.B * p.max_pages;
+  for (int64_t e = first; e < entries; e += step) {
+    const int b = (int)(e / p.max_pages);
+    p.block_table[e] = bt_page(p, w, b, (int)(e - (int64_t)b * p.max_pages));
+  }
+  for (int64_t t = first; t < p.T; t += step) {
+    const uint32_t at = (uint32_t)p.token_indices[t];
+    const int b = min((int)(at / (uint32_t)p.N), p.B - 1), pos = (int)(at - (uint32_t)b * (uint32_t)p.N);
+    const int old = w.old[b], rank = p.keep ? w.rank[t] : pos;
+    int64_t slot = -1;
+    if (rank >= 0 && rank < w.count[b]) {
+      const int a = old + rank, page = bt_page(p, w, b, a / FMLM_PAGE_ROWS);
+      if (page >= 0) slot = (int64_t)page * FMLM_PAGE_ROWS + a % FMLM_PAGE_ROWS;
+    }
+    p.slot_mapping[t] = slot;
+    p.positions[t] = old + pos;
+  }
+}
+
+// all of it in one workgroup
+__global__ __launch_bounds__(kBtThreads) void block_table_small_kernel(const BtParams p) {
+  const BtSpace w = bt_space(p);
+  if (p.keep) {
+    for (int b = threadIdx.x >> 6; b < p.B; b += kBtThreads / 64) bt_rank(p, w, b);
+    __syncthreads();
+  }
+  bt_scan(p, w);
+  __syncthreads();
+  bt_fill(p, w, threadIdx.x, kBtThreads);
+}
+
+__global__ __launch_bounds__(kBtFillThreads) void block_table_rank_kernel(const BtParams p) {
+  const int b = blockIdx.x * (kBtFillThreads / 64) + (threadIdx.x >> 6);
+  if (b < p.B) bt_rank(p, bt_space(p), b);
+}
+__global__ __launch_bounds__(kBtThreads) void block_table_scan_kernel(const BtParams p) { bt_scan(p, bt_space(p)); }
+__global__ __launch_bounds__(kBtFillThreads) void block_table_fill_kernel(const BtParams p) {
+  bt_fill(p, bt_space(p), (int64_t)blockIdx.x * kBtFillThreads + threadIdx.x, (int64_t)gridDim.x * kBtFillThreads);
+}
+
+// One workgroup up to this many table entries and tokens: beyond it the launches of the
+// three kernels cost less than what one workgroup takes for the fill.
+constexpr int64_t kBtSmall = 16384;
+
+static int bt_check(const BtParams& p) {
+  if (p.B < 0 || p.N < 0 || p.T < 0 || p.max_pages < 0 || p.in_pages < 0 || p.n_free < 0) return FMLM_E_ARG;
+  if ((int64_t)p.B * p.N > 0x7fffffff || p.T > (int64_t)p.B * p.N) return FMLM_E_ARG;
+  // lengths are 32-bit
+  if (p.max_pages > 0x7fffffff / FMLM_PAGE_ROWS || p.in_pages > 0x7fffffff / FMLM_PAGE_ROWS) return FMLM_E_ARG;
+  return 0;
+}
+
+// ---------------------------------------------------------------------------
+// Append
+// ---------------------------------------------------------------------------
+struct AppendPagedArgs {
+  fmlm_paged_tensor t[2];
+};
+constexpr int kApThreads = 256;
+constexpr int kApHeads = 4;  // heads per thread
+
+// VB bytes a lane; a row is cpr lanes.  blockIdx.y: chunk of heads, z: tensor
+template <typename V>
+__global__ __launch_bounds__(kApThreads) void paged_append_kernel(const AppendPagedArgs args, int es, int heads, int cpr,
+                                                                  int64_t row_bytes, int T, int N, int layout,
+                                                                  const int64_t* __restrict__ token_indices,
+                                                                  const int64_t* __restrict__ slots, int64_t pool_rows) {
+  const fmlm_paged_tensor& a = args.t[blockIdx.z];
+  const int64_t at = (int64_t)blockIdx.x * kApThreads + threadIdx.x;
+  const int64_t t = at / cpr;
+  if (t >= T) return;
+  const int c = (int)(at - t * cpr);
+  const int64_t slot = slots[t];
+  int64_t off = t * a.s_sn;
+  if (layout == FMLM_LAYOUT_PADDED) {
+    const uint32_t tok = (uint32_t)token_indices[t];
+    const uint32_t b = tok / (uint32_t)N;
+    off = (int64_t)b * a.s_sb + (int64_t)(tok - b * (uint32_t)N) * a.s_sn;
+  }
+  if (slot < 0 || slot >= pool_rows) return;
+  const char* src = (const char*)a.src + off * es + (int64_t)c * sizeof(V);
+  char* dst = (char*)a.pool + slot * row_bytes + (int64_t)c * sizeof(V);
+  const int64_t ss = a.s_sh * es, ds = pool_rows * row_bytes;
+  const int h0 = blockIdx.y * kApHeads;
+  V v[kApHeads];
+#pragma unroll
+  for (int u = 0; u < kApHeads; ++u)
+    if (h0 + u < heads) v[u] = *(const V*)(src + (h0 + u) * ss);
+#pragma unroll
+  for (int u = 0; u < kApHeads; ++u)
+    if (h0 + u < heads) *(V*)(dst + (h0 + u) * ds) = v[u];
+}
+
+}  // namespace fmlm
+
+using namespace fmlm;
+
+extern "C" int fmlm_block_table_params_size(void) { return (int)sizeof(fmlm_block_table_params); }
+
+extern "C" int64_t fmlm_block_table_workspace_bytes(const fmlm_block_table_params* pp) {
+  if (!pp) return FMLM_E_ARG;
+  const int rc = bt_check(*pp);
+  if (rc) return rc;
+  return 4 * (3 * (int64_t)pp->B + (pp->keep ? pp->T : 0));
+}
+
+extern "C" int fmlm_block_table(const fmlm_block_table_params* pp, void* stream) {
+  if (!pp) return FMLM_E_ARG;
+  const BtParams& p = *pp;
+  const int64_t need = fmlm_block_table_workspace_bytes(pp);
+  if (need < 0) return (int)need;
+  if (!p.cu_kv || !p.summary) return FMLM_E_ARG;
+  if (p.B > 0 && (!p.old_lens || !p.cu_seqlens || !p.new_lens)) return FMLM_E_ARG;
+  if (p.T > 0 && (!p.token_indices || !p.slot_mapping || !p.positions)) return FMLM_E_ARG;
+  if (((int64_t)p.B * p.max_pages > 0 && !p.block_table) || (p.n_free > 0 && !p.free_pages)) return FMLM_E_ARG;
+  if (need > 0 && (!p.workspace || p.workspace_bytes < need)) return FMLM_E_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t work = std::max<int64_t>((int64_t)p.B * p.max_pages, p.T);
+  if (work + p.B <= kBtSmall) {
+    hipLaunchKernelGGL(block_table_small_kernel, dim3(1), dim3(kBtThreads), 0, s, p);
+    return launch_status();
+  }
+  if (p.keep) {
+    hipLaunchKernelGGL(block_table_rank_kernel, dim3((p.B + 3) / 4), dim3(kBtFillThreads), 0, s, p);
+  }
+  hipLaunchKernelGGL(block_table_scan_kernel, dim3(1), dim3(kBtThreads), 0, s, p);
+  const unsigned blocks = (unsigned)std::min<int64_t>((work + kBtFillThreads - 1) / kBtFillThreads, 4096);
+  hipLaunchKernelGGL(block_table_fill_kernel, dim3(blocks), dim3(kBtFillThreads), 0, s, p);
+  return launch_status();
+}
+
+template <typename V>
+static int paged_append(const fmlm_paged_tensor* tensors, int n, int es, int heads, int64_t row_bytes, int T, int N,
+                        int layout, const int64_t* token_indices, const int64_t* slots, int64_t pool_rows,
+                        hipStream_t s) {
+  AppendPagedArgs args{};
+  for (int i = 0; i < n; ++i) args.t[i] = tensors[i];
+  const int64_t cpr = row_bytes / (int64_t)sizeof(V), blocks = (cpr * T + kApThreads - 1) / kApThreads;
+  if (blocks > 0x7fffffff || cpr > 0x7fffffff) return FMLM_E_ARG;
+  hipLaunchKernelGGL(paged_append_kernel<V>, dim3((unsigned)blocks, (heads + kApHeads - 1) / kApHeads, n),
+                     dim3(kApThreads), 0, s, args, es, heads, (int)cpr, row_bytes, T, N, layout, token_indices, slots,
+                     pool_rows);
+  return launch_status();
+}
+
+extern "C" int fmlm_paged_append(const fmlm_paged_tensor* tensors, int32_t n_tensors, int32_t elem_bytes, int32_t heads,
+                                 int32_t D, int32_t T, int32_t N, int32_t layout, const int64_t* token_indices,
+                                 const int64_t* slots, int64_t pool_rows, void* stream) {
+  if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4 && elem_bytes != 8) return FMLM_E_DTYPE;
+  if (!tensors || n_tensors < 1 || n_tensors > 2 || heads < 0 || D < 1 || T < 0 || pool_rows < 0) return FMLM_E_ARG;
+  if (layout != FMLM_LAYOUT_PADDED && layout != FMLM_LAYOUT_PACKED) return FMLM_E_ARG;
+  if (heads > 65535 * kApHeads) return FMLM_E_ARG;
+  if (T == 0 || heads == 0 || pool_rows == 0) return 0;
+  if (!slots || (layout == FMLM_LAYOUT_PADDED && (!token_indices || N < 1))) return FMLM_E_ARG;
+  const int64_t row_bytes = (int64_t)D * elem_bytes;
+  uint64_t all = (uint64_t)row_bytes;  // low bits common to every address
+  for (int i = 0; i < n_tensors; ++i) {
+    const fmlm_paged_tensor& t = tensors[i];
+    if (!t.src || !t.pool) return FMLM_E_ARG;
+    all |= (uint64_t)t.src | (uint64_t)t.pool | (uint64_t)(t.s_sb * elem_bytes) | (uint64_t)(t.s_sh * elem_bytes) |
+           (uint64_t)(t.s_sn * elem_bytes);
+  }
+  if (all % elem_bytes) return FMLM_E_ALIGN;
+  hipStream_t s = (hipStream_t)stream;
+  if (all % 16 == 0) return paged_append<u32x4>(tensors, n_tensors, elem_bytes, heads, row_bytes, T, N, layout, token_indices, slots, pool_rows, s);
+  if (all % 4 == 0) return paged_append<uint32_t>(tensors, n_tensors, elem_bytes, heads, row_bytes, T, N, layout, token_indices, slots, pool_rows, s);
+  if (all % 2 == 0) return paged_append<uint16_t>(tensors, n_tensors, elem_bytes, heads, row_bytes, T, N, layout, token_indices, slots, pool_rows, s);
+  return paged_append<uint8_t>(tensors, n_tensors, elem_bytes, heads, row_bytes, T, N, layout, token_indices, slots, pool_rows, s);
+}

@@ -1,0 +1,413 @@
+// Attention of drafted trees over a cached context.
+//
+// Query i of a sequence attends to the sequence's context and to those tokens j of its own
+// draft that are i or an ancestor of i:
+//   o_i = (sum_ctx e^{z} v + sum_{j in anc(i)} e^{z_ij} v_j) / (both sums of e^z),
+// z = scale q.k.  The context part is the forward kernels' ordinary work (they read every
+// key once, at the rate of a copy); it leaves o_c = its own softmax's output and l_c =
+// log2(sum 2^z) per row.  The tree kernel here computes m = max z and l = sum 2^(z - m) over
+// the ancestors and writes
+//   (2^(l_c - M) o_c + 2^(m - M) sum 2^(z - m) v) / (2^(l_c - M) + 2^(m - M) l),  M = max(l_c, m).
+// o_c is read as the attention kernel rounded it, to the input type: one rounding (half a
+// step of o_c) besides the last one, for half of the traffic of a 32-bit copy.
+//
+// A draft has at most 256 tokens, so its keys are few beside the context's: the kernel is
+// bound by latency, not by bandwidth or products.  One wave takes 16 rows of one head, so
+// that a few rows give many waves; steps of 32 keys in which no row of the wave has an
+// ancestor are skipped (an ancestor precedes its descendants, so the later ones).
+#include "fmlm_common.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace fmlm {
+
+// ---------------------------------------------------------------------------
+// Ancestor masks: one workgroup per sequence, thread i is token i.  After round k a token
+// knows its nearest 2^k ancestors, and the next one beyond them.
+// ---------------------------------------------------------------------------
+constexpr int kTreeWords = FMLM_MAX_TREE / 64;
+
+__global__ __launch_bounds__(FMLM_MAX_TREE) void tree_mask_kernel(const void* parents, int parents_i64,
+                                                                  const int32_t* __restrict__ cu, int N, int T, int words,
+                                                                  const void* ctx_lens, int ctx_i64,
+                                                                  uint64_t* __restrict__ mask,
+                                                                  int32_t* __restrict__ positions, int32_t* n_bad) {
+  __shared__ uint64_t s_bits[FMLM_MAX_TREE][kTreeWords];
+  __shared__ int s_next[FMLM_MAX_TREE];
+  const int b = blockIdx.x, i = threadIdx.x;
+  const int c0 = cu[b], n = max(0, min(min(cu[b + 1], T) - c0, min(N, FMLM_MAX_TREE)));
+  uint64_t bits[kTreeWords];
+  int next = -1;
+  if (i < n) {
+    const int64_t up = parents_i64 ? ((const int64_t*)parents)[c0 + i] : (int64_t)((const int32_t*)parents)[c0 + i];
+    if (up >= 0 && up < i) next = (int)up;
+    else if (up != -1 && n_bad) atomicAdd(n_bad, 1);
+#pragma unroll
+    for (int w = 0; w < kTreeWords; ++w) bits[w] = i / 64 == w ? 1ull << (i % 64) : 0;
+  }
+  for (int span = 1; span < n; span *= 2) {
+    if (i < n) {
+#pragma unroll
+      for (int w = 0; w < kTreeWords; ++w) s_bits[i][w] = bits[w];
+      s_next[i] = next;
+    }
+    __syncthreads();
+    if (i < n && next >= 0) {
+#pragma unroll
+      for (int w = 0; w < kTreeWords; ++w) bits[w] |= s_bits[next][w];
+      next = s_next[next];
+    }
+    __syncthreads();
+  }
+  if (i < n) {
+    int seen = 0;
+#pragma unroll
+    for (int w = 0; w < kTreeWords; ++w) {
+      if (w < words) mask[(int64_t)(c0 + i) * words + w] = bits[w];
+      seen += __popcll(bits[w]);
+    }
+    for (int w = kTreeWords; w < words; ++w) mask[(int64_t)(c0 + i) * words + w] = 0;
+    const int64_t ctx = !ctx_lens ? 0 : ctx_i64 ? ((const int64_t*)ctx_lens)[b] : (int64_t)((const int32_t*)ctx_lens)[b];
+    positions[c0 + i] = (int)ctx + seen - 1;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// What the two tree kernels share: the sequence, and the context's part of a row.
+// ---------------------------------------------------------------------------
+struct TreeSeq {
+  int q0, len;
+  bool has_ctx;
+  int64_t k0, v0;  // element offsets of the sequence's first main key and value of the head
+  int64_t k_sn, v_sn;
+};
+FMLM_DEV TreeSeq tree_seq(const fmlm_attn_params& p, int b, int h) {
+  const SeqInfo si = seq_info(p, b);
+  TreeSeq s;
+  s.q0 = si.q0;
+  s.len = min(si.len, FMLM_MAX_TREE);
+  s.has_ctx = si.ctx > 0;
+  const bool mla = p.flags & FMLM_FLAG_MLA, packed = p.kv_layout == FMLM_LAYOUT_PACKED;
+  const int64_t v_sb = mla ? p.k_sb : p.v_sb, v_sh = mla ? p.k_sh : p.v_sh;
+  s.k_sn = p.k_sn;
+  s.v_sn = mla ? p.k_sn : p.v_sn;
+  s.k0 = (packed ? (int64_t)s.q0 * s.k_sn : (int64_t)b * p.k_sb) + (int64_t)h * p.k_sh;
+  s.v0 = (packed ? (int64_t)s.q0 * s.v_sn : (int64_t)b * v_sb) + (int64_t)h * v_sh;
+  return s;
+}
+FMLM_DEV int64_t tree_row(int layout, int b, int h, int q0, int pos, int64_t sb, int64_t sh, int64_t sn) {
+  return layout == FMLM_LAYOUT_PACKED ? (int64_t)h * sh + (int64_t)(q0 + pos) * sn
+                                      : (int64_t)b * sb + (int64_t)h * sh + (int64_t)pos * sn;
+}
+// the weights of the two parts of a row, already divided by their sum (m, l: the tree's)
+struct TreeJoin {
+  float wc, wt;
+};
+FMLM_DEV TreeJoin tree_join(const fmlm_attn_params& p, const TreeSeq& s, int h, int pos, float m, float l) {
+  TreeJoin j{0.f, 0.f};
+  if (!s.has_ctx) {
+    if (l != 0.f) j.wt = 1.f / l;  // (NaN too; no key at all: 0)
+    return j;
+  }
+  const float lc = p.lse[(int64_t)h * p.total_q + s.q0 + pos];
+  const float top = vmax(lc, m);
+  j.wc = fast_exp2(lc - top);  // an infinite top: NaN, as inf - inf is
+  j.wt = m == -INFINITY ? 0.f : fast_exp2(m - top);
+  const float inv = 1.f / fmaf(j.wt, l, j.wc);
+  j.wc *= inv;
+  j.wt *= inv;
+  return j;
+}
+
+// ---------------------------------------------------------------------------
+// bf16 / fp16.  As in the forward kernels S^T = K Q^T and O^T = V^T P^T, so that a lane
+// (q + 16 g) holds keys 4g .. 4g+3 of query q and then columns 16 db + 4g .. of its output.
+// K fragments come straight from memory (a lane's 16 bytes of a key row are its operand);
+// V passes through LDS, whose transposing read makes its operand.  P is rounded to the input
+// type for the product, and its row sum is taken of the rounded values.
+// ---------------------------------------------------------------------------
+template <typename T, int D>
+__global__ __launch_bounds__(64) void attn_tree_kernel(const fmlm_attn_params p, const uint64_t* __restrict__ mask,
+                                                       int words) {
+  typedef typename Mfma<T>::v8 v8;
+  constexpr int KC = (D + 31) / 32, NDB = D / 16, BK = 32;
+  constexpr int PITCH = D * 2 + 16;  // 16 bytes apart: a column's rows fall into different banks
+  constexpr int CPR = D / 8, NL = BK * CPR / 64;
+  __shared__ __align__(16) char vt[BK * PITCH];
+  const int b = blockIdx.z, h = blockIdx.y, r0 = blockIdx.x * 16;
+  const TreeSeq s = tree_seq(p, b, h);
+  if (r0 >= s.len) return;
+  const int lane = threadIdx.x, l16 = lane & 15, g = lane >> 4;
+  const int pos = r0 + l16;
+  const bool ok = pos < s.len;
+  const float c = p.scale * kLog2e;
+  const T* const kp = (const T*)p.k + s.k0;
+  const T* const vp = (const T*)((p.flags & FMLM_FLAG_MLA) ? p.k : p.v) + s.v0;
+
+  v8 qf[KC];
+  {
+    const T* q = (const T*)p.q + tree_row(p.q_layout, b, h, s.q0, ok ? pos : s.len - 1, p.q_sb, p.q_sh, p.q_sn);
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) qf[kc] = kc * 32 + g * 8 < D ? *(const v8*)(q + kc * 32 + g * 8) : v8{};
+  }
+  f32x4 o[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+
+  const uint32_t vaddr = lds_addr(vt) + (4 * g + (l16 >> 2)) * PITCH + 8 * (l16 & 3);
+  for (int j0 = 0; j0 < s.len; j0 += BK) {
+    uint32_t seen = 0;  // keys j0 + bit that the lane's row attends to
+    if (ok && j0 / 64 < words) seen = (uint32_t)(mask[(int64_t)(s.q0 + pos) * words + j0 / 64] >> (j0 % 64));
+    if (s.len - j0 < BK) seen &= (1u << (s.len - j0)) - 1u;
+    if (!__builtin_amdgcn_ballot_w64(seen != 0)) continue;
+    // ---- V tile: rows past the sequence are zero, and so are rows with an element that is
+    // not finite: 0 times it would not be 0 in the rows that do not see it (see below)
+    uint32_t bad = 0;
+    {
+      u32x4 v[NL > 0 ? NL : 1];
+#pragma unroll
+      for (int n = 0; n < NL; ++n) {
+        const int at = n * 64 + lane, row = at / CPR;
+        v[n] = u32x4{0u, 0u, 0u, 0u};
+        if (j0 + row < s.len) v[n] = *(const u32x4*)(vp + (int64_t)(j0 + row) * s.v_sn + (at % CPR) * 8);
+      }
+      constexpr uint32_t E = std::is_same<T, bf16>::value ? 0x7f80u : 0x7c00u;  // exponent of inf and NaN
+      uint32_t mine = 0;
+#pragma unroll
+      for (int n = 0; n < NL; ++n) {
+        const int at = n * 64 + lane, row = at / CPR;
+        bool inf = false;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) inf |= (v[n][w] & E) == E || (v[n][w] >> 16 & E) == E;
+        if (inf) mine |= 1u << row;
+        *(u32x4*)(vt + row * PITCH + (at % CPR) * 16) = v[n];
+      }
+      if (__builtin_amdgcn_ballot_w64(mine != 0)) {
+        for (int r = 0; r < BK; ++r)
+          if (__builtin_amdgcn_ballot_w64(mine >> r & 1)) bad |= 1u << r;
+#pragma unroll
+        for (int n = 0; n < NL; ++n) {
+          const int at = n * 64 + lane, row = at / CPR;
+          if (bad >> row & 1) *(u32x4*)(vt + row * PITCH + (at % CPR) * 16) = u32x4{0u, 0u, 0u, 0u};
+        }
+      }
+    }
+    // ---- scores
+    f32x4 sc[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const T* k = kp + (int64_t)min(j0 + kb * 16 + l16, s.len - 1) * s.k_sn;
+      sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc) {
+        const v8 a = kc * 32 + g * 8 < D ? *(const v8*)(k + kc * 32 + g * 8) : v8{};
+        sc[kb] = Mfma<T>::run(a, qf[kc], sc[kb]);
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sc[kb][r] = (seen >> (kb * 16 + 4 * g + r) & 1) ? sc[kb][r] * c : -INFINITY;
+        mx = vmax(mx, sc[kb][r]);
+      }
+    const float m_new = vmax(m, lane_max_xor16_32(mx));
+    const float ref = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = fast_exp2(m - ref);
+    m = m_new;
+    v8 pf;
+    float sum = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const T x = (T)fast_exp2(sc[kb][r] - ref);
+        pf[kb * 4 + r] = x;
+        sum += (float)x;
+      }
+    l = l * alpha + sum;
+    wait_reads();  // the tile is in LDS (one wave: no barrier)
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      const s16x4 lo = lds_read_tr16_at(vaddr + db * 32), hi = lds_read_tr16_at(vaddr + db * 32 + 16 * PITCH);
+      const v8 a = __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      o[db] = Mfma<T>::run(a, pf, o[db] * alpha);
+    }
+    // ---- values that are not finite: by the rows that see them alone
+    for (uint32_t left = bad; left; left &= left - 1) {
+      const int j = __builtin_ctz(left), from = l16 + 16 * ((j & 15) >> 2);
+      float x = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e == (j >> 4) * 4 + (j & 3)) x = (float)pf[e];
+      x = __shfl(x, from);
+      if (seen >> j & 1) {
+        const T* v = vp + (int64_t)(j0 + j) * s.v_sn + 4 * g;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[db][r] = fmaf(x, (float)v[db * 16 + r], o[db][r]);
+      }
+    }
+    wait_reads();  // the next tile may overwrite this one
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (!ok) return;
+  const TreeJoin j = tree_join(p, s, h, pos, m, l);
+  T* const dst = (T*)p.o + tree_row(p.o_layout, b, h, s.q0, pos, p.o_sb, p.o_sh, p.o_sn) + 4 * g;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) {
+    f32x4 x = o[db] * j.wt;
+    if (s.has_ctx) {
+      const u32x2 raw = *(const u32x2*)(dst + db * 16);
+      T oc[4];
+      __builtin_memcpy(oc, &raw, 8);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = fmaf(j.wc, (float)oc[r], x[r]);
+    }
+    T y[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
+    u32x2 raw;
+    __builtin_memcpy(&raw, y, 8);
+    *(u32x2*)(dst + db * 16) = raw;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// fp32: one wave per row.  Lane j scores key j of a step of 64 keys; then the row's keys are
+// taken one by one, a lane holding D / 64 columns (the first D lanes one each below 64).
+// Keys that the row does not see are not read.
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(64) void attn_tree_f32_kernel(const fmlm_attn_params p, const uint64_t* __restrict__ mask,
+                                                           int words) {
+  constexpr int NC = (D + 63) / 64;
+  __shared__ __align__(16) float qs[D];
+  const int b = blockIdx.z, h = blockIdx.y, pos = blockIdx.x, lane = threadIdx.x;
+  const TreeSeq s = tree_seq(p, b, h);
+  if (pos >= s.len) return;
+  const float c = p.scale * kLog2e;
+  const float* const q = (const float*)p.q + tree_row(p.q_layout, b, h, s.q0, pos, p.q_sb, p.q_sh, p.q_sn);
+  const float* const kp = (const float*)p.k + s.k0;
+  const float* const vp = (const float*)((p.flags & FMLM_FLAG_MLA) ? p.k : p.v) + s.v0;
+  for (int d = lane; d < D; d += 64) qs[d] = q[d];
+  __syncthreads();
+  float o[NC];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) o[i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  for (int w = 0; w < words && w * 64 < s.len; ++w) {
+    uint64_t seen = mask[(int64_t)(s.q0 + pos) * words + w];
+    if (s.len - w * 64 < 64) seen &= (1ull << (s.len - w * 64)) - 1ull;
+    if (!seen) continue;
+    float z = -INFINITY;
+    if (seen >> lane & 1) {
+      const float* k = kp + (int64_t)(w * 64 + lane) * s.k_sn;
+      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int d = 0; d < D; d += 4) acc += *(const f32x4*)(qs + d) * *(const f32x4*)(k + d);
+      z = ((acc[0] + acc[1]) + (acc[2] + acc[3])) * c;
+    }
+    float mx = z;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) mx = vmax(mx, __shfl_xor(mx, off));
+    const float m_new = vmax(m, mx);
+    const float ref = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = fast_exp2(m - ref);
+    const float x = fast_exp2(z - ref);
+    m = m_new;
+    l = l * alpha + x;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) o[i] *= alpha;
+    for (uint64_t left = seen; left; left &= left - 1) {
+      const int j = __builtin_ctzll(left);
+      const float pj = __shfl(x, j);
+      const float* v = vp + (int64_t)(w * 64 + j) * s.v_sn;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (D >= 64 || lane < D) o[i] = fmaf(pj, v[lane + 64 * i], o[i]);
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off);
+  const TreeJoin j = tree_join(p, s, h, pos, m, l);
+  float* const dst = (float*)p.o + tree_row(p.o_layout, b, h, s.q0, pos, p.o_sb, p.o_sh, p.o_sn);
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+    if (D >= 64 || lane < D) {
+      float x = o[i] * j.wt;
+      if (s.has_ctx) x = fmaf(j.wc, dst[lane + 64 * i], x);
+      dst[lane + 64 * i] = x;
+    }
+}
+
+template <typename T>
+static int launch_tree(const fmlm_attn_params& p, const uint64_t* mask, int words, int longest, hipStream_t s) {
+  const dim3 grid((unsigned)((longest + 15) / 16), (unsigned)p.H, (unsigned)p.B);
+#define FMLM_TREE(DD) \
+  case DD: hipLaunchKernelGGL((attn_tree_kernel<T, DD>), grid, dim3(64), 0, s, p, mask, words); break;
+  switch (p.D) {
+    FMLM_TREE(16) FMLM_TREE(32) FMLM_TREE(64) FMLM_TREE(128) FMLM_TREE(256) FMLM_TREE(512)
+    default: return FMLM_E_HEAD_DIM;
+  }
+#undef FMLM_TREE
+  return launch_status();
+}
+static int launch_tree_f32(const fmlm_attn_params& p, const uint64_t* mask, int words, int longest, hipStream_t s) {
+  const dim3 grid((unsigned)longest, (unsigned)p.H, (unsigned)p.B);
+#define FMLM_TREE(DD) \
+  case DD: hipLaunchKernelGGL((attn_tree_f32_kernel<DD>), grid, dim3(64), 0, s, p, mask, words); break;
+  switch (p.D) {
+    FMLM_TREE(16) FMLM_TREE(32) FMLM_TREE(64) FMLM_TREE(128) FMLM_TREE(256) FMLM_TREE(512)
+    default: return FMLM_E_HEAD_DIM;
+  }
+#undef FMLM_TREE
+  return launch_status();
+}
+
+}  // namespace fmlm
+
+using namespace fmlm;
+
+extern "C" int fmlm_tree_mask(const void* parents, int32_t parents_i64, const int32_t* cu_seqlens, int32_t B, int32_t N,
+                              int32_t T, int32_t words, const void* ctx_lens, int32_t ctx_lens_i64, uint64_t* mask,
+                              int32_t* positions, int32_t* n_bad, void* stream) {
+  if (B < 0 || N < 0 || T < 0 || words < 0 || N > FMLM_MAX_TREE || (int64_t)words * 64 < N) return FMLM_E_ARG;
+  if (B == 0 || T == 0) return 0;
+  if (!parents || !cu_seqlens || !mask || !positions) return FMLM_E_ARG;
+  const int threads = std::max(64, (N + 63) / 64 * 64);
+  hipLaunchKernelGGL(tree_mask_kernel, dim3(B), dim3(threads), 0, (hipStream_t)stream, parents, parents_i64, cu_seqlens,
+                     N, T, words, ctx_lens, ctx_lens_i64, mask, positions, n_bad);
+  return launch_status();
+}
+
+extern "C" int fmlm_attn_tree_fwd(const fmlm_attn_params* pp, const uint64_t* mask, int32_t words, void* stream) {
+  if (!pp) return FMLM_E_ARG;
+  const fmlm_attn_params& p = *pp;
+  if (!(p.flags & FMLM_FLAG_CTX_ONLY) || (p.flags & (FMLM_FLAG_PREFILL | FMLM_FLAG_CAUSAL_SEQ))) return FMLM_E_ARG;
+  if (!p.cu_seqlens_q || !p.lse || p.N < 0 || p.N > FMLM_MAX_TREE || p.H > 65535 || p.B > 65535) return FMLM_E_ARG;
+  // packed inputs without a padded length: their sequences may be as long as all of them
+  const int longest = p.N > 0 ? std::min(p.N, p.total_q) : std::min(p.total_q, FMLM_MAX_TREE);
+  if (p.B > 0 && p.H > 0 && longest > 0 && (!mask || (int64_t)words * 64 < longest)) return FMLM_E_ARG;
+  const int es = elem_size(p.dtype);
+  if (!es) return FMLM_E_DTYPE;
+  for (int64_t st : {p.q_sb, p.q_sh, p.q_sn, p.k_sb, p.k_sh, p.k_sn, p.o_sb, p.o_sh, p.o_sn})
+    if ((st * es) % 16) return FMLM_E_ALIGN;
+  if (!(p.flags & FMLM_FLAG_MLA) && ((p.v_sb * es) % 16 || (p.v_sh * es) % 16 || (p.v_sn * es) % 16)) return FMLM_E_ALIGN;
+  if (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.o) & 15) return FMLM_E_ALIGN;
+  if (!(p.flags & FMLM_FLAG_MLA) && ((uintptr_t)p.v & 15)) return FMLM_E_ALIGN;
+  const int rc = fmlm_attn_fwd(pp, stream);  // checks the rest of p
+  if (rc) return rc;
+  if (p.B == 0 || p.H == 0 || longest <= 0) return 0;
+  hipStream_t s = (hipStream_t)stream;
+  switch (p.dtype) {
+    case FMLM_DTYPE_BF16: return launch_tree<bf16>(p, mask, words, longest, s);
+    case FMLM_DTYPE_F16: return launch_tree<f16>(p, mask, words, longest, s);
+    default: return launch_tree_f32(p, mask, words, longest, s);
+  }
+}

@@ -14,6 +14,9 @@ from flash_mlm.host.host import (
     flash_attn_mlm_precompressed,
 )
 from flash_mlm.host.host_utils import build_pack_metadata, unpack_from_kernel
+from flash_mlm.host.norm_rope import qk_norm_rope
+from flash_mlm.host.paged import PagedMetadata, build_block_table
+from flash_mlm.host.tree import TreeMetadata, build_tree_metadata, flash_attn_mlm_tree
 
 __version__ = "0.1.0"
 
@@ -26,4 +29,10 @@ __all__ = [
     "flash_attn_mlm",
     "flash_attn_mlm_compressed",
     "flash_attn_mlm_precompressed",
+    "qk_norm_rope",
+    "PagedMetadata",
+    "build_block_table",
+    "TreeMetadata",
+    "build_tree_metadata",
+    "flash_attn_mlm_tree",
 ]

@@ -27,6 +27,18 @@ FLAG_PREFILL = 2
 FLAG_CAUSAL_SEQ = 4
 FLAG_NOSPLIT = 8
 FLAG_OWN_RECORDS = 16
+FLAG_CTX_ONLY = 32
+
+NR_NORM = 1
+NR_INTERLEAVED = 2
+NR_POSITIONS_I64 = 4
+NR_OFFSETS_I64 = 8
+
+BT_OLD_I64 = 1
+BT_TABLE_I64 = 2
+BT_FREE_I64 = 4
+
+MAX_TREE = 256
 
 LAYOUT_PADDED = 0
 LAYOUT_PACKED = 1
@@ -138,6 +150,67 @@ class AttnGrads(ctypes.Structure):
     ]
 
 
+class NormRopeTensor(ctypes.Structure):
+    """Mirror of fmlm_norm_rope_tensor (include/flash_mlm_hip.h)."""
+
+    _fields_ = [
+        (name if s == "" else f"{name}{s}", _c_ptr if s == "" else _c_i64)
+        for name in ("x", "y", "dy")
+        for s in ("", "_sb", "_sh", "_sn")
+    ] + [
+        ("weight", _c_ptr),
+        ("dweight", _c_ptr),
+        ("w_sh", _c_i64),
+        ("heads", _c_i32),
+        ("reserved", _c_i32),
+    ]
+
+
+class NormRopeParams(ctypes.Structure):
+    """Mirror of fmlm_norm_rope_params (include/flash_mlm_hip.h)."""
+
+    _fields_ = [
+        ("dtype", _c_i32),
+        ("w_dtype", _c_i32),
+        ("flags", _c_i32),
+        ("layout", _c_i32),
+        ("B", _c_i32),
+        ("N", _c_i32),
+        ("D", _c_i32),
+        ("rotary_dim", _c_i32),
+        ("rows", _c_i64),
+        ("table_rows", _c_i64),
+        ("eps", ctypes.c_float),
+        ("reserved", _c_i32),
+        ("cos", _c_ptr),
+        ("sin", _c_ptr),
+        ("cu_seqlens", _c_ptr),
+        ("token_indices", _c_ptr),
+        ("positions", _c_ptr),
+        ("offsets", _c_ptr),
+        ("q", NormRopeTensor),
+        ("k", NormRopeTensor),
+        ("workspace", _c_ptr),
+        ("workspace_bytes", _c_i64),
+    ]
+
+
+class BlockTableParams(ctypes.Structure):
+    """Mirror of fmlm_block_table_params (include/flash_mlm_hip.h)."""
+
+    _fields_ = [(n, _c_i32) for n in ("flags", "B", "N", "T", "max_pages", "in_pages", "n_free", "reserved")] + [
+        (n, _c_ptr)
+        for n in ("old_lens", "cu_seqlens", "token_indices", "keep", "table_in", "free_pages", "block_table",
+                  "slot_mapping", "positions", "new_lens", "cu_kv", "summary", "workspace")
+    ] + [("workspace_bytes", _c_i64)]
+
+
+class PagedTensor(ctypes.Structure):
+    """Mirror of fmlm_paged_tensor (include/flash_mlm_hip.h)."""
+
+    _fields_ = [("src", _c_ptr), ("s_sb", _c_i64), ("s_sh", _c_i64), ("s_sn", _c_i64), ("pool", _c_ptr)]
+
+
 # (name, restype, argtypes) of every exported entry point
 SIGNATURES = {
     "fmlm_abi_version": (ctypes.c_int, []),
@@ -174,6 +247,23 @@ SIGNATURES = {
     "fmlm_attn_bwd_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(AttnParams)]),
     "fmlm_attn_bwd": (ctypes.c_int, [ctypes.POINTER(AttnParams), ctypes.POINTER(AttnGrads), _c_ptr]),
     "fmlm_attn_bwd_fill": (ctypes.c_int, [ctypes.POINTER(AttnParams), ctypes.POINTER(AttnGrads), _c_ptr]),
+    "fmlm_norm_rope_params_size": (ctypes.c_int, []),
+    "fmlm_norm_rope": (ctypes.c_int, [ctypes.POINTER(NormRopeParams), _c_ptr]),
+    "fmlm_norm_rope_bwd_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(NormRopeParams)]),
+    "fmlm_norm_rope_bwd": (ctypes.c_int, [ctypes.POINTER(NormRopeParams), _c_ptr]),
+    "fmlm_block_table_params_size": (ctypes.c_int, []),
+    "fmlm_block_table_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(BlockTableParams)]),
+    "fmlm_block_table": (ctypes.c_int, [ctypes.POINTER(BlockTableParams), _c_ptr]),
+    "fmlm_paged_append": (
+        ctypes.c_int,
+        [ctypes.POINTER(PagedTensor), _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_i64,
+         _c_ptr],
+    ),
+    "fmlm_tree_mask": (
+        ctypes.c_int,
+        [_c_ptr, _c_i32, _c_ptr, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr, _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
+    ),
+    "fmlm_attn_tree_fwd": (ctypes.c_int, [ctypes.POINTER(AttnParams), _c_ptr, _c_i32, _c_ptr]),
 }
 
 _lock = threading.Lock()
@@ -210,6 +300,10 @@ def load() -> ctypes.CDLL:
             raise RuntimeError("fmlm_pack_tensor layout mismatch between library and binding")
         if lib.fmlm_attn_grads_size() != ctypes.sizeof(AttnGrads):
             raise RuntimeError("fmlm_attn_grads layout mismatch between library and binding")
+        if lib.fmlm_norm_rope_params_size() != ctypes.sizeof(NormRopeParams):
+            raise RuntimeError("fmlm_norm_rope_params layout mismatch between library and binding")
+        if lib.fmlm_block_table_params_size() != ctypes.sizeof(BlockTableParams):
+            raise RuntimeError("fmlm_block_table_params layout mismatch between library and binding")
         _lib = lib
         return lib
 

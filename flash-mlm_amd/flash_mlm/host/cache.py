@@ -9,9 +9,13 @@ fields, the same lookup keys, the same ValueError messages, and the same
 
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
+from typing import TYPE_CHECKING
 
 import torch
+
+if TYPE_CHECKING:
+    from flash_mlm.host.paged import PagedMetadata
 
 
 @dataclass
@@ -415,6 +419,67 @@ class InferenceCache:
             head_dim=d,
             dtype=entry.dtype,
             device=dev,
+        )
+
+    def append_paged_kv_cache(
+        self,
+        layer_id: int | str,
+        *,
+        k: torch.Tensor,
+        v: torch.Tensor | None = None,
+        q_meta: PackMetadata,
+        plan: PagedMetadata,
+    ) -> None:
+        """Store new keys and values in ``layer_id``'s paged context.
+
+        This is an extension: the reference's roadmap lists paged KV (README.md:41).
+
+        ``k`` / ``v`` are the new tokens as the attention entry points take them: padded
+        [B, H, N, D] (MLA: head 0 of k is stored, ``v`` is ignored) or packed
+        [H_kv * T, D]; ``q_meta`` describes them and ``plan`` (:func:`build_block_table`, shared
+        by all layers of a step) says where they go.  Tokens with slot -1, or one outside the
+        pool, are not stored.  The rows are written into the pool in place by one HIP launch,
+        stream-ordered, without a gradient; nothing is read back.  Afterwards the entry has the
+        plan's block table and context lengths: attend before appending, or the new tokens are
+        both context and main keys.
+        """
+        key = self._layer_key(layer_id)
+        entry = self._layer_kv.get(key)
+        if entry is None:
+            raise ValueError(f"no cached KV entry for layer {layer_id!r}")
+        if entry.block_table is None:
+            raise ValueError("append_paged_kv_cache requires a paged entry (prefill_paged_kv_cache)")
+        h_kv = 1 if entry.is_mla else entry.num_heads
+        d, t = entry.head_dim, int(q_meta.total_tokens)
+        pairs = [(k, entry.k_cache)]
+        if not entry.is_mla:
+            if v is None:
+                raise ValueError("non-MLA append requires v")
+            pairs.append((v, entry.v_cache))
+        for (x, pool), what in zip(pairs, ("k", "v")):
+            shapes = ((q_meta.B, entry.num_heads, q_meta.N, d), (h_kv * t, d))
+            if tuple(x.shape) not in shapes or x.ndim != k.ndim:
+                raise ValueError(f"{what} must be padded [B, H, N, D] or packed [H_kv * T, D], as q_meta describes it")
+            if x.dtype != entry.dtype or x.device != entry.device:
+                raise ValueError(f"{what} dtype/device must match the cached entry")
+            if pool.requires_grad:
+                raise ValueError("a page pool that requires grad cannot be appended to in place")
+        slots, table, cu = plan.slot_mapping, plan.block_table, plan.cu_seqlens_kv
+        if slots.dtype != torch.int64 or tuple(slots.shape) != (t,):
+            raise ValueError("plan.slot_mapping must be int64 with one entry per packed token of q_meta")
+        if table.ndim != 2 or table.dtype != torch.int32 or int(table.shape[0]) < 1 \
+                or cu.dtype != torch.int32 or tuple(cu.shape) != (int(table.shape[0]) + 1,):
+            raise ValueError("plan.block_table must be rank-2 int32 and plan.cu_seqlens_kv have a row more than it")
+        if any(x.device != entry.device for x in (slots, table, cu, q_meta.token_indices)):
+            raise ValueError("plan and q_meta must be on the cached entry's device")
+        from flash_mlm.host.paged import paged_append
+
+        if t > 0:
+            paged_append(pairs, heads=h_kv, d=d, q_meta=q_meta, slots=slots.contiguous(),
+                         pool_rows=int(entry.total_context_len))
+        self._layer_kv[key] = replace(
+            entry, block_table=table.contiguous(), cu_seqlens_kv=cu.contiguous(),
+            context_batch_size=int(table.shape[0]),
         )
 
     def get_kv_cache(

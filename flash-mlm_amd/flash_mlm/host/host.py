@@ -69,6 +69,11 @@ class tile_config:
         return False
 
 
+def tile_config_value() -> int:
+    """The tile configuration in force (0: the library's own choice)."""
+    return _TILE_CONFIG
+
+
 def _aligned(t: torch.Tensor) -> bool:
     """Row-addressable by the kernel: unit stride in D, 16-byte aligned rows."""
     if t.numel() == 0:
@@ -81,6 +86,12 @@ def _aligned(t: torch.Tensor) -> bool:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if _aligned(t) else t.contiguous()
+
+
+def rows16(t: torch.Tensor) -> torch.Tensor:
+    """Rows that a kernel can address: ``t``, or an aligned copy (also of a contiguous ``t``
+    that starts at an odd address)."""
+    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _workspace(inference_cache: InferenceCache | None, nbytes: int, device: torch.device):
@@ -119,13 +130,14 @@ class AttnLaunch:
         # memory: let go of at once, it is reused behind the launch only
         self.records = 0
 
-    def __call__(self) -> None:
+    def own_buffers(self, row_stats: bool) -> None:
+        """Allocate what each run brings: the row statistics when it stores them, its records."""
         p = self.params
         # every run sets the field: a parameter block copied from a memo must not carry
         # an earlier call's buffer
         self.lse = None
         p.lse = None
-        if getattr(_ROW_STATS, "on", False) and p.H > 0 and p.total_q > 0:
+        if row_stats and p.H > 0 and p.total_q > 0:
             self.lse = torch.empty(p.H * p.total_q, dtype=torch.float32, device=self.device)
             p.lse = self.lse.data_ptr()
         if self.records:
@@ -135,8 +147,11 @@ class AttnLaunch:
                 with torch.cuda.stream(_torch_stream(self.stream, self.device)):
                     buf = torch.empty(self.records, dtype=torch.uint8, device=self.device)
             p.workspace, p.workspace_bytes = buf.data_ptr(), self.records
+
+    def __call__(self) -> None:
+        self.own_buffers(getattr(_ROW_STATS, "on", False))
         with _device_scope(self.device):
-            rc = self.lib.fmlm_attn_fwd(p, self.stream)
+            rc = self.lib.fmlm_attn_fwd(self.params, self.stream)
         _lib.check(rc, "fmlm_attn_fwd")
 
 
@@ -198,8 +213,9 @@ def _memo_store(memo: dict, key, m: _Memo) -> None:
     memo[key] = m
 
 
-def _memo_run(m: _Memo, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, entry):
-    """Run a memoised call on this call's q/k/v (laid out alike, by the memo key)."""
+def _memo_run(m: _Memo, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, entry, wrap=None):
+    """Run a memoised call on this call's q/k/v (laid out alike, by the memo key); ``wrap``
+    makes another kind of launch of it (host/tree.py)."""
     out = torch.empty(m.out_shape, dtype=q.dtype, device=q.device)
     p = _lib.AttnParams.from_buffer_copy(m.params)
     p.q, p.o = q.data_ptr(), out.data_ptr()
@@ -217,6 +233,8 @@ def _memo_run(m: _Memo, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, entry
         keep.append((entry.cu_seqlens_kv, entry.block_table))
     plan = AttnLaunch(_lib.load(), p, _lib.stream_of(q.device), q.device, tuple(keep))
     plan.unpack_kv, plan.records = m.unpack_kv, m.records
+    if wrap is not None:
+        plan = wrap(plan)
     plan()
     return out, plan
 

@@ -54,6 +54,9 @@ enum {
   FMLM_FLAG_CAUSAL_SEQ = 4, /* sequence b attends to main tokens [0, cu_q[b+1]) */
   FMLM_FLAG_NOSPLIT = 8,    /* key ranges are not split (no records, no merge launch); a
                                schedule is then built with this flag too               */
+  FMLM_FLAG_CTX_ONLY = 32,  /* no main keys: the queries attend to their context alone (forward
+                               only; a row without context keys has output 0 in bf16 / f16,
+                               no defined output in f32, and lse +inf)                     */
   FMLM_FLAG_OWN_RECORDS = 16 /* the schedule has no room for split partial results: every
                                fmlm_attn_fwd on it has this flag too and brings them in
                                its workspace                                           */
@@ -348,6 +351,158 @@ FMLM_API int fmlm_attn_bwd(const fmlm_attn_params* p, const fmlm_attn_grads* g, 
  * Gradients of keys shared by all heads (head stride 0) and of paged contexts still have to
  * be zeroed by the caller. */
 FMLM_API int fmlm_attn_bwd_fill(const fmlm_attn_params* p, const fmlm_attn_grads* g, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Norms of queries and keys for each head with the position rotation (no counterpart in
+ * the reference, whose entry points take q and k as they are).  A row is the D elements x
+ * of one head and token; in fp32, rounded once to dtype:
+ *   n_d = x_d (mean(x^2) + eps)^-1/2 w_d            (FMLM_NR_NORM; else n = x)
+ *   pairs (a, b) of n's first rotary_dim elements -> (a c - b s, a s + b c),
+ *   c, s = cos / sin[angle row, i]; pair i is elements (i, i + rotary_dim / 2), or
+ *   (2i, 2i + 1) with FMLM_NR_INTERLEAVED.
+ * Rows.  PADDED: row b * N + p at b * sb + h * sh + p * sn; rows p >= L_b (cu_seqlens) are
+ * written as zeros.  PACKED: token t at h * sh + t * sn, which is token token_indices[t] =
+ * b * N + p of the padded batch (NULL: B = 1 and t = p).
+ * Angle row of a token: positions[i] (i: the packed token, or b * N + p without
+ * cu_seqlens), else offsets[b] + p, else p; clamped to [0, table_rows).
+ * D in {16, 32, 64, 128, 256, 512}; rotary_dim a multiple of 16; rows, cos and sin 16-byte
+ * aligned with unit stride along D.
+ * ------------------------------------------------------------------------- */
+enum {
+  FMLM_NR_NORM = 1,
+  FMLM_NR_INTERLEAVED = 2,
+  FMLM_NR_POSITIONS_I64 = 4, /* positions are int64 (else int32) */
+  FMLM_NR_OFFSETS_I64 = 8    /* offsets are int64 (else int32)   */
+};
+
+typedef struct fmlm_norm_rope_tensor {
+  const void* x;  int64_t x_sb, x_sh, x_sn;
+  void* y;        int64_t y_sb, y_sh, y_sn;    /* forward: the rows out; backward: dx */
+  const void* dy; int64_t dy_sb, dy_sh, dy_sn; /* backward only: the gradient of the rows out */
+  const void* weight; /* gains, or NULL for 1: [D] (w_sh = 0) or [heads, D] (w_sh = D) */
+  void* dweight;      /* backward: laid out like weight, or NULL to skip it */
+  int64_t w_sh;
+  int32_t heads;      /* 0: no such tensor */
+  int32_t reserved;
+} fmlm_norm_rope_tensor;
+
+typedef struct fmlm_norm_rope_params {
+  int32_t dtype;   /* FMLM_DTYPE_* of the rows        */
+  int32_t w_dtype; /* FMLM_DTYPE_* of gains and dweight */
+  int32_t flags;   /* FMLM_NR_*                       */
+  int32_t layout;  /* FMLM_LAYOUT_*                   */
+  int32_t B, N, D;
+  int32_t rotary_dim; /* 0: no rotation */
+  int64_t rows;       /* B * N, or packed tokens      */
+  int64_t table_rows;
+  float eps;
+  int32_t reserved;
+  const float* cos; /* [table_rows, rotary_dim / 2] fp32 */
+  const float* sin;
+  const int32_t* cu_seqlens;    /* [B+1] or NULL */
+  const int64_t* token_indices; /* see above, or NULL */
+  const void* positions;        /* or NULL */
+  const void* offsets;          /* [B], or NULL */
+  fmlm_norm_rope_tensor q, k;
+  void* workspace; /* backward: fmlm_norm_rope_bwd_workspace_bytes(p) bytes (partial sums of dw) */
+  int64_t workspace_bytes;
+} fmlm_norm_rope_params;
+
+FMLM_API int fmlm_norm_rope_params_size(void);
+FMLM_API int fmlm_norm_rope(const fmlm_norm_rope_params* p, void* stream);
+/* Gradients of the same call: x and dy in, dx to y, dweight where given; dx of padding rows
+ * is zero.  Sums are taken in one order: the same call gives the same bits. */
+FMLM_API int64_t fmlm_norm_rope_bwd_workspace_bytes(const fmlm_norm_rope_params* p);
+FMLM_API int fmlm_norm_rope_bwd(const fmlm_norm_rope_params* p, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Block table and slots of a step's new tokens (no counterpart in the reference, whose
+ * roadmap lists paged KV, README.md:41).  Request b has old_lens[b] tokens in its context
+ * pages (FMLM_PAGE_ROWS rows each) and gets L_b = cu_seqlens[b+1] - cu_seqlens[b] new ones,
+ * or those of them with keep[t] != 0.  Requests take the pages they lack from free_pages
+ * in order:
+ *   have_b = ceil(old_b / 64), need_b = ceil((old_b + new_b) / 64) - have_b
+ *   block_table[b, i] = table_in[b, i] for i < have_b, then free_pages[sum of the needs
+ *       before b + i - have_b], and -1 from i = have_b + need_b on
+ *   slot_mapping[t] = page * 64 + row of the token's place (old_b + its rank among the kept
+ *       tokens of b), -1 for a token that is not kept
+ *   positions[t] = old_b + p, new_lens[b] = old_b + new_b, cu_kv its prefix sums
+ * table_in == NULL: no request has pages yet (old_lens must be 0).  A request that does not
+ * fit its table row or finds no free page keeps the tokens that fit (the others' slots are
+ * -1).  summary: {pages taken, pages lacking in free_pages, requests with an old length
+ * out of range or more tokens than the row holds, tokens stored}.
+ * workspace: fmlm_block_table_workspace_bytes(p) bytes.
+ * ------------------------------------------------------------------------- */
+enum {
+  FMLM_BT_OLD_I64 = 1,   /* old_lens are int64 (else int32)   */
+  FMLM_BT_TABLE_I64 = 2, /* table_in is int64 (else int32)    */
+  FMLM_BT_FREE_I64 = 4   /* free_pages are int64 (else int32) */
+};
+
+typedef struct fmlm_block_table_params {
+  int32_t flags;
+  int32_t B, N;      /* requests, padded length of their new tokens */
+  int32_t T;         /* new tokens: cu_seqlens[B] */
+  int32_t max_pages; /* entries of a row of block_table */
+  int32_t in_pages;  /* entries of a row of table_in */
+  int32_t n_free;
+  int32_t reserved;
+  const void* old_lens;         /* [B] */
+  const int32_t* cu_seqlens;    /* [B+1] */
+  const int64_t* token_indices; /* [T] b * N + p (fmlm_pack_metadata) */
+  const uint8_t* keep;          /* [T] or NULL */
+  const void* table_in;         /* [B, in_pages] or NULL */
+  const void* free_pages;       /* [n_free] */
+  int32_t* block_table;         /* [B, max_pages] */
+  int64_t* slot_mapping;        /* [T] */
+  int32_t* positions;           /* [T] */
+  int32_t* new_lens;            /* [B] */
+  int32_t* cu_kv;               /* [B+1] */
+  int32_t* summary;             /* [4] */
+  void* workspace;
+  int64_t workspace_bytes;
+} fmlm_block_table_params;
+
+FMLM_API int fmlm_block_table_params_size(void);
+FMLM_API int64_t fmlm_block_table_workspace_bytes(const fmlm_block_table_params* p);
+FMLM_API int fmlm_block_table(const fmlm_block_table_params* p, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged append: for up to 2 tensors (K, V), head h and token t < T, the D elements (h, t) of
+ * src go to row slots[t] of head h of the pool [heads, pool_rows, D]; slots outside [0,
+ * pool_rows) are skipped.  src rows: PADDED b * sb + h * sh + p * sn for token_indices[t] =
+ * b * N + p, PACKED h * sh + t * sn.  Moves bytes only.
+ * ------------------------------------------------------------------------- */
+typedef struct fmlm_paged_tensor {
+  const void* src;
+  int64_t s_sb, s_sh, s_sn;
+  void* pool;
+} fmlm_paged_tensor;
+
+FMLM_API int fmlm_paged_append(const fmlm_paged_tensor* tensors, int32_t n_tensors, int32_t elem_bytes, int32_t heads,
+                               int32_t D, int32_t T, int32_t N, int32_t layout, const int64_t* token_indices,
+                               const int64_t* slots, int64_t pool_rows, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Trees of drafted tokens.  parents[t] (int32 or int64) is the index, within its sequence,
+ * of the token that token t follows, -1 for a root.  A parent has to come before its child:
+ * other values count in *n_bad (may be NULL) and are taken as -1.
+ *   mask[t * words + j / 64], bit j % 64: token j of t's sequence is t or an ancestor of it
+ *   positions[t] = (ctx_lens ? ctx_lens[b] : 0) + number of t's ancestors
+ * words >= ceil(N / 64); at most FMLM_MAX_TREE tokens in a sequence (N).
+ * ------------------------------------------------------------------------- */
+#define FMLM_MAX_TREE 256
+
+FMLM_API int fmlm_tree_mask(const void* parents, int32_t parents_i64, const int32_t* cu_seqlens, int32_t B, int32_t N,
+                            int32_t T, int32_t words, const void* ctx_lens, int32_t ctx_lens_i64, uint64_t* mask,
+                            int32_t* positions, int32_t* n_bad, void* stream);
+
+/* Attention of drafted trees: fmlm_attn_fwd's packed call p in which token i of a sequence
+ * attends to [its context || the main tokens j of its sequence with mask bit j set].  p has
+ * FMLM_FLAG_CTX_ONLY set (its schedule too) and brings p->lse; N is at most FMLM_MAX_TREE.
+ * The context part runs as fmlm_attn_fwd(p); a second kernel then computes the tree's part
+ * and joins the two by their sums.  A row that sees no key has output 0.  No backward. */
+FMLM_API int fmlm_attn_tree_fwd(const fmlm_attn_params* p, const uint64_t* mask, int32_t words, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,413 @@
+"""qk_norm_rope: refusals (CPU) and, on the GPU, rows and gradients against the 64-bit
+restatement (oracle/paged_step_ref.py).
+
+Tolerances, u = 2^-24: a row's sum of squares takes 8 fused steps and up to 6 additions
+(14 u, half of it in its inverse root), the root and the products x r w and the rotation
+8 u more: 16 u of the magnitudes a result is made of, and half a step of the output type.  A
+gradient has two such factors and one more sum: 40 u.  dw sums at most `rows` terms.
+"""
+
+from __future__ import annotations
+
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+from flash_mlm import _lib, build_pack_metadata, qk_norm_rope
+from oracle import paged_step_ref as ref
+
+U = 2.0**-24
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _f(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _tables(n, r, device):
+    freq = 10000.0 ** (-torch.arange(0, r // 2, dtype=torch.float64) * 2 / r)
+    ang = torch.arange(n, dtype=torch.float64)[:, None] * freq
+    return ang.cos().float().to(device), ang.sin().float().to(device)
+
+
+def _half(dtype):
+    return 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+
+
+def _close(got, want, mag, dtype, steps):
+    bound = _half(dtype) * np.abs(want) + steps * U * mag * (1 + _half(dtype)) + 1e-30
+    if dtype == torch.float16:
+        bound = bound + 2.0**-25  # half a step of its smallest values
+    err = np.abs(got - want)
+    assert np.all(err <= bound), f"worst {np.max(err / bound):.3f} of the bound"
+
+
+# ---------------------------------------------------------------------------
+# CPU
+# ---------------------------------------------------------------------------
+def test_needs_gpu_tensors():
+    q = torch.zeros(1, 2, 3, 64)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        qk_norm_rope(q, q)
+
+
+@pytest.mark.parametrize("q, k, kw, match", [
+    ((1, 2, 64), (1, 2, 64), {}, "rank-4"),
+    ((1, 2, 3, 64), (6, 64), {}, "rank-4"),
+    ((1, 2, 3, 64), (1, 2, 3, 32), {}, "head_dim"),
+    ((1, 2, 3, 80), (1, 2, 3, 80), {}, "HEAD_DIM"),
+])
+def test_refuses_shapes(q, k, kw, match):
+    with pytest.raises(ValueError, match=match):
+        qk_norm_rope(torch.zeros(q), torch.zeros(k), **kw)
+
+
+def test_refuses_dtypes():
+    q = torch.zeros(1, 2, 3, 64, dtype=torch.float64)
+    with pytest.raises(ValueError, match="one dtype"):
+        qk_norm_rope(q, q)
+    with pytest.raises(ValueError, match="one dtype"):
+        qk_norm_rope(q.float(), q.half())
+
+
+def test_abi_refuses():
+    lib = _lib.load()
+    assert lib.fmlm_norm_rope(None, None) == -1
+    p = _lib.NormRopeParams()
+    p.dtype = 7
+    assert lib.fmlm_norm_rope(p, None) == -2
+    p.dtype, p.w_dtype, p.D = _lib.DTYPE_BF16, _lib.DTYPE_BF16, 48
+    assert lib.fmlm_norm_rope(p, None) == -3
+    p.D = 64
+    assert lib.fmlm_norm_rope(p, None) == 0  # no rows
+    p.B, p.N, p.rows = 1, 4, 5
+    assert lib.fmlm_norm_rope(p, None) == -1  # rows are not B * N
+    p.rows, p.q.heads = 4, 1
+    assert lib.fmlm_norm_rope(p, None) == -1  # no tensor
+    p.q.x, p.q.y = 256, 256 + 8
+    assert lib.fmlm_norm_rope(p, None) == -4
+    p.q.y, p.rotary_dim = 512, 24
+    assert lib.fmlm_norm_rope(p, None) == -1  # rotary_dim
+    p.rotary_dim = 32
+    assert lib.fmlm_norm_rope(p, None) == -1  # no tables
+    p.rotary_dim, p.layout, p.B, p.N, p.rows = 0, _lib.LAYOUT_PACKED, 2, 4, 4
+    assert lib.fmlm_norm_rope(p, None) == -1  # packed rows of two sequences without token indices
+    p.layout, p.rows, p.flags = _lib.LAYOUT_PADDED, 8, _lib.NR_NORM
+    assert lib.fmlm_norm_rope_bwd_workspace_bytes(p) == -1  # no dy
+    p.q.dy, p.q.weight, p.q.dweight = 1024, 2048, 4096
+    need = lib.fmlm_norm_rope_bwd_workspace_bytes(p)
+    assert need == 64 * 4  # one partial row
+    assert lib.fmlm_norm_rope_bwd(p, None) == -5
+
+
+# ---------------------------------------------------------------------------
+# GPU
+# ---------------------------------------------------------------------------
+def _case(device, dtype, *, H, Hk, D, lens, N, R, gain, packed, inter, where, norm=True, seed=0, grad=False):
+    g = torch.Generator().manual_seed(seed)
+    B, T = len(lens), sum(lens)
+
+    def rnd(*s):
+        return torch.randn(s, generator=g)
+
+    meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+    shape = (lambda h: (h * T, D)) if packed else (lambda h: (B, h, N, D))
+    q, k, dq, dk = ((rnd(*shape(h)) * (1 + i)).to(dtype).to(device) for i, h in enumerate((H, Hk, H, Hk)))
+    wq = wk = None
+    if gain != "none":
+        wq, wk = ((1 + 0.2 * rnd(*((h, D) if gain == "head" else (D,)))).to(dtype).to(device) for h in (H, Hk))
+    kw = dict(q_weight=wq, k_weight=wk, norm=norm, interleaved=inter, q_meta=meta, eps=1e-5)
+    b = np.repeat(np.arange(B), lens)
+    p = np.concatenate([np.arange(n) for n in lens]) if T else np.zeros(0, int)
+    cos = sin = None
+    if R:
+        kw["cos"], kw["sin"] = _tables(N + 40, R, device)
+        if where == "context":
+            start = torch.randint(0, 30, (B,), generator=g)
+            kw["context_lens"], pos = start.to(device), start.numpy()[b] + p
+        elif where == "positions":
+            pos = torch.randint(0, N + 40, (T,), generator=g).numpy()
+            kw["positions"] = torch.from_numpy(pos).to(torch.int32).to(device)
+        else:
+            pos = p
+        cos, sin = _f(kw["cos"])[pos], _f(kw["sin"])[pos]
+    if grad:
+        for t in (q, k, wq, wk):
+            if t is not None:
+                t.requires_grad_()
+
+    def tokens(x, h):  # [h, T, D]
+        x = _f(x)
+        return x.reshape(h, T, D) if packed else x[b, :, p].transpose(1, 0, 2)
+
+    def whole(y, h):
+        if packed:
+            return y.reshape(h * T, D)
+        out = np.zeros((B, h, N, D))
+        out[b, :, p] = y.transpose(1, 0, 2)
+        return out
+
+    return q, k, dq, dk, kw, cos, sin, tokens, whole
+
+
+def _check(device, dtype, *, grad=False, **c):
+    H, Hk, gain, inter, norm = c["H"], c["Hk"], c["gain"], c["inter"], c.get("norm", True)
+    q, k, dq, dk, kw, cos, sin, tokens, whole = _case(device, dtype, grad=grad, **c)
+    outs = qk_norm_rope(q, k, **kw)
+    opt = dict(eps=1e-5, norm=norm, interleaved=inter)
+    gains = []
+    for y, x, w, h in zip(outs, (q, k), (kw["q_weight"], kw["k_weight"]), (H, Hk)):
+        wd = None if w is None else _f(w)[:, None, :] if gain == "head" else _f(w)
+        gains.append(wd)
+        want, mag = ref.norm_rope(tokens(x, h), wd, cos, sin, **opt)
+        assert y.is_contiguous() and y.dtype == dtype and y.shape == x.shape
+        _close(_f(y), whole(want, h), whole(mag, h), dtype, 16)
+    if not grad:
+        return
+    leaves = [t for t in (q, k, kw["q_weight"], kw["k_weight"]) if t is not None]
+    grads = torch.autograd.grad(outs, leaves, (dq, dk))
+    for i, (x, dy, h) in enumerate(((q, dq, H), (k, dk, Hk))):
+        dx, mag, dw, dwm = ref.norm_rope_grads(tokens(x, h), gains[i], cos, sin, tokens(dy, h), **opt)
+        _close(_f(grads[i]), whole(dx, h), whole(mag, h), dtype, 40)
+        if gains[i] is not None:
+            axes = 1 if gain == "head" else (0, 1)
+            rows = dw.shape[1] * (1 if gain == "head" else h)
+            _close(_f(grads[2 + i]), dw.sum(axes), dwm.sum(axes), dtype, 40 + rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 256, 512])
+@pytest.mark.parametrize("inter", [False, True])
+def test_rows_and_gradients(dtype, D, inter, device):
+    _check(device, DT[dtype], H=5, Hk=3, D=D, lens=[37, 0, 1, 20], N=37, R=D, gain="shared", packed=False, inter=inter,
+           where="context", seed=D, grad=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("packed, gain, where, R", [
+    x for x in itertools.product([False, True], ["none", "shared", "head"], ["place", "positions"], [0, 16, 64])
+    if not (x[3] == 0 and x[2] == "positions")
+])
+def test_layouts_gains_and_positions(dtype, packed, gain, where, R, device):
+    _check(device, DT[dtype], H=4, Hk=1, D=128, lens=[3, 17, 9], N=19, R=R, gain=gain, packed=packed, inter=False,
+           where=where, seed=7, grad=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("inter", [False, True])
+def test_rotation_alone(inter, device):
+    _check(device, torch.float16, H=2, Hk=2, D=64, lens=[5, 8], N=8, R=32, gain="none", packed=False, inter=inter,
+           where="place", norm=False, grad=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens, N", [([1], 1), ([1] * 70, 1), ([0, 0], 4), ([2000, 1500, 1999], 2000)])
+@pytest.mark.parametrize("gain", ["shared", "head"])
+def test_lengths(lens, N, gain, device):
+    _check(device, torch.bfloat16, H=6, Hk=6, D=64, lens=lens, N=N, R=64, gain=gain, packed=False, inter=False,
+           where="context", seed=N, grad=True)
+
+
+@pytest.mark.gpu
+def test_mixed_gains(device):
+    """Gains per head for q, shared for k: one launch, two layouts of dw."""
+    q, k, dq, dk, kw, cos, sin, tokens, _ = _case(device, torch.float32, H=5, Hk=3, D=32, lens=[9, 30], N=30, R=32,
+                                                  gain="head", packed=False, inter=False, where="place", grad=True)
+    kw["k_weight"] = kw["k_weight"].detach()[0].clone().requires_grad_()
+    outs = qk_norm_rope(q, k, **kw)
+    gw = torch.autograd.grad(outs, (kw["q_weight"], kw["k_weight"]), (dq, dk))
+    for g, x, dy, w, h, axes in ((gw[0], q, dq, _f(kw["q_weight"])[:, None], 5, 1),
+                                 (gw[1], k, dk, _f(kw["k_weight"]), 3, (0, 1))):
+        _, _, t, m = ref.norm_rope_grads(tokens(x, h), w, cos, sin, tokens(dy, h), eps=1e-5)
+        _close(_f(g), t.sum(axes), m.sum(axes), torch.float32, 40 + 39 * 3)
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences(device):
+    """The gradient along a direction is what the (64-bit) loss does along it."""
+    q, k, dq, dk, kw, cos, sin, tokens, _ = _case(device, torch.float32, H=2, Hk=2, D=64, lens=[6], N=6, R=64,
+                                                  gain="shared", packed=False, inter=False, where="place", grad=True)
+    grads = torch.autograd.grad(qk_norm_rope(q, k, **kw), (q, kw["q_weight"]), (dq, dk))
+    rng = np.random.default_rng(0)
+    x, w, dy = tokens(q, 2), _f(kw["q_weight"]), tokens(dq, 2)
+    vx, vw = rng.standard_normal(x.shape), rng.standard_normal(w.shape)
+
+    def loss(e):
+        return (ref.norm_rope(x + e * vx, w + e * vw, cos, sin, eps=1e-5)[0] * dy).sum()
+
+    h = 1e-5  # differences at 64 bits: error about h^2
+    slope = (loss(h) - loss(-h)) / (2 * h)
+    got = (tokens(grads[0], 2) * vx).sum() + (_f(grads[1]) * vw).sum()
+    size = np.abs(tokens(grads[0], 2) * vx).sum() + np.abs(_f(grads[1]) * vw).sum()
+    assert abs(got - slope) <= 60 * U * size + 1e-7 * size
+
+
+@pytest.mark.gpu
+def test_strides_padding_and_alignment(device):
+    """q and k as views of one projection, NaN in padding rows, an unaligned view, a
+    gradient of other strides."""
+    B, N, H, D = 2, 13, 3, 64
+    g = torch.Generator().manual_seed(3)
+    qkv = torch.randn((B, N, 3, H, D), generator=g).to(torch.bfloat16).to(device)
+    meta = build_pack_metadata(torch.tensor([13, 4], device=device), N, 32)
+    qkv[1, 4:] = float("nan")
+    q, k = (qkv[:, :, i].transpose(1, 2) for i in range(2))
+    cos, sin = _tables(N, D, device)
+    kw = dict(cos=cos, sin=sin, q_meta=meta)
+    got = qk_norm_rope(q, k, **kw)
+    want = qk_norm_rope(q.contiguous(), k.contiguous(), **kw)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y) and not x[1, :, 4:].any()
+    flat = torch.empty(B * H * N * D + 1, dtype=torch.bfloat16, device=device)
+    odd = flat[1:].view(B, H, N, D).copy_(q)
+    assert odd.data_ptr() % 16
+    assert torch.equal(qk_norm_rope(odd, k, **kw)[0], want[0])
+    assert torch.equal(qk_norm_rope(q, k, cos=torch.cat([cos[:, :1], cos], 1)[:, 1:], sin=sin, q_meta=meta)[0], want[0])
+    ql = q.detach().clone().requires_grad_()
+    out = qk_norm_rope(ql, k, **kw)[0]
+    dy = torch.randn((B, N, H, D), generator=g).to(torch.bfloat16).to(device)
+    a = torch.autograd.grad(out, ql, dy.transpose(1, 2), retain_graph=True)[0]
+    assert torch.equal(a, torch.autograd.grad(out, ql, dy.transpose(1, 2).contiguous())[0])
+    assert not a[1, :, 4:].any()
+
+
+@pytest.mark.gpu
+def test_positions_are_clamped_on_the_gpu_and_refused_on_the_cpu(device):
+    q = torch.randn((1, 2, 4, 64), device=device)
+    cos, sin = _tables(8, 64, device)
+    far = torch.tensor([[-5, 3, 100, 7]], device=device)
+    near = torch.tensor([[0, 3, 7, 7]])
+    a = qk_norm_rope(q, q, cos=cos, sin=sin, positions=far)
+    b = qk_norm_rope(q, q, cos=cos, sin=sin, positions=near)
+    assert torch.equal(a[0], b[0])
+    with pytest.raises(ValueError, match="positions values"):
+        qk_norm_rope(q, q, cos=cos, sin=sin, positions=far.cpu())
+
+
+@pytest.mark.gpu
+def test_refusals(device):
+    q = torch.zeros((2, 3, 5, 64), device=device)
+    cos, sin = _tables(8, 64, device)
+    meta = build_pack_metadata(torch.tensor([5, 2], device=device), 5, 32)
+    w = torch.ones(64, device=device)
+    for match, kw in [
+        ("nothing to do", dict(norm=False)),
+        ("gains need", dict(norm=False, cos=cos, sin=sin, q_weight=w)),
+        ("same dtype", dict(q_weight=w, k_weight=w.half())),
+        ("head_dim", dict(q_weight=w[:32])),
+        ("come together", dict(cos=cos)),
+        ("fp32 tables", dict(cos=cos.half(), sin=sin.half())),
+        ("multiple of 16", dict(cos=cos[:, :4], sin=sin[:, :4])),
+        ("multiple of 16", dict(cos=cos[:0], sin=sin[:0])),
+        ("need cos", dict(context_lens=torch.zeros(2, dtype=torch.int32, device=device))),
+        ("exclusive", dict(cos=cos, sin=sin, context_lens=torch.zeros(2, dtype=torch.int32, device=device),
+                           positions=torch.zeros((2, 5), dtype=torch.int32, device=device))),
+        ("shape", dict(cos=cos, sin=sin, positions=torch.zeros(7, dtype=torch.int32, device=device))),
+        ("shape", dict(cos=cos, sin=sin, positions=torch.zeros((2, 5), device=device))),
+        ("eps", dict(eps=float("nan"))),
+        ("num_heads", dict(num_heads=4)),
+    ]:
+        with pytest.raises(ValueError, match=match):
+            qk_norm_rope(q, q, **kw)
+    with pytest.raises(ValueError, match="q_meta"):
+        qk_norm_rope(q[:1], q[:1], q_meta=meta)
+    with pytest.raises(ValueError, match="packed q needs"):
+        qk_norm_rope(q.view(-1, 64), q.view(-1, 64))
+    with pytest.raises(ValueError, match="multiple of the token count"):
+        qk_norm_rope(q.view(-1, 64), q.view(-1, 64), q_meta=meta)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        x = q.clone().requires_grad_()
+        starts = torch.zeros(2, dtype=torch.int32, device=device)
+        y = qk_norm_rope(x, q, cos=cos, sin=sin, context_lens=starts)[0]
+        starts += 1
+        y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_unused_outputs_and_partial_gradients(device):
+    q, k, dq, dk, kw, *_ = _case(device, torch.float32, H=2, Hk=2, D=64, lens=[6, 3], N=6, R=64, gain="shared",
+                                 packed=False, inter=False, where="place", grad=True)
+    wq, wk = kw["q_weight"], kw["k_weight"]
+    all_ = torch.autograd.grad(qk_norm_rope(q, k, **kw), (q, k, wq, wk), (dq, dk))
+    out = qk_norm_rope(q, k, **kw)
+    a = torch.autograd.grad(out[0], (q, k, wq, wk), dq, allow_unused=True)
+    assert torch.equal(a[0], all_[0]) and torch.equal(a[2], all_[2]) and a[1] is None and a[3] is None
+    kw["q_weight"] = wq.detach()
+    out = qk_norm_rope(q.detach(), k.detach(), **kw)
+    assert not out[0].requires_grad or out[1].requires_grad
+    assert torch.equal(torch.autograd.grad(out[1], wk, dk)[0], all_[3])
+
+
+@pytest.mark.gpu
+def test_same_bits_every_time_on_another_stream_and_in_a_graph(device):
+    q, k, dq, dk, kw, *_ = _case(device, torch.bfloat16, H=8, Hk=8, D=128, lens=[300, 411, 5], N=411, R=128,
+                                 gain="shared", packed=False, inter=False, where="context", grad=True)
+    leaves = (q, k, kw["q_weight"], kw["k_weight"])
+
+    def step():
+        out = qk_norm_rope(q, k, **kw)
+        return [*out, *torch.autograd.grad(out, leaves, (dq, dk))]
+
+    first = [t.detach().clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    side.synchronize()
+    for a, b in zip(first, other):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    # outputs of an eager call hold its autograd graph: the capture is refused until they are gone
+    with pytest.raises(ValueError, match="being captured"):
+        with torch.cuda.graph(graph):
+            qk_norm_rope(q, k, **kw)
+    del other, b
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+        twice = step()  # the same leaves again, in the same capture
+    captured, twice = ([t.detach() for t in x] for x in (captured, twice))
+    for seed in range(3):
+        with torch.no_grad():
+            q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(seed)).to(q.dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b, c in zip(captured, step(), twice):
+            assert torch.equal(a, b) and torch.equal(c, b)
+
+
+@pytest.mark.gpu
+def test_feeds_attention(device):
+    """The rows go into the packed attention as they come out, and gradients flow through both."""
+    from flash_mlm import flash_attn_mlm_compressed
+
+    B, H, N, D = 2, 4, 24, 64
+    g = torch.Generator().manual_seed(5)
+    q, k, v = (torch.randn((B, H, N, D), generator=g).to(device).requires_grad_() for _ in range(3))
+    meta = build_pack_metadata(torch.tensor([24, 9], device=device), N, 32)
+    cos, sin = _tables(N, D, device)
+    qn, kn = qk_norm_rope(q, k, cos=cos, sin=sin, q_meta=meta)
+    out = flash_attn_mlm_compressed(qn, kn, v, H, meta, 0.125)
+    dout = torch.randn(out.shape, generator=g).to(device)
+    got = torch.autograd.grad(out, (q, k, v), dout)
+    # the same in elementary operations at 64 bits
+    x = [t.detach().double().requires_grad_() for t in (q, k, v)]
+
+    def rot(t):
+        t = t / torch.sqrt(t.square().mean(-1, keepdim=True) + 1e-6)
+        a, b = t[..., :32], t[..., 32:]
+        c, s = cos.double(), sin.double()
+        return torch.cat((a * c - b * s, a * s + b * c), -1)
+
+    parts = []
+    for b, n in enumerate((24, 9)):
+        w = torch.softmax(0.125 * rot(x[0])[b, :, :n] @ rot(x[1])[b, :, :n].transpose(1, 2), -1)
+        parts.append(w @ x[2][b, :, :n])
+    want = torch.autograd.grad(torch.cat(parts, 1).reshape(H * 33, D), x, dout.double())
+    for a, b in zip(got, want):
+        # fp32 throughout: sums of up to 64 products a score, 24 keys a row
+        assert (a.double() - b).abs().max() <= 2000 * U * b.abs().max()

@@ -1,0 +1,430 @@
+"""build_tree_metadata and flash_attn_mlm_tree: refusals (CPU), and on the GPU masks against sets
+of ancestors, attention against its 64-bit restatement (oracle/paged_step_ref.py), and a
+speculative decoding loop over a paged cache.
+
+Tolerances.  With W = sum of w |v| of an output element, h half a step of the type and u =
+2^-24: the context's part is rounded once (h of it) and the output once more (h |o|); the
+probabilities of both parts are rounded (2 h W with their sums); a score's error e moves the
+result by at most 2 e W, and e is (D + 16) u S in fp32, S = scale * sum |q k|, plus h S where
+fp16 queries are scaled before the product; exponentials and sums add (keys + 64) u W at most.
+Fp16 probabilities below 2^-14 have an absolute error of 2^-25 each.
+"""
+
+from __future__ import annotations
+
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from flash_mlm import (
+    InferenceCache,
+    PackMetadata,
+    TreeMetadata,
+    _lib,
+    build_block_table,
+    build_pack_metadata,
+    build_tree_metadata,
+    flash_attn_mlm_tree,
+    qk_norm_rope,
+    unpack_from_kernel,
+)
+from oracle import paged_step_ref as ref
+
+PAGE, U = 64, 2.0**-24
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _f(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _random_parents(r, lens):
+    return [-1 if i == 0 or r.random() < 0.1 else (i - 1 if r.random() < 0.5 else r.randrange(i))
+            for n in lens for i in range(n)]
+
+
+def _cpu_meta(lens, N):
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32)
+    tok = torch.tensor([b * N + p for b, n in enumerate(lens) for p in range(n)], dtype=torch.int64)
+    return PackMetadata(B=len(lens), N=N, lengths=torch.tensor(lens, dtype=torch.int32), cu_seqlens=cu, token_indices=tok,
+                        total_tokens=sum(lens), batch_ids_block_n=32, batch_ids_q=cu, q_tile_starts_q=cu)
+
+
+# ---------------------------------------------------------------------------
+# CPU
+# ---------------------------------------------------------------------------
+def test_refusals_on_the_cpu():
+    meta = _cpu_meta([2, 1], 2)
+    par = torch.tensor([-1, 0, -1])
+    with pytest.raises(ValueError, match="no CPU compute path"):
+        build_tree_metadata(par, meta)
+    with pytest.raises(ValueError, match="parents must"):
+        build_tree_metadata(par[:2], meta)
+    with pytest.raises(ValueError, match="parents must"):
+        build_tree_metadata(par.float(), meta)
+    with pytest.raises(ValueError, match="context_lens must"):
+        build_tree_metadata(par, meta, context_lens=par)
+    with pytest.raises(ValueError, match="at most 256"):
+        build_tree_metadata(par, _cpu_meta([2, 1], 257))
+    tree = TreeMetadata(torch.zeros((3, 1), dtype=torch.int64), torch.zeros(3, dtype=torch.int32))
+    q = torch.zeros((2, 2, 2, 64), dtype=torch.float16)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        flash_attn_mlm_tree(q, q, q, 2, meta, tree, 1.0)
+    with pytest.raises(ValueError, match="num_heads"):
+        flash_attn_mlm_tree(q, q, q, 3, meta, tree, 1.0)
+    with pytest.raises(ValueError, match="q_meta"):
+        flash_attn_mlm_tree(q[:1], q[:1], q[:1], 2, meta, tree, 1.0)
+    with pytest.raises(ValueError, match="tree.mask"):
+        flash_attn_mlm_tree(q, q, q, 2, meta, TreeMetadata(tree.mask[:2], None), 1.0)
+    with pytest.raises(ValueError, match="no backward"):
+        flash_attn_mlm_tree(q.clone().requires_grad_(), q, q, 2, meta, tree, 1.0)
+
+
+def test_abi_refuses():
+    lib = _lib.load()
+    m = lib.fmlm_tree_mask
+    assert m(None, 0, None, 1, 257, 1, 5, None, 0, None, None, None, None) == -1  # too long
+    assert m(None, 0, None, 1, 65, 1, 1, None, 0, None, None, None, None) == -1  # too few words
+    assert m(None, 0, None, 1, 4, 4, 1, None, 0, None, None, None, None) == -1  # no tensors
+    assert m(None, 0, None, 0, 4, 0, 1, None, 0, None, None, None, None) == 0
+    a = lib.fmlm_attn_tree_fwd
+    assert a(None, None, 1, None) == -1
+    p = _lib.AttnParams()
+    p.dtype, p.B, p.H, p.D, p.N, p.total_q = _lib.DTYPE_BF16, 1, 1, 64, 4, 4
+    p.q = p.k = p.v = p.o = p.cu_seqlens_q = p.lse = 256
+    assert a(p, 256, 1, None) == -1  # not a context-only call
+    p.flags = _lib.FLAG_CTX_ONLY
+    assert a(p, None, 1, None) == -1  # no mask
+    p.lse = None
+    assert a(p, 256, 1, None) == -1  # no row statistics
+    p.lse, p.N = 256, 300
+    assert a(p, 256, 8, None) == -1  # too long
+    p.N, p.v = 4, 264
+    assert a(p, 256, 1, None) == -4
+    p.v, p.q_sn = 256, 60
+    assert a(p, 256, 1, None) == -4
+    p.q_sn = 64
+    assert a(p, 256, 1, None) == -5  # fmlm_attn_fwd's checks follow: no workspace
+    p.flags |= _lib.FLAG_PREFILL
+    assert a(p, 256, 1, None) == -1
+    assert lib.fmlm_attn_fwd(p, None) == -1
+    g = _lib.AttnGrads()
+    p.flags = _lib.FLAG_CTX_ONLY
+    g.dout = g.dq = g.dk = g.dv = 256
+    assert lib.fmlm_attn_bwd(p, g, None) == -1
+
+
+# ---------------------------------------------------------------------------
+# GPU
+# ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens, N", [([1], 1), ([2, 0, 1], 2), ([64, 63, 65], 65), ([256, 1, 129], 256),
+                                     ([7] * 300, 9)])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_masks(lens, N, dtype, device):
+    r = random.Random(N)
+    meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+    start = [r.randint(0, 100) for _ in lens]
+    b = np.repeat(np.arange(len(lens)), lens)
+    for parents in (_random_parents(r, lens), [i - 1 for n in lens for i in range(n)], [-1] * sum(lens)):
+        seen = ref.ancestors(parents, lens)
+        for ctx in (None, torch.tensor(start, dtype=dtype, device=device)):
+            tree = build_tree_metadata(torch.tensor(parents, dtype=dtype, device=device), meta, context_lens=ctx)
+            assert np.array_equal(tree.mask.cpu().numpy(), ref.mask_words(seen, tree.mask.shape[1]))
+            want = [len(s) - 1 + (0 if ctx is None else start[x]) for s, x in zip(seen, b)]
+            assert tree.positions.tolist() == want
+
+
+@pytest.mark.gpu
+def test_bad_parents(device):
+    meta = build_pack_metadata(torch.tensor([4, 3], device=device), 4, 32)
+    parents = [-1, 1, -2, 9, -1, 0, 2]
+    t = torch.tensor(parents, device=device)
+    with pytest.raises(ValueError, match="before their children"):
+        build_tree_metadata(t, meta)
+    tree = build_tree_metadata(t, meta, check=False)
+    assert np.array_equal(tree.mask.cpu().numpy(), ref.mask_words(ref.ancestors(parents, [4, 3]), 1))
+
+
+def _close(got, q, k, v, seen, scale, kc, vc, dtype):
+    o, w, c, s = ref.tree_attention(_f(q), _f(k), _f(v), seen, scale, _f(kc), _f(vc))
+    h = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    keys, D = kc.shape[0] + k.shape[0], q.shape[-1]
+    e = ((D + 16) * U + (h if dtype == torch.float16 else 0.0)) * s[:, None]
+    bound = h * (np.abs(o) + c) + (2 * h + 2 * e + (keys + 64) * U) * w
+    if dtype == torch.float16:
+        bound = bound + 2.0**-25 * (keys * np.abs(np.concatenate([_f(vc), _f(v)])).max() + 1)
+    err = np.abs(_f(got) - o)
+    assert np.all(err <= bound * 1.01 + 1e-30), f"worst {np.max(err / (bound + 1e-30)):.3f} of the bound"
+
+
+def _context(kind, lens, H, D, mla, dtype, device, seed=0):
+    """(cache, list of (k, v) [H_kv, C_b, D] of every sequence, extra arguments)"""
+    g = torch.Generator().manual_seed(seed)
+    hk, B = 1 if mla else H, len(lens)
+    cache, kw = InferenceCache(), {}
+    if kind == "none":
+        e = torch.empty((hk, 0, D), dtype=dtype, device=device)
+        return None, [(e, e)] * B, kw
+    n = {"shared": [lens[0]], "index": lens[:2]}.get(kind, lens)
+    rows = [[torch.randn((hk, c, D), generator=g).to(dtype).to(device) for _ in range(1 if mla else 2)] for c in n]
+    if kind in ("paged", "index"):
+        need = [-(-c // PAGE) for c in n]
+        P = sum(need) + 2
+        ids = torch.randperm(P, generator=g).tolist()
+        pools = [torch.full((hk, P, PAGE, D), float("nan"), dtype=dtype, device=device) for _ in range(1 if mla else 2)]
+        table = torch.full((len(n), max(need + [1])), -1, dtype=torch.int32)
+        for b, c in enumerate(n):
+            for i in range(need[b]):
+                page = ids.pop()
+                table[b, i] = page
+                for pool, x in zip(pools, rows[b]):
+                    part = x[:, i * PAGE : (i + 1) * PAGE]
+                    pool[:, page, : part.shape[1]] = part
+        cache.prefill_paged_kv_cache(0, k_pages=pools[0], v_pages=None if mla else pools[1], block_table=table.to(device),
+                                     context_lens=torch.tensor(n), is_mla=mla, num_heads=H, head_dim=D)
+    else:
+        flat = [torch.cat([x[i] for x in rows], 1).reshape(-1, D).contiguous() for i in range(1 if mla else 2)]
+        cu = torch.tensor([sum(n[:i]) for i in range(len(n) + 1)], dtype=torch.int32, device=device)
+        cache.prefill_kv_cache(0, k_cache=flat[0], v_cache=None if mla else flat[1], total_context_len=sum(n),
+                               cu_seqlens_kv=cu, context_batch_size=len(n), is_mla=mla, num_heads=H, head_dim=D)
+    pick = list(range(B))
+    if kind == "shared":
+        pick = [0] * B
+    if kind == "index":
+        pick = [b % 2 for b in range(B)]
+        kw["context_index"] = torch.tensor(pick, dtype=torch.int32, device=device)
+    return cache, [(rows[i][0], rows[i][-1]) for i in pick], kw
+
+
+def _run(device, dtype, *, lens, N, H, D, ctx, kind, mla=False, scale=None, seed=0, parents=None, spoil=None):
+    r = random.Random(seed)
+    g = torch.Generator().manual_seed(seed)
+    B = len(lens)
+    scale = D**-0.5 if scale is None else scale
+    q, k, v = (torch.randn((B, H, N, D), generator=g).to(dtype).to(device) for _ in range(3))
+    if mla:
+        v = k
+    parents = _random_parents(r, lens) if parents is None else parents
+    meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+    tree = build_tree_metadata(torch.tensor(parents, device=device), meta)
+    cache, rows, kw = _context(kind, ctx, H, D, mla, dtype, device, seed)
+    if spoil is not None:
+        spoil(k, v)
+    out = flash_attn_mlm_tree(q, k, v, H, meta, tree, scale, cache, None if cache is None else 0, is_mla=mla, **kw)
+    T, at, seen = sum(lens), 0, ref.ancestors(parents, lens)
+    got = out.view(H, T, D)
+    for b, n in enumerate(lens):
+        for h in range(H if n else 0):
+            j = 0 if mla else h
+            _close(got[h, at : at + n], q[b, h, :n], k[b, j, :n], v[b, j, :n], seen[at : at + n], scale,
+                   rows[b][0][j], rows[b][1][j], dtype)
+        at += n
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("kind", ["none", "packed", "paged"])
+def test_attention(dtype, D, kind, device):
+    if dtype == "fp32" and kind == "paged":
+        pytest.skip("paged contexts are bf16 / fp16")
+    if D == 16 and kind == "paged":
+        pytest.skip("no paged kernel of head dim 16")
+    _run(device, DT[dtype], lens=[40, 1, 0, 17], N=41, H=3, D=D, ctx=[70, 0, 5, 129], kind=kind, seed=D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("kind", ["none", "packed", "paged", "index"])
+def test_mla(dtype, kind, device):
+    _run(device, DT[dtype], lens=[5, 33, 1], N=33, H=4, D=512, ctx=[300, 65, 0], kind=kind, mla=True, seed=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, kind", [("bf16", "shared"), ("fp16", "index"), ("fp32", "shared"), ("bf16", "index")])
+def test_shared_and_indexed_contexts(dtype, kind, device):
+    _run(device, DT[dtype], lens=[9, 20, 3], N=20, H=2, D=64, ctx=[200, 77, 1], kind=kind, seed=4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("chain", [False, True])
+def test_long_drafts_and_long_contexts(dtype, chain, device):
+    lens = [256, 200, 1]
+    parents = [i - 1 for n in lens for i in range(n)] if chain else None
+    _run(device, DT[dtype], lens=lens, N=256, H=2, D=64, ctx=[5000, 1, 3], kind="packed", seed=5, parents=parents)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_scales(dtype, scale, device):
+    _run(device, DT[dtype], lens=[30, 2], N=30, H=2, D=64, ctx=[90, 0], kind="packed", scale=scale, seed=6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_values_that_are_not_finite(dtype, value, device):
+    """Token 3 holds NaN or an infinity in K or V: the rows that do not see it are as without it,
+    those that see it are not finite.  So is padding behind a sequence."""
+    lens, N, H, D = [40, 7], 44, 2, 64
+    parents = [-1 if i < 4 else i - 4 for n in lens for i in range(n)]  # four chains
+
+    def run(spoil):
+        r = torch.Generator().manual_seed(8)
+        q, k, v = (torch.randn((2, H, N, D), generator=r).to(DT[dtype]).to(device) for _ in range(3))
+        spoil(k, v)
+        meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+        tree = build_tree_metadata(torch.tensor(parents, device=device), meta)
+        cache, _, _ = _context("packed", [30, 3], H, D, False, DT[dtype], device, 1)
+        return unpack_from_kernel(flash_attn_mlm_tree(q, k, v, H, meta, tree, 0.125, cache, 0), meta, H)
+
+    clean = run(lambda k, v: None)
+    rows = torch.zeros((2, N), dtype=torch.bool, device=device)
+    rows[0, 3:40:4] = rows[1, 3] = True
+
+    def pad(k, v):
+        for b, n in enumerate(lens):
+            k[b, :, n:] = value
+            v[b, :, n:] = value
+
+    assert torch.equal(run(pad), clean)
+    for what in ("k", "v"):
+        def spoil(k, v):
+            (k if what == "k" else v)[:, :, 3, 5] = value
+
+        got = run(spoil)
+        for h in range(H):
+            assert torch.equal(got[:, h][~rows], clean[:, h][~rows])
+            if what == "v":
+                assert not got[:, h][rows][:, 5].isfinite().any()
+                keep = [d for d in range(D) if d != 5]
+                torch.testing.assert_close(got[:, h][rows][:, keep], clean[:, h][rows][:, keep], rtol=4 * torch.finfo(
+                    DT[dtype]).eps, atol=4 * torch.finfo(DT[dtype]).eps)
+            elif value != value:
+                assert got[:, h][rows].isnan().all()
+
+
+@pytest.mark.gpu
+def test_chain_of_one_is_the_ordinary_call(device):
+    """One token a sequence sees its context and itself, as in flash_attn_mlm_compressed."""
+    _run(device, torch.bfloat16, lens=[1] * 9, N=1, H=4, D=128, ctx=[700] * 9, kind="paged", seed=9)
+
+
+@pytest.mark.gpu
+def test_refusals(device):
+    q = torch.zeros((1, 2, 3, 64), dtype=torch.bfloat16, device=device)
+    meta = build_pack_metadata(torch.tensor([3], device=device), 3, 32)
+    tree = build_tree_metadata(torch.tensor([-1, 0, 0], device=device), meta)
+    with pytest.raises(ValueError, match="same dtype"):
+        flash_attn_mlm_tree(q, q.float(), q, 2, meta, tree, 1.0)
+    with pytest.raises(ValueError, match="layer_id|inference_cache"):
+        flash_attn_mlm_tree(q, q, q, 2, meta, tree, 1.0, InferenceCache())
+    with pytest.raises(ValueError, match="HEAD_DIM"):
+        x = torch.zeros((1, 2, 3, 48), device=device)
+        flash_attn_mlm_tree(x, x, x, 2, meta, tree, 1.0)
+    empty = build_pack_metadata(torch.tensor([0], device=device), 3, 32)
+    none = build_tree_metadata(torch.zeros(0, dtype=torch.int32, device=device), empty)
+    assert flash_attn_mlm_tree(q, q, q, 2, empty, none, 1.0).shape == (0, 64)
+
+
+@pytest.mark.gpu
+def test_repeated_calls_streams_and_graphs(device):
+    """The memoised second call, another layout, another stream, two captured graphs replayed in
+    turn with eager work between: all the bits of the first call."""
+    H, D, N, lens = 4, 64, 24, [24, 5, 11]
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn((3, H, N, D), generator=g).bfloat16().to(device) for _ in range(3))
+    meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+    trees = [build_tree_metadata(torch.tensor(_random_parents(random.Random(s), lens), device=device), meta)
+             for s in range(2)]
+    cache, _, _ = _context("paged", [900, 2000, 64], H, D, False, torch.bfloat16, device, 2)
+
+    def call(t, q=q):
+        return flash_attn_mlm_tree(q, k, v, H, meta, t, 0.125, cache, 0)
+
+    want = [call(t).clone() for t in trees]
+    assert not torch.equal(*want)
+    assert torch.equal(call(trees[0]), want[0])
+    strided = torch.empty((3, N, H, D), dtype=q.dtype, device=device).transpose(1, 2).copy_(q)
+    assert torch.equal(call(trees[0], strided), want[0])
+    odd = torch.empty(q.numel() + 1, dtype=q.dtype, device=device)[1:].view(q.shape).copy_(q)
+    assert torch.equal(call(trees[0], odd), want[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = call(trees[1])
+    side.synchronize()
+    assert torch.equal(other, want[1])
+    graphs, outs = [], []
+    for t in trees:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call(t))
+        graphs.append(graph)
+    for _ in range(3):
+        for i in (0, 1):
+            outs[i].fill_(7)
+            graphs[i].replay()
+            call(trees[1 - i])
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], want[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_speculative_decoding_over_a_paged_cache(dtype, device):
+    """The operators as a server uses them: prompts are stored, then drafted trees attend to the
+    pages, one branch is accepted and stored.  At every step the accepted branch's rows are what
+    attention over the whole accepted text gives them at 64 bits."""
+    dt, H, D, B, N = DT[dtype], 4, 64, 3, 12
+    r, g = random.Random(0), torch.Generator().manual_seed(0)
+    P, width = 20, 4
+    pools = [torch.full((H, P, PAGE, D), float("nan"), dtype=dt, device=device) for _ in range(2)]
+    free = torch.randperm(P, generator=g).to(torch.int32).to(device)
+    cos, sin = (f(torch.arange(300)[:, None] * 100.0 ** (-torch.arange(32) / 32)).float().to(device)
+                for f in (torch.cos, torch.sin))
+    lens = torch.zeros(B, dtype=torch.int32, device=device)
+    table = torch.full((B, width), -1, dtype=torch.int32, device=device)
+    cache = InferenceCache()
+    cache.prefill_paged_kv_cache(0, k_pages=pools[0], v_pages=pools[1], block_table=table, context_lens=lens,
+                                 is_mla=False, num_heads=H, head_dim=D)
+    text = [[torch.zeros((H, 0, D), device=device, dtype=dt) for _ in range(2)] for _ in range(B)]  # stored k, v
+
+    for step in range(6):
+        n_new = [r.randint(40, 100) for _ in range(B)] if step == 0 else [r.randint(1, N) for _ in range(B)]
+        n = max(n_new)
+        meta = build_pack_metadata(torch.tensor(n_new, device=device), n, 32)
+        q, k, v = (torch.randn((B, H, n, D), generator=g).to(dt).to(device) for _ in range(3))
+        parents = [i - 1 for m in n_new for i in range(m)] if step == 0 else _random_parents(r, n_new)
+        tree = build_tree_metadata(torch.tensor(parents, device=device), meta, context_lens=lens)
+        q, k = qk_norm_rope(q, k, cos=cos, sin=sin, positions=tree.positions, q_meta=meta)
+        out = flash_attn_mlm_tree(q, k, v, H, meta, tree, 0.125, cache, 0).view(H, -1, D)
+        seen = ref.ancestors(parents, n_new)
+        keep, at = [], 0
+        for b, m in enumerate(n_new):  # accept the branch that ends in a token drawn at random
+            branch = sorted(seen[at + (m - 1 if step == 0 else r.randrange(m))])
+            keep += [i in branch for i in range(m)]
+            idx = torch.tensor(branch, device=device)
+            kb, vb = (torch.cat([old, x[b, :, idx]], 1) for old, x in zip(text[b], (k, v)))
+            for h in range(H):
+                c = text[b][0].shape[1]
+                _close(out[h, at + idx], q[b, h, idx], kb[h, c:], vb[h, c:], [set(range(i + 1)) for i in range(len(branch))],
+                       0.125, kb[h, :c], vb[h, :c], dt)
+            text[b] = [kb, vb]
+            at += m
+        plan = build_block_table(meta, lens, free_pages=free, block_table=table,
+                                 keep=torch.tensor(keep, device=device))
+        cache.append_paged_kv_cache(0, k=k, v=v, q_meta=meta, plan=plan)
+        lens, table, free = plan.context_lens, plan.block_table, free[plan.pages_taken :]
+        assert lens.tolist() == [t[0].shape[1] for t in text]
+        for b in range(B):  # the pages hold the text
+            rows = torch.arange(int(lens[b]), device=device)
+            slot = table[b].long()[rows // PAGE] * PAGE + rows % PAGE
+            for pool, t in zip(pools, text[b]):
+                assert torch.equal(pool.view(H, -1, D)[:, slot], t)
