@@ -75,60 +75,70 @@ FMLM_DEV void bt_rank(const BtParams& p, const BtSpace& w, int b) {
   if (lane == 0) w.count[b] = n;
 }
 
-// the requests' prefix sums, by one workgroup of kBtThreads threads
+// The requests' prefix sums, by one workgroup of kBtThreads threads.  Each round scans the
+// pages that kBtThreads requests lack beside their old lengths, then the rows they end up
+// with (the free list may have cut them).
 FMLM_DEV void bt_scan(const BtParams& p, const BtSpace& w) {
   __shared__ int2 part[kBtThreads / 64];
   __shared__ int2 total;
-  __shared__ int sum[4];  // as summary
-  if (threadIdx.x < 4) sum[threadIdx.x] = 0;
+  __shared__ int bad;
+  if (threadIdx.x == 0) bad = 0;
   __syncthreads();
   const int cap_in = p.table_in ? min(p.in_pages, p.max_pages) * FMLM_PAGE_ROWS : 0;
   const int cap_out = p.max_pages * FMLM_PAGE_ROWS;
-  int taken = 0, stored = 0, lacking = 0, bad = 0;  // of this thread's requests
-  int2 carry = make_int2(0, 0);                     // pages, context rows of the requests before
+  int pages = 0, rows = 0, rows_old = 0;  // of the requests before
   for (int b0 = 0; b0 < p.B; b0 += kBtThreads) {
     const int b = b0 + threadIdx.x;
     int old = 0, cnt = 0, need = 0, have = 0;
+    bool over = false;
     if (b < p.B) {
       const int64_t raw = bt_index(p.old_lens, p.flags & FMLM_BT_OLD_I64, b);
-      old = (int)(raw < 0 ? 0 : raw > cap_in ? cap_in : raw);
       const int c0 = p.cu_seqlens[b], c1 = min(p.cu_seqlens[b + 1], p.T);
+      old = (int)(raw < 0 ? 0 : raw > cap_in ? cap_in : raw);
       cnt = p.keep ? w.count[b] : max(c1 - c0, 0);
-      const bool over = raw != old || cnt > cap_out - old;
-      bad += over;
+      over = raw != old || cnt > cap_out - old;
       cnt = min(cnt, cap_out - old);
       have = pages_of(old);
       need = pages_of(old + cnt) - have;
     }
-    // the free list: what a request lacks in it, its later tokens cannot be stored in
-    int2 v = block_scan<kBtThreads>(make_int2(need, 0), part);
-    const int base = carry.x + v.x - need;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(over);
+    if (m && (threadIdx.x & 63) == 0) atomicAdd(&bad, __popcll(m));
+    const int2 v = block_scan<kBtThreads>(make_int2(need, old), part);
+    const int base = pages + v.x - need;
+    // what the free list lacks, the request's later tokens cannot be stored in
     const int got = max(0, min(need, p.n_free - base));
     if (got < need) cnt = max(0, min(cnt, (have + got) * FMLM_PAGE_ROWS - old));
-    int2 r = block_scan<kBtThreads>(make_int2(0, b < p.B ? old + cnt : 0), part);
+    const int2 r = block_scan<kBtThreads>(make_int2(cnt, 0), part);
     if (b < p.B) {
       w.old[b] = old;
       w.base[b] = base;
       w.count[b] = cnt;
       p.new_lens[b] = old + cnt;
-      p.cu_kv[b + 1] = carry.y + r.y;
-      taken += got;
-      lacking += need - got;
-      stored += cnt;
+      p.cu_kv[b + 1] = rows + v.y + r.x;
     }
-    if (threadIdx.x == kBtThreads - 1) total = make_int2(v.x, r.y);
-    __syncthreads();
-    carry.x += total.x;
-    carry.y += total.y;
-    __syncthreads();
+    if (b0 + kBtThreads < p.B) {  // the next round's start
+      if (threadIdx.x == kBtThreads - 1) total = make_int2(v.x, v.y);
+      __syncthreads();
+      pages += total.x;
+      rows_old += total.y;
+      rows += total.y;
+      __syncthreads();
+      if (threadIdx.x == kBtThreads - 1) total.x = r.x;
+      __syncthreads();
+      rows += total.x;
+      __syncthreads();
+    } else if (threadIdx.x == kBtThreads - 1) {
+      const int need_all = pages + v.x, taken = min(need_all, p.n_free);
+      p.summary[0] = taken;
+      p.summary[1] = need_all - taken;
+      p.summary[2] = bad;  // the scans' barriers lie between
+      p.summary[3] = rows + v.y + r.x - (rows_old + v.y);
+    }
   }
-  atomicAdd(&sum[0], taken);
-  atomicAdd(&sum[1], lacking);
-  atomicAdd(&sum[2], bad);
-  atomicAdd(&sum[3], stored);
-  if (threadIdx.x == 0) p.cu_kv[0] = 0;
-  __syncthreads();
-  if (threadIdx.x < 4) p.summary[threadIdx.x] = sum[threadIdx.x];
+  if (threadIdx.x == 0) {
+    p.cu_kv[0] = 0;
+    if (p.B == 0) p.summary[0] = p.summary[1] = p.summary[2] = p.summary[3] = 0;
+  }
 }
 
 // page i of request b, or -1
@@ -143,7 +153,8 @@ FMLM_DEV int bt_page(const BtParams& p, const BtSpace& w, int b, int i) {
 FMLM_DEV void bt_fill(const BtParams& p, const BtSpace& w, int64_t first, int64_t step) {
   const int64_t entries = (int64_t)p.B * p.max_pages;
   for (int64_t e = first; e < entries; e += step) {
-    const int b = (int)(e / p.max_pages);
+    // (64-bit divisions take some hundred instructions)
+    const int b = entries <= 0x7fffffff ? (int)((uint32_t)e / (uint32_t)p.max_pages) : (int)(e / p.max_pages);
     p.block_table[e] = bt_page(p, w, b, (int)(e - (int64_t)b * p.max_pages));
   }
   for (int64_t t = first; t < p.T; t += step) {

@@ -9,7 +9,7 @@ fields, the same lookup keys, the same ValueError messages, and the same
 
 from __future__ import annotations
 
-from dataclasses import dataclass, field, replace
+from dataclasses import dataclass, field
 from typing import TYPE_CHECKING
 
 import torch
@@ -456,9 +456,9 @@ class InferenceCache:
             if v is None:
                 raise ValueError("non-MLA append requires v")
             pairs.append((v, entry.v_cache))
+        shape = (q_meta.B, entry.num_heads, q_meta.N, d) if k.ndim == 4 else (h_kv * t, d)
         for (x, pool), what in zip(pairs, ("k", "v")):
-            shapes = ((q_meta.B, entry.num_heads, q_meta.N, d), (h_kv * t, d))
-            if tuple(x.shape) not in shapes or x.ndim != k.ndim:
+            if x.shape != shape:
                 raise ValueError(f"{what} must be padded [B, H, N, D] or packed [H_kv * T, D], as q_meta describes it")
             if x.dtype != entry.dtype or x.device != entry.device:
                 raise ValueError(f"{what} dtype/device must match the cached entry")
@@ -470,16 +470,26 @@ class InferenceCache:
         if table.ndim != 2 or table.dtype != torch.int32 or int(table.shape[0]) < 1 \
                 or cu.dtype != torch.int32 or tuple(cu.shape) != (int(table.shape[0]) + 1,):
             raise ValueError("plan.block_table must be rank-2 int32 and plan.cu_seqlens_kv have a row more than it")
-        if any(x.device != entry.device for x in (slots, table, cu, q_meta.token_indices)):
+        dev = entry.device
+        if slots.device != dev or table.device != dev or cu.device != dev or q_meta.token_indices.device != dev:
             raise ValueError("plan and q_meta must be on the cached entry's device")
         from flash_mlm.host.paged import paged_append
 
         if t > 0:
             paged_append(pairs, heads=h_kv, d=d, q_meta=q_meta, slots=slots.contiguous(),
                          pool_rows=int(entry.total_context_len))
-        self._layer_kv[key] = replace(
-            entry, block_table=table.contiguous(), cu_seqlens_kv=cu.contiguous(),
+        self._layer_kv[key] = LayerKVEntry(
+            k_cache=entry.k_cache,
+            v_cache=entry.v_cache,
+            total_context_len=entry.total_context_len,
+            cu_seqlens_kv=cu.contiguous(),
             context_batch_size=int(table.shape[0]),
+            is_mla=entry.is_mla,
+            num_heads=entry.num_heads,
+            head_dim=d,
+            dtype=entry.dtype,
+            device=entry.device,
+            block_table=table.contiguous(),
         )
 
     def get_kv_cache(

@@ -15,7 +15,7 @@ import torch
 from flash_mlm import _lib
 from flash_mlm.host.cache import PackMetadata
 from flash_mlm.host.host import _wants_grad, rows16
-from flash_mlm.host.host_utils import _device_scope, require_cuda_tensors, validate_head_dim_supported
+from flash_mlm.host.host_utils import require_cuda_tensors, validate_head_dim_supported
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _INTS = (torch.int32, torch.int64)
@@ -28,75 +28,70 @@ def aligned16(t: torch.Tensor) -> torch.Tensor:
 
 
 class _Call:
-    """The checked arguments of one call, and its parameter blocks."""
+    """The checked arguments of one call as a parameter block without the rows' addresses."""
 
-    __slots__ = ("shapes", "heads", "layout", "B", "N", "D", "rows", "flags", "eps", "cu", "tokens", "table_rows", "R")
+    __slots__ = ("block", "packed", "shapes", "keep")
 
-    def params(self, xs, ws, cos, sin, positions, context_lens):
-        p = _lib.NormRopeParams()
-        p.dtype = _lib.dtype_code(xs[0].dtype)
-        w = ws[0] if ws[0] is not None else ws[1]
-        p.w_dtype = _lib.DTYPE_F32 if w is None else _lib.dtype_code(w.dtype)
-        p.flags, p.layout = self.flags, self.layout
-        p.B, p.N, p.D, p.rotary_dim = self.B, self.N, self.D, self.R
-        p.rows, p.table_rows, p.eps = self.rows, self.table_rows, self.eps
-        p.cos, p.sin = _lib.ptr(cos), _lib.ptr(sin)
-        p.cu_seqlens, p.token_indices = _lib.ptr(self.cu), _lib.ptr(self.tokens)
-        p.positions, p.offsets = _lib.ptr(positions), _lib.ptr(context_lens)
-        return p
-
-    def strides(self, x: torch.Tensor):
-        if self.layout == _lib.LAYOUT_PACKED:
-            return 0, self.rows * self.D, self.D
-        return x.stride(0), x.stride(1), x.stride(2)
-
-    def tensor(self, t, i: int, x, y, w, dy=None, dw=None) -> None:
-        t.heads = self.heads[i]
-        t.x, (t.x_sb, t.x_sh, t.x_sn) = x.data_ptr(), self.strides(x)
-        t.y, (t.y_sb, t.y_sh, t.y_sn) = y.data_ptr(), self.strides(y)
-        if dy is not None:
-            t.dy, (t.dy_sb, t.dy_sh, t.dy_sn) = dy.data_ptr(), self.strides(dy)
-        if w is not None:
-            t.weight = w.data_ptr()
-            t.w_sh = self.D if w.ndim == 2 else 0
-        t.dweight = _lib.ptr(dw)
+    def put(self, t, x, y) -> None:
+        """Rows in and out of tensor ``t`` of a block (packed rows: strides are the block's)."""
+        t.x, t.y = x.data_ptr(), y.data_ptr()
+        if not self.packed:
+            t.x_sb, t.x_sh, t.x_sn, _ = x.stride()
 
 
-def _forward(call: _Call, q, k, wq, wk, cos, sin, positions, context_lens):
-    outs = [torch.empty(s, dtype=q.dtype, device=q.device) for s in call.shapes]
-    if call.rows:
-        p = call.params((q, k), (wq, wk), cos, sin, positions, context_lens)
-        call.tensor(p.q, 0, q, outs[0], wq)
-        call.tensor(p.k, 1, k, outs[1], wk)
-        with _device_scope(q.device):
-            rc = _lib.load().fmlm_norm_rope(p, _lib.stream_of(q.device))
-        _lib.check(rc, "fmlm_norm_rope")
-    return tuple(outs)
+def _rows_out(call: _Call, q, k):
+    return (torch.empty(call.shapes[0], dtype=q.dtype, device=q.device),
+            torch.empty(call.shapes[1], dtype=k.dtype, device=k.device))
 
 
-def _backward(call: _Call, xs, ws, angles, dys, needs):
+def _run(entry, name: str, p, device) -> None:
+    if device.index == torch.cuda.current_device():
+        rc = entry(p, _lib.stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            rc = entry(p, _lib.stream_of(device))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _forward(call: _Call, q, k):
+    outs = _rows_out(call, q, k)
+    p = call.block
+    if p.rows:
+        call.put(p.q, q, outs[0])
+        call.put(p.k, k, outs[1])
+        _run(_lib.load().fmlm_norm_rope, "fmlm_norm_rope", p, q.device)
+    return outs
+
+
+def _backward(call: _Call, xs, ws, dys, needs):
     """Gradients (dq, dk, dwq, dwk); ``needs`` says which are wanted, None in ``dys`` is zero."""
     lib = _lib.load()
     dev = xs[0].device
-    p = call.params(xs, ws, *angles)
+    p = _lib.NormRopeParams.from_buffer_copy(call.block)  # (a graph can be walked more than once)
     dxs, dws, keep = [None, None], [None, None], []
     for i, t in enumerate((p.q, p.k)):
         if dys[i] is None or not (needs[i] or needs[2 + i]):
+            t.heads = 0
             continue
         dy = rows16(dys[i])
-        dxs[i] = torch.empty(call.shapes[i], dtype=xs[i].dtype, device=dev)
-        if ws[i] is not None and needs[2 + i]:
-            dws[i] = torch.empty(ws[i].shape, dtype=ws[i].dtype, device=dev)
-        call.tensor(t, i, xs[i], dxs[i], ws[i], dy, dws[i])
+        dx = dxs[i] = torch.empty(call.shapes[i], dtype=xs[i].dtype, device=dev)
+        call.put(t, xs[i], dx)
+        t.dy = dy.data_ptr()
+        if call.packed:
+            t.dy_sh, t.dy_sn = t.y_sh, t.y_sn
+        else:
+            t.dy_sb, t.dy_sh, t.dy_sn, _ = dy.stride()
+        if needs[2 + i]:
+            dw = dws[i] = torch.empty(ws[i].shape, dtype=ws[i].dtype, device=dev)
+            t.dweight = dw.data_ptr()
         keep.append(dy)
     if keep:
-        nbytes = int(lib.fmlm_norm_rope_bwd_workspace_bytes(p))
+        nbytes = lib.fmlm_norm_rope_bwd_workspace_bytes(p)
         _lib.check(nbytes if nbytes < 0 else 0, "fmlm_norm_rope_bwd_workspace_bytes")
-        ws_buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        p.workspace, p.workspace_bytes = ws_buf.data_ptr(), nbytes
-        with _device_scope(dev):
-            rc = lib.fmlm_norm_rope_bwd(p, _lib.stream_of(dev))
-        _lib.check(rc, "fmlm_norm_rope_bwd")
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        p.workspace, p.workspace_bytes = buf.data_ptr(), nbytes
+        _run(lib.fmlm_norm_rope_bwd, "fmlm_norm_rope_bwd", p, dev)
     return (*dxs, *dws)
 
 
@@ -107,13 +102,13 @@ class _NormRope(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         # saved so that autograd rejects a backward after any of them changed in place
         ctx.save_for_backward(q, k, wq, wk, cos, sin, positions, context_lens)
-        return _forward(call, q, k, wq, wk, cos, sin, positions, context_lens)
+        return _forward(call, q, k)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
-        q, k, wq, wk, *angles = ctx.saved_tensors
-        grads = _backward(ctx.call, (q, k), (wq, wk), angles, (dq, dk), ctx.needs_input_grad[1:5])
+        q, k, wq, wk, *_ = ctx.saved_tensors
+        grads = _backward(ctx.call, (q, k), (wq, wk), (dq, dk), ctx.needs_input_grad[1:5])
         return (None, *grads, None, None, None, None)
 
 
@@ -146,25 +141,22 @@ def _capture_leaves(*tensors) -> list[torch.Tensor]:
 
 
 def _check_gain(w, what: str, heads: int, d: int, device):
-    if w is None:
-        return None
-    if tuple(w.shape) not in ((d,), (heads, d)):
+    ws = w.shape
+    if ws[-1:] != (d,) or not (len(ws) == 1 or (len(ws) == 2 and ws[0] == heads)):
         raise ValueError(f"{what} must be [head_dim] or [heads, head_dim]")
     if w.dtype not in _FLOATS or w.device != device:
         raise ValueError(f"{what} must be bf16, fp16 or fp32 on the device of q and k")
     return aligned16(w)
 
 
-def _check_index(t, what: str, shape, device, lo_hi=None):
+def _check_index(t, what: str, shape, device, lo_hi):
     """An int32 / int64 tensor on ``device``; one on the CPU is range-checked and copied."""
-    if t is None:
-        return None
-    if not isinstance(t, torch.Tensor) or t.dtype not in _INTS or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what} must be an int32 or int64 tensor of shape {tuple(shape)}")
-    if not t.is_cuda and lo_hi is not None and t.numel():
+    if not isinstance(t, torch.Tensor) or t.dtype not in _INTS or t.shape != shape:
+        raise ValueError(f"{what} must be an int32 or int64 tensor of shape {shape}")
+    if not t.is_cuda and t.numel():
         if int(t.min()) < lo_hi[0] or int(t.max()) >= lo_hi[1]:
             raise ValueError(f"{what} values must lie in [{lo_hi[0]}, {lo_hi[1]})")
-    return t.to(device).contiguous()
+    return (t if t.device == device else t.to(device)).contiguous()
 
 
 def qk_norm_rope(
@@ -206,97 +198,129 @@ def qk_norm_rope(
     into a graph together with its backward raises ValueError while outputs of earlier calls
     on the same leaves are alive (autograd would run part of the backward on their stream).
     """
-    for t in (q, k):
-        if t.ndim not in (2, 4) or t.ndim != q.ndim:
-            raise ValueError("q and k must both be rank-4 [B, H, N, D] or packed rank-2 [H*T, D]")
-    d = int(q.shape[-1])
-    if int(k.shape[-1]) != d:
+    qs, ks, dtype, dev = q.shape, k.shape, q.dtype, q.device
+    rank = len(qs)
+    if rank not in (2, 4) or len(ks) != rank:
+        raise ValueError("q and k must both be rank-4 [B, H, N, D] or packed rank-2 [H*T, D]")
+    d = qs[-1]
+    if ks[-1] != d:
         raise ValueError("q and k must have the same head_dim")
     validate_head_dim_supported(d, is_mla=True)
-    if q.dtype not in _FLOATS or k.dtype != q.dtype:
+    if dtype not in _FLOATS or k.dtype != dtype:
         raise ValueError("q and k must be of one dtype: bf16, fp16 or fp32")
-    if k.device != q.device:
+    if k.device != dev:
         raise ValueError("q and k must be on one device")
     require_cuda_tensors(q, k, q_weight, k_weight, cos, sin)
-    dev = q.device
     if q_meta is not None and q_meta.cu_seqlens.device != dev:
         raise ValueError("q_meta must be on the device of q and k")
 
-    c = _Call()
-    c.D, c.cu, c.tokens = d, None, None
-    if q.ndim == 4:
-        b, _, n, _ = (int(x) for x in q.shape)
-        if (int(k.shape[0]), int(k.shape[2])) != (b, n):
+    call = _Call()
+    p = call.block = _lib.NormRopeParams()
+    cu = tokens = None
+    packed = call.packed = rank == 2
+    if not packed:
+        b, hq, n, _ = qs
+        hk = ks[1]
+        if ks[0] != b or ks[2] != n:
             raise ValueError("q and k must have the same batch and length")
         if q_meta is not None:
             if q_meta.B != b or q_meta.N != n:
                 raise ValueError("q_meta shape metadata does not match q/k padded shape")
-            c.cu = q_meta.cu_seqlens
-        if num_heads is not None and num_heads != int(q.shape[1]):
+            cu = q_meta.cu_seqlens
+        if num_heads is not None and num_heads != hq:
             raise ValueError("q head dimension must match num_heads")
-        c.layout, c.B, c.N, c.rows = _lib.LAYOUT_PADDED, b, n, b * n
-        c.heads = (int(q.shape[1]), int(k.shape[1]))
-        pos_shape = (b, n) if q_meta is None else (int(q_meta.total_tokens),)
+        rows = b * n
+        for t, h in ((p.q, hq), (p.k, hk)):
+            t.y_sb, t.y_sh, t.y_sn = h * n * d, n * d, d
     else:
         if q_meta is not None:
-            b, n, t = q_meta.B, q_meta.N, int(q_meta.total_tokens)
-            c.cu, c.tokens = q_meta.cu_seqlens, q_meta.token_indices
+            b, n, rows = q_meta.B, q_meta.N, q_meta.total_tokens
+            cu, tokens = q_meta.cu_seqlens, q_meta.token_indices
         else:
-            if num_heads is None or num_heads < 1 or int(q.shape[0]) % num_heads:
+            if num_heads is None or num_heads < 1 or qs[0] % num_heads:
                 raise ValueError("packed q needs q_meta, or num_heads that divides its rows")
-            b, t = 1, int(q.shape[0]) // num_heads
-            n = t
-        c.heads = tuple(int(x.shape[0]) // t if t else 0 for x in (q, k))
-        if any(int(x.shape[0]) != h * t for x, h in zip((q, k), c.heads)):
+            b, n = 1, qs[0] // num_heads
+            rows = n
+        hq, hk = (qs[0] // rows, ks[0] // rows) if rows else (0, 0)
+        if qs[0] != hq * rows or ks[0] != hk * rows:
             raise ValueError("packed q and k rows must be a multiple of the token count")
-        if num_heads is not None and t and num_heads != c.heads[0]:
+        if num_heads is not None and rows and num_heads != hq:
             raise ValueError("q first dim must equal num_heads * tokens")
-        c.layout, c.B, c.N, c.rows = _lib.LAYOUT_PACKED, b, n, t
-        pos_shape = (t,)
-    c.shapes = (tuple(q.shape), tuple(k.shape))
-    if c.B * c.N > 0x7FFFFFFF:
+        p.layout = _lib.LAYOUT_PACKED
+        for t in (p.q, p.k):
+            t.x_sh = t.y_sh = rows * d
+            t.x_sn = t.y_sn = d
+    call.shapes = (qs, ks)
+    if b * n > 0x7FFFFFFF:
         raise ValueError("q and k must have fewer than 2**31 tokens")
+    p.dtype = _lib.dtype_code(dtype)
+    p.B, p.N, p.D, p.rows = b, n, d, rows
+    p.q.heads, p.k.heads = hq, hk
+    if cu is not None:
+        p.cu_seqlens = cu.data_ptr()
+    if tokens is not None:
+        p.token_indices = tokens.data_ptr()
 
-    if not norm and (q_weight is not None or k_weight is not None):
+    flags = 0
+    p.w_dtype = _lib.DTYPE_F32
+    wq, wk = q_weight, k_weight
+    if norm:
+        if not (math.isfinite(eps) and eps >= 0):
+            raise ValueError("eps must be finite and >= 0")
+        p.eps = eps
+        flags = _lib.NR_NORM
+        if wq is not None:
+            wq = _check_gain(wq, "q_weight", hq, d, dev)
+            p.w_dtype = _lib.dtype_code(wq.dtype)
+            p.q.weight, p.q.w_sh = wq.data_ptr(), d if wq.ndim == 2 else 0
+        if wk is not None:
+            wk = _check_gain(wk, "k_weight", hk, d, dev)
+            if wq is not None and wq.dtype != wk.dtype:
+                raise ValueError("q_weight and k_weight must have the same dtype")
+            p.w_dtype = _lib.dtype_code(wk.dtype)
+            p.k.weight, p.k.w_sh = wk.data_ptr(), d if wk.ndim == 2 else 0
+    elif wq is not None or wk is not None:
         raise ValueError("gains need norm=True")
-    if not norm and cos is None:
+    elif cos is None:
         raise ValueError("nothing to do: norm=False and no cos/sin tables")
-    if norm and not (math.isfinite(eps) and eps >= 0):
-        raise ValueError("eps must be finite and >= 0")
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise ValueError("q_weight and k_weight must have the same dtype")
-    wq = _check_gain(q_weight, "q_weight", c.heads[0], d, dev)
-    wk = _check_gain(k_weight, "k_weight", c.heads[1], d, dev)
 
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
-    c.R, c.table_rows = 0, 0
     if cos is not None:
-        if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 \
+        cs = cos.shape
+        if len(cs) != 2 or cs != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 \
                 or cos.device != dev or sin.device != dev:
             raise ValueError("cos and sin must be fp32 tables [positions, rotary_dim / 2] on the device of q and k")
-        c.table_rows, c.R = int(cos.shape[0]), 2 * int(cos.shape[1])
-        if c.R < 16 or c.R % 16 or c.R > d or c.table_rows < 1:
+        table, r = cs[0], 2 * cs[1]
+        if r < 16 or r % 16 or r > d or table < 1:
             raise ValueError("rotary_dim must be a multiple of 16 and at most head_dim, with at least one position")
         cos, sin = aligned16(cos), aligned16(sin)
+        p.cos, p.sin, p.table_rows, p.rotary_dim = cos.data_ptr(), sin.data_ptr(), table, r
+        if interleaved:
+            flags |= _lib.NR_INTERLEAVED
+        if positions is not None:
+            if context_lens is not None:
+                raise ValueError("positions and context_lens are mutually exclusive")
+            shape = (b, n) if not packed and q_meta is None else (q_meta.total_tokens if q_meta is not None else rows,)
+            positions = _check_index(positions, "positions", shape, dev, (0, table))
+            p.positions = positions.data_ptr()
+            if positions.dtype == torch.int64:
+                flags |= _lib.NR_POSITIONS_I64
+        elif context_lens is not None:
+            context_lens = _check_index(context_lens, "context_lens", (b,), dev, (0, table))
+            p.offsets = context_lens.data_ptr()
+            if context_lens.dtype == torch.int64:
+                flags |= _lib.NR_OFFSETS_I64
     elif positions is not None or context_lens is not None:
         raise ValueError("positions and context_lens need cos and sin")
-    if positions is not None and context_lens is not None:
-        raise ValueError("positions and context_lens are mutually exclusive")
-    positions = _check_index(positions, "positions", pos_shape, dev, (0, c.table_rows))
-    context_lens = _check_index(context_lens, "context_lens", (c.B,), dev, (0, c.table_rows))
-
-    c.eps = float(eps)
-    c.flags = (_lib.NR_NORM if norm else 0) | (_lib.NR_INTERLEAVED if interleaved else 0)
-    if positions is not None and positions.dtype == torch.int64:
-        c.flags |= _lib.NR_POSITIONS_I64
-    if context_lens is not None and context_lens.dtype == torch.int64:
-        c.flags |= _lib.NR_OFFSETS_I64
-    args = (c, rows16(q), rows16(k), wq, wk, cos, sin, positions, context_lens)
+    p.flags = flags
+    q_, k_ = rows16(q), rows16(k)
     if _wants_grad(q, k, q_weight, k_weight):
+        # the block holds the addresses of what is saved, and of these
+        call.keep = (cu, tokens)
         leaves = _capture_leaves(q, k, q_weight, k_weight)
-        out = _NormRope.apply(*args)
+        out = _NormRope.apply(call, q_, k_, wq, wk, cos, sin, positions, context_lens)
         for t in leaves:  # this capture's own graph: later calls of it may share the leaf
             _accumulator(t).metadata["fmlm_captured"] = True
         return out
-    return _forward(*args)
+    return _forward(call, q_, k_)

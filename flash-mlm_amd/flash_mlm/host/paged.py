@@ -108,19 +108,20 @@ def build_block_table(
     p.B, p.N, p.T = b, int(q_meta.N), t
     p.max_pages, p.in_pages = max_pages, 0 if block_table is None else int(block_table.shape[1])
     p.n_free = int(free_pages.numel())
-    table = torch.empty((b, max_pages), dtype=torch.int32, device=dev)
+    p.keep = _lib.ptr(keep)
+    nbytes = lib.fmlm_block_table_workspace_bytes(p)
+    _lib.check(nbytes if nbytes < 0 else 0, "fmlm_block_table_workspace_bytes")
     slots = torch.empty(t, dtype=torch.int64, device=dev)
-    positions = torch.empty(t, dtype=torch.int32, device=dev)
-    small = torch.empty(2 * b + 5, dtype=torch.int32, device=dev)
-    new_lens, cu, summary = small[:b], small[b : 2 * b + 1], small[2 * b + 1 :]
+    # the 32-bit results share one allocation with the workspace
+    table, positions, new_lens, cu, summary, ws = torch.empty(
+        b * max_pages + t + 2 * b + 5 + nbytes // 4, dtype=torch.int32, device=dev
+    ).split_with_sizes((b * max_pages, t, b, b + 1, 4, nbytes // 4))
+    table = table.view(b, max_pages)
     p.old_lens, p.cu_seqlens, p.token_indices = context_lens.data_ptr(), q_meta.cu_seqlens.data_ptr(), \
         q_meta.token_indices.data_ptr()
-    p.keep, p.table_in, p.free_pages = _lib.ptr(keep), _lib.ptr(block_table), free_pages.data_ptr()
+    p.table_in, p.free_pages = _lib.ptr(block_table), free_pages.data_ptr()
     p.block_table, p.slot_mapping, p.positions = table.data_ptr(), slots.data_ptr(), positions.data_ptr()
     p.new_lens, p.cu_kv, p.summary = new_lens.data_ptr(), cu.data_ptr(), summary.data_ptr()
-    nbytes = int(lib.fmlm_block_table_workspace_bytes(p))
-    _lib.check(nbytes if nbytes < 0 else 0, "fmlm_block_table_workspace_bytes")
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
     with _device_scope(dev):
         rc = lib.fmlm_block_table(p, _lib.stream_of(dev))
@@ -136,10 +137,13 @@ def build_block_table(
     return plan
 
 
+_ONE, _PAIR = _lib.PagedTensor * 1, _lib.PagedTensor * 2
+
+
 def paged_append(pairs, *, heads: int, d: int, q_meta: PackMetadata, slots: torch.Tensor, pool_rows: int) -> None:
     """Rows of each (source, pool) pair to their slots in one HIP launch (fmlm_paged_append);
     the kernel of :meth:`InferenceCache.append_paged_kv_cache`."""
-    arr = (_lib.PagedTensor * len(pairs))()
+    arr = _PAIR() if len(pairs) == 2 else _ONE()
     packed = pairs[0][0].ndim == 2
     t = int(q_meta.total_tokens)
     keep = []
@@ -148,7 +152,10 @@ def paged_append(pairs, *, heads: int, d: int, q_meta: PackMetadata, slots: torc
             src = src.contiguous()
         keep.append(src)
         a.src, a.pool = src.data_ptr(), pool.data_ptr()
-        a.s_sb, a.s_sh, a.s_sn = (0, t * d, d) if packed else (src.stride(0), src.stride(1), src.stride(2))
+        if packed:
+            a.s_sh, a.s_sn = t * d, d
+        else:
+            a.s_sb, a.s_sh, a.s_sn, _ = src.stride()
     dev = slots.device
     with _device_scope(dev):
         rc = _lib.load().fmlm_paged_append(
