@@ -371,6 +371,9 @@ struct SplitArgs {
   char* records;
   int32_t rec_bytes;
   int32_t dense_parts;  // 1: not split
+  // FMLM_FLAG_TREE: row t * words of token t's mask over the main keys of its sequence
+  const uint64_t* mask;
+  int32_t words;
 };
 
 // key tiles [tb, te) of a unit's part: the whole range costs no division (the two 64-bit ones
@@ -537,7 +540,7 @@ FMLM_DEV bool resolve_work(const fmlm_attn_params& p, const int4* units, int u, 
       m.vbase = (int64_t)b * v_sb + (int64_t)h * v_sh;
     }
   }
-  if (p.flags & FMLM_FLAG_CTX_ONLY) m.n = 0;
+  if (p.flags & kFlagCtxOnly) m.n = 0;
   return true;
 }
 
@@ -956,11 +959,22 @@ struct Mfma3Cfg {
   static_assert(!PP || (NW == 8 && NINST % NW == 0 && PPB >= 3), "ping-pong: two groups of 4 waves, equal loads");
 };
 
-template <typename T, int D, int QB, int NW, int BK, bool PAGED, int PPB>
+// TREE: a query row attends to the main keys whose bits its mask (spa.mask) has set, one 64-bit
+// word per key tile.  The steps over context tiles are the plain kernel's.  Before a main tile's
+// softmax its scores are masked and their maxima taken again; rows that have seen no key yet
+// keep a maximum of -inf, with 0 in its place where scores are computed against it.  Values
+// that are not finite would spoil the rows that do not see them (0 times inf): a wave looks
+// through the V tile first (a pass over LDS, 0.2 us), and in the rare case takes such rows out of the
+// tile and adds their share row by row.  1 user, 32 drafted tokens, 16 heads, D = 128, 8000
+// paged context rows: the tree's tile adds 1.5 us to the context's 17.2 (a separate kernel for
+// the tree's part took 8.4); 24 users of up to 64 tokens and 500-6000 rows 130 us, the
+// context's part 125.
+template <typename T, int D, int QB, int NW, int BK, bool PAGED, int PPB, bool TREE = false>
 __global__ __launch_bounds__(NW * 64, NW >= 8 ? 1 : 2) void attn_mfma3_kernel(
     const fmlm_attn_params p, const int4* __restrict__ units, const int32_t* __restrict__ hdr, const SplitArgs spa) {
   typedef Mfma3Cfg<T, D, QB, NW, BK, PPB> C;
   typedef typename Mfma<T>::v8 v8;
+  static_assert(!TREE || (PPB == 0 && BK == 64), "a mask word per key tile");
   extern __shared__ __align__(16) char smem_raw[];
   char* const kbuf = smem_raw;                             // [NKBUF][TILEB]
   char* const vbuf = smem_raw + C::NKBUF * C::TILEB;       // [NVBUF][TILEB]
@@ -1267,7 +1281,26 @@ __global__ __launch_bounds__(NW * 64, NW >= 8 ? 1 : 2) void attn_mfma3_kernel(
   };
   // Rescale decision for tile t from the row maxima mx of S(t) (sc), and the -inf mask of
   // the keys past a partial tile's end.
-  auto prepare = [&](int t, f32x4 (&sc)[C::NKB][QB], float (&mx)[QB]) {
+  // the mask word of row block qb for main tile i
+  auto tree_word = [&](int qb, int i) {
+    const int row = (wave * QB + qb) * 16 + l16;
+    return row < w.qcount && i < spa.words ? spa.mask[(int64_t)(w.q0 + w.qpos0 + row) * spa.words + i] : 0ull;
+  };
+  auto tree_mask = [&](int t, f32x4 (&sc)[C::NKB][QB], float (&mx)[QB]) {
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      const uint64_t seen = tree_word(qb, t - nt0) >> (4 * g);  // bit kb*16 + r: the lane's key (kb, r)
+      const uint32_t half[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
+#pragma unroll
+      for (int kb = 0; kb < C::NKB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!(half[kb >> 1] >> ((kb & 1) * 16 + r) & 1)) sc[kb][qb][r] = -INFINITY;
+    }
+    row_max(sc, mx);
+  };
+  auto prepare = [&](auto tree, int t, f32x4 (&sc)[C::NKB][QB], float (&mx)[QB]) {
+    constexpr bool TR = decltype(tree)::value;
     bool need_rescale = false;
     float m_new[QB];
 #pragma unroll
@@ -1280,8 +1313,11 @@ __global__ __launch_bounds__(NW * 64, NW >= 8 ? 1 : 2) void attn_mfma3_kernel(
     if (__builtin_amdgcn_ballot_w64(need_rescale)) {
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
-        const float alpha = fast_exp2(m_i[qb] - m_new[qb]);  // 1 where unchanged, 0 on the first tile
-        const float shift = FP32_SCALE ? (sbase[qb] - m_new[qb]) * rc : sbase[qb] - m_new[qb];  // 0 where unchanged
+        const bool none = TR && m_new[qb] == -INFINITY;  // a row that has seen no key
+        const float alpha = none ? 1.f : fast_exp2(m_i[qb] - m_new[qb]);  // 1 where unchanged, 0 on the first tile
+        const float shift = none         ? 0.f
+                            : FP32_SCALE ? (sbase[qb] - m_new[qb]) * rc
+                                         : sbase[qb] - m_new[qb];  // 0 where unchanged
         m_i[qb] = m_new[qb];
         lsum[qb] *= alpha;
 #pragma unroll
@@ -1316,13 +1352,14 @@ __global__ __launch_bounds__(NW * 64, NW >= 8 ? 1 : 2) void attn_mfma3_kernel(
   constexpr int NMS = C::NKB * QB + QB;  // row-max steps
   u32x4 pf[C::NKS][QB];  // P(t) as packed pairs, the B operand of P V
   float mpart[QB], mhold[QB];
-  auto run_slots = [&](auto s0c, auto s1c, f32x4 (&sc)[C::NKB][QB], f32x4 (&sn)[C::NKB][QB],
+  auto run_slots = [&](auto tree, auto s0c, auto s1c, f32x4 (&sc)[C::NKB][QB], f32x4 (&sn)[C::NKB][QB],
                        float (&mx)[QB], uint32_t kn, uint32_t vt) {
     constexpr int S0 = decltype(s0c)::value, S1 = decltype(s1c)::value;
     f32x4 minit[QB];  // -m_i splat (in the accumulators' units): the initial S accumulators
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      const float mr = FP32_SCALE ? -m_i[qb] * rc : -m_i[qb];
+      float mr = FP32_SCALE ? -m_i[qb] * rc : -m_i[qb];
+      if (decltype(tree)::value && m_i[qb] == -INFINITY) mr = 0.f;
       minit[qb] = f32x4{mr, mr, mr, mr};
     }
     v8 fr[C::LEAD + 1];
@@ -1407,6 +1444,8 @@ __global__ __launch_bounds__(NW * 64, NW >= 8 ? 1 : 2) void attn_mfma3_kernel(
     }
     __builtin_amdgcn_s_setprio(0);
   };
+  typedef std::integral_constant<bool, false> Plain;
+  typedef std::integral_constant<bool, TREE> Tree;
   typedef std::integral_constant<int, 0> Slot0;
   typedef std::integral_constant<int, C::NKF> SlotB;
   typedef std::integral_constant<int, NF> SlotEnd;
@@ -1414,18 +1453,77 @@ __global__ __launch_bounds__(NW * 64, NW >= 8 ? 1 : 2) void attn_mfma3_kernel(
   // One pipeline step (single-group schedule): sc holds S(t) and mx its row maxima;
   // computes sn = S(t+1) from the K tile at byte offset kn and its maxima, consumes V(t) at
   // byte offset vt, refills kdst with K(t+2) and vdst with V(t+2).
-  auto step = [&](int t, f32x4 (&sc)[C::NKB][QB], f32x4 (&sn)[C::NKB][QB], float (&mx)[QB],
+  auto step = [&](auto tree, int t, f32x4 (&sc)[C::NKB][QB], f32x4 (&sn)[C::NKB][QB], float (&mx)[QB],
                   uint32_t kn, uint32_t vt, uint32_t kdst, uint32_t vdst) {
+    constexpr bool TR = decltype(tree)::value;
     if (t + 2 < te) fetch_pair(pc, kdst, vdst);
+    uint64_t bad = 0;  // rows of the V tile with an element that is not finite, taken out of it
+    if constexpr (TR) {
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      constexpr uint32_t E = std::is_same<T, bf16>::value ? 0x7f80u : 0x7c00u;  // exponent of inf and NaN
+      const uint32_t tile = lds_addr(vbuf) + vt;
+      auto piece = [&](int i) { return *(const FMLM_LDS u32x4*)(uintptr_t)(tile + i * 1024 + lane * 16); };
+      auto top = [&](u32x4 x) {  // the larger exponent field of each half
+        u16x2 m = u16x2{0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[e] & 0x7fff7fffu));
+        return m;
+      };
+      u16x2 all = u16x2{0, 0};
+#pragma unroll 4
+      for (int i = 0; i < C::TILEB / 1024; ++i) all = __builtin_elementwise_max(all, top(piece(i)));
+      if (__builtin_amdgcn_ballot_w64(all[0] >= E || all[1] >= E)) {  // the same in every wave
+        for (int i = 0; i < C::TILEB / 1024; ++i) {
+          const u16x2 m = top(piece(i));
+          const uint64_t lanes = __builtin_amdgcn_ballot_w64(m[0] >= E || m[1] >= E);
+          for (int r = 0; r < C::RPI; ++r)
+            if (lanes >> (r * C::CPR) & (C::CPR == 64 ? ~0ull : (1ull << C::CPR) - 1)) bad |= 1ull << (i * C::RPI + r);
+        }
+        __syncthreads();  // every wave has looked
+        for (int i = wave; i < C::TILEB / 1024; i += NW)
+          if (bad >> (i * C::RPI + lane / C::CPR) & 1)
+            *(FMLM_LDS u32x4*)(uintptr_t)(tile + i * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+        wait_reads();
+        __syncthreads();
+      }
+    }
     if (!wave_active) {  // every query row of this wave is padding: loads and barriers only
       vwait(t);
       __syncthreads();
       return;
     }
-    prepare(t, sc, mx);
-    run_slots(Slot0{}, SlotEnd{}, sc, sn, mx, kn, vt);
+    if constexpr (TR) tree_mask(t, sc, mx);
+    prepare(tree, t, sc, mx);
+    run_slots(tree, Slot0{}, SlotEnd{}, sc, sn, mx, kn, vt);
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) sbase[qb] = m_i[qb];
+    for (int qb = 0; qb < QB; ++qb) sbase[qb] = TR && m_i[qb] == -INFINITY ? 0.f : m_i[qb];
+    if constexpr (TR) {
+      const KvSeg& sg = w.seg[1];
+      const int j0 = (t - nt0) * BK;
+      for (; bad; bad &= bad - 1) {  // the values taken out, by the rows that see them
+        const int j = __builtin_ctzll(bad);
+        if (j0 + j >= sg.n) break;  // (rows behind the last key repeat it)
+        const T* v = (const T*)sg.v + sg.vbase + (int64_t)(j0 + j) * sg.vsn + 4 * g;
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          uint32_t pw = 0;  // the pair that holds key j: block j / 16, element j % 4 of lane group j / 4 % 4
+#pragma unroll
+          for (int ks = 0; ks < C::NKS; ++ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e == (j >> 4 & 1) * 2 + (j >> 1 & 1) && ks == j >> 5) pw = pf[ks][qb][e];
+          pw = (uint32_t)__shfl((int)pw, l16 + 16 * (j >> 2 & 3));
+          const uint16_t pb = (uint16_t)(j & 1 ? pw >> 16 : pw);
+          const float x = (float)__builtin_bit_cast(T, pb);
+          if (tree_word(qb, t - nt0) >> j & 1)
+#pragma unroll
+            for (int db = 0; db < C::NDB; ++db)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o[db][qb][r] = fmaf(x, (float)v[db * 16 + r], o[db][qb][r]);
+        }
+      }
+    }
     vwait(t);
     __syncthreads();
   };
@@ -1490,13 +1588,13 @@ __global__ __launch_bounds__(NW * 64, NW >= 8 ? 1 : 2) void attn_mfma3_kernel(
     };
     auto phase_a = [&](int i, uint32_t kn) {
       if (wave_active) {
-        prepare(tb + i, sa, mx);
-        run_slots(Slot0{}, SlotB{}, sa, sb, mx, kn, 0u);
+        prepare(Plain{}, tb + i, sa, mx);
+        run_slots(Plain{}, Slot0{}, SlotB{}, sa, sb, mx, kn, 0u);
       }
     };
     auto phase_b = [&](uint32_t vt) {
       if (wave_active) {
-        run_slots(SlotB{}, SlotEnd{}, sa, sb, mx, 0u, vt);
+        run_slots(Plain{}, SlotB{}, SlotEnd{}, sa, sb, mx, 0u, vt);
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) sbase[qb] = m_i[qb];
       }
@@ -1548,21 +1646,24 @@ __global__ __launch_bounds__(NW * 64, NW >= 8 ? 1 : 2) void attn_mfma3_kernel(
     // step i of the unit uses K buffer i % 2 and V buffer i % 3; six steps per iteration
     // make every buffer offset a constant of its step (an LDS read address is then the
     // lane's offset register plus an immediate), the remainder takes them at run time
-    auto step_i = [&](int t, int i) {
+    auto step_i = [&](auto tree, int t, int i) {
       const int cur = (i & 1) * C::TILEB, nxt = C::TILEB - cur;
       const int v3 = i % 3;
       const int vc = v3 * C::TILEB, vd = (v3 == 0 ? 2 : v3 - 1) * C::TILEB;
-      step(t, sa, sb, mx, nxt, vc, kl + cur, vl + vd);
+      step(tree, t, sa, sb, mx, nxt, vc, kl + cur, vl + vd);
 #pragma unroll
       for (int kb = 0; kb < C::NKB; ++kb)
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) sa[kb][qb] = sb[kb][qb];
     };
     int t = tb;
-    for (; t + 6 <= te; t += 6)
+    const int tm = TREE ? min(te, nt0) : te;  // masked tiles from here on
+    for (; t + 6 <= tm; t += 6)
 #pragma unroll
-      for (int i = 0; i < 6; ++i) step_i(t + i, i);
-    for (; t < te; ++t) step_i(t, t - tb);
+      for (int i = 0; i < 6; ++i) step_i(Plain{}, t + i, i);
+    for (; t < tm; ++t) step_i(Plain{}, t, t - tb);
+    if constexpr (TREE)
+      for (; t < te; ++t) step_i(Tree{}, t, t - tb);
   }
 
   // ---- split part: this part's record (O / l, then m and l per row, all fp32) for
@@ -1641,7 +1742,8 @@ struct MlaRowsCfg {
 // 4-7 keys 32-63, for calls of few rows (see mla_rows_launch): with 128 rows per tile a
 // sequence of 64 (head, position) rows leaves one working wave per SIMD, bound by the
 // latency of its own LDS reads.  The halves' sums are added through LDS at the end.
-template <typename T, bool PAGED, bool LSE, bool SPLIT, int KH>
+// F32OUT: the context's part of a tree call, rows of o in fp32 (kFlagF32Out).
+template <typename T, bool PAGED, bool LSE, bool SPLIT, int KH, bool F32OUT = false>
 __global__ __launch_bounds__(MlaRowsCfg::NT, 1) void attn_mla_rows_kernel(
     const fmlm_attn_params p, const int4* __restrict__ units, const int32_t* __restrict__ hdr, const SplitArgs spa) {
   typedef MlaRowsCfg C;
@@ -1661,7 +1763,7 @@ __global__ __launch_bounds__(MlaRowsCfg::NT, 1) void attn_mla_rows_kernel(
   // other kernels
   const int u = !hpack ? (int)blockIdx.x : SPLIT ? workgroup_unit(hdr) : queue_first(hdr, blockIdx.x);
   WorkItem w;
-  if (u < 0 || !resolve_work(p, units, u, BQ, w, SPLIT ? spa : SplitArgs{nullptr, 0, 1}, hpack)) return;
+  if (u < 0 || !resolve_work(p, units, u, BQ, w, SPLIT ? spa : SplitArgs{nullptr, 0, 1, nullptr, 0}, hpack)) return;
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -2012,6 +2114,10 @@ __global__ __launch_bounds__(MlaRowsCfg::NT, 1) void attn_mla_rows_kernel(
     char* dst = (char*)p.o + o_off * 2;
 #pragma unroll
     for (int db = 0; db < C::NDB; ++db) {
+      if constexpr (F32OUT) {
+        *(f32x4*)((float*)p.o + o_off + db * 16 + g * 4) = o[db] * inv;
+        continue;
+      }
       T v4[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) v4[r] = (T)(o[db][r] * inv);
@@ -2566,14 +2672,14 @@ static Launch f32_launch() {
   return L;
 }
 
-template <typename T, int D, int QB, int NW, int BK, int PPB = 0>
+template <typename T, int D, int QB, int NW, int BK, int PPB = 0, bool TREE = false>
 static Launch mfma3_launch(bool paged) {
   typedef Mfma3Cfg<T, D, QB, NW, BK, PPB> C;
   static_assert(BK == kSplitBK, "split planning assumes the kernel's key tile");
   static_assert(BK == FMLM_PAGE_ROWS, "a paged context tile is one page");
-  const void* fn = (const void*)&attn_mfma3_kernel<T, D, QB, NW, BK, false, PPB>;
+  const void* fn = (const void*)&attn_mfma3_kernel<T, D, QB, NW, BK, false, PPB, TREE>;
   if constexpr (PPB == 0) {
-    if (paged) fn = (const void*)&attn_mfma3_kernel<T, D, QB, NW, BK, true, PPB>;
+    if (paged) fn = (const void*)&attn_mfma3_kernel<T, D, QB, NW, BK, true, PPB, TREE>;
   } else if (paged) {  // the ping-pong configurations read contiguous contexts only
     fn = nullptr;
   }
@@ -2587,7 +2693,10 @@ static Launch mfma3_launch(bool paged) {
 // contiguous kernel (at 256 VGPRs) does not have; the LSE one only for calls that store
 // the row statistics
 template <typename T, bool SPLIT, int KH>
-static const void* mla_rows_fn(bool paged, bool lse) {
+static const void* mla_rows_fn(bool paged, bool lse, bool f32_out) {
+  if (f32_out)
+    return paged ? (const void*)&attn_mla_rows_kernel<T, true, true, SPLIT, KH, true>
+                 : (const void*)&attn_mla_rows_kernel<T, false, true, SPLIT, KH, true>;
   return paged ? (lse ? (const void*)&attn_mla_rows_kernel<T, true, true, SPLIT, KH>
                       : (const void*)&attn_mla_rows_kernel<T, true, false, SPLIT, KH>)
                : (lse ? (const void*)&attn_mla_rows_kernel<T, false, true, SPLIT, KH>
@@ -2596,24 +2705,38 @@ static const void* mla_rows_fn(bool paged, bool lse) {
 template <typename T>
 static Launch mla_rows_launch(const fmlm_attn_params& p) {
   static_assert(MlaRowsCfg::BK == FMLM_PAGE_ROWS, "a paged context tile is one page");
-  const bool paged = p.ctx_block_table != nullptr, lse = p.lse != nullptr;
+  const bool paged = p.ctx_block_table != nullptr, lse = p.lse != nullptr, f32 = p.flags & kFlagF32Out;
   // Key halves for calls of up to 4096 (head, position) rows, 64 tiles of 64: 16 sequences of
   // 1-4 tokens, 64 heads, 1400-7800 latent rows 50 us (128-row tiles 59); 4 sequences of 8,
   // 32 heads 39 (47).  At 8192 rows (16 sequences of 8 tokens, 64 heads) they are slower, 115
   // us against 103: every latent tile is then read by twice the workgroups.
   if (p.cu_seqlens_q && (int64_t)p.H * p.total_q <= 4096) {
-    const void* fn = mla_rows_fn<T, true, 2>(paged, lse);
+    const void* fn = mla_rows_fn<T, true, 2>(paged, lse, f32);
     return Launch{MlaRowsCfg::BQ / 2, MlaRowsCfg::NT, MlaRowsCfg::LDS_BYTES + 2048, fn, true, true, true, fn, 2.f};
   }
-  return Launch{MlaRowsCfg::BQ, MlaRowsCfg::NT, MlaRowsCfg::LDS_BYTES, mla_rows_fn<T, false, 1>(paged, lse), true,
-                true, true, mla_rows_fn<T, true, 1>(paged, lse), 3.4f};
+  return Launch{MlaRowsCfg::BQ, MlaRowsCfg::NT, MlaRowsCfg::LDS_BYTES, mla_rows_fn<T, false, 1>(paged, lse, f32), true,
+                true, true, mla_rows_fn<T, true, 1>(paged, lse, f32), 3.4f};
 }
 
 // MFMA kernels by head dim.  The pipelined kernel and the 512-wide latent kernel need
 // linear main-key addressing; causal_query_seq_attn over padded K/V (a per-row sequence
 // lookup) takes the register-staged kernel.  The latent kernel also needs K = V (MLA).
 template <typename T>
+static bool pick_tree(const fmlm_attn_params& p, Launch& L) {
+  const bool paged = p.ctx_block_table != nullptr;
+  if (p.tile_config > 1) return false;
+  switch (p.D) {
+    case 16: L = mfma3_launch<T, 16, 1, 4, 64, 0, true>(paged); return true;
+    case 32: L = mfma3_launch<T, 32, 1, 4, 64, 0, true>(paged); return true;
+    case 64: L = mfma3_launch<T, 64, 1, 4, 64, 0, true>(paged); return true;
+    case 128: L = mfma3_launch<T, 128, 1, 4, 64, 0, true>(paged); return true;
+    case 256: L = mfma3_launch<T, 256, 1, 4, 64, 0, true>(paged); return true;
+    default: return false;
+  }
+}
+template <typename T>
 static bool pick_mfma(const fmlm_attn_params& p, Launch& L) {
+  if (p.flags & FMLM_FLAG_TREE) return pick_tree<T>(p, L);
   const bool lookup = (p.flags & FMLM_FLAG_CAUSAL_SEQ) && p.cu_seqlens_q &&
                       p.kv_layout != FMLM_LAYOUT_PACKED;
   if (lookup) {
@@ -2717,6 +2840,25 @@ static bool pick_f32(const fmlm_attn_params& p, Launch& L) {
   }
 }
 
+// Tree calls: the MFMA kernels of 16-bit types up to D = 256 mask the main keys themselves; the
+// others (the 512-wide latent, fp32) run a context-only call beside a kernel of the tree's part
+// (fmlm_tree.hip).  A call's parameters as its launches use them:
+static bool tree_fused(const fmlm_attn_params& p) { return p.dtype != FMLM_DTYPE_F32 && p.D <= 256; }
+static fmlm_attn_params effective(const fmlm_attn_params& p) {
+  fmlm_attn_params e = p;
+  e.flags &= ~(kFlagCtxOnly | kFlagF32Out);
+  if ((p.flags & FMLM_FLAG_TREE) && !tree_fused(p)) {
+    e.flags = (e.flags & ~FMLM_FLAG_TREE) | kFlagCtxOnly | (p.dtype == FMLM_DTYPE_F32 ? 0 : kFlagF32Out);
+    e.o_layout = FMLM_LAYOUT_PACKED;
+    e.o_sb = 0;
+    e.o_sh = (int64_t)p.total_q * p.D;
+    e.o_sn = p.D;
+    // (the output and the row statistics are the tree workspace's)
+    e.lse = (float*)(uintptr_t)16;
+  }
+  return e;
+}
+
 static int pick_launch(const fmlm_attn_params& p, Launch& L) {
   bool ok = false;
   if (p.tile_config < 0) return FMLM_E_ARG;
@@ -2727,6 +2869,7 @@ static int pick_launch(const fmlm_attn_params& p, Launch& L) {
     default: return FMLM_E_DTYPE;
   }
   if (!ok) return p.tile_config > 1 ? FMLM_E_ARG : FMLM_E_HEAD_DIM;
+  if ((p.flags & kFlagF32Out) && !L.hpack) return FMLM_E_HEAD_DIM;  // the latent kernel's alone
   // a paged context needs a kernel whose key tile is one page (not fp32, not per-row
   // lookups), and a configuration with a paged instantiation
   if (p.ctx_block_table && !(p.flags & FMLM_FLAG_PREFILL) && !L.paged) return FMLM_E_ARG;
@@ -2880,7 +3023,8 @@ static int check_params(const fmlm_attn_params& p) {
     if (sn < 0 || sn >= kMaxRowStride) return FMLM_E_ARG;
   if (!p.q || !p.o || !p.k || (!(p.flags & FMLM_FLAG_MLA) && !p.v)) return FMLM_E_ARG;
   if ((p.flags & FMLM_FLAG_CAUSAL_SEQ) && !p.cu_seqlens_q) return FMLM_E_ARG;
-  if ((p.flags & FMLM_FLAG_CTX_ONLY) && (p.flags & (FMLM_FLAG_CAUSAL_SEQ | FMLM_FLAG_PREFILL))) return FMLM_E_ARG;
+  if ((p.flags & FMLM_FLAG_TREE) && (!p.cu_seqlens_q || (p.flags & (FMLM_FLAG_CAUSAL_SEQ | FMLM_FLAG_PREFILL))))
+    return FMLM_E_ARG;
   if (!(p.flags & FMLM_FLAG_PREFILL)) {
     const bool has_ctx = p.cu_seqlens_kv || p.ctx_len > 0;
     if (has_ctx && !p.cu_seqlens_kv && p.ctx_len > 0 && !p.k_ctx) return FMLM_E_ARG;
@@ -2911,7 +3055,8 @@ static int launch_schedule(const fmlm_attn_params& p, const Launch& L, const Spl
 // the schedule was (or is) built with; records: where split parts go, NULL for the
 // schedule's own record area.
 static int launch_attention(const fmlm_attn_params& p, const Launch& L, const SplitCfg& sc, char* sched,
-                            bool build, char* records, hipStream_t s) {
+                            bool build, char* records, hipStream_t s, const uint64_t* mask = nullptr,
+                            int words = 0) {
   const void* const fn = sc.rec_cap > 0 && L.split_fn ? L.split_fn : L.fn;
   int rc = allow_lds(fn, L.lds);
   if (rc) return rc;
@@ -2929,7 +3074,7 @@ static int launch_attention(const fmlm_attn_params& p, const Launch& L, const Sp
   if (gx <= 0) return 0;
   if (gx > 0x7fffffff) return FMLM_E_ARG;
   fmlm_attn_params pc = p;
-  SplitArgs spa{records, (int32_t)sc.rec_bytes, sc.dense_parts};
+  SplitArgs spa{records, (int32_t)sc.rec_bytes, sc.dense_parts, mask, words};
   void* args[] = {(void*)&pc, (void*)&units, (void*)&header, (void*)&spa};
   hipError_t e = hipLaunchKernel(fn, dim3((unsigned)gx), dim3(L.threads), args, (size_t)L.lds, s);
   if (e != hipSuccess) return (int)e;
@@ -2937,7 +3082,9 @@ static int launch_attention(const fmlm_attn_params& p, const Launch& L, const Sp
     const int64_t groups = p.cu_seqlens_q ? sc.rec_cap / 2 : sc.rec_cap / sc.dense_parts;
     const int hp = L.hpack && p.cu_seqlens_q;
     const dim3 mg((unsigned)std::min<int64_t>(groups * merge_chunks(p, L.bq, hp), 4096));
-    if (p.dtype == FMLM_DTYPE_BF16)
+    if (p.flags & kFlagF32Out)
+      hipLaunchKernelGGL(merge_kernel<float>, mg, dim3(kMergeThreads), 0, s, p, L.bq, (const int32_t*)header, spa, hp);
+    else if (p.dtype == FMLM_DTYPE_BF16)
       hipLaunchKernelGGL(merge_kernel<bf16>, mg, dim3(kMergeThreads), 0, s, p, L.bq, (const int32_t*)header, spa, hp);
     else if (p.dtype == FMLM_DTYPE_F16)
       hipLaunchKernelGGL(merge_kernel<f16>, mg, dim3(kMergeThreads), 0, s, p, L.bq, (const int32_t*)header, spa, hp);
@@ -2998,42 +3145,42 @@ using namespace fmlm;
 extern "C" int fmlm_attn_schedule(const fmlm_attn_params* pp, void* schedule,
                                   int64_t schedule_bytes, void* stream) {
   if (!pp || !schedule || !pp->cu_seqlens_q || pp->B < 1) return FMLM_E_ARG;
+  const fmlm_attn_params p = effective(*pp);
   Launch L;
-  const int rc = pick_launch(*pp, L);
+  const int rc = pick_launch(p, L);
   if (rc) return rc;
-  const SplitCfg sc = split_cfg(*pp, L);
-  const bool own = pp->flags & FMLM_FLAG_OWN_RECORDS;
-  if (schedule_bytes < workspace_for(*pp, L, sc) - (own ? records_for(sc) : 0)) return FMLM_E_WORKSPACE;
-  return launch_schedule(*pp, L, sc, (char*)schedule, own, (hipStream_t)stream);
+  const SplitCfg sc = split_cfg(p, L);
+  const bool own = p.flags & FMLM_FLAG_OWN_RECORDS;
+  if (schedule_bytes < workspace_for(p, L, sc) - (own ? records_for(sc) : 0)) return FMLM_E_WORKSPACE;
+  return launch_schedule(p, L, sc, (char*)schedule, own, (hipStream_t)stream);
 }
 
 extern "C" int fmlm_attn_params_size(void) { return (int)sizeof(fmlm_attn_params); }
 
-extern "C" int64_t fmlm_attn_workspace_bytes(const fmlm_attn_params* p) {
-  if (!p) return FMLM_E_ARG;
+extern "C" int64_t fmlm_attn_workspace_bytes(const fmlm_attn_params* pp) {
+  if (!pp) return FMLM_E_ARG;
+  const fmlm_attn_params p = effective(*pp);
   Launch L;
-  const int rc = pick_launch(*p, L);
+  const int rc = pick_launch(p, L);
   if (rc) return rc;
-  return workspace_for(*p, L, split_cfg(*p, L));
+  return workspace_for(p, L, split_cfg(p, L));
 }
 
-extern "C" int64_t fmlm_attn_records_bytes(const fmlm_attn_params* p) {
-  if (!p) return FMLM_E_ARG;
+extern "C" int64_t fmlm_attn_records_bytes(const fmlm_attn_params* pp) {
+  if (!pp) return FMLM_E_ARG;
+  const fmlm_attn_params p = effective(*pp);
   Launch L;
-  const int rc = pick_launch(*p, L);
+  const int rc = pick_launch(p, L);
   if (rc) return rc;
   // a packed call whose longest key range is one part at most cannot split
-  if (p->cu_seqlens_q && max_key_tiles(*p) <= split_min_tiles(L)) return 0;
-  return records_for(split_cfg(*p, L));
+  if (p.cu_seqlens_q && max_key_tiles(p) <= split_min_tiles(L)) return 0;
+  return records_for(split_cfg(p, L));
 }
 
-extern "C" int fmlm_attn_fwd(const fmlm_attn_params* pp, void* stream) {
-  if (!pp) return FMLM_E_ARG;
-  const fmlm_attn_params& p = *pp;
-  int rc = check_params(p);
-  if (rc) return rc;
+// the forward of checked parameters (effective), with the masks of a tree call
+static int attn_fwd(const fmlm_attn_params& p, const uint64_t* mask, int words, void* stream) {
   Launch L;
-  rc = pick_launch(p, L);
+  const int rc = pick_launch(p, L);
   if (rc) return rc;
   if (p.B == 0 || p.H == 0) return 0;
   SplitCfg sc = split_cfg(p, L);
@@ -3047,17 +3194,57 @@ extern "C" int fmlm_attn_fwd(const fmlm_attn_params* pp, void* stream) {
   if (p.schedule) {
     const bool own = p.flags & FMLM_FLAG_OWN_RECORDS;
     if (own && have < records_for(sc)) return FMLM_E_WORKSPACE;
-    return launch_attention(p, L, sc, (char*)p.schedule, false, own ? ws : nullptr, (hipStream_t)stream);
+    return launch_attention(p, L, sc, (char*)p.schedule, false, own ? ws : nullptr, (hipStream_t)stream, mask, words);
   }
   if (need > 0 && have < need) return FMLM_E_WORKSPACE;
-  return launch_attention(p, L, sc, ws, true, nullptr, (hipStream_t)stream);
+  return launch_attention(p, L, sc, ws, true, nullptr, (hipStream_t)stream, mask, words);
+}
+
+extern "C" int fmlm_attn_fwd(const fmlm_attn_params* pp, void* stream) {
+  if (!pp) return FMLM_E_ARG;
+  if (pp->flags & FMLM_FLAG_TREE) return FMLM_E_ARG;  // fmlm_attn_tree_fwd
+  const int rc = check_params(*pp);
+  if (rc) return rc;
+  return attn_fwd(effective(*pp), nullptr, 0, stream);
+}
+
+extern "C" int64_t fmlm_attn_tree_workspace_bytes(const fmlm_attn_params* pp) {
+  if (!pp || pp->H < 0 || pp->D < 1 || pp->total_q < 0) return FMLM_E_ARG;
+  return tree_fused(*pp) ? 0 : 4 * (int64_t)pp->H * pp->total_q * (pp->D + 1);
+}
+
+extern "C" int fmlm_attn_tree_fwd(const fmlm_attn_params* pp, const uint64_t* mask, int32_t words, void* tree_workspace,
+                                  int64_t tree_workspace_bytes, void* stream) {
+  if (!pp || !(pp->flags & FMLM_FLAG_TREE)) return FMLM_E_ARG;
+  const fmlm_attn_params& p = *pp;
+  int rc = check_params(p);
+  if (rc) return rc;
+  if (p.N > FMLM_MAX_TREE || p.H > 65535 || p.B > 65535) return FMLM_E_ARG;
+  // packed inputs without a padded length: a sequence may be as long as all of them
+  const int longest = p.N > 0 ? std::min(p.N, p.total_q) : p.total_q;
+  if (longest > FMLM_MAX_TREE || (int64_t)words * 64 < longest) return FMLM_E_ARG;
+  if (p.B > 0 && p.H > 0 && longest > 0 && !mask) return FMLM_E_ARG;
+  const int64_t need = fmlm_attn_tree_workspace_bytes(pp);
+  if (need > 0 && (!tree_workspace || tree_workspace_bytes < need)) return FMLM_E_WORKSPACE;
+  fmlm_attn_params e = effective(p);
+  if (tree_fused(p)) {
+    e.lse = nullptr;
+    return attn_fwd(e, mask, words, stream);
+  }
+  if (((uintptr_t)tree_workspace & 15) != 0 || !tree_part_aligned(p)) return FMLM_E_ALIGN;
+  e.o = tree_workspace;
+  e.lse = (float*)tree_workspace + (int64_t)p.H * p.total_q * p.D;
+  rc = attn_fwd(e, nullptr, 0, stream);
+  if (rc || p.B == 0 || p.H == 0 || longest <= 0) return rc;
+  return launch_tree_part(e, p, mask, words, longest, stream);
 }
 
 extern "C" int fmlm_attn_fwd_noalloc(const fmlm_attn_params* pp, void* stream) {
   if (!pp) return FMLM_E_ARG;
-  const fmlm_attn_params& p = *pp;
-  int rc = check_params(p);
+  if (pp->flags & FMLM_FLAG_TREE) return FMLM_E_ARG;
+  int rc = check_params(*pp);
   if (rc) return rc;
+  const fmlm_attn_params p = effective(*pp);
   Launch L;
   rc = pick_launch(p, L);
   if (rc) return rc;

@@ -2449,7 +2449,7 @@ static bool row_ok(const void* ptr, int64_t sb, int64_t sh, int64_t sn) {
 
 static int check_bwd(const fmlm_attn_params& p, const fmlm_attn_grads& g, BwdFns& f) {
   if (p.B < 0 || p.H < 0 || p.N < 0 || p.total_q < 0 || p.ctx_len < 0) return FMLM_E_ARG;
-  if (p.flags & FMLM_FLAG_CTX_ONLY) return FMLM_E_ARG;  // forward only
+  if (p.flags & FMLM_FLAG_TREE) return FMLM_E_ARG;  // forward only
   const bool mla = p.flags & FMLM_FLAG_MLA;
   if (!p.q || !p.o || !p.k || (!mla && !p.v) || !g.dout || !g.dq || !g.dk || (!mla && !g.dv)) return FMLM_E_ARG;
   // MFMA kernels for bf16 / f16 (the 512-wide one only for the MLA latent), SIMT otherwise

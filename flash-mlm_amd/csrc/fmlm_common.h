@@ -62,6 +62,10 @@ FMLM_DEV int find_seq(const int32_t* cu, int B, int j) {
   return lo;
 }
 
+// ---- flags of a call's launches besides the caller's (fmlm_attn.hip, effective())
+constexpr int kFlagCtxOnly = 1 << 16;  // no main keys
+constexpr int kFlagF32Out = 1 << 17;   // the rows of o are fp32
+
 // ---- per-sequence ranges of an attention call
 struct SeqInfo {
   int q0, len;       // packed start and clamped length of sequence b
@@ -107,9 +111,15 @@ FMLM_DEV SeqInfo seq_info(const fmlm_attn_params& p, int b) {
     ctx_range(p, ctx_batch_of(p, b), c0, c1);
     s.ctx = max(c1 - c0, 0);
   }
-  s.mainlen = (p.flags & FMLM_FLAG_CTX_ONLY) ? 0 : ((p.flags & FMLM_FLAG_CAUSAL_SEQ) && cu) ? s.q0 + L : L;
+  s.mainlen = (p.flags & kFlagCtxOnly) ? 0 : ((p.flags & FMLM_FLAG_CAUSAL_SEQ) && cu) ? s.q0 + L : L;
   return s;
 }
+
+// The tree's part of a tree call whose context part (`ctx`: its o and lse) has run, joined into
+// call.o (fmlm_tree.hip)
+bool tree_part_aligned(const fmlm_attn_params& call);
+int launch_tree_part(const fmlm_attn_params& ctx, const fmlm_attn_params& call, const uint64_t* mask, int words,
+                     int longest, void* stream);
 
 FMLM_DEV float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -1,15 +1,13 @@
-// Attention of drafted trees over a cached context.
+// Drafted trees: ancestor masks, and the tree's part of the attention calls whose main kernel
+// does not mask its keys itself.
 //
 // Query i of a sequence attends to the sequence's context and to those tokens j of its own
-// draft that are i or an ancestor of i:
-//   o_i = (sum_ctx e^{z} v + sum_{j in anc(i)} e^{z_ij} v_j) / (both sums of e^z),
-// z = scale q.k.  The context part is the forward kernels' ordinary work (they read every
-// key once, at the rate of a copy); it leaves o_c = its own softmax's output and l_c =
-// log2(sum 2^z) per row.  The tree kernel here computes m = max z and l = sum 2^(z - m) over
-// the ancestors and writes
+// draft that are i or an ancestor of i.  The MFMA kernels of 16-bit types up to D = 256 do all of it
+// (fmlm_attn.hip).  For the 512-wide latent and fp32 the context's part runs by itself and
+// leaves, per row, its own softmax's output o_c (fp32) and l_c = log2(sum 2^z), z =
+// scale log2(e) q.k.  A kernel here computes m = max z and l = sum 2^(z - m) over the ancestors
+// and writes
 //   (2^(l_c - M) o_c + 2^(m - M) sum 2^(z - m) v) / (2^(l_c - M) + 2^(m - M) l),  M = max(l_c, m).
-// o_c is read as the attention kernel rounded it, to the input type: one rounding (half a
-// step of o_c) besides the last one, for half of the traffic of a 32-bit copy.
 //
 // A draft has at most 256 tokens, so its keys are few beside the context's: the kernel is
 // bound by latency, not by bandwidth or products.  One wave takes 16 rows of one head, so
@@ -104,13 +102,14 @@ FMLM_DEV int64_t tree_row(int layout, int b, int h, int q0, int pos, int64_t sb,
 struct TreeJoin {
   float wc, wt;
 };
-FMLM_DEV TreeJoin tree_join(const fmlm_attn_params& p, const TreeSeq& s, int h, int pos, float m, float l) {
+FMLM_DEV TreeJoin tree_join(const fmlm_attn_params& p, const float* lse, const TreeSeq& s, int h, int pos, float m,
+                            float l) {
   TreeJoin j{0.f, 0.f};
   if (!s.has_ctx) {
     if (l != 0.f) j.wt = 1.f / l;  // (NaN too; no key at all: 0)
     return j;
   }
-  const float lc = p.lse[(int64_t)h * p.total_q + s.q0 + pos];
+  const float lc = lse[(int64_t)h * p.total_q + s.q0 + pos];
   const float top = vmax(lc, m);
   j.wc = fast_exp2(lc - top);  // an infinite top: NaN, as inf - inf is
   j.wt = m == -INFINITY ? 0.f : fast_exp2(m - top);
@@ -121,15 +120,16 @@ FMLM_DEV TreeJoin tree_join(const fmlm_attn_params& p, const TreeSeq& s, int h, 
 }
 
 // ---------------------------------------------------------------------------
-// bf16 / fp16.  As in the forward kernels S^T = K Q^T and O^T = V^T P^T, so that a lane
+// bf16 / fp16, the 512-wide latent.  As in the forward kernels S^T = K Q^T and O^T = V^T P^T, so that a lane
 // (q + 16 g) holds keys 4g .. 4g+3 of query q and then columns 16 db + 4g .. of its output.
 // K fragments come straight from memory (a lane's 16 bytes of a key row are its operand);
 // V passes through LDS, whose transposing read makes its operand.  P is rounded to the input
 // type for the product, and its row sum is taken of the rounded values.
 // ---------------------------------------------------------------------------
 template <typename T, int D>
-__global__ __launch_bounds__(64) void attn_tree_kernel(const fmlm_attn_params p, const uint64_t* __restrict__ mask,
-                                                       int words) {
+__global__ __launch_bounds__(64) void attn_tree_kernel(const fmlm_attn_params p, const float* __restrict__ octx,
+                                                       const float* __restrict__ lse,
+                                                       const uint64_t* __restrict__ mask, int words) {
   typedef typename Mfma<T>::v8 v8;
   constexpr int KC = (D + 31) / 32, NDB = D / 16, BK = 32;
   constexpr int PITCH = D * 2 + 16;  // 16 bytes apart: a column's rows fall into different banks
@@ -257,18 +257,13 @@ __global__ __launch_bounds__(64) void attn_tree_kernel(const fmlm_attn_params p,
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
   if (!ok) return;
-  const TreeJoin j = tree_join(p, s, h, pos, m, l);
+  const TreeJoin j = tree_join(p, lse, s, h, pos, m, l);
   T* const dst = (T*)p.o + tree_row(p.o_layout, b, h, s.q0, pos, p.o_sb, p.o_sh, p.o_sn) + 4 * g;
+  const float* const oc = octx + ((int64_t)h * p.total_q + s.q0 + pos) * D + 4 * g;
 #pragma unroll
   for (int db = 0; db < NDB; ++db) {
     f32x4 x = o[db] * j.wt;
-    if (s.has_ctx) {
-      const u32x2 raw = *(const u32x2*)(dst + db * 16);
-      T oc[4];
-      __builtin_memcpy(oc, &raw, 8);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = fmaf(j.wc, (float)oc[r], x[r]);
-    }
+    if (s.has_ctx) x += j.wc * *(const f32x4*)(oc + db * 16);
     T y[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
@@ -284,8 +279,9 @@ __global__ __launch_bounds__(64) void attn_tree_kernel(const fmlm_attn_params p,
 // Keys that the row does not see are not read.
 // ---------------------------------------------------------------------------
 template <int D>
-__global__ __launch_bounds__(64) void attn_tree_f32_kernel(const fmlm_attn_params p, const uint64_t* __restrict__ mask,
-                                                           int words) {
+__global__ __launch_bounds__(64) void attn_tree_f32_kernel(const fmlm_attn_params p, const float* __restrict__ octx,
+                                                           const float* __restrict__ lse,
+                                                           const uint64_t* __restrict__ mask, int words) {
   constexpr int NC = (D + 63) / 64;
   __shared__ __align__(16) float qs[D];
   const int b = blockIdx.z, h = blockIdx.y, pos = blockIdx.x, lane = threadIdx.x;
@@ -335,33 +331,43 @@ __global__ __launch_bounds__(64) void attn_tree_f32_kernel(const fmlm_attn_param
   }
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off);
-  const TreeJoin j = tree_join(p, s, h, pos, m, l);
+  const TreeJoin j = tree_join(p, lse, s, h, pos, m, l);
   float* const dst = (float*)p.o + tree_row(p.o_layout, b, h, s.q0, pos, p.o_sb, p.o_sh, p.o_sn);
+  const float* const oc = octx + ((int64_t)h * p.total_q + s.q0 + pos) * D;
 #pragma unroll
   for (int i = 0; i < NC; ++i)
     if (D >= 64 || lane < D) {
       float x = o[i] * j.wt;
-      if (s.has_ctx) x = fmaf(j.wc, dst[lane + 64 * i], x);
+      if (s.has_ctx) x = fmaf(j.wc, oc[lane + 64 * i], x);
       dst[lane + 64 * i] = x;
     }
 }
 
-template <typename T>
-static int launch_tree(const fmlm_attn_params& p, const uint64_t* mask, int words, int longest, hipStream_t s) {
-  const dim3 grid((unsigned)((longest + 15) / 16), (unsigned)p.H, (unsigned)p.B);
-#define FMLM_TREE(DD) \
-  case DD: hipLaunchKernelGGL((attn_tree_kernel<T, DD>), grid, dim3(64), 0, s, p, mask, words); break;
-  switch (p.D) {
-    FMLM_TREE(16) FMLM_TREE(32) FMLM_TREE(64) FMLM_TREE(128) FMLM_TREE(256) FMLM_TREE(512)
-    default: return FMLM_E_HEAD_DIM;
-  }
-#undef FMLM_TREE
-  return launch_status();
+bool tree_part_aligned(const fmlm_attn_params& p) {
+  const int es = elem_size(p.dtype);
+  const bool mla = p.flags & FMLM_FLAG_MLA;
+  for (int64_t st : {p.q_sb, p.q_sh, p.q_sn, p.k_sb, p.k_sh, p.k_sn, p.o_sb, p.o_sh, p.o_sn})
+    if ((st * es) % 16) return false;
+  if (!mla && ((p.v_sb * es) % 16 || (p.v_sh * es) % 16 || (p.v_sn * es) % 16)) return false;
+  return (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.o | (mla ? 0 : (uintptr_t)p.v)) & 15) == 0;
 }
-static int launch_tree_f32(const fmlm_attn_params& p, const uint64_t* mask, int words, int longest, hipStream_t s) {
+
+int launch_tree_part(const fmlm_attn_params& ctx, const fmlm_attn_params& p, const uint64_t* mask, int words,
+                     int longest, void* stream) {
+  const hipStream_t s = (hipStream_t)stream;
+  const float* const octx = (const float*)ctx.o;
+  if (p.dtype != FMLM_DTYPE_F32) {
+    const dim3 grid((unsigned)((longest + 15) / 16), (unsigned)p.H, (unsigned)p.B);
+    if (p.D != 512) return FMLM_E_HEAD_DIM;
+    if (p.dtype == FMLM_DTYPE_BF16)
+      hipLaunchKernelGGL((attn_tree_kernel<bf16, 512>), grid, dim3(64), 0, s, p, octx, ctx.lse, mask, words);
+    else
+      hipLaunchKernelGGL((attn_tree_kernel<f16, 512>), grid, dim3(64), 0, s, p, octx, ctx.lse, mask, words);
+    return launch_status();
+  }
   const dim3 grid((unsigned)longest, (unsigned)p.H, (unsigned)p.B);
 #define FMLM_TREE(DD) \
-  case DD: hipLaunchKernelGGL((attn_tree_f32_kernel<DD>), grid, dim3(64), 0, s, p, mask, words); break;
+  case DD: hipLaunchKernelGGL((attn_tree_f32_kernel<DD>), grid, dim3(64), 0, s, p, octx, ctx.lse, mask, words); break;
   switch (p.D) {
     FMLM_TREE(16) FMLM_TREE(32) FMLM_TREE(64) FMLM_TREE(128) FMLM_TREE(256) FMLM_TREE(512)
     default: return FMLM_E_HEAD_DIM;
@@ -384,30 +390,4 @@ extern "C" int fmlm_tree_mask(const void* parents, int32_t parents_i64, const in
   hipLaunchKernelGGL(tree_mask_kernel, dim3(B), dim3(threads), 0, (hipStream_t)stream, parents, parents_i64, cu_seqlens,
                      N, T, words, ctx_lens, ctx_lens_i64, mask, positions, n_bad);
   return launch_status();
-}
-
-extern "C" int fmlm_attn_tree_fwd(const fmlm_attn_params* pp, const uint64_t* mask, int32_t words, void* stream) {
-  if (!pp) return FMLM_E_ARG;
-  const fmlm_attn_params& p = *pp;
-  if (!(p.flags & FMLM_FLAG_CTX_ONLY) || (p.flags & (FMLM_FLAG_PREFILL | FMLM_FLAG_CAUSAL_SEQ))) return FMLM_E_ARG;
-  if (!p.cu_seqlens_q || !p.lse || p.N < 0 || p.N > FMLM_MAX_TREE || p.H > 65535 || p.B > 65535) return FMLM_E_ARG;
-  // packed inputs without a padded length: their sequences may be as long as all of them
-  const int longest = p.N > 0 ? std::min(p.N, p.total_q) : std::min(p.total_q, FMLM_MAX_TREE);
-  if (p.B > 0 && p.H > 0 && longest > 0 && (!mask || (int64_t)words * 64 < longest)) return FMLM_E_ARG;
-  const int es = elem_size(p.dtype);
-  if (!es) return FMLM_E_DTYPE;
-  for (int64_t st : {p.q_sb, p.q_sh, p.q_sn, p.k_sb, p.k_sh, p.k_sn, p.o_sb, p.o_sh, p.o_sn})
-    if ((st * es) % 16) return FMLM_E_ALIGN;
-  if (!(p.flags & FMLM_FLAG_MLA) && ((p.v_sb * es) % 16 || (p.v_sh * es) % 16 || (p.v_sn * es) % 16)) return FMLM_E_ALIGN;
-  if (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.o) & 15) return FMLM_E_ALIGN;
-  if (!(p.flags & FMLM_FLAG_MLA) && ((uintptr_t)p.v & 15)) return FMLM_E_ALIGN;
-  const int rc = fmlm_attn_fwd(pp, stream);  // checks the rest of p
-  if (rc) return rc;
-  if (p.B == 0 || p.H == 0 || longest <= 0) return 0;
-  hipStream_t s = (hipStream_t)stream;
-  switch (p.dtype) {
-    case FMLM_DTYPE_BF16: return launch_tree<bf16>(p, mask, words, longest, s);
-    case FMLM_DTYPE_F16: return launch_tree<f16>(p, mask, words, longest, s);
-    default: return launch_tree_f32(p, mask, words, longest, s);
-  }
 }

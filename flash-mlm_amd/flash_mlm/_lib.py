@@ -27,7 +27,7 @@ FLAG_PREFILL = 2
 FLAG_CAUSAL_SEQ = 4
 FLAG_NOSPLIT = 8
 FLAG_OWN_RECORDS = 16
-FLAG_CTX_ONLY = 32
+FLAG_TREE = 32
 
 NR_NORM = 1
 NR_INTERLEAVED = 2
@@ -263,7 +263,8 @@ SIGNATURES = {
         ctypes.c_int,
         [_c_ptr, _c_i32, _c_ptr, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr, _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
     ),
-    "fmlm_attn_tree_fwd": (ctypes.c_int, [ctypes.POINTER(AttnParams), _c_ptr, _c_i32, _c_ptr]),
+    "fmlm_attn_tree_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(AttnParams)]),
+    "fmlm_attn_tree_fwd": (ctypes.c_int, [ctypes.POINTER(AttnParams), _c_ptr, _c_i32, _c_ptr, _c_i64, _c_ptr]),
 }
 
 _lock = threading.Lock()

@@ -113,9 +113,12 @@ class TreeLaunch(AttnLaunch):
     __slots__ = ("mask",)
 
     def __call__(self) -> None:
-        self.own_buffers(row_stats=True)
+        self.own_buffers(row_stats=False)
+        nbytes = self.lib.fmlm_attn_tree_workspace_bytes(self.params)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes > 0 else None
         with _device_scope(self.device):
-            rc = self.lib.fmlm_attn_tree_fwd(self.params, self.mask.data_ptr(), int(self.mask.shape[1]), self.stream)
+            rc = self.lib.fmlm_attn_tree_fwd(self.params, self.mask.data_ptr(), int(self.mask.shape[1]), _lib.ptr(ws),
+                                             nbytes, self.stream)
         _lib.check(rc, "fmlm_attn_tree_fwd")
 
     @classmethod
@@ -239,7 +242,7 @@ def flash_attn_mlm_tree(
         ctx_batch=cbs,
         ctx_rows=_ctx_rows(ctx),
         scale=scale,
-        flags=_lib.FLAG_CTX_ONLY | (_lib.FLAG_MLA if is_mla else 0),
+        flags=_lib.FLAG_TREE | (_lib.FLAG_MLA if is_mla else 0),
         inference_cache=inference_cache,
         schedule_cache=q_meta.kernel_schedules,
         ctx_index=ctx_index,

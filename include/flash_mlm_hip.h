@@ -54,9 +54,7 @@ enum {
   FMLM_FLAG_CAUSAL_SEQ = 4, /* sequence b attends to main tokens [0, cu_q[b+1]) */
   FMLM_FLAG_NOSPLIT = 8,    /* key ranges are not split (no records, no merge launch); a
                                schedule is then built with this flag too               */
-  FMLM_FLAG_CTX_ONLY = 32,  /* no main keys: the queries attend to their context alone (forward
-                               only; a row without context keys has output 0 in bf16 / f16,
-                               no defined output in f32, and lse +inf)                     */
+  FMLM_FLAG_TREE = 32,      /* the call (and its schedule) is for fmlm_attn_tree_fwd         */
   FMLM_FLAG_OWN_RECORDS = 16 /* the schedule has no room for split partial results: every
                                fmlm_attn_fwd on it has this flag too and brings them in
                                its workspace                                           */
@@ -497,12 +495,17 @@ FMLM_API int fmlm_tree_mask(const void* parents, int32_t parents_i64, const int3
                             int32_t T, int32_t words, const void* ctx_lens, int32_t ctx_lens_i64, uint64_t* mask,
                             int32_t* positions, int32_t* n_bad, void* stream);
 
-/* Attention of drafted trees: fmlm_attn_fwd's packed call p in which token i of a sequence
- * attends to [its context || the main tokens j of its sequence with mask bit j set].  p has
- * FMLM_FLAG_CTX_ONLY set (its schedule too) and brings p->lse; N is at most FMLM_MAX_TREE.
- * The context part runs as fmlm_attn_fwd(p); a second kernel then computes the tree's part
- * and joins the two by their sums.  A row that sees no key has output 0.  No backward. */
-FMLM_API int fmlm_attn_tree_fwd(const fmlm_attn_params* p, const uint64_t* mask, int32_t words, void* stream);
+/* Attention of drafted trees: fmlm_attn_fwd's packed call p (linear main keys, no
+ * FMLM_FLAG_PREFILL or CAUSAL_SEQ) with FMLM_FLAG_TREE, in which token i of a sequence attends
+ * to [its context || the main tokens j of its sequence with mask bit j set]; bits at or past
+ * the sequence's end are ignored.  A row that sees no key has output 0.  At most FMLM_MAX_TREE
+ * tokens in a sequence (N, or total_q where N is 0).  p->lse is not used; no backward.
+ * bf16 / f16 up to D = 256 mask the main keys in the attention kernel.  For D = 512 (MLA) and
+ * f32 a second kernel computes the tree's part, and the context's part goes through
+ * tree_workspace: fmlm_attn_tree_workspace_bytes(p) bytes (0 in the first case). */
+FMLM_API int64_t fmlm_attn_tree_workspace_bytes(const fmlm_attn_params* p);
+FMLM_API int fmlm_attn_tree_fwd(const fmlm_attn_params* p, const uint64_t* mask, int32_t words, void* tree_workspace,
+                                int64_t tree_workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -89,31 +89,47 @@ def test_abi_refuses():
     assert m(None, 0, None, 1, 65, 1, 1, None, 0, None, None, None, None) == -1  # too few words
     assert m(None, 0, None, 1, 4, 4, 1, None, 0, None, None, None, None) == -1  # no tensors
     assert m(None, 0, None, 0, 4, 0, 1, None, 0, None, None, None, None) == 0
-    a = lib.fmlm_attn_tree_fwd
-    assert a(None, None, 1, None) == -1
+    f = lib.fmlm_attn_tree_fwd
+
+    def a(p, mask, words, ws=None, n=0):
+        return f(p, mask, words, ws, n, None)
+
+    assert a(None, None, 1) == -1
     p = _lib.AttnParams()
     p.dtype, p.B, p.H, p.D, p.N, p.total_q = _lib.DTYPE_BF16, 1, 1, 64, 4, 4
-    p.q = p.k = p.v = p.o = p.cu_seqlens_q = p.lse = 256
-    assert a(p, 256, 1, None) == -1  # not a context-only call
-    p.flags = _lib.FLAG_CTX_ONLY
-    assert a(p, None, 1, None) == -1  # no mask
-    p.lse = None
-    assert a(p, 256, 1, None) == -1  # no row statistics
-    p.lse, p.N = 256, 300
-    assert a(p, 256, 8, None) == -1  # too long
-    p.N, p.v = 4, 264
-    assert a(p, 256, 1, None) == -4
-    p.v, p.q_sn = 256, 60
-    assert a(p, 256, 1, None) == -4
-    p.q_sn = 64
-    assert a(p, 256, 1, None) == -5  # fmlm_attn_fwd's checks follow: no workspace
+    p.q = p.k = p.v = p.o = p.cu_seqlens_q = 256
+    assert a(p, 256, 1) == -1  # not a tree call
+    p.flags = _lib.FLAG_TREE
+    assert a(p, None, 1) == -1  # no mask
+    p.N = p.total_q = 300
+    assert a(p, 256, 8) == -1  # too long
+    p.N, p.total_q = 0, 257
+    assert a(p, 256, 8) == -1  # too long, for all that is known
+    p.N, p.total_q = 4, 4
+    assert a(p, 256, 0) == -1  # no words
+    assert a(p, 256, 1) == -5  # the attention kernel's workspace
+    assert lib.fmlm_attn_tree_workspace_bytes(p) == 0
+    p.cu_seqlens_q = None
+    assert a(p, 256, 1) == -1  # dense
+    p.cu_seqlens_q = 256
     p.flags |= _lib.FLAG_PREFILL
-    assert a(p, 256, 1, None) == -1
+    assert a(p, 256, 1) == -1
+    p.flags = _lib.FLAG_TREE
     assert lib.fmlm_attn_fwd(p, None) == -1
+    assert lib.fmlm_attn_fwd_noalloc(p, None) == -1
     g = _lib.AttnGrads()
-    p.flags = _lib.FLAG_CTX_ONLY
     g.dout = g.dq = g.dk = g.dv = 256
     assert lib.fmlm_attn_bwd(p, g, None) == -1
+    p.dtype = _lib.DTYPE_F32  # the tree's part in a kernel of its own
+    assert lib.fmlm_attn_tree_workspace_bytes(p) == 4 * 4 * 65
+    assert a(p, 256, 1) == -5
+    p.v = 264
+    assert a(p, 256, 1, 256, 4 * 4 * 65) == -4
+    p.dtype, p.D = _lib.DTYPE_BF16, 512  # only the latent
+    assert lib.fmlm_attn_workspace_bytes(p) == -3
+    assert a(p, 256, 1, 256, 4 * 4 * 513) == -4
+    p.v = 256
+    assert a(p, 256, 1, 256, 4 * 4 * 513) == -3
 
 
 # ---------------------------------------------------------------------------
@@ -232,8 +248,6 @@ def _run(device, dtype, *, lens, N, H, D, ctx, kind, mla=False, scale=None, seed
 def test_attention(dtype, D, kind, device):
     if dtype == "fp32" and kind == "paged":
         pytest.skip("paged contexts are bf16 / fp16")
-    if D == 16 and kind == "paged":
-        pytest.skip("no paged kernel of head dim 16")
     _run(device, DT[dtype], lens=[40, 1, 0, 17], N=41, H=3, D=D, ctx=[70, 0, 5, 129], kind=kind, seed=D)
 
 
