@@ -9,10 +9,9 @@
 // and writes
 //   (2^(l_c - M) o_c + 2^(m - M) sum 2^(z - m) v) / (2^(l_c - M) + 2^(m - M) l),  M = max(l_c, m).
 //
-// A draft has at most 256 tokens, so its keys are few beside the context's: the kernel is
-// bound by latency, not by bandwidth or products.  One wave takes 16 rows of one head, so
-// that a few rows give many waves; steps of 32 keys in which no row of the wave has an
-// ancestor are skipped (an ancestor precedes its descendants, so the later ones).
+// A draft has at most 256 tokens, so its keys are few beside the context's: these kernels are
+// bound by latency, not by bandwidth or products.  Steps in which no row has an ancestor are
+// skipped (an ancestor precedes its descendants, so the later ones).
 #include "fmlm_common.h"
 
 #include <algorithm>
@@ -102,14 +101,12 @@ FMLM_DEV int64_t tree_row(int layout, int b, int h, int q0, int pos, int64_t sb,
 struct TreeJoin {
   float wc, wt;
 };
-FMLM_DEV TreeJoin tree_join(const fmlm_attn_params& p, const float* lse, const TreeSeq& s, int h, int pos, float m,
-                            float l) {
+FMLM_DEV TreeJoin tree_join(bool has_ctx, float lc, float m, float l) {
   TreeJoin j{0.f, 0.f};
-  if (!s.has_ctx) {
+  if (!has_ctx) {
     if (l != 0.f) j.wt = 1.f / l;  // (NaN too; no key at all: 0)
     return j;
   }
-  const float lc = lse[(int64_t)h * p.total_q + s.q0 + pos];
   const float top = vmax(lc, m);
   j.wc = fast_exp2(lc - top);  // an infinite top: NaN, as inf - inf is
   j.wt = m == -INFINITY ? 0.f : fast_exp2(m - top);
@@ -120,91 +117,117 @@ FMLM_DEV TreeJoin tree_join(const fmlm_attn_params& p, const float* lse, const T
 }
 
 // ---------------------------------------------------------------------------
-// bf16 / fp16, the 512-wide latent.  As in the forward kernels S^T = K Q^T and O^T = V^T P^T, so that a lane
-// (q + 16 g) holds keys 4g .. 4g+3 of query q and then columns 16 db + 4g .. of its output.
-// K fragments come straight from memory (a lane's 16 bytes of a key row are its operand);
-// V passes through LDS, whose transposing read makes its operand.  P is rounded to the input
-// type for the product, and its row sum is taken of the rounded values.
+// bf16 / fp16, the 512-wide latent (K = V = one row for all heads).  A workgroup of 4 waves takes 16
+// rows of one head.  As in the forward kernels S^T = K Q^T and O^T = V^T P^T, so that a lane
+// (q + 16 g) holds keys 4g .. 4g+3 of query q and then columns 16 db + 4g .. of its output.  Steps of
+// 32 keys pass through LDS once and serve both products: b128 reads make K's operand,
+// transposing reads V's.  Every wave computes all scores (32 MFMAs) and the output of its own 128
+// columns, which needs no exchange and leaves registers for the context's rows, loaded at the
+// start: what the kernel takes is the latency of its loads, and those of a step and of
+// the context's rows then overlap.  P is rounded to the input type for the product, and its row
+// sum is taken of the rounded values.
+// 16 sequences of up to 16 tokens, 64 heads: one wave a tile, keys and values read apart and the
+// context's rows at the end took 22.4 us.
 // ---------------------------------------------------------------------------
-template <typename T, int D>
-__global__ __launch_bounds__(64) void attn_tree_kernel(const fmlm_attn_params p, const float* __restrict__ octx,
-                                                       const float* __restrict__ lse,
-                                                       const uint64_t* __restrict__ mask, int words) {
+constexpr int kLatentD = 512, kLatentWaves = 4;
+
+template <typename T>
+__global__ __launch_bounds__(kLatentWaves * 64) void attn_tree_latent_kernel(const fmlm_attn_params p,
+                                                                             const float* __restrict__ octx,
+                                                                             const float* __restrict__ lse,
+                                                                             const uint64_t* __restrict__ mask,
+                                                                             int words) {
   typedef typename Mfma<T>::v8 v8;
-  constexpr int KC = (D + 31) / 32, NDB = D / 16, BK = 32;
+  constexpr int D = kLatentD, NW = kLatentWaves, KC = D / 32, NDB = D / 16 / NW, BK = 32;
   constexpr int PITCH = D * 2 + 16;  // 16 bytes apart: a column's rows fall into different banks
-  constexpr int CPR = D / 8, NL = BK * CPR / 64;
-  __shared__ __align__(16) char vt[BK * PITCH];
+  constexpr int NL = BK / NW;        // rows (1 KiB, one load) per wave and step
+  __shared__ __align__(16) char tile[BK * PITCH];
+  __shared__ uint32_t s_bad[NW];
   const int b = blockIdx.z, h = blockIdx.y, r0 = blockIdx.x * 16;
   const TreeSeq s = tree_seq(p, b, h);
   if (r0 >= s.len) return;
-  const int lane = threadIdx.x, l16 = lane & 15, g = lane >> 4;
-  const int pos = r0 + l16;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pos = r0 + l16, at = min(pos, s.len - 1), c0 = wave * NDB * 16;
   const bool ok = pos < s.len;
   const float c = p.scale * kLog2e;
   const T* const kp = (const T*)p.k + s.k0;
-  const T* const vp = (const T*)((p.flags & FMLM_FLAG_MLA) ? p.k : p.v) + s.v0;
 
+  u32x4 v[NL];
+  auto load = [&](int j0) {  // this wave's rows of a step; rows past the sequence are zero
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int row = j0 + wave * NL + n;
+      v[n] = u32x4{0u, 0u, 0u, 0u};
+      if (row < s.len) v[n] = *(const u32x4*)(kp + (int64_t)row * s.k_sn + lane * 8);
+    }
+  };
+  load(0);
   v8 qf[KC];
   {
-    const T* q = (const T*)p.q + tree_row(p.q_layout, b, h, s.q0, ok ? pos : s.len - 1, p.q_sb, p.q_sh, p.q_sn);
+    const T* q = (const T*)p.q + tree_row(p.q_layout, b, h, s.q0, at, p.q_sb, p.q_sh, p.q_sn);
 #pragma unroll
-    for (int kc = 0; kc < KC; ++kc) qf[kc] = kc * 32 + g * 8 < D ? *(const v8*)(q + kc * 32 + g * 8) : v8{};
+    for (int kc = 0; kc < KC; ++kc) qf[kc] = *(const v8*)(q + kc * 32 + g * 8);
+  }
+  f32x4 oc[NDB];
+  float lc = 0.f;
+  if (s.has_ctx) {
+    const int64_t row = (int64_t)h * p.total_q + s.q0 + at;
+    lc = lse[row];
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) oc[db] = *(const f32x4*)(octx + row * D + c0 + db * 16 + 4 * g);
   }
   f32x4 o[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
 
-  const uint32_t vaddr = lds_addr(vt) + (4 * g + (l16 >> 2)) * PITCH + 8 * (l16 & 3);
+  const uint32_t kaddr = lds_addr(tile) + l16 * PITCH + 16 * g;
+  const uint32_t vaddr = lds_addr(tile) + (4 * g + (l16 >> 2)) * PITCH + 8 * (l16 & 3) + 2 * c0;
   for (int j0 = 0; j0 < s.len; j0 += BK) {
     uint32_t seen = 0;  // keys j0 + bit that the lane's row attends to
     if (ok && j0 / 64 < words) seen = (uint32_t)(mask[(int64_t)(s.q0 + pos) * words + j0 / 64] >> (j0 % 64));
     if (s.len - j0 < BK) seen &= (1u << (s.len - j0)) - 1u;
-    if (!__builtin_amdgcn_ballot_w64(seen != 0)) continue;
-    // ---- V tile: rows past the sequence are zero, and so are rows with an element that is
-    // not finite: 0 times it would not be 0 in the rows that do not see it (see below)
-    uint32_t bad = 0;
-    {
-      u32x4 v[NL > 0 ? NL : 1];
-#pragma unroll
-      for (int n = 0; n < NL; ++n) {
-        const int at = n * 64 + lane, row = at / CPR;
-        v[n] = u32x4{0u, 0u, 0u, 0u};
-        if (j0 + row < s.len) v[n] = *(const u32x4*)(vp + (int64_t)(j0 + row) * s.v_sn + (at % CPR) * 8);
-      }
-      constexpr uint32_t E = std::is_same<T, bf16>::value ? 0x7f80u : 0x7c00u;  // exponent of inf and NaN
-      uint32_t mine = 0;
-#pragma unroll
-      for (int n = 0; n < NL; ++n) {
-        const int at = n * 64 + lane, row = at / CPR;
-        bool inf = false;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) inf |= (v[n][w] & E) == E || (v[n][w] >> 16 & E) == E;
-        if (inf) mine |= 1u << row;
-        *(u32x4*)(vt + row * PITCH + (at % CPR) * 16) = v[n];
-      }
-      if (__builtin_amdgcn_ballot_w64(mine != 0)) {
-        for (int r = 0; r < BK; ++r)
-          if (__builtin_amdgcn_ballot_w64(mine >> r & 1)) bad |= 1u << r;
-#pragma unroll
-        for (int n = 0; n < NL; ++n) {
-          const int at = n * 64 + lane, row = at / CPR;
-          if (bad >> row & 1) *(u32x4*)(vt + row * PITCH + (at % CPR) * 16) = u32x4{0u, 0u, 0u, 0u};
-        }
-      }
+    // (the same in every wave; a step up to the rows' own has keys they see)
+    if (j0 >= r0 + 16 && !__builtin_amdgcn_ballot_w64(seen != 0)) continue;
+    if (j0 > 0) {
+      load(j0);
+      __syncthreads();  // the tile's last readers are done
     }
+    // ---- the tile, and which of its rows have an element that is not finite: 0 times it would
+    // not be 0 in the rows that do not see it (below)
+    constexpr uint32_t E = std::is_same<T, bf16>::value ? 0x7f80u : 0x7c00u;  // exponent of inf and NaN
+    uint32_t mine = 0;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int row = wave * NL + n;
+      bool inf = false;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) inf |= (v[n][w] & E) == E || (v[n][w] >> 16 & E) == E;
+      if (__builtin_amdgcn_ballot_w64(inf)) mine |= 1u << row;
+      *(u32x4*)(tile + row * PITCH + lane * 16) = v[n];
+    }
+    if (lane == 0) s_bad[wave] = mine;
+    __syncthreads();
     // ---- scores
     f32x4 sc[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      const T* k = kp + (int64_t)min(j0 + kb * 16 + l16, s.len - 1) * s.k_sn;
       sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kc = 0; kc < KC; ++kc) {
-        const v8 a = kc * 32 + g * 8 < D ? *(const v8*)(k + kc * 32 + g * 8) : v8{};
-        sc[kb] = Mfma<T>::run(a, qf[kc], sc[kb]);
-      }
+      for (int kc = 0; kc < KC; ++kc)
+        sc[kb] = Mfma<T>::run(*(const FMLM_LDS v8*)(uintptr_t)(kaddr + kb * 16 * PITCH + kc * 64), qf[kc], sc[kb]);
+    }
+    uint32_t bad = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) bad |= s_bad[w];
+    bad = __builtin_amdgcn_readfirstlane(bad);
+    if (bad) {
+      __syncthreads();  // every wave has its scores
+#pragma unroll
+      for (int n = 0; n < NL; ++n)
+        if (bad >> (wave * NL + n) & 1) *(u32x4*)(tile + (wave * NL + n) * PITCH + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+      __syncthreads();
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -229,7 +252,6 @@ __global__ __launch_bounds__(64) void attn_tree_kernel(const fmlm_attn_params p,
         sum += (float)x;
       }
     l = l * alpha + sum;
-    wait_reads();  // the tile is in LDS (one wave: no barrier)
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
       const s16x4 lo = lds_read_tr16_at(vaddr + db * 32), hi = lds_read_tr16_at(vaddr + db * 32 + 16 * PITCH);
@@ -245,25 +267,23 @@ __global__ __launch_bounds__(64) void attn_tree_kernel(const fmlm_attn_params p,
         if (e == (j >> 4) * 4 + (j & 3)) x = (float)pf[e];
       x = __shfl(x, from);
       if (seen >> j & 1) {
-        const T* v = vp + (int64_t)(j0 + j) * s.v_sn + 4 * g;
+        const T* vj = kp + (int64_t)(j0 + j) * s.k_sn + c0 + 4 * g;
 #pragma unroll
         for (int db = 0; db < NDB; ++db)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[db][r] = fmaf(x, (float)v[db * 16 + r], o[db][r]);
+          for (int r = 0; r < 4; ++r) o[db][r] = fmaf(x, (float)vj[db * 16 + r], o[db][r]);
       }
     }
-    wait_reads();  // the next tile may overwrite this one
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
   if (!ok) return;
-  const TreeJoin j = tree_join(p, lse, s, h, pos, m, l);
-  T* const dst = (T*)p.o + tree_row(p.o_layout, b, h, s.q0, pos, p.o_sb, p.o_sh, p.o_sn) + 4 * g;
-  const float* const oc = octx + ((int64_t)h * p.total_q + s.q0 + pos) * D + 4 * g;
+  const TreeJoin j = tree_join(s.has_ctx, lc, m, l);
+  T* const dst = (T*)p.o + tree_row(p.o_layout, b, h, s.q0, pos, p.o_sb, p.o_sh, p.o_sn) + c0 + 4 * g;
 #pragma unroll
   for (int db = 0; db < NDB; ++db) {
     f32x4 x = o[db] * j.wt;
-    if (s.has_ctx) x += j.wc * *(const f32x4*)(oc + db * 16);
+    if (s.has_ctx) x += j.wc * oc[db];
     T y[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
@@ -331,7 +351,7 @@ __global__ __launch_bounds__(64) void attn_tree_f32_kernel(const fmlm_attn_param
   }
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off);
-  const TreeJoin j = tree_join(p, lse, s, h, pos, m, l);
+  const TreeJoin j = tree_join(s.has_ctx, s.has_ctx ? lse[(int64_t)h * p.total_q + s.q0 + pos] : 0.f, m, l);
   float* const dst = (float*)p.o + tree_row(p.o_layout, b, h, s.q0, pos, p.o_sb, p.o_sh, p.o_sn);
   const float* const oc = octx + ((int64_t)h * p.total_q + s.q0 + pos) * D;
 #pragma unroll
@@ -358,11 +378,12 @@ int launch_tree_part(const fmlm_attn_params& ctx, const fmlm_attn_params& p, con
   const float* const octx = (const float*)ctx.o;
   if (p.dtype != FMLM_DTYPE_F32) {
     const dim3 grid((unsigned)((longest + 15) / 16), (unsigned)p.H, (unsigned)p.B);
-    if (p.D != 512) return FMLM_E_HEAD_DIM;
+    const dim3 block(kLatentWaves * 64);
+    if (p.D != kLatentD || !(p.flags & FMLM_FLAG_MLA)) return FMLM_E_HEAD_DIM;
     if (p.dtype == FMLM_DTYPE_BF16)
-      hipLaunchKernelGGL((attn_tree_kernel<bf16, 512>), grid, dim3(64), 0, s, p, octx, ctx.lse, mask, words);
+      hipLaunchKernelGGL(attn_tree_latent_kernel<bf16>, grid, block, 0, s, p, octx, ctx.lse, mask, words);
     else
-      hipLaunchKernelGGL((attn_tree_kernel<f16, 512>), grid, dim3(64), 0, s, p, octx, ctx.lse, mask, words);
+      hipLaunchKernelGGL(attn_tree_latent_kernel<f16>, grid, block, 0, s, p, octx, ctx.lse, mask, words);
     return launch_status();
   }
   const dim3 grid((unsigned)longest, (unsigned)p.H, (unsigned)p.B);
