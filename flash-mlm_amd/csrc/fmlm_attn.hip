@@ -2718,22 +2718,35 @@ static Launch mla_rows_launch(const fmlm_attn_params& p) {
                 true, true, mla_rows_fn<T, true, 1>(paged, lse, f32), 3.4f};
 }
 
-// MFMA kernels by head dim.  The pipelined kernel and the 512-wide latent kernel need
-// linear main-key addressing; causal_query_seq_attn over padded K/V (a per-row sequence
-// lookup) takes the register-staged kernel.  The latent kernel also needs K = V (MLA).
+// Tree calls take 64-row workgroups: drafts are short.  Longer ones gain nothing from two row
+// blocks a wave (D = 64 and 128, 8 sequences of 64-128 or 120-256 tokens over 4000 rows, 16 heads: 44.6
+// / 61.4 / 61.4 / 89.0 us against 45.8 / 62.0 / 62.8 / 84.1).  At D = 256, where a workgroup
+// fills a CU, 128 rows on 8 waves pay when sequences have more than 64, contexts are long (2048 rows
+// on average) and 128-row tiles are at least 48: 8 heads, 4000 rows, 8 sequences of 64-128 tokens 69.3 us
+// against 76.0, of 120-256 93.6 against 110.3, 24 of 60-80 over 3000 rows 121.5 against 154.8; but
+// 8 of 100-128 over 300 rows 29.5 against 25.4, one of 256 over 4000 rows 43.8 against 38.8.
 template <typename T>
 static bool pick_tree(const fmlm_attn_params& p, Launch& L) {
   const bool paged = p.ctx_block_table != nullptr;
-  if (p.tile_config > 1) return false;
+  const int64_t rows = paged ? (int64_t)p.ctx_pages_per_batch * FMLM_PAGE_ROWS : p.ctx_rows / std::max(p.ctx_batch, 1);
+  const bool wide = p.D == 256 && p.total_q > 64LL * p.B && rows >= 2048 &&
+                    (int64_t)p.H * (p.total_q / 128 + p.B / 2) >= 48;
+  const int k = p.tile_config > 0 ? p.tile_config : wide ? 2 : 1;
+  if (k > (p.D == 256 ? 2 : 1)) return false;
   switch (p.D) {
     case 16: L = mfma3_launch<T, 16, 1, 4, 64, 0, true>(paged); return true;
     case 32: L = mfma3_launch<T, 32, 1, 4, 64, 0, true>(paged); return true;
     case 64: L = mfma3_launch<T, 64, 1, 4, 64, 0, true>(paged); return true;
     case 128: L = mfma3_launch<T, 128, 1, 4, 64, 0, true>(paged); return true;
-    case 256: L = mfma3_launch<T, 256, 1, 4, 64, 0, true>(paged); return true;
+    case 256:
+      L = k == 2 ? mfma3_launch<T, 256, 1, 8, 64, 0, true>(paged) : mfma3_launch<T, 256, 1, 4, 64, 0, true>(paged);
+      return true;
     default: return false;
   }
 }
+// MFMA kernels by head dim.  The pipelined kernel and the 512-wide latent kernel need
+// linear main-key addressing; causal_query_seq_attn over padded K/V (a per-row sequence
+// lookup) takes the register-staged kernel.  The latent kernel also needs K = V (MLA).
 template <typename T>
 static bool pick_mfma(const fmlm_attn_params& p, Launch& L) {
   if (p.flags & FMLM_FLAG_TREE) return pick_tree<T>(p, L);

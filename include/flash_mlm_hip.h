@@ -253,7 +253,8 @@ typedef struct fmlm_attn_params {
    * 2 = (256, 8), 3 = (64, 4), 4 = (256, 8) ping-pong; D = 128: 1 = (128, 4),
    * 2 = (256, 8), 3 = (64, 4), 4 = (128, 8), 5 = (256, 8) ping-pong; D = 256:
    * 1 = (64, 4), 2 = (128, 8); MLA D = 512: 1 = (128, 8), in packed calls of at most 4096
-   * (head, position) rows (64, 8).  Ping-pong: the 8 waves run as
+   * (head, position) rows (64, 8).  Tree calls (FMLM_FLAG_TREE): 1 = (64, 4), D = 256 also 2 = (128, 8).
+   * Ping-pong: the 8 waves run as
    * two groups half a key tile apart, so that one wave of each SIMD computes softmax
    * while the other issues MFMAs.  Replaces the reference's autotuned
    * BLOCK_M / BLOCK_N / num_warps (mlm_kernel.py:57-166).  Ignored by f32 inputs.       */

@@ -274,6 +274,22 @@ def test_long_drafts_and_long_contexts(dtype, chain, device):
 
 
 @pytest.mark.gpu
+def test_wide_head_dim_tiles(device):
+    """D = 256: 64- and 128-row workgroups, and the library's choice of the latter"""
+    from flash_mlm.host.host import tile_config
+
+    run = dict(lens=[200, 140, 3], N=200, H=2, D=256, ctx=[130, 64, 300], kind="packed", seed=2)
+    with tile_config(1):
+        a = _run(device, torch.bfloat16, **run)
+    with tile_config(2):
+        b = _run(device, torch.bfloat16, **run)
+    assert a.shape == b.shape
+    with tile_config(2), pytest.raises(RuntimeError, match="invalid argument"):
+        _run(device, torch.bfloat16, lens=[9], N=9, H=2, D=64, ctx=[9], kind="packed")
+    _run(device, torch.float16, lens=[70] * 8, N=70, H=8, D=256, ctx=[2300] * 8, kind="paged", seed=3)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_scales(dtype, scale, device):
