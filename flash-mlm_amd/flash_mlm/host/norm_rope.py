@@ -14,11 +14,12 @@ import torch
 
 from flash_mlm import _lib
 from flash_mlm.host.cache import PackMetadata
-from flash_mlm.host.host import _wants_grad, rows16
+from flash_mlm.host.host import rows16
 from flash_mlm.host.host_utils import require_cuda_tensors, validate_head_dim_supported
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _INTS = (torch.int32, torch.int64)
+_HEAD_DIMS = (16, 32, 64, 128, 256, 512)
 
 
 def aligned16(t: torch.Tensor) -> torch.Tensor:
@@ -30,7 +31,7 @@ def aligned16(t: torch.Tensor) -> torch.Tensor:
 class _Call:
     """The checked arguments of one call as a parameter block without the rows' addresses."""
 
-    __slots__ = ("block", "packed", "shapes", "keep")
+    __slots__ = ("block", "packed", "keep")
 
     def put(self, t, x, y) -> None:
         """Rows in and out of tensor ``t`` of a block (packed rows: strides are the block's)."""
@@ -39,9 +40,8 @@ class _Call:
             t.x_sb, t.x_sh, t.x_sn, _ = x.stride()
 
 
-def _rows_out(call: _Call, q, k):
-    return (torch.empty(call.shapes[0], dtype=q.dtype, device=q.device),
-            torch.empty(call.shapes[1], dtype=k.dtype, device=k.device))
+def _out(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _run(entry, name: str, p, device) -> None:
@@ -55,7 +55,7 @@ def _run(entry, name: str, p, device) -> None:
 
 
 def _forward(call: _Call, q, k):
-    outs = _rows_out(call, q, k)
+    outs = _out(q), _out(k)
     p = call.block
     if p.rows:
         call.put(p.q, q, outs[0])
@@ -69,13 +69,15 @@ def _backward(call: _Call, xs, ws, dys, needs):
     lib = _lib.load()
     dev = xs[0].device
     p = _lib.NormRopeParams.from_buffer_copy(call.block)  # (a graph can be walked more than once)
+    if p.rows == 0:
+        return tuple(torch.zeros_like(t) if n else None for t, n in zip((*xs, *ws), needs))
     dxs, dws, keep = [None, None], [None, None], []
     for i, t in enumerate((p.q, p.k)):
         if dys[i] is None or not (needs[i] or needs[2 + i]):
             t.heads = 0
             continue
         dy = rows16(dys[i])
-        dx = dxs[i] = torch.empty(call.shapes[i], dtype=xs[i].dtype, device=dev)
+        dx = dxs[i] = _out(xs[i])
         call.put(t, xs[i], dx)
         t.dy = dy.data_ptr()
         if call.packed:
@@ -83,7 +85,7 @@ def _backward(call: _Call, xs, ws, dys, needs):
         else:
             t.dy_sb, t.dy_sh, t.dy_sn, _ = dy.stride()
         if needs[2 + i]:
-            dw = dws[i] = torch.empty(ws[i].shape, dtype=ws[i].dtype, device=dev)
+            dw = dws[i] = torch.empty_like(ws[i])
             t.dweight = dw.data_ptr()
         keep.append(dy)
     if keep:
@@ -205,12 +207,14 @@ def qk_norm_rope(
     d = qs[-1]
     if ks[-1] != d:
         raise ValueError("q and k must have the same head_dim")
-    validate_head_dim_supported(d, is_mla=True)
+    if d not in _HEAD_DIMS:
+        validate_head_dim_supported(d, is_mla=True)
     if dtype not in _FLOATS or k.dtype != dtype:
         raise ValueError("q and k must be of one dtype: bf16, fp16 or fp32")
     if k.device != dev:
         raise ValueError("q and k must be on one device")
-    require_cuda_tensors(q, k, q_weight, k_weight, cos, sin)
+    if not q.is_cuda:
+        require_cuda_tensors(q)
     if q_meta is not None and q_meta.cu_seqlens.device != dev:
         raise ValueError("q_meta must be on the device of q and k")
 
@@ -250,7 +254,6 @@ def qk_norm_rope(
         for t in (p.q, p.k):
             t.x_sh = t.y_sh = rows * d
             t.x_sn = t.y_sn = d
-    call.shapes = (qs, ks)
     if b * n > 0x7FFFFFFF:
         raise ValueError("q and k must have fewer than 2**31 tokens")
     p.dtype = _lib.dtype_code(dtype)
@@ -315,7 +318,11 @@ def qk_norm_rope(
         raise ValueError("positions and context_lens need cos and sin")
     p.flags = flags
     q_, k_ = rows16(q), rows16(k)
-    if _wants_grad(q, k, q_weight, k_weight):
+    grad = torch.is_grad_enabled()
+    if grad and cos is not None and (cos.requires_grad or sin.requires_grad):
+        raise ValueError("cos and sin are constants: qk_norm_rope has no gradient of them")
+    if grad and (q.requires_grad or k.requires_grad or (wq is not None and wq.requires_grad)
+                 or (wk is not None and wk.requires_grad)):
         # the block holds the addresses of what is saved, and of these
         call.keep = (cu, tokens)
         leaves = _capture_leaves(q, k, q_weight, k_weight)

@@ -213,6 +213,27 @@ def test_lengths(lens, N, gain, device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("shape", [(2, 0), (0, 3)])
+def test_no_tokens(packed, shape, device):
+    """Outputs and gradients of nothing are empty, the gains' gradients zero."""
+    B, N = shape
+    if packed:
+        meta = build_pack_metadata(torch.zeros(2, dtype=torch.int32, device=device), 4, 32)
+        q = torch.zeros((0, 64), device=device, requires_grad=True)
+        kw = dict(q_meta=meta)
+    else:
+        q = torch.zeros((B, 3, N, 64), device=device, requires_grad=True)
+        kw = {}
+    w = torch.ones(64, device=device, requires_grad=True)
+    cos, sin = _tables(4, 64, device)
+    out = qk_norm_rope(q, q, q_weight=w, k_weight=w, cos=cos, sin=sin, **kw)
+    assert out[0].shape == q.shape
+    dq, dw = torch.autograd.grad(out, (q, w), tuple(torch.zeros_like(x) for x in out))
+    assert dq.shape == q.shape and dw.shape == w.shape and not dw.any()
+
+
+@pytest.mark.gpu
 def test_mixed_gains(device):
     """Gains per head for q, shared for k: one launch, two layouts of dw."""
     q, k, dq, dk, kw, cos, sin, tokens, _ = _case(device, torch.float32, H=5, Hk=3, D=32, lens=[9, 30], N=30, R=32,
@@ -313,6 +334,8 @@ def test_refusals(device):
     ]:
         with pytest.raises(ValueError, match=match):
             qk_norm_rope(q, q, **kw)
+    with pytest.raises(ValueError, match="constants"):
+        qk_norm_rope(q, q, cos=cos.clone().requires_grad_(), sin=sin)
     with pytest.raises(ValueError, match="q_meta"):
         qk_norm_rope(q[:1], q[:1], q_meta=meta)
     with pytest.raises(ValueError, match="packed q needs"):
