@@ -2175,7 +2175,10 @@ struct F32Cfg {
   static_assert(BK == NW * 16, "16 keys of a tile per wave");
 };
 
-template <int D, int QB>
+// TREE: main keys masked by spa.mask as in attn_mfma3_kernel, in the wave's own 16 keys of a tile.
+// 8 sequences of 200-256 drafted tokens, 12 heads, D = 128, 500-1000 context rows: 129 us, the same
+// call without masks 134; with the tree's part in a kernel of its own 168 to 339, by the depth.
+template <int D, int QB, bool TREE = false>
 __global__ __launch_bounds__(256, (F32Cfg<D, QB>::WPS)) void attn_f32_kernel(
     const fmlm_attn_params p, const int4* __restrict__ units, const int32_t* __restrict__ hdr, const SplitArgs spa) {
   typedef F32Cfg<D, QB> C;
@@ -2240,6 +2243,14 @@ __global__ __launch_bounds__(256, (F32Cfg<D, QB>::WPS)) void attn_f32_kernel(
     else TL::load(src, pitch, nkeys(t) - 1 - j0, v ? vt : kt, lane);
   };
 
+  // the wave's 16 bits of the row's mask word for tile t
+  auto tree_bits = [&](int qb, int t) {
+    const int row = qb * 16 + l16, i = t - nt0;
+    return row < w.qcount && i < spa.words
+               ? (uint32_t)(spa.mask[(int64_t)(w.q0 + w.qpos0 + row) * spa.words + i] >> (wave * 16)) & 0xffffu
+               : 0u;
+  };
+
   f32x4 o[QB][C::NG][C::E];
   float m_i[QB], l_i[QB];
 #pragma unroll
@@ -2275,6 +2286,39 @@ __global__ __launch_bounds__(256, (F32Cfg<D, QB>::WPS)) void attn_f32_kernel(
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) s[qb][r] = -INFINITY;
       }
+      uint32_t bad = 0;  // the wave's keys of a masked tile with values that are not finite
+      if (TREE && t >= nt0) {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          const uint32_t seen = tree_bits(qb, t) >> (4 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!(seen >> r & 1)) s[qb][r] = -INFINITY;
+        }
+        wait_loads<TL::NL>();  // V (the next K's loads came later)
+        constexpr uint32_t E = 0x7f800000u;
+        auto not_finite = [&](int i) {
+          const u32x4 x = *(const FMLM_LDS u32x4*)(uintptr_t)(vt + i * 1024 + lane * 16);
+          return (x[0] & E) == E || (x[1] & E) == E || (x[2] & E) == E || (x[3] & E) == E;
+        };
+        bool any = false;
+#pragma unroll 4
+        for (int i = 0; i < TL::NL; ++i) any |= not_finite(i);
+        if (__builtin_amdgcn_ballot_w64(any)) {  // out of the tile; added below by the rows that see them
+          for (int i = 0; i < TL::NL; ++i) {
+            const int row = (i * 1024 + lane * 16) / TL::PITCH;
+            uint32_t mine = not_finite(i) ? 1u << row : 0u;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) mine |= (uint32_t)__shfl_xor((int)mine, off);
+            bad |= mine;
+          }
+          bad = __builtin_amdgcn_readfirstlane(bad);
+          for (int i = 0; i < TL::NL; ++i)
+            if (bad >> ((i * 1024 + lane * 16) / TL::PITCH) & 1)
+              *(FMLM_LDS u32x4*)(uintptr_t)(vt + i * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+          wait_reads();
+        }
+      }
       float mx[QB];  // the lane's largest score of the row
       bool grow = false;
 #pragma unroll
@@ -2305,6 +2349,28 @@ __global__ __launch_bounds__(256, (F32Cfg<D, QB>::WPS)) void attn_f32_kernel(
       }
       wait_loads<TL::NL>();  // V (the next K's loads came later)
       mma_cols<D, QB>(vt, l16, g, s, o);
+      if constexpr (TREE)
+        for (; bad; bad &= bad - 1) {
+          const int j = __builtin_ctz(bad);
+          if (j >= nk) break;  // (rows behind the last key are zero)
+          const float* v = vp1 + (int64_t)(key0(t) + j) * w.seg[1].vsn + 4 * C::E * g;
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) {
+            float x = 0.f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (r == (j & 3)) x = s[qb][r];
+            x = __shfl(x, l16 + 16 * (j >> 2));
+            if (tree_bits(qb, t) >> j & 1)
+#pragma unroll
+              for (int dg = 0; dg < C::NG; ++dg)
+#pragma unroll
+                for (int e = 0; e < C::E; ++e)
+#pragma unroll
+                  for (int r = 0; r < 4; ++r)
+                    o[qb][dg][e][r] = fmaf(x, v[16 * C::E * dg + C::E * r + e], o[qb][dg][e][r]);
+          }
+        }
       wait_reads();
       load(tl, true);
       t = tn;
@@ -2356,8 +2422,9 @@ __global__ __launch_bounds__(256, (F32Cfg<D, QB>::WPS)) void attn_f32_kernel(
         ml[C::BQ + row] = L;
       }
     } else {
-      // L is 0 only where every score is -inf (a row has keys, its own): NaN, as 0 * (1 / 0)
-      *(f32x4*)((float*)p.o + w.o_row0 + (int64_t)row * w.o_sn + col) = acc * (1.f / L);
+      // L is 0 only where every score is -inf (a row has keys, its own): NaN, as 0 * (1 / 0);
+      // TREE: or where the row sees no key
+      *(f32x4*)((float*)p.o + w.o_row0 + (int64_t)row * w.o_sn + col) = acc * (TREE && M == -INFINITY ? 0.f : 1.f / L);
       if (p.lse && col == 0) store_lse(p, w.h, w.q0, w.qpos0 + row, M, L);
     }
   }
@@ -2664,10 +2731,10 @@ static Launch simt_launch() {
   return Launch{C::RPW, C::NT, C::LDS_BYTES, (const void*)&attn_simt_kernel<T, D>};
 }
 
-template <int D, int QB>
+template <int D, int QB, bool TREE>
 static Launch f32_launch() {
   typedef F32Cfg<D, QB> C;
-  Launch L{C::BQ, C::NT, C::LDS_BYTES, (const void*)&attn_f32_kernel<D, QB>, true};
+  Launch L{C::BQ, C::NT, C::LDS_BYTES, (const void*)&attn_f32_kernel<D, QB, TREE>, true};
   L.tile_us = 0.3f + 0.6f * QB * D / 64;
   return L;
 }
@@ -2839,24 +2906,25 @@ static bool pick_simt(int D, Launch& L) {
 // D = 64 below 256 tiles of 32 rows (2 x 8 heads x 128: 6.4 us); at D = 128 below 64, since
 // long contexts split anyway and wide tiles then merge less (4 x 8 x 100 queries, 1000
 // context rows: 32 us against 38).
+template <bool TREE>
 static bool pick_f32(const fmlm_attn_params& p, Launch& L) {
   if ((p.flags & FMLM_FLAG_CAUSAL_SEQ) && p.cu_seqlens_q && p.kv_layout != FMLM_LAYOUT_PACKED) return false;
   const int64_t rows = p.cu_seqlens_q ? p.total_q : (int64_t)p.B * p.N;
   const bool small = p.H * rows < (p.D == 64 ? 256 : 64) * 32;
   switch (p.D) {
-    case 16: L = f32_launch<16, 4>(); return true;
-    case 32: L = f32_launch<32, 2>(); return true;
-    case 64: L = small ? f32_launch<64, 1>() : f32_launch<64, 2>(); return true;
-    case 128: L = small ? f32_launch<128, 1>() : f32_launch<128, 2>(); return true;
-    case 256: L = small ? f32_launch<256, 1>() : f32_launch<256, 2>(); return true;
+    case 16: L = f32_launch<16, 4, TREE>(); return true;
+    case 32: L = f32_launch<32, 2, TREE>(); return true;
+    case 64: L = small ? f32_launch<64, 1, TREE>() : f32_launch<64, 2, TREE>(); return true;
+    case 128: L = small ? f32_launch<128, 1, TREE>() : f32_launch<128, 2, TREE>(); return true;
+    case 256: L = small ? f32_launch<256, 1, TREE>() : f32_launch<256, 2, TREE>(); return true;
     default: return false;
   }
 }
 
-// Tree calls: the MFMA kernels of 16-bit types up to D = 256 mask the main keys themselves; the
-// others (the 512-wide latent, fp32) run a context-only call beside a kernel of the tree's part
-// (fmlm_tree.hip).  A call's parameters as its launches use them:
-static bool tree_fused(const fmlm_attn_params& p) { return p.dtype != FMLM_DTYPE_F32 && p.D <= 256; }
+// Tree calls: the MFMA kernels up to D = 256 mask the main keys themselves; at D = 512 (MLA) a
+// context-only call runs beside a kernel of the tree's part (fmlm_tree.hip).  A call's
+// parameters as its launches use them:
+static bool tree_fused(const fmlm_attn_params& p) { return p.D <= 256; }
 static fmlm_attn_params effective(const fmlm_attn_params& p) {
   fmlm_attn_params e = p;
   e.flags &= ~(kFlagCtxOnly | kFlagF32Out);
@@ -2875,10 +2943,13 @@ static fmlm_attn_params effective(const fmlm_attn_params& p) {
 static int pick_launch(const fmlm_attn_params& p, Launch& L) {
   bool ok = false;
   if (p.tile_config < 0) return FMLM_E_ARG;
+  const bool simt = p.tile_config <= 1 && !(p.flags & FMLM_FLAG_TREE);
   switch (p.dtype) {
-    case FMLM_DTYPE_BF16: ok = pick_mfma<bf16>(p, L) || (p.tile_config <= 1 && pick_simt<bf16>(p.D, L)); break;
-    case FMLM_DTYPE_F16: ok = pick_mfma<f16>(p, L) || (p.tile_config <= 1 && pick_simt<f16>(p.D, L)); break;
-    case FMLM_DTYPE_F32: ok = pick_f32(p, L) || pick_simt<float>(p.D, L); break;
+    case FMLM_DTYPE_BF16: ok = pick_mfma<bf16>(p, L) || (simt && pick_simt<bf16>(p.D, L)); break;
+    case FMLM_DTYPE_F16: ok = pick_mfma<f16>(p, L) || (simt && pick_simt<f16>(p.D, L)); break;
+    case FMLM_DTYPE_F32:
+      ok = (p.flags & FMLM_FLAG_TREE) ? pick_f32<true>(p, L) : pick_f32<false>(p, L) || pick_simt<float>(p.D, L);
+      break;
     default: return FMLM_E_DTYPE;
   }
   if (!ok) return p.tile_config > 1 ? FMLM_E_ARG : FMLM_E_HEAD_DIM;

@@ -2,8 +2,8 @@
 // does not mask its keys itself.
 //
 // Query i of a sequence attends to the sequence's context and to those tokens j of its own
-// draft that are i or an ancestor of i.  The MFMA kernels of 16-bit types up to D = 256 do all of it
-// (fmlm_attn.hip).  For the 512-wide latent and fp32 the context's part runs by itself and
+// draft that are i or an ancestor of i.  The MFMA kernels up to D = 256 do all of it
+// (fmlm_attn.hip).  For the 512-wide latent the context's part runs by itself and
 // leaves, per row, its own softmax's output o_c (fp32) and l_c = log2(sum 2^z), z =
 // scale log2(e) q.k.  A kernel here computes m = max z and l = sum 2^(z - m) over the ancestors
 // and writes
@@ -294,15 +294,15 @@ __global__ __launch_bounds__(kLatentWaves * 64) void attn_tree_latent_kernel(con
 }
 
 // ---------------------------------------------------------------------------
-// fp32: one wave per row.  Lane j scores key j of a step of 64 keys; then the row's keys are
-// taken one by one, a lane holding D / 64 columns (the first D lanes one each below 64).
+// fp32 latent (whose context runs on the SIMT kernel): one wave per row.  Lane j scores key j of a step of 64 keys; then the row's keys are
+// taken one by one, a lane holding D / 64 columns.
 // Keys that the row does not see are not read.
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ __launch_bounds__(64) void attn_tree_f32_kernel(const fmlm_attn_params p, const float* __restrict__ octx,
                                                            const float* __restrict__ lse,
                                                            const uint64_t* __restrict__ mask, int words) {
-  constexpr int NC = (D + 63) / 64;
+  constexpr int NC = D / 64;
   __shared__ __align__(16) float qs[D];
   const int b = blockIdx.z, h = blockIdx.y, pos = blockIdx.x, lane = threadIdx.x;
   const TreeSeq s = tree_seq(p, b, h);
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(64) void attn_tree_f32_kernel(const fmlm_attn_param
       const float* v = vp + (int64_t)(w * 64 + j) * s.v_sn;
 #pragma unroll
       for (int i = 0; i < NC; ++i)
-        if (D >= 64 || lane < D) o[i] = fmaf(pj, v[lane + 64 * i], o[i]);
+        o[i] = fmaf(pj, v[lane + 64 * i], o[i]);
     }
   }
 #pragma unroll
@@ -355,12 +355,11 @@ __global__ __launch_bounds__(64) void attn_tree_f32_kernel(const fmlm_attn_param
   float* const dst = (float*)p.o + tree_row(p.o_layout, b, h, s.q0, pos, p.o_sb, p.o_sh, p.o_sn);
   const float* const oc = octx + ((int64_t)h * p.total_q + s.q0 + pos) * D;
 #pragma unroll
-  for (int i = 0; i < NC; ++i)
-    if (D >= 64 || lane < D) {
-      float x = o[i] * j.wt;
-      if (s.has_ctx) x = fmaf(j.wc, oc[lane + 64 * i], x);
-      dst[lane + 64 * i] = x;
-    }
+  for (int i = 0; i < NC; ++i) {
+    float x = o[i] * j.wt;
+    if (s.has_ctx) x = fmaf(j.wc, oc[lane + 64 * i], x);
+    dst[lane + 64 * i] = x;
+  }
 }
 
 bool tree_part_aligned(const fmlm_attn_params& p) {
@@ -387,13 +386,8 @@ int launch_tree_part(const fmlm_attn_params& ctx, const fmlm_attn_params& p, con
     return launch_status();
   }
   const dim3 grid((unsigned)longest, (unsigned)p.H, (unsigned)p.B);
-#define FMLM_TREE(DD) \
-  case DD: hipLaunchKernelGGL((attn_tree_f32_kernel<DD>), grid, dim3(64), 0, s, p, octx, ctx.lse, mask, words); break;
-  switch (p.D) {
-    FMLM_TREE(16) FMLM_TREE(32) FMLM_TREE(64) FMLM_TREE(128) FMLM_TREE(256) FMLM_TREE(512)
-    default: return FMLM_E_HEAD_DIM;
-  }
-#undef FMLM_TREE
+  if (p.D != kLatentD) return FMLM_E_HEAD_DIM;
+  hipLaunchKernelGGL(attn_tree_f32_kernel<kLatentD>, grid, dim3(64), 0, s, p, octx, ctx.lse, mask, words);
   return launch_status();
 }
 

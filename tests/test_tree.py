@@ -120,11 +120,12 @@ def test_abi_refuses():
     g = _lib.AttnGrads()
     g.dout = g.dq = g.dk = g.dv = 256
     assert lib.fmlm_attn_bwd(p, g, None) == -1
-    p.dtype = _lib.DTYPE_F32  # the tree's part in a kernel of its own
-    assert lib.fmlm_attn_tree_workspace_bytes(p) == 4 * 4 * 65
+    p.dtype = _lib.DTYPE_F32
+    assert lib.fmlm_attn_tree_workspace_bytes(p) == 0 and a(p, 256, 1) == -5
+    p.D, p.v = 512, 264  # the tree's part in a kernel of its own
+    assert lib.fmlm_attn_tree_workspace_bytes(p) == 4 * 4 * 513
     assert a(p, 256, 1) == -5
-    p.v = 264
-    assert a(p, 256, 1, 256, 4 * 4 * 65) == -4
+    assert a(p, 256, 1, 256, 4 * 4 * 513) == -4
     p.dtype, p.D = _lib.DTYPE_BF16, 512  # only the latent
     assert lib.fmlm_attn_workspace_bytes(p) == -3
     assert a(p, 256, 1, 256, 4 * 4 * 513) == -4
@@ -252,9 +253,12 @@ def test_attention(dtype, D, kind, device):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("kind", ["none", "packed", "paged", "index"])
 def test_mla(dtype, kind, device):
+    if dtype == "fp32" and kind in ("paged", "index"):
+        pytest.skip("paged contexts are bf16 / fp16")
+    _run(device, DT[dtype], lens=[7, 40], N=40, H=2, D=128, ctx=[30, 100], kind=kind, mla=True, seed=2)
     _run(device, DT[dtype], lens=[5, 33, 1], N=33, H=4, D=512, ctx=[300, 65, 0], kind=kind, mla=True, seed=3)
 
 
