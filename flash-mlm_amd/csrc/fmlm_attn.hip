@@ -2176,8 +2176,8 @@ struct F32Cfg {
 };
 
 // TREE: main keys masked by spa.mask as in attn_mfma3_kernel, in the wave's own 16 keys of a tile.
-// 8 sequences of 200-256 drafted tokens, 12 heads, D = 128, 500-1000 context rows: 129 us, the same
-// call without masks 134; with the tree's part in a kernel of its own 168 to 339, by the depth.
+// 8 sequences of 200-256 drafted tokens, 12 heads, D = 128, 500-1000 context rows: 131 us, the same
+// call without masks 136; with the tree's part in a kernel of its own 168 to 339, by the depth.
 template <int D, int QB, bool TREE = false>
 __global__ __launch_bounds__(256, (F32Cfg<D, QB>::WPS)) void attn_f32_kernel(
     const fmlm_attn_params p, const int4* __restrict__ units, const int32_t* __restrict__ hdr, const SplitArgs spa) {
@@ -2906,17 +2906,21 @@ static bool pick_simt(int D, Launch& L) {
 // D = 64 below 256 tiles of 32 rows (2 x 8 heads x 128: 6.4 us); at D = 128 below 64, since
 // long contexts split anyway and wide tiles then merge less (4 x 8 x 100 queries, 1000
 // context rows: 32 us against 38).
+// Tree calls have short drafts and the masks' registers: 16-row tiles from D = 128 on (8
+// sequences of 200-256 tokens, 12 heads, 500-1000 rows, D = 128: 131 us, 148 with 32; 4 of 60-64, 16
+// heads, D = 256: 68 and 77).
 template <bool TREE>
 static bool pick_f32(const fmlm_attn_params& p, Launch& L) {
   if ((p.flags & FMLM_FLAG_CAUSAL_SEQ) && p.cu_seqlens_q && p.kv_layout != FMLM_LAYOUT_PACKED) return false;
   const int64_t rows = p.cu_seqlens_q ? p.total_q : (int64_t)p.B * p.N;
   const bool small = p.H * rows < (p.D == 64 ? 256 : 64) * 32;
+  constexpr int wide = TREE ? 1 : 2;  // tree calls have no 32-row tiles from D = 128 on
   switch (p.D) {
     case 16: L = f32_launch<16, 4, TREE>(); return true;
     case 32: L = f32_launch<32, 2, TREE>(); return true;
     case 64: L = small ? f32_launch<64, 1, TREE>() : f32_launch<64, 2, TREE>(); return true;
-    case 128: L = small ? f32_launch<128, 1, TREE>() : f32_launch<128, 2, TREE>(); return true;
-    case 256: L = small ? f32_launch<256, 1, TREE>() : f32_launch<256, 2, TREE>(); return true;
+    case 128: L = small || TREE ? f32_launch<128, 1, TREE>() : f32_launch<128, wide, TREE>(); return true;
+    case 256: L = small || TREE ? f32_launch<256, 1, TREE>() : f32_launch<256, wide, TREE>(); return true;
     default: return false;
   }
 }
