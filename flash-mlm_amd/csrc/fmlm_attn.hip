@@ -2792,6 +2792,10 @@ static Launch mla_rows_launch(const fmlm_attn_params& p) {
 // on average) and 128-row tiles are at least 48: 8 heads, 4000 rows, 8 sequences of 64-128 tokens 69.3 us
 // against 76.0, of 120-256 93.6 against 110.3, 24 of 60-80 over 3000 rows 121.5 against 154.8; but
 // 8 of 100-128 over 300 rows 29.5 against 25.4, one of 256 over 4000 rows 43.8 against 38.8.
+// What a key tile takes in a call of few rows, where the latency of its loads counts and not D: the
+// split plan's ranges that are worth cutting follow from it (D = 32, 2 sequences of 9-10 tokens, 4
+// heads, 1830-2489 rows: 28.4 us with 0.47, unsplit; 14.9).
+constexpr float kTreeTileUs = 0.8f;
 template <typename T>
 static bool pick_tree(const fmlm_attn_params& p, Launch& L) {
   const bool paged = p.ctx_block_table != nullptr;
@@ -2801,15 +2805,17 @@ static bool pick_tree(const fmlm_attn_params& p, Launch& L) {
   const int k = p.tile_config > 0 ? p.tile_config : wide ? 2 : 1;
   if (k > (p.D == 256 ? 2 : 1)) return false;
   switch (p.D) {
-    case 16: L = mfma3_launch<T, 16, 1, 4, 64, 0, true>(paged); return true;
-    case 32: L = mfma3_launch<T, 32, 1, 4, 64, 0, true>(paged); return true;
-    case 64: L = mfma3_launch<T, 64, 1, 4, 64, 0, true>(paged); return true;
-    case 128: L = mfma3_launch<T, 128, 1, 4, 64, 0, true>(paged); return true;
+    case 16: L = mfma3_launch<T, 16, 1, 4, 64, 0, true>(paged); break;
+    case 32: L = mfma3_launch<T, 32, 1, 4, 64, 0, true>(paged); break;
+    case 64: L = mfma3_launch<T, 64, 1, 4, 64, 0, true>(paged); break;
+    case 128: L = mfma3_launch<T, 128, 1, 4, 64, 0, true>(paged); break;
     case 256:
       L = k == 2 ? mfma3_launch<T, 256, 1, 8, 64, 0, true>(paged) : mfma3_launch<T, 256, 1, 4, 64, 0, true>(paged);
-      return true;
+      break;
     default: return false;
   }
+  L.tile_us = std::max(L.tile_us, kTreeTileUs);
+  return true;
 }
 // MFMA kernels by head dim.  The pipelined kernel and the 512-wide latent kernel need
 // linear main-key addressing; causal_query_seq_attn over padded K/V (a per-row sequence

@@ -25,16 +25,19 @@ FMLM_DEV int64_t bt_index(const void* a, bool i64, int64_t i) {
 FMLM_DEV int pages_of(int n) { return (n + FMLM_PAGE_ROWS - 1) / FMLM_PAGE_ROWS; }
 
 // workspace: per request its old length (clamped), the place of its first new page in the
-// free list, the tokens it may store and, with keep, per token its rank among the kept
+// free list, the tokens it may store and, with keep, the kept tokens before each token (T + 1
+// entries): of the whole call (small calls), or of its request, the requests' own ends then
+// being in `kept`
 struct BtSpace {
-  int32_t *old, *base, *count, *rank;
+  int32_t *old, *base, *count, *kept, *rank;
 };
 __host__ __device__ inline BtSpace bt_space(const BtParams& p) {
   BtSpace s;
   s.old = (int32_t*)p.workspace;
   s.base = s.old + p.B;
   s.count = s.base + p.B;
-  s.rank = s.count + p.B;
+  s.kept = s.count + p.B;
+  s.rank = s.kept + p.B;
   return s;
 }
 
@@ -60,26 +63,55 @@ FMLM_DEV int2 block_scan(int2 v, int2* s) {
   return v;
 }
 
-// ranks of the kept tokens of sequence b, and their number, by one wave: 64 tokens a step
-FMLM_DEV void bt_rank(const BtParams& p, const BtSpace& w, int b) {
-  const int lane = threadIdx.x & 63;
-  const int c0 = p.cu_seqlens[b], c1 = min(p.cu_seqlens[b + 1], p.T);
-  int n = 0;
-  for (int t = c0; t < c1; t += 64) {
-    const bool k = t + lane < c1 && p.keep[t + lane];
-    const uint64_t m = __builtin_amdgcn_ballot_w64(k);
-    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
-    if (t + lane < c1) w.rank[t + lane] = k ? n + before : -1;
-    n += __popcll(m);
+// Kept tokens of [t0, t1) before each of them, into rank[t0 .. t1); returns their number.  By a
+// workgroup of NT threads, 16 tokens a thread: up to 16 NT tokens take one round.
+template <int NT>
+FMLM_DEV int bt_rank(const BtParams& p, int t0, int t1, int32_t* rank, int2* part, int* last) {
+  constexpr int PER = 16;
+  int before = 0;
+  for (int base = t0; base < t1; base += PER * NT) {
+    const int first = base + PER * threadIdx.x;
+    uint32_t bits = 0;
+    const bool wide = first + PER <= t1;
+    if (wide && ((uintptr_t)(p.keep + first) & 15) == 0) {
+      const u32x4 x = *(const u32x4*)(p.keep + first);
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (x[i / 4] >> (8 * (i % 4)) & 0xffu) bits |= 1u << i;
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (first + i < t1 && p.keep[first + i]) bits |= 1u << i;
+    }
+    const int n = __popc(bits);
+    const int2 v = block_scan<NT>(make_int2(n, 0), part);
+    const int r0 = before + v.x - n;
+    if (wide && ((uintptr_t)(rank + first) & 15) == 0) {
+#pragma unroll
+      for (int i = 0; i < PER; i += 4) {
+        u32x4 x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = (uint32_t)(r0 + __popc(bits & ((1u << (i + j)) - 1u)));
+        *(u32x4*)(rank + first + i) = x;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (first + i < t1) rank[first + i] = r0 + __popc(bits & ((1u << i) - 1u));
+    }
+    if (threadIdx.x == NT - 1) *last = v.x;
+    __syncthreads();
+    before += *last;
+    __syncthreads();
   }
-  if (lane == 0) w.count[b] = n;
+  return before;
 }
 
 // The requests' prefix sums, by one workgroup of kBtThreads threads.  Each round scans the
 // pages that kBtThreads requests lack beside their old lengths, then the rows they end up
-// with (the free list may have cut them).
-FMLM_DEV void bt_scan(const BtParams& p, const BtSpace& w) {
-  __shared__ int2 part[kBtThreads / 64];
+// with (the free list may have cut them).  SMALL: ranks are the whole call's.
+template <bool SMALL>
+FMLM_DEV void bt_scan(const BtParams& p, const BtSpace& w, int2* part) {
   __shared__ int2 total;
   __shared__ int bad;
   if (threadIdx.x == 0) bad = 0;
@@ -95,7 +127,7 @@ FMLM_DEV void bt_scan(const BtParams& p, const BtSpace& w) {
       const int64_t raw = bt_index(p.old_lens, p.flags & FMLM_BT_OLD_I64, b);
       const int c0 = p.cu_seqlens[b], c1 = min(p.cu_seqlens[b + 1], p.T);
       old = (int)(raw < 0 ? 0 : raw > cap_in ? cap_in : raw);
-      cnt = p.keep ? w.count[b] : max(c1 - c0, 0);
+      cnt = !p.keep ? max(c1 - c0, 0) : SMALL ? w.rank[max(c0, c1)] - w.rank[c0] : w.kept[b];
       over = raw != old || cnt > cap_out - old;
       cnt = min(cnt, cap_out - old);
       have = pages_of(old);
@@ -141,60 +173,130 @@ FMLM_DEV void bt_scan(const BtParams& p, const BtSpace& w) {
   }
 }
 
-// page i of request b, or -1
-FMLM_DEV int bt_page(const BtParams& p, const BtSpace& w, int b, int i) {
-  const int old = w.old[b], have = pages_of(old), all = pages_of(old + w.count[b]);
-  if (i < have) return (int)bt_index(p.table_in, p.flags & FMLM_BT_TABLE_I64, (int64_t)b * p.in_pages + i);
-  if (i >= all) return -1;
-  return (int)bt_index(p.free_pages, p.flags & FMLM_BT_FREE_I64, w.base[b] + i - have);
+// Table entries and tokens, kBtUnroll at a time per thread, `step` apart, so that the loads of a
+// stage overlap: an entry waits for its request's sums and then for its page, a token for its
+// index before that.
+constexpr int kBtUnroll = 4;
+struct BtPlace {
+  int b, i;  // page i of request b
+};
+FMLM_DEV void bt_pages(const BtParams& p, const BtSpace& w, const BtPlace (&at)[kBtUnroll], const bool (&want)[kBtUnroll],
+                       int (&page)[kBtUnroll]) {
+  int old[kBtUnroll], count[kBtUnroll], base[kBtUnroll];
+#pragma unroll
+  for (int u = 0; u < kBtUnroll; ++u) {
+    old[u] = w.old[at[u].b];
+    count[u] = w.count[at[u].b];
+    base[u] = w.base[at[u].b];
+  }
+#pragma unroll
+  for (int u = 0; u < kBtUnroll; ++u) {
+    const int have = pages_of(old[u]), all = pages_of(old[u] + count[u]), i = at[u].i;
+    page[u] = -1;
+    if (want[u] && i < have)
+      page[u] = (int)bt_index(p.table_in, p.flags & FMLM_BT_TABLE_I64, (int64_t)at[u].b * p.in_pages + i);
+    else if (want[u] && i < all)
+      page[u] = (int)bt_index(p.free_pages, p.flags & FMLM_BT_FREE_I64, base[u] + i - have);
+  }
 }
 
-// table entries and tokens from `first` on, every `step`-th
+template <bool SMALL>
 FMLM_DEV void bt_fill(const BtParams& p, const BtSpace& w, int64_t first, int64_t step) {
   const int64_t entries = (int64_t)p.B * p.max_pages;
-  for (int64_t e = first; e < entries; e += step) {
-    // (64-bit divisions take some hundred instructions)
-    const int b = entries <= 0x7fffffff ? (int)((uint32_t)e / (uint32_t)p.max_pages) : (int)(e / p.max_pages);
-    p.block_table[e] = bt_page(p, w, b, (int)(e - (int64_t)b * p.max_pages));
-  }
-  for (int64_t t = first; t < p.T; t += step) {
-    const uint32_t at = (uint32_t)p.token_indices[t];
-    const int b = min((int)(at / (uint32_t)p.N), p.B - 1), pos = (int)(at - (uint32_t)b * (uint32_t)p.N);
-    const int old = w.old[b], rank = p.keep ? w.rank[t] : pos;
-    int64_t slot = -1;
-    if (rank >= 0 && rank < w.count[b]) {
-      const int a = old + rank, page = bt_page(p, w, b, a / FMLM_PAGE_ROWS);
-      if (page >= 0) slot = (int64_t)page * FMLM_PAGE_ROWS + a % FMLM_PAGE_ROWS;
+  for (int64_t e0 = first; e0 < entries; e0 += kBtUnroll * step) {
+    BtPlace at[kBtUnroll];
+    bool want[kBtUnroll];
+    int page[kBtUnroll];
+#pragma unroll
+    for (int u = 0; u < kBtUnroll; ++u) {
+      const int64_t e = e0 + u * step;
+      want[u] = e < entries;
+      const int64_t x = want[u] ? e : 0;
+      // (64-bit divisions take some hundred instructions)
+      at[u].b = entries <= 0x7fffffff ? (int)((uint32_t)x / (uint32_t)p.max_pages) : (int)(x / p.max_pages);
+      at[u].i = (int)(x - (int64_t)at[u].b * p.max_pages);
     }
-    p.slot_mapping[t] = slot;
-    p.positions[t] = old + pos;
+    bt_pages(p, w, at, want, page);
+#pragma unroll
+    for (int u = 0; u < kBtUnroll; ++u)
+      if (want[u]) p.block_table[e0 + u * step] = page[u];
+  }
+  for (int64_t t0 = first; t0 < p.T; t0 += kBtUnroll * step) {
+    uint32_t tok[kBtUnroll];
+    int rank[kBtUnroll], old[kBtUnroll], count[kBtUnroll], pos[kBtUnroll], page[kBtUnroll];
+    bool real[kBtUnroll], kept[kBtUnroll];
+    BtPlace at[kBtUnroll];
+#pragma unroll
+    for (int u = 0; u < kBtUnroll; ++u) {
+      const int64_t t = t0 + u * step;
+      real[u] = t < p.T;
+      tok[u] = (uint32_t)p.token_indices[real[u] ? t : 0];
+      kept[u] = real[u] && (!p.keep || p.keep[t]);
+      rank[u] = p.keep && real[u] ? w.rank[t] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < kBtUnroll; ++u) {
+      at[u].b = min((int)(tok[u] / (uint32_t)p.N), p.B - 1);
+      pos[u] = (int)(tok[u] - (uint32_t)at[u].b * (uint32_t)p.N);
+      if (!p.keep) rank[u] = pos[u];
+      else if (SMALL && kept[u]) rank[u] -= w.rank[t0 + u * step - pos[u]];
+      old[u] = w.old[at[u].b];
+      count[u] = w.count[at[u].b];
+    }
+#pragma unroll
+    for (int u = 0; u < kBtUnroll; ++u) {
+      kept[u] = kept[u] && rank[u] < count[u];
+      at[u].i = (old[u] + rank[u]) / FMLM_PAGE_ROWS;
+    }
+    bt_pages(p, w, at, kept, page);
+#pragma unroll
+    for (int u = 0; u < kBtUnroll; ++u) {
+      if (!real[u]) continue;
+      const int64_t t = t0 + u * step;
+      p.slot_mapping[t] =
+          page[u] >= 0 ? (int64_t)page[u] * FMLM_PAGE_ROWS + (old[u] + rank[u]) % FMLM_PAGE_ROWS : (int64_t)-1;
+      p.positions[t] = old[u] + pos[u];
+    }
   }
 }
 
 // all of it in one workgroup
 __global__ __launch_bounds__(kBtThreads) void block_table_small_kernel(const BtParams p) {
+  __shared__ int2 part[kBtThreads / 64];
+  __shared__ int last;
   const BtSpace w = bt_space(p);
   if (p.keep) {
-    for (int b = threadIdx.x >> 6; b < p.B; b += kBtThreads / 64) bt_rank(p, w, b);
+    const int all = bt_rank<kBtThreads>(p, 0, p.T, w.rank, part, &last);
+    if (threadIdx.x == 0) w.rank[p.T] = all;
     __syncthreads();
   }
-  bt_scan(p, w);
+  bt_scan<true>(p, w, part);
   __syncthreads();
-  bt_fill(p, w, threadIdx.x, kBtThreads);
+  bt_fill<true>(p, w, threadIdx.x, kBtThreads);
 }
 
+// one workgroup per request
 __global__ __launch_bounds__(kBtFillThreads) void block_table_rank_kernel(const BtParams p) {
-  const int b = blockIdx.x * (kBtFillThreads / 64) + (threadIdx.x >> 6);
-  if (b < p.B) bt_rank(p, bt_space(p), b);
+  __shared__ int2 part[kBtFillThreads / 64];
+  __shared__ int last;
+  const BtSpace w = bt_space(p);
+  const int b = blockIdx.x, c0 = p.cu_seqlens[b], c1 = min(p.cu_seqlens[b + 1], p.T);
+  const int n = bt_rank<kBtFillThreads>(p, c0, c1, w.rank, part, &last);
+  if (threadIdx.x == 0) w.kept[b] = n;
 }
-__global__ __launch_bounds__(kBtThreads) void block_table_scan_kernel(const BtParams p) { bt_scan(p, bt_space(p)); }
+__global__ __launch_bounds__(kBtThreads) void block_table_scan_kernel(const BtParams p) {
+  __shared__ int2 part[kBtThreads / 64];
+  bt_scan<false>(p, bt_space(p), part);
+}
 __global__ __launch_bounds__(kBtFillThreads) void block_table_fill_kernel(const BtParams p) {
-  bt_fill(p, bt_space(p), (int64_t)blockIdx.x * kBtFillThreads + threadIdx.x, (int64_t)gridDim.x * kBtFillThreads);
+  bt_fill<false>(p, bt_space(p), (int64_t)blockIdx.x * kBtFillThreads + threadIdx.x, (int64_t)gridDim.x * kBtFillThreads);
 }
 
-// One workgroup up to this many table entries and tokens: beyond it the launches of the
-// three kernels cost less than what one workgroup takes for the fill.
-constexpr int64_t kBtSmall = 16384;
+// One workgroup up to this many table entries, tokens and requests: beyond it the launches of the
+// other kernels cost less than what one workgroup takes.  64 requests: 64 tokens each 8.5 us against
+// 9.1 (with keep 11.5 against 12.4), 128 each 10.8 against 8.9 (14.8 against 12.7); one token each,
+// tables of 94 pages, 64 requests 8.5 against 8.2, 256 15.1 against 8.3.
+constexpr int64_t kBtSmall = 6144;
 
 static int bt_check(const BtParams& p) {
   if (p.B < 0 || p.N < 0 || p.T < 0 || p.max_pages < 0 || p.in_pages < 0 || p.n_free < 0) return FMLM_E_ARG;
@@ -255,7 +357,7 @@ extern "C" int64_t fmlm_block_table_workspace_bytes(const fmlm_block_table_param
   if (!pp) return FMLM_E_ARG;
   const int rc = bt_check(*pp);
   if (rc) return rc;
-  return 4 * (3 * (int64_t)pp->B + (pp->keep ? pp->T : 0));
+  return 4 * (4 * (int64_t)pp->B + (pp->keep ? (int64_t)pp->T + 1 : 0));
 }
 
 extern "C" int fmlm_block_table(const fmlm_block_table_params* pp, void* stream) {
@@ -269,13 +371,13 @@ extern "C" int fmlm_block_table(const fmlm_block_table_params* pp, void* stream)
   if (((int64_t)p.B * p.max_pages > 0 && !p.block_table) || (p.n_free > 0 && !p.free_pages)) return FMLM_E_ARG;
   if (need > 0 && (!p.workspace || p.workspace_bytes < need)) return FMLM_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  const int64_t work = std::max<int64_t>((int64_t)p.B * p.max_pages, p.T);
-  if (work + p.B <= kBtSmall) {
+  const int64_t entries = (int64_t)p.B * p.max_pages, work = std::max<int64_t>(entries, p.T);
+  if (entries + p.T + p.B <= kBtSmall) {
     hipLaunchKernelGGL(block_table_small_kernel, dim3(1), dim3(kBtThreads), 0, s, p);
     return launch_status();
   }
   if (p.keep) {
-    hipLaunchKernelGGL(block_table_rank_kernel, dim3((p.B + 3) / 4), dim3(kBtFillThreads), 0, s, p);
+    hipLaunchKernelGGL(block_table_rank_kernel, dim3(p.B), dim3(kBtFillThreads), 0, s, p);
   }
   hipLaunchKernelGGL(block_table_scan_kernel, dim3(1), dim3(kBtThreads), 0, s, p);
   const unsigned blocks = (unsigned)std::min<int64_t>((work + kBtFillThreads - 1) / kBtFillThreads, 4096);

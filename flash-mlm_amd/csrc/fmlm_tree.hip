@@ -117,22 +117,26 @@ FMLM_DEV TreeJoin tree_join(bool has_ctx, float lc, float m, float l) {
 }
 
 // ---------------------------------------------------------------------------
-// bf16 / fp16, the 512-wide latent (K = V = one row for all heads).  A workgroup of 4 waves takes 16
-// rows of one head.  As in the forward kernels S^T = K Q^T and O^T = V^T P^T, so that a lane
-// (q + 16 g) holds keys 4g .. 4g+3 of query q and then columns 16 db + 4g .. of its output.  Steps of
-// 32 keys pass through LDS once and serve both products: b128 reads make K's operand,
-// transposing reads V's.  Every wave computes all scores (32 MFMAs) and the output of its own 128
-// columns, which needs no exchange and leaves registers for the context's rows, loaded at the
-// start: what the kernel takes is the latency of its loads, and those of a step and of
-// the context's rows then overlap.  P is rounded to the input type for the product, and its row
-// sum is taken of the rounded values.
-// 16 sequences of up to 16 tokens, 64 heads: one wave a tile, keys and values read apart and the
-// context's rows at the end took 22.4 us.
+// bf16 / fp16, the 512-wide latent (K = V = one row for all heads).  A workgroup of 4 waves takes 16 of
+// a sequence's (head, position) rows: all heads have the same keys, and a tile of one head would be
+// mostly empty for a draft of a few tokens.  As in the forward kernels S^T = K Q^T and
+// O^T = V^T P^T, so that a lane (q + 16 g) holds keys 4g .. 4g+3 of query q and then columns
+// 16 db + 4g .. of its output.  Steps of 32 keys pass through LDS once and serve both products: b128
+// reads make K's operand, transposing reads V's.  Every wave computes all scores (32 MFMAs)
+// and the output of its own 128 columns, which needs no exchange.  What the kernel takes is the
+// latency of its loads: those of a step and of the context's rows are issued together at the start, and
+// the queries pass through LDS so that three workgroups fit a CU.  P is rounded to the input type
+// for the product, and its row sum is taken of the rounded values.
+// 16 sequences of up to 16 tokens, 64 heads: one wave a tile of one head, keys and values read apart
+// and the context's rows at the end took 22.4 us, four waves with all of it at the start 16.9, tiles over
+// heads with two workgroups a CU 17.5, with three 12.5.
+// Merging the parts of a split context here as well, instead of the 15 us of a launch of its own, took
+// 40: these workgroups are too few to read the parts' records.
 // ---------------------------------------------------------------------------
 constexpr int kLatentD = 512, kLatentWaves = 4;
 
 template <typename T>
-__global__ __launch_bounds__(kLatentWaves * 64) void attn_tree_latent_kernel(const fmlm_attn_params p,
+__global__ __launch_bounds__(kLatentWaves * 64, 3) void attn_tree_latent_kernel(const fmlm_attn_params p,
                                                                              const float* __restrict__ octx,
                                                                              const float* __restrict__ lse,
                                                                              const uint64_t* __restrict__ mask,
@@ -142,14 +146,17 @@ __global__ __launch_bounds__(kLatentWaves * 64) void attn_tree_latent_kernel(con
   constexpr int PITCH = D * 2 + 16;  // 16 bytes apart: a column's rows fall into different banks
   constexpr int NL = BK / NW;        // rows (1 KiB, one load) per wave and step
   __shared__ __align__(16) char tile[BK * PITCH];
+  __shared__ __align__(16) char qs[16 * PITCH];
   __shared__ uint32_t s_bad[NW];
-  const int b = blockIdx.z, h = blockIdx.y, r0 = blockIdx.x * 16;
-  const TreeSeq s = tree_seq(p, b, h);
-  if (r0 >= s.len) return;
+  const int b = blockIdx.y, r0 = blockIdx.x * 16;
+  const TreeSeq s = tree_seq(p, b, 0);
+  const int rows = p.H * s.len;
+  if (r0 >= rows) return;
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int pos = r0 + l16, at = min(pos, s.len - 1), c0 = wave * NDB * 16;
-  const bool ok = pos < s.len;
+  const int row = r0 + l16, c0 = wave * NDB * 16;
+  const bool ok = row < rows;
+  const int h = min(row, rows - 1) / s.len, pos = min(row, rows - 1) - h * s.len;
   const float c = p.scale * kLog2e;
   const T* const kp = (const T*)p.k + s.k0;
 
@@ -157,39 +164,40 @@ __global__ __launch_bounds__(kLatentWaves * 64) void attn_tree_latent_kernel(con
   auto load = [&](int j0) {  // this wave's rows of a step; rows past the sequence are zero
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-      const int row = j0 + wave * NL + n;
+      const int j = j0 + wave * NL + n;
       v[n] = u32x4{0u, 0u, 0u, 0u};
-      if (row < s.len) v[n] = *(const u32x4*)(kp + (int64_t)row * s.k_sn + lane * 8);
+      if (j < s.len) v[n] = *(const u32x4*)(kp + (int64_t)j * s.k_sn + lane * 8);
     }
   };
   load(0);
-  v8 qf[KC];
-  {
-    const T* q = (const T*)p.q + tree_row(p.q_layout, b, h, s.q0, at, p.q_sb, p.q_sh, p.q_sn);
+  // the queries (in registers they would cost a CU a workgroup)
 #pragma unroll
-    for (int kc = 0; kc < KC; ++kc) qf[kc] = *(const v8*)(q + kc * 32 + g * 8);
+  for (int n = 0; n < 16 / NW; ++n) {
+    const int i = wave * (16 / NW) + n, r = min(r0 + i, rows - 1), hq = r / s.len;
+    const T* q = (const T*)p.q + tree_row(p.q_layout, b, hq, s.q0, r - hq * s.len, p.q_sb, p.q_sh, p.q_sn);
+    *(u32x4*)(qs + i * PITCH + lane * 16) = *(const u32x4*)(q + lane * 8);
   }
   f32x4 oc[NDB];
   float lc = 0.f;
   if (s.has_ctx) {
-    const int64_t row = (int64_t)h * p.total_q + s.q0 + at;
-    lc = lse[row];
+    const int64_t at = (int64_t)h * p.total_q + s.q0 + pos;
+    lc = lse[at];
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) oc[db] = *(const f32x4*)(octx + row * D + c0 + db * 16 + 4 * g);
+    for (int db = 0; db < NDB; ++db) oc[db] = *(const f32x4*)(octx + at * D + c0 + db * 16 + 4 * g);
   }
   f32x4 o[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
 
-  const uint32_t kaddr = lds_addr(tile) + l16 * PITCH + 16 * g;
+  const uint32_t qaddr = lds_addr(qs) + l16 * PITCH + 16 * g, kaddr = lds_addr(tile) + l16 * PITCH + 16 * g;
   const uint32_t vaddr = lds_addr(tile) + (4 * g + (l16 >> 2)) * PITCH + 8 * (l16 & 3) + 2 * c0;
   for (int j0 = 0; j0 < s.len; j0 += BK) {
     uint32_t seen = 0;  // keys j0 + bit that the lane's row attends to
     if (ok && j0 / 64 < words) seen = (uint32_t)(mask[(int64_t)(s.q0 + pos) * words + j0 / 64] >> (j0 % 64));
     if (s.len - j0 < BK) seen &= (1u << (s.len - j0)) - 1u;
-    // (the same in every wave; a step up to the rows' own has keys they see)
-    if (j0 >= r0 + 16 && !__builtin_amdgcn_ballot_w64(seen != 0)) continue;
+    // (the same in every wave)
+    if (j0 > 0 && !__builtin_amdgcn_ballot_w64(seen != 0)) continue;
     if (j0 > 0) {
       load(j0);
       __syncthreads();  // the tile's last readers are done
@@ -211,12 +219,13 @@ __global__ __launch_bounds__(kLatentWaves * 64) void attn_tree_latent_kernel(con
     __syncthreads();
     // ---- scores
     f32x4 sc[2];
+    sc[0] = sc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int kc = 0; kc < KC; ++kc) {
+      const v8 q = *(const FMLM_LDS v8*)(uintptr_t)(qaddr + kc * 64);
 #pragma unroll
-      for (int kc = 0; kc < KC; ++kc)
-        sc[kb] = Mfma<T>::run(*(const FMLM_LDS v8*)(uintptr_t)(kaddr + kb * 16 * PITCH + kc * 64), qf[kc], sc[kb]);
+      for (int kb = 0; kb < 2; ++kb)
+        sc[kb] = Mfma<T>::run(*(const FMLM_LDS v8*)(uintptr_t)(kaddr + kb * 16 * PITCH + kc * 64), q, sc[kb]);
     }
     uint32_t bad = 0;
 #pragma unroll
@@ -376,7 +385,7 @@ int launch_tree_part(const fmlm_attn_params& ctx, const fmlm_attn_params& p, con
   const hipStream_t s = (hipStream_t)stream;
   const float* const octx = (const float*)ctx.o;
   if (p.dtype != FMLM_DTYPE_F32) {
-    const dim3 grid((unsigned)((longest + 15) / 16), (unsigned)p.H, (unsigned)p.B);
+    const dim3 grid((unsigned)(((int64_t)longest * p.H + 15) / 16), (unsigned)p.B);
     const dim3 block(kLatentWaves * 64);
     if (p.D != kLatentD || !(p.flags & FMLM_FLAG_MLA)) return FMLM_E_HEAD_DIM;
     if (p.dtype == FMLM_DTYPE_BF16)

@@ -113,9 +113,9 @@ def build_block_table(
     _lib.check(nbytes if nbytes < 0 else 0, "fmlm_block_table_workspace_bytes")
     slots = torch.empty(t, dtype=torch.int64, device=dev)
     # the 32-bit results share one allocation with the workspace
-    table, positions, new_lens, cu, summary, ws = torch.empty(
+    ws, table, positions, new_lens, cu, summary = torch.empty(
         b * max_pages + t + 2 * b + 5 + nbytes // 4, dtype=torch.int32, device=dev
-    ).split_with_sizes((b * max_pages, t, b, b + 1, 4, nbytes // 4))
+    ).split_with_sizes((nbytes // 4, b * max_pages, t, b, b + 1, 4))
     table = table.view(b, max_pages)
     p.old_lens, p.cu_seqlens, p.token_indices = context_lens.data_ptr(), q_meta.cu_seqlens.data_ptr(), \
         q_meta.token_indices.data_ptr()

@@ -85,9 +85,9 @@ def test_abi_refuses():
     p.B, p.N, p.T = 2, 3, 7
     assert lib.fmlm_block_table_workspace_bytes(p) == -1  # more tokens than the batch holds
     p.T = 5
-    assert lib.fmlm_block_table_workspace_bytes(p) == 4 * 6
+    assert lib.fmlm_block_table_workspace_bytes(p) == 4 * 8
     p.keep = 256
-    assert lib.fmlm_block_table_workspace_bytes(p) == 4 * (6 + 5)
+    assert lib.fmlm_block_table_workspace_bytes(p) == 4 * (8 + 6)
     p.max_pages = 1 << 26
     assert lib.fmlm_block_table_workspace_bytes(p) == -1  # lengths past 32 bits
     p.max_pages = 4
@@ -160,7 +160,7 @@ def _expect(case, plan):
 @pytest.mark.parametrize("keep", [False, True])
 @pytest.mark.parametrize("B, N, ctx, lo", [
     (1, 1, 0, 1), (1, 1, 64, 1), (1, 200, 300, 200), (7, 5, 200, 0), (64, 1, 6000, 1), (64, 1, 1000, 0),
-    (33, 130, 64, 0), (1500, 2, 130, 0), (300, 40, 5000, 0), (5, 5000, 700, 0),
+    (33, 130, 64, 0), (1500, 2, 130, 0), (2, 9000, 64, 0), (90, 700, 300, 0), (300, 40, 5000, 0), (5, 5000, 700, 0),
 ])
 def test_table(B, N, ctx, lo, keep, device):
     """one workgroup (small) and three kernels (the last lines), with and without `keep`"""

@@ -263,6 +263,16 @@ def test_mla(dtype, kind, device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["packed", "paged"])
+@pytest.mark.parametrize("lens, H, ctx", [([5, 33, 1, 0, 2], 16, [4000, 65, 900, 70, 0]), ([1], 32, [3800]),
+                                          ([9, 12], 64, [600, 2000])])
+def test_mla_split_contexts(kind, lens, H, ctx, device):
+    """Long latent contexts of few rows are split; the tree's kernel merges the parts, beside
+    sequences that are not split or have no context."""
+    _run(device, torch.bfloat16, lens=lens, N=max(lens), H=H, D=512, ctx=ctx, kind=kind, mla=True, seed=5)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype, kind", [("bf16", "shared"), ("fp16", "index"), ("fp32", "shared"), ("bf16", "index")])
 def test_shared_and_indexed_contexts(dtype, kind, device):
     _run(device, DT[dtype], lens=[9, 20, 3], N=20, H=2, D=64, ctx=[200, 77, 1], kind=kind, seed=4)
