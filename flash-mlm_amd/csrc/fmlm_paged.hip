@@ -8,7 +8,11 @@
 // few bytes per token and table entry: what it costs is the launches and the latency of
 // its dependent loads.
 //
-// Append.  A copy of rows; the slot of a token is read once and used for several heads.
+// 64 requests of one token, tables of 94 pages: 7.5 us in one workgroup; 512 requests of up to 32
+// tokens with a keep mask, tables of 129 pages: 5.0 + 3.6 + 5.4 us.
+//
+// Append.  A copy of rows; the slot of a token is read once and used for several heads.  32 sequences
+// of 256-1024 tokens, 16 heads of k and v, D = 128: 355 MB in 71 us, 5.0 TB/s (a large copy: 5.16).
 #include "fmlm_common.h"
 
 #include <algorithm>
