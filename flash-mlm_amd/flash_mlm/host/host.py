@@ -91,8 +91,6 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def rows16(t: torch.Tensor) -> torch.Tensor:
     """Rows that a kernel can address: ``t``, or an aligned copy (also of a contiguous ``t``
     that starts at an odd address)."""
-    if t.is_contiguous() and (t.shape[-1] * t.element_size()) % 16 == 0 and t.data_ptr() % 16 == 0:
-        return t
     return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
 
 

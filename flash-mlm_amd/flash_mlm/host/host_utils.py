@@ -41,6 +41,21 @@ def _device_scope(device: torch.device):
     return torch.cuda.device(device)
 
 
+def pack_indices(q_meta: PackMetadata, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    """(cu_seqlens int32, token_indices int64) of ``q_meta`` as the kernels read them, checked
+    against its counts (also of metadata that was not made by build_pack_metadata)."""
+    cu, tokens = q_meta.cu_seqlens, q_meta.token_indices
+    if cu.device != device or tokens.device != device:
+        raise ValueError("q_meta must be on the device of the call's tensors")
+    if cu.dtype != torch.int32 or not cu.is_contiguous():
+        cu = cu.to(torch.int32).contiguous()
+    if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+        tokens = tokens.to(torch.int64).contiguous()
+    if cu.numel() != q_meta.B + 1 or tokens.numel() != q_meta.total_tokens:
+        raise ValueError("q_meta: cu_seqlens or token_indices do not match its B and total_tokens")
+    return cu, tokens
+
+
 class _NullScope:
     def __enter__(self):
         return self

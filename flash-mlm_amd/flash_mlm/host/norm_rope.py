@@ -15,7 +15,7 @@ import torch
 from flash_mlm import _lib
 from flash_mlm.host.cache import PackMetadata
 from flash_mlm.host.host import rows16
-from flash_mlm.host.host_utils import require_cuda_tensors, validate_head_dim_supported
+from flash_mlm.host.host_utils import pack_indices, require_cuda_tensors, validate_head_dim_supported
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _INTS = (torch.int32, torch.int64)
@@ -76,7 +76,7 @@ def _backward(call: _Call, xs, ws, dys, needs):
         if dys[i] is None or not (needs[i] or needs[2 + i]):
             t.heads = 0
             continue
-        dy = rows16(dys[i])
+        dy = aligned16(dys[i]) if call.packed else rows16(dys[i])
         dx = dxs[i] = _out(xs[i])
         call.put(t, xs[i], dx)
         t.dy = dy.data_ptr()
@@ -196,9 +196,10 @@ def qk_norm_rope(
     not read back, and the kernel clamps them to the tables.
 
     With ``q_meta``, rows of padding tokens come out as zeros, whatever they held.
-    Differentiable in q, k and the gains; gradients of padding rows are zero.  A call captured
-    into a graph together with its backward raises ValueError while outputs of earlier calls
-    on the same leaves are alive (autograd would run part of the backward on their stream).
+    Differentiable in q, k and the gains; gradients of padding rows are zero.  A call that is
+    captured into a graph and takes leaves that require grad raises ValueError while
+    outputs of earlier calls on them are alive (autograd would run part of a captured backward
+    on their stream); capture a forward alone under ``torch.no_grad()``.
     """
     qs, ks, dtype, dev = q.shape, k.shape, q.dtype, q.device
     rank = len(qs)
@@ -215,12 +216,12 @@ def qk_norm_rope(
         raise ValueError("q and k must be on one device")
     if not q.is_cuda:
         require_cuda_tensors(q)
-    if q_meta is not None and q_meta.cu_seqlens.device != dev:
-        raise ValueError("q_meta must be on the device of q and k")
+    cu = tokens = None
+    if q_meta is not None:
+        cu, tokens = pack_indices(q_meta, dev)
 
     call = _Call()
     p = call.block = _lib.NormRopeParams()
-    cu = tokens = None
     packed = call.packed = rank == 2
     if not packed:
         b, hq, n, _ = qs
@@ -230,7 +231,7 @@ def qk_norm_rope(
         if q_meta is not None:
             if q_meta.B != b or q_meta.N != n:
                 raise ValueError("q_meta shape metadata does not match q/k padded shape")
-            cu = q_meta.cu_seqlens
+            tokens = None
         if num_heads is not None and num_heads != hq:
             raise ValueError("q head dimension must match num_heads")
         rows = b * n
@@ -239,7 +240,6 @@ def qk_norm_rope(
     else:
         if q_meta is not None:
             b, n, rows = q_meta.B, q_meta.N, q_meta.total_tokens
-            cu, tokens = q_meta.cu_seqlens, q_meta.token_indices
         else:
             if num_heads is None or num_heads < 1 or qs[0] % num_heads:
                 raise ValueError("packed q needs q_meta, or num_heads that divides its rows")
@@ -317,7 +317,7 @@ def qk_norm_rope(
     elif positions is not None or context_lens is not None:
         raise ValueError("positions and context_lens need cos and sin")
     p.flags = flags
-    q_, k_ = rows16(q), rows16(k)
+    q_, k_ = (aligned16(q), aligned16(k)) if packed else (rows16(q), rows16(k))
     grad = torch.is_grad_enabled()
     if grad and cos is not None and (cos.requires_grad or sin.requires_grad):
         raise ValueError("cos and sin are constants: qk_norm_rope has no gradient of them")

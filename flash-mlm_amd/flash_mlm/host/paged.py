@@ -10,7 +10,7 @@ import torch
 
 from flash_mlm import _lib
 from flash_mlm.host.cache import PAGE_ROWS, PackMetadata
-from flash_mlm.host.host_utils import _device_scope, _require_device
+from flash_mlm.host.host_utils import _device_scope, _require_device, pack_indices
 
 _INTS = (torch.int32, torch.int64)
 
@@ -117,8 +117,8 @@ def build_block_table(
         b * max_pages + t + 2 * b + 5 + nbytes // 4, dtype=torch.int32, device=dev
     ).split_with_sizes((nbytes // 4, b * max_pages, t, b, b + 1, 4))
     table = table.view(b, max_pages)
-    p.old_lens, p.cu_seqlens, p.token_indices = context_lens.data_ptr(), q_meta.cu_seqlens.data_ptr(), \
-        q_meta.token_indices.data_ptr()
+    cu_q, tokens = pack_indices(q_meta, dev)
+    p.old_lens, p.cu_seqlens, p.token_indices = context_lens.data_ptr(), cu_q.data_ptr(), tokens.data_ptr()
     p.table_in, p.free_pages = _lib.ptr(block_table), free_pages.data_ptr()
     p.block_table, p.slot_mapping, p.positions = table.data_ptr(), slots.data_ptr(), positions.data_ptr()
     p.new_lens, p.cu_kv, p.summary = new_lens.data_ptr(), cu.data_ptr(), summary.data_ptr()
@@ -157,10 +157,11 @@ def paged_append(pairs, *, heads: int, d: int, q_meta: PackMetadata, slots: torc
         else:
             a.s_sb, a.s_sh, a.s_sn, _ = src.stride()
     dev = slots.device
+    tokens = pack_indices(q_meta, dev)[1]
     with _device_scope(dev):
         rc = _lib.load().fmlm_paged_append(
             arr, len(pairs), pairs[0][0].element_size(), heads, d, t, int(q_meta.N),
-            _lib.LAYOUT_PACKED if packed else _lib.LAYOUT_PADDED, q_meta.token_indices.data_ptr(), slots.data_ptr(),
+            _lib.LAYOUT_PACKED if packed else _lib.LAYOUT_PADDED, tokens.data_ptr(), slots.data_ptr(),
             pool_rows, _lib.stream_of(dev),
         )
     _lib.check(rc, "fmlm_paged_append")

@@ -34,6 +34,7 @@ from flash_mlm.host.host_utils import (
     _maybe_get_cache_context,
     _require_device,
     make_contiguous,
+    pack_indices,
     require_cuda_tensors,
     validate_cache_request,
     validate_cu_seqlens_rank1_min2,
@@ -91,13 +92,14 @@ def build_tree_metadata(
         raise ValueError("parents and context_lens must be on the device of q_meta")
     parents = parents.contiguous()
     context_lens = None if context_lens is None else context_lens.contiguous()
+    cu = pack_indices(q_meta, dev)[0]
     words = max(1, -(-n // 64))
     mask = torch.empty((t, words), dtype=torch.int64, device=dev)
     positions = torch.empty(t, dtype=torch.int32, device=dev)
     bad = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
     with _device_scope(dev):
         rc = _lib.load().fmlm_tree_mask(
-            parents.data_ptr(), int(parents.dtype == torch.int64), q_meta.cu_seqlens.data_ptr(), b, n, t, words,
+            parents.data_ptr(), int(parents.dtype == torch.int64), cu.data_ptr(), b, n, t, words,
             _lib.ptr(context_lens), int(context_lens is not None and context_lens.dtype == torch.int64),
             mask.data_ptr(), positions.data_ptr(), _lib.ptr(bad), _lib.stream_of(dev),
         )
@@ -212,10 +214,13 @@ def flash_attn_mlm_tree(
         return out
     q_, k_, v_ = rows16(q), rows16(k), rows16(v)
     k_cache, v_cache = make_contiguous(ctx.k_cache, ctx.v_cache)
-    cu_q = q_meta.cu_seqlens.to(torch.int32).contiguous()
+    cu_q = pack_indices(q_meta, q.device)[0]
     cu_kv = ctx.cu_seqlens_kv.to(torch.int32).contiguous()
     k_strides = (k_.stride(0), 0 if is_mla else k_.stride(1), k_.stride(2))
     v_strides = k_strides if is_mla else (v_.stride(0), v_.stride(1), v_.stride(2))
+    # a schedule or parameter block made during a capture lives in the graph's memory and is filled
+    # by its replays: it stays this call's own
+    capturing = torch.cuda.is_current_stream_capturing()
     plan = _prepare(
         q=q_,
         out=out,
@@ -244,13 +249,13 @@ def flash_attn_mlm_tree(
         scale=scale,
         flags=_lib.FLAG_TREE | (_lib.FLAG_MLA if is_mla else 0),
         inference_cache=inference_cache,
-        schedule_cache=q_meta.kernel_schedules,
+        schedule_cache=dict(q_meta.kernel_schedules) if capturing else q_meta.kernel_schedules,
         ctx_index=ctx_index,
         block_table=ctx.block_table,
         page_stride=_page_stride(ctx, num_heads, d, is_mla),
     )
     TreeLaunch.of(plan, mask.contiguous())()
-    if (key is not None and q_ is q and k_ is k and v_ is v and k_cache is ctx.k_cache and v_cache is ctx.v_cache
+    if (key is not None and not capturing and q_ is q and k_ is k and v_ is v and k_cache is ctx.k_cache and v_cache is ctx.v_cache
             and plan.keep[10] is None and mask.is_contiguous()):
         extra = (cu_q, cu_kv, k_cache if entry is None else None, v_cache if entry is None else None)
         _memo_store(memo, key, _Memo(plan, entry, extra, tuple(out.shape)))

@@ -297,6 +297,50 @@ def test_strides_padding_and_alignment(device):
 
 
 @pytest.mark.gpu
+def test_packed_rows_of_other_strides_and_metadata(device):
+    """Packed rows and gradients that are columns of a wider tensor; metadata of other integer
+    types; metadata whose tables do not fit its counts"""
+    import dataclasses
+
+    lens, D = [5, 9], 64
+    meta = build_pack_metadata(torch.tensor(lens, device=device), 9, 32)
+    wide = torch.randn((2 * 14, 3 * D), device=device).half()
+    q, k = wide[:, :D], wide[:, D : 2 * D]
+    cos, sin = _tables(9, D, device)
+    ql = q.contiguous().requires_grad_()
+    want = qk_norm_rope(ql, k.contiguous(), cos=cos, sin=sin, q_meta=meta)
+    dy = torch.randn((2 * 14, 2 * D), device=device).half()[:, D:]
+    gw = torch.autograd.grad(want[0], ql, dy.contiguous(), retain_graph=True)[0]
+    got = qk_norm_rope(q, k, cos=cos, sin=sin, q_meta=meta)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(torch.autograd.grad(want[0], ql, dy)[0], gw)
+    other = dataclasses.replace(meta, cu_seqlens=meta.cu_seqlens.long(), token_indices=meta.token_indices.int())
+    assert torch.equal(qk_norm_rope(q, k, cos=cos, sin=sin, q_meta=other)[0], want[0])
+    for bad in (dict(token_indices=meta.token_indices[:-1]), dict(cu_seqlens=meta.cu_seqlens[:-1])):
+        with pytest.raises(ValueError, match="do not match"):
+            qk_norm_rope(q, k, q_meta=dataclasses.replace(meta, **bad))
+    with pytest.raises(ValueError, match="device"):
+        qk_norm_rope(q, k, q_meta=dataclasses.replace(meta, cu_seqlens=meta.cu_seqlens.cpu()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wt", ["fp16", "fp32"])
+def test_gains_of_another_type(wt, device):
+    """bf16 rows with gains of their own type: rows and gradients as at 64 bits"""
+    q, k, dq, dk, kw, cos, sin, tokens, whole = _case(device, torch.bfloat16, H=3, Hk=2, D=64, lens=[7, 12], N=12, R=64,
+                                                      gain="shared", packed=False, inter=False, where="place")
+    w = kw["q_weight"] = kw["q_weight"].to(DT[wt]).requires_grad_()
+    kw["k_weight"] = kw["k_weight"].to(DT[wt])
+    out = qk_norm_rope(q, k, **kw)
+    want, mag = ref.norm_rope(tokens(q, 3), _f(w), cos, sin, eps=1e-5)
+    _close(_f(out[0]), whole(want, 3), whole(mag, 3), torch.bfloat16, 16)
+    g = torch.autograd.grad(out[0], w, dq)[0]
+    _, _, t, m = ref.norm_rope_grads(tokens(q, 3), _f(w), cos, sin, tokens(dq, 3), eps=1e-5)
+    assert g.dtype == DT[wt]
+    _close(_f(g), t.sum((0, 1)), m.sum((0, 1)), DT[wt], 40 + 57)
+
+
+@pytest.mark.gpu
 def test_positions_are_clamped_on_the_gpu_and_refused_on_the_cpu(device):
     q = torch.randn((1, 2, 4, 64), device=device)
     cos, sin = _tables(8, 64, device)

@@ -421,6 +421,35 @@ def test_repeated_calls_streams_and_graphs(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D, mla", [(64, False), (512, True)])
+def test_first_call_of_a_metadata_in_a_graph(D, mla, device):
+    """A capture leaves nothing behind on the metadata that only its replays fill: an eager call
+    before the first replay, and the replays, give what an eager call gives."""
+    H, N, lens = 4, 20, [20, 3]
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn((2, H, N, D), generator=g).bfloat16().to(device) for _ in range(3))
+    cache, _, _ = _context("paged", [1500, 70], H, D, mla, torch.bfloat16, device, 4)
+
+    def call(meta, tree):
+        return flash_attn_mlm_tree(q, k, v, H, meta, tree, 0.125, cache, 0, is_mla=mla)
+
+    metas = []
+    for _ in range(2):
+        meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+        metas.append((meta, build_tree_metadata(torch.tensor([-1] + [0] * 19 + [-1, 0, 1], device=device), meta)))
+    want = call(*metas[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(*metas[1])
+    assert torch.equal(call(*metas[1]), want)
+    for _ in range(3):
+        out.fill_(5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(call(*metas[1]), want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_speculative_decoding_over_a_paged_cache(dtype, device):
     """The operators as a server uses them: prompts are stored, then drafted trees attend to the
