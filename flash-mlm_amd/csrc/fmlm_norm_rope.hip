@@ -20,8 +20,8 @@
 //
 // Measured (a large copy reaches 5.16 TB/s).  Forward, 32 sequences of 256-1024 tokens, 16 heads of
 // q and k, D = 128, fp16, padding rows written as zeros: 457 MB in 90 us, 5.1 TB/s; packed rows
-// with gains per head, 359 MB in 67.  Backward of the latter, 539 MB in 123 + 5 us (4.4 TB/s; 117 with
-// shared gains, whose kernel has fewer registers).  64 decoding tokens: 4.4 us, latency.
+// with gains per head, 359 MB in 67.  Backward of the latter, 539 MB in 114 + 5 us (4.5 TB/s), and
+// 112 + 5 with shared gains.  64 decoding tokens: 4.4 us, latency.
 #include "fmlm_common.h"
 
 #include <algorithm>
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(kNrThreads) void norm_rope_kernel(const NrParams p,
 // workspace, or with PERHEAD (a tensor has gains per head) to head * gridDim.x + blockIdx.x
 // for each of its heads.
 template <typename T, int LPR, bool PERHEAD>
-__global__ __launch_bounds__(kNrThreads) void norm_rope_bwd_kernel(const NrParams p, float* part_q, float* part_k) {
+__global__ __launch_bounds__(kNrThreads, sizeof(T) == 2 ? 4 : 3) void norm_rope_bwd_kernel(const NrParams p, float* part_q, float* part_k) {
   constexpr int RPB = kNrThreads / LPR, D = 8 * LPR;
   constexpr int U = kNrHeads, NA = PERHEAD ? U : 1;
   __shared__ __align__(16) float red[kNrThreads / 64][D];
@@ -330,9 +330,18 @@ __global__ __launch_bounds__(kNrThreads) void norm_rope_bwd_kernel(const NrParam
   const NrTensor& t = *ck.t;
   float* const part = ck.tensor ? part_k : part_q;
   const bool norm = p.flags & FMLM_NR_NORM, inter = p.flags & FMLM_NR_INTERLEAVED;
-  float w[NA][8];
-#pragma unroll
-  for (int u = 0; u < NA; ++u) load_gain(p, t, min(ck.h0 + u, ck.h1 - 1), 8 * c, w[u]);
+  // gains per head in LDS: in 32 registers of a thread the kernel had 3 waves a SIMD and took 7 us more
+  __shared__ __align__(16) float gains[PERHEAD ? U * D : 1];
+  float w[8];
+  if constexpr (PERHEAD) {
+    for (int at = 8 * threadIdx.x; at < (ck.h1 - ck.h0) * D; at += 8 * kNrThreads) {
+      load_gain(p, t, ck.h0 + at / D, at % D, w);
+      oct_store(gains + at, w);
+    }
+    __syncthreads();
+  } else {
+    load_gain(p, t, 0, 8 * c, w);
+  }
   float dw[NA][8];
 #pragma unroll
   for (int u = 0; u < NA; ++u)
@@ -366,6 +375,7 @@ __global__ __launch_bounds__(kNrThreads) void norm_rope_bwd_kernel(const NrParam
       if (ck.h0 + u >= ck.h1) break;
       const int iu = PERHEAD ? u : 0;
       float g[8], gr[8], xv[8];
+      if constexpr (PERHEAD) oct_floats(oct_load(gains + u * D + 8 * c), w);
       oct_floats(dy[u], gr);
       if (p.rotary_dim > 0 && !inter) {
         float q[8];
@@ -382,7 +392,7 @@ __global__ __launch_bounds__(kNrThreads) void norm_rope_bwd_kernel(const NrParam
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           ss = fmaf(xv[j], xv[j], ss);
-          ux = fmaf(g[j] * w[iu][j], xv[j], ux);
+          ux = fmaf(g[j] * w[j], xv[j], ux);
         }
         ss = lane_sum<LPR>(ss);
         ux = lane_sum<LPR>(ux);
@@ -392,7 +402,7 @@ __global__ __launch_bounds__(kNrThreads) void norm_rope_bwd_kernel(const NrParam
         for (int j = 0; j < 8; ++j) {
           const float xh = xv[j] * rs;
           dw[iu][j] = fmaf(g[j], xh, dw[iu][j]);
-          g[j] = rs * fmaf(-xh, m, g[j] * w[iu][j]);
+          g[j] = rs * fmaf(-xh, m, g[j] * w[j]);
         }
       }
       oct_store(dst + (ck.h0 + u) * t.y_sh, g);
