@@ -41,8 +41,8 @@ class PagedMetadata:
 def _ints(t: torch.Tensor, what: str, ndim: int, device) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.ndim != ndim or t.dtype not in _INTS:
         raise ValueError(f"{what} must be a rank-{ndim} int32 or int64 tensor")
-    _require_device(t, what="build_block_table")
     if t.device != device:
+        _require_device(t, what="build_block_table")
         raise ValueError(f"{what} must be on the device of q_meta")
     return t.contiguous()
 
@@ -76,6 +76,7 @@ def build_block_table(
     """
     dev = q_meta.cu_seqlens.device
     b, t = int(q_meta.B), int(q_meta.total_tokens)
+    _require_device(q_meta.cu_seqlens, what="build_block_table")
     context_lens = _ints(context_lens, "context_lens", 1, dev)
     free_pages = _ints(free_pages, "free_pages", 1, dev)
     if int(context_lens.numel()) != b:

@@ -297,6 +297,37 @@ def test_strides_padding_and_alignment(device):
 
 
 @pytest.mark.gpu
+def test_repeated_calls(device):
+    """A call laid out like an earlier one takes its parameter block: with other tensors, after the
+    metadata's fields were replaced, in another mode"""
+    import dataclasses
+
+    cos, sin = _tables(30, 64, device)
+    meta = build_pack_metadata(torch.tensor([9, 4], device=device), 9, 32)
+
+    def fresh(q, k, **kw):  # the same call on metadata that has seen none
+        m = dataclasses.replace(meta, launch_memo={})
+        return qk_norm_rope(q, k, cos=cos, sin=sin, q_meta=m, **kw)
+
+    g = torch.Generator().manual_seed(0)
+    for i in range(4):
+        q, k = (torch.randn((2, 3, 9, 64), generator=g).to(device) for _ in range(2))
+        w = torch.rand(64, generator=g).to(device)
+        start = torch.randint(0, 20, (2,), generator=g).to(device)
+        pos = torch.randint(0, 30, (13,), generator=g).to(device)
+        for kw in (dict(), dict(q_weight=w), dict(q_weight=w, k_weight=w + 1, context_lens=start), dict(positions=pos),
+                   dict(positions=pos, interleaved=True), dict(context_lens=start.int(), eps=0.5)):
+            got, want = qk_norm_rope(q, k, cos=cos, sin=sin, q_meta=meta, **kw), fresh(q, k, **kw)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    other = build_pack_metadata(torch.tensor([2, 9], device=device), 9, 32)
+    meta.cu_seqlens, meta.token_indices, meta.total_tokens = other.cu_seqlens, other.token_indices, other.total_tokens
+    assert torch.equal(qk_norm_rope(q, k, cos=cos, sin=sin, q_meta=meta)[0],
+                       qk_norm_rope(q, k, cos=cos, sin=sin, q_meta=other)[0])
+    a = qk_norm_rope(q, k)
+    assert torch.equal(qk_norm_rope(k, q)[0], a[1]) and torch.equal(qk_norm_rope(q, k)[0], a[0])
+
+
+@pytest.mark.gpu
 def test_packed_rows_of_other_strides_and_metadata(device):
     """Packed rows and gradients that are columns of a wider tensor; metadata of other integer
     types; metadata whose tables do not fit its counts"""
@@ -369,6 +400,7 @@ def test_refusals(device):
         ("multiple of 16", dict(cos=cos[:, :4], sin=sin[:, :4])),
         ("multiple of 16", dict(cos=cos[:0], sin=sin[:0])),
         ("need cos", dict(context_lens=torch.zeros(2, dtype=torch.int32, device=device))),
+        ("shape", dict(cos=cos, sin=sin, positions=[0, 1])),
         ("exclusive", dict(cos=cos, sin=sin, context_lens=torch.zeros(2, dtype=torch.int32, device=device),
                            positions=torch.zeros((2, 5), dtype=torch.int32, device=device))),
         ("shape", dict(cos=cos, sin=sin, positions=torch.zeros(7, dtype=torch.int32, device=device))),

@@ -39,10 +39,6 @@ def test_table_refusals_on_the_cpu():
     i32 = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="no CPU compute path"):
         build_block_table(meta, i32, free_pages=i32)
-    with pytest.raises(ValueError, match="rank-1"):
-        build_block_table(meta, i32.float(), free_pages=i32)
-    with pytest.raises(ValueError, match="rank-1"):
-        build_block_table(meta, i32[None], free_pages=i32)
 
 
 def test_append_refusals_on_the_cpu():
@@ -218,6 +214,12 @@ def test_table_of_new_requests_and_checks(device):
             build_block_table(meta, z, free_pages=f, **kw)
     with pytest.raises(ValueError, match="one entry per sequence"):
         build_block_table(meta, z[:4], free_pages=f)
+    for bad in (z.float(), z[None], z.tolist()):
+        with pytest.raises(ValueError, match="rank-1"):
+            build_block_table(meta, bad, free_pages=f)
+    for kw in (dict(free_pages=f.cpu()), dict(free_pages=f, block_table=f.cpu().view(5, 8))):
+        with pytest.raises(ValueError, match="no CPU compute path"):
+            build_block_table(meta, z, **kw)
 
 
 @pytest.mark.gpu
