@@ -130,9 +130,12 @@ class AttnLaunch:
         # memory: let go of at once, it is reused behind the launch only
         self.records = 0
 
-    def own_buffers(self, row_stats: bool) -> None:
-        """Allocate what each run brings: the row statistics when it stores them, its records."""
+    def own_buffers(self, row_stats: bool) -> torch.Tensor | None:
+        """Allocate what each run brings: the row statistics when it stores them, its records.
+        Returns the records: until its launch is made the caller holds them, or its next
+        allocation takes their memory."""
         p = self.params
+        buf = None
         # every run sets the field: a parameter block copied from a memo must not carry
         # an earlier call's buffer
         self.lse = None
@@ -147,11 +150,13 @@ class AttnLaunch:
                 with torch.cuda.stream(_torch_stream(self.stream, self.device)):
                     buf = torch.empty(self.records, dtype=torch.uint8, device=self.device)
             p.workspace, p.workspace_bytes = buf.data_ptr(), self.records
+        return buf
 
     def __call__(self) -> None:
-        self.own_buffers(getattr(_ROW_STATS, "on", False))
+        records = self.own_buffers(getattr(_ROW_STATS, "on", False))
         with _device_scope(self.device):
             rc = self.lib.fmlm_attn_fwd(self.params, self.stream)
+        del records  # held until here
         _lib.check(rc, "fmlm_attn_fwd")
 
 

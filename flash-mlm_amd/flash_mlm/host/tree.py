@@ -115,12 +115,13 @@ class TreeLaunch(AttnLaunch):
     __slots__ = ("mask",)
 
     def __call__(self) -> None:
-        self.own_buffers(row_stats=False)
+        records = self.own_buffers(row_stats=False)
         nbytes = self.lib.fmlm_attn_tree_workspace_bytes(self.params)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes > 0 else None
         with _device_scope(self.device):
             rc = self.lib.fmlm_attn_tree_fwd(self.params, self.mask.data_ptr(), int(self.mask.shape[1]), _lib.ptr(ws),
                                              nbytes, self.stream)
+        del records  # held until here
         _lib.check(rc, "fmlm_attn_tree_fwd")
 
     @classmethod

@@ -273,6 +273,26 @@ def test_mla_split_contexts(kind, lens, H, ctx, device):
 
 
 @pytest.mark.gpu
+def test_buffers_of_a_launch_are_apart(device, monkeypatch):
+    """The records of a split context and the rows that the tree's part reads live at once."""
+    lib, seen = _lib.load(), []
+    launch = lib.fmlm_attn_tree_fwd
+
+    def spy(p, mask, words, ws, n, stream):
+        seen.append((p.workspace, p.workspace_bytes, ws, n))
+        return launch(p, mask, words, ws, n, stream)
+
+    monkeypatch.setattr(lib, "fmlm_attn_tree_fwd", spy)
+    lens = [9, 9, 9, 8, 9, 9, 9, 8, 9, 7, 8, 9, 8]
+    ctx = [5858, 6266, 5193, 3825, 4380, 5922, 3749, 2784, 5662, 7539, 4647, 4385, 2065]
+    _run(device, torch.float16, lens=lens, N=9, H=32, D=512, ctx=ctx, kind="paged", mla=True)
+    assert seen
+    for rec, rec_bytes, ws, n in seen:
+        assert rec and rec_bytes > 0 and ws and n > 0
+        assert rec + rec_bytes <= ws or ws + n <= rec
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype, kind", [("bf16", "shared"), ("fp16", "index"), ("fp32", "shared"), ("bf16", "index")])
 def test_shared_and_indexed_contexts(dtype, kind, device):
     _run(device, DT[dtype], lens=[9, 20, 3], N=20, H=2, D=64, ctx=[200, 77, 1], kind=kind, seed=4)
