@@ -5,8 +5,8 @@ speculative decoding loop over a paged cache.
 Tolerances.  With W = sum of w |v| of an output element, h half a step of the type and u =
 2^-24: the context's part is rounded once (h of it) and the output once more (h |o|); the
 probabilities of both parts are rounded (2 h W with their sums); a score's error e moves the
-result by at most 2 e W, and e is (D + 16) u S in fp32, S = scale * sum |q k|, plus h S where
-fp16 queries are scaled before the product; exponentials and sums add (keys + 64) u W at most.
+result by at most 2 e W, and e is (D + 16) u S in fp32, S = scale * sum |q k|; exponentials and
+sums add (keys + 64) u W at most.
 Fp16 probabilities below 2^-14 have an absolute error of 2^-25 each.
 """
 
@@ -169,7 +169,7 @@ def _close(got, q, k, v, seen, scale, kc, vc, dtype):
     o, w, c, s = ref.tree_attention(_f(q), _f(k), _f(v), seen, scale, _f(kc), _f(vc))
     h = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
     keys, D = kc.shape[0] + k.shape[0], q.shape[-1]
-    e = ((D + 16) * U + (h if dtype == torch.float16 else 0.0)) * s[:, None]
+    e = (D + 16) * U * s[:, None]
     bound = h * (np.abs(o) + c) + (2 * h + 2 * e + (keys + 64) * U) * w
     if dtype == torch.float16:
         bound = bound + 2.0**-25 * (keys * np.abs(np.concatenate([_f(vc), _f(v)])).max() + 1)
