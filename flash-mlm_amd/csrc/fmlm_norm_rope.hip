@@ -20,7 +20,7 @@
 //
 // Measured (a large copy reaches 5.16 TB/s).  Forward, 32 sequences of 256-1024 tokens, 16 heads of
 // q and k, D = 128, fp16, padding rows written as zeros: 457 MB in 90 us, 5.1 TB/s; packed rows
-// with gains per head, 359 MB in 67.  Backward of the latter, 539 MB in 114 + 5 us (4.5 TB/s), and
+// with gains per head, 359 MB in 67.  Backward of the latter, 539 MB in 119 to 124 + 5 us (4.4 TB/s), and
 // 112 + 5 with shared gains.  64 decoding tokens: 4.4 us, latency.
 #include "fmlm_common.h"
 
