@@ -11,7 +11,6 @@ import torch
 from flash_mlm import _lib
 from flash_mlm.host.cache import InferenceCache, PackMetadata
 from flash_mlm.host.host import (
-    _cache_tensors,
     _check_cache_dtype,
     _context_index,
     _ctx_rows,
@@ -155,7 +154,18 @@ def flash_attn_mlm_tree(
     changed: store the accepted tokens with :meth:`InferenceCache.append_paged_kv_cache`.
     No gradients: inputs that require grad raise ValueError (use ``torch.no_grad()``).
     """
-    memo, entry = q_meta.launch_memo, _entry_of(inference_cache, layer_id)
+    memo, entry, mask = q_meta.launch_memo, _entry_of(inference_cache, layer_id), tree.mask
+    if _wants_grad(q, k, v, *((entry.k_cache, entry.v_cache) if entry is not None else ())):
+        raise ValueError("flash_attn_mlm_tree has no backward; call it under torch.no_grad()")
+    key = None
+    if context_index is None and all(isinstance(t, torch.Tensor) for t in (q, k, v, mask)):
+        # all that the checks below depend on
+        key = ("tree", _tkey(q), _tkey(k), _tkey(v), _tkey(mask), num_heads, q_meta.B, q_meta.N, q_meta.total_tokens,
+               float(scale), is_mla, context_batch_size, tile_config_value(), None if entry is None else id(entry),
+               inference_cache is None)
+        m = _memo_lookup(memo, key, entry)
+        if m is not None:
+            return _memo_run(m, q, k, v, entry, wrap=lambda plan: TreeLaunch.of(plan, mask))[0]
     b, h, n, d = validate_qkv_same_shape_rank4(q, k, v, error_prefix="q/k/v")
     if h != num_heads:
         raise ValueError("q/k/v head dimension must match num_heads")
@@ -164,18 +174,8 @@ def flash_attn_mlm_tree(
     if n > MAX_TREE_TOKENS:
         raise ValueError(f"a drafted tree has at most {MAX_TREE_TOKENS} tokens (q_meta.N)")
     T = int(q_meta.total_tokens)
-    mask = tree.mask
     if mask.ndim != 2 or mask.dtype != torch.int64 or int(mask.shape[0]) != T or int(mask.shape[1]) * 64 < n:
         raise ValueError("tree.mask must be [tokens, words] int64, built for this q_meta")
-    if _wants_grad(q, k, v, *_cache_tensors(inference_cache, layer_id, False)[:2]):
-        raise ValueError("flash_attn_mlm_tree has no backward; call it under torch.no_grad()")
-    key = None
-    if context_index is None:
-        key = ("tree", _tkey(q), _tkey(k), _tkey(v), float(scale), is_mla, context_batch_size, tile_config_value(),
-               None if entry is None else id(entry), inference_cache is None, mask.is_contiguous(), mask.device)
-        m = _memo_lookup(memo, key, entry)
-        if m is not None:
-            return _memo_run(m, q, k, v, entry, wrap=lambda plan: TreeLaunch.of(plan, mask))[0]
     validate_cache_request(prefill=False, inference_cache=inference_cache, layer_id=layer_id)
     ctx = _maybe_get_cache_context(
         inference_cache=inference_cache,
