@@ -510,3 +510,16 @@ def test_feeds_attention(device):
     for a, b in zip(got, want):
         # fp32 throughout: sums of up to 64 products a score, 24 keys a row
         assert (a.double() - b).abs().max() <= 2000 * U * b.abs().max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("through", [False, True])  # whether the incoming gradients have one
+def test_gradients_have_no_gradient(through, device):
+    q, k = (torch.randn((1, 2, 5, 64), device=device, requires_grad=True) for _ in range(2))
+    a, b = qk_norm_rope(q, k)
+    plain = torch.autograd.grad((a, b), (q, k), (torch.ones_like(a), torch.ones_like(b)), retain_graph=True)
+    ones = [torch.ones_like(a).requires_grad_(through), torch.ones_like(b).requires_grad_(through)]
+    dq, dk = torch.autograd.grad((a, b), (q, k), ones, create_graph=True)
+    assert torch.equal(dq, plain[0]) and torch.equal(dk, plain[1])
+    with pytest.raises(RuntimeError, match="once_differentiable" if through else "does not require grad"):
+        torch.autograd.grad(dq.sum(), q)
