@@ -323,6 +323,65 @@ def test_append_of_views_and_bad_slots(device):
 
 
 @pytest.mark.gpu
+def test_append_on_another_stream_and_in_a_graph(device):
+    """A step's table and append, captured: replays with new lengths, rows and kept tokens."""
+    H, D, N, lens = 3, 64, 20, [20, 1, 0, 13]
+    k, v, meta, plan, kp, vp, cache = _append_case(device, torch.bfloat16, H, D, False, lens, N, False, False, 5)
+    want = [_expected_pool(p, x, meta, plan.slot_mapping, H) for p, x in ((kp, k), (vp, v))]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.append_paged_kv_cache(0, k=k, v=v, q_meta=meta, plan=plan)
+    side.synchronize()
+    assert torch.equal(kp, want[0]) and torch.equal(vp, want[1])
+    old = torch.tensor([3, 60, 0, 64], dtype=torch.int32, device=device)
+    table = torch.tensor([[0, -1], [1, -1], [-1, -1], [2, -1]], dtype=torch.int32, device=device)
+    free = torch.arange(3, 8, dtype=torch.int32, device=device)
+    kept = torch.ones(sum(lens), dtype=torch.bool, device=device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step = build_block_table(meta, old, free_pages=free, block_table=table, keep=kept, check=False)
+        cache.append_paged_kv_cache(0, k=k, v=v, q_meta=meta, plan=step)
+    g = torch.Generator().manual_seed(1)
+    for ctx in ([3, 60, 0, 64], [64, 0, 0, 50], [44, 64, 0, 1]):
+        old.copy_(torch.tensor(ctx))
+        kept.copy_(torch.rand(sum(lens), generator=g) < 0.7)
+        k.copy_(torch.randn(k.shape, generator=g))
+        v.copy_(torch.randn(v.shape, generator=g))
+        eager = build_block_table(meta, old, free_pages=free, block_table=table, keep=kept)
+        want = [_expected_pool(p, x, meta, eager.slot_mapping, H) for p, x in ((kp, k), (vp, v))]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(step.slot_mapping, eager.slot_mapping)
+        assert torch.equal(step.block_table, eager.block_table)
+        assert torch.equal(kp, want[0]) and torch.equal(vp, want[1])
+
+
+@pytest.mark.gpu
+def test_append_past_32_bits(device):
+    """A pool of more than 2^32 elements: rows of its first and last pages."""
+    D, N, lens, P = 512, 70, [70, 5], 131100
+    pool = torch.empty((1, P, PAGE, D), dtype=torch.bfloat16, device=device)
+    ends = [0, 1, P - 3, P - 2, P - 1]
+    pool[:, ends] = 0
+    cache = InferenceCache()
+    table = torch.tensor([[P - 1, -1], [0, -1]], dtype=torch.int32, device=device)
+    old = torch.tensor([60, 63], dtype=torch.int32, device=device)
+    cache.prefill_paged_kv_cache(0, k_pages=pool, block_table=table, context_lens=old, is_mla=True, num_heads=2, head_dim=D)
+    meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+    free = torch.tensor([P - 3, 1, P - 2], dtype=torch.int32, device=device)
+    plan = build_block_table(meta, old, free_pages=free, block_table=table, max_pages=3)
+    assert plan.pages_taken == 3 and int(plan.slot_mapping.max()) * D > 2**32
+    k = torch.randn((2, 2, N, D), device=device).bfloat16()
+    cache.append_paged_kv_cache(0, k=k, q_meta=meta, plan=plan)
+    rows = torch.cat([k[0, 0, :70], k[1, 0, :5]])
+    flat = pool.view(-1, D)
+    assert torch.equal(flat[plan.slot_mapping], rows)
+    left = pool[:, ends]
+    assert int((left != 0).any(-1).sum()) == sum(lens)
+
+
+@pytest.mark.gpu
 def test_appended_context_is_what_attention_reads(device):
     """Attend, append, attend: the second call over the pages equals one over the same rows
     stored contiguously, bit for bit; rows of the pool that hold no token may be NaN."""

@@ -441,6 +441,33 @@ def test_repeated_calls_streams_and_graphs(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H, D, mla, P", [(2, 128, False, 262200), (4, 512, True, 131100)])
+def test_contexts_past_32_bits(H, D, mla, P, device):
+    """Pages at the ends of a pool of more than 2^32 elements: the bits of a small pool's."""
+    hk, N, lens, ctx = 1 if mla else H, 6, [6, 2], [150, 64]
+    g = torch.Generator().manual_seed(7)
+    meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+    tree = build_tree_metadata(torch.tensor([-1, 0, 0, 1, 1, 2, -1, 0], device=device), meta)
+    q, k, v = (torch.randn((2, H, N, D), generator=g).bfloat16().to(device) for _ in range(3))
+    small = [torch.randn((hk, 4, PAGE, D), generator=g).bfloat16().to(device) for _ in range(1 if mla else 2)]
+    outs = []
+    for far in (False, True):
+        pages = [P - 1, 0, P - 2, P - 3] if far else [0, 1, 2, 3]
+        pools = small
+        if far:
+            pools = [torch.empty((hk, P, PAGE, D), dtype=torch.bfloat16, device=device) for _ in small]
+            assert pools[0].numel() > 2**32
+            for big, x in zip(pools, small):
+                big[:, pages] = x
+        table = torch.tensor([pages[:3], [pages[3], -1, -1]], dtype=torch.int32, device=device)
+        cache = InferenceCache()
+        cache.prefill_paged_kv_cache(0, k_pages=pools[0], v_pages=None if mla else pools[1], block_table=table,
+                                     context_lens=torch.tensor(ctx), is_mla=mla, num_heads=H, head_dim=D)
+        outs.append(flash_attn_mlm_tree(q, k, v, H, meta, tree, D**-0.5, cache, 0, is_mla=mla))
+    assert torch.isfinite(outs[0]).all() and torch.equal(*outs)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D, mla", [(64, False), (512, True)])
 def test_first_call_of_a_metadata_in_a_graph(D, mla, device):
     """A capture leaves nothing behind on the metadata that only its replays fill: an eager call
