@@ -523,3 +523,24 @@ def test_gradients_have_no_gradient(through, device):
     assert torch.equal(dq, plain[0]) and torch.equal(dk, plain[1])
     with pytest.raises(RuntimeError, match="once_differentiable" if through else "does not require grad"):
         dq.sum().backward()
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bits(device):
+    """Rows at both ends of a tensor of more than 2^32 elements: the bits of the same rows alone."""
+    H, N, D, n = 2, 4194400, 512, 3
+    q = torch.empty((1, H, N, D), dtype=torch.bfloat16, device=device).normal_()
+    k = torch.empty((1, 1, N, D), dtype=torch.bfloat16, device=device).normal_()
+    assert q.numel() > 2**32
+    angle = torch.arange(8, device=device)[:, None] * torch.linspace(1, 0.01, 128, device=device)
+    cos, sin = angle.cos(), angle.sin()
+    pos = (torch.arange(N, dtype=torch.int32, device=device) % 8)[None]
+    q.requires_grad_(), k.requires_grad_()
+    a, b = qk_norm_rope(q, k, cos=cos, sin=sin, positions=pos)
+    dq, dk = torch.autograd.grad((a, b), (q, k), (q.detach(), k.detach()))
+    for part in (slice(0, n), slice(N // 2, N // 2 + n), slice(N - n, N)):
+        x, y = (t.detach()[:, :, part].contiguous().requires_grad_() for t in (q, k))
+        c, d = qk_norm_rope(x, y, cos=cos, sin=sin, positions=pos[:, part])
+        dx, dy = torch.autograd.grad((c, d), (x, y), (x.detach(), y.detach()))
+        for big, small in ((a, c), (b, d), (dq, dx), (dk, dy)):
+            assert torch.equal(big[:, :, part], small)
