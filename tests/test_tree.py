@@ -375,6 +375,50 @@ def test_values_that_are_not_finite(dtype, value, device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("D, mla, ctx", [(512, True, [300, 0]), (512, True, [0, 4000]), (128, True, [70, 3]),
+                                         (256, False, [2100, 64])])
+def test_wide_rows_that_are_not_finite(dtype, value, D, mla, ctx, device):
+    """As above at the widths that other kernels or tiles take; MLA rows are key and value at once."""
+    lens, N, H = [70, 7], 75, 2
+    parents = [-1 if i < 4 else i - 4 for n in lens for i in range(n)]  # four chains
+
+    def run(spoil):
+        r = torch.Generator().manual_seed(9)
+        q, k, v = (torch.randn((2, H, N, D), generator=r).to(DT[dtype]).to(device) for _ in range(3))
+        v = k if mla else v
+        spoil(k, v)
+        meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+        tree = build_tree_metadata(torch.tensor(parents, device=device), meta)
+        cache, _, _ = _context("packed", ctx, H, D, mla, DT[dtype], device, 1)
+        return unpack_from_kernel(
+            flash_attn_mlm_tree(q, k, v, H, meta, tree, D**-0.5, cache, 0, is_mla=mla), meta, H)
+
+    clean = run(lambda k, v: None)
+    assert clean.isfinite().all()
+
+    def pad(k, v):
+        for b, n in enumerate(lens):
+            k[b, :, n:] = value
+            v[b, :, n:] = value
+
+    assert torch.equal(run(pad), clean)
+    for token in (3, 66):  # of the first and of a later key tile
+        rows = torch.zeros((2, N), dtype=torch.bool, device=device)
+        rows[0, token:70:4] = True
+        rows[1, token:7:4] = True
+
+        def spoil(k, v):
+            v[:, :, token, 5] = value
+
+        got = run(spoil)
+        for h in range(H):
+            assert torch.equal(got[:, h][~rows], clean[:, h][~rows])
+            assert not got[:, h][rows][:, 5].isfinite().any()
+
+
+@pytest.mark.gpu
 def test_chain_of_one_is_the_ordinary_call(device):
     """One token a sequence sees its context and itself, as in flash_attn_mlm_compressed."""
     _run(device, torch.bfloat16, lens=[1] * 9, N=1, H=4, D=128, ctx=[700] * 9, kind="paged", seed=9)
