@@ -149,7 +149,8 @@ def flash_attn_mlm_tree(
     ancestors in ``tree``] instead of all tokens of its sequence.
 
     Returns the packed output [H * T, D] (head-major).  A chain (``parents = i - 1``) is ordinary
-    causal decoding of several tokens.  Context, ``is_mla`` and ``context_index`` are as in
+    causal decoding of several tokens; ``tree.mask`` may also be set bit by bit, to what no tree
+    is, and a row that sees no key at all is zero.  Context, ``is_mla`` and ``context_index`` are as in
     :func:`flash_attn_mlm_compressed`; at most 256 tokens a sequence.  The context is not
     changed: store the accepted tokens with :meth:`InferenceCache.append_paged_kv_cache`.
     No gradients: inputs that require grad raise ValueError (use ``torch.no_grad()``).

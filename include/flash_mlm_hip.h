@@ -501,8 +501,9 @@ FMLM_API int fmlm_tree_mask(const void* parents, int32_t parents_i64, const int3
  * to [its context || the main tokens j of its sequence with mask bit j set]; bits at or past
  * the sequence's end are ignored.  A row that sees no key has output 0.  At most FMLM_MAX_TREE
  * tokens in a sequence (N, or total_q where N is 0).  p->lse is not used; no backward.
- * Up to D = 256 the attention kernel masks the main keys itself.  For D = 512 (MLA) a second kernel computes the tree's part, and the context's part goes through
- * tree_workspace: fmlm_attn_tree_workspace_bytes(p) bytes (0 in the first case). */
+ * Up to D = 256 the attention kernel masks the main keys itself.  For D = 512 (MLA) a second
+ * kernel computes the tree's part, and the context's part goes through tree_workspace:
+ * fmlm_attn_tree_workspace_bytes(p) bytes (0 in the first case). */
 FMLM_API int64_t fmlm_attn_tree_workspace_bytes(const fmlm_attn_params* p);
 FMLM_API int fmlm_attn_tree_fwd(const fmlm_attn_params* p, const uint64_t* mask, int32_t words, void* tree_workspace,
                                 int64_t tree_workspace_bytes, void* stream);

@@ -332,6 +332,42 @@ def test_scales(dtype, scale, device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("D, mla", [(32, False), (64, False), (128, False), (256, False), (512, True)])
+@pytest.mark.parametrize("ctx", [[0, 0, 0], [70, 0, 4000]])
+def test_masks_of_any_kind(dtype, D, mla, ctx, device):
+    """Masks that no tree has: rows that see nothing (they have the context alone, or are zero), rows
+    that see later tokens or only another key tile's, bits past the sequence, a word too many."""
+    r, H, lens, N = random.Random(D), 2, [90, 3, 150], 151
+    g = torch.Generator().manual_seed(D)
+    q, k, v = (torch.randn((3, H, N, D), generator=g).to(DT[dtype]).to(device) for _ in range(3))
+    v = k if mla else v
+    meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+    seen = []
+    for n in lens:
+        kinds = [set(), set(range(n)), {n - 1}, set(range(64, n)), set(range(min(64, n)))]
+        seen += [kinds[i] if i < 5 else {j for j in range(n) if r.random() < 0.3} if i % 7 else set() for i in range(n)]
+    words = np.zeros((sum(lens), 4), dtype=np.uint64)
+    past = [n for n in lens for _ in range(n)]
+    for t, (s, n) in enumerate(zip(seen, past)):
+        for j in list(s) + [x for x in (n, n + 1, 200, 255) if r.random() < 0.5]:
+            words[t, j // 64] |= np.uint64(1 << (j % 64))
+    tree = TreeMetadata(torch.from_numpy(words.view(np.int64)).to(device), None)
+    cache, rows, kw = _context("packed", ctx, H, D, mla, DT[dtype], device, 3)
+    got = flash_attn_mlm_tree(q, k, v, H, meta, tree, D**-0.5, cache, 0, is_mla=mla, **kw).view(H, -1, D)
+    at = 0
+    for b, n in enumerate(lens):
+        some = [i for i in range(n) if seen[at + i] or ctx[b]]
+        none = [at + i for i in range(n) if not seen[at + i] and not ctx[b]]
+        for h in range(H):
+            j = 0 if mla else h
+            _close(got[h, [at + i for i in some]], q[b, h, some], k[b, j, :n], v[b, j, :n], [seen[at + i] for i in some],
+                   D**-0.5, rows[b][0][j], rows[b][1][j], DT[dtype])
+        assert not got[:, none].any()
+        at += n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
 def test_values_that_are_not_finite(dtype, value, device):
     """Token 3 holds NaN or an infinity in K or V: the rows that do not see it are as without it,
