@@ -2799,13 +2799,21 @@ static Launch mla_rows_launch(const fmlm_attn_params& p) {
 // split plan's ranges that are worth cutting follow from it (D = 32, 2 sequences of 9-10 tokens, 4
 // heads, 1830-2489 rows: 28.4 us with 0.47, unsplit; 14.9).
 constexpr float kTreeTileUs = 0.8f;
+// The context's part in that choice is advice (fmlm_attn_tree_tile), which the caller puts into
+// tile_config: a schedule is made for one tile and serves calls over other contexts, so the tile
+// may only depend on what a schedule is known by.
+static int tree_tile(const fmlm_attn_params& p) {
+  if (p.tile_config > 0) return p.tile_config;
+  if (p.dtype == FMLM_DTYPE_F32 || p.D != 256) return 0;
+  const int64_t rows = p.ctx_block_table ? (int64_t)p.ctx_pages_per_batch * FMLM_PAGE_ROWS
+                                         : p.ctx_rows / std::max(p.ctx_batch, 1);
+  const bool wide = p.total_q > 64LL * p.B && rows >= 2048 && (int64_t)p.H * (p.total_q / 128 + p.B / 2) >= 48;
+  return wide ? 2 : 1;
+}
 template <typename T>
 static bool pick_tree(const fmlm_attn_params& p, Launch& L) {
   const bool paged = p.ctx_block_table != nullptr;
-  const int64_t rows = paged ? (int64_t)p.ctx_pages_per_batch * FMLM_PAGE_ROWS : p.ctx_rows / std::max(p.ctx_batch, 1);
-  const bool wide = p.D == 256 && p.total_q > 64LL * p.B && rows >= 2048 &&
-                    (int64_t)p.H * (p.total_q / 128 + p.B / 2) >= 48;
-  const int k = p.tile_config > 0 ? p.tile_config : wide ? 2 : 1;
+  const int k = p.tile_config > 0 ? p.tile_config : 1;
   if (k > (p.D == 256 ? 2 : 1)) return false;
   switch (p.D) {
     case 16: L = mfma3_launch<T, 16, 1, 4, 64, 0, true>(paged); break;
@@ -3303,6 +3311,11 @@ extern "C" int fmlm_attn_fwd(const fmlm_attn_params* pp, void* stream) {
   const int rc = check_params(*pp);
   if (rc) return rc;
   return attn_fwd(effective(*pp), nullptr, 0, stream);
+}
+
+extern "C" int fmlm_attn_tree_tile(const fmlm_attn_params* pp) {
+  if (!pp || !(pp->flags & FMLM_FLAG_TREE)) return FMLM_E_ARG;
+  return tree_tile(*pp);
 }
 
 extern "C" int64_t fmlm_attn_tree_workspace_bytes(const fmlm_attn_params* pp) {

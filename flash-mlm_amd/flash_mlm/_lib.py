@@ -263,6 +263,7 @@ SIGNATURES = {
         ctypes.c_int,
         [_c_ptr, _c_i32, _c_ptr, _c_i32, _c_i32, _c_i32, _c_i32, _c_ptr, _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
     ),
+    "fmlm_attn_tree_tile": (ctypes.c_int, [ctypes.POINTER(AttnParams)]),
     "fmlm_attn_tree_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(AttnParams)]),
     "fmlm_attn_tree_fwd": (ctypes.c_int, [ctypes.POINTER(AttnParams), _c_ptr, _c_i32, _c_ptr, _c_i64, _c_ptr]),
 }

@@ -473,6 +473,8 @@ def _prepare(
     p.k_ctx = k_ctx.data_ptr() if k_ctx.numel() else None
     p.v_ctx = v_ctx.data_ptr() if (v_ctx is not None and v_ctx.numel()) else p.k_ctx
     p.c_sb, p.c_sh, p.c_sn = c_strides
+    if flags & _lib.FLAG_TREE and D == 256 and not p.tile_config:
+        p.tile_config = lib.fmlm_attn_tree_tile(p)  # by the context too, so part of the schedule's key
     records = int(lib.fmlm_attn_records_bytes(p))
     _lib.check(records if records < 0 else 0, "fmlm_attn_records_bytes")
     if records == 0:
@@ -487,7 +489,7 @@ def _prepare(
         # what the unit list depends on: the kernel (dtype, head dim, flags, K/V
         # layout, paged context or not), whose tile size and occupancy fix the slots,
         # the split records and the grid, and the shape (B, H, N, total_q); context
-        # lengths only steer where key ranges are split
+        # lengths only steer where key ranges are split, and at most the tile configuration
         if records:
             p.flags |= _lib.FLAG_OWN_RECORDS
         key = (p.dtype, D, B, H, N, total_q, p.flags, p.kv_layout, block_table is not None, p.tile_config)

@@ -218,9 +218,9 @@ typedef struct fmlm_attn_params {
   void* workspace;         /* device scratch for the work schedule                  */
   int64_t workspace_bytes;
   const void* schedule;    /* NULL, or a schedule built by fmlm_attn_schedule for the same
-                              cu_seqlens_q contents, B, H, total_q, dtype, D, flags (with
-                              others than it was built for, rows stay unwritten) and
-                              kv_layout: then fmlm_attn_fwd launches the attention
+                              cu_seqlens_q contents, B, H, N, total_q, dtype, D, flags,
+                              tile_config (with others than it was built for, rows stay
+                              unwritten) and kv_layout: then fmlm_attn_fwd launches the attention
                               kernel (plus the split merge) only.  Context lengths may
                               differ; they only steer where key ranges are split.  The
                               buffer also holds split partial results: launches that may
@@ -253,7 +253,8 @@ typedef struct fmlm_attn_params {
    * 2 = (256, 8), 3 = (64, 4), 4 = (256, 8) ping-pong; D = 128: 1 = (128, 4),
    * 2 = (256, 8), 3 = (64, 4), 4 = (128, 8), 5 = (256, 8) ping-pong; D = 256:
    * 1 = (64, 4), 2 = (128, 8); MLA D = 512: 1 = (128, 8), in packed calls of at most 4096
-   * (head, position) rows (64, 8).  Tree calls (FMLM_FLAG_TREE): 1 = (64, 4), D = 256 also 2 = (128, 8).
+   * (head, position) rows (64, 8).  Tree calls (FMLM_FLAG_TREE): 1 = (64, 4), which 0 is, D = 256 also
+   * 2 = (128, 8): fmlm_attn_tree_tile says when it pays.
    * Ping-pong: the 8 waves run as
    * two groups half a key tile apart, so that one wave of each SIMD computes softmax
    * while the other issues MFMAs.  Replaces the reference's autotuned
@@ -504,6 +505,9 @@ FMLM_API int fmlm_tree_mask(const void* parents, int32_t parents_i64, const int3
  * Up to D = 256 the attention kernel masks the main keys itself.  For D = 512 (MLA) a second
  * kernel computes the tree's part, and the context's part goes through tree_workspace:
  * fmlm_attn_tree_workspace_bytes(p) bytes (0 in the first case). */
+FMLM_API int fmlm_attn_tree_tile(const fmlm_attn_params* p); /* the tile_config that the call's
+                               shape and context ask for (p's own when set; 0: there is no
+                               choice), or FMLM_E_ARG.  Set it before the sizes are asked for */
 FMLM_API int64_t fmlm_attn_tree_workspace_bytes(const fmlm_attn_params* p);
 FMLM_API int fmlm_attn_tree_fwd(const fmlm_attn_params* p, const uint64_t* mask, int32_t words, void* tree_workspace,
                                 int64_t tree_workspace_bytes, void* stream);

@@ -628,3 +628,64 @@ def test_speculative_decoding_over_a_paged_cache(dtype, device):
             slot = table[b].long()[rows // PAGE] * PAGE + rows % PAGE
             for pool, t in zip(pools, text[b]):
                 assert torch.equal(pool.view(H, -1, D)[:, slot], t)
+
+
+def test_schedules_do_not_depend_on_contexts():
+    """A schedule serves calls over other contexts (one metadata, several layers): its size, so the
+    rows a unit of it stands for, follows from what its key holds.  The context's share in the
+    choice of a tile is advice, which the caller puts into tile_config."""
+    lib = _lib.load()
+    p = _lib.AttnParams()
+    p.flags = _lib.FLAG_TREE | _lib.FLAG_NOSPLIT
+    p.cu_seqlens_q = p.cu_seqlens_kv = p.q = p.k = p.v = p.o = p.k_ctx = p.v_ctx = 256
+    for dtype in (_lib.DTYPE_BF16, _lib.DTYPE_F16, _lib.DTYPE_F32):
+        for d in (16, 32, 64, 128, 256):
+            for B, H, n in ((8, 8, 100), (1, 16, 256), (3, 2, 9)):
+                p.dtype, p.D, p.B, p.H, p.N, p.total_q, p.tile_config = dtype, d, B, H, n, B * n, 0
+                sizes, advice = set(), set()
+                for paged in (False, True) if dtype != _lib.DTYPE_F32 else (False,):
+                    for pages in (1, 20, 33, 500):
+                        p.ctx_batch, p.ctx_rows, p.ctx_block_table, p.ctx_pages_per_batch = B, B * pages * PAGE, None, 0
+                        if paged:
+                            p.ctx_rows, p.ctx_block_table, p.ctx_pages_per_batch = B * pages, 256, pages
+                            p.ctx_page_stride = PAGE * d
+                        sizes.add(lib.fmlm_attn_workspace_bytes(p))
+                        advice.add((pages >= 32, lib.fmlm_attn_tree_tile(p)))
+                assert len(sizes) == 1, (dtype, d, B, H, n)
+                wide = dtype != _lib.DTYPE_F32 and d == 256
+                if (B, H, n) == (8, 8, 100) and wide:
+                    assert advice == {(False, 1), (True, 2)}
+                else:
+                    assert {x for _, x in advice} == {1 if wide else 0}
+    p.dtype, p.D, p.tile_config = _lib.DTYPE_BF16, 256, 2
+    assert lib.fmlm_attn_tree_tile(p) == 2  # the caller's own
+    p.flags = 0
+    assert lib.fmlm_attn_tree_tile(p) == -1 and lib.fmlm_attn_tree_tile(None) == -1  # tree calls
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["paged", "packed"])
+@pytest.mark.parametrize("order", [(33, 20), (20, 33), (33, 20, 33, 1)])
+def test_layers_of_one_metadata_with_other_contexts(kind, order, device):
+    """D = 256: layers whose contexts ask for 64- and for 128-row workgroups, one metadata"""
+    H, D, lens, N = 8, 256, [100] * 8, 100
+    meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+    parents = _random_parents(random.Random(1), lens)
+    tree = build_tree_metadata(torch.tensor(parents, device=device), meta)
+    seen = ref.ancestors(parents, lens)
+    layers = []
+    for i, pages in enumerate(order):
+        g = torch.Generator().manual_seed(i)
+        q, k, v = (torch.randn((8, H, N, D), generator=g).bfloat16().to(device) for _ in range(3))
+        layers.append((q, k, v, *_context(kind, [pages * PAGE - b for b in range(8)], H, D, False, torch.bfloat16, device, i)))
+    for _ in range(2):  # the second time by the memos of the first
+        for q, k, v, cache, rows, _ in layers:
+            poison = torch.full((H * sum(lens), D), float("nan"), dtype=torch.bfloat16, device=device)
+            del poison  # rows that no workgroup writes
+            got = flash_attn_mlm_tree(q, k, v, H, meta, tree, D**-0.5, cache, 0).view(H, -1, D)
+            for b in (0, 5):
+                part = slice(100 * b, 100 * b + 100)
+                for h in (0, 7):
+                    _close(got[h, part], q[b, h], k[b, h], v[b, h], seen[part], D**-0.5, rows[b][0][h], rows[b][1][h],
+                           torch.bfloat16)
+            assert bool(got.isfinite().all())
