@@ -31,7 +31,7 @@ def aligned16(t: torch.Tensor) -> torch.Tensor:
 class _Call:
     """The checked arguments of one call as a parameter block without the rows' addresses."""
 
-    __slots__ = ("block", "packed", "keep")
+    __slots__ = ("block", "packed", "keep", "sizes")
 
     def put(self, t, x, y) -> None:
         """Rows in and out of tensor ``t`` of a block (packed rows: strides are the block's)."""
@@ -58,11 +58,11 @@ def _layout(t):
 
 
 class _Memo:
-    __slots__ = ("block", "packed", "keep", "meta")
+    __slots__ = ("block", "packed", "keep", "sizes", "meta")
 
     def __init__(self, call: _Call, q_meta):
         self.block = _lib.NormRopeParams.from_buffer_copy(call.block)
-        self.packed, self.keep = call.packed, call.keep
+        self.packed, self.keep, self.sizes = call.packed, call.keep, call.sizes
         self.meta = None
         if q_meta is not None:
             self.meta = (q_meta.cu_seqlens, q_meta.token_indices, q_meta.total_tokens, q_meta.B, q_meta.N)
@@ -76,7 +76,7 @@ class _Memo:
     def call_for(self, wq, wk, cos, sin, idx, offsets: bool) -> _Call:
         call = _Call()
         p = call.block = _lib.NormRopeParams.from_buffer_copy(self.block)
-        call.packed, call.keep = self.packed, self.keep
+        call.packed, call.keep, call.sizes = self.packed, self.keep, self.sizes
         if wq is not None:
             p.q.weight = wq.data_ptr()
         if wk is not None:
@@ -115,13 +115,49 @@ def _forward(call: _Call, q, k):
     return outs
 
 
-def _backward(call: _Call, xs, ws, dys, needs):
+def _saved(t: torch.Tensor, size: int, dtype, device: int, layout) -> torch.Tensor:
+    """``t`` of the saved tensors as the kernel reads it (``layout`` of it where it is not)."""
+    if t.numel() != size or t.dtype is not dtype or t.get_device() != device:
+        raise RuntimeError("qk_norm_rope: a saved tensor came back with another size or type, or on another device")
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else layout(t)
+
+
+def _rebind(call: _Call, p, saved) -> tuple:
+    """Rows and gains of the saved tensors, and the block's other addresses from them.  They need not be where
+    the forward's were: a checkpoint recomputes them and a saved-tensor hook brings copies, laid out
+    as it likes.  The last of the tuple is held until the launch."""
+    q, k, wq, wk, cos, sin, positions, context_lens = saved
+    nq, nk, dtype, nwq, nwk, w_dtype, table, indices, i_dtype, dev = call.sizes
+    layout = aligned16 if call.packed else rows16
+    q, k = _saved(q, nq, dtype, dev, layout), _saved(k, nk, dtype, dev, layout)
+    if wq is not None:
+        wq = _saved(wq, nwq, w_dtype, dev, aligned16)
+        p.q.weight = wq.data_ptr()
+    if wk is not None:
+        wk = _saved(wk, nwk, w_dtype, dev, aligned16)
+        p.k.weight = wk.data_ptr()
+    index = positions if positions is not None else context_lens
+    if cos is not None:
+        cos = _saved(cos, table, torch.float32, dev, aligned16)
+        sin = _saved(sin, table, torch.float32, dev, aligned16)
+        p.cos, p.sin = cos.data_ptr(), sin.data_ptr()
+        if index is not None:
+            index = _saved(index, indices, i_dtype, dev, aligned16)
+            if positions is not None:
+                p.positions = index.data_ptr()
+            else:
+                p.offsets = index.data_ptr()
+    return (q, k), (wq, wk), (cos, sin, index)
+
+
+def _backward(call: _Call, saved, dys, needs):
     """Gradients (dq, dk, dwq, dwk); ``needs`` says which are wanted, None in ``dys`` is zero."""
     lib = _lib.load()
-    dev = xs[0].device
+    dev = saved[0].device
     p = _lib.NormRopeParams.from_buffer_copy(call.block)  # (a graph can be walked more than once)
     if p.rows == 0:
-        return tuple(torch.zeros_like(t) if n else None for t, n in zip((*xs, *ws), needs))
+        return tuple(torch.zeros_like(t) if n else None for t, n in zip(saved, needs))
+    xs, ws, _tables = _rebind(call, p, saved)
     dxs, dws, keep = [None, None], [None, None], []
     for i, t in enumerate((p.q, p.k)):
         if dys[i] is None or not (needs[i] or needs[2 + i]):
@@ -153,7 +189,8 @@ class _NormRope(torch.autograd.Function):
     def forward(ctx, call, q, k, wq, wk, cos, sin, positions, context_lens):
         ctx.call = call
         ctx.set_materialize_grads(False)
-        # saved so that autograd rejects a backward after any of them changed in place
+        # saved so that autograd rejects a backward after any of them changed in place, and read
+        # from there: autograd may free these and bring others (_rebind)
         ctx.save_for_backward(q, k, wq, wk, cos, sin, positions, context_lens)
         return _forward(call, q, k)
 
@@ -165,8 +202,7 @@ class _NormRope(torch.autograd.Function):
 
 
 def _backward_node(ctx, dq, dk):
-    q, k, wq, wk, *_ = ctx.saved_tensors
-    grads = _backward(ctx.call, (q, k), (wq, wk), (dq, dk), ctx.needs_input_grad[1:5])
+    grads = _backward(ctx.call, ctx.saved_tensors, (dq, dk), ctx.needs_input_grad[1:5])
     return (None, *grads, None, None, None, None)
 
 
@@ -389,6 +425,10 @@ def qk_norm_rope(
     p.flags = flags
     q_, k_ = (aligned16(q), aligned16(k)) if packed else (rows16(q), rows16(k))
     call.keep = (cu, tokens)
+    # elements, types and device of what the backward reads (_rebind)
+    call.sizes = (q.numel(), k.numel(), dtype, *((None if w is None else w.numel()) for w in (wq, wk)),
+                  next((w.dtype for w in (wq, wk) if w is not None), None), None if cos is None else cos.numel(),
+                  *((None, None) if idx is None else (idx.numel(), idx.dtype)), q.get_device())
     own = q_meta is None or ((cu is None or cu is q_meta.cu_seqlens) and (tokens is None or tokens is q_meta.token_indices))
     if q_ is q and k_ is k and wq is q_weight and wk is k_weight and cos is cos_ and sin is sin_ and idx is idx_ and own:
         if len(memo) >= _MEMO_MAX:

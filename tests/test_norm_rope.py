@@ -544,3 +544,96 @@ def test_rows_past_32_bits(device):
         dx, dy = torch.autograd.grad((c, d), (x, y), (x.detach(), y.detach()))
         for big, small in ((a, c), (b, d), (dq, dx), (dk, dy)):
             assert torch.equal(big[:, :, part], small)
+
+
+def _hooked_layer(device, dtype, seed=3):
+    """A layer whose gains, tables and positions are temporaries: (leaves, function of them, gradients in)"""
+    g = torch.Generator().manual_seed(seed)
+    B, H, N, D, R = 2, 3, 20, 64, 32
+    meta = build_pack_metadata(torch.tensor([20, 9], device=device), N, 32) if device.type == "cuda" else None
+    q, k, dq, dk = (torch.randn((B, H, N, D), generator=g).to(dtype).to(device) for _ in range(4))
+    w = (1 + 0.2 * torch.randn((2, H, D), generator=g)).to(device)
+
+    def layer(q, k, w):
+        cos, sin = _tables(N + 40, R, device)
+        if meta is None:
+            where = dict(positions=(torch.arange(B * N, device=device) % 50).view(B, N) + 3)
+        else:
+            where = dict(q_meta=meta, context_lens=torch.tensor([5, 30], device=device))
+        wide = torch.stack([w, w], -1).to(dtype)[..., 0]  # a strided temporary: copied inside the call
+        return qk_norm_rope(q, k, q_weight=wide[0], k_weight=wide[1], cos=cos, sin=sin, eps=1e-5, **where)
+
+    for t in (q, k, w):
+        t.requires_grad_()
+    return (q, k, w), layer, (dq, dk)
+
+
+def test_backward_reads_what_autograd_kept(monkeypatch):
+    """Saved tensors may come back at other addresses (checkpoints, offload hooks): the gradient's block
+    holds those, not the forward's."""
+    import ctypes
+
+    from flash_mlm.host import norm_rope as nr
+
+    blocks = []
+
+    def run(entry, name, p, device):
+        def at(ptr, n, ctype):
+            return list((ctype * n).from_address(ptr)) if ptr else None
+
+        rows = p.rows * p.D
+        blocks.append((name, [at(t.x, t.heads * rows, ctypes.c_float) for t in (p.q, p.k)],
+                       [at(t.weight, t.heads * p.D, ctypes.c_float) for t in (p.q, p.k)],
+                       [at(x, p.table_rows * p.rotary_dim // 2, ctypes.c_float) for x in (p.cos, p.sin)],
+                       at(p.positions, p.rows, ctypes.c_int64)))
+
+    monkeypatch.setattr(nr, "_run", run)
+    monkeypatch.setattr(nr, "require_cuda_tensors", lambda *t: None)
+    monkeypatch.setattr(nr, "_capture_leaves", lambda *t: [])
+    originals = []
+
+    def pack(t):
+        originals.append(t)
+        return t.detach().clone()
+
+    for unpack in (lambda t: t, lambda t: torch.stack([t, t], -1)[..., 0]):  # as they were, and strided
+        blocks.clear()
+        originals.clear()
+        leaves, layer, dys = _hooked_layer(torch.device("cpu"), torch.float32)
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            out = layer(*leaves)
+        for t in originals:  # their memory belongs to something else by now
+            t.data.fill_(7)
+        torch.autograd.grad(out, leaves, dys)
+        assert [b[0] for b in blocks] == ["fmlm_norm_rope", "fmlm_norm_rope_bwd"]
+        assert blocks[0][1:] == blocks[1][1:]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.flatten()[:8]):
+        out = layer(*_hooked_layer(torch.device("cpu"), torch.float32)[0])
+    with pytest.raises(RuntimeError, match="saved tensor"):
+        out[0].sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("way", ["checkpoint", "clone", "strided", "cpu"])
+def test_gradients_of_checkpointed_and_hooked_calls(dtype, way, device):
+    from torch.utils.checkpoint import checkpoint
+
+    leaves, layer, dys = _hooked_layer(device, DT[dtype])
+    want = torch.autograd.grad(layer(*leaves), leaves, dys)
+    if way == "checkpoint":
+        out = checkpoint(layer, *leaves, use_reentrant=False)
+    else:
+        pack, unpack = {"clone": (lambda t: t.clone(), lambda t: t), "cpu": (lambda t: t.cpu(), lambda t: t.to(device)),
+                        "strided": (lambda t: torch.stack([t, t], -1), lambda t: t[..., 0])}[way]
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            out = layer(*leaves)
+    spoil = [torch.full((n,), float("nan"), device=device) for n in (32, 96, 192, 480, 960, 1920, 7680) for _ in range(40)]
+    got = torch.autograd.grad(out, leaves, dys)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    del spoil
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.cpu()):
+        out = layer(*leaves)
+    with pytest.raises(RuntimeError, match="another device"):
+        torch.autograd.grad(out, leaves, dys)
