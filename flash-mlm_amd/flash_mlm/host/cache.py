@@ -439,7 +439,8 @@ class InferenceCache:
         [H_kv * T, D]; ``q_meta`` describes them and ``plan`` (:func:`build_block_table`, shared
         by all layers of a step) says where they go.  Tokens with slot -1, or one outside the
         pool, are not stored.  The rows are written into the pool in place by one HIP launch,
-        stream-ordered, without a gradient; nothing is read back.  Afterwards the entry has the
+        stream-ordered, without a gradient; nothing is read back.  To autograd that is a change in place:
+        the backward of an earlier call on the pool has to run before it.  Afterwards the entry has the
         plan's block table and context lengths: attend before appending, or the new tokens are
         both context and main keys.
         """
@@ -478,6 +479,9 @@ class InferenceCache:
         if t > 0:
             paged_append(pairs, heads=h_kv, d=d, q_meta=q_meta, slots=slots.contiguous(),
                          pool_rows=int(entry.total_context_len))
+            for _, pool in pairs:  # written behind autograd's back: what it saved of them is stale
+                if not pool.is_inference():
+                    torch.autograd.graph.increment_version(pool)
         self._layer_kv[key] = LayerKVEntry(
             k_cache=entry.k_cache,
             v_cache=entry.v_cache,

@@ -413,3 +413,60 @@ def test_appended_context_is_what_attention_reads(device):
     assert np.diff(plan2.cu_seqlens_kv.tolist()).tolist() == [91, 3, 51]
     c = flash_attn_mlm_compressed(q1, k1, v1, H, meta1, 0.1, cache, 0)
     assert not torch.equal(a, c) and bool(c.isfinite().all())
+
+
+def test_append_is_a_change_in_place_to_autograd(monkeypatch):
+    """What was saved of the pools before an append is refused in a backward after it."""
+    from flash_mlm.host import paged
+
+    calls = []
+    monkeypatch.setattr(paged, "paged_append", lambda pairs, **kw: calls.append(len(pairs)))
+    for mla in (False, True):
+        for inference in (False, True):
+            with torch.inference_mode(inference):
+                pages = torch.zeros((1 if mla else 2, 3, PAGE, 16), dtype=torch.float16)
+                vpages = None if mla else pages.clone()
+                k = torch.zeros((2, 2, 2, 16), dtype=torch.float16)
+            table, zero = torch.zeros((2, 1), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+            cache = InferenceCache()
+            cache.prefill_paged_kv_cache(0, k_pages=pages, v_pages=vpages, block_table=table, context_lens=zero, is_mla=mla,
+                                         num_heads=2, head_dim=16)
+
+            def append(lens):
+                plan = PagedMetadata(table, torch.zeros(sum(lens), dtype=torch.int64), None, zero,
+                                     torch.zeros(3, dtype=torch.int32))
+                cache.append_paged_kv_cache(0, k=k, v=k, q_meta=_cpu_meta(lens, 2), plan=plan)
+
+            if inference:  # these count no versions
+                append([2, 1])
+                continue
+            saved = [torch.ones(t.shape, requires_grad=True) * t for t in (pages, vpages) if t is not None]
+            before = pages._version
+            append([0, 0])  # nothing is written
+            assert pages._version == before
+            append([2, 1])
+            assert pages._version > before and (mla or vpages._version > 0)
+            for x in saved:
+                with pytest.raises(RuntimeError, match="modified by an inplace"):
+                    x.sum().backward()
+    assert calls == [2, 2, 1, 1]
+
+
+@pytest.mark.gpu
+def test_backward_after_an_append_is_refused(device):
+    """Attention's backward reads the pool again: after an append it raises, as after any change in
+    place, instead of differentiating the new rows."""
+    H, D, N = 3, 64, 20
+    k, v, meta, plan, kp, vp, cache = _append_case(device, torch.bfloat16, H, D, False, [20, 1, 0, 13], N, False, False, 6)
+    q = torch.randn((4, H, N, D), device=device).bfloat16().requires_grad_()
+
+    def attend():
+        return flash_attn_mlm_compressed(q, k, v, H, meta, 0.125, cache, 0)
+
+    want = torch.autograd.grad(attend().sum(), q)[0]
+    out, other = attend(), attend()
+    assert torch.equal(torch.autograd.grad(other.sum(), q)[0], want)
+    cache.append_paged_kv_cache(0, k=k, v=v, q_meta=meta, plan=plan)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.sum().backward()
+    assert torch.autograd.grad(attend().sum(), q)[0].isfinite().all()
