@@ -301,7 +301,7 @@ def qk_norm_rope(
     cos_, sin_ = cos, sin
     memo = _MEMO if q_meta is None else q_meta.launch_memo
     key = ("norm_rope", _layout(q), _layout(k), _layout(q_weight), _layout(k_weight), _layout(cos), _layout(sin),
-           _layout(idx), positions is None, eps, norm, interleaved, num_heads)
+           _layout(idx), positions is None, positions is None or context_lens is None, eps, norm, interleaved, num_heads)
     m = memo.get(key)
     if m is not None and m.fits(q_meta):
         call = m.call_for(q_weight, k_weight, cos, sin, idx, positions is None)

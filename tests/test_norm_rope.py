@@ -637,3 +637,29 @@ def test_gradients_of_checkpointed_and_hooked_calls(dtype, way, device):
         out = layer(*leaves)
     with pytest.raises(RuntimeError, match="another device"):
         torch.autograd.grad(out, leaves, dys)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+def test_refusals_after_a_legal_call(packed, device):
+    """A wrong call is refused whatever ran before it: also when all but its fault is like an earlier call"""
+    meta = build_pack_metadata(torch.tensor([5, 2], device=device), 5, 32)
+    q = torch.randn((21, 64) if packed else (2, 3, 5, 64), device=device)
+    cos, sin = _tables(8, 64, device)
+    pos, starts = torch.zeros(7, dtype=torch.int32, device=device), torch.zeros(2, dtype=torch.int32, device=device)
+    for q_meta in (meta, None):
+        kw = dict(cos=cos, sin=sin, q_meta=q_meta)
+        at = pos if q_meta is not None or packed else torch.zeros((2, 5), dtype=torch.int32, device=device)
+        if q_meta is None and packed:
+            kw["num_heads"] = 3
+        for _ in range(2):
+            qk_norm_rope(q, q, positions=at, **kw)
+            for bad in (starts, torch.zeros(9, device=device), [1, 2]):
+                with pytest.raises(ValueError, match="exclusive"):
+                    qk_norm_rope(q, q, positions=at, context_lens=bad, **kw)
+            with pytest.raises(ValueError, match="come together"):
+                qk_norm_rope(q, q, positions=at, **{**kw, "sin": None})
+            with pytest.raises(ValueError, match="shape"):
+                qk_norm_rope(q, q, positions=at.float(), **kw)
+            with pytest.raises(ValueError, match="gains need"):
+                qk_norm_rope(q, q, positions=at, norm=False, q_weight=torch.ones(64, device=device), **kw)
