@@ -163,7 +163,7 @@ def flash_attn_mlm_tree(
         # all that the checks below depend on
         key = ("tree", _tkey(q), _tkey(k), _tkey(v), _tkey(mask), num_heads, q_meta.B, q_meta.N, q_meta.total_tokens,
                float(scale), is_mla, context_batch_size, tile_config_value(), None if entry is None else id(entry),
-               inference_cache is None)
+               inference_cache is None, layer_id is None)
         m = _memo_lookup(memo, key, entry)
         if m is not None:
             return _memo_run(m, q, k, v, entry, wrap=lambda plan: TreeLaunch.of(plan, mask))[0]

@@ -689,3 +689,25 @@ def test_layers_of_one_metadata_with_other_contexts(kind, order, device):
                     _close(got[h, part], q[b, h], k[b, h], v[b, h], seen[part], D**-0.5, rows[b][0][h], rows[b][1][h],
                            torch.bfloat16)
             assert bool(got.isfinite().all())
+
+
+@pytest.mark.gpu
+def test_refusals_after_legal_calls(device):
+    """A wrong call is refused whatever ran before it."""
+    meta = build_pack_metadata(torch.tensor([3, 1], device=device), 3, 32)
+    tree = build_tree_metadata(torch.tensor([-1, 0, 0, -1], device=device), meta)
+    q = torch.randn((2, 2, 3, 64), device=device).bfloat16()
+    cache, _, _ = _context("packed", [5, 70], 2, 64, False, torch.bfloat16, device)
+    for _ in range(2):
+        flash_attn_mlm_tree(q, q, q, 2, meta, tree, 1.0)
+        flash_attn_mlm_tree(q, q, q, 2, meta, tree, 1.0, cache, "no such layer")
+        flash_attn_mlm_tree(q, q, q, 2, meta, tree, 1.0, cache, 0)
+        for args in ((None, 0), (cache, None)):
+            with pytest.raises(ValueError, match="provided together"):
+                flash_attn_mlm_tree(q, q, q, 2, meta, tree, 1.0, *args)
+        with pytest.raises(ValueError, match="num_heads"):
+            flash_attn_mlm_tree(q, q, q, 1, meta, tree, 1.0)
+        with pytest.raises(ValueError, match="tree.mask"):
+            flash_attn_mlm_tree(q, q, q, 2, meta, TreeMetadata(tree.mask[:3], None), 1.0)
+        with pytest.raises(ValueError, match="no backward"):
+            flash_attn_mlm_tree(q.clone().requires_grad_(), q, q, 2, meta, tree, 1.0)
