@@ -471,6 +471,8 @@ class InferenceCache:
         if table.ndim != 2 or table.dtype != torch.int32 or int(table.shape[0]) < 1 \
                 or cu.dtype != torch.int32 or tuple(cu.shape) != (int(table.shape[0]) + 1,):
             raise ValueError("plan.block_table must be rank-2 int32 and plan.cu_seqlens_kv have a row more than it")
+        if int(table.shape[0]) != int(q_meta.B):
+            raise ValueError("plan and q_meta must have the same number of requests")
         dev = entry.device
         if slots.device != dev or table.device != dev or cu.device != dev or q_meta.token_indices.device != dev:
             raise ValueError("plan and q_meta must be on the cached entry's device")

@@ -470,3 +470,19 @@ def test_backward_after_an_append_is_refused(device):
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         out.sum().backward()
     assert torch.autograd.grad(attend().sum(), q)[0].isfinite().all()
+
+
+@pytest.mark.parametrize("b", [1, 3, 5])
+def test_append_refuses_the_plan_of_another_step(b):
+    """A plan for another number of requests than q_meta has"""
+    pages = torch.zeros((2, 3, PAGE, 16), dtype=torch.float16)
+    k, zero = torch.zeros((2, 2, 2, 16), dtype=torch.float16), torch.zeros(2, dtype=torch.int32)
+    cache = InferenceCache()
+    cache.prefill_paged_kv_cache(0, k_pages=pages, v_pages=pages.clone(), block_table=zero.view(2, 1), context_lens=zero,
+                                 is_mla=False, num_heads=2, head_dim=16)
+    entry = cache.layer_entry(0)
+    plan = PagedMetadata(torch.zeros((b, 1), dtype=torch.int32), torch.zeros(3, dtype=torch.int64), None,
+                         torch.zeros(b, dtype=torch.int32), torch.zeros(b + 1, dtype=torch.int32))
+    with pytest.raises(ValueError, match="requests"):
+        cache.append_paged_kv_cache(0, k=k, v=k, q_meta=_cpu_meta([2, 1], 2), plan=plan)
+    assert cache.layer_entry(0) is entry
