@@ -13,6 +13,7 @@ from dataclasses import dataclass
 from typing import TYPE_CHECKING
 
 import torch
+from torch.autograd import forward_ad
 
 from flash_mlm import _lib
 from flash_mlm.host.cache import InferenceCache, PackMetadata
@@ -54,6 +55,15 @@ def pack_indices(q_meta: PackMetadata, device: torch.device) -> tuple[torch.Tens
     if cu.numel() != q_meta.B + 1 or tokens.numel() != q_meta.total_tokens:
         raise ValueError("q_meta: cu_seqlens or token_indices do not match its B and total_tokens")
     return cu, tokens
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """ValueError for a tensor with a forward-mode tangent: a kernel would drop it without a word."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{what} has no forward-mode derivative")
 
 
 class _NullScope:

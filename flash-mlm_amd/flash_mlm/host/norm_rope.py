@@ -15,7 +15,7 @@ import torch
 from flash_mlm import _lib
 from flash_mlm.host.cache import PackMetadata
 from flash_mlm.host.host import rows16
-from flash_mlm.host.host_utils import pack_indices, require_cuda_tensors, validate_head_dim_supported
+from flash_mlm.host.host_utils import pack_indices, refuse_tangents, require_cuda_tensors, validate_head_dim_supported
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _INTS = (torch.int32, torch.int64)
@@ -291,7 +291,8 @@ def qk_norm_rope(
     not read back, and the kernel clamps them to the tables.
 
     With ``q_meta``, rows of padding tokens come out as zeros, whatever they held.
-    Differentiable in q, k and the gains; gradients of padding rows are zero.  A call that is
+    Differentiable in q, k and the gains; gradients of padding rows are zero.  No forward-mode
+    derivative: inputs with a tangent raise ValueError.  A call that is
     captured into a graph and takes leaves that require grad raises ValueError while
     outputs of earlier calls on them are alive (autograd would run part of a captured backward
     on their stream); capture a forward alone under ``torch.no_grad()``.
@@ -438,6 +439,7 @@ def qk_norm_rope(
 
 
 def _apply(call: _Call, q, k, wq, wk, cos, sin, positions, context_lens):
+    refuse_tangents("qk_norm_rope", q, k, wq, wk, cos, sin)
     if torch.is_grad_enabled():
         if cos is not None and (cos.requires_grad or sin.requires_grad):
             raise ValueError("cos and sin are constants: qk_norm_rope has no gradient of them")

@@ -34,6 +34,7 @@ from flash_mlm.host.host_utils import (
     _require_device,
     make_contiguous,
     pack_indices,
+    refuse_tangents,
     require_cuda_tensors,
     validate_cache_request,
     validate_cu_seqlens_rank1_min2,
@@ -153,10 +154,13 @@ def flash_attn_mlm_tree(
     is, and a row that sees no key at all is zero.  Context, ``is_mla`` and ``context_index`` are as in
     :func:`flash_attn_mlm_compressed`; at most 256 tokens a sequence.  The context is not
     changed: store the accepted tokens with :meth:`InferenceCache.append_paged_kv_cache`.
-    No gradients: inputs that require grad raise ValueError (use ``torch.no_grad()``).
+    No gradients: inputs that require grad raise ValueError (use ``torch.no_grad()``), those with
+    a forward-mode tangent too.
     """
     memo, entry, mask = q_meta.launch_memo, _entry_of(inference_cache, layer_id), tree.mask
-    if _wants_grad(q, k, v, *((entry.k_cache, entry.v_cache) if entry is not None else ())):
+    context = (entry.k_cache, entry.v_cache) if entry is not None else ()
+    refuse_tangents("flash_attn_mlm_tree", q, k, v, *context)
+    if _wants_grad(q, k, v, *context):
         raise ValueError("flash_attn_mlm_tree has no backward; call it under torch.no_grad()")
     key = None
     if context_index is None and all(isinstance(t, torch.Tensor) for t in (q, k, v, mask)):

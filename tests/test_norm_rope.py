@@ -589,6 +589,7 @@ def test_backward_reads_what_autograd_kept(monkeypatch):
 
     monkeypatch.setattr(nr, "_run", run)
     monkeypatch.setattr(nr, "require_cuda_tensors", lambda *t: None)
+    monkeypatch.setattr(nr, "_MEMO", {})  # (real calls must not find these)
     monkeypatch.setattr(nr, "_capture_leaves", lambda *t: [])
     originals = []
 
@@ -663,3 +664,45 @@ def test_refusals_after_a_legal_call(packed, device):
                 qk_norm_rope(q, q, positions=at.float(), **kw)
             with pytest.raises(ValueError, match="gains need"):
                 qk_norm_rope(q, q, positions=at, norm=False, q_weight=torch.ones(64, device=device), **kw)
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_refuses_tangents(which, monkeypatch):
+    """Forward-mode tangents are refused, not dropped, in a first call and in one like an earlier one"""
+    from flash_mlm.host import norm_rope as nr
+    from torch.autograd import forward_ad as fw
+
+    monkeypatch.setattr(nr, "_run", lambda *a: None)
+    monkeypatch.setattr(nr, "require_cuda_tensors", lambda *t: None)
+    monkeypatch.setattr(nr, "_MEMO", {})  # (real calls must not find these)
+    cos, sin = _tables(8, 32, "cpu")
+    args = [torch.randn(1, 2, 3, 64), torch.randn(1, 2, 3, 64), torch.ones(64), torch.ones(64), cos, sin]
+
+    def call(a):
+        return qk_norm_rope(a[0], a[1], q_weight=a[2], k_weight=a[3], cos=a[4], sin=a[5], eps=1e-5 * (1 + which))
+
+    for _ in range(2):
+        with fw.dual_level():
+            dual = list(args)
+            dual[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
+            with pytest.raises(ValueError, match="forward-mode"):
+                call(dual)
+            call(args)
+        call(args)
+
+
+@pytest.mark.gpu
+def test_refuses_tangents_on_the_gpu(device):
+    from torch.autograd import forward_ad as fw
+
+    q = torch.randn((1, 2, 3, 64), device=device)
+    want = qk_norm_rope(q, q)
+    with fw.dual_level():
+        dual = fw.make_dual(q, torch.ones_like(q))
+        for x in (dual, dual.detach().requires_grad_(), dual.transpose(1, 2).contiguous().transpose(1, 2)):
+            if x is dual or fw.unpack_dual(x).tangent is not None:
+                with pytest.raises(ValueError, match="forward-mode"):
+                    qk_norm_rope(x, q)
+        assert torch.equal(qk_norm_rope(q, q)[0], want[0])
+    with pytest.raises(Exception):
+        torch.func.jvp(lambda x: qk_norm_rope(x, q)[0], (q,), (torch.ones_like(q),))

@@ -711,3 +711,24 @@ def test_refusals_after_legal_calls(device):
             flash_attn_mlm_tree(q, q, q, 2, meta, TreeMetadata(tree.mask[:3], None), 1.0)
         with pytest.raises(ValueError, match="no backward"):
             flash_attn_mlm_tree(q.clone().requires_grad_(), q, q, 2, meta, tree, 1.0)
+
+
+def test_refuses_tangents():
+    from torch.autograd import forward_ad as fw
+
+    meta = _cpu_meta([2, 1], 2)
+    tree = TreeMetadata(torch.zeros((3, 1), dtype=torch.int64), torch.zeros(3, dtype=torch.int32))
+    with fw.dual_level():
+        args = [torch.zeros((2, 2, 2, 64), dtype=torch.float16) for _ in range(3)]
+        for i in range(3):
+            some = list(args)
+            some[i] = fw.make_dual(args[i], args[i])
+            with pytest.raises(ValueError, match="forward-mode"):
+                flash_attn_mlm_tree(*some, 2, meta, tree, 1.0)
+        pool = torch.zeros((2, 1, PAGE, 64), dtype=torch.float16)
+        cache = InferenceCache()
+        cache.prefill_paged_kv_cache(0, k_pages=pool, v_pages=fw.make_dual(pool.clone(), pool), is_mla=False, num_heads=2,
+                                     block_table=torch.zeros((2, 1), dtype=torch.int32), head_dim=64,
+                                     context_lens=torch.zeros(2, dtype=torch.int32))
+        with pytest.raises(ValueError, match="forward-mode"):
+            flash_attn_mlm_tree(*args, 2, meta, tree, 1.0, cache, 0)
