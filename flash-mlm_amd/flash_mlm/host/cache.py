@@ -27,7 +27,8 @@ class PackMetadata:
     the launchers size padded workspaces without a device-to-host synchronisation.
     ``kernel_schedules`` caches the attention kernel's device work lists built from
     ``cu_seqlens`` (one per kernel tile size), so repeated layers skip rebuilding them;
-    ``launch_memo`` the parameter blocks of earlier compressed calls on this metadata.
+    ``launch_memo`` the parameter blocks of earlier compressed calls on this metadata.  Both
+    are used only with the ``cu_seqlens`` tensor that they were made with.
     """
 
     B: int

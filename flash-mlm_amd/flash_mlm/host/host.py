@@ -188,13 +188,14 @@ def _tkey(t: torch.Tensor):
 
 
 class _Memo:
-    __slots__ = ("params", "entry_ref", "extra", "out_shape", "repack", "unpack_kv", "records")
+    __slots__ = ("params", "entry_ref", "extra", "out_shape", "repack", "unpack_kv", "records", "cu")
 
-    def __init__(self, plan: AttnLaunch, entry, extra, out_shape, repack=None):
+    def __init__(self, plan: AttnLaunch, entry, extra, out_shape, repack=None, cu=None):
         self.params = _lib.AttnParams.from_buffer_copy(plan.params)
         self.entry_ref = None if entry is None else weakref.ref(entry)
-        self.extra, self.out_shape, self.repack, self.unpack_kv = extra, out_shape, repack, plan.unpack_kv
-        self.records = plan.records
+        self.out_shape, self.repack, self.unpack_kv, self.records = out_shape, repack, plan.unpack_kv, plan.records
+        self.cu = cu  # the metadata's cu_seqlens, which can be replaced
+        self.extra = (extra, plan.keep[11])  # and the schedule, which another's may take the place of
 
 
 def _entry_of(inference_cache: InferenceCache | None, layer_id):
@@ -203,9 +204,9 @@ def _entry_of(inference_cache: InferenceCache | None, layer_id):
     return inference_cache.layer_entry(layer_id)
 
 
-def _memo_lookup(memo: dict, key, entry) -> _Memo | None:
+def _memo_lookup(memo: dict, key, entry, cu=None) -> _Memo | None:
     m = memo.get(key)
-    if m is None:
+    if m is None or m.cu is not cu:
         return None
     if (m.entry_ref() if m.entry_ref is not None else None) is not entry:
         return None
@@ -439,6 +440,7 @@ def _prepare(
     flags: int,
     inference_cache: InferenceCache | None,
     schedule_cache: dict | None = None,
+    schedule_of: torch.Tensor | None = None,
     ctx_index: torch.Tensor | None = None,
     block_table: torch.Tensor | None = None,
     page_stride: int = 0,
@@ -494,12 +496,13 @@ def _prepare(
             p.flags |= _lib.FLAG_OWN_RECORDS
         key = (p.dtype, D, B, H, N, total_q, p.flags, p.kv_layout, block_table is not None, p.tile_config)
         sched = schedule_cache.get(key)
-        if sched is None:
+        if sched is None or sched.schedule_of is not schedule_of:  # (a metadata's cu_seqlens can be replaced)
             nbytes = ws_bytes - records
             sched = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
             with _device_scope(q.device):
                 rc = lib.fmlm_attn_schedule(p, sched.data_ptr(), nbytes, stream)
             _lib.check(rc, "fmlm_attn_schedule")
+            sched.schedule_of = schedule_of
             schedule_cache[key] = sched
         p.schedule = sched.data_ptr()
     elif ws_bytes > 0:
@@ -777,7 +780,7 @@ def _compressed_impl(
                     block_n, auto_tune_tiles, causal_query_seq_attn, _TILE_CONFIG,
                     None if entry is None else id(entry), inference_cache is None,
                     owned_buffers and causal_query_seq_attn)
-        m = _memo_lookup(memo, memo_key, entry)
+        m = _memo_lookup(memo, memo_key, entry, q_meta.cu_seqlens)
         if m is not None:
             res = _memo_run(m, q, k, v, entry)
             if res is not None:
@@ -944,6 +947,7 @@ def _compressed_impl(
         flags=flags,
         inference_cache=inference_cache,
         schedule_cache=q_meta.kernel_schedules if isinstance(q_meta, PackMetadata) else None,
+        schedule_of=cu_seqlens_q,
         ctx_index=ctx_index,
         block_table=ctx.block_table,
         page_stride=_page_stride(ctx, num_heads, d, is_mla),
@@ -957,7 +961,7 @@ def _compressed_impl(
                                     cu_q=cu_q)
         # the offsets the launch reads when they are not the metadata's or the entry's own
         extra = (cu_q, cu_kv, k_cache if entry is None else None, v_cache if entry is None else None)
-        _memo_store(memo, memo_key, _Memo(plan, entry, extra, tuple(out.shape), repack))
+        _memo_store(memo, memo_key, _Memo(plan, entry, extra, tuple(out.shape), repack, cu_seqlens_q))
     return out, plan
 
 

@@ -168,7 +168,7 @@ def flash_attn_mlm_tree(
         key = ("tree", _tkey(q), _tkey(k), _tkey(v), _tkey(mask), num_heads, q_meta.B, q_meta.N, q_meta.total_tokens,
                float(scale), is_mla, context_batch_size, tile_config_value(), None if entry is None else id(entry),
                inference_cache is None, layer_id is None)
-        m = _memo_lookup(memo, key, entry)
+        m = _memo_lookup(memo, key, entry, q_meta.cu_seqlens)
         if m is not None:
             return _memo_run(m, q, k, v, entry, wrap=lambda plan: TreeLaunch.of(plan, mask))[0]
     b, h, n, d = validate_qkv_same_shape_rank4(q, k, v, error_prefix="q/k/v")
@@ -256,6 +256,7 @@ def flash_attn_mlm_tree(
         flags=_lib.FLAG_TREE | (_lib.FLAG_MLA if is_mla else 0),
         inference_cache=inference_cache,
         schedule_cache=dict(q_meta.kernel_schedules) if capturing else q_meta.kernel_schedules,
+        schedule_of=q_meta.cu_seqlens,
         ctx_index=ctx_index,
         block_table=ctx.block_table,
         page_stride=_page_stride(ctx, num_heads, d, is_mla),
@@ -264,5 +265,5 @@ def flash_attn_mlm_tree(
     if (key is not None and not capturing and q_ is q and k_ is k and v_ is v and k_cache is ctx.k_cache and v_cache is ctx.v_cache
             and plan.keep[10] is None and mask.is_contiguous()):
         extra = (cu_q, cu_kv, k_cache if entry is None else None, v_cache if entry is None else None)
-        _memo_store(memo, key, _Memo(plan, entry, extra, tuple(out.shape)))
+        _memo_store(memo, key, _Memo(plan, entry, extra, tuple(out.shape), cu=q_meta.cu_seqlens))
     return out

@@ -732,3 +732,49 @@ def test_refuses_tangents():
                                      context_lens=torch.zeros(2, dtype=torch.int32))
         with pytest.raises(ValueError, match="forward-mode"):
             flash_attn_mlm_tree(*args, 2, meta, tree, 1.0, cache, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, kind, D, mla", [("bf16", "paged", 64, False), ("fp16", "packed", 512, True),
+                                                 ("fp32", "packed", 64, False)])
+@pytest.mark.parametrize("first", [[40, 1, 23], [23, 40, 1]])
+def test_metadata_whose_fields_were_replaced(first, dtype, kind, D, mla, device):
+    """Parameter blocks and schedules kept on a metadata are those of its index tensors: other offsets
+    (as many tokens), other integer types, and the first offsets again"""
+    import dataclasses
+
+    from flash_mlm import flash_attn_mlm_compressed
+
+    H, N, ctx = 3, 40, [3000, 70, 200]
+    second = first[1:] + first[:1]
+    g = torch.Generator().manual_seed(11)
+    q, k, v = (torch.randn((3, H, N, D), generator=g).to(DT[dtype]).to(device) for _ in range(3))
+    v = k if mla else v
+    cache, _, _ = _context(kind, ctx, H, D, mla, DT[dtype], device, 2)
+
+    def calls(meta, tree):
+        return (flash_attn_mlm_tree(q, k, v, H, meta, tree, D**-0.5, cache, 0, is_mla=mla),
+                flash_attn_mlm_compressed(q, k, v, H, meta, D**-0.5, cache, 0, is_mla=mla))
+
+    fresh = [build_pack_metadata(torch.tensor(lens, device=device), N, 32) for lens in (first, second)]
+    trees = [build_tree_metadata(torch.tensor([i - 1 for n in lens for i in range(n)], device=device), m)
+             for lens, m in zip((first, second), fresh)]
+    want = [[x.clone() for x in calls(m, t)] for m, t in zip(fresh, trees)]
+    assert not torch.equal(want[0][0], want[1][0])
+    meta = build_pack_metadata(torch.tensor(first, device=device), N, 32)
+    shared = dataclasses.replace(meta, cu_seqlens=fresh[1].cu_seqlens, token_indices=fresh[1].token_indices)
+
+    def put(i, cast=lambda t: t):
+        for f in ("lengths", "cu_seqlens", "token_indices", "batch_ids_q", "q_tile_starts_q"):
+            setattr(meta, f, cast(getattr(fresh[i], f)))
+
+    for i in (0, 0, 1, 1, 0, 1):
+        put(i)
+        for a, b in zip(calls(meta, trees[i]), want[i]):
+            assert torch.equal(a, b)
+        for a, b in zip(calls(shared, trees[1]), want[1]):  # a copy that shares what is kept
+            assert torch.equal(a, b)
+    put(0, lambda t: t.long())
+    for _ in range(2):
+        for a, b in zip(calls(meta, trees[0]), want[0]):
+            assert torch.equal(a, b)
