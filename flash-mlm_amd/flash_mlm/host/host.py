@@ -917,6 +917,10 @@ def _compressed_impl(
         | (_lib.FLAG_PREFILL if prefill else 0)
         | (_lib.FLAG_CAUSAL_SEQ if causal_query_seq_attn else 0)
     )
+    # a schedule or parameter block made during a capture lives in the graph's memory and is filled
+    # by its replays: it stays this call's own
+    kept = q_meta.kernel_schedules if isinstance(q_meta, PackMetadata) else None
+    capturing = kept is not None and torch.cuda.is_current_stream_capturing()
     plan = _launch(
         run=run,
         q=q_,
@@ -946,14 +950,14 @@ def _compressed_impl(
         scale=scale,
         flags=flags,
         inference_cache=inference_cache,
-        schedule_cache=q_meta.kernel_schedules if isinstance(q_meta, PackMetadata) else None,
+        schedule_cache=dict(kept) if capturing else kept,
         schedule_of=cu_seqlens_q,
         ctx_index=ctx_index,
         block_table=ctx.block_table,
         page_stride=_page_stride(ctx, num_heads, d, is_mla),
     )
     plan.unpack_kv = unpack_kv
-    if (memo_key is not None and q_ is q and k_cache is ctx.k_cache and v_cache is ctx.v_cache
+    if (memo_key is not None and not capturing and q_ is q and k_cache is ctx.k_cache and v_cache is ctx.v_cache
             and plan.keep[10] is None and (causal_query_seq_attn or (k_ is k and v_ is v))):
         repack = None
         if causal_query_seq_attn:

@@ -1187,3 +1187,30 @@ def test_mla_latent512_dense(cbs, device):
     ref = ar.mlm_attention_dense(_np(q), _np(k), _np(k), 1.0 / math.sqrt(D), is_mla=True, k_cache=_np(kc),
                                  context_len=C, context_batch_size=cbs)
     _close(out, ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D, mla", [(64, False), (512, True)])
+def test_first_packed_call_of_a_metadata_in_a_graph(D, mla, causal, device):
+    """A capture leaves no schedule or parameter block on the metadata that only its replays fill: an
+    eager call before the first replay, and the replays, give what an eager call gives."""
+    H, N, lens = 4, 20, [20, 3]
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn((2, H, N, D), generator=g).bfloat16().to(device) for _ in range(3))
+    metas = [build_pack_metadata(torch.tensor(lens, device=device), N, 32) for _ in range(2)]
+
+    def call(meta):
+        return flash_attn_mlm_compressed(q, k, v, H, meta, 0.125, is_mla=mla, causal_query_seq_attn=causal)
+
+    want = call(metas[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(metas[1])
+    assert not metas[1].kernel_schedules and not metas[1].launch_memo
+    assert torch.equal(call(metas[1]), want)
+    for _ in range(3):
+        out.fill_(5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(call(metas[1]), want)
