@@ -113,6 +113,29 @@ def _torch_stream(handle: int, device: torch.device):
     return torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
 
 
+class _Made:
+    """The point on a stream at which something that later calls share (a schedule, derived offsets)
+    has been made on the GPU."""
+
+    __slots__ = ("event", "streams")
+
+    def __init__(self, stream: int, device: torch.device):
+        self.event = torch.cuda.Event()
+        self.event.record(torch.cuda.current_stream(device))
+        self.streams = {stream}
+
+    def before(self, stream: int, device: torch.device, tensors) -> None:
+        """Orders the current stream (handle ``stream``) behind it, once, and keeps the tensors' memory
+        for its work.  (A capture began after a synchronisation, and cannot wait for events before it.)"""
+        if stream in self.streams or torch.cuda.is_current_stream_capturing():
+            return
+        current = torch.cuda.current_stream(device)
+        current.wait_event(self.event)
+        for t in tensors:
+            t.record_stream(current)
+        self.streams.add(stream)
+
+
 class AttnLaunch:
     """A prepared fmlm_attn_fwd call: the parameter block plus the tensors it points to."""
 
@@ -188,14 +211,19 @@ def _tkey(t: torch.Tensor):
 
 
 class _Memo:
-    __slots__ = ("params", "entry_ref", "extra", "out_shape", "repack", "unpack_kv", "records", "cu")
+    __slots__ = ("params", "entry_ref", "extra", "out_shape", "repack", "unpack_kv", "records", "cu", "made", "shared")
 
     def __init__(self, plan: AttnLaunch, entry, extra, out_shape, repack=None, cu=None):
         self.params = _lib.AttnParams.from_buffer_copy(plan.params)
         self.entry_ref = None if entry is None else weakref.ref(entry)
         self.out_shape, self.repack, self.unpack_kv, self.records = out_shape, repack, plan.unpack_kv, plan.records
         self.cu = cu  # the metadata's cu_seqlens, which can be replaced
-        self.extra = (extra, plan.keep[11])  # and the schedule, which another's may take the place of
+        sched = plan.keep[11]
+        self.extra = (extra, sched)  # and the schedule, which another's may take the place of
+        # what other streams' calls share: the schedule, and offsets that the call derived
+        self.shared = () if sched is None else (sched, plan.keep[6], plan.keep[7])
+        derived = sched is not None and (plan.keep[6] is not cu or entry is None or plan.keep[7] is not entry.cu_seqlens_kv)
+        self.made = _Made(plan.stream, plan.device) if derived else getattr(sched, "made", None)
 
 
 def _entry_of(inference_cache: InferenceCache | None, layer_id):
@@ -237,7 +265,10 @@ def _memo_run(m: _Memo, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, entry
     keep = [q, out, k, None if mla else v, kc, vc, m.extra]
     if entry is not None:
         keep.append((entry.cu_seqlens_kv, entry.block_table))
-    plan = AttnLaunch(_lib.load(), p, _lib.stream_of(q.device), q.device, tuple(keep))
+    stream = _lib.stream_of(q.device)
+    if m.made is not None:
+        m.made.before(stream, q.device, m.shared)
+    plan = AttnLaunch(_lib.load(), p, stream, q.device, tuple(keep))
     plan.unpack_kv, plan.records = m.unpack_kv, m.records
     if wrap is not None:
         plan = wrap(plan)
@@ -503,7 +534,11 @@ def _prepare(
                 rc = lib.fmlm_attn_schedule(p, sched.data_ptr(), nbytes, stream)
             _lib.check(rc, "fmlm_attn_schedule")
             sched.schedule_of = schedule_of
+            if not torch.cuda.is_current_stream_capturing():
+                sched.made = _Made(stream, q.device)
             schedule_cache[key] = sched
+        else:
+            sched.made.before(stream, q.device, (sched,))
         p.schedule = sched.data_ptr()
     elif ws_bytes > 0:
         ws = _workspace(inference_cache, ws_bytes, q.device)

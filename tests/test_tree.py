@@ -778,3 +778,53 @@ def test_metadata_whose_fields_were_replaced(first, dtype, kind, D, mla, device)
     for _ in range(2):
         for a, b in zip(calls(meta, trees[0]), want[0]):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D, mla, kind", [(64, False, "paged"), (512, True, "packed"), (64, False, "none")])
+@pytest.mark.parametrize("wide", [False, True])
+def test_first_calls_of_a_metadata_on_two_streams(D, mla, kind, wide, device):
+    """The schedule, and offsets that a call derives (``wide``: of int64 metadata), are made on the first
+    call's stream; calls on other streams wait for them, by the memo (layer 0) or without (layer 1)."""
+    from flash_mlm import flash_attn_mlm_compressed
+
+    H, N, lens = 4, 20, [20, 3]
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn((2, H, N, D), generator=g).bfloat16().to(device) for _ in range(3))
+    v = k if mla else v
+    caches = [_context(kind, c, H, D, mla, torch.bfloat16, device, 4)[0] for c in ([1500, 70], [64, 3000])]
+    cast = torch.Tensor.long if wide else lambda t: t
+    parents = torch.tensor([-1] + [0] * 19 + [-1, 0, 1], device=device)
+
+    def fresh():
+        meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+        meta.cu_seqlens = cast(meta.cu_seqlens)
+        return meta, build_tree_metadata(parents, meta)
+
+    def calls(meta, tree, i):
+        args = (caches[i], None if caches[i] is None else 0)
+        return (flash_attn_mlm_tree(q, k, v, H, meta, tree, 0.125, *args, is_mla=mla),
+                flash_attn_mlm_compressed(q, k, v, H, meta, 0.125, *args, is_mla=mla))
+
+    meta, tree = fresh()  # (layer 0's contexts steer where both layers' key ranges are split)
+    want = [calls(meta, tree, i) for i in range(2)]
+    busy = torch.randn((8192, 8192), device=device)
+    for _ in range(3):
+        meta, tree = fresh()
+        streams = [torch.cuda.Stream() for _ in range(3)]
+        torch.cuda.synchronize()
+        got, done = [], torch.cuda.Event()
+        with torch.cuda.stream(streams[0]):
+            for _ in range(4):
+                torch.mm(busy, busy)
+            done.record()
+            got.append((0, calls(meta, tree, 0)))
+        for s in streams[1:]:
+            with torch.cuda.stream(s):
+                got += [(i, calls(meta, tree, i)) for i in (0, 1, 0)]
+        overlapped = not done.query()
+        torch.cuda.synchronize()
+        assert overlapped  # the first stream was still busy when the last call was made
+        for i, outs in got:
+            for a, b in zip(outs, want[i]):
+                assert torch.equal(a, b)
