@@ -214,6 +214,15 @@ def _accumulator(leaf: torch.Tensor):
     return leaf.view_as(leaf).grad_fn.next_functions[0][0]
 
 
+def _lives(leaf: torch.Tensor) -> bool:
+    """Whether another graph than one of this capture holds the leaf's accumulator.  (In a frame of its
+    own: a refusal's traceback must not be what holds it in the next attempt.)"""
+    token = object()
+    _accumulator(leaf).metadata["fmlm_probe"] = token
+    node = _accumulator(leaf)
+    return node.metadata.get("fmlm_probe") is token and "fmlm_captured" not in node.metadata
+
+
 def _capture_leaves(*tensors) -> list[torch.Tensor]:
     """The leaves among ``tensors`` when the current stream is being captured (else none), checked.
 
@@ -222,14 +231,11 @@ def _capture_leaves(*tensors) -> list[torch.Tensor]:
     capture, which ends the process when the capture ends.  An accumulator outlives its
     last reference here exactly when another live graph holds it.
     """
-    if not torch.cuda.is_current_stream_capturing():
+    leaves = [t for t in tensors if isinstance(t, torch.Tensor) and t.requires_grad and t.is_leaf]
+    if not leaves or not torch.cuda.is_current_stream_capturing():
         return []
-    leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
     for t in leaves:
-        token = object()
-        _accumulator(t).metadata["fmlm_probe"] = token
-        node = _accumulator(t)
-        if node.metadata.get("fmlm_probe") is token and "fmlm_captured" not in node.metadata:
+        if _lives(t):
             raise ValueError(
                 "qk_norm_rope is being captured into a graph while another autograd graph of one of its leaves "
                 "lives: drop the outputs of the earlier calls on it first"
@@ -371,6 +377,8 @@ def qk_norm_rope(
     if tokens is not None:
         p.token_indices = tokens.data_ptr()
 
+    # before the copies below, which would hide a leaf and hold its accumulator themselves
+    leaves = _capture_leaves(q, k, q_weight, k_weight) if torch.is_grad_enabled() else []
     flags = 0
     p.w_dtype = _lib.DTYPE_F32
     wq, wk = q_weight, k_weight
@@ -435,17 +443,18 @@ def qk_norm_rope(
         if len(memo) >= _MEMO_MAX:
             memo.clear()
         memo[key] = _Memo(call, q_meta)
-    return _apply(call, q_, k_, wq, wk, cos, sin, positions, context_lens)
+    return _apply(call, q_, k_, wq, wk, cos, sin, positions, context_lens, leaves)
 
 
-def _apply(call: _Call, q, k, wq, wk, cos, sin, positions, context_lens):
+def _apply(call: _Call, q, k, wq, wk, cos, sin, positions, context_lens, leaves=None):
     refuse_tangents("qk_norm_rope", q, k, wq, wk, cos, sin)
     if torch.is_grad_enabled():
         if cos is not None and (cos.requires_grad or sin.requires_grad):
             raise ValueError("cos and sin are constants: qk_norm_rope has no gradient of them")
         if q.requires_grad or k.requires_grad or (wq is not None and wq.requires_grad) \
                 or (wk is not None and wk.requires_grad):
-            leaves = _capture_leaves(q, k, wq, wk)
+            if leaves is None:
+                leaves = _capture_leaves(q, k, wq, wk)
             out = _NormRope.apply(call, q, k, wq, wk, cos, sin, positions, context_lens)
             for t in leaves:  # this capture's own graph: later calls of it may share the leaf
                 _accumulator(t).metadata["fmlm_captured"] = True

@@ -706,3 +706,50 @@ def test_refuses_tangents_on_the_gpu(device):
         assert torch.equal(qk_norm_rope(q, q)[0], want[0])
     with pytest.raises(Exception):
         torch.func.jvp(lambda x: qk_norm_rope(x, q)[0], (q,), (torch.ones_like(q),))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["q", "k", "gain", "packed"])
+def test_captures_of_leaves_that_are_copied(which, device):
+    """A leaf that the call copies for its kernel (an odd start, another stride) is checked as any other: no
+    capture while an eager graph of it lives, and captured gradients replay."""
+    g = torch.Generator().manual_seed(4)
+    B, H, N, D = 2, 3, 9, 64
+
+    def odd(*shape):
+        n = int(np.prod(shape))
+        t = torch.empty(n + 1, dtype=torch.bfloat16, device=device)[1:].view(shape)
+        return t.copy_(torch.randn(shape, generator=g)).requires_grad_()
+
+    shape = (H * B * N, D) if which == "packed" else (B, H, N, D)
+    q, k = (odd(*shape) if which in (n, "packed") else
+            torch.randn(shape, generator=g).bfloat16().to(device).requires_grad_() for n in "qk")
+    w = torch.ones((D, 2), dtype=torch.bfloat16, device=device)[:, 0] if which == "gain" else torch.ones(D, device=device).bfloat16()
+    w.requires_grad_()
+    kw = dict(q_weight=w, k_weight=w, num_heads=H)
+    dys = [torch.randn(shape, generator=g).bfloat16().to(device) for _ in range(2)]
+    leaves = (q, k, w)
+    assert all(t.is_leaf for t in leaves)
+
+    def step():
+        out = qk_norm_rope(q, k, **kw)
+        return [*out, *torch.autograd.grad(out, leaves, dys)]
+
+    alive = qk_norm_rope(q, k, **kw)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(ValueError, match="being captured") as refusal:
+        with torch.cuda.graph(graph):
+            qk_norm_rope(q, k, **kw)
+    del alive  # (the refusal's traceback lives on)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+        twice = step()
+    captured, twice = ([t.detach() for t in x] for x in (captured, twice))
+    for seed in range(3):
+        with torch.no_grad():
+            q.copy_(torch.randn(shape, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b, c in zip(captured, step(), twice):
+            assert torch.equal(a, b) and torch.equal(c, b)
