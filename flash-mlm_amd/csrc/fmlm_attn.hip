@@ -2681,8 +2681,9 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const fmlm_attn_pa
         l[sp] = M == -INFINITY ? 0.f : fast_exp2(m[sp] - M) * l[sp];
         L += l[sp];
       }
-      // L is 0 only where every score of the row is -inf (a row has keys, its own): NaN
-      const float inv = 1.f / L;
+      // L is 0 only where every score of the row is -inf (a row has keys, its own): NaN.  A row of a
+      // tree call may see no key at all: zero, as in an unsplit call
+      const float inv = (p.flags & FMLM_FLAG_TREE) && M == -INFINITY ? 0.f : 1.f / L;
 #pragma unroll
       for (int sp = 0; sp < kMaxSplits; ++sp) s_w[r][sp] = l[sp] * inv;
       if (p.lse) store_lse(p, hq, si.q0, pos, M, L);

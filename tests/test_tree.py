@@ -828,3 +828,37 @@ def test_first_calls_of_a_metadata_on_two_streams(D, mla, kind, wide, device):
         for i, outs in got:
             for a, b in zip(outs, want[i]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, D, kind", [("bf16", 64, "paged"), ("fp16", 128, "packed"), ("bf16", 256, "paged"),
+                                            ("fp32", 64, "packed"), ("fp32", 128, "packed"), ("bf16", 512, "paged")])
+def test_rows_that_see_nothing_in_a_split_call(dtype, D, kind, device):
+    """A schedule cuts sequence 0 for one layer's long context; in the next layer that context is empty, and
+    rows whose masks are empty too are zero, as unsplit rows are."""
+    H, N, lens, mla = 2, 70, [70, 5], D == 512
+    meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+    r = random.Random(D)
+    seen = [set() if i % 3 == 0 else {j for j in range(n) if r.random() < 0.2} - ({i} if i % 2 else set())
+            for n in lens for i in range(n)]
+    tree = TreeMetadata(torch.from_numpy(ref.mask_words(seen, 2)).to(device), None)
+    g = torch.Generator().manual_seed(D)
+    q, k, v = (torch.randn((2, H, N, D), generator=g).to(DT[dtype]).to(device) for _ in range(3))
+    v = k if mla else v
+    for ctx in ([9000, 100], [0, 9000], [9000, 0]):
+        cache, rows, _ = _context(kind, ctx, H, D, mla, DT[dtype], device, 3)
+        for _ in range(2):
+            got = flash_attn_mlm_tree(q, k, v, H, meta, tree, D**-0.5, cache, 0, is_mla=mla).view(H, -1, D)
+            at = 0
+            for b, n in enumerate(lens):
+                some = [i for i in range(n) if seen[at + i] or ctx[b]]
+                none = [at + i for i in range(n) if not seen[at + i] and not ctx[b]]
+                for h in range(H):
+                    j = 0 if mla else h
+                    _close(got[h, [at + i for i in some]], q[b, h, some], k[b, j, :n], v[b, j, :n],
+                           [seen[at + i] for i in some], D**-0.5, rows[b][0][j], rows[b][1][j], DT[dtype])
+                assert not got[:, none].any()
+                at += n
+    # the first layer's schedule was a split one
+    (sched,) = meta.kernel_schedules.values()
+    assert int(sched[:8].view(torch.int32)[1]) > 0
