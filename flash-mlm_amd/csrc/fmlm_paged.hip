@@ -296,11 +296,16 @@ __global__ __launch_bounds__(kBtFillThreads) void block_table_fill_kernel(const 
   bt_fill<false>(p, bt_space(p), (int64_t)blockIdx.x * kBtFillThreads + threadIdx.x, (int64_t)gridDim.x * kBtFillThreads);
 }
 
-// One workgroup up to this many table entries, tokens and requests: beyond it the launches of the
-// other kernels cost less than what one workgroup takes.  64 requests: 64 tokens each 8.5 us against
-// 9.1 (with keep 11.5 against 12.4), 128 each 10.8 against 8.9 (14.8 against 12.7); one token each,
-// tables of 94 pages, 64 requests 8.5 against 8.2, 256 15.1 against 8.3.
-constexpr int64_t kBtSmall = 6144;
+// One workgroup for two rounds of table entries and one of tokens (a round: what its threads fill at
+// once).  A further round of entries takes it 1.2 to 1.8 us, one of tokens 2 and with keep 3; the other kernels
+// cost 1 to 1.5 us more to begin with (with keep, one more, 2), and as much again where the host's launches
+// are what counts.  us a call, one workgroup against the others, in a graph (on a stream):
+//   entries, no keep: 4096 6.3 : 7.1 (6.3 : 8.7), 8192 7.5-8.0 : 7.2-7.5 (7.5-8.0 : 8.7), 9024 8.8 : 7.2 (8.8 : 8.7)
+//   with keep:        8192 10.0-10.5 : 10.4-10.8 (10.0-10.5 : 11.2), 9024 11.3 : 10.7 (11.2 : 11.0)
+//   tokens, no keep:  3100 7.1 : 8.3 (7.1 : 8.7), 6200 8.7 : 7.3 (8.6 : 9.0)
+//   with keep:        3100 10.2 : 12.3 (10.2 : 12.7), 6200 13.0 : 11.5 (12.9 : 11.8)
+constexpr int64_t kBtRound = kBtUnroll * kBtThreads;
+static bool bt_small(int64_t entries, int64_t tokens) { return entries <= 2 * kBtRound && tokens <= kBtRound; }
 
 static int bt_check(const BtParams& p) {
   if (p.B < 0 || p.N < 0 || p.T < 0 || p.max_pages < 0 || p.in_pages < 0 || p.n_free < 0) return FMLM_E_ARG;
@@ -376,7 +381,7 @@ extern "C" int fmlm_block_table(const fmlm_block_table_params* pp, void* stream)
   if (need > 0 && (!p.workspace || p.workspace_bytes < need)) return FMLM_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   const int64_t entries = (int64_t)p.B * p.max_pages, work = std::max<int64_t>(entries, p.T);
-  if (entries + p.T + p.B <= kBtSmall) {
+  if (bt_small(entries, p.T)) {
     hipLaunchKernelGGL(block_table_small_kernel, dim3(1), dim3(kBtThreads), 0, s, p);
     return launch_status();
   }

@@ -486,3 +486,20 @@ def test_append_refuses_the_plan_of_another_step(b):
     with pytest.raises(ValueError, match="requests"):
         cache.append_paged_kv_cache(0, k=k, v=k, q_meta=_cpu_meta([2, 1], 2), plan=plan)
     assert cache.layer_entry(0) is entry
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("B, n, width", [(64, 1, 128), (64, 1, 129), (2048, 1, 4), (2049, 2, 3), (2731, 1, 3), (1, 4096, 70),
+                                         (1, 4097, 70), (4, 1024, 2048), (8192, 0, 1), (4096, 1, 2), (4097, 1, 2)])
+def test_table_around_the_sizes_of_one_workgroup(B, n, width, keep, device):
+    """Two rounds of table entries, one of tokens, more requests than threads: and one more of each"""
+    r = random.Random(B + n + width)
+    lens = [n] * B
+    old = [r.randint(0, min(min(width, 40) * PAGE, width * PAGE - n)) if r.random() < 0.9 else 0 for _ in lens]
+    ids = r.sample(range(10 * B * 40 + 100), B * min(width, 40) + 2 * B + 70)
+    table = [ids[b * min(width, 40) :][: min(width, 40)] + [-1] * (width - min(width, 40)) for b in range(B)]
+    free = ids[B * min(width, 40) :]
+    kept = [r.random() < 0.5 for _ in range(n * B)] if keep else None
+    case = (lens, old, table, free, width, kept)
+    _expect(case, _run_table(case, max(n, 1), device)[1])
