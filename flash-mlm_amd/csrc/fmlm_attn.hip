@@ -2789,9 +2789,12 @@ static Launch mla_rows_launch(const fmlm_attn_params& p) {
                 true, true, mla_rows_fn<T, true, 1>(paged, lse, f32), 3.4f};
 }
 
-// Tree calls take 64-row workgroups: drafts are short.  Longer ones gain nothing from two row
-// blocks a wave (D = 64 and 128, 8 sequences of 64-128 or 120-256 tokens over 4000 rows, 16 heads: 44.6
-// / 61.4 / 61.4 / 89.0 us against 45.8 / 62.0 / 62.8 / 84.1).  At D = 256, where a workgroup
+// Tree calls take 64-row workgroups: drafts are short.  Two row blocks a wave lose up to 3% on drafts
+// of up to 128 tokens and gain 5.5% on longer ones at D = 128 (D = 64 and 128, 8 sequences of 64-128 or
+// 120-256 tokens over 4000 rows, 16 heads: 44.6 / 61.4 / 61.4 / 89.0 us against 45.8 / 62.0 / 62.8 / 84.1),
+// which was left for the instantiations that it saves.  Long drafts take twice their floor (the products): each
+// 64-row workgroup brings all keys of its head through LDS, at 0.5 PFLOP/s where the plain kernel's
+// 8-wave workgroups reach 0.8; 8-wave tree instantiations at D = 64 and 128 are not built.  At D = 256, where a workgroup
 // fills a CU, 128 rows on 8 waves pay when sequences have more than 64, contexts are long (2048 rows
 // on average) and 128-row tiles are at least 48: 8 heads, 4000 rows, 8 sequences of 64-128 tokens 69.3 us
 // against 76.0, of 120-256 93.6 against 110.3, 24 of 60-80 over 3000 rows 121.5 against 154.8; but

@@ -330,7 +330,9 @@ __global__ __launch_bounds__(kNrThreads, sizeof(T) == 2 ? 4 : 3) void norm_rope_
   const NrTensor& t = *ck.t;
   float* const part = ck.tensor ? part_k : part_q;
   const bool norm = p.flags & FMLM_NR_NORM, inter = p.flags & FMLM_NR_INTERLEAVED;
-  // gains per head in LDS: in 32 registers of a thread the kernel had 3 waves a SIMD and took 7 us more
+  // gains per head in LDS: in 32 registers of a thread the kernel had 3 waves a SIMD and took 7 us more.
+  // The sums of dw for each head still cost the 16-bit types 3 to 5 spilled registers at four waves (16
+  // to 24 bytes of scratch a lane): 539 MB in 119 to 124 us where shared gains, unspilled, take 112
   __shared__ __align__(16) float gains[PERHEAD ? U * D : 1];
   float w[8];
   if constexpr (PERHEAD) {

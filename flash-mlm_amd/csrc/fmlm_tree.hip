@@ -306,7 +306,9 @@ __global__ __launch_bounds__(kLatentWaves * 64, 3) void attn_tree_latent_kernel(
 // ---------------------------------------------------------------------------
 // fp32 latent (whose context runs on the SIMT kernel): one wave per row.  Lane j scores key j of a step of 64 keys; then the row's keys are
 // taken one by one, a lane holding D / 64 columns.
-// Keys that the row does not see are not read.
+// Keys that the row does not see are not read.  Chains of 8 tokens, 4 sequences, 16 heads: 15 us beside the
+// 1156 of their 1000 context rows; of 64 tokens, 8 sequences: 156 beside 1972.  The context's SIMT kernel,
+// which plain fp32 latent calls have too, is what such calls take (floors: 7 and 112 us).
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ __launch_bounds__(64) void attn_tree_f32_kernel(const fmlm_attn_params p, const float* __restrict__ octx,

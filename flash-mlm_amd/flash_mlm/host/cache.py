@@ -482,9 +482,8 @@ class InferenceCache:
         if t > 0:
             paged_append(pairs, heads=h_kv, d=d, q_meta=q_meta, slots=slots.contiguous(),
                          pool_rows=int(entry.total_context_len))
-            for _, pool in pairs:  # written behind autograd's back: what it saved of them is stale
-                if not pool.is_inference():
-                    torch.autograd.graph.increment_version(pool)
+            # written behind autograd's back: what it saved of the pools is stale
+            torch.autograd.graph.increment_version([pool for _, pool in pairs if not pool.is_inference()])
         self._layer_kv[key] = LayerKVEntry(
             k_cache=entry.k_cache,
             v_cache=entry.v_cache,
