@@ -862,3 +862,23 @@ def test_rows_that_see_nothing_in_a_split_call(dtype, D, kind, device):
     # the first layer's schedule was a split one
     (sched,) = meta.kernel_schedules.values()
     assert int(sched[:8].view(torch.int32)[1]) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D, mla, ctx", [(64, False, [300, 3000]), (128, False, [65, 0]), (256, False, [900, 64]),
+                                         (512, True, [300, 3000])])
+def test_the_context_part_is_not_rounded(dtype, D, mla, ctx, device, monkeypatch):
+    """As the tolerances above, without a rounding of the context's part (h of it): the parts of a row meet
+    in fp32 in every kernel."""
+    def close(got, q, k, v, seen, scale, kc, vc, dt):
+        o, w, _, s = ref.tree_attention(_f(q), _f(k), _f(v), seen, scale, _f(kc), _f(vc))
+        h, keys = torch.finfo(dt).eps / 2, kc.shape[0] + k.shape[0]
+        bound = h * np.abs(o) + (2 * h + 2 * (D + 16) * U * s[:, None] + (keys + 64) * U) * w
+        if dt == torch.float16:
+            bound = bound + 2.0**-25 * (keys * np.abs(np.concatenate([_f(vc), _f(v)])).max() + 1)
+        # (1.01: the products of the terms above with each other, each below 1 / 100 of them)
+        assert np.all(np.abs(_f(got) - o) <= bound * 1.01)
+
+    monkeypatch.setitem(_run.__globals__, "_close", close)
+    _run(device, DT[dtype], lens=[30, 12], N=30, H=3, D=D, ctx=ctx, kind="packed", mla=mla, seed=D)
