@@ -139,9 +139,8 @@ FMLM_DEV NrRow nr_row(const NrParams& p, int i) {
   NrRow r;
   uint32_t at = (uint32_t)i;
   if (p.layout == FMLM_LAYOUT_PACKED && p.token_indices) at = (uint32_t)p.token_indices[i];
-  r.b = (int)(at / (uint32_t)p.N);
+  r.b = (int)min(at / (uint32_t)p.N, (uint32_t)p.B - 1u);
   r.pos = (int)(at - (uint32_t)r.b * (uint32_t)p.N);
-  r.b = min(r.b, p.B - 1);
   r.real = true;
   int64_t tok = i;  // index into positions
   if (p.cu_seqlens && p.layout == FMLM_LAYOUT_PADDED) {
@@ -152,6 +151,7 @@ FMLM_DEV NrRow nr_row(const NrParams& p, int i) {
   r.angle = 0;
   if (p.rotary_dim > 0 && r.real) {
     int64_t s = r.pos;
+    if (p.n_positions > 0) tok = min(max(tok, (int64_t)0), (int64_t)p.n_positions - 1);
     if (p.positions) s = index_at(p.positions, p.flags & FMLM_NR_POSITIONS_I64, tok);
     else if (p.offsets) s += index_at(p.offsets, p.flags & FMLM_NR_OFFSETS_I64, r.b);
     r.angle = s < 0 ? 0 : s < p.table_rows ? s : p.table_rows - 1;

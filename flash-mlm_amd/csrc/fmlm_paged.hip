@@ -26,6 +26,11 @@ constexpr int kBtFillThreads = 256;
 FMLM_DEV int64_t bt_index(const void* a, bool i64, int64_t i) {
   return i64 ? ((const int64_t*)a)[i] : (int64_t)((const int32_t*)a)[i];
 }
+// packed tokens [c0, c1) of request b, within the call's whatever the offsets hold
+FMLM_DEV void bt_tokens(const BtParams& p, int b, int& c0, int& c1) {
+  c0 = min(max(p.cu_seqlens[b], 0), p.T);
+  c1 = min(max(p.cu_seqlens[b + 1], c0), p.T);
+}
 FMLM_DEV int pages_of(int n) { return (n + FMLM_PAGE_ROWS - 1) / FMLM_PAGE_ROWS; }
 
 // workspace: per request its old length (clamped), the place of its first new page in the
@@ -129,9 +134,10 @@ FMLM_DEV void bt_scan(const BtParams& p, const BtSpace& w, int2* part) {
     bool over = false;
     if (b < p.B) {
       const int64_t raw = bt_index(p.old_lens, p.flags & FMLM_BT_OLD_I64, b);
-      const int c0 = p.cu_seqlens[b], c1 = min(p.cu_seqlens[b + 1], p.T);
+      int c0, c1;
+      bt_tokens(p, b, c0, c1);
       old = (int)(raw < 0 ? 0 : raw > cap_in ? cap_in : raw);
-      cnt = !p.keep ? max(c1 - c0, 0) : SMALL ? w.rank[max(c0, c1)] - w.rank[c0] : w.kept[b];
+      cnt = !p.keep ? c1 - c0 : SMALL ? w.rank[c1] - w.rank[c0] : w.kept[b];
       over = raw != old || cnt > cap_out - old;
       cnt = min(cnt, cap_out - old);
       have = pages_of(old);
@@ -240,10 +246,11 @@ FMLM_DEV void bt_fill(const BtParams& p, const BtSpace& w, int64_t first, int64_
     }
 #pragma unroll
     for (int u = 0; u < kBtUnroll; ++u) {
-      at[u].b = min((int)(tok[u] / (uint32_t)p.N), p.B - 1);
-      pos[u] = (int)(tok[u] - (uint32_t)at[u].b * (uint32_t)p.N);
+      at[u].b = (int)min(tok[u] / (uint32_t)p.N, (uint32_t)p.B - 1u);
+      pos[u] = (int)min(tok[u] - (uint32_t)at[u].b * (uint32_t)p.N, (uint32_t)p.N - 1u);
       if (!p.keep) rank[u] = pos[u];
-      else if (SMALL && kept[u]) rank[u] -= w.rank[t0 + u * step - pos[u]];
+      else if (SMALL && kept[u]) rank[u] -= w.rank[max(t0 + u * step - pos[u], (int64_t)0)];
+      rank[u] = max(rank[u], 0);  // (not so only where the metadata contradicts itself)
       old[u] = w.old[at[u].b];
       count[u] = w.count[at[u].b];
     }
@@ -284,7 +291,9 @@ __global__ __launch_bounds__(kBtFillThreads) void block_table_rank_kernel(const 
   __shared__ int2 part[kBtFillThreads / 64];
   __shared__ int last;
   const BtSpace w = bt_space(p);
-  const int b = blockIdx.x, c0 = p.cu_seqlens[b], c1 = min(p.cu_seqlens[b + 1], p.T);
+  const int b = blockIdx.x;
+  int c0, c1;
+  bt_tokens(p, b, c0, c1);
   const int n = bt_rank<kBtFillThreads>(p, c0, c1, w.rank, part, &last);
   if (threadIdx.x == 0) w.kept[b] = n;
 }
@@ -339,8 +348,10 @@ __global__ __launch_bounds__(kApThreads) void paged_append_kernel(const AppendPa
   int64_t off = t * a.s_sn;
   if (layout == FMLM_LAYOUT_PADDED) {
     const uint32_t tok = (uint32_t)token_indices[t];
-    const uint32_t b = tok / (uint32_t)N;
-    off = (int64_t)b * a.s_sb + (int64_t)(tok - b * (uint32_t)N) * a.s_sn;
+    uint32_t b = tok / (uint32_t)N;
+    const uint32_t p = tok - b * (uint32_t)N;
+    if (a.batch > 0) b = min(b, (uint32_t)a.batch - 1u);
+    off = (int64_t)b * a.s_sb + (int64_t)p * a.s_sn;
   }
   if (slot < 0 || slot >= pool_rows) return;
   const char* src = (const char*)a.src + off * es + (int64_t)c * sizeof(V);

@@ -34,7 +34,7 @@ __global__ __launch_bounds__(FMLM_MAX_TREE) void tree_mask_kernel(const void* pa
   __shared__ uint64_t s_bits[FMLM_MAX_TREE][kTreeWords];
   __shared__ int s_next[FMLM_MAX_TREE];
   const int b = blockIdx.x, i = threadIdx.x;
-  const int c0 = cu[b], n = max(0, min(min(cu[b + 1], T) - c0, min(N, FMLM_MAX_TREE)));
+  const int c0 = min(max(cu[b], 0), T), n = max(0, min(min(cu[b + 1], T) - c0, min(N, FMLM_MAX_TREE)));
   uint64_t bits[kTreeWords];
   int next = -1;
   if (i < n) {

@@ -16,7 +16,7 @@ import torch
 LIB_NAME = "libflash_mlm_hip.so"
 _LIB_PATH = Path(os.environ.get("FMLM_LIB_PATH", Path(__file__).resolve().parent / "_native" / LIB_NAME))
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 DTYPE_BF16 = 0
 DTYPE_F16 = 1
@@ -181,7 +181,7 @@ class NormRopeParams(ctypes.Structure):
         ("rows", _c_i64),
         ("table_rows", _c_i64),
         ("eps", ctypes.c_float),
-        ("reserved", _c_i32),
+        ("n_positions", _c_i32),
         ("cos", _c_ptr),
         ("sin", _c_ptr),
         ("cu_seqlens", _c_ptr),
@@ -208,7 +208,8 @@ class BlockTableParams(ctypes.Structure):
 class PagedTensor(ctypes.Structure):
     """Mirror of fmlm_paged_tensor (include/flash_mlm_hip.h)."""
 
-    _fields_ = [("src", _c_ptr), ("s_sb", _c_i64), ("s_sh", _c_i64), ("s_sn", _c_i64), ("pool", _c_ptr)]
+    _fields_ = [("src", _c_ptr), ("s_sb", _c_i64), ("s_sh", _c_i64), ("s_sn", _c_i64), ("pool", _c_ptr),
+                ("batch", _c_i64)]
 
 
 # (name, restype, argtypes) of every exported entry point

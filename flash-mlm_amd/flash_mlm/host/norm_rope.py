@@ -421,7 +421,7 @@ def qk_norm_rope(
                 raise ValueError("positions and context_lens are mutually exclusive")
             shape = (b, n) if not packed and q_meta is None else (q_meta.total_tokens if q_meta is not None else rows,)
             idx = positions = _check_index(positions, "positions", shape, dev, (0, table))
-            p.positions = positions.data_ptr()
+            p.positions, p.n_positions = positions.data_ptr(), positions.numel()
             if positions.dtype == torch.int64:
                 flags |= _lib.NR_POSITIONS_I64
         elif context_lens is not None:

@@ -157,6 +157,7 @@ def paged_append(pairs, *, heads: int, d: int, q_meta: PackMetadata, slots: torc
             a.s_sh, a.s_sn = t * d, d
         else:
             a.s_sb, a.s_sh, a.s_sn, _ = src.stride()
+            a.batch = src.shape[0]
     dev = slots.device
     tokens = pack_indices(q_meta, dev)[1]
     with _device_scope(dev):

@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define FMLM_ABI_VERSION 5
+#define FMLM_ABI_VERSION 6
 
 /* element types */
 enum {
@@ -396,7 +396,7 @@ typedef struct fmlm_norm_rope_params {
   int64_t rows;       /* B * N, or packed tokens      */
   int64_t table_rows;
   float eps;
-  int32_t reserved;
+  int32_t n_positions; /* entries of positions, to which its index is clamped; 0: not said */
   const float* cos; /* [table_rows, rotary_dim / 2] fp32 */
   const float* sin;
   const int32_t* cu_seqlens;    /* [B+1] or NULL */
@@ -477,6 +477,7 @@ typedef struct fmlm_paged_tensor {
   const void* src;
   int64_t s_sb, s_sh, s_sn;
   void* pool;
+  int64_t batch; /* PADDED: sequences in src, to which those of token_indices are clamped; 0: not said */
 } fmlm_paged_tensor;
 
 FMLM_API int fmlm_paged_append(const fmlm_paged_tensor* tensors, int32_t n_tensors, int32_t elem_bytes, int32_t heads,

@@ -503,3 +503,51 @@ def test_table_around_the_sizes_of_one_workgroup(B, n, width, keep, device):
     kept = [r.random() < 0.5 for _ in range(n * B)] if keep else None
     case = (lens, old, table, free, width, kept)
     _expect(case, _run_table(case, max(n, 1), device)[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", ["offsets", "tokens"])
+def test_inconsistent_metadata_stays_in_bounds(bad, device):
+    """Metadata that was not made by build_pack_metadata: offsets and token indices far out of range.  What
+    they say is clamped to the tensors; requests whose own are right get what is theirs."""
+    import dataclasses
+
+    from flash_mlm import build_tree_metadata, qk_norm_rope
+
+    B, N, H, D, far = 4, 3000, 2, 64, 2**30
+    for lens in ([3, 0, 7, 5], [3000, 10, 2900, 7]):  # one workgroup, and three kernels
+        T = sum(lens)
+        meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+        cu, tok = meta.cu_seqlens.clone(), meta.token_indices.clone()
+        if bad == "offsets":
+            cu[:] = torch.tensor([-far, far, 2, -7, far], device=device)
+        else:
+            tok[1:] = torch.randint(-(2**40), 2**40, (T - 1,), device=device)
+            tok[1::2] = 2**32 - 1
+        wrong = dataclasses.replace(meta, cu_seqlens=cu, token_indices=tok, launch_memo={}, kernel_schedules={})
+        old = torch.tensor([5, 70, 0, 64], dtype=torch.int32, device=device)
+        free = torch.arange(400, dtype=torch.int32, device=device)
+        table = torch.full((B, 100), 399, dtype=torch.int32, device=device)
+        for keep in (None, torch.rand(T, device=device) < 0.5):
+            plan = build_block_table(wrong, old, free_pages=free, block_table=table, keep=keep, check=False)
+            assert int(plan.slot_mapping.max()) < 400 * PAGE and int(plan.slot_mapping.min()) >= -1
+        q, k = (torch.randn((B, H, N, D), device=device) for _ in range(2))
+        cos, sin = torch.ones((50, 32), device=device), torch.zeros((50, 32), device=device)
+        for where in (dict(positions=torch.zeros(T, dtype=torch.int32, device=device)),
+                      dict(context_lens=torch.zeros(B, dtype=torch.int64, device=device))):
+            a, b = qk_norm_rope(q, k, cos=cos, sin=sin, q_meta=wrong, **where)
+            assert bool(a.isfinite().all()) and bool(b.isfinite().all())
+            a, b = qk_norm_rope(torch.randn((H * T, D), device=device), torch.randn((H * T, D), device=device), cos=cos,
+                                sin=sin, q_meta=wrong, **where)
+            assert bool(a.isfinite().all())
+        cache = InferenceCache()
+        kp, vp = (torch.zeros((H, 400, PAGE, D), dtype=torch.bfloat16, device=device) for _ in range(2))
+        cache.prefill_paged_kv_cache(0, k_pages=kp, v_pages=vp, block_table=table, context_lens=old, is_mla=False, num_heads=H,
+                                     head_dim=D)
+        good = build_block_table(meta, old, free_pages=free, block_table=table, check=False)
+        cache.append_paged_kv_cache(0, k=q.bfloat16(), v=k.bfloat16(), q_meta=wrong, plan=good)
+        assert torch.equal(kp.view(H, -1, D)[:, good.slot_mapping[0]], q[0, :, 0].bfloat16())
+        small = dataclasses.replace(wrong, N=200)
+        tree = build_tree_metadata(torch.full((T,), -1, device=device), small, check=False)
+        assert tree.mask.shape == (T, 4)
+        torch.cuda.synchronize()
