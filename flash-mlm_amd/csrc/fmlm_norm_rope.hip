@@ -139,19 +139,20 @@ FMLM_DEV NrRow nr_row(const NrParams& p, int i) {
   NrRow r;
   uint32_t at = (uint32_t)i;
   if (p.layout == FMLM_LAYOUT_PACKED && p.token_indices) at = (uint32_t)p.token_indices[i];
-  r.b = (int)min(at / (uint32_t)p.N, (uint32_t)p.B - 1u);
-  r.pos = (int)(at - (uint32_t)r.b * (uint32_t)p.N);
+  const uint32_t b = at / (uint32_t)p.N;
+  r.pos = (int)(at - b * (uint32_t)p.N);
+  r.b = (int)min(b, (uint32_t)p.B - 1u);
   r.real = true;
   int64_t tok = i;  // index into positions
   if (p.cu_seqlens && p.layout == FMLM_LAYOUT_PADDED) {
-    const int c0 = p.cu_seqlens[r.b];
-    r.real = r.pos < p.cu_seqlens[r.b + 1] - c0;
-    tok = (int64_t)c0 + r.pos;
+    // (a token past the positions is none, whatever the offsets say)
+    const int c0 = p.cu_seqlens[r.b], at = c0 + r.pos;
+    r.real = r.pos < p.cu_seqlens[r.b + 1] - c0 && (p.n_positions == 0 || (uint32_t)at < (uint32_t)p.n_positions);
+    tok = at;
   }
   r.angle = 0;
   if (p.rotary_dim > 0 && r.real) {
     int64_t s = r.pos;
-    if (p.n_positions > 0) tok = min(max(tok, (int64_t)0), (int64_t)p.n_positions - 1);
     if (p.positions) s = index_at(p.positions, p.flags & FMLM_NR_POSITIONS_I64, tok);
     else if (p.offsets) s += index_at(p.offsets, p.flags & FMLM_NR_OFFSETS_I64, r.b);
     r.angle = s < 0 ? 0 : s < p.table_rows ? s : p.table_rows - 1;
@@ -331,8 +332,8 @@ __global__ __launch_bounds__(kNrThreads, sizeof(T) == 2 ? 4 : 3) void norm_rope_
   float* const part = ck.tensor ? part_k : part_q;
   const bool norm = p.flags & FMLM_NR_NORM, inter = p.flags & FMLM_NR_INTERLEAVED;
   // gains per head in LDS: in 32 registers of a thread the kernel had 3 waves a SIMD and took 7 us more.
-  // The sums of dw for each head still cost the 16-bit types 3 to 5 spilled registers at four waves (16
-  // to 24 bytes of scratch a lane): 539 MB in 119 to 124 us where shared gains, unspilled, take 112
+  // The sums of dw for each head still cost the 16-bit types 4 to 6 spilled registers at four waves (20
+  // to 28 bytes of scratch a lane): 539 MB in 119 to 124 us where shared gains, unspilled, take 112
   __shared__ __align__(16) float gains[PERHEAD ? U * D : 1];
   float w[8];
   if constexpr (PERHEAD) {

@@ -396,7 +396,7 @@ typedef struct fmlm_norm_rope_params {
   int64_t rows;       /* B * N, or packed tokens      */
   int64_t table_rows;
   float eps;
-  int32_t n_positions; /* entries of positions, to which its index is clamped; 0: not said */
+  int32_t n_positions; /* entries of positions: a padded row past them is no token; 0: not said */
   const float* cos; /* [table_rows, rotary_dim / 2] fp32 */
   const float* sin;
   const int32_t* cu_seqlens;    /* [B+1] or NULL */
