@@ -16,7 +16,7 @@ import torch
 LIB_NAME = "libflash_mlm_hip.so"
 _LIB_PATH = Path(os.environ.get("FMLM_LIB_PATH", Path(__file__).resolve().parent / "_native" / LIB_NAME))
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 DTYPE_BF16 = 0
 DTYPE_F16 = 1
@@ -37,6 +37,13 @@ NR_OFFSETS_I64 = 8
 BT_OLD_I64 = 1
 BT_TABLE_I64 = 2
 BT_FREE_I64 = 4
+
+WINDOW_APPENDED = 1
+WINDOW_FP4 = 2
+
+AP_INTERLEAVED = 1
+AP_FP4 = 2
+AP_POSITIONS_I64 = 4
 
 MAX_TREE = 256
 
@@ -212,6 +219,32 @@ class PagedTensor(ctypes.Structure):
                 ("batch", _c_i64)]
 
 
+class Window(ctypes.Structure):
+    """Mirror of fmlm_window (include/flash_mlm_hip.h)."""
+
+    _fields_ = [(n, _c_i32) for n in ("left", "right", "sinks", "flags")] + [("k_scales", _c_ptr), ("v_scales", _c_ptr)]
+
+
+class AppendRows(ctypes.Structure):
+    """Mirror of fmlm_append_rows (include/flash_mlm_hip.h)."""
+
+    _fields_ = [
+        (name if s == "" else f"{pre}{s}", _c_ptr if s == "" else _c_i64)
+        for name, pre in (("src", "s"), ("dst", "d"))
+        for s in ("", "_sb", "_sh", "_sn")
+    ] + [("scales", _c_ptr)]
+
+
+class AppendParams(ctypes.Structure):
+    """Mirror of fmlm_append_params (include/flash_mlm_hip.h)."""
+
+    _fields_ = [
+        (n, _c_i32) for n in ("dtype", "flags", "layout", "B", "H", "N", "D", "rotary_dim", "T", "reserved")
+    ] + [("table_rows", _c_i64), ("pool_rows", _c_i64)] + [
+        (n, _c_ptr) for n in ("cos", "sin", "positions", "cu_seqlens", "slots")
+    ] + [(n, AppendRows) for n in ("q", "k", "v")]
+
+
 # (name, restype, argtypes) of every exported entry point
 SIGNATURES = {
     "fmlm_abi_version": (ctypes.c_int, []),
@@ -267,6 +300,16 @@ SIGNATURES = {
     "fmlm_attn_tree_tile": (ctypes.c_int, [ctypes.POINTER(AttnParams)]),
     "fmlm_attn_tree_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(AttnParams)]),
     "fmlm_attn_tree_fwd": (ctypes.c_int, [ctypes.POINTER(AttnParams), _c_ptr, _c_i32, _c_ptr, _c_i64, _c_ptr]),
+    "fmlm_window_size": (ctypes.c_int, []),
+    "fmlm_window_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(AttnParams), ctypes.POINTER(Window)]),
+    "fmlm_window_fwd": (ctypes.c_int, [ctypes.POINTER(AttnParams), ctypes.POINTER(Window), _c_ptr]),
+    "fmlm_window_bwd": (
+        ctypes.c_int,
+        [ctypes.POINTER(AttnParams), ctypes.POINTER(Window), ctypes.POINTER(AttnGrads), _c_ptr],
+    ),
+    "fmlm_append_params_size": (ctypes.c_int, []),
+    "fmlm_rotate_append": (ctypes.c_int, [ctypes.POINTER(AppendParams), _c_ptr]),
+    "fmlm_fp4_values": (ctypes.c_int, [_c_i32, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i32, _c_ptr]),
 }
 
 _lock = threading.Lock()
@@ -307,6 +350,10 @@ def load() -> ctypes.CDLL:
             raise RuntimeError("fmlm_norm_rope_params layout mismatch between library and binding")
         if lib.fmlm_block_table_params_size() != ctypes.sizeof(BlockTableParams):
             raise RuntimeError("fmlm_block_table_params layout mismatch between library and binding")
+        if lib.fmlm_window_size() != ctypes.sizeof(Window):
+            raise RuntimeError("fmlm_window layout mismatch between library and binding")
+        if lib.fmlm_append_params_size() != ctypes.sizeof(AppendParams):
+            raise RuntimeError("fmlm_append_params layout mismatch between library and binding")
         _lib = lib
         return lib
 

@@ -10,6 +10,7 @@ from flash_mlm.host.host_utils import build_pack_metadata, unpack_from_kernel
 from flash_mlm.host.norm_rope import qk_norm_rope
 from flash_mlm.host.paged import PagedMetadata, build_block_table
 from flash_mlm.host.tree import TreeMetadata, build_tree_metadata, flash_attn_mlm_tree
+from flash_mlm.host.window import flash_attn_mlm_window
 
 __all__ = [
     "flash_attn_mlm",
@@ -26,4 +27,5 @@ __all__ = [
     "TreeMetadata",
     "build_tree_metadata",
     "flash_attn_mlm_tree",
+    "flash_attn_mlm_window",
 ]

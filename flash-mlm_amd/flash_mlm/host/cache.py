@@ -121,9 +121,14 @@ class LayerKVEntry:
     # like the packed entries), total_context_len = P * PAGE_ROWS, cu_seqlens_kv the prefix
     # sums of the batch lengths
     block_table: torch.Tensor | None = None
+    # 4-bit paged entries (InferenceCache.prefill_paged_fp4_cache): k_cache / v_cache are the
+    # codes (uint8, two values a byte), these their scales; dtype is that of the values
+    k_scales: torch.Tensor | None = None
+    v_scales: torch.Tensor | None = None
 
 
 PAGE_ROWS = 64  # rows per page of a paged context (FMLM_PAGE_ROWS, the kernels' key tile)
+FP4_BLOCK = 32  # values of a 4-bit row that share a scale
 
 
 def _check_rank2(t: torch.Tensor, what: str) -> None:
@@ -278,6 +283,28 @@ class InferenceCache:
             device=k_cache.device,
         )
 
+    @staticmethod
+    def _page_index(block_table: torch.Tensor, context_lens: torch.Tensor, dev: torch.device) -> dict:
+        """The block-table fields of a paged entry, checked."""
+        if block_table.ndim != 2 or block_table.dtype not in (torch.int32, torch.int64):
+            raise ValueError("block_table must be a rank-2 integer tensor [context_batch, max_pages]")
+        n_batch, max_pages = int(block_table.shape[0]), int(block_table.shape[1])
+        if n_batch < 1:
+            raise ValueError("block_table needs at least one context batch")
+        if context_lens.ndim != 1 or int(context_lens.numel()) != n_batch:
+            raise ValueError("context_lens must have one entry per block_table row")
+        if not context_lens.is_cuda and n_batch:
+            lo, hi = int(context_lens.min()), int(context_lens.max())
+            if lo < 0 or hi > max_pages * PAGE_ROWS:
+                raise ValueError(f"context_lens must lie in [0, {max_pages * PAGE_ROWS}]")
+        cu = torch.zeros(n_batch + 1, dtype=torch.int32, device=dev)
+        cu[1:] = torch.cumsum(context_lens.to(device=dev, dtype=torch.int32), 0)
+        return dict(
+            cu_seqlens_kv=cu,
+            context_batch_size=n_batch,
+            block_table=block_table.to(device=dev, dtype=torch.int32).contiguous(),
+        )
+
     def prefill_paged_kv_cache(
         self,
         layer_id: int | str,
@@ -318,34 +345,91 @@ class InferenceCache:
             raise ValueError("non-MLA paged cache requires contiguous v_pages shaped like k_pages")
         if k_pages.dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("paged KV contexts need bf16 or fp16 pages")
-        if block_table.ndim != 2 or block_table.dtype not in (torch.int32, torch.int64):
-            raise ValueError("block_table must be a rank-2 integer tensor [context_batch, max_pages]")
-        n_batch, max_pages = int(block_table.shape[0]), int(block_table.shape[1])
-        if n_batch < 1:
-            raise ValueError("block_table needs at least one context batch")
-        if context_lens.ndim != 1 or int(context_lens.numel()) != n_batch:
-            raise ValueError("context_lens must have one entry per block_table row")
-        if not context_lens.is_cuda and n_batch:
-            lo, hi = int(context_lens.min()), int(context_lens.max())
-            if lo < 0 or hi > max_pages * PAGE_ROWS:
-                raise ValueError(f"context_lens must lie in [0, {max_pages * PAGE_ROWS}]")
         dev = k_pages.device
         n_pages = int(k_pages.shape[1])
-        cu = torch.zeros(n_batch + 1, dtype=torch.int32, device=dev)
-        cu[1:] = torch.cumsum(context_lens.to(device=dev, dtype=torch.int32), 0)
         self._layer_kv[self._layer_key(layer_id)] = LayerKVEntry(
             k_cache=k_pages.view(n_pages * h_kv * PAGE_ROWS, head_dim),
             v_cache=None if is_mla else v_pages.view(n_pages * h_kv * PAGE_ROWS, head_dim),
             total_context_len=n_pages * PAGE_ROWS,
-            cu_seqlens_kv=cu,
-            context_batch_size=n_batch,
             is_mla=bool(is_mla),
             num_heads=int(num_heads),
             head_dim=int(head_dim),
             dtype=k_pages.dtype,
             device=dev,
-            block_table=block_table.to(device=dev, dtype=torch.int32).contiguous(),
+            **self._page_index(block_table, context_lens, dev),
         )
+
+    def prefill_paged_fp4_cache(
+        self,
+        layer_id: int | str,
+        *,
+        k_pages: torch.Tensor,
+        k_scales: torch.Tensor,
+        v_pages: torch.Tensor,
+        v_scales: torch.Tensor,
+        block_table: torch.Tensor,
+        context_lens: torch.Tensor,
+        num_heads: int,
+        head_dim: int,
+        dtype: torch.dtype,
+    ) -> None:
+        """Store a paged context in 4 bits as ``layer_id``'s entry (no copy).
+
+        An extension, like :meth:`prefill_paged_kv_cache`, whose ``block_table`` and
+        ``context_lens`` it takes.  ``k_pages`` / ``v_pages`` are uint8 pools
+        [H, P, 64, D / 2] of E2M1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign), element 2i of a row
+        in the low and 2i + 1 in the high half of byte i; ``k_scales`` / ``v_scales`` uint8
+        [H, P, 64, D / 32]: 32 neighbouring elements have the scale 2^(x - 127).  D is 32, 64, 128
+        or 256.  ``dtype`` (bf16 or fp16) is the type of the values, hence of the queries; fp16
+        holds those of scale bytes 104 to 140, bf16 of bytes up to 252.  A pool of zeros is a valid
+        empty one: :meth:`append_paged_kv_cache` fills it.  Served by
+        :func:`flash_attn_mlm_compressed` and :func:`flash_attn_mlm_window`; no gradients.
+        """
+        if num_heads < 1:
+            raise ValueError("num_heads must be >= 1")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("4-bit contexts hold bf16 or fp16 values")
+        if head_dim not in (32, 64, 128, 256):
+            raise ValueError("4-bit contexts need head_dim 32, 64, 128 or 256")
+        pools = {"k_pages": k_pages, "v_pages": v_pages, "k_scales": k_scales, "v_scales": v_scales}
+        dev, n_pages = k_pages.device, int(k_pages.shape[1]) if k_pages.ndim == 4 else -1
+        for name, x in pools.items():
+            cols = head_dim // (2 if name.endswith("pages") else FP4_BLOCK)
+            if x.dtype != torch.uint8 or tuple(x.shape) != (num_heads, n_pages, PAGE_ROWS, cols):
+                raise ValueError(f"{name} must be uint8 [num_heads, pages, {PAGE_ROWS}, {cols}]")
+            if not x.is_contiguous() or x.device != dev or (x.numel() and x.data_ptr() % 16):
+                raise ValueError(f"{name} must be contiguous, 16-byte aligned and on the device of k_pages")
+        self._layer_kv[self._layer_key(layer_id)] = LayerKVEntry(
+            k_cache=k_pages.view(num_heads * n_pages * PAGE_ROWS, head_dim // 2),
+            v_cache=v_pages.view(num_heads * n_pages * PAGE_ROWS, head_dim // 2),
+            total_context_len=n_pages * PAGE_ROWS,
+            is_mla=False,
+            num_heads=int(num_heads),
+            head_dim=int(head_dim),
+            dtype=dtype,
+            device=dev,
+            k_scales=k_scales,
+            v_scales=v_scales,
+            **self._page_index(block_table, context_lens, dev),
+        )
+
+    def paged_kv_values(self, layer_id: int | str) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """The pages of ``layer_id``'s paged context as values: (k, v) [H_kv, P, 64, D] of the entry's
+        dtype (v None for MLA).  Of a 16-bit context the pools themselves, of a 4-bit one new
+        tensors, by one HIP launch each.  The block table says which pages are in use; the others hold
+        whatever their memory does."""
+        entry = self._layer_kv.get(self._layer_key(layer_id))
+        if entry is None:
+            raise ValueError(f"no cached KV entry for layer {layer_id!r}")
+        if entry.block_table is None:
+            raise ValueError("paged_kv_values requires a paged entry")
+        shape = (1 if entry.is_mla else entry.num_heads, entry.total_context_len // PAGE_ROWS, PAGE_ROWS, entry.head_dim)
+        if entry.k_scales is None:
+            return entry.k_cache.view(shape), None if entry.v_cache is None else entry.v_cache.view(shape)
+        from flash_mlm.host.paged import fp4_values
+
+        return (fp4_values(entry.k_cache, entry.k_scales, shape, entry.dtype),
+                fp4_values(entry.v_cache, entry.v_scales, shape, entry.dtype))
 
     def append_kv_cache(
         self,
@@ -430,7 +514,12 @@ class InferenceCache:
         v: torch.Tensor | None = None,
         q_meta: PackMetadata,
         plan: PagedMetadata,
-    ) -> None:
+        q: torch.Tensor | None = None,
+        cos: torch.Tensor | None = None,
+        sin: torch.Tensor | None = None,
+        positions: torch.Tensor | None = None,
+        interleaved: bool = False,
+    ) -> torch.Tensor | None:
         """Store new keys and values in ``layer_id``'s paged context.
 
         This is an extension: the reference's roadmap lists paged KV (README.md:41).
@@ -444,6 +533,19 @@ class InferenceCache:
         the backward of an earlier call on the pool has to run before it.  Afterwards the entry has the
         plan's block table and context lengths: attend before appending, or the new tokens are
         both context and main keys.
+
+        With ``cos`` / ``sin`` (fp32 tables [positions, R/2] as of :func:`qk_norm_rope`, not for MLA)
+        the keys are rotated on the way, and so is ``q``, laid out like ``k``, when it is given: the
+        call returns it rotated, contiguous, padding rows as zeros, without a gradient.  The tokens'
+        rows of the tables are ``positions`` [T] (int; default the plan's), range-checked on the CPU
+        and clamped on the GPU; ``interleaved`` as of :func:`qk_norm_rope`.  Attention of tokens
+        that have been appended: :func:`flash_attn_mlm_window` without k and v.
+
+        A 4-bit context (:meth:`prefill_paged_fp4_cache`) stores 4-bit rows: of 32 neighbouring
+        values the scale is the smallest 2^e with which all are below 7 * 2^e (e in [-23, 13] for
+        fp16, [-125, 125] for bf16), and each is rounded to the nearest code, halfway to the even
+        one, the largest to 6.  Infinities count as the largest finite value, NaN as 0.  Slots must be
+        distinct, as a plan's are.
         """
         key = self._layer_key(layer_id)
         entry = self._layer_kv.get(key)
@@ -451,6 +553,10 @@ class InferenceCache:
             raise ValueError(f"no cached KV entry for layer {layer_id!r}")
         if entry.block_table is None:
             raise ValueError("append_paged_kv_cache requires a paged entry (prefill_paged_kv_cache)")
+        if cos is None and (sin is not None or q is not None or positions is not None or interleaved):
+            raise ValueError("q, sin, positions and interleaved need cos")
+        if cos is not None and entry.is_mla:
+            raise ValueError("MLA latents are stored as they are: no cos and sin")
         h_kv = 1 if entry.is_mla else entry.num_heads
         d, t = entry.head_dim, int(q_meta.total_tokens)
         pairs = [(k, entry.k_cache)]
@@ -477,13 +583,20 @@ class InferenceCache:
         dev = entry.device
         if slots.device != dev or table.device != dev or cu.device != dev or q_meta.token_indices.device != dev:
             raise ValueError("plan and q_meta must be on the cached entry's device")
-        from flash_mlm.host.paged import paged_append
+        from flash_mlm.host.paged import paged_append, rotate_append
 
-        if t > 0:
+        rotated = None
+        if cos is not None or entry.k_scales is not None:
+            rotated = rotate_append(entry, q, k, v, q_meta=q_meta, slots=slots.contiguous(), cos=cos, sin=sin,
+                                    positions=plan.positions if positions is None else positions,
+                                    interleaved=interleaved)
+        elif t > 0:
             paged_append(pairs, heads=h_kv, d=d, q_meta=q_meta, slots=slots.contiguous(),
                          pool_rows=int(entry.total_context_len))
+        if t > 0:
             # written behind autograd's back: what it saved of the pools is stale
-            torch.autograd.graph.increment_version([pool for _, pool in pairs if not pool.is_inference()])
+            pools = [pool for _, pool in pairs] + [x for x in (entry.k_scales, entry.v_scales) if x is not None]
+            torch.autograd.graph.increment_version([x for x in pools if not x.is_inference()])
         self._layer_kv[key] = LayerKVEntry(
             k_cache=entry.k_cache,
             v_cache=entry.v_cache,
@@ -496,7 +609,10 @@ class InferenceCache:
             dtype=entry.dtype,
             device=entry.device,
             block_table=table.contiguous(),
+            k_scales=entry.k_scales,
+            v_scales=entry.v_scales,
         )
+        return rotated
 
     def get_kv_cache(
         self,

@@ -26,12 +26,14 @@ import torch
 from flash_mlm import _lib
 from flash_mlm.host.cache import PAGE_ROWS, InferenceCache, PackMetadata
 from flash_mlm.host.host_utils import (
+    _aligned,
     _compute_total_q_len_padded,
     _device_scope,
     _maybe_get_cache_context,
     _pack_rows,
     make_contiguous,
     require_cuda_tensors,
+    rows16,
     validate_cache_request,
     validate_cu_seqlens_rank1_min2,
     validate_head_dim_supported,
@@ -74,24 +76,8 @@ def tile_config_value() -> int:
     return _TILE_CONFIG
 
 
-def _aligned(t: torch.Tensor) -> bool:
-    """Row-addressable by the kernel: unit stride in D, 16-byte aligned rows."""
-    if t.numel() == 0:
-        return True
-    es = t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16:
-        return False
-    return all((s * es) % 16 == 0 for s in t.stride()[:-1])
-
-
 def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if _aligned(t) else t.contiguous()
-
-
-def rows16(t: torch.Tensor) -> torch.Tensor:
-    """Rows that a kernel can address: ``t``, or an aligned copy (also of a contiguous ``t``
-    that starts at an odd address)."""
-    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _workspace(inference_cache: InferenceCache | None, nbytes: int, device: torch.device):
@@ -230,6 +216,13 @@ def _entry_of(inference_cache: InferenceCache | None, layer_id):
     if inference_cache is None or layer_id is None:
         return None
     return inference_cache.layer_entry(layer_id)
+
+
+def _refuse_fp4(inference_cache: InferenceCache | None, layer_id) -> None:
+    """For the entry points that read 16-bit contexts only."""
+    entry = _entry_of(inference_cache, layer_id)
+    if entry is not None and entry.k_scales is not None:
+        raise ValueError("a 4-bit context serves flash_attn_mlm_compressed and flash_attn_mlm_window")
 
 
 def _memo_lookup(memo: dict, key, entry, cu=None) -> _Memo | None:
@@ -606,6 +599,9 @@ def flash_attn_mlm(
     layer's new context with context_batch_size = B.  ``context_index`` (int [B], an
     extension) maps sequence b to cached context batch ``context_index[b]``.
     """
+    if not prefill:
+        _refuse_fp4(inference_cache, layer_id)
+
     def impl(owned: bool):
         return _dense_impl(
             q, k, v, scale, inference_cache, layer_id, is_mla, context_batch_size, prefill,
@@ -789,7 +785,16 @@ def flash_attn_mlm_compressed(
     K/V [H_kv * T_pad, D] as the layer's context (cu_seqlens_kv = q_meta.cu_seqlens,
     context_batch_size = B) before the attention runs.  ``context_index`` (int [B], an
     extension) maps sequence b to cached context batch ``context_index[b]`` instead.
+    A context in 4 bits (:meth:`InferenceCache.prefill_paged_fp4_cache`, an extension) is read in
+    place too, without ``causal_query_seq_attn``, MLA and gradients.
     """
+    entry = None if prefill else _entry_of(inference_cache, layer_id)
+    if entry is not None and entry.k_scales is not None:
+        return _compressed_fp4(
+            q, k, v, num_heads, q_meta, scale, inference_cache, layer_id, is_mla, context_batch_size, block_n,
+            causal_query_seq_attn, context_index,
+        )
+
     def impl(owned: bool):
         return _compressed_impl(
             q, k, v, num_heads, q_meta, scale, inference_cache, layer_id, is_mla, context_batch_size,
@@ -798,6 +803,32 @@ def flash_attn_mlm_compressed(
         )
 
     return _run(impl, q, k, v, inference_cache, layer_id, prefill, is_mla)
+
+
+def _compressed_fp4(
+    q, k, v, num_heads, q_meta, scale, inference_cache, layer_id, is_mla, context_batch_size, block_n,
+    causal_query_seq_attn, context_index,
+):
+    """:func:`flash_attn_mlm_compressed` over a 4-bit context: window attention without a limit."""
+    from flash_mlm.host.window import flash_attn_mlm_window
+
+    if is_mla or causal_query_seq_attn:
+        raise ValueError("a 4-bit context has neither MLA nor causal_query_seq_attn")
+    validate_qkv_same_shape_rank4(q, k, v, error_prefix="q/k/v")
+    if q_meta.batch_ids_block_n != block_n:
+        raise ValueError("q_meta was built with different block_n")
+    stored = inference_cache.layer_entry(layer_id).context_batch_size
+    if context_batch_size is not None:
+        if context_index is not None:
+            raise ValueError("context_index and context_batch_size are mutually exclusive")
+        if context_batch_size != stored:
+            raise ValueError(
+                f"context_batch_size ({context_batch_size}) must match cached entry context_batch_size ({stored})"
+            )
+    return flash_attn_mlm_window(
+        q, k, v, num_heads, q_meta, scale, inference_cache=inference_cache, layer_id=layer_id,
+        context_index=context_index,
+    )
 
 
 def _compressed_impl(
@@ -1064,6 +1095,8 @@ def flash_attn_mlm_precompressed(
     validated as in the reference.  ``prefill=True`` stores k / v (views) as the
     layer's context after the launch.
     """
+    if not prefill:
+        _refuse_fp4(inference_cache, layer_id)
 
     def impl(owned: bool):
         return _precompressed_impl(

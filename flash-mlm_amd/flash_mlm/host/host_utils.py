@@ -66,6 +66,68 @@ def refuse_tangents(what: str, *tensors) -> None:
             raise ValueError(f"{what} has no forward-mode derivative")
 
 
+def _aligned(t: torch.Tensor) -> bool:
+    """Row-addressable by the kernel: unit stride in D, 16-byte aligned rows."""
+    if t.numel() == 0:
+        return True
+    es = t.element_size()
+    if t.stride(-1) != 1 or t.data_ptr() % 16:
+        return False
+    return all((s * es) % 16 == 0 for s in t.stride()[:-1])
+
+
+def rows16(t: torch.Tensor) -> torch.Tensor:
+    """Rows that a kernel can address: ``t``, or an aligned copy (also of a contiguous ``t``
+    that starts at an odd address)."""
+    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def aligned16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and 16-byte aligned (a copy where it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _accumulator(leaf: torch.Tensor):
+    """The node that autograd delivers the leaf's gradient to: one for all live graphs."""
+    return leaf.view_as(leaf).grad_fn.next_functions[0][0]
+
+
+def _lives(leaf: torch.Tensor) -> bool:
+    """Whether another graph than one of this capture holds the leaf's accumulator.  (In a frame of its
+    own: a refusal's traceback must not be what holds it in the next attempt.)"""
+    token = object()
+    _accumulator(leaf).metadata["fmlm_probe"] = token
+    node = _accumulator(leaf)
+    return node.metadata.get("fmlm_probe") is token and "fmlm_captured" not in node.metadata
+
+
+def capture_leaves(what: str, *tensors) -> list[torch.Tensor]:
+    """The leaves among ``tensors`` when the current stream is being captured (else none), checked.
+
+    Autograd runs a leaf's accumulator on the stream of the graph that made it.  When that is an
+    eager graph on the default stream, a captured backward drags the default stream into the
+    capture, which ends the process when the capture ends.  An accumulator outlives its
+    last reference here exactly when another live graph holds it.
+    """
+    leaves = [t for t in tensors if isinstance(t, torch.Tensor) and t.requires_grad and t.is_leaf]
+    if not leaves or not torch.cuda.is_current_stream_capturing():
+        return []
+    for t in leaves:
+        if _lives(t):
+            raise ValueError(
+                f"{what} is being captured into a graph while another autograd graph of one of its leaves "
+                "lives: drop the outputs of the earlier calls on it first"
+            )
+    return leaves
+
+
+def keep_leaves(leaves) -> None:
+    """Marks the leaves of a capture's own graph (capture_leaves): later calls of it may share them."""
+    for t in leaves:
+        _accumulator(t).metadata["fmlm_captured"] = True
+
+
 class _NullScope:
     def __enter__(self):
         return self
@@ -343,6 +405,8 @@ def _maybe_get_cache_context(
                 device=device,
             )
         except ValueError:
+            entry = None
+        if entry is not None and entry.k_scales is not None:  # in 4 bits: callers refuse it, or do without a context
             entry = None
 
     if entry is None:

@@ -14,18 +14,20 @@ import torch
 
 from flash_mlm import _lib
 from flash_mlm.host.cache import PackMetadata
-from flash_mlm.host.host import rows16
-from flash_mlm.host.host_utils import pack_indices, refuse_tangents, require_cuda_tensors, validate_head_dim_supported
+from flash_mlm.host.host_utils import (
+    aligned16,
+    capture_leaves,
+    keep_leaves,
+    pack_indices,
+    refuse_tangents,
+    require_cuda_tensors,
+    rows16,
+    validate_head_dim_supported,
+)
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _INTS = (torch.int32, torch.int64)
 _HEAD_DIMS = (16, 32, 64, 128, 256, 512)
-
-
-def aligned16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous and 16-byte aligned (a copy where it is not)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 class _Call:
@@ -209,38 +211,8 @@ def _backward_node(ctx, dq, dk):
 _backward_once = torch.autograd.function.once_differentiable(_backward_node)
 
 
-def _accumulator(leaf: torch.Tensor):
-    """The node that autograd delivers the leaf's gradient to: one for all live graphs."""
-    return leaf.view_as(leaf).grad_fn.next_functions[0][0]
-
-
-def _lives(leaf: torch.Tensor) -> bool:
-    """Whether another graph than one of this capture holds the leaf's accumulator.  (In a frame of its
-    own: a refusal's traceback must not be what holds it in the next attempt.)"""
-    token = object()
-    _accumulator(leaf).metadata["fmlm_probe"] = token
-    node = _accumulator(leaf)
-    return node.metadata.get("fmlm_probe") is token and "fmlm_captured" not in node.metadata
-
-
 def _capture_leaves(*tensors) -> list[torch.Tensor]:
-    """The leaves among ``tensors`` when the current stream is being captured (else none), checked.
-
-    Autograd runs a leaf's accumulator on the stream of the graph that made it.  When that is an
-    eager graph on the default stream, a captured backward drags the default stream into the
-    capture, which ends the process when the capture ends.  An accumulator outlives its
-    last reference here exactly when another live graph holds it.
-    """
-    leaves = [t for t in tensors if isinstance(t, torch.Tensor) and t.requires_grad and t.is_leaf]
-    if not leaves or not torch.cuda.is_current_stream_capturing():
-        return []
-    for t in leaves:
-        if _lives(t):
-            raise ValueError(
-                "qk_norm_rope is being captured into a graph while another autograd graph of one of its leaves "
-                "lives: drop the outputs of the earlier calls on it first"
-            )
-    return leaves
+    return capture_leaves("qk_norm_rope", *tensors)
 
 
 def _check_gain(w, what: str, heads: int, d: int, device):
@@ -456,7 +428,6 @@ def _apply(call: _Call, q, k, wq, wk, cos, sin, positions, context_lens, leaves=
             if leaves is None:
                 leaves = _capture_leaves(q, k, wq, wk)
             out = _NormRope.apply(call, q, k, wq, wk, cos, sin, positions, context_lens)
-            for t in leaves:  # this capture's own graph: later calls of it may share the leaf
-                _accumulator(t).metadata["fmlm_captured"] = True
+            keep_leaves(leaves)
             return out
     return _forward(call, q, k)

@@ -10,7 +10,14 @@ import torch
 
 from flash_mlm import _lib
 from flash_mlm.host.cache import PAGE_ROWS, PackMetadata
-from flash_mlm.host.host_utils import _device_scope, _require_device, pack_indices
+from flash_mlm.host.host_utils import (
+    _device_scope,
+    _require_device,
+    aligned16,
+    pack_indices,
+    refuse_tangents,
+    rows16,
+)
 
 _INTS = (torch.int32, torch.int64)
 
@@ -167,3 +174,99 @@ def paged_append(pairs, *, heads: int, d: int, q_meta: PackMetadata, slots: torc
             pool_rows, _lib.stream_of(dev),
         )
     _lib.check(rc, "fmlm_paged_append")
+
+
+def fp4_values(codes: torch.Tensor, scales: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tensor:
+    """The values of 4-bit rows as a new tensor (fmlm_fp4_values); the kernel of
+    :meth:`InferenceCache.paged_kv_values`."""
+    _require_device(codes, what="paged_kv_values")
+    out = torch.empty(shape, dtype=dtype, device=codes.device)
+    if out.numel():
+        with _device_scope(codes.device):
+            rc = _lib.load().fmlm_fp4_values(_lib.dtype_code(dtype), codes.data_ptr(), scales.data_ptr(), out.data_ptr(),
+                                             out.numel() // shape[-1], shape[-1], _lib.stream_of(codes.device))
+        _lib.check(rc, "fmlm_fp4_values")
+    return out
+
+
+def _tables(cos, sin, positions, *, d: int, t: int, dev):
+    """(cos, sin, positions) of a rotating append, checked and as the kernel reads them."""
+    if sin is None:
+        raise ValueError("cos and sin come together")
+    if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 \
+            or cos.device != dev or sin.device != dev:
+        raise ValueError("cos and sin must be fp32 tables [positions, rotary_dim / 2] on the cached entry's device")
+    r = 2 * int(cos.shape[1])
+    if r < 16 or r % 16 or r > d or cos.shape[0] < 1:
+        raise ValueError("rotary_dim must be a multiple of 16 and at most head_dim, with at least one position")
+    if positions is None:
+        raise ValueError("a rotating append needs positions (the plan has none)")
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in _INTS or tuple(positions.shape) != (t,):
+        raise ValueError("positions must be an int32 or int64 tensor with one entry per packed token")
+    if positions.device != dev:
+        if positions.is_cuda:
+            raise ValueError("positions must be on the cached entry's device or on the CPU")
+        if t and (int(positions.min()) < 0 or int(positions.max()) >= cos.shape[0]):
+            raise ValueError(f"positions must lie in [0, {int(cos.shape[0])})")
+        positions = positions.to(dev)
+    return aligned16(cos), aligned16(sin), positions.contiguous()
+
+
+def rotate_append(entry, q, k, v, *, q_meta: PackMetadata, slots, cos, sin, positions, interleaved: bool):
+    """The rows of k and v, k rotated, to their slots of ``entry``'s pools, and q rotated, in one
+    HIP launch (fmlm_rotate_append); the kernel of :meth:`InferenceCache.append_paged_kv_cache`
+    for calls that rotate and for 4-bit contexts.  Returns the rotated q (None without)."""
+    dev, d, h, t = entry.device, entry.head_dim, entry.num_heads, int(q_meta.total_tokens)
+    _require_device(k, what="append_paged_kv_cache")
+    if cos is not None:
+        cos, sin, positions = _tables(cos, sin, positions, d=d, t=t, dev=dev)
+    packed = k.ndim == 2
+    out = None
+    if q is not None:
+        if q.shape != k.shape:
+            raise ValueError("q must be laid out like k")
+        if q.dtype != entry.dtype or q.device != dev:
+            raise ValueError("q dtype/device must match the cached entry")
+        refuse_tangents("append_paged_kv_cache", q)
+        if q.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the rotated q has no gradient; use qk_norm_rope, or call under torch.no_grad()")
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    cu = pack_indices(q_meta, dev)[0]
+    if k.numel() == 0:
+        return out
+    p = _lib.AppendParams()
+    p.dtype = _lib.dtype_code(entry.dtype)
+    p.flags = (
+        (_lib.AP_INTERLEAVED if interleaved else 0)
+        | (_lib.AP_FP4 if entry.k_scales is not None else 0)
+        | (_lib.AP_POSITIONS_I64 if cos is not None and positions.dtype == torch.int64 else 0)
+    )
+    p.layout = _lib.LAYOUT_PACKED if packed else _lib.LAYOUT_PADDED
+    p.B, p.H, p.N, p.D, p.T = int(q_meta.B), h, int(q_meta.N), d, t
+    if p.B * p.N > 0x7FFFFFFF:
+        raise ValueError("the call must have fewer than 2**31 tokens")
+    p.pool_rows = int(entry.total_context_len)
+    p.cu_seqlens, p.slots = cu.data_ptr(), slots.data_ptr()
+    if cos is not None:
+        p.cos, p.sin, p.positions = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
+        p.rotary_dim, p.table_rows = 2 * int(cos.shape[1]), int(cos.shape[0])
+    keep = []
+    for a, src, dst, scales in ((p.q, q, out, None), (p.k, k, entry.k_cache, entry.k_scales),
+                                (p.v, v, entry.v_cache, entry.v_scales)):
+        if src is None or dst.numel() == 0:
+            continue
+        src = aligned16(src) if packed else rows16(src)
+        keep.append(src)
+        a.src, a.dst, a.scales = src.data_ptr(), dst.data_ptr(), _lib.ptr(scales)
+        if packed:
+            a.s_sh, a.s_sn = t * d, d
+        else:
+            a.s_sb, a.s_sh, a.s_sn, _ = src.stride()
+    if packed:
+        p.q.d_sh, p.q.d_sn = t * d, d
+    else:
+        p.q.d_sb, p.q.d_sh, p.q.d_sn = h * p.N * d, p.N * d, d
+    with _device_scope(dev):
+        rc = _lib.load().fmlm_rotate_append(p, _lib.stream_of(dev))
+    _lib.check(rc, "fmlm_rotate_append")
+    return out

@@ -22,6 +22,7 @@ from flash_mlm.host.host import (
     _packed_context,
     _page_stride,
     _prepare,
+    _refuse_fp4,
     _tkey,
     _wants_grad,
     AttnLaunch,
@@ -158,6 +159,7 @@ def flash_attn_mlm_tree(
     a forward-mode tangent too.
     """
     memo, entry, mask = q_meta.launch_memo, _entry_of(inference_cache, layer_id), tree.mask
+    _refuse_fp4(inference_cache, layer_id)
     context = (entry.k_cache, entry.v_cache) if entry is not None else ()
     refuse_tangents("flash_attn_mlm_tree", q, k, v, *context)
     if _wants_grad(q, k, v, *context):

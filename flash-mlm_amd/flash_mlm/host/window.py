@@ -1,0 +1,303 @@
+"""Window attention with sinks: attention of a sequence's tokens to a window of recent keys and a
+few first ones, over cached contexts in 16 or 4 bits and for training.  An extension: the
+reference's queries see all keys."""
+
+from __future__ import annotations
+
+import weakref
+
+import torch
+
+from flash_mlm import _lib
+from flash_mlm.host.cache import PAGE_ROWS, InferenceCache, PackMetadata
+from flash_mlm.host.host import _context_index, _entry_of, _tkey, rows16
+from flash_mlm.host.host_utils import (
+    _device_scope,
+    aligned16,
+    capture_leaves,
+    keep_leaves,
+    pack_indices,
+    refuse_tangents,
+    require_cuda_tensors,
+    validate_cache_request,
+)
+
+_HEAD_DIMS = (32, 64, 128, 256)
+_MAX = (1 << 30) - 2
+_MEMO_MAX = 16
+
+
+def _limit(x, what: str) -> int:
+    if x is None:
+        return -1
+    if isinstance(x, bool) or not isinstance(x, int) or x < 0:
+        raise ValueError(f"{what} must be an integer >= 0 (window sides: or None, no limit)")
+    return min(x, _MAX)
+
+
+class _Call:
+    """The checked arguments of a call as parameter blocks without the addresses of its own rows."""
+
+    __slots__ = ("params", "window", "nbytes", "out_shape", "entry_ref", "keep", "cu")
+
+    def run(self, q, k, v, lse=None):
+        """One launch on rows laid out as the call's; returns the output."""
+        p = _lib.AttnParams.from_buffer_copy(self.params)
+        dev = q.device
+        out = torch.empty(self.out_shape, dtype=q.dtype, device=dev)
+        p.q, p.o = q.data_ptr(), out.data_ptr()
+        if k is not None:
+            p.k, p.v = k.data_ptr(), v.data_ptr()
+        lib = _lib.load()
+        ws, nbytes = None, self.nbytes
+        if lse is not None:
+            p.lse = lse.data_ptr()
+        elif nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
+        with _device_scope(dev):
+            rc = lib.fmlm_window_fwd(p, self.window, _lib.stream_of(dev))
+        del ws  # held until here
+        _lib.check(rc, "fmlm_window_fwd")
+        return out
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    return rows16(t) if t.ndim == 4 else aligned16(t)
+
+
+def _strides(t: torch.Tensor, tokens: int):
+    """Element strides (batch, head, position) of padded rows [B, H, N, D] or packed ones [H * T, D]."""
+    if t.ndim == 4:
+        return t.stride()[:3]
+    return 0, tokens * int(t.shape[1]), int(t.shape[1])
+
+
+def _context(entry, p, w, *, b: int, context_index, appended: bool, device):
+    """The fields of the cached context ``entry``; returns the tensors they point to."""
+    cu_kv = entry.cu_seqlens_kv
+    if cu_kv is None:
+        raise ValueError("window attention needs a packed or paged context (with cu_seqlens_kv)")
+    cbs, total, d = entry.context_batch_size, int(entry.total_context_len), entry.head_dim
+    index = _context_index(context_index, b=b, cbs=cbs, prefill=False, context_batch_size=None, device=device)
+    if index is None and 1 < cbs < b:
+        raise ValueError("context_batch_size must be 1 or at least the batch size")
+    if index is None and appended and cbs < b:
+        raise ValueError("tokens in the context need a context batch for each sequence")
+    cu_kv = cu_kv.to(torch.int32).contiguous()
+    p.cu_seqlens_kv, p.ctx_batch, p.ctx_index = cu_kv.data_ptr(), cbs, _lib.ptr(index)
+    p.ctx_rows, p.c_sh, p.c_sn = total, total * d, d
+    k, v = entry.k_cache, entry.v_cache
+    if entry.block_table is not None:
+        p.ctx_block_table, p.ctx_pages_per_batch = entry.block_table.data_ptr(), int(entry.block_table.shape[1])
+        p.ctx_page_stride, p.ctx_rows = PAGE_ROWS * d, total // PAGE_ROWS
+        if total == 0:  # no page to read
+            p.ctx_pages_per_batch = 0
+    elif k.numel():
+        k, v = aligned16(k), aligned16(v)
+    if k.numel():
+        p.k_ctx, p.v_ctx = k.data_ptr(), v.data_ptr()
+    if entry.k_scales is not None:
+        w.flags |= _lib.WINDOW_FP4
+        w.k_scales, w.v_scales = entry.k_scales.data_ptr(), entry.v_scales.data_ptr()
+    return k, v, cu_kv, index
+
+
+def _build(q, k, v, num_heads: int, q_meta: PackMetadata, scale, left, right, sinks, entry, context_index) -> _Call:
+    """The checks of a call, and its parameter blocks."""
+    if q.ndim not in (2, 4):
+        raise ValueError("q must be padded [B, H, N, D] or packed [H * T, D]")
+    if (k is None) != (v is None):
+        raise ValueError("k and v come together")
+    if k is not None and (k.shape != q.shape or v.shape != q.shape):
+        raise ValueError("q, k, v must have the same shape")
+    t, d, dev = int(q_meta.total_tokens), int(q.shape[-1]), q.device
+    if num_heads < 1:
+        raise ValueError("num_heads must be >= 1")
+    if q.ndim == 4:
+        if q.shape[1] != num_heads:
+            raise ValueError("q/k/v head dimension must match num_heads")
+        if q.shape[0] != q_meta.B or q.shape[2] != q_meta.N:
+            raise ValueError("q_meta shape metadata does not match q/k/v padded shape")
+    elif q.shape[0] != num_heads * t:
+        raise ValueError("q first dim must equal num_heads * q_meta.total_tokens")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("window attention needs bf16 or fp16 inputs")
+    if d not in _HEAD_DIMS:
+        raise ValueError("window attention needs head_dim 32, 64, 128 or 256")
+    if k is not None and (k.dtype != q.dtype or v.dtype != q.dtype):
+        raise ValueError("q, k and v must have the same dtype")
+    if k is not None and (k.device != dev or v.device != dev):
+        raise ValueError("q, k and v must be on one device")
+    if t >= _MAX or int(q_meta.B) * int(q_meta.N) > 0x7FFFFFFF:
+        raise ValueError("the call must have fewer than 2**30 tokens")
+    require_cuda_tensors(q, k, v)
+    cu = pack_indices(q_meta, dev)[0]
+
+    call = _Call()
+    p, w = call.params, call.window = _lib.AttnParams(), _lib.Window()
+    p.dtype = _lib.dtype_code(q.dtype)
+    p.B, p.H, p.D, p.N, p.total_q = int(q_meta.B), num_heads, d, int(q_meta.N), t
+    p.scale, p.cu_seqlens_q = float(scale), cu.data_ptr()
+    w.left, w.right, w.sinks = left, right, sinks
+    context = None
+    if k is None:
+        w.flags = _lib.WINDOW_APPENDED
+        if entry is None:
+            raise ValueError("without k and v the tokens must be in the layer's cached context")
+    if entry is not None:
+        if (entry.is_mla, entry.num_heads, entry.head_dim) != (False, num_heads, d):
+            raise ValueError("the layer's cached context has another mode (MLA), num_heads or head_dim")
+        if entry.dtype != q.dtype or entry.device != dev:
+            raise ValueError("cached context dtype/device must match q")
+        context = _context(entry, p, w, b=p.B, context_index=context_index, appended=k is None, device=dev)
+    elif context_index is not None:
+        raise ValueError("context_index needs a cached context")
+    # layouts, from rows as the kernel reads them
+    q_, k_, v_ = _rows(q), None if k is None else _rows(k), None if v is None else _rows(v)
+    layout = _lib.LAYOUT_PADDED if q.ndim == 4 else _lib.LAYOUT_PACKED
+    p.q_layout, p.kv_layout, p.o_layout = layout, layout, _lib.LAYOUT_PACKED
+    p.q_sb, p.q_sh, p.q_sn = _strides(q_, t)
+    p.o_sh, p.o_sn = t * d, d
+    if k is not None:
+        p.k_sb, p.k_sh, p.k_sn = _strides(k_, t)
+        p.v_sb, p.v_sh, p.v_sn = _strides(v_, t)
+    call.out_shape = (num_heads * t, d)
+    call.entry_ref = None if entry is None else weakref.ref(entry)
+    call.cu = q_meta.cu_seqlens
+    call.keep = (cu, context)
+    # sizes of the split's records: the addresses that the checks ask for come with each run
+    p.q = p.o = 256
+    if k is not None:
+        p.k = p.v = 256
+    nbytes = _lib.load().fmlm_window_workspace_bytes(p, w) if t else 0
+    _lib.check(nbytes if nbytes < 0 else 0, "fmlm_window_workspace_bytes")
+    call.nbytes = nbytes
+    return call, (q_, k_, v_)
+
+
+class _Window(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, call, q, k, v):
+        rows = _rows(q), _rows(k), _rows(v)
+        lse = torch.empty(call.params.H * call.params.total_q, dtype=torch.float32, device=q.device)
+        out = call.run(*rows, lse=lse)
+        ctx.call = call
+        # read from there in the backward: autograd may free these and bring others
+        ctx.save_for_backward(q, k, v, out, lse)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        call = ctx.call
+        q, k, v, out, lse = ctx.saved_tensors
+        t = call.params.total_q
+        if dout.shape != out.shape:
+            raise ValueError("gradient of the attention output has the wrong shape")
+        q, k, v, out, lse, dout = *(_rows(x) for x in (q, k, v)), *(aligned16(x) for x in (out, lse, dout))
+        p = _lib.AttnParams.from_buffer_copy(call.params)
+        g = _lib.AttnGrads()
+        p.q, p.k, p.v, p.o, p.lse = (x.data_ptr() for x in (q, k, v, out, lse))
+        p.q_sb, p.q_sh, p.q_sn = _strides(q, t)
+        p.k_sb, p.k_sh, p.k_sn = _strides(k, t)
+        p.v_sb, p.v_sh, p.v_sn = _strides(v, t)
+        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+        g.dout, g.dq, g.dk, g.dv = (x.data_ptr() for x in (dout, dq, dk, dv))
+        g.do_sh, g.do_sn = p.o_sh, p.o_sn
+        g.dq_sb, g.dq_sh, g.dq_sn = _strides(dq, t)
+        g.dk_sb, g.dk_sh, g.dk_sn = _strides(dk, t)
+        g.dv_sb, g.dv_sh, g.dv_sn = _strides(dv, t)
+        ws = torch.empty(p.H * t, dtype=torch.float32, device=q.device)
+        g.workspace, g.workspace_bytes = ws.data_ptr(), 4 * ws.numel()
+        with _device_scope(q.device):
+            rc = _lib.load().fmlm_window_bwd(p, call.window, g, _lib.stream_of(q.device))
+        _lib.check(rc, "fmlm_window_bwd")
+        return None, dq, dk, dv
+
+
+def flash_attn_mlm_window(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    v: torch.Tensor | None,
+    num_heads: int,
+    q_meta: PackMetadata,
+    scale: float,
+    *,
+    window: tuple[int | None, int | None] = (None, None),
+    sinks: int = 0,
+    inference_cache: InferenceCache | None = None,
+    layer_id: int | str | None = None,
+    context_index: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention within a window of positions, with a few first tokens that stay visible.
+
+    q, k, v: padded [B, H, N, D] or packed [H * T, D], the tokens that ``q_meta`` describes.  Returns
+    the packed output [H * T, D] (head-major).  Keys are numbered from the first row of the sequence's
+    cached context, the new tokens after them, and token i of a sequence with n context rows is at
+    position s = n + i.  With ``window`` = (left, right) it sees the keys j with
+
+      j <= s + right  and  (j >= s - left  or  j < sinks)
+
+    None is no limit: (255, 0) is causal over 256 tokens, (64, 64) local both ways, (None, None)
+    what :func:`flash_attn_mlm_compressed` computes.  A row that sees no key is zero.
+
+    ``k`` and ``v`` None: the new tokens have been appended already
+    (:meth:`InferenceCache.append_paged_kv_cache`) and are the last L_b rows of their sequence's
+    context; s = n - L_b + i.
+
+    The context is the layer's packed, paged or 4-bit entry (none: no context), with
+    ``context_index`` as in :func:`flash_attn_mlm_compressed`.  bf16 and fp16, D = 32, 64, 128 or 256,
+    no MLA.  Differentiable in q, k and v without a cached context, for finite inputs; gradients are
+    the same bits every time, those of padding rows zero.  With a context, inputs that
+    require grad raise ValueError (use ``torch.no_grad()``); with a forward-mode tangent always.  A
+    call that is captured into a graph and takes leaves that require grad raises ValueError while
+    outputs of earlier calls on them are alive.
+    """
+    entry = _entry_of(inference_cache, layer_id)
+    refuse_tangents("flash_attn_mlm_window", q, k, v)
+    grad = torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v))
+    call = key = None
+    if context_index is None and isinstance(window, tuple):
+        # all that the checks depend on
+        key = ("window", _tkey(q), None if k is None else _tkey(k), None if v is None else _tkey(v), num_heads,
+               q_meta.B, q_meta.N, q_meta.total_tokens, float(scale), window, sinks, None if entry is None else id(entry),
+               inference_cache is None, layer_id is None)
+        call = q_meta.launch_memo.get(key)
+        if call is not None and (call.cu is not q_meta.cu_seqlens or
+                                 (None if call.entry_ref is None else call.entry_ref()) is not entry):
+            call = None
+    rows = (q, k, v)
+    if call is None:
+        validate_cache_request(prefill=False, inference_cache=inference_cache, layer_id=layer_id)
+        if not isinstance(window, (tuple, list)) or len(window) != 2:
+            raise ValueError("window must be a pair (left, right)")
+        left, right = (_limit(x, "window") for x in window)
+        if sinks is None:
+            raise ValueError("sinks must be an integer >= 0")
+        call, rows = _build(q, k, v, num_heads, q_meta, scale, left, right, _limit(sinks, "sinks"), entry, context_index)
+        cu, context = call.keep
+        if (key is not None and rows[0] is q and rows[1] is k and rows[2] is v and cu is q_meta.cu_seqlens
+                and (context is None or (context[0] is entry.k_cache and context[1] is entry.v_cache
+                                         and context[2] is entry.cu_seqlens_kv))):
+            if len(q_meta.launch_memo) >= _MEMO_MAX:
+                q_meta.launch_memo.clear()
+            # the entry's tensors are held by the entry alone, as in the other memos
+            stored = _Call()
+            for name in _Call.__slots__:
+                setattr(stored, name, getattr(call, name))
+            stored.keep = None
+            q_meta.launch_memo[key] = stored
+    if grad:
+        if entry is not None:
+            raise ValueError("flash_attn_mlm_window has no backward over a cached context; call it under torch.no_grad()")
+        leaves = capture_leaves("flash_attn_mlm_window", q, k, v)
+        if call.params.total_q:
+            out = _Window.apply(call, q, k, v)
+            keep_leaves(leaves)
+            return out
+    if entry is not None and torch.is_grad_enabled() and entry.k_cache.requires_grad:
+        raise ValueError("flash_attn_mlm_window has no gradient of a cached context; call it under torch.no_grad()")
+    if call.params.total_q == 0:
+        return torch.empty(call.out_shape, dtype=q.dtype, device=q.device)
+    return call.run(*rows)

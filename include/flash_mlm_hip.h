@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define FMLM_ABI_VERSION 6
+#define FMLM_ABI_VERSION 7
 
 /* element types */
 enum {
@@ -512,6 +512,87 @@ FMLM_API int fmlm_attn_tree_tile(const fmlm_attn_params* p); /* the tile_config 
 FMLM_API int64_t fmlm_attn_tree_workspace_bytes(const fmlm_attn_params* p);
 FMLM_API int fmlm_attn_tree_fwd(const fmlm_attn_params* p, const uint64_t* mask, int32_t words, void* tree_workspace,
                                 int64_t tree_workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Window attention.  fmlm_attn_fwd's call p with a limit on what a query sees: keys are numbered
+ * from the first context row on, the main keys after them, and the query of token i of a
+ * sequence with n context rows is at position n + i (FMLM_WINDOW_APPENDED: n - L + i, the
+ * sequence's L tokens are its last context rows already and there are no main keys).  The
+ * query at position s sees key j if
+ *   j <= s + right  and  (j >= s - left  or  j < sinks).
+ * left, right < 0: no limit.  A row that sees no key has output 0.
+ *
+ * p: bf16 or fp16, D = 32, 64, 128 or 256, flags 0, packed sequences (cu_seqlens_q); q, k and v
+ * padded or packed, the output packed or padded; main keys linear; the context packed
+ * (cu_seqlens_kv), paged, or none (cu_seqlens_kv NULL, ctx_len 0); ctx_index as there.  p->schedule
+ * and tile_config are not used.
+ *
+ * 4-bit context (FMLM_WINDOW_FP4, paged only): rows of E2M1 codes, element 2i in the low and
+ * 2i + 1 in the high half of byte i, and for every 32 elements of a row the scale 2^(x - 127) as a
+ * byte x.  p->k_ctx / v_ctx are the codes, c_sh, c_sn and ctx_page_stride count elements (so
+ * offset / 2 bytes of codes, offset / 32 scales).  fp16 holds every value of scale bytes 104 to
+ * 140, bf16 of those up to 252.
+ * ------------------------------------------------------------------------- */
+enum { FMLM_WINDOW_APPENDED = 1, FMLM_WINDOW_FP4 = 2 };
+
+typedef struct fmlm_window {
+  int32_t left, right, sinks, flags;
+  const uint8_t* k_scales; /* FMLM_WINDOW_FP4 */
+  const uint8_t* v_scales;
+} fmlm_window;
+
+FMLM_API int fmlm_window_size(void);
+/* p->workspace: fmlm_window_workspace_bytes(p, w) (0 where key ranges are not split; p->lse, and
+ * FMLM_FLAG_NOSPLIT in p->flags, rule that out) */
+FMLM_API int64_t fmlm_window_workspace_bytes(const fmlm_attn_params* p, const fmlm_window* w);
+FMLM_API int fmlm_window_fwd(const fmlm_attn_params* p, const fmlm_window* w, void* stream);
+/* Gradients of a call without a context whose forward stored p->lse; g as in fmlm_attn_bwd (no
+ * dk_ctx, dv_ctx), of which it writes every row of every sequence, padding rows as zeros.
+ * g->workspace: H * total_q floats. */
+FMLM_API int fmlm_window_bwd(const fmlm_attn_params* p, const fmlm_window* w, const fmlm_attn_grads* g, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Appends to a paged context with the position rotation on the way: of the packed tokens t, with
+ * c, s = cos, sin[positions[t]] (rows of rotary_dim / 2 floats), the first rotary_dim elements of
+ * q's and k's rows become (a c - b s, a s + b c) for the pairs (a, b) = (i, i + rotary_dim / 2), or
+ * (2i, 2i + 1) with FMLM_AP_INTERLEAVED.  q goes to q.dst (padding rows as zeros), k and v to row
+ * slots[t] of their pools (heads pool_rows rows apart); slots outside [0, pool_rows) are not
+ * stored.  Positions are clamped to the table_rows of the tables.  With FMLM_AP_FP4 the pools hold
+ * 4-bit rows (see above): the scale of a block is the smallest 2^e with which its magnitudes are
+ * below 7 2^e, e within [-23, 13] (fp16) or [-125, 125] (bf16); codes are rounded to nearest
+ * even, to at most 6; infinities count as the type's largest value, NaN as 0.
+ * k's values are rotated in 64 bits there, so that no rounding but the codes' decides a code.
+ * A tensor with dst NULL is left out; cos NULL (rotary_dim 0): nothing is rotated.
+ * ------------------------------------------------------------------------- */
+enum { FMLM_AP_INTERLEAVED = 1, FMLM_AP_FP4 = 2, FMLM_AP_POSITIONS_I64 = 4 };
+
+typedef struct fmlm_append_rows {
+  const void* src;
+  int64_t s_sb, s_sh, s_sn; /* padded: b*sb + h*sh + p*sn, packed: h*sh + t*sn                */
+  void* dst;                /* q: rows of its own strides; k, v: the pool                    */
+  int64_t d_sb, d_sh, d_sn; /* q only                                                        */
+  uint8_t* scales;          /* k, v with FMLM_AP_FP4                                         */
+} fmlm_append_rows;
+
+typedef struct fmlm_append_params {
+  int32_t dtype, flags, layout;
+  int32_t B, H, N, D, rotary_dim, T;
+  int32_t reserved;
+  int64_t table_rows, pool_rows;
+  const float* cos;
+  const float* sin;
+  const void* positions;      /* [T]                                                         */
+  const int32_t* cu_seqlens;  /* [B + 1]                                                     */
+  const int64_t* slots;       /* [T]                                                         */
+  fmlm_append_rows q, k, v;
+} fmlm_append_params;
+
+FMLM_API int fmlm_append_params_size(void);
+FMLM_API int fmlm_rotate_append(const fmlm_append_params* p, void* stream);
+
+/* The values of `rows` 4-bit rows of D elements (contiguous codes and scales), as bf16 or fp16. */
+FMLM_API int fmlm_fp4_values(int32_t dtype, const uint8_t* codes, const uint8_t* scales, void* out, int64_t rows,
+                             int32_t D, void* stream);
 
 #ifdef __cplusplus
 }
