@@ -16,7 +16,6 @@
 #include "fmlm_common.h"
 
 #include <algorithm>
-#include <mutex>
 #include <type_traits>
 
 #include "fmlm_fp4.h"
@@ -42,6 +41,7 @@ struct WinArgs {
   const uint8_t* k_scales;
   const uint8_t* v_scales;
   float* records;
+  void* o_low;  // what the rounding of o took away, for the backward
 };
 
 // ---- a sequence of the call: its tokens, its keys, the position of its first token
@@ -120,11 +120,27 @@ struct WTile {
     const s16x4 lo = lds_read_tr16(a), hi = lds_read_tr16(a + 16 * ROWB);
     return __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
+  // the lane's offsets of a whole tile of ROWS rows at `pitch` bytes, and its loads with them
+  template <int ROWS>
+  static FMLM_DEV void offsets(uint32_t pitch, int wave, int lane, uint32_t (&off)[ROWS / (RPI * kNW)]) {
+#pragma unroll
+    for (int j = 0; j < ROWS / (RPI * kNW); ++j) {
+      const int row = (wave + j * kNW) * RPI + lane / CPR;
+      off[j] = (uint32_t)row * pitch + 16u * (uint32_t)((lane % CPR) ^ kv_swz<D>(row));
+    }
+  }
+  template <int ROWS>
+  static FMLM_DEV void load_at(const char* src, const uint32_t (&off)[ROWS / (RPI * kNW)], uint32_t lds, int wave) {
+#pragma unroll
+    for (int j = 0; j < ROWS / (RPI * kNW); ++j)
+      dma16_sbase(src, off[j], __builtin_amdgcn_readfirstlane(lds + (wave + j * kNW) * 1024));
+  }
   // starts the loads of ROWS rows from src at `pitch` bytes; rows past `last` repeat it
   template <int ROWS>
   static FMLM_DEV void load(const char* src, uint32_t pitch, int last, uint32_t lds, int wave, int lane) {
     src = uniform_ptr(src);
     pitch = __builtin_amdgcn_readfirstlane(pitch);
+    asm volatile("" : "+v"(lane));  // (offsets of a rare tile: computed here, not kept)
 #pragma unroll
     for (int j = 0; j < ROWS / (RPI * kNW); ++j) {
       const int i = wave + j * kNW, row = i * RPI + lane / CPR;
@@ -152,25 +168,40 @@ FMLM_DEV uint32_t pack2(float x, float y) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, typename Pair<T>::type));
 }
 
-template <int D>
+// K tiles are double-buffered, V tiles have a third buffer where it fits beside a second workgroup
+// on the CU (80 KB each): their loads then have two steps to land.
+template <int D, bool FP4>
 struct FwdCfg {
   static constexpr int TILEB = kBK * D * 2;
-  static constexpr int LDS = 4 * TILEB;  // two K and two V tiles
+  static constexpr int NV = FP4 || D == 256 ? 2 : 3;
+  static constexpr bool STAGE = FP4 && D == 128;  // codes wait in LDS (else in registers)
+  static constexpr int LDS = (2 + NV) * TILEB + (STAGE ? 2 * kNW * 1024 : 0);
   static constexpr int WPS = D <= 128 ? 2 : 1;
   static constexpr int KC = D / 32, NDB = D / 16;
+  static constexpr int LEAD = D <= 64 ? 2 : 3;  // LDS fragment reads in flight ahead of use
+  static constexpr int NKF = KC * 4, NVF = 2 * NDB;  // K and V fragments of a tile
+  static constexpr int CW = D / 32;                  // dwords of codes of a thread: a quarter row
+  static constexpr int CS = FP4 && D == 256 ? 2 : 1;  // and their scales
 };
 
 // ---------------------------------------------------------------------------
-// Forward
+// Forward.  Step v of the walk computes S(v + 1) beside the exponentials of P(v), then O += V(v)^T P(v)
+// beside the row maxima of S(v + 1): fenced slots, each the MFMAs of one LDS fragment and a share of
+// the other work, the fragment of LEAD slots later being read.  In the same step the tiles of later
+// ones load: K(v + 2) into K(v)'s buffer and V(v + NV - 1) into V(v - 1)'s.  4-bit tiles are a step
+// ahead of that: their codes arrive in step v and are converted, by the wave that loaded them, at
+// the start of step v + 1.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int QB, bool FP4>
-__global__ __launch_bounds__(kNW * 64, FwdCfg<D>::WPS) void window_fwd_kernel(const fmlm_attn_params p, const WinArgs a) {
-  typedef FwdCfg<D> C;
+__global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_kernel(const fmlm_attn_params p, const WinArgs a) {
+  typedef FwdCfg<D, FP4> C;
   typedef typename Mfma<T>::v8 v8;
-  constexpr int BQ = kNW * QB * 16;
+  constexpr int BQ = kNW * QB * 16, CW = C::CW, CS = C::CS;
   extern __shared__ __align__(16) char smem[];
-  auto kbuf = [&](int i) { return smem + i * C::TILEB; };
-  auto vbuf = [&](int i) { return smem + (2 + i) * C::TILEB; };
+  // buffers of tile v; a step takes them from its place among NU unrolled ones, as constants
+  constexpr int NU = C::NV == 2 ? 2 : 6;
+  auto kbuf = [&](int v) { return smem + (v & 1) * C::TILEB; };
+  auto vbuf = [&](int v) { return smem + (2 + v % C::NV) * C::TILEB; };
 
   int g, part, tile;
   win_unit(a, a.parts, g, part, tile);
@@ -182,7 +213,7 @@ __global__ __launch_bounds__(kNW * 64, FwdCfg<D>::WPS) void window_fwd_kernel(co
   const WinTiles wt = win_tiles(a, s, s.first + row0, s.first + row0 + rows - 1);
   const int parts = win_parts(wt.n, a.parts);
   if (part >= parts) return;
-  const int vb = (int)((int64_t)wt.n * part / parts), ve = (int)((int64_t)wt.n * (part + 1) / parts);
+  const int vb = (int)((int64_t)wt.n * part / parts), n = (int)((int64_t)wt.n * (part + 1) / parts) - vb;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, gq = lane >> 4;
@@ -192,144 +223,281 @@ __global__ __launch_bounds__(kNW * 64, FwdCfg<D>::WPS) void window_fwd_kernel(co
   const uint32_t qsign = p.scale < 0.f ? 0x80008000u : 0u;
   const float c = fmaxf(fabsf(p.scale) * kLog2e, 1e-30f);
 
-  v8 qf[QB][C::KC];
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const int row = (wave * QB + qb) * 16 + l16;
-    const int64_t off = row_at(p.q_layout, s.b, s.h, s.q0, row0 + row, p.q_sb, p.q_sh, p.q_sn);
-#pragma unroll
-    for (int kc = 0; kc < C::KC; ++kc) {
-      const u32x4 r = __builtin_bit_cast(u32x4, ld_frag<T>(p.q, off + kc * 32 + gq * 8, row < rows));
-      qf[qb][kc] = __builtin_bit_cast(v8, r ^ qsign);
-    }
-  }
-
-  // ---- loads
+  // ---- loads of tile v of this part: t(v) of the walk
+  auto tile_at = [&](int v) { return __builtin_amdgcn_readfirstlane(wt.tile(vb + v)); };
   const int cb = ctx_batch_of(p, s.b);
   int ctx0 = 0, ctx1;
   ctx_range(p, cb, ctx0, ctx1);
   const int32_t* const pages = p.ctx_block_table ? p.ctx_block_table + (int64_t)cb * p.ctx_pages_per_batch : nullptr;
   auto keys_in = [&](int t) { return min(kBK, t < wt.nt0 ? s.ctx - t * kBK : s.total - s.ctx - (t - wt.nt0) * kBK); };
+  // Page ids of 64 consecutive tiles, one a lane: a tile then costs a lane read.  (One load a tile
+  // would wait, with everything in flight, a round trip each.)
+  int win_ids = 0, win_first = -(1 << 30);
+  auto page_of = [&](int t) {
+    if ((unsigned)(t - win_first) >= 64u) {
+      win_first = t;
+      win_ids = pages[min(t + lane, max(p.ctx_pages_per_batch - 1, 0))];
+      asm volatile("" ::"v"(win_ids));  // (the wait for it stays here)
+    }
+    return min(max(__builtin_amdgcn_readlane(win_ids, t - win_first), 0), max(p.ctx_rows - 1, 0));
+  };
   // context tile t's first row, in elements of a pool or a packed context
   auto ctx_elem = [&](int t) {
-    if (!pages) return (int64_t)s.h * p.c_sh + (int64_t)(ctx0 + t * kBK) * p.c_sn;
-    const int pg = min(max(ldc(pages, t), 0), max(p.ctx_rows - 1, 0));
-    return (int64_t)s.h * p.c_sh + (int64_t)pg * p.ctx_page_stride;
+    return (int64_t)s.h * p.c_sh + (pages ? (int64_t)page_of(t) * p.ctx_page_stride : (int64_t)(ctx0 + t * kBK) * p.c_sn);
   };
-  // a 4-bit tile: a quarter of a row each of 256 threads, D / 8 bytes
-  constexpr int CW = FP4 ? D / 32 : 1;  // dwords of codes
-  constexpr int CS = FP4 && D == 256 ? 2 : 1;  // scales
-  uint32_t kcode[CW], vcode[CW], ksc[CS], vsc[CS];
-  auto load_codes = [&](const void* codes, const uint8_t* scales, int64_t e, uint32_t (&w)[CW], uint32_t (&sc)[CS]) {
-    const char* src = (const char*)codes + e / 2;
-    if constexpr (CW == 1) w[0] = *(const uint32_t*)src;
-    else if constexpr (CW == 2) { const u32x2 x = *(const u32x2*)src; w[0] = x[0]; w[1] = x[1]; }
-    else
+  // a 16-bit tile's loads
+  auto fetch = [&](int t, bool is_v, char* to) {
+    const int last = keys_in(t) - 1;
+    if (t < wt.nt0) {
+      WTile<T, D>::template load<kBK>((const char*)(is_v ? p.v_ctx : p.k_ctx) + ctx_elem(t) * 2, (uint32_t)p.c_sn * 2u, last,
+                                      lds_addr(to), wave, lane);
+    } else {
+      const int64_t sb = is_v ? p.v_sb : p.k_sb, sh = is_v ? p.v_sh : p.k_sh, sn = is_v ? p.v_sn : p.k_sn;
+      WTile<T, D>::template load<kBK>((const char*)(is_v ? p.v : p.k) + row_at(p.kv_layout, s.b, s.h, s.q0, (t - wt.nt0) * kBK, sb, sh, sn) * 2,
+                                      (uint32_t)sn * 2u, last, lds_addr(to), wave, lane);
+    }
+  };
+  // The walk of the 16-bit tiles: the next tile's first rows of K and V, moved on by their pitch, a page or
+  // (the first tile of the band, and of the new tokens) from the segment's start.
+  struct Walk {
+    const char *k, *v;
+    uint32_t rk, rv;
+    int at, t;
+  } wk{nullptr, nullptr, 0, 0, 0, 0};
+  auto seek = [&](int v) {  // to tile v of this part
+    wk.at = v;
+    wk.t = tile_at(v);
+    if (wk.t < wt.nt0) {
+      const int64_t e = ctx_elem(wk.t) * 2;
+      wk.rk = wk.rv = __builtin_amdgcn_readfirstlane((uint32_t)p.c_sn * 2u);
+      wk.k = uniform_ptr((const char*)p.k_ctx + e);
+      wk.v = uniform_ptr((const char*)p.v_ctx + e);
+    } else {
+      const int j = (wk.t - wt.nt0) * kBK;
+      wk.rk = __builtin_amdgcn_readfirstlane((uint32_t)p.k_sn * 2u);
+      wk.rv = __builtin_amdgcn_readfirstlane((uint32_t)p.v_sn * 2u);
+      wk.k = uniform_ptr((const char*)p.k + row_at(p.kv_layout, s.b, s.h, s.q0, j, p.k_sb, p.k_sh, p.k_sn) * 2);
+      wk.v = uniform_ptr((const char*)p.v + row_at(p.kv_layout, s.b, s.h, s.q0, j, p.v_sb, p.v_sh, p.v_sn) * 2);
+    }
+  };
+  const int jump = wt.sink - vb;  // the first tile of the band, in this part's count
+  auto move = [&]() {
+    const int v = wk.at + 1;
+    if (v >= n) return;
+    if (v == jump || wk.t + 1 == wt.nt0 || (pages && wk.t < wt.nt0)) {
+      seek(v);
+      return;
+    }
+    wk.at = v;
+    wk.t += 1;
+    wk.k += (size_t)wk.rk * kBK;
+    wk.v += (size_t)wk.rv * kBK;
+  };
+  // lane offsets of a whole tile at the pitch of most of them
+  typedef WTile<T, D> Tile;
+  constexpr int NL = kBK / (Tile::RPI * kNW);
+  uint32_t off0[FP4 ? 1 : NL];
+  uint32_t pitch0 = 0;
+  auto load_rows = [&](const char* src, uint32_t pitch, int last, char* to) {
+    if constexpr (!FP4) {
+      if (last == kBK - 1 && pitch == pitch0) {
+        Tile::template load_at<kBK>(src, off0, lds_addr(to), wave);
+        return;
+      }
+    }
+    Tile::template load<kBK>(src, pitch, last, lds_addr(to), wave, lane);
+  };
+  // a 4-bit tile: thread i has quarter i % 4 of row i / 4, CW dwords
+  uint32_t code[2][C::STAGE ? 1 : CW], csc[2][CS];
+  auto fetch_codes = [&](int t, bool is_v) {
+    const int row = min(tid >> 2, keys_in(t) - 1), x = is_v ? 1 : 0;
+    const int64_t e0 = ctx_elem(t);
+    const uint32_t at = (uint32_t)row * D + (tid & 3) * (D / 4);
+    const char* const src = uniform_ptr((const char*)(is_v ? p.v_ctx : p.k_ctx) + e0 / 2);
+    const char* const ssc = uniform_ptr((const char*)(is_v ? a.v_scales : a.k_scales) + e0 / kFp4Block);
+    if constexpr (C::STAGE) {
+      dma16_sbase(src, at / 2, __builtin_amdgcn_readfirstlane(lds_addr(smem) + (2 + C::NV) * C::TILEB + (2 * wave + x) * 1024));
+    } else if constexpr (CW == 1) {
+      code[x][0] = *(const uint32_t*)(src + at / 2);
+    } else if constexpr (CW == 2) {
+      const u32x2 w = *(const u32x2*)(src + at / 2);
+      code[x][0] = w[0];
+      code[x][1] = w[1];
+    } else {
 #pragma unroll
       for (int i = 0; i < CW; i += 4) {
-        const u32x4 x = *(const u32x4*)(src + 4 * i);
+        const u32x4 w = *(const u32x4*)(src + at / 2 + 4 * i);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[i + j] = x[j];
+        for (int j = 0; j < 4; ++j) code[x][i + j] = w[j];
       }
+    }
 #pragma unroll
-    for (int i = 0; i < CS; ++i) sc[i] = scales[e / kFp4Block + i];
+    for (int i = 0; i < CS; ++i) csc[x][i] = (uint8_t)ssc[at / kFp4Block + i];
   };
-  auto issue = [&](int v) {
-    const int t = wt.tile(v), buf = (v - vb) & 1, last = keys_in(t) - 1;
-    if (t < wt.nt0) {
-      const int64_t e = ctx_elem(t);
-      if constexpr (FP4) {
-        const int64_t at = e + (int64_t)min(tid >> 2, last) * D + (tid & 3) * (D / 4);
-        load_codes(p.k_ctx, a.k_scales, at, kcode, ksc);
-        load_codes(p.v_ctx, a.v_scales, at, vcode, vsc);
-      } else {
-        WTile<T, D>::template load<kBK>((const char*)p.k_ctx + e * 2, (uint32_t)p.c_sn * 2u, last, lds_addr(kbuf(buf)), wave, lane);
-        WTile<T, D>::template load<kBK>((const char*)p.v_ctx + e * 2, (uint32_t)p.c_sn * 2u, last, lds_addr(vbuf(buf)), wave, lane);
-      }
+  // the loaded codes as a 16-bit tile (STAGE: this wave's load has landed)
+  auto put_codes = [&](bool is_v, char* to) {
+    const int row = tid >> 2, x = is_v ? 1 : 0;
+    uint32_t w[CW];
+    if constexpr (C::STAGE) {
+      const u32x4 r = *(const u32x4*)(smem + (2 + C::NV) * C::TILEB + (2 * wave + x) * 1024 + 16 * lane);
+#pragma unroll
+      for (int i = 0; i < CW; ++i) w[i] = r[i];
     } else {
-      const int j = (t - wt.nt0) * kBK;
-      WTile<T, D>::template load<kBK>((const char*)p.k + row_at(p.kv_layout, s.b, s.h, s.q0, j, p.k_sb, p.k_sh, p.k_sn) * 2,
-                                      (uint32_t)p.k_sn * 2u, last, lds_addr(kbuf(buf)), wave, lane);
-      WTile<T, D>::template load<kBK>((const char*)p.v + row_at(p.kv_layout, s.b, s.h, s.q0, j, p.v_sb, p.v_sh, p.v_sn) * 2,
-                                      (uint32_t)p.v_sn * 2u, last, lds_addr(vbuf(buf)), wave, lane);
-    }
-  };
-  // the loaded codes as a 16-bit tile
-  auto put_codes = [&](char* tile, const uint32_t (&w)[CW], const uint32_t (&sc)[CS]) {
-    const int row = tid >> 2;
 #pragma unroll
-    for (int i = 0; i < CW; ++i) {
-      const int chunk = (tid & 3) * CW + i;
-      *(u32x4*)(tile + row * (D * 2) + 16 * (chunk ^ kv_swz<D>(row))) = fp4_oct<T>(w[i], fp4_scale(sc[i / 4 % CS]));
+      for (int i = 0; i < CW; ++i) w[i] = code[x][i];
     }
+#pragma unroll
+    for (int i = 0; i < CW; ++i)
+      *(u32x4*)(to + row * (D * 2) + 16 * (((tid & 3) * CW + i) ^ kv_swz<D>(row))) = fp4_oct<T>(w[i], fp4_scale(csc[x][i / 4 % CS]));
   };
+  auto is_code = [&](int t) { return FP4 && t < wt.nt0; };
 
+  v8 qf[QB][C::KC];
   f32x4 o[C::NDB][QB], lsum[QB];
-  float m[QB];
+  float m[QB], mx[QB];
+  f32x4 sa[4][QB], sb[4][QB];
   v8 ones;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = (T)1.0f;
+  pin(ones);
 
-  // Values that are not finite in keys that a row does not see would reach it as 0 inf.  That is
-  // looked for in the result; if it is there, the tiles on an edge are added key by key in a
-  // second pass.
-  for (bool careful = false;; careful = true) {
+  // raw row maxima of a score tile
+  auto row_max = [&](const f32x4 (&x)[4][QB]) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      m[qb] = -INFINITY;
-      lsum[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      float y = vmax(vmax(x[0][qb][0], x[0][qb][1]), vmax(x[0][qb][2], x[0][qb][3]));
 #pragma unroll
-      for (int db = 0; db < C::NDB; ++db) o[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int kb = 1; kb < 4; ++kb)
+        y = vmax(vmax(y, vmax(x[kb][qb][0], x[kb][qb][1])), vmax(x[kb][qb][2], x[kb][qb][3]));
+      mx[qb] = lane_max_xor16_32(y);
     }
-    if (vb < ve) issue(vb);
-    for (int v = vb; v < ve; ++v) {
-      const int t = wt.tile(v), buf = (v - vb) & 1, nk = keys_in(t);
-      if (FP4 && t < wt.nt0) {  // (its buffer was last read two tiles ago)
-        put_codes(kbuf(buf), kcode, ksc);
-        put_codes(vbuf(buf), vcode, vsc);
-      }
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
-      if (v + 1 < ve) issue(v + 1);
-      if (!active) continue;
-      const char *kt = kbuf(buf), *vt = vbuf(buf);
-      f32x4 sc[4][QB];
+  };
+  const int w0 = s.first + row0 + wave * QB * 16, w1 = min(w0 + QB * 16, s.first + row0 + rows) - 1;
+  // scores of keys that a row does not see to -inf; returns whether there can be any
+  auto mask = [&](int t, f32x4 (&x)[4][QB]) {
+    const int nk = keys_in(t), kp = t < wt.nt0 ? t * kBK : s.ctx + (t - wt.nt0) * kBK;
+    if (!(nk < kBK || kp + kBK - 1 > w0 + a.right || (kp < w1 - a.left && kp + kBK > a.sinks))) return false;
 #pragma unroll
-      for (int kc = 0; kc < C::KC; ++kc)
+    for (int qb = 0; qb < QB; ++qb) {
+      const int pos = w0 + qb * 16 + l16, k0 = kp + 4 * gq;  // element (kb, r) is key k0 + 16 kb + r
+      const int top = min(pos + a.right - k0, nk - 1 - 4 * gq), low = pos - a.left - k0, snk = a.sinks - k0;
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-          const v8 x = tr.row(kt, kb, kc);
+      for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-          for (int qb = 0; qb < QB; ++qb)
-            sc[kb][qb] = Mfma<T>::run(x, qf[qb][kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[kb][qb]);
+        for (int r = 0; r < 4; ++r) {
+          const int j = kb * 16 + r;
+          if (!(j <= top && (j >= low || j < snk))) x[kb][qb][r] = -INFINITY;
         }
-      // the tile's keys are at positions from kp on; the wave's rows at [w0, w1]
-      const int kp = t < wt.nt0 ? t * kBK : s.ctx + (t - wt.nt0) * kBK;
-      const int w0 = s.first + row0 + wave * QB * 16, w1 = min(w0 + QB * 16, s.first + row0 + rows) - 1;
-      const bool edge = nk < kBK || kp + kBK - 1 > w0 + a.right || (kp < w1 - a.left && kp + kBK > a.sinks);
-      if (edge) {
+    }
+    return true;
+  };
+
+  // ---- the slots.  Slot s runs the MFMAs of fragment s: [0, NKF) of K(v + 1) (sn += K Q^T, beside a
+  // share of P(v)'s exponentials), [NKF, NF) of V(v) (O += V^T P, beside a share of sn's maxima).
+  constexpr int NF = C::NKF + C::NVF, NP = 4 * QB * 2, NMS = 4 * QB + QB;
+  u32x4 pf[2][QB];
+  auto slots = [&](f32x4 (&sc)[4][QB], f32x4 (&sn)[4][QB], const char* kn, const char* vt) {
+    float ref[QB], mpart[QB], mhold[QB];
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-          const int pos = w0 + qb * 16 + l16, k0 = kp + 4 * gq;  // element (kb, r) is key k0 + 16 kb + r
-          const int top = min(pos + a.right - k0, nk - 1 - 4 * gq), low = pos - a.left - k0, snk = a.sinks - k0;
-#pragma unroll
-          for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int j = kb * 16 + r;
-              if (!(j <= top && (j >= low || j < snk))) sc[kb][qb][r] = -INFINITY;
-            }
+    for (int qb = 0; qb < QB; ++qb) ref[qb] = m[qb] == -INFINITY ? 0.f : -m[qb];  // (no key yet: every score is -inf)
+    v8 fr[C::LEAD + 1];
+    auto issue = [&](int r) {
+      if (r < C::NKF) fr[r % (C::LEAD + 1)] = tr.row(kn, r % 4, r / 4);
+      else fr[r % (C::LEAD + 1)] = tr.col(vt, (r - C::NKF) / C::NDB, (r - C::NKF) % C::NDB);
+    };
+    auto exp_pair = [&](int pi) {
+      const int qb = pi / 8, kb = (pi >> 1) % 4, r = (pi & 1) * 2;
+      if (r == 0) pin(sc[kb][qb]);
+      uint32_t w = pack2<T>(fast_exp2(fmaf(sc[kb][qb][r], c, ref[qb])), fast_exp2(fmaf(sc[kb][qb][r + 1], c, ref[qb])));
+      pin(w);
+      pf[kb >> 1][qb][(kb & 1) * 2 + (pi & 1)] = w;
+    };
+    auto max_step = [&](int k) {
+      if (k < 4 * QB) {
+        const int qb = k / 4, kb = k % 4;
+        pin(sn[kb][qb]);
+        const f32x4 x = sn[kb][qb];
+        if (kb == 0) {
+          mpart[qb] = vmax(vmax(x[0], x[1]), x[2]);
+        } else {
+          mpart[qb] = vmax(vmax(mpart[qb], mhold[qb]), x[0]);
+          mpart[qb] = vmax(vmax(mpart[qb], x[1]), x[2]);
         }
+        mhold[qb] = x[3];
+        if (kb == 3) mpart[qb] = vmax(mpart[qb], mhold[qb]);
+        pin(mpart[qb]);
+      } else {
+        const int qb = k - 4 * QB;
+        mx[qb] = lane_max_xor16_32(mpart[qb]);
+        pin(mx[qb]);
       }
-      float mx[QB];
+    };
+#pragma unroll
+    for (int r = 0; r < C::LEAD; ++r) issue(r);
+    __builtin_amdgcn_s_setprio(1);  // ahead of a wave that waits or loads, the second half highest
+#pragma unroll
+    for (int sl = 0; sl < NF; ++sl) {
+      if (sl + C::LEAD < NF) issue(sl + C::LEAD);
+      if (sl == C::NKF) __builtin_amdgcn_s_setprio(2);
+      const v8 x = fr[sl % (C::LEAD + 1)];
+      if (sl < C::NKF) {
+        const int kb = sl % 4, kc = sl / 4;
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+          sn[kb][qb] = Mfma<T>::run(x, qf[qb][kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sn[kb][qb]);
+#pragma unroll
+        for (int pi = sl * NP / C::NKF; pi < (sl + 1) * NP / C::NKF; ++pi) exp_pair(pi);
+      } else {
+        const int j = sl - C::NKF, ks = j / C::NDB, db = j % C::NDB;
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) o[db][qb] = Mfma<T>::run(x, __builtin_bit_cast(v8, pf[ks][qb]), o[db][qb]);
+        if (db == C::NDB - 1)
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) lsum[qb] = Mfma<T>::run(ones, __builtin_bit_cast(v8, pf[ks][qb]), lsum[qb]);
+#pragma unroll
+        for (int k = j * NMS / C::NVF; k < (j + 1) * NMS / C::NVF; ++k) max_step(k);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  const char* v_next = nullptr;
+  uint32_t v_pitch = 0;
+  int v_last = 0;
+  auto step = [&](int v, int u, f32x4 (&sc)[4][QB], f32x4 (&sn)[4][QB]) {
+    if constexpr (FP4) {
+      const int tk = v + 2 < n ? tile_at(v + 2) : -1, tv = v + 1 < n ? tile_at(v + 1) : -1;
+      if (tk >= 0 && is_code(tk)) put_codes(false, kbuf(u));
+      if (tv >= 0 && is_code(tv)) put_codes(true, vbuf(u + 1));
+      if constexpr (C::STAGE) wait_reads();  // the loads below overwrite what the wave has just read
+      if (tk >= 0 && !is_code(tk)) fetch(tk, false, kbuf(u));
+      if (tv >= 0 && !is_code(tv)) fetch(tv, true, vbuf(u + 1));
+      const int nk = v + 3 < n ? tile_at(v + 3) : -1;
+      if (nk >= 0 && is_code(nk)) fetch_codes(nk, false);
+      if (tk >= 0 && is_code(tk)) fetch_codes(tk, true);
+    } else {
+      // the walk stands at tile v + 2, V's last pointer (two buffers) at v + 1
+      if constexpr (C::NV == 2)
+        if (v + 1 < n) load_rows(v_next, v_pitch, v_last, vbuf(u + 1));
+      if (v + 2 < n) {
+        const int last = keys_in(wk.t) - 1;
+        load_rows(wk.k, wk.rk, last, kbuf(u));
+        if constexpr (C::NV == 3) {
+          load_rows(wk.v, wk.rv, last, vbuf(u + 2));
+        } else {
+          v_next = wk.v;
+          v_pitch = wk.rv;
+          v_last = last;
+        }
+        move();
+      }
+    }
+    if (active) {
+      if (mask(tile_at(v), sc)) row_max(sc);
       bool grow = false;
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
-        float x = vmax(vmax(sc[0][qb][0], sc[0][qb][1]), vmax(sc[0][qb][2], sc[0][qb][3]));
-#pragma unroll
-        for (int kb = 1; kb < 4; ++kb)
-          x = vmax(vmax(x, vmax(sc[kb][qb][0], sc[kb][qb][1])), vmax(sc[kb][qb][2], sc[kb][qb][3]));
-        mx[qb] = lane_max_xor16_32(x) * c;
+        mx[qb] *= c;
         grow = grow || mx[qb] > m[qb] + kSlack;
       }
       if (__builtin_amdgcn_ballot_w64(grow)) {
@@ -344,139 +512,572 @@ __global__ __launch_bounds__(kNW * 64, FwdCfg<D>::WPS) void window_fwd_kernel(co
           for (int db = 0; db < C::NDB; ++db) o[db][qb] *= alpha;
         }
       }
-      u32x4 pf[2][QB];
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        const float ref = m[qb] == -INFINITY ? 0.f : m[qb];  // (no key yet: every score is -inf)
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-          for (int r = 0; r < 4; r += 2)
-            pf[kb >> 1][qb][(kb & 1) * 2 + r / 2] = pack2<T>(fast_exp2(fmaf(sc[kb][qb][r], c, -ref)),
-                                                             fast_exp2(fmaf(sc[kb][qb][r + 1], c, -ref)));
-      }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) lsum[qb] = Mfma<T>::run(ones, __builtin_bit_cast(v8, pf[ks][qb]), lsum[qb]);
-      if (careful && edge) {
-        // key j = 16 kb + 4 x + r of the tile: its weight is in lane l16 + 16 x
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-          for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int j = kb * 16 + 4 * x + r;
-#pragma unroll
-              for (int qb = 0; qb < QB; ++qb) {
-                const uint32_t pw = (uint32_t)__shfl((int)pf[kb >> 1][qb][(kb & 1) * 2 + r / 2], l16 + 16 * x);
-                const float wgt = (float)__builtin_bit_cast(T, (uint16_t)(r & 1 ? pw >> 16 : pw));
-                if (wgt != 0.f) {
-#pragma unroll
-                  for (int db = 0; db < C::NDB; ++db) {
-                    const int chunk = 2 * db + (gq >> 1);
-                    const T* val = (const T*)(vt + j * (D * 2) + 16 * (chunk ^ kv_swz<D>(j)) + 8 * (gq & 1));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[db][qb][e] = fmaf(wgt, (float)val[e], o[db][qb][e]);
-                  }
-                }
-              }
-            }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int db = 0; db < C::NDB; ++db) {
-            const v8 x = tr.col(vt, ks, db);
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) o[db][qb] = Mfma<T>::run(x, __builtin_bit_cast(v8, pf[ks][qb]), o[db][qb]);
-          }
+      slots(sc, sn, kbuf(u + 1), vbuf(u));
+    }
+    // the loads of the next step's tiles have landed: all but V(v + 2)'s, the last ones issued
+    constexpr int VPW = kBK / (WTile<T, D>::RPI * kNW);
+    if (C::NV == 3 && v + 2 < n) __builtin_amdgcn_s_waitcnt((VPW & 15) | (7 << 4) | (0 << 8) | ((VPW >> 4) << 14));
+    else __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  };
+
+  // fragment kc of the lane's row of block qb
+  auto q_frag = [&](int qb, int kc) {
+    const int row = (wave * QB + qb) * 16 + l16;
+    const int64_t off = row_at(p.q_layout, s.b, s.h, s.q0, row0 + row, p.q_sb, p.q_sh, p.q_sn);
+    return __builtin_bit_cast(v8, __builtin_bit_cast(u32x4, ld_frag<T>(p.q, off + kc * 32 + gq * 8, row < rows)) ^ qsign);
+  };
+  // tile v, with the wait for it
+  auto bring = [&](int v, bool is_v, char* to) {
+    const int t = tile_at(v);
+    if constexpr (FP4) {
+      if (is_code(t)) {
+        fetch_codes(t, is_v);
+        __builtin_amdgcn_s_waitcnt(0);
+        put_codes(is_v, to);
+        if constexpr (C::STAGE) wait_reads();
+        return;
       }
     }
-    if (careful) break;
-    float bad = 0.f;
+    fetch(t, is_v, to);
+  };
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    m[qb] = -INFINITY;
+    lsum[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int db = 0; db < C::NDB; ++db) o[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (n > 0) {
+    // tiles 0 and 1 (V(1) only with a third buffer), and of 4-bit ones the codes of the next
+    if constexpr (FP4) {
+      bring(0, false, kbuf(0));
+      bring(0, true, vbuf(0));
+      if (n > 1) bring(1, false, kbuf(1));
+      if (n > 2 && is_code(tile_at(2))) fetch_codes(tile_at(2), false);
+      if (n > 1 && is_code(tile_at(1))) fetch_codes(tile_at(1), true);
+    } else {
+      seek(0);
+      pitch0 = wk.rk;
+      Tile::template offsets<kBK>(pitch0, wave, lane, off0);
+      load_rows(wk.k, wk.rk, keys_in(wk.t) - 1, kbuf(0));
+      load_rows(wk.v, wk.rv, keys_in(wk.t) - 1, vbuf(0));
+      move();
+      if (n > 1) {
+        v_last = keys_in(wk.t) - 1;
+        load_rows(wk.k, wk.rk, v_last, kbuf(1));
+        if constexpr (C::NV == 3) load_rows(wk.v, wk.rv, v_last, vbuf(1));
+        v_next = wk.v;
+        v_pitch = wk.rv;
+        move();
+      }
+    }
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-      for (int db = 0; db < C::NDB; ++db)
+      for (int kc = 0; kc < C::KC; ++kc) qf[qb][kc] = q_frag(qb, kc);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (active) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) bad = fmaf(o[db][qb][r], 0.f, bad);
-    if (!__syncthreads_or(bad != bad)) break;  // (and every wave is done with the tiles)
+      for (int kc = 0; kc < C::KC; ++kc)
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          const v8 x = tr.row(kbuf(0), kb, kc);
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb)
+            sa[kb][qb] = Mfma<T>::run(x, qf[qb][kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sa[kb][qb]);
+        }
+      row_max(sa);
+    }
+    __syncthreads();  // every wave is done with K(0): its buffer may be refilled
+  }
+  for (int v = 0; v < n;) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      if (v >= n) break;
+      if (u & 1) step(v, u, sb, sa);
+      else step(v, u, sa, sb);
+      ++v;
+    }
   }
 
-  if (!active) return;
-  if (parts > 1) {  // this part's record: O, then m and l of each row
-    const int64_t unit = ((int64_t)(a.tiles - 1 - tile) * a.groups + g) * a.parts + part;
-    float* const rec = a.records + unit * a.rec_rows * (D + 4);
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      const int row = (wave * QB + qb) * 16 + l16;
-      if (row >= rows) continue;
-#pragma unroll
-      for (int db = 0; db < C::NDB; ++db) *(f32x4*)(rec + (int64_t)row * D + db * 16 + gq * 4) = o[db][qb];
-      if (gq == 0) {
-        rec[(int64_t)a.rec_rows * D + 2 * row] = m[qb];
-        rec[(int64_t)a.rec_rows * D + 2 * row + 1] = lsum[qb][0];
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
+  // a row's result: a part's record (O, m, l), or the output
+  float* const rec = a.records + (((int64_t)(a.tiles - 1 - tile) * a.groups + g) * a.parts + part) * a.rec_rows * (D + 4);
+  auto put = [&](int qb, const f32x4 (&x)[C::NDB], float mrow, float l) {
     const int row = (wave * QB + qb) * 16 + l16;
-    if (row >= rows) continue;
-    const float l = lsum[qb][0], inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    if (row >= rows) return;
+    if (parts > 1) {
+#pragma unroll
+      for (int db = 0; db < C::NDB; ++db) *(f32x4*)(rec + (int64_t)row * D + db * 16 + gq * 4) = x[db];
+      if (gq == 0) {
+        rec[(int64_t)a.rec_rows * D + 2 * row] = mrow;
+        rec[(int64_t)a.rec_rows * D + 2 * row + 1] = l;
+      }
+      return;
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     if (p.lse && gq == 0)
-      p.lse[(int64_t)s.h * p.total_q + s.q0 + row0 + row] = l > 0.f ? m[qb] + __log2f(l) : l != l ? l : INFINITY;
+      p.lse[(int64_t)s.h * p.total_q + s.q0 + row0 + row] = l > 0.f ? mrow + __log2f(l) : l != l ? l : INFINITY;
     const int64_t off = row_at(p.o_layout, s.b, s.h, s.q0, row0 + row, p.o_sb, p.o_sh, p.o_sn);
 #pragma unroll
     for (int db = 0; db < C::NDB; ++db) {
-      const f32x4 x = o[db][qb] * inv;
-      *(u32x2*)((char*)p.o + (off + db * 16 + gq * 4) * 2) = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+      const f32x4 y = x[db] * inv;
+      const u32x2 hi = u32x2{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+      *(u32x2*)((char*)p.o + (off + db * 16 + gq * 4) * 2) = hi;
+      if (a.o_low) {
+        f32x4 z;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t w = hi[r / 2];
+          z[r] = y[r] - (float)__builtin_bit_cast(T, (uint16_t)(r & 1 ? w >> 16 : w));
+        }
+        *(u32x2*)((char*)a.o_low + (off + db * 16 + gq * 4) * 2) = u32x2{pack2<T>(z[0], z[1]), pack2<T>(z[2], z[3])};
+      }
     }
+  };
+  float bad = 0.f;
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    f32x4 x[C::NDB];
+#pragma unroll
+    for (int db = 0; db < C::NDB; ++db) {
+      x[db] = o[db][qb];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bad = fmaf(x[db][r], 0.f, bad);
+    }
+    put(qb, x, m[qb], lsum[qb][0]);
+  }
+  // Values that are not finite in keys that a row does not see have reached it as 0 inf.  If there may
+  // be any, the rows are computed again, a tile and a block of rows at a time, key by key.
+  // (The tiles' LDS is free: every wave has passed the last step's barrier.)
+  if (lane == 0) ((int*)smem)[wave] = __builtin_amdgcn_ballot_w64(bad != bad) != 0;
+  __syncthreads();
+  const int any = ((const int*)smem)[0] | ((const int*)smem)[1] | ((const int*)smem)[2] | ((const int*)smem)[3];
+  __syncthreads();
+  if (!any) return;
+  T* const pw = (T*)(kbuf(1) + wave * 2048);  // the wave's weights [16][64], behind K(0): kbuf(1), V(0) follows 8 KB on
+  char* const vt = smem + C::LDS - (C::STAGE ? 2 * kNW * 1024 : 0) - C::TILEB;  // the last V buffer
+  for (int qb = 0; qb < QB; ++qb) {
+    float mr = -INFINITY, l = 0.f;
+    f32x4 x[C::NDB];
+#pragma unroll
+    for (int db = 0; db < C::NDB; ++db) x[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int v = 0; v < n; ++v) {
+      bring(v, false, kbuf(0));
+      bring(v, true, vt);
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      const int t = tile_at(v), nk = keys_in(t), kp = t < wt.nt0 ? t * kBK : s.ctx + (t - wt.nt0) * kBK;
+      f32x4 sc[4];
+#pragma unroll
+      for (int kc = 0; kc < C::KC; ++kc) {
+        const v8 f = q_frag(qb, kc);
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+          sc[kb] = Mfma<T>::run(tr.row(kbuf(0), kb, kc), f, kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[kb]);
+      }
+      const int pos = w0 + qb * 16 + l16, k0 = kp + 4 * gq;
+      const int top = min(pos + a.right - k0, nk - 1 - 4 * gq), low = pos - a.left - k0, snk = a.sinks - k0;
+      float y = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = kb * 16 + r;
+          if (!(j <= top && (j >= low || j < snk))) sc[kb][r] = -INFINITY;
+          y = vmax(y, sc[kb][r]);
+        }
+      const float mn = vmax(mr, lane_max_xor16_32(y) * c), ref = mn == -INFINITY ? 0.f : mn;
+      const float alpha = fast_exp2((mr == -INFINITY ? ref : mr) - ref);
+      mr = mn;
+      l *= alpha;
+#pragma unroll
+      for (int db = 0; db < C::NDB; ++db) x[db] *= alpha;
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) pw[l16 * 64 + kb * 16 + 4 * gq + r] = (T)fast_exp2(fmaf(sc[kb][r], c, -ref));
+      asm volatile("" ::: "memory");
+#pragma clang loop unroll(disable)
+      for (int j = 0; j < kBK; ++j) {
+        const float w = (float)pw[l16 * 64 + j];
+        l += w;
+        if (w != 0.f) {
+#pragma unroll
+          for (int db = 0; db < C::NDB; ++db) {
+            const T* val = (const T*)(vt + j * (D * 2) + 16 * ((2 * db + (gq >> 1)) ^ kv_swz<D>(j)) + 8 * (gq & 1));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[db][e] = fmaf(w, (float)val[e], x[db][e]);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    put(qb, x, mr, l);
   }
 }
 
 // ---------------------------------------------------------------------------
-// The parts' records joined: 8 columns of a row a thread
+// Forward of few rows (at most 16 a sequence) over a 4-bit context: a wave has all rows and walks
+// tiles of its own, without a barrier.  Lane l16 + 16 g loads quarter g of the rows 16 kb + l16 of a
+// tile, D / 8 bytes, which are whole lines for the wave, and a dword of it is a fragment of
+// S^T = K Q^T: the contraction takes the elements in the order (quarter, fragment), and q comes in
+// that order too.  V is converted the same way into a wave's own 32 rows of LDS and read back
+// transposed.  A tile's registers are loaded again as soon as they have been converted.  The four
+// waves' sums meet in LDS at the end.
 // ---------------------------------------------------------------------------
+constexpr int kFewRows = 16;
+
+template <int D>
+struct FewCfg {
+  static constexpr int KC = D / 32, NDB = D / 16;
+  static constexpr int CS = D == 256 ? 2 : 1;             // scales of a quarter row
+  static constexpr int WAVEB = 32 * D * 2;                // V rows; at the end 16 rows of fp32
+  static constexpr int LDS = kNW * (WAVEB + 2 * kFewRows * 4);  // ... and m and l of each
+  static constexpr int WPS = D <= 128 ? 3 : 2;
+};
+
 template <typename T, int D>
+__global__ __launch_bounds__(kNW * 64, FewCfg<D>::WPS) void window_fp4_few_kernel(const fmlm_attn_params p, const WinArgs a) {
+  typedef FewCfg<D> C;
+  typedef typename Mfma<T>::v8 v8;
+  extern __shared__ __align__(16) char smem[];
+  int g, part, tile;
+  win_unit(a, a.parts, g, part, tile);
+  if (g >= p.B * p.H) return;
+  const WinSeq s = win_seq(p, a, g / p.H, g % p.H);
+  const int rows = min(kFewRows, s.len);
+  if (rows <= 0) return;
+  const WinTiles wt = win_tiles(a, s, s.first, s.first + rows - 1);
+  const int parts = win_parts(wt.n, a.parts);
+  if (part >= parts) return;
+  const int vb = (int)((int64_t)wt.n * part / parts), ve = (int)((int64_t)wt.n * (part + 1) / parts);
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, gq = lane >> 4;
+  const WTile<T, D> tr(l16, gq);
+  char* const vt = smem + wave * C::WAVEB;
+  const uint32_t qsign = p.scale < 0.f ? 0x80008000u : 0u;
+  const float c = fmaxf(fabsf(p.scale) * kLog2e, 1e-30f);
+  v8 qf[C::KC];
+  {
+    const int64_t off = row_at(p.q_layout, s.b, s.h, s.q0, l16, p.q_sb, p.q_sh, p.q_sn) + gq * (D / 4);
+#pragma unroll
+    for (int kc = 0; kc < C::KC; ++kc)
+      qf[kc] = __builtin_bit_cast(v8, __builtin_bit_cast(u32x4, ld_frag<T>(p.q, off + kc * 8, l16 < rows)) ^ qsign);
+  }
+  const int cb = ctx_batch_of(p, s.b);
+  const int32_t* const pages = p.ctx_block_table + (int64_t)cb * p.ctx_pages_per_batch;
+  auto page_of = [&](int v) {  // of context tile v of the walk (any, past its end)
+    const int t = min(wt.tile(v), max(wt.nt0 - 1, 0));
+    return wt.nt0 > 0 ? min(max(ldc(pages, t), 0), max(p.ctx_rows - 1, 0)) : 0;
+  };
+  uint32_t kw[4][C::KC], vw[4][C::KC], ks[4][C::CS], vs[4][C::CS];
+  auto load = [&](const void* codes, const uint8_t* scales, int page, int last, uint32_t (&w)[4][C::KC],
+                  uint32_t (&sc)[4][C::CS]) {
+    const int64_t e0 = (int64_t)s.h * p.c_sh + (int64_t)page * p.ctx_page_stride;
+    const char* const src = uniform_ptr((const char*)codes + e0 / 2);
+    const char* const ssc = uniform_ptr((const char*)scales + e0 / kFp4Block);
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      const uint32_t row = (uint32_t)min(kb * 16 + l16, last), at = row * (D / 2) + gq * (D / 8);
+      if constexpr (C::KC == 1) w[kb][0] = *(const uint32_t*)(src + at);
+      else if constexpr (C::KC == 2) {
+        const u32x2 x = *(const u32x2*)(src + at);
+        w[kb][0] = x[0];
+        w[kb][1] = x[1];
+      } else {
+#pragma unroll
+        for (int i = 0; i < C::KC; i += 4) {
+          const u32x4 x = *(const u32x4*)(src + at + 4 * i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[kb][i + j] = x[j];
+        }
+      }
+      const uint32_t sat = row * (D / kFp4Block) + gq * (D / 4) / kFp4Block;
+#pragma unroll
+      for (int i = 0; i < C::CS; ++i) sc[kb][i] = (uint8_t)ssc[sat + i];
+    }
+  };
+  auto keys_in = [&](int t) { return min(kBK, t < wt.nt0 ? s.ctx - t * kBK : s.total - s.ctx - (t - wt.nt0) * kBK); };
+
+  f32x4 o[C::NDB], lsum = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY;
+#pragma unroll
+  for (int db = 0; db < C::NDB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  v8 ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = (T)1.0f;
+
+  // scores of a tile of nk keys from position kp on: masked, the running maximum and P
+  u32x4 pf[2];
+  bool edge;
+  auto softmax = [&](f32x4 (&sc)[4], int kp, int nk) {
+    edge = nk < kBK || kp + kBK - 1 > s.first + a.right || (kp < s.first + rows - 1 - a.left && kp + kBK > a.sinks);
+    if (edge) {
+      const int pos = s.first + l16, k0 = kp + 4 * gq;
+      const int top = min(pos + a.right - k0, nk - 1 - 4 * gq), low = pos - a.left - k0, snk = a.sinks - k0;
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = kb * 16 + r;
+          if (!(j <= top && (j >= low || j < snk))) sc[kb][r] = -INFINITY;
+        }
+    }
+    float mx = vmax(vmax(sc[0][0], sc[0][1]), vmax(sc[0][2], sc[0][3]));
+#pragma unroll
+    for (int kb = 1; kb < 4; ++kb) mx = vmax(vmax(mx, vmax(sc[kb][0], sc[kb][1])), vmax(sc[kb][2], sc[kb][3]));
+    mx = lane_max_xor16_32(mx) * c;
+    if (__builtin_amdgcn_ballot_w64(mx > m + kSlack)) {
+      const float mn = mx > m + kSlack ? mx : m;
+      const float alpha = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+      m = mn;
+      lsum *= alpha;
+#pragma unroll
+      for (int db = 0; db < C::NDB; ++db) o[db] *= alpha;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2)
+        pf[kb >> 1][(kb & 1) * 2 + r / 2] =
+            pack2<T>(fast_exp2(fmaf(sc[kb][r], c, -ref)), fast_exp2(fmaf(sc[kb][r + 1], c, -ref)));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) lsum = Mfma<T>::run(ones, __builtin_bit_cast(v8, pf[h]), lsum);
+  };
+  // O += P V of the 32 keys in LDS
+  auto values = [&](int h) {
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int db = 0; db < C::NDB; ++db) o[db] = Mfma<T>::run(tr.col(vt, 0, db), __builtin_bit_cast(v8, pf[h]), o[db]);
+    asm volatile("" ::: "memory");
+  };
+
+  int page = page_of(vb + wave), next = page_of(vb + wave + kNW);
+  if (vb + wave < ve && wt.tile(vb + wave) < wt.nt0) {
+    const int last = keys_in(wt.tile(vb + wave)) - 1;
+    load(p.k_ctx, a.k_scales, page, last, kw, ks);
+    load(p.v_ctx, a.v_scales, page, last, vw, vs);
+  }
+  for (int v = vb + wave; v < ve; v += kNW) {
+    const int t = wt.tile(v), nk = keys_in(t);
+    if (t >= wt.nt0) break;  // the new tokens, at most 16: one tile, the last
+    f32x4 sc[4];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kc = 0; kc < C::KC; ++kc)
+        sc[kb] = Mfma<T>::run(__builtin_bit_cast(v8, fp4_oct<T>(kw[kb][kc], fp4_scale(ks[kb][kc / 4 % C::CS]))), qf[kc], sc[kb]);
+    }
+    const bool more = v + kNW < ve && wt.tile(v + kNW) < wt.nt0;
+    const int nlast = more ? keys_in(wt.tile(v + kNW)) - 1 : 0;
+    page = next;
+    if (more) load(p.k_ctx, a.k_scales, page, nlast, kw, ks);
+    next = page_of(v + 2 * kNW);
+    softmax(sc, t * kBK, nk);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int kc = 0; kc < C::KC; ++kc)
+          *(u32x4*)(vt + (i * 16 + l16) * (D * 2) + 16 * ((gq * C::KC + kc) ^ kv_swz<D>(l16))) =
+              fp4_oct<T>(vw[2 * h + i][kc], fp4_scale(vs[2 * h + i][kc / 4 % C::CS]));
+      values(h);
+    }
+    if (more) load(p.v_ctx, a.v_scales, page, nlast, vw, vs);
+  }
+  // the new tokens' own keys, by the wave whose turn it is
+  if (ve > vb && wt.tile(ve - 1) >= wt.nt0 && (ve - 1 - vb) % kNW == wave) {
+    const int nk = keys_in(wt.tile(ve - 1));
+    const int64_t ko = row_at(p.kv_layout, s.b, s.h, s.q0, min(l16, nk - 1), p.k_sb, p.k_sh, p.k_sn) + gq * (D / 4);
+    const int64_t vo = row_at(p.kv_layout, s.b, s.h, s.q0, min(l16, nk - 1), p.v_sb, p.v_sh, p.v_sn) + gq * (D / 4);
+    f32x4 sc[4];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    u32x4 vrow[C::KC];
+#pragma unroll
+    for (int kc = 0; kc < C::KC; ++kc) {
+      sc[0] = Mfma<T>::run(ld_frag<T>(p.k, ko + kc * 8, true), qf[kc], sc[0]);
+      vrow[kc] = *(const u32x4*)((const char*)p.v + (vo + kc * 8) * 2);
+    }
+    softmax(sc, s.ctx, nk);
+    // values that are not finite: a row that does not see them must not meet them as 0 inf, so they are added
+    // key by key then
+    float bad = 0.f;
+#pragma unroll
+    for (int kc = 0; kc < C::KC; ++kc) {
+      const v8 x = __builtin_bit_cast(v8, vrow[kc]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bad = fmaf((float)x[e], 0.f, bad);
+    }
+    const bool careful = __builtin_amdgcn_ballot_w64(bad != bad) != 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int kc = 0; kc < C::KC; ++kc)
+        *(u32x4*)(vt + (i * 16 + l16) * (D * 2) + 16 * ((gq * C::KC + kc) ^ kv_swz<D>(l16))) =
+            i || careful ? u32x4{0u, 0u, 0u, 0u} : vrow[kc];
+    values(0);
+    if (careful) {
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {  // key 4 x + r: its weight is in lane l16 + 16 x
+          const uint32_t pw = (uint32_t)__shfl((int)pf[0][r / 2], l16 + 16 * x);
+          const float wgt = (float)__builtin_bit_cast(T, (uint16_t)(r & 1 ? pw >> 16 : pw));
+          const int j = 4 * x + r;
+          if (j < nk && wgt != 0.f) {
+            const T* const val = (const T*)p.v + row_at(p.kv_layout, s.b, s.h, s.q0, j, p.v_sb, p.v_sh, p.v_sn) + 4 * gq;
+#pragma unroll
+            for (int db = 0; db < C::NDB; ++db)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[db][e] = fmaf(wgt, (float)val[db * 16 + e], o[db][e]);
+          }
+        }
+    }
+  }
+
+  // ---- the four waves' parts: O to LDS (over V), m and l behind
+  float* const stat = (float*)(smem + kNW * C::WAVEB);
+  asm volatile("" ::: "memory");
+  if (l16 < rows) {
+#pragma unroll
+    for (int db = 0; db < C::NDB; ++db) *(f32x4*)(vt + (l16 * D + db * 16 + gq * 4) * 4) = o[db];
+    if (gq == 0) {
+      stat[(wave * kFewRows + l16) * 2] = m;
+      stat[(wave * kFewRows + l16) * 2 + 1] = lsum[0];
+    }
+  }
+  __syncthreads();
+  const int64_t unit = (int64_t)g * a.parts + part;
+  float* const rec = a.records + unit * a.rec_rows * (D + 4);
+  for (int i = tid; i < rows * (D / 8); i += kNW * 64) {
+    const int row = i / (D / 8), d = (i % (D / 8)) * 8;
+    float top = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < kNW; ++k) top = vmax(top, stat[(k * kFewRows + row) * 2]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll
+    for (int k = 0; k < kNW; ++k) {
+      const float w = fast_exp2(stat[(k * kFewRows + row) * 2] - ref);
+      const f32x4* src = (const f32x4*)(smem + k * C::WAVEB + (row * D + d) * 4);
+      l = fmaf(w, stat[(k * kFewRows + row) * 2 + 1], l);
+      x += src[0] * w;
+      y += src[1] * w;
+    }
+    if (parts > 1) {
+      *(f32x4*)(rec + row * D + d) = x;
+      *(f32x4*)(rec + row * D + d + 4) = y;
+      if (d == 0) {
+        rec[(int64_t)a.rec_rows * D + 2 * row] = top;
+        rec[(int64_t)a.rec_rows * D + 2 * row + 1] = l;
+      }
+      continue;
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    x *= inv;
+    y *= inv;
+    const int64_t off = row_at(p.o_layout, s.b, s.h, s.q0, row, p.o_sb, p.o_sh, p.o_sn);
+    *(u32x4*)((char*)p.o + (off + d) * 2) =
+        u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The parts' records joined.  A workgroup takes RR rows of a query tile (blockIdx.y), 8 columns of a
+// row a thread; with RR < 256 / (D / 8) the other threads share a row's parts, and meet in LDS.  A
+// thread has kMergeLoads records in flight (one after the other: 9 us for 32 parts of one row, of
+// 19 in all).
+// ---------------------------------------------------------------------------
+constexpr int kMergeLoads = 4;
+template <typename T, int D, int RR>
 __global__ __launch_bounds__(256) void window_merge_kernel(const fmlm_attn_params p, const WinArgs a, int bq) {
-  constexpr int CPR = D / 8;
+  constexpr int CPR = D / 8, GG = 256 / (CPR * RR);  // columns and part groups
+  __shared__ __align__(16) float sums[GG][RR][D];
+  __shared__ float stat[GG][RR][2];
   int g, part, tile;
   win_unit(a, 1, g, part, tile);
   if (g >= p.B * p.H) return;
   tile = a.tiles - 1 - tile;
   const WinSeq s = win_seq(p, a, g / p.H, g % p.H);
   const int row0 = tile * bq, rows = min(bq, s.len - row0);
-  if (rows <= 0) return;
+  const int tid = threadIdx.x, c8 = tid % CPR, rr = (tid / CPR) % RR, gg = tid / (CPR * RR);
+  const int row = blockIdx.y * RR + rr;
+  if ((int)blockIdx.y * RR >= rows) return;
   const int parts = win_parts(win_tiles(a, s, s.first + row0, s.first + row0 + rows - 1).n, a.parts);
   if (parts <= 1) return;
   const int64_t unit = ((int64_t)(a.tiles - 1 - tile) * a.groups + g) * a.parts, pitch = (int64_t)a.rec_rows * (D + 4);
-  const float* const rec = a.records + unit * pitch;
-  for (int i = threadIdx.x; i < rows * CPR; i += 256) {
-    const int row = i / CPR, d = (i % CPR) * 8;
-    const float* const st = rec + (int64_t)a.rec_rows * D + 2 * row;
-    float top = -INFINITY;
-    for (int k = 0; k < parts; ++k) top = vmax(top, st[k * pitch]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float l = 0.f;
-    f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
-#pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
-      const float w = fast_exp2(st[k * pitch] - ref);
-      const f32x4* src = (const f32x4*)(rec + k * pitch + (int64_t)row * D + d);
-      l = fmaf(w, st[k * pitch + 1], l);
-      x += src[0] * w;
-      y += src[1] * w;
+  const float* const rec = a.records + unit * pitch + (int64_t)row * D + c8 * 8;
+  const float* const st = a.records + unit * pitch + (int64_t)a.rec_rows * D + 2 * row;
+  float top = -INFINITY, l = 0.f;
+  f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
+  if (row < rows)
+    for (int k0 = gg; k0 < parts; k0 += GG * kMergeLoads) {
+      float mk[kMergeLoads], lk[kMergeLoads];
+      f32x4 xk[kMergeLoads], yk[kMergeLoads];
+#pragma unroll
+      for (int i = 0; i < kMergeLoads; ++i) {
+        const int64_t at = min(k0 + i * GG, parts - 1) * pitch;
+        mk[i] = st[at];
+        lk[i] = st[at + 1];
+        xk[i] = *(const f32x4*)(rec + at);
+        yk[i] = *(const f32x4*)(rec + at + 4);
+      }
+      float mt = top;
+#pragma unroll
+      for (int i = 0; i < kMergeLoads; ++i) {
+        if (k0 + i * GG >= parts) mk[i] = -INFINITY;
+        mt = vmax(mt, mk[i]);
+      }
+      const float ref = mt == -INFINITY ? 0.f : mt, w0 = fast_exp2((top == -INFINITY ? ref : top) - ref);
+      top = mt;
+      l *= w0;
+      x *= w0;
+      y *= w0;
+#pragma unroll
+      for (int i = 0; i < kMergeLoads; ++i) {
+        if (k0 + i * GG >= parts) continue;
+        const float w = fast_exp2(mk[i] - ref);
+        l = fmaf(w, lk[i], l);
+        x += xk[i] * w;
+        y += yk[i] * w;
+      }
     }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    x *= inv;
-    y *= inv;
-    const int64_t off = row_at(p.o_layout, s.b, s.h, s.q0, row0 + row, p.o_sb, p.o_sh, p.o_sn);
-    *(u32x4*)((char*)p.o + (off + d) * 2) =
-        u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+  if constexpr (GG > 1) {
+    *(f32x4*)&sums[gg][rr][c8 * 8] = x;
+    *(f32x4*)&sums[gg][rr][c8 * 8 + 4] = y;
+    if (c8 == 0) {
+      stat[gg][rr][0] = top;
+      stat[gg][rr][1] = l;
+    }
+    __syncthreads();
+    if (gg > 0) return;
+    float all = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < GG; ++i) all = vmax(all, stat[i][rr][0]);
+    const float ref = all == -INFINITY ? 0.f : all;
+    l = 0.f;
+    x = y = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < GG; ++i) {
+      const float w = fast_exp2(stat[i][rr][0] - ref);
+      l = fmaf(w, stat[i][rr][1], l);
+      x += *(const f32x4*)&sums[i][rr][c8 * 8] * w;
+      y += *(const f32x4*)&sums[i][rr][c8 * 8 + 4] * w;
+    }
   }
+  if (row >= rows) return;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  x *= inv;
+  y *= inv;
+  const int64_t off = row_at(p.o_layout, s.b, s.h, s.q0, row0 + row, p.o_sb, p.o_sh, p.o_sn);
+  *(u32x4*)((char*)p.o + (off + c8 * 8) * 2) =
+      u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
 }
 
 // ---------------------------------------------------------------------------
@@ -532,7 +1133,8 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(con
   const WinTiles wt = win_tiles(a, s, row0, row0 + rows - 1);
   const WTile<T, D> tr(l16, gq);
   const bool active = wave * QB * 16 < rows;
-  const float c = p.scale * kLog2e;
+  // (a scale of 0 would lose the masked scores' infinity; this one leaves every other 2^(c s) at 1)
+  const float c = p.scale != 0.f ? p.scale * kLog2e : 1e-30f;
 
   v8 qf[QB][C::KC], df[QB][C::KC];
   float delta[QB], lse[QB];
@@ -549,9 +1151,9 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(con
       const int col = kc * 32 + gq * 8;
       qf[qb][kc] = ld_frag<T>(p.q, qo + col, ok);
       df[qb][kc] = ld_frag<T>(gr.dout, po + col, ok);
-      const v8 ov = ld_frag<T>(p.o, oo + col, ok);
+      const v8 ov = ld_frag<T>(p.o, oo + col, ok), lv = ld_frag<T>(a.o_low, oo + col, ok && a.o_low);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf((float)df[qb][kc][e], (float)ov[e], sum);
+      for (int e = 0; e < 8; ++e) sum = fmaf((float)df[qb][kc][e], (float)ov[e] + (float)lv[e], sum);
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -581,29 +1183,46 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(con
     if (v + 1 < wt.n) issue(v + 1);
     if (!active) continue;
     const char *kt = kbuf(buf), *vt = vbuf(buf);
+    // ---- fenced slots, each the MFMAs of one LDS fragment: NSS of S^T (step kc, key block kb), NSS of
+    // dP^T (block by block), 2 NDB of dq^T; the fragment of slot s + LEAD is read at slot s.  Block
+    // kb's P and dS are made beside block kb + 1's dP, the last one's beside the first dq slots.
+    constexpr int NSS = 4 * C::KC, NR = 2 * NSS, NS = NR + 2 * C::NDB, LEAD = 3;
     f32x4 sc[4][QB], dp[4][QB];
-#pragma unroll
-    for (int kc = 0; kc < C::KC; ++kc)
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb) {
-        const v8 x = tr.row(kt, kb, kc), y = tr.row(vt, kb, kc);
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-          sc[kb][qb] = Mfma<T>::run(x, qf[qb][kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[kb][qb]);
-          dp[kb][qb] = Mfma<T>::run(y, df[qb][kc],
-                                    kc == 0 ? f32x4{-delta[qb], -delta[qb], -delta[qb], -delta[qb]} : dp[kb][qb]);
-        }
-      }
-    const int kp = t * kBK, w0 = row0 + wave * QB * 16, w1 = min(w0 + QB * 16, row0 + rows) - 1;
-    const bool edge = nk < kBK || kp + kBK - 1 > w0 + a.right || (kp < w1 - a.left && kp + kBK > a.sinks);
     u32x4 ds[2][QB];
+    v8 fr[LEAD + 1];
+    auto read = [&](int r) {
+      if (r < NSS) fr[r % (LEAD + 1)] = tr.row(kt, r % 4, r / 4);
+      else if (r < NR) fr[r % (LEAD + 1)] = tr.row(vt, (r - NSS) / C::KC, (r - NSS) % C::KC);
+      else fr[r % (LEAD + 1)] = tr.col(kt, (r - NR) / C::NDB, (r - NR) % C::NDB);
+    };
+    // elements r, r + 1 of block kb, rows qb (e = 2 qb + r / 2)
+    auto soft = [&](int kb, int e) {
+      const int qb = e >> 1, r = (e & 1) * 2;
+      if (r == 0) pin(dp[kb][qb]);
+      uint32_t w = pack2<T>(fast_exp2(fmaf(sc[kb][qb][r], c, -lse[qb])) * dp[kb][qb][r],
+                            fast_exp2(fmaf(sc[kb][qb][r + 1], c, -lse[qb])) * dp[kb][qb][r + 1]);
+      pin(w);
+      ds[kb >> 1][qb][(kb & 1) * 2 + (r >> 1)] = w;
+    };
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
+    for (int r = 0; r < LEAD; ++r) read(r);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
+    for (int sl = 0; sl < NSS; ++sl) {
+      read(sl + LEAD);
+      const v8 x = fr[sl % (LEAD + 1)];
+      const int kb = sl % 4, kc = sl / 4;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) dp[kb][qb][r] *= fast_exp2(fmaf(sc[kb][qb][r], c, -lse[qb]));
-      if (edge) {
+      for (int qb = 0; qb < QB; ++qb)
+        sc[kb][qb] = Mfma<T>::run(x, qf[qb][kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[kb][qb]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const int kp = t * kBK, w0 = row0 + wave * QB * 16, w1 = min(w0 + QB * 16, row0 + rows) - 1;
+    if (nk < kBK || kp + kBK - 1 > w0 + a.right || (kp < w1 - a.left && kp + kBK > a.sinks)) {
+      asm volatile("");  // (a real branch.)  What a row does not see: P = 0
+      const float none = c < 0.f ? INFINITY : -INFINITY;
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
         const int pos = w0 + qb * 16 + l16, k0 = kp + 4 * gq;
         const int top = min(pos + a.right - k0, nk - 1 - 4 * gq), low = pos - a.left - k0, snk = a.sinks - k0;
 #pragma unroll
@@ -611,23 +1230,39 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(con
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int j = kb * 16 + r;
-            if (!(j <= top && (j >= low || j < snk))) dp[kb][qb][r] = 0.f;
+            if (!(j <= top && (j >= low || j < snk))) sc[kb][qb][r] = none;
           }
       }
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int r = 0; r < 4; r += 2)
-          ds[kb >> 1][qb][(kb & 1) * 2 + r / 2] = pack2<T>(dp[kb][qb][r], dp[kb][qb][r + 1]);
     }
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
+    for (int sl = NSS; sl < NR; ++sl) {
+      read(sl + LEAD);
+      const v8 x = fr[sl % (LEAD + 1)];
+      const int j = sl - NSS, kb = j / C::KC, kc = j % C::KC;
 #pragma unroll
-      for (int db = 0; db < C::NDB; ++db) {
-        const v8 x = tr.col(kt, ks, db);
+      for (int qb = 0; qb < QB; ++qb)
+        dp[kb][qb] = Mfma<T>::run(x, df[qb][kc], kc == 0 ? f32x4{-delta[qb], -delta[qb], -delta[qb], -delta[qb]} : dp[kb][qb]);
+      if (kb > 0) {
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) dq[db][qb] = Mfma<T>::run(x, __builtin_bit_cast(v8, ds[ks][qb]), dq[db][qb]);
+        for (int e = kc * 2 * QB / C::KC; e < (kc + 1) * 2 * QB / C::KC; ++e) soft(kb - 1, e);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(2);
+#pragma unroll
+    for (int sl = NR; sl < NS; ++sl) {
+      if (sl + LEAD < NS) read(sl + LEAD);
+      const v8 x = fr[sl % (LEAD + 1)];
+      const int j = sl - NR, ks = j / C::NDB, db = j % C::NDB;
+      if (ks == 0) {
+#pragma unroll
+        for (int e = j * 2 * QB / C::NDB; e < (j + 1) * 2 * QB / C::NDB; ++e) soft(3, e);
+      }
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) dq[db][qb] = Mfma<T>::run(x, __builtin_bit_cast(v8, ds[ks][qb]), dq[db][qb]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
   }
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
@@ -672,7 +1307,7 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dkv_kernel(co
   }
   if (j0 >= s.len) return;
   const WTile<T, D> tr(l16, gq);
-  const float c = p.scale * kLog2e;
+  const float c = p.scale != 0.f ? p.scale * kLog2e : 1e-30f, none = c < 0.f ? INFINITY : -INFINITY;
   v8 kf[C::KC], vf[C::KC];
   {
     const int64_t ko = row_at(p.kv_layout, s.b, s.h, s.q0, key, p.k_sb, p.k_sh, p.k_sn);
@@ -720,41 +1355,77 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dkv_kernel(co
     const bool edge = k1 >= s.len || k1 > p0 + a.right || (k0 < p0 + QS - 1 - a.left && k1 >= a.sinks);
     // rows pos with lo <= pos <= hi see the lane's key
     const int lo = key - a.right - p0, hi = !kok ? -1 : key < a.sinks ? QS : key + a.left - p0;
+    // ---- fenced slots as in the dq kernel: per block of 16 rows its S and dP (fragments of q and do in turn),
+    // the block before's P and dS beside them; then per 32 rows dV^T and dK^T
+    constexpr int RBS = 2 * C::KC, NR = NRB * RBS, NCS = 2 * C::NDB, NS = NR + NRB / 2 * NCS, LEAD = 3;
+    f32x4 sc[NRB], dp[NRB], L4[NRB], D4[NRB];
     u32x4 pw[NRB / 2], dw[NRB / 2];
-#pragma unroll
-    for (int rb = 0; rb < NRB; ++rb) {
-      f32x4 sc, dp;
-#pragma unroll
-      for (int kc = 0; kc < C::KC; ++kc) {
-        sc = Mfma<T>::run(tr.row(qt, rb, kc), kf[kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc);
-        dp = Mfma<T>::run(tr.row(ot, rb, kc), vf[kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : dp);
-      }
-      const f32x4 L = *(const f32x4*)(ls + rb * 16 + gq * 4), Dl = *(const f32x4*)(ls + QS + rb * 16 + gq * 4);
-      f32x4 pv, dsv;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        pv[r] = fast_exp2(fmaf(sc[r], c, -L[r]));
-        dsv[r] = pv[r] * (dp[r] - Dl[r]);
-      }
+    v8 fr[LEAD + 1];
+    auto read = [&](int r) {
+      if (r < NR) fr[r % (LEAD + 1)] = tr.row((r & 1) ? ot : qt, r / RBS, (r % RBS) >> 1);
+      else fr[r % (LEAD + 1)] = tr.col(((r - NR) & 1) ? qt : ot, (r - NR) / NCS, ((r - NR) % NCS) >> 1);
+    };
+    // a block whose scores are done: its statistics, and what does not see the key
+    auto ready = [&](int rb) {
+      L4[rb] = *(const f32x4*)(ls + rb * 16 + gq * 4);
+      D4[rb] = *(const f32x4*)(ls + QS + rb * 16 + gq * 4);
       if (edge) {
+        asm volatile("");  // (a real branch)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int pos = rb * 16 + gq * 4 + r;
-          if (!(pos >= lo && pos <= hi)) pv[r] = dsv[r] = 0.f;
+          if (!(pos >= lo && pos <= hi)) sc[rb][r] = none;
         }
       }
-      pw[rb >> 1][(rb & 1) * 2] = pack2<T>(pv[0], pv[1]);
-      pw[rb >> 1][(rb & 1) * 2 + 1] = pack2<T>(pv[2], pv[3]);
-      dw[rb >> 1][(rb & 1) * 2] = pack2<T>(dsv[0], dsv[1]);
-      dw[rb >> 1][(rb & 1) * 2 + 1] = pack2<T>(dsv[2], dsv[3]);
+    };
+    // elements 2 e, 2 e + 1 of block rb
+    auto soft = [&](int rb, int e) {
+      if (e == 0) {
+        pin(sc[rb]);
+        pin(dp[rb]);
+      }
+      float pv[2], dv2[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        pv[i] = fast_exp2(fmaf(sc[rb][2 * e + i], c, -L4[rb][2 * e + i]));
+        dv2[i] = pv[i] * (dp[rb][2 * e + i] - D4[rb][2 * e + i]);
+      }
+      uint32_t x = pack2<T>(pv[0], pv[1]), y = pack2<T>(dv2[0], dv2[1]);
+      pin(x);
+      pin(y);
+      pw[rb >> 1][(rb & 1) * 2 + e] = x;
+      dw[rb >> 1][(rb & 1) * 2 + e] = y;
+    };
+#pragma unroll
+    for (int r = 0; r < LEAD; ++r) read(r);
+#pragma unroll
+    for (int sl = 0; sl < NR; ++sl) {
+      read(sl + LEAD);
+      const v8 x = fr[sl % (LEAD + 1)];
+      const int rb = sl / RBS, kc = (sl % RBS) >> 1, loc = sl % RBS;
+      if (rb > 0 && loc == 0) ready(rb - 1);
+      if ((sl & 1) == 0) sc[rb] = Mfma<T>::run(x, kf[kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[rb]);
+      else dp[rb] = Mfma<T>::run(x, vf[kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : dp[rb]);
+      if (rb > 0) {
+#pragma unroll
+        for (int e = loc * 2 / RBS; e < (loc + 1) * 2 / RBS; ++e) soft(rb - 1, e);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int ks = 0; ks < NRB / 2; ++ks)
+    for (int sl = NR; sl < NS; ++sl) {
+      if (sl + LEAD < NS) read(sl + LEAD);
+      const v8 x = fr[sl % (LEAD + 1)];
+      const int j = sl - NR, grp = j / NCS, db = (j % NCS) >> 1;
+      if (j == 0) ready(NRB - 1);
+      if (NRB == 2 ? j == 0 : grp == 0) {  // the last block's (with one group, before its products)
 #pragma unroll
-      for (int db = 0; db < C::NDB; ++db) {
-        dv[db] = Mfma<T>::run(tr.col(ot, ks, db), __builtin_bit_cast(v8, pw[ks]), dv[db]);
-        dk[db] = Mfma<T>::run(tr.col(qt, ks, db), __builtin_bit_cast(v8, dw[ks]), dk[db]);
+        for (int e = NRB == 2 ? 0 : j * 2 / NCS; e < (NRB == 2 ? 2 : (j + 1) * 2 / NCS); ++e) soft(NRB - 1, e);
       }
+      if ((j & 1) == 0) dv[db] = Mfma<T>::run(x, __builtin_bit_cast(v8, pw[grp]), dv[db]);
+      else dk[db] = Mfma<T>::run(x, __builtin_bit_cast(v8, dw[grp]), dk[db]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
   if (!kok) return;
 #pragma unroll
@@ -775,23 +1446,67 @@ int allow_lds(const void* fn, int bytes) {
   return e == hipSuccess ? 0 : (int)e;
 }
 
+int longest(const fmlm_attn_params& p) { return p.N > 0 && p.N < p.total_q ? p.N : p.total_q; }
+
+int limit(int x) { return x < 0 || x >= kNoLimit ? kNoLimit - 2 : x; }
+
+// keys that `rows` neighbouring rows walk over, about (a packed context's batches are taken to have
+// up to twice their average)
+int64_t max_keys(const fmlm_attn_params& p, const fmlm_window& w, int rows) {
+  int64_t keys = w.flags & FMLM_WINDOW_APPENDED ? 0 : longest(p);
+  if (p.cu_seqlens_kv)
+    keys += p.ctx_block_table ? (int64_t)p.ctx_pages_per_batch * FMLM_PAGE_ROWS
+                              : std::min((int64_t)p.ctx_rows, 2 * (int64_t)p.ctx_rows / std::max(p.ctx_batch, 1));
+  return std::min(keys, (int64_t)limit(w.left) + limit(w.right) + std::max(w.sinks, 0) + rows);
+}
+
+constexpr int kWideTiles = 12;
+
 struct FwdLaunch {
   const void* fn;
-  const void* merge;
+  const void* merge[2];  // by one row a workgroup, by as many as it has threads for
+  int merge_rows;        // ... that many
   int bq, lds;
 };
+template <typename T, int D>
+void merge_of(FwdLaunch& f) {
+  f.merge_rows = 256 / (D / 8);
+  f.merge[0] = (const void*)window_merge_kernel<T, D, 1>;
+  f.merge[1] = (const void*)window_merge_kernel<T, D, 256 / (D / 8)>;
+}
 template <typename T, int D, int QB>
 FwdLaunch fwd_of(bool fp4) {
   FwdLaunch f;
   f.fn = fp4 ? (const void*)window_fwd_kernel<T, D, QB, true> : (const void*)window_fwd_kernel<T, D, QB, false>;
-  f.merge = (const void*)window_merge_kernel<T, D>;
+  merge_of<T, D>(f);
   f.bq = kNW * QB * 16;
-  f.lds = FwdCfg<D>::LDS;
+  f.lds = fp4 ? FwdCfg<D, true>::LDS : FwdCfg<D, false>::LDS;
+  return f;
+}
+template <typename T, int D>
+FwdLaunch few_of() {
+  FwdLaunch f;
+  f.fn = (const void*)window_fp4_few_kernel<T, D>;
+  merge_of<T, D>(f);
+  f.bq = kFewRows;
+  f.lds = FewCfg<D>::LDS;
   return f;
 }
 template <typename T>
-FwdLaunch pick_fwd(const fmlm_attn_params& p, bool fp4) {
-  const bool wide = p.N == 0 || p.N > 64;  // 128 rows share a tile's loads
+FwdLaunch pick_fwd(const fmlm_attn_params& p, const fmlm_window& w) {
+  const bool fp4 = w.flags & FMLM_WINDOW_FP4;
+  if (fp4 && p.N > 0 && p.N <= kFewRows && !p.lse && !w.o_low) {
+    switch (p.D) {
+      case 32: return few_of<T, 32>();
+      case 64: return few_of<T, 64>();
+      case 128: return few_of<T, 128>();
+      default: return few_of<T, 256>();
+    }
+  }
+  // 128 rows that share a tile's loads, from walks of kWideTiles tiles on; below, more and smaller
+  // workgroups (kernel us, 64 against 128 rows: walks of 4-5 tiles, D = 64, 31 : 44; of 12, D = 128,
+  // 79 : 81; of 20, 210 : 174; of 50 in 4 bits 139 : 96)
+  const bool wide = longest(p) > 64 && max_keys(p, w, 128) > kWideTiles * kBK;
   switch (p.D) {
     case 32: return wide ? fwd_of<T, 32, 2>(fp4) : fwd_of<T, 32, 1>(fp4);
     case 64: return wide ? fwd_of<T, 64, 2>(fp4) : fwd_of<T, 64, 1>(fp4);
@@ -799,15 +1514,13 @@ FwdLaunch pick_fwd(const fmlm_attn_params& p, bool fp4) {
     default: return fwd_of<T, 256, 1>(fp4);  // (two blocks of 16 rows spill)
   }
 }
-FwdLaunch pick_fwd(const fmlm_attn_params& p, bool fp4) {
-  return p.dtype == FMLM_DTYPE_BF16 ? pick_fwd<bf16>(p, fp4) : pick_fwd<f16>(p, fp4);
+FwdLaunch pick_fwd(const fmlm_attn_params& p, const fmlm_window& w) {
+  return p.dtype == FMLM_DTYPE_BF16 ? pick_fwd<bf16>(p, w) : pick_fwd<f16>(p, w);
 }
 
 bool row_ok(const void* base, int64_t sb, int64_t sh, int64_t sn) {
   return base && (uint64_t)base % 16 == 0 && sb % 8 == 0 && sh % 8 == 0 && sn % 8 == 0 && sn >= 0 && sn < (1 << 22);
 }
-
-int longest(const fmlm_attn_params& p) { return p.N > 0 && p.N < p.total_q ? p.N : p.total_q; }
 
 int check_window(const fmlm_attn_params& p, const fmlm_window& w) {
   if (p.dtype != FMLM_DTYPE_BF16 && p.dtype != FMLM_DTYPE_F16) return FMLM_E_DTYPE;
@@ -836,11 +1549,10 @@ int check_window(const fmlm_attn_params& p, const fmlm_window& w) {
     }
   }
   if (!row_ok(p.q, p.q_sb, p.q_sh, p.q_sn) || !row_ok(p.o, p.o_sb, p.o_sh, p.o_sn)) return FMLM_E_ALIGN;
+  if (w.o_low && (uint64_t)w.o_low % 16) return FMLM_E_ALIGN;
   if (!appended && (!row_ok(p.k, p.k_sb, p.k_sh, p.k_sn) || !row_ok(p.v, p.v_sb, p.v_sh, p.v_sn))) return FMLM_E_ALIGN;
   return 0;
 }
-
-int limit(int x) { return x < 0 || x >= kNoLimit ? kNoLimit - 2 : x; }
 
 WinArgs win_args(const fmlm_attn_params& p, const fmlm_window& w, int rows) {
   WinArgs a{};
@@ -853,6 +1565,7 @@ WinArgs win_args(const fmlm_attn_params& p, const fmlm_window& w, int rows) {
   a.parts = 1;
   a.k_scales = w.k_scales;
   a.v_scales = w.v_scales;
+  a.o_low = w.o_low;
   return a;
 }
 
@@ -860,13 +1573,9 @@ WinArgs win_args(const fmlm_attn_params& p, const fmlm_window& w, int rows) {
 void plan_parts(const fmlm_attn_params& p, const fmlm_window& w, const FwdLaunch& f, WinArgs& a) {
   a.rec_rows = std::min(f.bq, longest(p));
   const int64_t units = (int64_t)p.B * p.H * a.tiles;
-  if (p.lse || (p.flags & FMLM_FLAG_NOSPLIT) || units >= 1024) return;
-  int64_t keys = longest(p);
-  if (p.cu_seqlens_kv)
-    keys += p.ctx_block_table ? (int64_t)p.ctx_pages_per_batch * FMLM_PAGE_ROWS
-                              : std::min((int64_t)p.ctx_rows, 2 * (int64_t)p.ctx_rows / std::max(p.ctx_batch, 1));
-  keys = std::min(keys, (int64_t)a.left + a.right + a.sinks + f.bq);
-  const int64_t tiles = keys / kBK + 2, want = (2048 + units - 1) / units;
+  const int64_t fill = f.bq == kFewRows ? 4096 : a.rec_rows <= 64 ? 1024 : 512;
+  if (p.lse || w.o_low || (p.flags & FMLM_FLAG_NOSPLIT) || units >= fill) return;
+  const int64_t tiles = max_keys(p, w, f.bq) / kBK + 2, want = (fill + units - 1) / units;
   a.parts = (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / kMinPartTiles, kMaxParts}));
 }
 
@@ -912,7 +1621,7 @@ extern "C" int64_t fmlm_window_workspace_bytes(const fmlm_attn_params* pp, const
   const int rc = check_window(*pp, *ww);
   if (rc) return rc;
   if (pp->B == 0 || pp->H == 0 || pp->total_q == 0) return 0;
-  const FwdLaunch f = pick_fwd(*pp, ww->flags & FMLM_WINDOW_FP4);
+  const FwdLaunch f = pick_fwd(*pp, *ww);
   WinArgs a = win_args(*pp, *ww, f.bq);
   plan_parts(*pp, *ww, f, a);
   return record_bytes(*pp, a);
@@ -924,7 +1633,7 @@ extern "C" int fmlm_window_fwd(const fmlm_attn_params* pp, const fmlm_window* ww
   int rc = check_window(p, *ww);
   if (rc) return rc;
   if (p.B == 0 || p.H == 0 || p.total_q == 0) return 0;
-  const FwdLaunch f = pick_fwd(p, ww->flags & FMLM_WINDOW_FP4);
+  const FwdLaunch f = pick_fwd(p, *ww);
   WinArgs a = win_args(p, *ww, f.bq);
   plan_parts(p, *ww, f, a);
   const int64_t need = record_bytes(p, a), blocks = (int64_t)a.tiles * a.groups * a.parts;
@@ -942,7 +1651,11 @@ extern "C" int fmlm_window_fwd(const fmlm_attn_params* pp, const fmlm_window* ww
   if (a.parts > 1) {
     int bq = f.bq;
     void* margs[3] = {&p, &a, &bq};
-    e = hipLaunchKernel(f.merge, dim3((unsigned)(a.tiles * a.groups)), dim3(256), margs, 0, s);
+    // few rows: a workgroup each, its threads share the parts
+    const bool wide = a.rec_rows > 4;
+    const int per = wide ? f.merge_rows : 1;
+    e = hipLaunchKernel(f.merge[wide], dim3((unsigned)(a.tiles * a.groups), (a.rec_rows + per - 1) / per), dim3(256), margs,
+                        0, s);
     if (e != hipSuccess) return (int)e;
   }
   return launch_status();

@@ -222,7 +222,9 @@ class PagedTensor(ctypes.Structure):
 class Window(ctypes.Structure):
     """Mirror of fmlm_window (include/flash_mlm_hip.h)."""
 
-    _fields_ = [(n, _c_i32) for n in ("left", "right", "sinks", "flags")] + [("k_scales", _c_ptr), ("v_scales", _c_ptr)]
+    _fields_ = [(n, _c_i32) for n in ("left", "right", "sinks", "flags")] + [
+        ("k_scales", _c_ptr), ("v_scales", _c_ptr), ("o_low", _c_ptr)
+    ]
 
 
 class AppendRows(ctypes.Structure):

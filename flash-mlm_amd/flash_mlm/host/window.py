@@ -40,8 +40,9 @@ class _Call:
 
     __slots__ = ("params", "window", "nbytes", "out_shape", "entry_ref", "keep", "cu")
 
-    def run(self, q, k, v, lse=None):
-        """One launch on rows laid out as the call's; returns the output."""
+    def run(self, q, k, v, lse=None, low=None):
+        """One launch on rows laid out as the call's; returns the output.  ``lse`` and ``low`` take what
+        the backward reads: the rows' statistics, and what the output's rounding took away."""
         p = _lib.AttnParams.from_buffer_copy(self.params)
         dev = q.device
         out = torch.empty(self.out_shape, dtype=q.dtype, device=dev)
@@ -49,14 +50,16 @@ class _Call:
         if k is not None:
             p.k, p.v = k.data_ptr(), v.data_ptr()
         lib = _lib.load()
-        ws, nbytes = None, self.nbytes
+        ws, nbytes, w = None, self.nbytes, self.window
         if lse is not None:
             p.lse = lse.data_ptr()
+            w = _lib.Window.from_buffer_copy(w)
+            w.o_low = low.data_ptr()
         elif nbytes:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
         with _device_scope(dev):
-            rc = lib.fmlm_window_fwd(p, self.window, _lib.stream_of(dev))
+            rc = lib.fmlm_window_fwd(p, w, _lib.stream_of(dev))
         del ws  # held until here
         _lib.check(rc, "fmlm_window_fwd")
         return out
@@ -181,21 +184,25 @@ class _Window(torch.autograd.Function):
     def forward(ctx, call, q, k, v):
         rows = _rows(q), _rows(k), _rows(v)
         lse = torch.empty(call.params.H * call.params.total_q, dtype=torch.float32, device=q.device)
-        out = call.run(*rows, lse=lse)
+        low = torch.empty(call.out_shape, dtype=q.dtype, device=q.device)
+        out = call.run(*rows, lse=lse, low=low)
         ctx.call = call
         # read from there in the backward: autograd may free these and bring others
-        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.save_for_backward(q, k, v, out, lse, low)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         call = ctx.call
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, lse, low = ctx.saved_tensors
         t = call.params.total_q
         if dout.shape != out.shape:
             raise ValueError("gradient of the attention output has the wrong shape")
-        q, k, v, out, lse, dout = *(_rows(x) for x in (q, k, v)), *(aligned16(x) for x in (out, lse, dout))
+        q, k, v = (_rows(x) for x in (q, k, v))
+        out, lse, low, dout = (aligned16(x) for x in (out, lse, low, dout))
+        w = _lib.Window.from_buffer_copy(call.window)
+        w.o_low = low.data_ptr()
         p = _lib.AttnParams.from_buffer_copy(call.params)
         g = _lib.AttnGrads()
         p.q, p.k, p.v, p.o, p.lse = (x.data_ptr() for x in (q, k, v, out, lse))
@@ -211,7 +218,7 @@ class _Window(torch.autograd.Function):
         ws = torch.empty(p.H * t, dtype=torch.float32, device=q.device)
         g.workspace, g.workspace_bytes = ws.data_ptr(), 4 * ws.numel()
         with _device_scope(q.device):
-            rc = _lib.load().fmlm_window_bwd(p, call.window, g, _lib.stream_of(q.device))
+            rc = _lib.load().fmlm_window_bwd(p, w, g, _lib.stream_of(q.device))
         _lib.check(rc, "fmlm_window_bwd")
         return None, dq, dk, dv
 

@@ -539,6 +539,9 @@ typedef struct fmlm_window {
   int32_t left, right, sinks, flags;
   const uint8_t* k_scales; /* FMLM_WINDOW_FP4 */
   const uint8_t* v_scales;
+  void* o_low; /* NULL, or laid out like o: what o's rounding took away (o + o_low is the result to
+                  twice the type's digits).  A backward with it has delta = rowsum(do o) without
+                  that rounding, whose part in dq and dk is largest in narrow windows */
 } fmlm_window;
 
 FMLM_API int fmlm_window_size(void);
