@@ -15,8 +15,7 @@
 //
 // Bound by memory: every row is read once and written once.  A row belongs to D / 8 neighbouring
 // lanes, 8 elements each, so that a block's maximum is a maximum of four lanes; a thread keeps its
-// row's angles over its heads.  The partner of a half-split pair is loaded again, from the row
-// that the lane beside just read.
+// row's angles over its heads.  The partner of a half-split pair comes from its lane, as read.
 #include "fmlm_common.h"
 
 #include <algorithm>
@@ -129,17 +128,13 @@ __global__ __launch_bounds__(kRaThreads) void rotate_append_kernel(const RaParam
   }
   const bool turn = which < 2 && d < p.rotary_dim, pairs = p.flags & FMLM_AP_INTERLEAVED;
   const int half = p.rotary_dim / 2;
-  const int other = d < half ? half : -half;  // half-split: from an element to its partner
+  // half-split: the lane of the row that holds the partners (every lane of a row has come this far)
+  const int from = (threadIdx.x & 63) + (!turn ? 0 : d < half ? half / 8 : -half / 8);
   const T* in = (const T*)a.src + src + d;
-  u32x4 x[kRaHeads], y[kRaHeads];
+  u32x4 x[kRaHeads];
 #pragma unroll
   for (int u = 0; u < kRaHeads; ++u)
     if (u < nh) x[u] = *(const u32x4*)(in + (h0 + u) * a.s_sh);
-  if (turn && !pairs) {
-#pragma unroll
-    for (int u = 0; u < kRaHeads; ++u)
-      if (u < nh) y[u] = *(const u32x4*)(in + (h0 + u) * a.s_sh + other);
-  }
   float cs[8], sn[8];  // sn with the pair member's sign: element j becomes x_j cs_j + partner_j sn_j
   if (turn) {
     int64_t s = p.flags & FMLM_AP_POSITIONS_I64 ? ((const int64_t*)p.positions)[t] : ((const int32_t*)p.positions)[t];
@@ -169,13 +164,14 @@ __global__ __launch_bounds__(kRaThreads) void rotate_append_kernel(const RaParam
     if (u >= nh) break;
     float f[8], g[8];
     oct_of<T>(x[u], f);
-    if (turn) {
-      if (pairs) {
+    if (pairs) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = f[j ^ 1];
-      } else {
-        oct_of<T>(y[u], g);
-      }
+      for (int j = 0; j < 8; ++j) g[j] = f[j ^ 1];
+    } else if (which < 2 && p.rotary_dim > 0) {  // (the same in a wave: every lane gives its own)
+      u32x4 y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * from, (int)x[u][j]);
+      oct_of<T>(y, g);
     }
     if (FP4 && which > 0) {
       if (turn) {
@@ -201,12 +197,16 @@ __global__ __launch_bounds__(kRaThreads) void rotate_append_kernel(const RaParam
   }
 }
 
-// 8 values a thread and step
+// 8 values a thread and step; blockIdx.y: pool
 constexpr int kFvSteps = 4;
+struct Fp4Pools {
+  fmlm_fp4_rows t[2];
+};
 template <typename T>
-__global__ __launch_bounds__(256) void fp4_values_kernel(const uint32_t* __restrict__ codes,
-                                                         const uint8_t* __restrict__ scales, u32x4* __restrict__ out,
-                                                         int64_t n) {
+__global__ __launch_bounds__(256) void fp4_values_kernel(const Fp4Pools pools, int64_t n) {
+  const fmlm_fp4_rows& p = pools.t[blockIdx.y];
+  const uint32_t* const codes = (const uint32_t*)p.codes;
+  u32x4* const out = (u32x4*)p.out;
   const int64_t first = (int64_t)blockIdx.x * (256 * kFvSteps) + threadIdx.x;
   uint32_t c[kFvSteps], s[kFvSteps];
 #pragma unroll
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256) void fp4_values_kernel(const uint32_t* __restr
     const int64_t at = first + i * 256;
     if (at < n) {
       c[i] = codes[at];
-      s[i] = scales[at / (kFp4Block / 8)];
+      s[i] = p.scales[at / (kFp4Block / 8)];
     }
   }
 #pragma unroll
@@ -282,22 +282,23 @@ extern "C" int fmlm_rotate_append(const fmlm_append_params* pp, void* stream) {
   return launch_status();
 }
 
-extern "C" int fmlm_fp4_values(int32_t dtype, const uint8_t* codes, const uint8_t* scales, void* out, int64_t rows,
-                               int32_t D, void* stream) {
+extern "C" int fmlm_fp4_values(int32_t dtype, const fmlm_fp4_rows* tensors, int32_t n_tensors, int64_t rows, int32_t D,
+                               void* stream) {
   if (dtype != FMLM_DTYPE_BF16 && dtype != FMLM_DTYPE_F16) return FMLM_E_DTYPE;
   if (D < kFp4Block || D % kFp4Block) return FMLM_E_HEAD_DIM;
-  if (rows < 0) return FMLM_E_ARG;
+  if (!tensors || n_tensors < 1 || n_tensors > 2 || rows < 0) return FMLM_E_ARG;
   if (rows == 0) return 0;
-  if (!codes || !scales || !out) return FMLM_E_ARG;
-  if ((uint64_t)codes % 4 || (uint64_t)out % 16) return FMLM_E_ALIGN;
+  Fp4Pools pools{};
+  for (int i = 0; i < n_tensors; ++i) {
+    const fmlm_fp4_rows& t = pools.t[i] = tensors[i];
+    if (!t.codes || !t.scales || !t.out) return FMLM_E_ARG;
+    if ((uint64_t)t.codes % 4 || (uint64_t)t.out % 16) return FMLM_E_ALIGN;
+  }
   const int64_t n = rows * (D / 8), blocks = (n + 256 * kFvSteps - 1) / (256 * kFvSteps);
   if (blocks > 0x7fffffff) return FMLM_E_ARG;
+  const dim3 grid((unsigned)blocks, n_tensors);
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == FMLM_DTYPE_BF16)
-    hipLaunchKernelGGL(fp4_values_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, s, (const uint32_t*)codes, scales,
-                       (u32x4*)out, n);
-  else
-    hipLaunchKernelGGL(fp4_values_kernel<f16>, dim3((unsigned)blocks), dim3(256), 0, s, (const uint32_t*)codes, scales,
-                       (u32x4*)out, n);
+  if (dtype == FMLM_DTYPE_BF16) hipLaunchKernelGGL(fp4_values_kernel<bf16>, grid, dim3(256), 0, s, pools, n);
+  else hipLaunchKernelGGL(fp4_values_kernel<f16>, grid, dim3(256), 0, s, pools, n);
   return launch_status();
 }

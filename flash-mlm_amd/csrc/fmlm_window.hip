@@ -24,7 +24,8 @@ namespace fmlm {
 namespace {
 
 constexpr int kNW = 4;    // waves of a workgroup
-constexpr int kBK = 64;   // keys of a tile
+constexpr int kBK = 64;   // keys of a tile; 32 at D = 256, where two workgroups of them fit a CU
+constexpr int tile_keys(int D) { return D == 256 ? 32 : kBK; }
 constexpr int kMaxParts = 32;
 constexpr int kMinPartTiles = 4;  // key tiles of a part at least
 constexpr int kNoLimit = 1 << 30;  // a window without a limit; positions stay below
@@ -38,6 +39,7 @@ struct WinArgs {
   int groups;  // (sequence, head) pairs, rounded up to a multiple of the XCDs
   int parts;   // parts of a key range at most
   int rec_rows;  // rows of a part's record
+  int lg;        // log2 of the keys of a tile of the records' walk
   const uint8_t* k_scales;
   const uint8_t* v_scales;
   float* records;
@@ -64,15 +66,15 @@ FMLM_DEV WinSeq win_seq(const fmlm_attn_params& p, const WinArgs& a, int b, int 
 }
 
 // ---- the key tiles that the rows at positions [p0, p1] see: tiles [0, sink) and then [lo, ...),
-// n in all; tile t < nt0 is context keys 64 t.., the others main keys 64 (t - nt0)..
+// n in all; of tiles of 2^lg keys, t < nt0 is context keys 2^lg t.., the others main keys
 struct WinTiles {
   int sink, lo, n, nt0;
   FMLM_DEV int tile(int v) const { return v < sink ? v : lo + (v - sink); }
 };
-FMLM_DEV WinTiles win_tiles(const WinArgs& a, const WinSeq& s, int p0, int p1) {
+FMLM_DEV WinTiles win_tiles(const WinArgs& a, const WinSeq& s, int p0, int p1, int lg) {
   WinTiles w;
-  w.nt0 = (s.ctx + kBK - 1) / kBK;
-  auto tile_of = [&](int key) { return key < s.ctx ? key / kBK : w.nt0 + (key - s.ctx) / kBK; };
+  w.nt0 = (s.ctx + (1 << lg) - 1) >> lg;
+  auto tile_of = [&](int key) { return key < s.ctx ? key >> lg : w.nt0 + ((key - s.ctx) >> lg); };
   const int hi = min(s.total, p1 + a.right + 1), lo = max(0, p0 - a.left);
   w.sink = w.lo = w.n = 0;
   if (hi <= 0) return w;
@@ -172,16 +174,15 @@ FMLM_DEV uint32_t pack2(float x, float y) {
 // on the CU (80 KB each): their loads then have two steps to land.
 template <int D, bool FP4>
 struct FwdCfg {
-  static constexpr int TILEB = kBK * D * 2;
-  static constexpr int NV = FP4 || D == 256 ? 2 : 3;
-  static constexpr bool STAGE = FP4 && D == 128;  // codes wait in LDS (else in registers)
+  static constexpr int BK = tile_keys(D), TILEB = BK * D * 2;
+  static constexpr int NV = FP4 ? 2 : 3;
+  static constexpr int TPR = kNW * 64 / BK;    // threads that share a 4-bit row
+  static constexpr int CW = D / TPR / 8;       // dwords of codes of each
+  static constexpr bool STAGE = FP4 && CW == 4;  // codes wait in LDS (else in registers)
   static constexpr int LDS = (2 + NV) * TILEB + (STAGE ? 2 * kNW * 1024 : 0);
-  static constexpr int WPS = D <= 128 ? 2 : 1;
-  static constexpr int KC = D / 32, NDB = D / 16;
+  static constexpr int KC = D / 32, NDB = D / 16, NKB = BK / 16, NKS = BK / 32;
   static constexpr int LEAD = D <= 64 ? 2 : 3;  // LDS fragment reads in flight ahead of use
-  static constexpr int NKF = KC * 4, NVF = 2 * NDB;  // K and V fragments of a tile
-  static constexpr int CW = D / 32;                  // dwords of codes of a thread: a quarter row
-  static constexpr int CS = FP4 && D == 256 ? 2 : 1;  // and their scales
+  static constexpr int NKF = KC * NKB, NVF = NKS * NDB;  // K and V fragments of a tile
 };
 
 // ---------------------------------------------------------------------------
@@ -193,10 +194,10 @@ struct FwdCfg {
 // the start of step v + 1.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int QB, bool FP4>
-__global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_kernel(const fmlm_attn_params p, const WinArgs a) {
+__global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn_params p, const WinArgs a) {
   typedef FwdCfg<D, FP4> C;
   typedef typename Mfma<T>::v8 v8;
-  constexpr int BQ = kNW * QB * 16, CW = C::CW, CS = C::CS;
+  constexpr int BQ = kNW * QB * 16, CW = C::CW, BK = C::BK, NKB = C::NKB, NKS = C::NKS;
   extern __shared__ __align__(16) char smem[];
   // buffers of tile v; a step takes them from its place among NU unrolled ones, as constants
   constexpr int NU = C::NV == 2 ? 2 : 6;
@@ -210,7 +211,7 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
   const WinSeq s = win_seq(p, a, g / p.H, g % p.H);
   const int row0 = tile * BQ, rows = min(BQ, s.len - row0);
   if (rows <= 0) return;
-  const WinTiles wt = win_tiles(a, s, s.first + row0, s.first + row0 + rows - 1);
+  const WinTiles wt = win_tiles(a, s, s.first + row0, s.first + row0 + rows - 1, BK == 64 ? 6 : 5);
   const int parts = win_parts(wt.n, a.parts);
   if (part >= parts) return;
   const int vb = (int)((int64_t)wt.n * part / parts), n = (int)((int64_t)wt.n * (part + 1) / parts) - vb;
@@ -229,8 +230,8 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
   int ctx0 = 0, ctx1;
   ctx_range(p, cb, ctx0, ctx1);
   const int32_t* const pages = p.ctx_block_table ? p.ctx_block_table + (int64_t)cb * p.ctx_pages_per_batch : nullptr;
-  auto keys_in = [&](int t) { return min(kBK, t < wt.nt0 ? s.ctx - t * kBK : s.total - s.ctx - (t - wt.nt0) * kBK); };
-  // Page ids of 64 consecutive tiles, one a lane: a tile then costs a lane read.  (One load a tile
+  auto keys_in = [&](int t) { return min(BK, t < wt.nt0 ? s.ctx - t * BK : s.total - s.ctx - (t - wt.nt0) * BK); };
+  // Ids of 64 consecutive pages, one a lane: a tile then costs a lane read.  (One load a tile
   // would wait, with everything in flight, a round trip each.)
   int win_ids = 0, win_first = -(1 << 30);
   auto page_of = [&](int t) {
@@ -243,17 +244,19 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
   };
   // context tile t's first row, in elements of a pool or a packed context
   auto ctx_elem = [&](int t) {
-    return (int64_t)s.h * p.c_sh + (pages ? (int64_t)page_of(t) * p.ctx_page_stride : (int64_t)(ctx0 + t * kBK) * p.c_sn);
+    constexpr int PT = FMLM_PAGE_ROWS / BK;  // tiles of a page
+    return (int64_t)s.h * p.c_sh + (pages ? (int64_t)page_of(t / PT) * p.ctx_page_stride + (t % PT) * BK * p.c_sn
+                                          : (int64_t)(ctx0 + t * BK) * p.c_sn);
   };
   // a 16-bit tile's loads
   auto fetch = [&](int t, bool is_v, char* to) {
     const int last = keys_in(t) - 1;
     if (t < wt.nt0) {
-      WTile<T, D>::template load<kBK>((const char*)(is_v ? p.v_ctx : p.k_ctx) + ctx_elem(t) * 2, (uint32_t)p.c_sn * 2u, last,
+      WTile<T, D>::template load<BK>((const char*)(is_v ? p.v_ctx : p.k_ctx) + ctx_elem(t) * 2, (uint32_t)p.c_sn * 2u, last,
                                       lds_addr(to), wave, lane);
     } else {
       const int64_t sb = is_v ? p.v_sb : p.k_sb, sh = is_v ? p.v_sh : p.k_sh, sn = is_v ? p.v_sn : p.k_sn;
-      WTile<T, D>::template load<kBK>((const char*)(is_v ? p.v : p.k) + row_at(p.kv_layout, s.b, s.h, s.q0, (t - wt.nt0) * kBK, sb, sh, sn) * 2,
+      WTile<T, D>::template load<BK>((const char*)(is_v ? p.v : p.k) + row_at(p.kv_layout, s.b, s.h, s.q0, (t - wt.nt0) * BK, sb, sh, sn) * 2,
                                       (uint32_t)sn * 2u, last, lds_addr(to), wave, lane);
     }
   };
@@ -273,7 +276,7 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
       wk.k = uniform_ptr((const char*)p.k_ctx + e);
       wk.v = uniform_ptr((const char*)p.v_ctx + e);
     } else {
-      const int j = (wk.t - wt.nt0) * kBK;
+      const int j = (wk.t - wt.nt0) * BK;
       wk.rk = __builtin_amdgcn_readfirstlane((uint32_t)p.k_sn * 2u);
       wk.rv = __builtin_amdgcn_readfirstlane((uint32_t)p.v_sn * 2u);
       wk.k = uniform_ptr((const char*)p.k + row_at(p.kv_layout, s.b, s.h, s.q0, j, p.k_sb, p.k_sh, p.k_sn) * 2);
@@ -290,29 +293,29 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
     }
     wk.at = v;
     wk.t += 1;
-    wk.k += (size_t)wk.rk * kBK;
-    wk.v += (size_t)wk.rv * kBK;
+    wk.k += (size_t)wk.rk * BK;
+    wk.v += (size_t)wk.rv * BK;
   };
   // lane offsets of a whole tile at the pitch of most of them
   typedef WTile<T, D> Tile;
-  constexpr int NL = kBK / (Tile::RPI * kNW);
+  constexpr int NL = BK / (Tile::RPI * kNW);
   uint32_t off0[FP4 ? 1 : NL];
   uint32_t pitch0 = 0;
   auto load_rows = [&](const char* src, uint32_t pitch, int last, char* to) {
     if constexpr (!FP4) {
-      if (last == kBK - 1 && pitch == pitch0) {
-        Tile::template load_at<kBK>(src, off0, lds_addr(to), wave);
+      if (last == BK - 1 && pitch == pitch0) {
+        Tile::template load_at<BK>(src, off0, lds_addr(to), wave);
         return;
       }
     }
-    Tile::template load<kBK>(src, pitch, last, lds_addr(to), wave, lane);
+    Tile::template load<BK>(src, pitch, last, lds_addr(to), wave, lane);
   };
-  // a 4-bit tile: thread i has quarter i % 4 of row i / 4, CW dwords
-  uint32_t code[2][C::STAGE ? 1 : CW], csc[2][CS];
+  // a 4-bit tile: thread i has part i % TPR of row i / TPR, CW dwords
+  uint32_t code[2][C::STAGE ? 1 : CW], csc[2];
   auto fetch_codes = [&](int t, bool is_v) {
-    const int row = min(tid >> 2, keys_in(t) - 1), x = is_v ? 1 : 0;
+    const int row = min(tid / C::TPR, keys_in(t) - 1), x = is_v ? 1 : 0;
     const int64_t e0 = ctx_elem(t);
-    const uint32_t at = (uint32_t)row * D + (tid & 3) * (D / 4);
+    const uint32_t at = (uint32_t)row * D + (tid % C::TPR) * (D / C::TPR);
     const char* const src = uniform_ptr((const char*)(is_v ? p.v_ctx : p.k_ctx) + e0 / 2);
     const char* const ssc = uniform_ptr((const char*)(is_v ? a.v_scales : a.k_scales) + e0 / kFp4Block);
     if constexpr (C::STAGE) {
@@ -323,20 +326,12 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
       const u32x2 w = *(const u32x2*)(src + at / 2);
       code[x][0] = w[0];
       code[x][1] = w[1];
-    } else {
-#pragma unroll
-      for (int i = 0; i < CW; i += 4) {
-        const u32x4 w = *(const u32x4*)(src + at / 2 + 4 * i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) code[x][i + j] = w[j];
-      }
     }
-#pragma unroll
-    for (int i = 0; i < CS; ++i) csc[x][i] = (uint8_t)ssc[at / kFp4Block + i];
+    csc[x] = (uint8_t)ssc[at / kFp4Block];
   };
   // the loaded codes as a 16-bit tile (STAGE: this wave's load has landed)
   auto put_codes = [&](bool is_v, char* to) {
-    const int row = tid >> 2, x = is_v ? 1 : 0;
+    const int row = tid / C::TPR, x = is_v ? 1 : 0;
     uint32_t w[CW];
     if constexpr (C::STAGE) {
       const u32x4 r = *(const u32x4*)(smem + (2 + C::NV) * C::TILEB + (2 * wave + x) * 1024 + 16 * lane);
@@ -348,41 +343,41 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
     }
 #pragma unroll
     for (int i = 0; i < CW; ++i)
-      *(u32x4*)(to + row * (D * 2) + 16 * (((tid & 3) * CW + i) ^ kv_swz<D>(row))) = fp4_oct<T>(w[i], fp4_scale(csc[x][i / 4 % CS]));
+      *(u32x4*)(to + row * (D * 2) + 16 * (((tid % C::TPR) * CW + i) ^ kv_swz<D>(row))) = fp4_oct<T>(w[i], fp4_scale(csc[x]));
   };
   auto is_code = [&](int t) { return FP4 && t < wt.nt0; };
 
   v8 qf[QB][C::KC];
   f32x4 o[C::NDB][QB], lsum[QB];
   float m[QB], mx[QB];
-  f32x4 sa[4][QB], sb[4][QB];
+  f32x4 sa[NKB][QB], sb[NKB][QB];
   v8 ones;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = (T)1.0f;
   pin(ones);
 
   // raw row maxima of a score tile
-  auto row_max = [&](const f32x4 (&x)[4][QB]) {
+  auto row_max = [&](const f32x4 (&x)[NKB][QB]) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       float y = vmax(vmax(x[0][qb][0], x[0][qb][1]), vmax(x[0][qb][2], x[0][qb][3]));
 #pragma unroll
-      for (int kb = 1; kb < 4; ++kb)
+      for (int kb = 1; kb < NKB; ++kb)
         y = vmax(vmax(y, vmax(x[kb][qb][0], x[kb][qb][1])), vmax(x[kb][qb][2], x[kb][qb][3]));
       mx[qb] = lane_max_xor16_32(y);
     }
   };
   const int w0 = s.first + row0 + wave * QB * 16, w1 = min(w0 + QB * 16, s.first + row0 + rows) - 1;
   // scores of keys that a row does not see to -inf; returns whether there can be any
-  auto mask = [&](int t, f32x4 (&x)[4][QB]) {
-    const int nk = keys_in(t), kp = t < wt.nt0 ? t * kBK : s.ctx + (t - wt.nt0) * kBK;
-    if (!(nk < kBK || kp + kBK - 1 > w0 + a.right || (kp < w1 - a.left && kp + kBK > a.sinks))) return false;
+  auto mask = [&](int t, f32x4 (&x)[NKB][QB]) {
+    const int nk = keys_in(t), kp = t < wt.nt0 ? t * BK : s.ctx + (t - wt.nt0) * BK;
+    if (!(nk < BK || kp + BK - 1 > w0 + a.right || (kp < w1 - a.left && kp + BK > a.sinks))) return false;
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       const int pos = w0 + qb * 16 + l16, k0 = kp + 4 * gq;  // element (kb, r) is key k0 + 16 kb + r
       const int top = min(pos + a.right - k0, nk - 1 - 4 * gq), low = pos - a.left - k0, snk = a.sinks - k0;
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
+      for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = kb * 16 + r;
@@ -394,27 +389,27 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
 
   // ---- the slots.  Slot s runs the MFMAs of fragment s: [0, NKF) of K(v + 1) (sn += K Q^T, beside a
   // share of P(v)'s exponentials), [NKF, NF) of V(v) (O += V^T P, beside a share of sn's maxima).
-  constexpr int NF = C::NKF + C::NVF, NP = 4 * QB * 2, NMS = 4 * QB + QB;
-  u32x4 pf[2][QB];
-  auto slots = [&](f32x4 (&sc)[4][QB], f32x4 (&sn)[4][QB], const char* kn, const char* vt) {
+  constexpr int NF = C::NKF + C::NVF, NP = NKB * QB * 2, NMS = NKB * QB + QB;
+  u32x4 pf[NKS][QB];
+  auto slots = [&](f32x4 (&sc)[NKB][QB], f32x4 (&sn)[NKB][QB], const char* kn, const char* vt) {
     float ref[QB], mpart[QB], mhold[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) ref[qb] = m[qb] == -INFINITY ? 0.f : -m[qb];  // (no key yet: every score is -inf)
     v8 fr[C::LEAD + 1];
     auto issue = [&](int r) {
-      if (r < C::NKF) fr[r % (C::LEAD + 1)] = tr.row(kn, r % 4, r / 4);
+      if (r < C::NKF) fr[r % (C::LEAD + 1)] = tr.row(kn, r % NKB, r / NKB);
       else fr[r % (C::LEAD + 1)] = tr.col(vt, (r - C::NKF) / C::NDB, (r - C::NKF) % C::NDB);
     };
     auto exp_pair = [&](int pi) {
-      const int qb = pi / 8, kb = (pi >> 1) % 4, r = (pi & 1) * 2;
+      const int qb = pi / (2 * NKB), kb = (pi >> 1) % NKB, r = (pi & 1) * 2;
       if (r == 0) pin(sc[kb][qb]);
       uint32_t w = pack2<T>(fast_exp2(fmaf(sc[kb][qb][r], c, ref[qb])), fast_exp2(fmaf(sc[kb][qb][r + 1], c, ref[qb])));
       pin(w);
       pf[kb >> 1][qb][(kb & 1) * 2 + (pi & 1)] = w;
     };
     auto max_step = [&](int k) {
-      if (k < 4 * QB) {
-        const int qb = k / 4, kb = k % 4;
+      if (k < NKB * QB) {
+        const int qb = k / NKB, kb = k % NKB;
         pin(sn[kb][qb]);
         const f32x4 x = sn[kb][qb];
         if (kb == 0) {
@@ -424,10 +419,10 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
           mpart[qb] = vmax(vmax(mpart[qb], x[1]), x[2]);
         }
         mhold[qb] = x[3];
-        if (kb == 3) mpart[qb] = vmax(mpart[qb], mhold[qb]);
+        if (kb == NKB - 1) mpart[qb] = vmax(mpart[qb], mhold[qb]);
         pin(mpart[qb]);
       } else {
-        const int qb = k - 4 * QB;
+        const int qb = k - NKB * QB;
         mx[qb] = lane_max_xor16_32(mpart[qb]);
         pin(mx[qb]);
       }
@@ -441,7 +436,7 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
       if (sl == C::NKF) __builtin_amdgcn_s_setprio(2);
       const v8 x = fr[sl % (C::LEAD + 1)];
       if (sl < C::NKF) {
-        const int kb = sl % 4, kc = sl / 4;
+        const int kb = sl % NKB, kc = sl / NKB;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
           sn[kb][qb] = Mfma<T>::run(x, qf[qb][kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sn[kb][qb]);
@@ -464,7 +459,7 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
   const char* v_next = nullptr;
   uint32_t v_pitch = 0;
   int v_last = 0;
-  auto step = [&](int v, int u, f32x4 (&sc)[4][QB], f32x4 (&sn)[4][QB]) {
+  auto step = [&](int v, int u, f32x4 (&sc)[NKB][QB], f32x4 (&sn)[NKB][QB]) {
     if constexpr (FP4) {
       const int tk = v + 2 < n ? tile_at(v + 2) : -1, tv = v + 1 < n ? tile_at(v + 1) : -1;
       if (tk >= 0 && is_code(tk)) put_codes(false, kbuf(u));
@@ -515,7 +510,7 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
       slots(sc, sn, kbuf(u + 1), vbuf(u));
     }
     // the loads of the next step's tiles have landed: all but V(v + 2)'s, the last ones issued
-    constexpr int VPW = kBK / (WTile<T, D>::RPI * kNW);
+    constexpr int VPW = BK / (WTile<T, D>::RPI * kNW);
     if (C::NV == 3 && v + 2 < n) __builtin_amdgcn_s_waitcnt((VPW & 15) | (7 << 4) | (0 << 8) | ((VPW >> 4) << 14));
     else __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
@@ -559,7 +554,7 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
     } else {
       seek(0);
       pitch0 = wk.rk;
-      Tile::template offsets<kBK>(pitch0, wave, lane, off0);
+      Tile::template offsets<BK>(pitch0, wave, lane, off0);
       load_rows(wk.k, wk.rk, keys_in(wk.t) - 1, kbuf(0));
       load_rows(wk.v, wk.rv, keys_in(wk.t) - 1, vbuf(0));
       move();
@@ -582,7 +577,7 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
 #pragma unroll
       for (int kc = 0; kc < C::KC; ++kc)
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
+        for (int kb = 0; kb < NKB; ++kb) {
           const v8 x = tr.row(kbuf(0), kb, kc);
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb)
@@ -668,20 +663,20 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
       bring(v, true, vt);
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
-      const int t = tile_at(v), nk = keys_in(t), kp = t < wt.nt0 ? t * kBK : s.ctx + (t - wt.nt0) * kBK;
-      f32x4 sc[4];
+      const int t = tile_at(v), nk = keys_in(t), kp = t < wt.nt0 ? t * BK : s.ctx + (t - wt.nt0) * BK;
+      f32x4 sc[NKB];
 #pragma unroll
       for (int kc = 0; kc < C::KC; ++kc) {
         const v8 f = q_frag(qb, kc);
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
+        for (int kb = 0; kb < NKB; ++kb)
           sc[kb] = Mfma<T>::run(tr.row(kbuf(0), kb, kc), f, kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[kb]);
       }
       const int pos = w0 + qb * 16 + l16, k0 = kp + 4 * gq;
       const int top = min(pos + a.right - k0, nk - 1 - 4 * gq), low = pos - a.left - k0, snk = a.sinks - k0;
       float y = -INFINITY;
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
+      for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = kb * 16 + r;
@@ -695,12 +690,12 @@ __global__ __launch_bounds__(kNW * 64, (FwdCfg<D, FP4>::WPS)) void window_fwd_ke
 #pragma unroll
       for (int db = 0; db < C::NDB; ++db) x[db] *= alpha;
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
+      for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) pw[l16 * 64 + kb * 16 + 4 * gq + r] = (T)fast_exp2(fmaf(sc[kb][r], c, -ref));
       asm volatile("" ::: "memory");
 #pragma clang loop unroll(disable)
-      for (int j = 0; j < kBK; ++j) {
+      for (int j = 0; j < BK; ++j) {
         const float w = (float)pw[l16 * 64 + j];
         l += w;
         if (w != 0.f) {
@@ -749,7 +744,7 @@ __global__ __launch_bounds__(kNW * 64, FewCfg<D>::WPS) void window_fp4_few_kerne
   const WinSeq s = win_seq(p, a, g / p.H, g % p.H);
   const int rows = min(kFewRows, s.len);
   if (rows <= 0) return;
-  const WinTiles wt = win_tiles(a, s, s.first, s.first + rows - 1);
+  const WinTiles wt = win_tiles(a, s, s.first, s.first + rows - 1, 6);
   const int parts = win_parts(wt.n, a.parts);
   if (part >= parts) return;
   const int vb = (int)((int64_t)wt.n * part / parts), ve = (int)((int64_t)wt.n * (part + 1) / parts);
@@ -1009,7 +1004,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const fmlm_attn_param
   const int tid = threadIdx.x, c8 = tid % CPR, rr = (tid / CPR) % RR, gg = tid / (CPR * RR);
   const int row = blockIdx.y * RR + rr;
   if ((int)blockIdx.y * RR >= rows) return;
-  const int parts = win_parts(win_tiles(a, s, s.first + row0, s.first + row0 + rows - 1).n, a.parts);
+  const int parts = win_parts(win_tiles(a, s, s.first + row0, s.first + row0 + rows - 1, a.lg).n, a.parts);
   if (parts <= 1) return;
   const int64_t unit = ((int64_t)(a.tiles - 1 - tile) * a.groups + g) * a.parts, pitch = (int64_t)a.rec_rows * (D + 4);
   const float* const rec = a.records + unit * pitch + (int64_t)row * D + c8 * 8;
@@ -1088,12 +1083,12 @@ struct BwdCfg {
   static constexpr int QB = D == 128 ? 2 : 1;   // dq: 16-row blocks of a wave
   static constexpr int BQ = kNW * QB * 16;
   static constexpr int QS = D == 256 ? 32 : 64;  // dK / dV: query rows of a step
-  static constexpr int TILEB = kBK * D * 2;
+  static constexpr int BK = tile_keys(D), NKB = BK / 16, NKS = BK / 32;  // dq: keys of a tile
+  static constexpr int TILEB = BK * D * 2;
   static constexpr int DQ_LDS = 4 * TILEB;
   static constexpr int STEPB = QS * D * 2;
   static constexpr int SB = 2 * STEPB + 2 * QS * 4;  // a step: q rows, do rows, lse, delta
   static constexpr int DKV_LDS = 2 * SB;
-  static constexpr int WPS = D <= 128 ? 2 : 1;
   static constexpr int KC = D / 32, NDB = D / 16;
 };
 
@@ -1103,11 +1098,11 @@ FMLM_DEV void zero_row4(void* base, int64_t elem) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(const fmlm_attn_params p, const WinArgs a,
+__global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_params p, const WinArgs a,
                                                                              const fmlm_attn_grads gr) {
   typedef BwdCfg<D> C;
   typedef typename Mfma<T>::v8 v8;
-  constexpr int QB = C::QB;
+  constexpr int QB = C::QB, BK = C::BK, NKB = C::NKB, NKS = C::NKS;
   extern __shared__ __align__(16) char smem[];
   auto kbuf = [&](int i) { return smem + i * C::TILEB; };
   auto vbuf = [&](int i) { return smem + (2 + i) * C::TILEB; };
@@ -1130,12 +1125,21 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(con
     }
   }
   if (rows <= 0) return;
-  const WinTiles wt = win_tiles(a, s, row0, row0 + rows - 1);
+  const WinTiles wt = win_tiles(a, s, row0, row0 + rows - 1, BK == 64 ? 6 : 5);
   const WTile<T, D> tr(l16, gq);
   const bool active = wave * QB * 16 < rows;
   // (a scale of 0 would lose the masked scores' infinity; this one leaves every other 2^(c s) at 1)
   const float c = p.scale != 0.f ? p.scale * kLog2e : 1e-30f;
 
+  auto keys_in = [&](int t) { return min(BK, s.total - t * BK); };
+  auto issue = [&](int v) {
+    const int t = wt.tile(v), buf = v & 1, last = keys_in(t) - 1;
+    WTile<T, D>::template load<BK>((const char*)p.k + row_at(p.kv_layout, s.b, s.h, s.q0, t * BK, p.k_sb, p.k_sh, p.k_sn) * 2,
+                                    (uint32_t)p.k_sn * 2u, last, lds_addr(kbuf(buf)), wave, lane);
+    WTile<T, D>::template load<BK>((const char*)p.v + row_at(p.kv_layout, s.b, s.h, s.q0, t * BK, p.v_sb, p.v_sh, p.v_sn) * 2,
+                                    (uint32_t)p.v_sn * 2u, last, lds_addr(vbuf(buf)), wave, lane);
+  };
+  if (wt.n > 0) issue(0);
   v8 qf[QB][C::KC], df[QB][C::KC];
   float delta[QB], lse[QB];
 #pragma unroll
@@ -1162,20 +1166,11 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(con
     lse[qb] = ok ? p.lse[at] : INFINITY;
     if (ok && gq == 0) ((float*)gr.workspace)[at] = sum;  // for the dK / dV kernel
   }
-  auto keys_in = [&](int t) { return min(kBK, s.total - t * kBK); };
-  auto issue = [&](int v) {
-    const int t = wt.tile(v), buf = v & 1, last = keys_in(t) - 1;
-    WTile<T, D>::template load<kBK>((const char*)p.k + row_at(p.kv_layout, s.b, s.h, s.q0, t * kBK, p.k_sb, p.k_sh, p.k_sn) * 2,
-                                    (uint32_t)p.k_sn * 2u, last, lds_addr(kbuf(buf)), wave, lane);
-    WTile<T, D>::template load<kBK>((const char*)p.v + row_at(p.kv_layout, s.b, s.h, s.q0, t * kBK, p.v_sb, p.v_sh, p.v_sn) * 2,
-                                    (uint32_t)p.v_sn * 2u, last, lds_addr(vbuf(buf)), wave, lane);
-  };
   f32x4 dq[C::NDB][QB];
 #pragma unroll
   for (int db = 0; db < C::NDB; ++db)
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) dq[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (wt.n > 0) issue(0);
   for (int v = 0; v < wt.n; ++v) {
     const int t = wt.tile(v), buf = v & 1, nk = keys_in(t);
     __builtin_amdgcn_s_waitcnt(0);
@@ -1186,12 +1181,12 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(con
     // ---- fenced slots, each the MFMAs of one LDS fragment: NSS of S^T (step kc, key block kb), NSS of
     // dP^T (block by block), 2 NDB of dq^T; the fragment of slot s + LEAD is read at slot s.  Block
     // kb's P and dS are made beside block kb + 1's dP, the last one's beside the first dq slots.
-    constexpr int NSS = 4 * C::KC, NR = 2 * NSS, NS = NR + 2 * C::NDB, LEAD = 3;
-    f32x4 sc[4][QB], dp[4][QB];
-    u32x4 ds[2][QB];
+    constexpr int NSS = NKB * C::KC, NR = 2 * NSS, NS = NR + NKS * C::NDB, LEAD = 3;
+    f32x4 sc[NKB][QB], dp[NKB][QB];
+    u32x4 ds[NKS][QB];
     v8 fr[LEAD + 1];
     auto read = [&](int r) {
-      if (r < NSS) fr[r % (LEAD + 1)] = tr.row(kt, r % 4, r / 4);
+      if (r < NSS) fr[r % (LEAD + 1)] = tr.row(kt, r % NKB, r / NKB);
       else if (r < NR) fr[r % (LEAD + 1)] = tr.row(vt, (r - NSS) / C::KC, (r - NSS) % C::KC);
       else fr[r % (LEAD + 1)] = tr.col(kt, (r - NR) / C::NDB, (r - NR) % C::NDB);
     };
@@ -1211,14 +1206,14 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(con
     for (int sl = 0; sl < NSS; ++sl) {
       read(sl + LEAD);
       const v8 x = fr[sl % (LEAD + 1)];
-      const int kb = sl % 4, kc = sl / 4;
+      const int kb = sl % NKB, kc = sl / NKB;
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb)
         sc[kb][qb] = Mfma<T>::run(x, qf[qb][kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[kb][qb]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    const int kp = t * kBK, w0 = row0 + wave * QB * 16, w1 = min(w0 + QB * 16, row0 + rows) - 1;
-    if (nk < kBK || kp + kBK - 1 > w0 + a.right || (kp < w1 - a.left && kp + kBK > a.sinks)) {
+    const int kp = t * BK, w0 = row0 + wave * QB * 16, w1 = min(w0 + QB * 16, row0 + rows) - 1;
+    if (nk < BK || kp + BK - 1 > w0 + a.right || (kp < w1 - a.left && kp + BK > a.sinks)) {
       asm volatile("");  // (a real branch.)  What a row does not see: P = 0
       const float none = c < 0.f ? INFINITY : -INFINITY;
 #pragma unroll
@@ -1226,7 +1221,7 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(con
         const int pos = w0 + qb * 16 + l16, k0 = kp + 4 * gq;
         const int top = min(pos + a.right - k0, nk - 1 - 4 * gq), low = pos - a.left - k0, snk = a.sinks - k0;
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
+        for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int j = kb * 16 + r;
@@ -1254,9 +1249,9 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(con
       if (sl + LEAD < NS) read(sl + LEAD);
       const v8 x = fr[sl % (LEAD + 1)];
       const int j = sl - NR, ks = j / C::NDB, db = j % C::NDB;
-      if (ks == 0) {
+      if (NKS == 1 ? j == 0 : ks == 0) {  // the last block's (with one key step, before its products)
 #pragma unroll
-        for (int e = j * 2 * QB / C::NDB; e < (j + 1) * 2 * QB / C::NDB; ++e) soft(3, e);
+        for (int e = NKS == 1 ? 0 : j * 2 * QB / C::NDB; e < (NKS == 1 ? 2 * QB : (j + 1) * 2 * QB / C::NDB); ++e) soft(NKB - 1, e);
       }
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) dq[db][qb] = Mfma<T>::run(x, __builtin_bit_cast(v8, ds[ks][qb]), dq[db][qb]);
@@ -1278,7 +1273,7 @@ __global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dq_kernel(con
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kNW * 64, BwdCfg<D>::WPS) void window_dkv_kernel(const fmlm_attn_params p, const WinArgs a,
+__global__ __launch_bounds__(kNW * 64, 2) void window_dkv_kernel(const fmlm_attn_params p, const WinArgs a,
                                                                               const fmlm_attn_grads gr) {
   typedef BwdCfg<D> C;
   typedef typename Mfma<T>::v8 v8;
@@ -1466,7 +1461,7 @@ struct FwdLaunch {
   const void* fn;
   const void* merge[2];  // by one row a workgroup, by as many as it has threads for
   int merge_rows;        // ... that many
-  int bq, lds;
+  int bq, lds, lg;  // rows of a workgroup, its LDS, log2 of a tile's keys
 };
 template <typename T, int D>
 void merge_of(FwdLaunch& f) {
@@ -1481,6 +1476,7 @@ FwdLaunch fwd_of(bool fp4) {
   merge_of<T, D>(f);
   f.bq = kNW * QB * 16;
   f.lds = fp4 ? FwdCfg<D, true>::LDS : FwdCfg<D, false>::LDS;
+  f.lg = tile_keys(D) == 64 ? 6 : 5;
   return f;
 }
 template <typename T, int D>
@@ -1490,6 +1486,7 @@ FwdLaunch few_of() {
   merge_of<T, D>(f);
   f.bq = kFewRows;
   f.lds = FewCfg<D>::LDS;
+  f.lg = 6;
   return f;
 }
 template <typename T>
@@ -1572,10 +1569,11 @@ WinArgs win_args(const fmlm_attn_params& p, const fmlm_window& w, int rows) {
 // parts that key ranges are cut into at most, and a record's rows
 void plan_parts(const fmlm_attn_params& p, const fmlm_window& w, const FwdLaunch& f, WinArgs& a) {
   a.rec_rows = std::min(f.bq, longest(p));
+  a.lg = f.lg;
   const int64_t units = (int64_t)p.B * p.H * a.tiles;
   const int64_t fill = f.bq == kFewRows ? 4096 : a.rec_rows <= 64 ? 1024 : 512;
   if (p.lse || w.o_low || (p.flags & FMLM_FLAG_NOSPLIT) || units >= fill) return;
-  const int64_t tiles = max_keys(p, w, f.bq) / kBK + 2, want = (fill + units - 1) / units;
+  const int64_t tiles = (max_keys(p, w, f.bq) >> f.lg) + 2, want = (fill + units - 1) / units;
   a.parts = (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / kMinPartTiles, kMaxParts}));
 }
 

@@ -237,6 +237,12 @@ class AppendRows(ctypes.Structure):
     ] + [("scales", _c_ptr)]
 
 
+class Fp4Rows(ctypes.Structure):
+    """Mirror of fmlm_fp4_rows (include/flash_mlm_hip.h)."""
+
+    _fields_ = [("codes", _c_ptr), ("scales", _c_ptr), ("out", _c_ptr)]
+
+
 class AppendParams(ctypes.Structure):
     """Mirror of fmlm_append_params (include/flash_mlm_hip.h)."""
 
@@ -311,7 +317,7 @@ SIGNATURES = {
     ),
     "fmlm_append_params_size": (ctypes.c_int, []),
     "fmlm_rotate_append": (ctypes.c_int, [ctypes.POINTER(AppendParams), _c_ptr]),
-    "fmlm_fp4_values": (ctypes.c_int, [_c_i32, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i32, _c_ptr]),
+    "fmlm_fp4_values": (ctypes.c_int, [_c_i32, ctypes.POINTER(Fp4Rows), _c_i32, _c_i64, _c_i32, _c_ptr]),
 }
 
 _lock = threading.Lock()

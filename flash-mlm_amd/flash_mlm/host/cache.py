@@ -428,8 +428,7 @@ class InferenceCache:
             return entry.k_cache.view(shape), None if entry.v_cache is None else entry.v_cache.view(shape)
         from flash_mlm.host.paged import fp4_values
 
-        return (fp4_values(entry.k_cache, entry.k_scales, shape, entry.dtype),
-                fp4_values(entry.v_cache, entry.v_scales, shape, entry.dtype))
+        return fp4_values(entry, shape)
 
     def append_kv_cache(
         self,
@@ -588,7 +587,7 @@ class InferenceCache:
         rotated = None
         if cos is not None or entry.k_scales is not None:
             rotated = rotate_append(entry, q, k, v, q_meta=q_meta, slots=slots.contiguous(), cos=cos, sin=sin,
-                                    positions=plan.positions if positions is None else positions,
+                                    positions=None if cos is None else plan.positions if positions is None else positions,
                                     interleaved=interleaved)
         elif t > 0:
             paged_append(pairs, heads=h_kv, d=d, q_meta=q_meta, slots=slots.contiguous(),

@@ -176,15 +176,19 @@ def paged_append(pairs, *, heads: int, d: int, q_meta: PackMetadata, slots: torc
     _lib.check(rc, "fmlm_paged_append")
 
 
-def fp4_values(codes: torch.Tensor, scales: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tensor:
-    """The values of 4-bit rows as a new tensor (fmlm_fp4_values); the kernel of
+def fp4_values(entry, shape) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values of a 4-bit entry's pools as new tensors (fmlm_fp4_values); the kernel of
     :meth:`InferenceCache.paged_kv_values`."""
-    _require_device(codes, what="paged_kv_values")
-    out = torch.empty(shape, dtype=dtype, device=codes.device)
-    if out.numel():
-        with _device_scope(codes.device):
-            rc = _lib.load().fmlm_fp4_values(_lib.dtype_code(dtype), codes.data_ptr(), scales.data_ptr(), out.data_ptr(),
-                                             out.numel() // shape[-1], shape[-1], _lib.stream_of(codes.device))
+    dev = entry.device
+    _require_device(entry.k_cache, what="paged_kv_values")
+    out = torch.empty((2, *shape), dtype=entry.dtype, device=dev).unbind(0)
+    if entry.k_cache.numel():
+        rows = (_lib.Fp4Rows * 2)()
+        for r, codes, scales, x in zip(rows, (entry.k_cache, entry.v_cache), (entry.k_scales, entry.v_scales), out):
+            r.codes, r.scales, r.out = codes.data_ptr(), scales.data_ptr(), x.data_ptr()
+        with _device_scope(dev):
+            rc = _lib.load().fmlm_fp4_values(_lib.dtype_code(entry.dtype), rows, 2, int(entry.k_cache.shape[0]),
+                                             entry.head_dim, _lib.stream_of(dev))
         _lib.check(rc, "fmlm_fp4_values")
     return out
 
@@ -212,12 +216,55 @@ def _tables(cos, sin, positions, *, d: int, t: int, dev):
     return aligned16(cos), aligned16(sin), positions.contiguous()
 
 
+_MEMO_MAX = 16
+
+
+class _Append:
+    """The checked arguments of a rotating append as a parameter block, for calls laid out alike."""
+
+    __slots__ = ("block", "cu", "meta")
+
+
+def _put(p, entry, q, k, v, out, slots, cos, sin, positions) -> None:
+    """A block's addresses."""
+    p.slots = slots.data_ptr()
+    if cos is not None:
+        p.cos, p.sin, p.positions = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
+    if q is not None:
+        p.q.src, p.q.dst = q.data_ptr(), out.data_ptr()
+    if entry.k_cache.numel():
+        a, b = p.k, p.v
+        a.src, a.dst = k.data_ptr(), entry.k_cache.data_ptr()
+        b.src, b.dst = v.data_ptr(), entry.v_cache.data_ptr()
+        if entry.k_scales is not None:
+            a.scales, b.scales = entry.k_scales.data_ptr(), entry.v_scales.data_ptr()
+
+
+def _layout(x):
+    return None if x is None else (x.data_ptr() & 15, x.shape, x.stride(), x.dtype, x.device)
+
+
 def rotate_append(entry, q, k, v, *, q_meta: PackMetadata, slots, cos, sin, positions, interleaved: bool):
     """The rows of k and v, k rotated, to their slots of ``entry``'s pools, and q rotated, in one
     HIP launch (fmlm_rotate_append); the kernel of :meth:`InferenceCache.append_paged_kv_cache`
     for calls that rotate and for 4-bit contexts.  Returns the rotated q (None without)."""
     dev, d, h, t = entry.device, entry.head_dim, entry.num_heads, int(q_meta.total_tokens)
+    if q is not None:
+        refuse_tangents("append_paged_kv_cache", q)
+        if q.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the rotated q has no gradient; use qk_norm_rope, or call under torch.no_grad()")
+    # all that the checks below and the block depend on, but addresses (the caller has checked k, v and slots)
+    key = ("append", _layout(q), _layout(k), _layout(v), _layout(cos), _layout(sin), _layout(positions), interleaved,
+           entry.dtype, dev, h, d, entry.total_context_len, entry.k_scales is None)
+    memo = q_meta.launch_memo
+    m = memo.get(key)
+    if m is not None and m.cu is q_meta.cu_seqlens and m.meta == (q_meta.B, q_meta.N, t):
+        p = _lib.AppendParams.from_buffer_copy(m.block)
+        out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=dev)
+        _put(p, entry, q, k, v, out, slots, cos, sin, positions)
+        return _run_append(p, dev, out)
     _require_device(k, what="append_paged_kv_cache")
+    given = q, k, v, cos, sin, positions
     if cos is not None:
         cos, sin, positions = _tables(cos, sin, positions, d=d, t=t, dev=dev)
     packed = k.ndim == 2
@@ -227,9 +274,6 @@ def rotate_append(entry, q, k, v, *, q_meta: PackMetadata, slots, cos, sin, posi
             raise ValueError("q must be laid out like k")
         if q.dtype != entry.dtype or q.device != dev:
             raise ValueError("q dtype/device must match the cached entry")
-        refuse_tangents("append_paged_kv_cache", q)
-        if q.requires_grad and torch.is_grad_enabled():
-            raise ValueError("the rotated q has no gradient; use qk_norm_rope, or call under torch.no_grad()")
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     cu = pack_indices(q_meta, dev)[0]
     if k.numel() == 0:
@@ -246,26 +290,30 @@ def rotate_append(entry, q, k, v, *, q_meta: PackMetadata, slots, cos, sin, posi
     if p.B * p.N > 0x7FFFFFFF:
         raise ValueError("the call must have fewer than 2**31 tokens")
     p.pool_rows = int(entry.total_context_len)
-    p.cu_seqlens, p.slots = cu.data_ptr(), slots.data_ptr()
+    p.cu_seqlens = cu.data_ptr()
     if cos is not None:
-        p.cos, p.sin, p.positions = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
         p.rotary_dim, p.table_rows = 2 * int(cos.shape[1]), int(cos.shape[0])
-    keep = []
-    for a, src, dst, scales in ((p.q, q, out, None), (p.k, k, entry.k_cache, entry.k_scales),
-                                (p.v, v, entry.v_cache, entry.v_scales)):
-        if src is None or dst.numel() == 0:
-            continue
-        src = aligned16(src) if packed else rows16(src)
-        keep.append(src)
-        a.src, a.dst, a.scales = src.data_ptr(), dst.data_ptr(), _lib.ptr(scales)
+    as_read = aligned16 if packed else rows16
+    q, k, v = None if q is None else as_read(q), as_read(k), as_read(v)
+    for a, x in ((p.q, q), (p.k, k), (p.v, v)):
         if packed:
             a.s_sh, a.s_sn = t * d, d
-        else:
-            a.s_sb, a.s_sh, a.s_sn, _ = src.stride()
+        elif x is not None:
+            a.s_sb, a.s_sh, a.s_sn, _ = x.stride()
     if packed:
         p.q.d_sh, p.q.d_sn = t * d, d
     else:
         p.q.d_sb, p.q.d_sh, p.q.d_sn = h * p.N * d, p.N * d, d
+    if cu is q_meta.cu_seqlens and all(a is b for a, b in zip(given, (q, k, v, cos, sin, positions))):
+        if len(memo) >= _MEMO_MAX:
+            memo.clear()
+        m = memo[key] = _Append()
+        m.block, m.cu, m.meta = _lib.AppendParams.from_buffer_copy(p), cu, (q_meta.B, q_meta.N, t)
+    _put(p, entry, q, k, v, out, slots, cos, sin, positions)
+    return _run_append(p, dev, out)
+
+
+def _run_append(p, dev, out):
     with _device_scope(dev):
         rc = _lib.load().fmlm_rotate_append(p, _lib.stream_of(dev))
     _lib.check(rc, "fmlm_rotate_append")

@@ -38,7 +38,7 @@ def _limit(x, what: str) -> int:
 class _Call:
     """The checked arguments of a call as parameter blocks without the addresses of its own rows."""
 
-    __slots__ = ("params", "window", "nbytes", "out_shape", "entry_ref", "keep", "cu")
+    __slots__ = ("params", "window", "nbytes", "out_shape", "entry_ref", "keep", "cu", "strides", "grads")
 
     def run(self, q, k, v, lse=None, low=None):
         """One launch on rows laid out as the call's; returns the output.  ``lse`` and ``low`` take what
@@ -166,6 +166,15 @@ def _build(q, k, v, num_heads: int, q_meta: PackMetadata, scale, left, right, si
         p.k_sb, p.k_sh, p.k_sn = _strides(k_, t)
         p.v_sb, p.v_sh, p.v_sn = _strides(v_, t)
     call.out_shape = (num_heads * t, d)
+    if k is not None:  # of the backward: rows laid out like these, and contiguous gradients
+        call.strides = q_.stride(), k_.stride(), v_.stride()
+        g = call.grads = _lib.AttnGrads()
+        g.do_sh, g.do_sn = p.o_sh, p.o_sn
+        n = p.N * d
+        s3 = (num_heads * n, n, d) if q.ndim == 4 else (0, t * d, d)
+        g.dq_sb, g.dq_sh, g.dq_sn = s3
+        g.dk_sb, g.dk_sh, g.dk_sn = s3
+        g.dv_sb, g.dv_sh, g.dv_sn = s3
     call.entry_ref = None if entry is None else weakref.ref(entry)
     call.cu = q_meta.cu_seqlens
     call.keep = (cu, context)
@@ -196,29 +205,27 @@ class _Window(torch.autograd.Function):
     def backward(ctx, dout):
         call = ctx.call
         q, k, v, out, lse, low = ctx.saved_tensors
-        t = call.params.total_q
         if dout.shape != out.shape:
             raise ValueError("gradient of the attention output has the wrong shape")
-        q, k, v = (_rows(x) for x in (q, k, v))
-        out, lse, low, dout = (aligned16(x) for x in (out, lse, low, dout))
+        p = _lib.AttnParams.from_buffer_copy(call.params)
+        if (q.stride(), k.stride(), v.stride()) != call.strides or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+            q, k, v = _rows(q), _rows(k), _rows(v)  # (brought back by a hook, or copied by the forward too)
+            t = p.total_q
+            p.q_sb, p.q_sh, p.q_sn = _strides(q, t)
+            p.k_sb, p.k_sh, p.k_sn = _strides(k, t)
+            p.v_sb, p.v_sh, p.v_sn = _strides(v, t)
+        out, lse, low, dout = aligned16(out), aligned16(lse), aligned16(low), aligned16(dout)
+        dev = q.device
+        dq, dk, dv = (torch.empty(q.shape, dtype=q.dtype, device=dev) for _ in range(3))
+        ws = torch.empty_like(lse)
+        p.q, p.k, p.v, p.o, p.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr()
+        g = _lib.AttnGrads.from_buffer_copy(call.grads)
+        g.dout, g.dq, g.dk, g.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        g.workspace, g.workspace_bytes = ws.data_ptr(), 4 * ws.numel()
         w = _lib.Window.from_buffer_copy(call.window)
         w.o_low = low.data_ptr()
-        p = _lib.AttnParams.from_buffer_copy(call.params)
-        g = _lib.AttnGrads()
-        p.q, p.k, p.v, p.o, p.lse = (x.data_ptr() for x in (q, k, v, out, lse))
-        p.q_sb, p.q_sh, p.q_sn = _strides(q, t)
-        p.k_sb, p.k_sh, p.k_sn = _strides(k, t)
-        p.v_sb, p.v_sh, p.v_sn = _strides(v, t)
-        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-        g.dout, g.dq, g.dk, g.dv = (x.data_ptr() for x in (dout, dq, dk, dv))
-        g.do_sh, g.do_sn = p.o_sh, p.o_sn
-        g.dq_sb, g.dq_sh, g.dq_sn = _strides(dq, t)
-        g.dk_sb, g.dk_sh, g.dk_sn = _strides(dk, t)
-        g.dv_sb, g.dv_sh, g.dv_sn = _strides(dv, t)
-        ws = torch.empty(p.H * t, dtype=torch.float32, device=q.device)
-        g.workspace, g.workspace_bytes = ws.data_ptr(), 4 * ws.numel()
-        with _device_scope(q.device):
-            rc = _lib.load().fmlm_window_bwd(p, w, g, _lib.stream_of(q.device))
+        with _device_scope(dev):
+            rc = _lib.load().fmlm_window_bwd(p, w, g, _lib.stream_of(dev))
         _lib.check(rc, "fmlm_window_bwd")
         return None, dq, dk, dv
 
@@ -292,7 +299,7 @@ def flash_attn_mlm_window(
             # the entry's tensors are held by the entry alone, as in the other memos
             stored = _Call()
             for name in _Call.__slots__:
-                setattr(stored, name, getattr(call, name))
+                setattr(stored, name, getattr(call, name, None))
             stored.keep = None
             q_meta.launch_memo[key] = stored
     if grad:

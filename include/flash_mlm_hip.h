@@ -593,9 +593,16 @@ typedef struct fmlm_append_params {
 FMLM_API int fmlm_append_params_size(void);
 FMLM_API int fmlm_rotate_append(const fmlm_append_params* p, void* stream);
 
-/* The values of `rows` 4-bit rows of D elements (contiguous codes and scales), as bf16 or fp16. */
-FMLM_API int fmlm_fp4_values(int32_t dtype, const uint8_t* codes, const uint8_t* scales, void* out, int64_t rows,
-                             int32_t D, void* stream);
+/* The values of `rows` 4-bit rows of D elements (contiguous codes and scales) of one or two tensors,
+ * as bf16 or fp16. */
+typedef struct fmlm_fp4_rows {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  void* out;
+} fmlm_fp4_rows;
+
+FMLM_API int fmlm_fp4_values(int32_t dtype, const fmlm_fp4_rows* tensors, int32_t n_tensors, int64_t rows, int32_t D,
+                             void* stream);
 
 #ifdef __cplusplus
 }

@@ -258,12 +258,15 @@ def test_argument_rejection_without_launch():
     p.B = p.N = 1 << 17
     p.flags = 0
     assert lib.fmlm_rotate_append(p, None) == -1  # too many rows
-    assert lib.fmlm_fp4_values(2, 256, 256, 256, 1, 64, None) == -2
-    assert lib.fmlm_fp4_values(0, 256, 256, 256, 1, 48, None) == -3
-    assert lib.fmlm_fp4_values(0, 256, 256, 256, -1, 64, None) == -1
-    assert lib.fmlm_fp4_values(0, None, 256, 256, 1, 64, None) == -1
-    assert lib.fmlm_fp4_values(0, 256, 256, 264, 1, 64, None) == -4
-    assert lib.fmlm_fp4_values(0, None, None, None, 0, 64, None) == 0
+    r = (_lib.Fp4Rows * 2)()
+    values = lambda dtype=0, n=1, rows=1, D=64: lib.fmlm_fp4_values(dtype, r, n, rows, D, None)  # noqa: E731
+    assert values(dtype=2) == -2 and values(D=48) == -3 and values(rows=-1) == -1 and values(n=3) == -1
+    assert values() == -1 and values(rows=0) == 0
+    r[0].codes = r[0].scales = r[0].out = 256
+    assert values(n=2) == -1
+    r[0].out = 264
+    assert values() == -4
+    assert lib.fmlm_fp4_values(0, None, 1, 1, 64, None) == -1
 
 
 # ---------------------------------------------------------------------------
