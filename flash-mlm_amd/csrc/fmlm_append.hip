@@ -26,7 +26,11 @@
 namespace fmlm {
 
 constexpr int kRaThreads = 256;
-constexpr int kRaHeads = 4;  // heads per thread, all their loads in flight
+constexpr int kRaHeads = 4;  // heads of a thread whose loads are in flight
+
+constexpr int kRaHeads4 = 2;  // ... of the 4-bit kernel, whose 64-bit rotation takes registers
+constexpr int kRaMany = 16;
+constexpr int64_t kRaManyThreads = 256 * 2048 / 3;  // threads of one of q, k, v that fill their share of the GPU
 
 typedef fmlm_append_params RaParams;
 
@@ -61,10 +65,17 @@ FMLM_DEV float round_to_odd(double x) {
   return __builtin_bit_cast(float, u);
 }
 
-// x of the lanes whose number differs in bit 0 / bit 1
+// the larger of x and x of the lane whose number differs in bit 0 / bit 1 (NaN if either is)
 template <int CTRL>
-FMLM_DEV uint32_t quad_max(uint32_t x) {
-  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true));
+FMLM_DEV float quad_max(float x) {
+  const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true);
+  return vmax(x, __builtin_bit_cast(float, y));
+}
+FMLM_DEV float block_max(const float (&x)[8]) {
+  float a = fabsf(x[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) a = vmax(a, fabsf(x[i]));
+  return quad_max<0x4E>(quad_max<0xB1>(a));
 }
 
 // the codes of 8 values, a quarter of their block, whose other quarters the three lanes beside hold
@@ -73,15 +84,15 @@ FMLM_DEV uint32_t fp4_encode(float (&x)[8], uint32_t& scale_byte) {
   constexpr bool BF = std::is_same<T, bf16>::value;
   constexpr float top = BF ? 0x1.fep127f : 65504.f;
   constexpr int lo = BF ? -125 : -23, hi = BF ? 125 : 13;
-  uint32_t a = 0;
+  float a = block_max(x);
+  if (__builtin_amdgcn_ballot_w64(!(a <= top))) {  // an infinity, NaN or a rotated value past the type's
+    asm volatile("");  // (a real branch)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = x[i] == x[i] ? fminf(fmaxf(x[i], -top), top) : 0.f;
-    a = max(a, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
+    for (int i = 0; i < 8; ++i) x[i] = x[i] == x[i] ? fminf(fmaxf(x[i], -top), top) : 0.f;
+    a = block_max(x);
   }
-  a = quad_max<0xB1>(a);
-  a = quad_max<0x4E>(a);
-  int e = (int)(a >> 23) - 127 - ((a & 0x7fffffu) < 0x600000u ? 2 : 1);
+  const uint32_t u = __builtin_bit_cast(uint32_t, a);
+  int e = (int)(u >> 23) - 127 - ((u & 0x7fffffu) < 0x600000u ? 2 : 1);
   e = min(max(e, lo), hi);
   scale_byte = (uint32_t)(e + 127);
   const float s = fp4_scale(scale_byte);
@@ -93,9 +104,10 @@ FMLM_DEV uint32_t fp4_encode(float (&x)[8], uint32_t& scale_byte) {
   return c;
 }
 
-// blockIdx.y: chunk of heads, z: q, k, v.  Rows: padded ones b * N + pos, or packed tokens
+// blockIdx.y: chunk of `heads` heads, z: q, k, v.  Rows: padded ones b * N + pos, or packed tokens
 template <typename T, bool FP4>
-__global__ __launch_bounds__(kRaThreads) void rotate_append_kernel(const RaParams p, int lpr_log2) {
+__global__ __launch_bounds__(kRaThreads) void rotate_append_kernel(const RaParams p, int lpr_log2, int heads) {
+  constexpr int NH = FP4 ? kRaHeads4 : kRaHeads;
   const int which = blockIdx.z;
   const fmlm_append_rows& a = which == 0 ? p.q : which == 1 ? p.k : p.v;
   if (!a.dst) return;
@@ -114,11 +126,12 @@ __global__ __launch_bounds__(kRaThreads) void rotate_append_kernel(const RaParam
     src = (int64_t)b * a.s_sb + (int64_t)pos * a.s_sn;
     dst = (int64_t)b * a.d_sb + (int64_t)pos * a.d_sn;
   }
-  const int h0 = blockIdx.y * kRaHeads, nh = min(kRaHeads, p.H - h0);
+  int h0 = blockIdx.y * heads;
+  const int h1 = min(h0 + heads, p.H);
   T* const out = (T*)a.dst + dst + d;
   if (!real) {
     if (which == 0)
-      for (int u = 0; u < nh; ++u) *(u32x4*)(out + (h0 + u) * a.d_sh) = u32x4{0u, 0u, 0u, 0u};
+      for (int h = h0; h < h1; ++h) *(u32x4*)(out + h * a.d_sh) = u32x4{0u, 0u, 0u, 0u};
     return;
   }
   int64_t slot = 0;
@@ -131,10 +144,13 @@ __global__ __launch_bounds__(kRaThreads) void rotate_append_kernel(const RaParam
   // half-split: the lane of the row that holds the partners (every lane of a row has come this far)
   const int from = (threadIdx.x & 63) + (!turn ? 0 : d < half ? half / 8 : -half / 8);
   const T* in = (const T*)a.src + src + d;
-  u32x4 x[kRaHeads];
+  u32x4 x[NH];
+  auto load = [&](int h) {
 #pragma unroll
-  for (int u = 0; u < kRaHeads; ++u)
-    if (u < nh) x[u] = *(const u32x4*)(in + (h0 + u) * a.s_sh);
+    for (int u = 0; u < NH; ++u)
+      if (h + u < h1) x[u] = *(const u32x4*)(in + (h + u) * a.s_sh);
+  };
+  load(h0);
   float cs[8], sn[8];  // sn with the pair member's sign: element j becomes x_j cs_j + partner_j sn_j
   if (turn) {
     int64_t s = p.flags & FMLM_AP_POSITIONS_I64 ? ((const int64_t*)p.positions)[t] : ((const int32_t*)p.positions)[t];
@@ -159,18 +175,23 @@ __global__ __launch_bounds__(kRaThreads) void rotate_append_kernel(const RaParam
       }
     }
   }
+  for (; h0 < h1; h0 += NH) {
+  u32x4 cur[NH];
 #pragma unroll
-  for (int u = 0; u < kRaHeads; ++u) {
-    if (u >= nh) break;
+  for (int u = 0; u < NH; ++u) cur[u] = x[u];
+  if (h0 + NH < h1) load(h0 + NH);
+#pragma unroll
+  for (int u = 0; u < NH; ++u) {
+    if (h0 + u >= h1) break;
     float f[8], g[8];
-    oct_of<T>(x[u], f);
+    oct_of<T>(cur[u], f);
     if (pairs) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) g[j] = f[j ^ 1];
     } else if (which < 2 && p.rotary_dim > 0) {  // (the same in a wave: every lane gives its own)
       u32x4 y;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * from, (int)x[u][j]);
+      for (int j = 0; j < 4; ++j) y[j] = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * from, (int)cur[u][j]);
       oct_of<T>(y, g);
     }
     if (FP4 && which > 0) {
@@ -184,7 +205,7 @@ __global__ __launch_bounds__(kRaThreads) void rotate_append_kernel(const RaParam
       *(uint32_t*)((char*)a.dst + e / 2) = c;
       if (d % kFp4Block == 0) a.scales[e / kFp4Block] = (uint8_t)sb;
     } else {
-      u32x4 v = x[u];
+      u32x4 v = cur[u];
       if (turn) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = fmaf(f[j], cs[j], g[j] * sn[j]);
@@ -194,7 +215,7 @@ __global__ __launch_bounds__(kRaThreads) void rotate_append_kernel(const RaParam
                                : (T*)a.dst + ((int64_t)(h0 + u) * p.pool_rows + slot) * p.D + d;
       *(u32x4*)to = v;
     }
-  }
+  }  }
 }
 
 // 8 values a thread and step; blockIdx.y: pool
@@ -269,15 +290,19 @@ extern "C" int fmlm_rotate_append(const fmlm_append_params* pp, void* stream) {
   const int lpr = p.D / 8, lpr_log2 = __builtin_ctz(lpr);
   const int64_t blocks = (rows * lpr + kRaThreads - 1) / kRaThreads;
   if (blocks > 0x7fffffff) return FMLM_E_ARG;
-  const dim3 grid((unsigned)blocks, (p.H + kRaHeads - 1) / kRaHeads, 3);
+  // Many rows: the angles, the slot and the sequence of a row serve kRaMany heads (fp16, 20 thousand rows of 16
+  // heads, D = 128: 130 us with 4 heads a thread, 116 with 16); few: all the threads there are (64
+  // rows of 16 heads 5.1 us, with 16 heads a thread 8.5)
+  const int heads = rows * lpr >= kRaManyThreads ? kRaMany : kRaHeads;
+  const dim3 grid((unsigned)blocks, (p.H + heads - 1) / heads, 3);
   hipStream_t s = (hipStream_t)stream;
   const bool fp4 = p.flags & FMLM_AP_FP4;
   if (p.dtype == FMLM_DTYPE_BF16) {
-    if (fp4) hipLaunchKernelGGL((rotate_append_kernel<bf16, true>), grid, dim3(kRaThreads), 0, s, p, lpr_log2);
-    else hipLaunchKernelGGL((rotate_append_kernel<bf16, false>), grid, dim3(kRaThreads), 0, s, p, lpr_log2);
+    if (fp4) hipLaunchKernelGGL((rotate_append_kernel<bf16, true>), grid, dim3(kRaThreads), 0, s, p, lpr_log2, heads);
+    else hipLaunchKernelGGL((rotate_append_kernel<bf16, false>), grid, dim3(kRaThreads), 0, s, p, lpr_log2, heads);
   } else {
-    if (fp4) hipLaunchKernelGGL((rotate_append_kernel<f16, true>), grid, dim3(kRaThreads), 0, s, p, lpr_log2);
-    else hipLaunchKernelGGL((rotate_append_kernel<f16, false>), grid, dim3(kRaThreads), 0, s, p, lpr_log2);
+    if (fp4) hipLaunchKernelGGL((rotate_append_kernel<f16, true>), grid, dim3(kRaThreads), 0, s, p, lpr_log2, heads);
+    else hipLaunchKernelGGL((rotate_append_kernel<f16, false>), grid, dim3(kRaThreads), 0, s, p, lpr_log2, heads);
   }
   return launch_status();
 }
