@@ -16,6 +16,7 @@
 #include "fmlm_common.h"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "fmlm_fp4.h"
@@ -1434,11 +1435,18 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dkv_kernel(const fmlm_attn
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-// a kernel's LDS beyond 64 KB has to be allowed once a device
-int allow_lds(const void* fn, int bytes) {
+// A kernel's LDS beyond 64 KB has to be allowed, once a device (2 us a call); `done`: the devices where it is
+int allow_lds(const void* fn, int bytes, std::atomic<uint64_t>& done) {
   if (bytes <= 65536) return 0;
-  hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  return e == hipSuccess ? 0 : (int)e;
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return (int)e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return 0;
+  e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return (int)e;
+  if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
 }
 
 int longest(const fmlm_attn_params& p) { return p.N > 0 && p.N < p.total_q ? p.N : p.total_q; }
@@ -1461,6 +1469,7 @@ struct FwdLaunch {
   const void* fn;
   const void* merge[2];  // by one row a workgroup, by as many as it has threads for
   int merge_rows;        // ... that many
+  std::atomic<uint64_t>* allowed;
   int bq, lds, lg;  // rows of a workgroup, its LDS, log2 of a tile's keys
 };
 template <typename T, int D>
@@ -1471,7 +1480,9 @@ void merge_of(FwdLaunch& f) {
 }
 template <typename T, int D, int QB>
 FwdLaunch fwd_of(bool fp4) {
+  static std::atomic<uint64_t> allowed[2];
   FwdLaunch f;
+  f.allowed = &allowed[fp4];
   f.fn = fp4 ? (const void*)window_fwd_kernel<T, D, QB, true> : (const void*)window_fwd_kernel<T, D, QB, false>;
   merge_of<T, D>(f);
   f.bq = kNW * QB * 16;
@@ -1481,7 +1492,9 @@ FwdLaunch fwd_of(bool fp4) {
 }
 template <typename T, int D>
 FwdLaunch few_of() {
+  static std::atomic<uint64_t> allowed;
   FwdLaunch f;
+  f.allowed = &allowed;
   f.fn = (const void*)window_fp4_few_kernel<T, D>;
   merge_of<T, D>(f);
   f.bq = kFewRows;
@@ -1590,8 +1603,9 @@ int launch_bwd(const fmlm_attn_params& p, const fmlm_window& w, const fmlm_attn_
   if (p.N > 0 && p.kv_layout == FMLM_LAYOUT_PADDED) b.tiles = (p.N + kBK - 1) / kBK;
   if ((int64_t)a.tiles * a.groups > 0x7fffffff || (int64_t)b.tiles * b.groups > 0x7fffffff) return FMLM_E_ARG;
   const void *dq = (const void*)window_dq_kernel<T, D>, *dkv = (const void*)window_dkv_kernel<T, D>;
-  int rc = allow_lds(dq, C::DQ_LDS);
-  if (!rc) rc = allow_lds(dkv, C::DKV_LDS);
+  static std::atomic<uint64_t> allowed[2];
+  int rc = allow_lds(dq, C::DQ_LDS, allowed[0]);
+  if (!rc) rc = allow_lds(dkv, C::DKV_LDS, allowed[1]);
   if (rc) return rc;
   hipLaunchKernelGGL((window_dq_kernel<T, D>), dim3((unsigned)(a.tiles * a.groups)), dim3(kNW * 64), C::DQ_LDS, s, p, a, g);
   hipLaunchKernelGGL((window_dkv_kernel<T, D>), dim3((unsigned)(b.tiles * b.groups)), dim3(kNW * 64), C::DKV_LDS, s, p, b, g);
@@ -1640,7 +1654,7 @@ extern "C" int fmlm_window_fwd(const fmlm_attn_params* pp, const fmlm_window* ww
   if (blocks > 0x7fffffff) return FMLM_E_ARG;
   a.records = (float*)p.workspace;
   p.flags = p.cu_seqlens_kv ? 0 : FMLM_FLAG_PREFILL;  // (without a context)
-  rc = allow_lds(f.fn, f.lds);
+  rc = allow_lds(f.fn, f.lds, *f.allowed);
   if (rc) return rc;
   hipStream_t s = (hipStream_t)stream;
   void* args[2] = {&p, &a};

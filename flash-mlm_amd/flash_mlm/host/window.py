@@ -169,7 +169,7 @@ def _build(q, k, v, num_heads: int, q_meta: PackMetadata, scale, left, right, si
     if k is not None:  # of the backward: rows laid out like these, and contiguous gradients
         call.strides = q_.stride(), k_.stride(), v_.stride()
         g = call.grads = _lib.AttnGrads()
-        g.do_sh, g.do_sn = p.o_sh, p.o_sn
+        g.do_sh, g.do_sn, g.workspace_bytes = p.o_sh, p.o_sn, 4 * num_heads * t
         n = p.N * d
         s3 = (num_heads * n, n, d) if q.ndim == 4 else (0, t * d, d)
         g.dq_sb, g.dq_sh, g.dq_sn = s3
@@ -191,43 +191,55 @@ def _build(q, k, v, num_heads: int, q_meta: PackMetadata, scale, left, right, si
 class _Window(torch.autograd.Function):
     @staticmethod
     def forward(ctx, call, q, k, v):
-        rows = _rows(q), _rows(k), _rows(v)
-        lse = torch.empty(call.params.H * call.params.total_q, dtype=torch.float32, device=q.device)
+        p = call.params
+        lse = torch.empty(p.H * p.total_q, dtype=torch.float32, device=q.device)
         low = torch.empty(call.out_shape, dtype=q.dtype, device=q.device)
-        out = call.run(*rows, lse=lse, low=low)
+        out = call.run(_rows(q), _rows(k), _rows(v), lse, low)
         ctx.call = call
         # read from there in the backward: autograd may free these and bring others
         ctx.save_for_backward(q, k, v, out, lse, low)
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        call = ctx.call
-        q, k, v, out, lse, low = ctx.saved_tensors
-        if dout.shape != out.shape:
-            raise ValueError("gradient of the attention output has the wrong shape")
-        p = _lib.AttnParams.from_buffer_copy(call.params)
-        if (q.stride(), k.stride(), v.stride()) != call.strides or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
-            q, k, v = _rows(q), _rows(k), _rows(v)  # (brought back by a hook, or copied by the forward too)
-            t = p.total_q
-            p.q_sb, p.q_sh, p.q_sn = _strides(q, t)
-            p.k_sb, p.k_sh, p.k_sn = _strides(k, t)
-            p.v_sb, p.v_sh, p.v_sn = _strides(v, t)
-        out, lse, low, dout = aligned16(out), aligned16(lse), aligned16(low), aligned16(dout)
-        dev = q.device
-        dq, dk, dv = (torch.empty(q.shape, dtype=q.dtype, device=dev) for _ in range(3))
-        ws = torch.empty_like(lse)
-        p.q, p.k, p.v, p.o, p.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr()
-        g = _lib.AttnGrads.from_buffer_copy(call.grads)
-        g.dout, g.dq, g.dk, g.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        g.workspace, g.workspace_bytes = ws.data_ptr(), 4 * ws.numel()
-        w = _lib.Window.from_buffer_copy(call.window)
-        w.o_low = low.data_ptr()
-        with _device_scope(dev):
-            rc = _lib.load().fmlm_window_bwd(p, w, g, _lib.stream_of(dev))
+        # grad mode: create_graph, where the gradients must refuse to be differentiated (the wrapper's
+        # grad-mode switches cost 4 us)
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dout)
+
+
+def _backward(ctx, dout):
+    call = ctx.call
+    q, k, v, out, lse, low = ctx.saved_tensors
+    if dout.shape != out.shape:
+        raise ValueError("gradient of the attention output has the wrong shape")
+    p = _lib.AttnParams.from_buffer_copy(call.params)
+    p.q, p.k, p.v = ptrs = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if (q.stride(), k.stride(), v.stride()) != call.strides or (ptrs[0] | ptrs[1] | ptrs[2]) & 15:
+        q, k, v = _rows(q), _rows(k), _rows(v)  # (brought back by a hook, or copied by the forward too)
+        t = p.total_q
+        p.q, p.k, p.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        p.q_sb, p.q_sh, p.q_sn = _strides(q, t)
+        p.k_sb, p.k_sh, p.k_sn = _strides(k, t)
+        p.v_sb, p.v_sh, p.v_sn = _strides(v, t)
+    out, lse, low, dout = aligned16(out), aligned16(lse), aligned16(low), aligned16(dout)
+    shape, dtype, dev = q.shape, q.dtype, q.device
+    dq = torch.empty(shape, dtype=dtype, device=dev)
+    dk = torch.empty(shape, dtype=dtype, device=dev)
+    dv = torch.empty(shape, dtype=dtype, device=dev)
+    ws = torch.empty_like(lse)
+    p.o, p.lse = out.data_ptr(), lse.data_ptr()
+    g = _lib.AttnGrads.from_buffer_copy(call.grads)
+    g.dout, g.dq, g.dk, g.dv, g.workspace = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr()
+    w = _lib.Window.from_buffer_copy(call.window)
+    w.o_low = low.data_ptr()
+    with _device_scope(dev):
+        rc = _lib.load().fmlm_window_bwd(p, w, g, _lib.stream_of(dev))
+    if rc:
         _lib.check(rc, "fmlm_window_bwd")
-        return None, dq, dk, dv
+    return None, dq, dk, dv
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def flash_attn_mlm_window(
@@ -270,7 +282,8 @@ def flash_attn_mlm_window(
     """
     entry = _entry_of(inference_cache, layer_id)
     refuse_tangents("flash_attn_mlm_window", q, k, v)
-    grad = torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v))
+    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)
+                                        or (v is not None and v.requires_grad))
     call = key = None
     if context_index is None and isinstance(window, tuple):
         # all that the checks depend on
