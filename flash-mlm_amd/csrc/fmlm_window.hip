@@ -98,6 +98,26 @@ FMLM_DEV void win_unit(const WinArgs& a, int parts, int& g, int& part, int& tile
   part = (int)(r - (uint32_t)tile * (uint32_t)parts);
 }
 
+// ---- which of a lane's elements are in view, as bits: element (block b, r) is bit 16 b + r, b < 4, r < 4.
+// A conditional per element becomes a branch each (three compares, two saves of exec); a bit spread
+// over a word and one bitwise select are two instructions and serve both edges and the sinks alike.
+struct InView {
+  int w[2];
+  InView() = default;
+  // elements [low, top], and [0, sinks) up to top
+  FMLM_DEV InView(int low, int top, int sinks) {
+    const uint64_t x = ~from(top + 1) & (from(low) | ~from(sinks));
+    w[0] = (int)x;
+    w[1] = (int)(x >> 32);
+  }
+  FMLM_DEV static uint64_t from(int n) { return ~0ull << min(max(n, 0), 63); }  // (bit 63 is no element)
+  FMLM_DEV float pick(int b, int r, float x, float none) const {
+    int keep = __builtin_amdgcn_sbfe(w[b >> 1], (b & 1) * 16 + r, 1);
+    asm("" : "+v"(keep));  // (else a compare and two selects)
+    return __int_as_float((__float_as_int(x) & keep) | (__float_as_int(none) & ~keep));
+  }
+};
+
 // ---- a 64-row (or 32-row) tile of D 16-bit elements in LDS, 16-byte chunks swizzled by kv_swz
 template <typename T, int D>
 struct WTile {
@@ -376,14 +396,11 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       const int pos = w0 + qb * 16 + l16, k0 = kp + 4 * gq;  // element (kb, r) is key k0 + 16 kb + r
-      const int top = min(pos + a.right - k0, nk - 1 - 4 * gq), low = pos - a.left - k0, snk = a.sinks - k0;
+      const InView view(pos - a.left - k0, min(pos + a.right - k0, nk - 1 - 4 * gq), a.sinks - k0);
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int j = kb * 16 + r;
-          if (!(j <= top && (j >= low || j < snk))) x[kb][qb][r] = -INFINITY;
-        }
+        for (int r = 0; r < 4; ++r) x[kb][qb][r] = view.pick(kb, r, x[kb][qb][r], -INFINITY);
     }
     return true;
   };
@@ -813,14 +830,11 @@ __global__ __launch_bounds__(kNW * 64, FewCfg<D>::WPS) void window_fp4_few_kerne
     edge = nk < kBK || kp + kBK - 1 > s.first + a.right || (kp < s.first + rows - 1 - a.left && kp + kBK > a.sinks);
     if (edge) {
       const int pos = s.first + l16, k0 = kp + 4 * gq;
-      const int top = min(pos + a.right - k0, nk - 1 - 4 * gq), low = pos - a.left - k0, snk = a.sinks - k0;
+      const InView view(pos - a.left - k0, min(pos + a.right - k0, nk - 1 - 4 * gq), a.sinks - k0);
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int j = kb * 16 + r;
-          if (!(j <= top && (j >= low || j < snk))) sc[kb][r] = -INFINITY;
-        }
+        for (int r = 0; r < 4; ++r) sc[kb][r] = view.pick(kb, r, sc[kb][r], -INFINITY);
     }
     float mx = vmax(vmax(sc[0][0], sc[0][1]), vmax(sc[0][2], sc[0][3]));
 #pragma unroll
@@ -1220,14 +1234,11 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         const int pos = w0 + qb * 16 + l16, k0 = kp + 4 * gq;
-        const int top = min(pos + a.right - k0, nk - 1 - 4 * gq), low = pos - a.left - k0, snk = a.sinks - k0;
+        const InView view(pos - a.left - k0, min(pos + a.right - k0, nk - 1 - 4 * gq), a.sinks - k0);
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = kb * 16 + r;
-            if (!(j <= top && (j >= low || j < snk))) sc[kb][qb][r] = none;
-          }
+          for (int r = 0; r < 4; ++r) sc[kb][qb][r] = view.pick(kb, r, sc[kb][qb][r], none);
       }
     }
 #pragma unroll
@@ -1349,8 +1360,11 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dkv_kernel(const fmlm_attn
     if (i + 1 < steps) issue(i + 1);
     const int k0 = j0 + wave * 16, k1 = k0 + 15;
     const bool edge = k1 >= s.len || k1 > p0 + a.right || (k0 < p0 + QS - 1 - a.left && k1 >= a.sinks);
-    // rows pos with lo <= pos <= hi see the lane's key
-    const int lo = key - a.right - p0, hi = !kok ? -1 : key < a.sinks ? QS : key + a.left - p0;
+    InView view;  // of the lane's key: rows key - right to key + left
+    if (edge) {
+      asm volatile("");  // (a real branch)
+      view = InView(key - a.right - p0 - 4 * gq, (!kok ? -1 : key < a.sinks ? QS : key + a.left - p0) - 4 * gq, 0);
+    }
     // ---- fenced slots as in the dq kernel: per block of 16 rows its S and dP (fragments of q and do in turn),
     // the block before's P and dS beside them; then per 32 rows dV^T and dK^T
     constexpr int RBS = 2 * C::KC, NR = NRB * RBS, NCS = 2 * C::NDB, NS = NR + NRB / 2 * NCS, LEAD = 3;
@@ -1368,10 +1382,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dkv_kernel(const fmlm_attn
       if (edge) {
         asm volatile("");  // (a real branch)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int pos = rb * 16 + gq * 4 + r;
-          if (!(pos >= lo && pos <= hi)) sc[rb][r] = none;
-        }
+        for (int r = 0; r < 4; ++r) sc[rb][r] = view.pick(rb, r, sc[rb][r], none);
       }
     };
     // elements 2 e, 2 e + 1 of block rb
