@@ -389,9 +389,15 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
     }
   };
   const int w0 = s.first + row0 + wave * QB * 16, w1 = min(w0 + QB * 16, s.first + row0 + rows) - 1;
+  // position of a tile's first key; whether any of the wave's rows sees a key of it
+  auto key_at = [&](int t) { return t < wt.nt0 ? t * BK : s.ctx + (t - wt.nt0) * BK; };
+  auto seen = [&](int t) {
+    const int kp = key_at(t);
+    return kp <= w1 + a.right && (kp + BK > w0 - a.left || kp < a.sinks);
+  };
   // scores of keys that a row does not see to -inf; returns whether there can be any
   auto mask = [&](int t, f32x4 (&x)[NKB][QB]) {
-    const int nk = keys_in(t), kp = t < wt.nt0 ? t * BK : s.ctx + (t - wt.nt0) * BK;
+    const int nk = keys_in(t), kp = key_at(t);
     if (!(nk < BK || kp + BK - 1 > w0 + a.right || (kp < w1 - a.left && kp + BK > a.sinks))) return false;
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
@@ -505,7 +511,13 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
         move();
       }
     }
-    if (active) {
+    // A wave that sees neither tile leaves the matrix cores and LDS to the others; the scores that it has
+    // then not made are all masked when one of the two tiles is in view.  With 128-row tiles a window of
+    // 1024 keys takes 176 us with this and 180 without; with 64-row ones, whose waves differ by less
+    // than a tile, 72 without and 74 with it, with 4 bits (no window) 93 and 95.
+    bool look = active;
+    if constexpr (QB == 2 && !FP4) look = active && (seen(tile_at(v)) || (v + 1 < n && seen(tile_at(v + 1))));
+    if (look) {
       if (mask(tile_at(v), sc)) row_max(sc);
       bool grow = false;
 #pragma unroll
@@ -1191,7 +1203,8 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (v + 1 < wt.n) issue(v + 1);
-    if (!active) continue;
+    const int kp = t * BK, w0 = row0 + wave * QB * 16, w1 = min(w0 + QB * 16, row0 + rows) - 1;
+    if (!active || kp > w1 + a.right || (kp + BK <= w0 - a.left && kp >= a.sinks)) continue;  // none in view
     const char *kt = kbuf(buf), *vt = vbuf(buf);
     // ---- fenced slots, each the MFMAs of one LDS fragment: NSS of S^T (step kc, key block kb), NSS of
     // dP^T (block by block), 2 NDB of dq^T; the fragment of slot s + LEAD is read at slot s.  Block
@@ -1227,7 +1240,6 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
         sc[kb][qb] = Mfma<T>::run(x, qf[qb][kc], kc == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[kb][qb]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    const int kp = t * BK, w0 = row0 + wave * QB * 16, w1 = min(w0 + QB * 16, row0 + rows) - 1;
     if (nk < BK || kp + BK - 1 > w0 + a.right || (kp < w1 - a.left && kp + BK > a.sinks)) {
       asm volatile("");  // (a real branch.)  What a row does not see: P = 0
       const float none = c < 0.f ? INFINITY : -INFINITY;
@@ -1359,6 +1371,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dkv_kernel(const fmlm_attn
     __syncthreads();
     if (i + 1 < steps) issue(i + 1);
     const int k0 = j0 + wave * 16, k1 = k0 + 15;
+    if (k0 >= s.len || k0 >= p0 + QS + a.right || (k1 < p0 - a.left && k0 >= a.sinks)) continue;  // none in view
     const bool edge = k1 >= s.len || k1 > p0 + a.right || (k0 < p0 + QS - 1 - a.left && k1 >= a.sinks);
     InView view;  // of the lane's key: rows key - right to key + left
     if (edge) {
@@ -1474,7 +1487,7 @@ int64_t max_keys(const fmlm_attn_params& p, const fmlm_window& w, int rows) {
   return std::min(keys, (int64_t)limit(w.left) + limit(w.right) + std::max(w.sinks, 0) + rows);
 }
 
-constexpr int kWideTiles = 12;
+constexpr int kWideTiles = 9;
 
 struct FwdLaunch {
   const void* fn;
@@ -1525,8 +1538,8 @@ FwdLaunch pick_fwd(const fmlm_attn_params& p, const fmlm_window& w) {
     }
   }
   // 128 rows that share a tile's loads, from walks of kWideTiles tiles on; below, more and smaller
-  // workgroups (kernel us, 64 against 128 rows: walks of 4-5 tiles, D = 64, 31 : 44; of 12, D = 128,
-  // 79 : 81; of 20, 210 : 174; of 50 in 4 bits 139 : 96)
+  // workgroups (kernel us, 64 against 128 rows: walks of 4-5 tiles, D = 64, 31 : 44; of 10, D = 128,
+  // 72 : 69; of 20, 210 : 174; of 50 in 4 bits 139 : 96)
   const bool wide = longest(p) > 64 && max_keys(p, w, 128) > kWideTiles * kBK;
   switch (p.D) {
     case 32: return wide ? fwd_of<T, 32, 2>(fp4) : fwd_of<T, 32, 1>(fp4);
