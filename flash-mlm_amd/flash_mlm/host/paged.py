@@ -241,7 +241,11 @@ def _put(p, entry, q, k, v, out, slots, cos, sin, positions) -> None:
 
 
 def _layout(x):
-    return None if x is None else (x.data_ptr() & 15, x.shape, x.stride(), x.dtype, x.device)
+    if x is None:
+        return None
+    if not isinstance(x, torch.Tensor):
+        raise ValueError("q, cos, sin and positions must be tensors")
+    return x.data_ptr() & 15, x.shape, x.stride(), x.dtype, x.device
 
 
 def rotate_append(entry, q, k, v, *, q_meta: PackMetadata, slots, cos, sin, positions, interleaved: bool):
@@ -249,13 +253,13 @@ def rotate_append(entry, q, k, v, *, q_meta: PackMetadata, slots, cos, sin, posi
     HIP launch (fmlm_rotate_append); the kernel of :meth:`InferenceCache.append_paged_kv_cache`
     for calls that rotate and for 4-bit contexts.  Returns the rotated q (None without)."""
     dev, d, h, t = entry.device, entry.head_dim, entry.num_heads, int(q_meta.total_tokens)
+    # all that the checks below and the block depend on, but addresses (the caller has checked k, v and slots)
+    key = ("append", _layout(q), _layout(k), _layout(v), _layout(cos), _layout(sin), _layout(positions), interleaved,
+           entry.dtype, dev, h, d, entry.total_context_len, entry.k_scales is None)
     if q is not None:
         refuse_tangents("append_paged_kv_cache", q)
         if q.requires_grad and torch.is_grad_enabled():
             raise ValueError("the rotated q has no gradient; use qk_norm_rope, or call under torch.no_grad()")
-    # all that the checks below and the block depend on, but addresses (the caller has checked k, v and slots)
-    key = ("append", _layout(q), _layout(k), _layout(v), _layout(cos), _layout(sin), _layout(positions), interleaved,
-           entry.dtype, dev, h, d, entry.total_context_len, entry.k_scales is None)
     memo = q_meta.launch_memo
     m = memo.get(key)
     if m is not None and m.cu is q_meta.cu_seqlens and m.meta == (q_meta.B, q_meta.N, t):

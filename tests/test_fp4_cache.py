@@ -193,6 +193,9 @@ def test_append_refusals(fp4):
             cache.append_paged_kv_cache(0, **{**args, **kw})
     with pytest.raises(ValueError, match="no CPU compute path"):  # checked before anything else of the call
         cache.append_paged_kv_cache(0, **args, cos=cos, sin=cos)
+    for kw in (dict(positions=[0, 1, 0]), dict(sin=cos.numpy()), dict(q=k.tolist())):
+        with pytest.raises(ValueError, match="must be tensors"):
+            cache.append_paged_kv_cache(0, **{**args, "cos": cos, "sin": cos, **kw})
 
 
 def test_rotating_append_checks():
