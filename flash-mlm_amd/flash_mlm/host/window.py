@@ -284,12 +284,19 @@ def flash_attn_mlm_window(
     refuse_tangents("flash_attn_mlm_window", q, k, v)
     grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)
                                         or (v is not None and v.requires_grad))
+    # (before the kept calls are asked: 1.0 and True equal 1 there)
+    if not isinstance(window, (tuple, list)) or len(window) != 2:
+        raise ValueError("window must be a pair (left, right)")
+    left, right = _limit(window[0], "window"), _limit(window[1], "window")
+    if sinks is None:
+        raise ValueError("sinks must be an integer >= 0")
+    sinks = _limit(sinks, "sinks")
     call = key = None
-    if context_index is None and isinstance(window, tuple):
+    if context_index is None and type(num_heads) is int:
         # all that the checks depend on
         key = ("window", _tkey(q), None if k is None else _tkey(k), None if v is None else _tkey(v), num_heads,
-               q_meta.B, q_meta.N, q_meta.total_tokens, float(scale), window, sinks, None if entry is None else id(entry),
-               inference_cache is None, layer_id is None)
+               q_meta.B, q_meta.N, q_meta.total_tokens, float(scale), left, right, sinks,
+               None if entry is None else id(entry), inference_cache is None, layer_id is None)
         call = q_meta.launch_memo.get(key)
         if call is not None and (call.cu is not q_meta.cu_seqlens or
                                  (None if call.entry_ref is None else call.entry_ref()) is not entry):
@@ -297,12 +304,7 @@ def flash_attn_mlm_window(
     rows = (q, k, v)
     if call is None:
         validate_cache_request(prefill=False, inference_cache=inference_cache, layer_id=layer_id)
-        if not isinstance(window, (tuple, list)) or len(window) != 2:
-            raise ValueError("window must be a pair (left, right)")
-        left, right = (_limit(x, "window") for x in window)
-        if sinks is None:
-            raise ValueError("sinks must be an integer >= 0")
-        call, rows = _build(q, k, v, num_heads, q_meta, scale, left, right, _limit(sinks, "sinks"), entry, context_index)
+        call, rows = _build(q, k, v, num_heads, q_meta, scale, left, right, sinks, entry, context_index)
         cu, context = call.keep
         if (key is not None and rows[0] is q and rows[1] is k and rows[2] is v and cu is q_meta.cu_seqlens
                 and (context is None or (context[0] is entry.k_cache and context[1] is entry.v_cache

@@ -453,6 +453,59 @@ def test_values_that_are_not_finite_where_a_row_does_not_look(device, kind, bad,
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["packed", "paged", "fp4", None])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_that_are_not_finite_under_long_windows(device, kind, D):
+    """The same where tiles of rows are tall and waves pass tiles that their own rows do not see"""
+    n, H, window, sinks = (150 if kind else 850), 2, (600, 4), 3
+    g, q, k, v, meta = _inputs(device, "bf16", [n], n, H, D, 13)
+    layer = _Layer(kind, "bf16", H, D, [700], device, g) if kind else None
+    first = 700 if kind else 0
+    run = lambda: flash_attn_mlm_window(q, k, v, H, meta, 0.1, window=window, sinks=sinks,  # noqa: E731
+                                        inference_cache=layer.cache if kind else None, layer_id=0 if kind else None)
+    out = run()
+    _check(out, q, k, v, [n], [700], layer, window, sinks, 0.1, "bf16")
+    spots = [first + 133] if kind else [40, 41, 845]
+    if kind:
+        behind = [layer.at[0][j] for j in (100, 101, 130)]
+        if kind == "fp4":
+            for name in ("k_scales", "v_scales"):
+                layer.pools[name].view(H, -1, D // 32)[:, behind] = 255
+        else:
+            for x in layer.rows:
+                x[:, behind] = float("inf")
+        spots += [100, 101, 130]
+    for s in spots:
+        if s >= first:
+            k[0, :, s - first] = v[0, :, s - first] = float("nan")
+    clean = [i for i in range(n) if not any(first + i - 600 <= s <= first + i + 4 for s in spots)]
+    assert len(clean) > 90
+    got, was = (_f64(x).reshape(H, n, D) for x in (run(), out))
+    for h in range(H):
+        vv = _f64(v[0, h]) if layer is None else np.concatenate((layer.v[0][h], _f64(v[0, h])))
+        # the same sums in another order at most: each is off by what _check allows
+        size = np.abs(np.where(np.isfinite(vv), vv, 0)).max(0)
+        assert (np.abs(got[h, clean] - was[h, clean]) <= 2 * (3 * _half("bf16") + 1e-4) * size).all()
+    dirty = [i for i in range(n) if i not in clean]
+    assert not np.isfinite(got[:, dirty]).all(2).any()
+
+
+@pytest.mark.gpu
+def test_refusals_after_a_legal_call(device):
+    """What equals a legal argument and is none is refused also when the legal one's call is kept"""
+    _, q, k, v, meta = _inputs(device, "bf16", [3, 5], 5, 2, 64, 14)
+    run = lambda H=2, **kw: flash_attn_mlm_window(q, k, v, H, meta, 0.1, **kw)  # noqa: E731
+    run(window=(1, 0), sinks=1)
+    for kw in (dict(window=(1.0, 0), sinks=1), dict(window=(1, False), sinks=1), dict(window=(1, 0), sinks=True),
+               dict(window=(1, 0), sinks=1.0), dict(window=(1, 0), sinks=1, layer_id=0)):
+        with pytest.raises(ValueError):
+            run(**kw)
+    with pytest.raises((TypeError, ValueError)):
+        run(H=2.0, window=(1, 0), sinks=1)
+    assert torch.equal(run(window=(1, 0), sinks=1), run(window=[1, 0], sinks=1))
+
+
+@pytest.mark.gpu
 def test_scores_of_infinite_size(device):
     """Scores far below the others, and the largest scores a type can make, in a row's last keys"""
     lens, N, H, D = [130], 130, 1, 64
