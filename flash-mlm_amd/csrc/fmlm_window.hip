@@ -480,9 +480,6 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
     }
     __builtin_amdgcn_s_setprio(0);
   };
-  const char* v_next = nullptr;
-  uint32_t v_pitch = 0;
-  int v_last = 0;
   auto step = [&](int v, int u, f32x4 (&sc)[NKB][QB], f32x4 (&sn)[NKB][QB]) {
     if constexpr (FP4) {
       const int tk = v + 2 < n ? tile_at(v + 2) : -1, tv = v + 1 < n ? tile_at(v + 1) : -1;
@@ -495,19 +492,10 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
       if (nk >= 0 && is_code(nk)) fetch_codes(nk, false);
       if (tk >= 0 && is_code(tk)) fetch_codes(tk, true);
     } else {
-      // the walk stands at tile v + 2, V's last pointer (two buffers) at v + 1
-      if constexpr (C::NV == 2)
-        if (v + 1 < n) load_rows(v_next, v_pitch, v_last, vbuf(u + 1));
-      if (v + 2 < n) {
+      if (v + 2 < n) {  // the walk stands at tile v + 2
         const int last = keys_in(wk.t) - 1;
         load_rows(wk.k, wk.rk, last, kbuf(u));
-        if constexpr (C::NV == 3) {
-          load_rows(wk.v, wk.rv, last, vbuf(u + 2));
-        } else {
-          v_next = wk.v;
-          v_pitch = wk.rv;
-          v_last = last;
-        }
+        load_rows(wk.v, wk.rv, last, vbuf(u + 2));
         move();
       }
     }
@@ -574,7 +562,10 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
     for (int db = 0; db < C::NDB; ++db) o[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   if (n > 0) {
-    // tiles 0 and 1 (V(1) only with a third buffer), and of 4-bit ones the codes of the next
+    // Tiles 0 and 1 (V(1) only with a third buffer), and of 4-bit ones the codes of the next.  Workgroups that
+    // start together all wait for memory here: what S(0) needs comes first, q by LDS too, where V(1) and
+    // V(2) follow it, and S(0) does not wait for the others.
+    constexpr int VPW = BK / (Tile::RPI * kNW);
     if constexpr (FP4) {
       bring(0, false, kbuf(0));
       bring(0, true, vbuf(0));
@@ -582,27 +573,35 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
       if (n > 2 && is_code(tile_at(2))) fetch_codes(tile_at(2), false);
       if (n > 1 && is_code(tile_at(1))) fetch_codes(tile_at(1), true);
     } else {
+      static_assert(C::NV == 3 && QB * 16 * kNW <= 2 * BK, "q's rows in V(1) and V(2)");
+      Tile::template load<QB * 16 * kNW>((const char*)p.q + row_at(p.q_layout, s.b, s.h, s.q0, row0, p.q_sb, p.q_sh, p.q_sn) * 2,
+                                         (uint32_t)p.q_sn * 2u, rows - 1, lds_addr(vbuf(1)), wave, lane);
       seek(0);
       pitch0 = wk.rk;
       Tile::template offsets<BK>(pitch0, wave, lane, off0);
       load_rows(wk.k, wk.rk, keys_in(wk.t) - 1, kbuf(0));
       load_rows(wk.v, wk.rv, keys_in(wk.t) - 1, vbuf(0));
       move();
-      if (n > 1) {
-        v_last = keys_in(wk.t) - 1;
-        load_rows(wk.k, wk.rk, v_last, kbuf(1));
-        if constexpr (C::NV == 3) load_rows(wk.v, wk.rv, v_last, vbuf(1));
-        v_next = wk.v;
-        v_pitch = wk.rv;
-        move();
-      }
+      if (n > 1) load_rows(wk.k, wk.rk, keys_in(wk.t) - 1, kbuf(1));
     }
+    if constexpr (FP4) {
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
+      for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-      for (int kc = 0; kc < C::KC; ++kc) qf[qb][kc] = q_frag(qb, kc);
-    __builtin_amdgcn_s_waitcnt(0);
+        for (int kc = 0; kc < C::KC; ++kc) qf[qb][kc] = q_frag(qb, kc);
+      __builtin_amdgcn_s_waitcnt(0);
+    } else {  // q and K(0) have landed
+      if (n > 1) __builtin_amdgcn_s_waitcnt(((2 * VPW) & 15) | (7 << 4) | (0 << 8) | (((2 * VPW) >> 4) << 14));
+      else __builtin_amdgcn_s_waitcnt((VPW & 15) | (7 << 4) | (0 << 8) | ((VPW >> 4) << 14));
+    }
     __syncthreads();
+    if constexpr (!FP4) {
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int kc = 0; kc < C::KC; ++kc)
+          qf[qb][kc] = __builtin_bit_cast(v8, __builtin_bit_cast(u32x4, tr.row(vbuf(1), wave * QB + qb, kc)) ^ qsign);
+    }
     if (active) {
 #pragma unroll
       for (int kc = 0; kc < C::KC; ++kc)
@@ -615,7 +614,14 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
         }
       row_max(sa);
     }
-    __syncthreads();  // every wave is done with K(0): its buffer may be refilled
+    if constexpr (!FP4) __builtin_amdgcn_s_waitcnt(0);  // V(0) and K(1)
+    __syncthreads();  // every wave is done with K(0) and q: their buffers may be refilled
+    if constexpr (!FP4) {
+      if (n > 1) {
+        load_rows(wk.v, wk.rv, keys_in(wk.t) - 1, vbuf(1));
+        move();
+      }
+    }
   }
   for (int v = 0; v < n;) {
 #pragma unroll
