@@ -29,6 +29,8 @@ constexpr int kBK = 64;   // keys of a tile; 32 at D = 256, where two workgroups
 constexpr int tile_keys(int D) { return D == 256 ? 32 : kBK; }
 constexpr int kMaxParts = 32;
 constexpr int kMinPartTiles = 4;  // key tiles of a part at least
+constexpr int kFewTiles = 8;      // ... where its waves walk apart
+constexpr int kFill = 512;        // workgroups: two a CU
 constexpr int kNoLimit = 1 << 30;  // a window without a limit; positions stay below
 // the running maximum moves only when a new one exceeds it by more than this (log2 units)
 constexpr float kSlack = 8.0f;
@@ -1494,6 +1496,8 @@ int64_t max_keys(const fmlm_attn_params& p, const fmlm_window& w, int rows) {
 }
 
 constexpr int kWideTiles = 9;
+// calls whose key ranges stay whole: the backward reads a row's statistics from one workgroup
+bool unsplit(const fmlm_attn_params& p, const fmlm_window& w) { return p.lse || w.o_low || (p.flags & FMLM_FLAG_NOSPLIT); }
 
 struct FwdLaunch {
   const void* fn;
@@ -1508,17 +1512,21 @@ void merge_of(FwdLaunch& f) {
   f.merge[0] = (const void*)window_merge_kernel<T, D, 1>;
   f.merge[1] = (const void*)window_merge_kernel<T, D, 256 / (D / 8)>;
 }
-template <typename T, int D, int QB>
-FwdLaunch fwd_of(bool fp4) {
-  static std::atomic<uint64_t> allowed[2];
+template <typename T, int D, int QB, bool FP4>
+FwdLaunch fwd_of() {
+  static std::atomic<uint64_t> allowed;
   FwdLaunch f;
-  f.allowed = &allowed[fp4];
-  f.fn = fp4 ? (const void*)window_fwd_kernel<T, D, QB, true> : (const void*)window_fwd_kernel<T, D, QB, false>;
+  f.allowed = &allowed;
+  f.fn = (const void*)window_fwd_kernel<T, D, QB, FP4>;
   merge_of<T, D>(f);
   f.bq = kNW * QB * 16;
-  f.lds = fp4 ? FwdCfg<D, true>::LDS : FwdCfg<D, false>::LDS;
+  f.lds = FwdCfg<D, FP4>::LDS;
   f.lg = tile_keys(D) == 64 ? 6 : 5;
   return f;
+}
+template <typename T, int D, int QB>
+FwdLaunch fwd_of(bool fp4) {
+  return fp4 ? fwd_of<T, D, QB, true>() : fwd_of<T, D, QB, false>();
 }
 template <typename T, int D>
 FwdLaunch few_of() {
@@ -1543,14 +1551,21 @@ FwdLaunch pick_fwd(const fmlm_attn_params& p, const fmlm_window& w) {
       default: return few_of<T, 256>();
     }
   }
-  // 128 rows that share a tile's loads, from walks of kWideTiles tiles on; below, more and smaller
-  // workgroups (kernel us, 64 against 128 rows: walks of 4-5 tiles, D = 64, 31 : 44; of 10, D = 128,
-  // 72 : 69; of 20, 210 : 174; of 50 in 4 bits 139 : 96)
-  const bool wide = longest(p) > 64 && max_keys(p, w, 128) > kWideTiles * kBK;
+  const int64_t tiles = max_keys(p, w, 128) / kBK, units = (int64_t)p.B * p.H * ((longest(p) + 127) / 128);
+  const bool tall = longest(p) > 64;
+  // 128 rows that share a tile.  In 16 bits where its fragments are longest beside the rest (D = 128) and
+  // such workgroups are two a CU, parts counted (us with 64 against 128 rows: 8 x 16 x 2048 rows, windows
+  // of 100, 450 and 1200, 85 : 79, 135 : 115, 188 : 153, at D = 64 38 : 51, 63 : 74, 95 : 101; 2 x 16 x 512
+  // rows 12 : 17; 256 rows over 511 of 8192 keys 14 : 18, over 16384 keys 75 : 54).
+  const bool wide = !fp4 && tall && units * (unsplit(p, w) ? 1 : std::max<int64_t>(tiles / kMinPartTiles, 1)) >= kFill;
+  // In 4 bits they share its conversion too: at every D, but for short walks, whose workgroups are all start
+  // and end (4 x 16 x 512 rows over 4096 keys 84 : 77 at D = 64, 78 : 63 at 32, over 255 of 4000 16 : 18.6
+  // and 13 : 14.8).
+  const bool wide4 = fp4 && tall && tiles > kWideTiles;
   switch (p.D) {
-    case 32: return wide ? fwd_of<T, 32, 2>(fp4) : fwd_of<T, 32, 1>(fp4);
-    case 64: return wide ? fwd_of<T, 64, 2>(fp4) : fwd_of<T, 64, 1>(fp4);
-    case 128: return wide ? fwd_of<T, 128, 2>(fp4) : fwd_of<T, 128, 1>(fp4);
+    case 32: return wide4 ? fwd_of<T, 32, 2, true>() : fwd_of<T, 32, 1>(fp4);
+    case 64: return wide4 ? fwd_of<T, 64, 2, true>() : fwd_of<T, 64, 1>(fp4);
+    case 128: return wide ? fwd_of<T, 128, 2, false>() : wide4 ? fwd_of<T, 128, 2, true>() : fwd_of<T, 128, 1>(fp4);
     default: return fwd_of<T, 256, 1>(fp4);  // (two blocks of 16 rows spill)
   }
 }
@@ -1609,14 +1624,24 @@ WinArgs win_args(const fmlm_attn_params& p, const fmlm_window& w, int rows) {
   return a;
 }
 
-// parts that key ranges are cut into at most, and a record's rows
+// Parts that key ranges are cut into at most, and a record's rows.  Parts until there are kFill workgroups,
+// two a CU (us a call in 16 bits, with 256 / 512 / 1024: 2 x 64 rows, 8192 keys, D = 128, 34 / 36 / 47; 8
+// single rows, D = 64, 66 / 52 / 53; 256 rows, D = 256, 88 / 68 / 97; the 512 against 256 and 1024 of
+// 128-row tiles: 85 : 116 : 111), each with kMinPartTiles tiles; of few rows in 4 bits, where the four waves
+// walk apart, with kFewTiles (16 rows, 8192 keys: 16.4 with 4, 13.8 with 8, 15.8 with 16).  Between 512 and 2048
+// units of those, parts of 32 tiles even out the last round (64 users with 4096 keys: 119 whole, 114 in
+// two, 121 in four; with 500 to 8192 keys, in two 131, in four 128); smaller ones cost more than that (32 x 4
+// rows, 1000 keys: 18.5 whole, 27 in two).
 void plan_parts(const fmlm_attn_params& p, const fmlm_window& w, const FwdLaunch& f, WinArgs& a) {
   a.rec_rows = std::min(f.bq, longest(p));
   a.lg = f.lg;
-  const int64_t units = (int64_t)p.B * p.H * a.tiles;
-  const int64_t fill = f.bq == kFewRows ? 4096 : a.rec_rows <= 64 ? 1024 : 512;
-  if (p.lse || w.o_low || (p.flags & FMLM_FLAG_NOSPLIT) || units >= fill) return;
-  const int64_t tiles = (max_keys(p, w, f.bq) >> f.lg) + 2, want = (fill + units - 1) / units;
+  if (unsplit(p, w)) return;
+  const int64_t units = (int64_t)p.B * p.H * a.tiles, tiles = (max_keys(p, w, f.bq) >> f.lg) + 2;
+  int64_t want = (kFill + units - 1) / units;
+  if (f.bq == kFewRows) {
+    if (units >= kFill && units < 4 * kFill) want = std::min<int64_t>(4, tiles / (4 * kFewTiles));
+    want = std::min(want, tiles / kFewTiles);
+  }
   a.parts = (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / kMinPartTiles, kMaxParts}));
 }
 

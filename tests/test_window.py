@@ -319,6 +319,37 @@ def test_long_rows_over_contexts(device, kind, window, sinks):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", WINDOWS, ids=str)
+@pytest.mark.parametrize("kind,dtype", [("packed", "fp16"), ("paged", "bf16")])
+def test_tall_tiles_over_contexts(device, kind, dtype, window, sinks):
+    """Enough heads for 128-row tiles in 16 bits; the first ones are checked"""
+    lens, N, H, D, ctx = [200, 129, 0, 1], 200, 64, 128, [100, 0, 5, 300]
+    g, q, k, v, meta = _inputs(device, dtype, lens, N, H, D, 31)
+    layer = _Layer(kind, dtype, H, D, ctx, device, g)
+    out = flash_attn_mlm_window(q, k, v, H, meta, 0.1, window=window, sinks=sinks, inference_cache=layer.cache, layer_id=0)
+    _check(out[: 2 * sum(lens)], q[:, :2], k[:, :2], v[:, :2], lens, ctx, layer, window, sinks, 0.1, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", WINDOWS + [((150, 20), 3)], ids=str)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_tall_tiles_and_their_gradients(device, dtype, window, sinks):
+    """Enough heads for 128-row tiles; the first two are checked, the others repeat them"""
+    lens, N, H, D = [200, 129, 0, 300], 301, 64, 128
+    g, q, k, v, meta = _inputs(device, dtype, lens, N, 2, D, 32)
+    leaves = [x.repeat(1, H // 2, 1, 1).requires_grad_() for x in (q, k, v)]
+    out = flash_attn_mlm_window(*leaves, H, meta, 0.15, window=window, sinks=sinks)
+    two = 2 * sum(lens)
+    assert torch.equal(out, out[:two].repeat(H // 2, 1))
+    _check(out[:two], q, k, v, lens, None, None, window, sinks, 0.15, dtype)
+    do = _rand(g, (two, D), out.dtype)
+    grads = torch.autograd.grad(out, leaves, do.repeat(H // 2, 1))
+    assert all(torch.equal(x, x[:, :2].repeat(1, H // 2, 1, 1)) for x in grads)
+    got = [_by_sequence(x[:, :2], lens, 2, D) for x in grads]
+    _grad_check(got, q, k, v, _f64(do).reshape(2, -1, D), lens, window, sinks, 0.15, dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["packed", "paged", "fp4"])
 def test_context_index_and_shared_contexts(device, kind):
     lens, N, H, D = [2, 1, 3], 3, 2, 64
@@ -457,14 +488,15 @@ def test_values_that_are_not_finite_where_a_row_does_not_look(device, kind, bad,
 @pytest.mark.parametrize("D", [64, 128])
 def test_values_that_are_not_finite_under_long_windows(device, kind, D):
     """The same where tiles of rows are tall and waves pass tiles that their own rows do not see"""
-    n, H, window, sinks = (150 if kind else 850), 2, (600, 4), 3
+    # (heads: calls of fewer workgroups take 64-row tiles in 16 bits)
+    n, H, window, sinks = (150 if kind else 850), (2 if kind == "fp4" or D < 128 else 128 if kind else 74), (600, 4), 3
     g, q, k, v, meta = _inputs(device, "bf16", [n], n, H, D, 13)
     layer = _Layer(kind, "bf16", H, D, [700], device, g) if kind else None
     first = 700 if kind else 0
     run = lambda: flash_attn_mlm_window(q, k, v, H, meta, 0.1, window=window, sinks=sinks,  # noqa: E731
                                         inference_cache=layer.cache if kind else None, layer_id=0 if kind else None)
     out = run()
-    _check(out, q, k, v, [n], [700], layer, window, sinks, 0.1, "bf16")
+    _check(out[: 2 * n], q[:, :2], k[:, :2], v[:, :2], [n], [700], layer, window, sinks, 0.1, "bf16")
     spots = [first + 133] if kind else [40, 41, 845]
     if kind:
         behind = [layer.at[0][j] for j in (100, 101, 130)]
