@@ -215,6 +215,18 @@ struct FwdCfg {
 // ones load: K(v + 2) into K(v)'s buffer and V(v + NV - 1) into V(v - 1)'s.  4-bit tiles are a step
 // ahead of that: their codes arrive in step v and are converted, by the wave that loaded them, at
 // the start of step v + 1.
+//
+// P goes to the input type as an operand of the matrix cores, off by half a step; l adds up the same
+// rounded values (a product with ones), so that what all of a row's probabilities share cancels.  Scores, maxima,
+// l and O stay in 32 bits.
+//
+// Bound: fp16, 4 x 16 causal sequences of 4096 rows of 128: a window of 64 takes 66 us (268 MB, 81% of a
+// large copy's rate), all keys 231 us (1190 TFLOP/s, a large matrix product's rate).  Between them
+// the two add up (1024 keys: 150 us; 31% of the matrix cores, 37% of the VALU), as workgroups read their first
+// tiles and rows while few others compute; another order of the tiles, staggered starts or more fragments in
+// flight changed nothing.  Single rows over 1024 keys of a paged context (64 users) are at a copy's rate.
+// 4 bits: 93 us for the 46 GFLOP of four chunks of 300 to 512 rows over 2000 to 4000 keys, 21% of the matrix
+// cores and 26% of the VALU (the conversions among it) at 1.2 waves a SIMD: 512 workgroups, of unequal length.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int QB, bool FP4>
 __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn_params p, const WinArgs a) {
@@ -758,7 +770,9 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
 // S^T = K Q^T: the contraction takes the elements in the order (quarter, fragment), and q comes in
 // that order too.  V is converted the same way into a wave's own 32 rows of LDS and read back
 // transposed.  A tile's registers are loaded again as soon as they have been converted.  The four
-// waves' sums meet in LDS at the end.
+// waves' sums meet in LDS at the end.  Bound by memory: 64 users over 500 to 8192 keys of 16 heads, D = 128, 633 MB of
+// codes and scales in 128 us, 96% of a large copy's rate; the same through window_fwd_kernel's
+// shared tiles 226 us with 4096 keys each, here 114 (16 rows a sequence: 73 and 35).
 // ---------------------------------------------------------------------------
 constexpr int kFewRows = 16;
 
@@ -1111,7 +1125,16 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const fmlm_attn_param
 }
 
 // ---------------------------------------------------------------------------
-// Backward
+// Backward, with the forward's row statistics: P = 2^(c s - lse) again, no running maximum.  P and dS go to
+// the input type as operands, off by half a step each; delta comes from o and o_low in 32 bits, or
+// o's rounding, the same for all of a row's keys, would be the largest error of dq and dk (1.55 times
+// the plain form's in fp16, with o_low 1.4).  dq by query tiles, then dK and dV by key tiles, which repeats S
+// and dP (2 of 7 products) and needs no atomics: the same bits every time.
+//
+// Bound (fp16, 4 x 16 sequences of 2000 to 4096 rows of 128, windows of 1024): dq 205 us, 37% of the matrix
+// cores and 41% of the VALU; dK / dV 314 us, 33% and 40%, with 38% of LDS: its 16 keys a wave take a fragment
+// from LDS for each product.  32 keys a wave halve that and leave one wave a SIMD: 404 us.  At D = 256 dK
+// / dV spill 12 registers with two waves a SIMD, 107 us for 8 x 8 x 300 to 1024 rows with windows of 511 (one wave a SIMD and no spills: 5% more).
 // ---------------------------------------------------------------------------
 template <int D>
 struct BwdCfg {
