@@ -110,9 +110,9 @@ def capture_leaves(what: str, *tensors) -> list[torch.Tensor]:
     capture, which ends the process when the capture ends.  An accumulator outlives its
     last reference here exactly when another live graph holds it.
     """
-    if not torch.cuda.is_current_stream_capturing():
-        return []
     leaves = [t for t in tensors if isinstance(t, torch.Tensor) and t.requires_grad and t.is_leaf]
+    if not leaves or not torch.cuda.is_current_stream_capturing():
+        return []
     for t in leaves:
         if _lives(t):
             raise ValueError(
