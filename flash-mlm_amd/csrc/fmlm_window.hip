@@ -1128,10 +1128,11 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const fmlm_attn_param
 // Backward, with the forward's row statistics: P = 2^(c s - lse) again, no running maximum.  P and dS go to
 // the input type as operands, off by half a step each; delta comes from o and o_low in 32 bits, or
 // o's rounding, the same for all of a row's keys, would be the largest error of dq and dk (1.55 times
-// the plain form's in fp16, with o_low 1.4).  dq by query tiles, then dK and dV by key tiles, which repeats S
+// the plain form's in fp16, with o_low 1.4).  What is left in it of the rounding of the forward's P goes
+// for dK: the dq kernel adds up what each row's dS, unrounded, lacks to a sum of 0.  dq by query tiles, then dK and dV by key tiles, which repeats S
 // and dP (2 of 7 products) and needs no atomics: the same bits every time.
 //
-// Bound (fp16, 4 x 16 sequences of 2000 to 4096 rows of 128, windows of 1024): dq 205 us, 37% of the matrix
+// Bound (fp16, 4 x 16 sequences of 2000 to 4096 rows of 128, windows of 1024): dq 217 us, 37% of the matrix
 // cores and 41% of the VALU; dK / dV 314 us, 33% and 40%, with 38% of LDS: its 16 keys a wave take a fragment
 // from LDS for each product.  32 keys a wave halve that and leave one wave a SIMD: 404 us.  At D = 256 dK
 // / dV spill 12 registers with two waves a SIMD, 107 us for 8 x 8 x 300 to 1024 rows with windows of 511 (one wave a SIMD and no spills: 5% more).
@@ -1199,7 +1200,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
   };
   if (wt.n > 0) issue(0);
   v8 qf[QB][C::KC], df[QB][C::KC];
-  float delta[QB], lse[QB];
+  float delta[QB], lse[QB], rest[QB];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int row = (wave * QB + qb) * 16 + l16;
@@ -1220,9 +1221,8 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
     delta[qb] = sum;
-    const int64_t at = (int64_t)s.h * p.total_q + s.q0 + row0 + row;
-    lse[qb] = ok ? p.lse[at] : INFINITY;
-    if (ok && gq == 0) ((float*)gr.workspace)[at] = sum;  // for the dK / dV kernel
+    lse[qb] = ok ? p.lse[(int64_t)s.h * p.total_q + s.q0 + row0 + row] : INFINITY;
+    rest[qb] = 0.f;
   }
   f32x4 dq[C::NDB][QB];
 #pragma unroll
@@ -1253,8 +1253,10 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
     auto soft = [&](int kb, int e) {
       const int qb = e >> 1, r = (e & 1) * 2;
       if (r == 0) pin(dp[kb][qb]);
-      uint32_t w = pack2<T>(fast_exp2(fmaf(sc[kb][qb][r], c, -lse[qb])) * dp[kb][qb][r],
-                            fast_exp2(fmaf(sc[kb][qb][r + 1], c, -lse[qb])) * dp[kb][qb][r + 1]);
+      const float x = fast_exp2(fmaf(sc[kb][qb][r], c, -lse[qb])) * dp[kb][qb][r];
+      const float y = fast_exp2(fmaf(sc[kb][qb][r + 1], c, -lse[qb])) * dp[kb][qb][r + 1];
+      rest[qb] += x + y;
+      uint32_t w = pack2<T>(x, y);
       pin(w);
       ds[kb >> 1][qb][(kb & 1) * 2 + (r >> 1)] = w;
     };
@@ -1317,7 +1319,11 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int row = (wave * QB + qb) * 16 + l16;
+    rest[qb] += __shfl_xor(rest[qb], 16);
+    rest[qb] += __shfl_xor(rest[qb], 32);
     if (row >= rows) continue;
+    // dS' = P (dP - delta') sums to delta - delta' over a row's keys: delta without the rounding of the forward's P
+    if (gq == 0) ((float*)gr.workspace)[(int64_t)s.h * p.total_q + s.q0 + row0 + row] = delta[qb] + rest[qb];
     const int64_t off = row_at(p.q_layout, s.b, s.h, s.q0, row0 + row, gr.dq_sb, gr.dq_sh, gr.dq_sn);
 #pragma unroll
     for (int db = 0; db < C::NDB; ++db) {
