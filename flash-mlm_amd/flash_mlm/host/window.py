@@ -81,6 +81,8 @@ def _context(entry, p, w, *, b: int, context_index, appended: bool, device):
     cu_kv = entry.cu_seqlens_kv
     if cu_kv is None:
         raise ValueError("window attention needs a packed or paged context (with cu_seqlens_kv)")
+    if cu_kv.device != device:  # (stored as given: a host address would reach the kernel)
+        raise ValueError("cu_seqlens_kv of the cached context must be on the device of q")
     cbs, total, d = entry.context_batch_size, int(entry.total_context_len), entry.head_dim
     index = _context_index(context_index, b=b, cbs=cbs, prefill=False, context_batch_size=None, device=device)
     if index is None and 1 < cbs < b:

@@ -125,6 +125,19 @@ def test_context_refusals():
         run("packed", 2, appended=True)
 
 
+def test_offsets_of_a_context_on_another_device_are_refused():
+    """A packed entry keeps the offsets that it was given: their host address must not reach the kernel."""
+    from flash_mlm.host.window import _context
+
+    cache, rows = InferenceCache(), torch.zeros((2 * 6, 64), dtype=torch.bfloat16)
+    cache.prefill_kv_cache(0, k_cache=rows, v_cache=rows, total_context_len=6,
+                           cu_seqlens_kv=torch.tensor([0, 2, 6], dtype=torch.int32), context_batch_size=2, is_mla=False,
+                           num_heads=2, head_dim=64)
+    with pytest.raises(ValueError, match="cu_seqlens_kv of the cached context must be on the device"):
+        _context(cache.layer_entry(0), _lib.AttnParams(), _lib.Window(), b=2, context_index=None, appended=False,
+                 device=torch.device("meta"))
+
+
 def test_argument_rejection_without_launch():
     lib = _lib.load()
     p, w = _lib.AttnParams(), _lib.Window()
