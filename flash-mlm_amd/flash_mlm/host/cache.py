@@ -183,6 +183,9 @@ class InferenceCache:
                 raise ValueError("v_cache second dim must match head_dim")
             if not v_cache.is_contiguous():
                 raise ValueError("v_cache must be contiguous")
+            # an entry has one dtype and device, those of k_cache, with which the kernels read both
+            if v_cache.dtype != k_cache.dtype or v_cache.device != k_cache.device:
+                raise ValueError("v_cache dtype/device must match k_cache")
         rows = total_context_len * (1 if is_mla else num_heads)
         if k_cache.shape[0] != rows:
             raise ValueError(f"k_cache first dim mismatch: expected {rows} rows for is_mla={is_mla}")

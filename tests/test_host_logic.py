@@ -167,6 +167,17 @@ def test_inference_cache_validation_messages():
         cache.prefill_kv_cache(0, k_cache=k, v_cache=k, cu_seqlens_kv=torch.tensor([0, 3]), context_batch_size=2, is_mla=False, num_heads=2, head_dim=4)
 
 
+def test_a_context_of_two_dtypes_or_devices_is_refused():
+    """An entry has one dtype and device: the kernels read v_cache with those of k_cache."""
+    k = torch.zeros((6, 16), dtype=torch.bfloat16)
+    args = dict(total_context_len=3, context_batch_size=1, is_mla=False, num_heads=2, head_dim=16)
+    for cu in (None, torch.tensor([0, 3], dtype=torch.int32)):
+        for v in (k.to(torch.float8_e4m3fn), k.float(), k.half(), k.to("meta")):
+            with pytest.raises(ValueError, match="v_cache dtype/device must match"):
+                InferenceCache().prefill_kv_cache(0, k_cache=k, v_cache=v, cu_seqlens_kv=cu, **args)
+        InferenceCache().prefill_kv_cache(0, k_cache=k, v_cache=k.clone(), cu_seqlens_kv=cu, **args)
+
+
 def test_inference_cache_stores_views_and_replaces():
     cache = InferenceCache()
     k1, v1 = torch.zeros(6, 4), torch.ones(6, 4)
