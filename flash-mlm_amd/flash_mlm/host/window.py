@@ -38,7 +38,7 @@ def _limit(x, what: str) -> int:
 class _Call:
     """The checked arguments of a call as parameter blocks without the addresses of its own rows."""
 
-    __slots__ = ("params", "window", "nbytes", "out_shape", "entry_ref", "keep", "cu", "strides", "grads")
+    __slots__ = ("params", "window", "nbytes", "out_shape", "entry_ref", "keep", "cu", "shape", "strides", "grads")
 
     def run(self, q, k, v, lse=None, low=None):
         """One launch on rows laid out as the call's; returns the output.  ``lse`` and ``low`` take what
@@ -169,7 +169,7 @@ def _build(q, k, v, num_heads: int, q_meta: PackMetadata, scale, left, right, si
         p.v_sb, p.v_sh, p.v_sn = _strides(v_, t)
     call.out_shape = (num_heads * t, d)
     if k is not None:  # of the backward: rows laid out like these, and contiguous gradients
-        call.strides = q_.stride(), k_.stride(), v_.stride()
+        call.shape, call.strides = q.shape, (q_.stride(), k_.stride(), v_.stride())
         g = call.grads = _lib.AttnGrads()
         g.do_sh, g.do_sn, g.workspace_bytes = p.o_sh, p.o_sn, 4 * num_heads * t
         n = p.N * d
@@ -194,7 +194,7 @@ class _Window(torch.autograd.Function):
     @staticmethod
     def forward(ctx, call, q, k, v):
         p = call.params
-        lse = torch.empty(p.H * p.total_q, dtype=torch.float32, device=q.device)
+        lse = torch.empty(call.out_shape[:1], dtype=torch.float32, device=q.device)
         low = torch.empty(call.out_shape, dtype=q.dtype, device=q.device)
         out = call.run(_rows(q), _rows(k), _rows(v), lse, low)
         ctx.call = call
@@ -209,9 +209,19 @@ class _Window(torch.autograd.Function):
         return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dout)
 
 
+def _check_saved(call, saved, dtype, device) -> None:
+    """A saved-tensor hook may bring any tensors: the kernels read these addresses with the call's sizes."""
+    rows, out = call.shape, call.out_shape
+    for t, shape, kind in zip(saved, (rows, rows, rows, out, out[:1], out), (dtype, dtype, dtype, dtype, torch.float32, dtype)):
+        if t.shape != shape or t.dtype is not kind or t.device != device:
+            raise RuntimeError(
+                "flash_attn_mlm_window: a saved tensor came back with another shape or type, or on another device")
+
+
 def _backward(ctx, dout):
     call = ctx.call
-    q, k, v, out, lse, low = ctx.saved_tensors
+    q, k, v, out, lse, low = saved = ctx.saved_tensors
+    _check_saved(call, saved, dout.dtype, dout.device)
     if dout.shape != out.shape:
         raise ValueError("gradient of the attention output has the wrong shape")
     p = _lib.AttnParams.from_buffer_copy(call.params)

@@ -138,6 +138,24 @@ def test_offsets_of_a_context_on_another_device_are_refused():
                  device=torch.device("meta"))
 
 
+def test_saved_tensors_that_do_not_fit_are_refused():
+    """What a saved-tensor hook brings back is checked before its address is used."""
+    from flash_mlm.host.window import _Call, _check_saved
+
+    call, dev, dt = _Call(), torch.device("cpu"), torch.bfloat16
+    call.shape, call.out_shape = torch.Size((2, 3, 5, 32)), (3 * 7, 32)
+    rows, out = [torch.zeros(call.shape, dtype=dt) for _ in range(3)], torch.zeros(call.out_shape, dtype=dt)
+    saved = [*rows, out, torch.zeros(21), out.clone()]
+    _check_saved(call, saved, dt, dev)
+    _check_saved(call, [rows[0].transpose(0, 1).contiguous().transpose(0, 1), *saved[1:]], dt, dev)
+    for i, x in enumerate(saved):
+        for y in (x[:1], x.view(-1), x[None], x.half(), x.to(torch.float8_e4m3fn), x.to("meta")):
+            if y.shape == x.shape and y.dtype == x.dtype and y.device == x.device:
+                continue  # (the statistics have one dimension)
+            with pytest.raises(RuntimeError, match="saved tensor came back"):
+                _check_saved(call, [*saved[:i], y, *saved[i + 1:]], dt, dev)
+
+
 def test_argument_rejection_without_launch():
     lib = _lib.load()
     p, w = _lib.AttnParams(), _lib.Window()
@@ -838,6 +856,18 @@ def test_checkpoints_and_saved_tensor_hooks(device):
         out = run(*xs)
     got = torch.autograd.grad(out, xs, do)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_hooks_that_bring_other_tensors_are_refused(device):
+    g, q, k, v, meta = _inputs(device, "bf16", [33, 2], 33, 2, 64, 25)
+    q.requires_grad_()
+    for back in (lambda x: x.cpu(), lambda x: x.to(torch.float8_e4m3fn), lambda x: x[:1], lambda x: x.view(-1)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, back):
+            out = flash_attn_mlm_window(q, k, v, 2, meta, 0.1)
+        with pytest.raises(RuntimeError, match="saved tensor came back"):
+            out.float().sum().backward()
+    assert q.grad is None
 
 
 @pytest.mark.gpu
