@@ -178,7 +178,7 @@ def _build(q, k, v, num_heads: int, q_meta: PackMetadata, scale, left, right, si
         g.dk_sb, g.dk_sh, g.dk_sn = s3
         g.dv_sb, g.dv_sh, g.dv_sn = s3
     call.entry_ref = None if entry is None else weakref.ref(entry)
-    call.cu = q_meta.cu_seqlens
+    call.cu = cu
     call.keep = (cu, context)
     # sizes of the split's records: the addresses that the checks ask for come with each run
     p.q = p.o = 256
@@ -197,7 +197,7 @@ class _Window(torch.autograd.Function):
         lse = torch.empty(call.out_shape[:1], dtype=torch.float32, device=q.device)
         low = torch.empty(call.out_shape, dtype=q.dtype, device=q.device)
         out = call.run(_rows(q), _rows(k), _rows(v), lse, low)
-        ctx.call = call
+        ctx.call, ctx.cu_version = call, _version(call)
         # read from there in the backward: autograd may free these and bring others
         ctx.save_for_backward(q, k, v, out, lse, low)
         return out
@@ -207,6 +207,12 @@ class _Window(torch.autograd.Function):
         # grad mode: create_graph, where the gradients must refuse to be differentiated (the wrapper's
         # grad-mode switches cost 4 us)
         return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dout)
+
+
+def _version(call):
+    """How often the call's offsets have been changed in place (a copy of the metadata's never is)."""
+    cu = call.cu
+    return None if cu.is_inference() else cu._version
 
 
 def _check_saved(call, saved, dtype, device) -> None:
@@ -222,6 +228,8 @@ def _backward(ctx, dout):
     call = ctx.call
     q, k, v, out, lse, low = saved = ctx.saved_tensors
     _check_saved(call, saved, dout.dtype, dout.device)
+    if _version(call) != ctx.cu_version:
+        raise RuntimeError("flash_attn_mlm_window: q_meta.cu_seqlens has been modified by an inplace operation since the forward")
     if dout.shape != out.shape:
         raise ValueError("gradient of the attention output has the wrong shape")
     p = _lib.AttnParams.from_buffer_copy(call.params)

@@ -156,6 +156,24 @@ def test_saved_tensors_that_do_not_fit_are_refused():
                 _check_saved(call, [*saved[:i], y, *saved[i + 1:]], dt, dev)
 
 
+def test_offsets_changed_since_the_forward_are_refused():
+    """The row statistics belong to the offsets that the forward read."""
+    from types import SimpleNamespace
+
+    from flash_mlm.host.window import _backward, _Call, _version
+
+    call, dt = _Call(), torch.bfloat16
+    call.shape, call.out_shape, call.cu = torch.Size((21, 32)), (21, 32), torch.tensor([0, 3, 7])
+    x = torch.zeros((21, 32), dtype=dt)
+    ctx = SimpleNamespace(call=call, cu_version=_version(call), saved_tensors=(x, x, x, x, torch.zeros(21), x))
+    call.cu.copy_(torch.tensor([0, 5, 7]))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        _backward(ctx, x)
+    with torch.inference_mode():
+        call.cu = call.cu.clone()
+    assert _version(call) is None  # (such a tensor counts no changes)
+
+
 def test_argument_rejection_without_launch():
     lib = _lib.load()
     p, w = _lib.AttnParams(), _lib.Window()
@@ -856,6 +874,19 @@ def test_checkpoints_and_saved_tensor_hooks(device):
         out = run(*xs)
     got = torch.autograd.grad(out, xs, do)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_offsets_changed_between_forward_and_backward(device):
+    g, q, k, v, meta = _inputs(device, "bf16", [3, 2], 3, 2, 64, 25)
+    q.requires_grad_()
+    run = lambda: flash_attn_mlm_window(q, k, v, 2, meta, 0.1)  # noqa: E731
+    run().float().sum().backward()
+    out = run()
+    meta.cu_seqlens.copy_(torch.tensor([0, 2, 5], device=device))
+    with pytest.raises(RuntimeError, match="cu_seqlens has been modified"):
+        out.float().sum().backward()
+    run().float().sum().backward()  # a new forward has the new offsets
 
 
 @pytest.mark.gpu
