@@ -900,6 +900,40 @@ __global__ __launch_bounds__(kNW * 64, FewCfg<D>::WPS) void window_fp4_few_kerne
     asm volatile("" ::: "memory");
   };
 
+  // of the loaded codes: scores, and the values of keys 32 h.. as 16-bit rows in LDS
+  auto scores = [&](f32x4 (&sc)[4]) {
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kc = 0; kc < C::KC; ++kc)
+        sc[kb] = Mfma<T>::run(__builtin_bit_cast(v8, fp4_oct<T>(kw[kb][kc], fp4_scale(ks[kb][kc / 4 % C::CS]))), qf[kc], sc[kb]);
+    }
+  };
+  auto put_row = [&](int i, int kc, u32x4 x) {  // chunk kc of the lane's quarter of row 16 i + l16
+    *(u32x4*)(vt + (i * 16 + l16) * (D * 2) + 16 * ((gq * C::KC + kc) ^ kv_swz<D>(l16))) = x;
+  };
+  auto put_values = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int kc = 0; kc < C::KC; ++kc)
+        put_row(i, kc, fp4_oct<T>(vw[2 * h + i][kc], fp4_scale(vs[2 * h + i][kc / 4 % C::CS])));
+  };
+  // scores of the new tokens' own keys, nk of them, and their values in LDS
+  auto own_tile = [&](f32x4 (&sc)[4], int nk) {
+    const int64_t ko = row_at(p.kv_layout, s.b, s.h, s.q0, min(l16, nk - 1), p.k_sb, p.k_sh, p.k_sn) + gq * (D / 4);
+    const int64_t vo = row_at(p.kv_layout, s.b, s.h, s.q0, min(l16, nk - 1), p.v_sb, p.v_sh, p.v_sn) + gq * (D / 4);
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kc = 0; kc < C::KC; ++kc) {
+      sc[0] = Mfma<T>::run(ld_frag<T>(p.k, ko + kc * 8, true), qf[kc], sc[0]);
+      put_row(0, kc, *(const u32x4*)((const char*)p.v + (vo + kc * 8) * 2));
+      put_row(1, kc, u32x4{0u, 0u, 0u, 0u});
+    }
+  };
+
   int page = page_of(vb + wave), next = page_of(vb + wave + kNW);
   if (vb + wave < ve && wt.tile(vb + wave) < wt.nt0) {
     const int last = keys_in(wt.tile(vb + wave)) - 1;
@@ -910,13 +944,7 @@ __global__ __launch_bounds__(kNW * 64, FewCfg<D>::WPS) void window_fp4_few_kerne
     const int t = wt.tile(v), nk = keys_in(t);
     if (t >= wt.nt0) break;  // the new tokens, at most 16: one tile, the last
     f32x4 sc[4];
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) {
-      sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kc = 0; kc < C::KC; ++kc)
-        sc[kb] = Mfma<T>::run(__builtin_bit_cast(v8, fp4_oct<T>(kw[kb][kc], fp4_scale(ks[kb][kc / 4 % C::CS]))), qf[kc], sc[kb]);
-    }
+    scores(sc);
     const bool more = v + kNW < ve && wt.tile(v + kNW) < wt.nt0;
     const int nlast = more ? keys_in(wt.tile(v + kNW)) - 1 : 0;
     page = next;
@@ -925,12 +953,7 @@ __global__ __launch_bounds__(kNW * 64, FewCfg<D>::WPS) void window_fp4_few_kerne
     softmax(sc, t * kBK, nk);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int kc = 0; kc < C::KC; ++kc)
-          *(u32x4*)(vt + (i * 16 + l16) * (D * 2) + 16 * ((gq * C::KC + kc) ^ kv_swz<D>(l16))) =
-              fp4_oct<T>(vw[2 * h + i][kc], fp4_scale(vs[2 * h + i][kc / 4 % C::CS]));
+      put_values(h);
       values(h);
     }
     if (more) load(p.v_ctx, a.v_scales, page, nlast, vw, vs);
@@ -938,50 +961,63 @@ __global__ __launch_bounds__(kNW * 64, FewCfg<D>::WPS) void window_fp4_few_kerne
   // the new tokens' own keys, by the wave whose turn it is
   if (ve > vb && wt.tile(ve - 1) >= wt.nt0 && (ve - 1 - vb) % kNW == wave) {
     const int nk = keys_in(wt.tile(ve - 1));
-    const int64_t ko = row_at(p.kv_layout, s.b, s.h, s.q0, min(l16, nk - 1), p.k_sb, p.k_sh, p.k_sn) + gq * (D / 4);
-    const int64_t vo = row_at(p.kv_layout, s.b, s.h, s.q0, min(l16, nk - 1), p.v_sb, p.v_sh, p.v_sn) + gq * (D / 4);
     f32x4 sc[4];
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-    u32x4 vrow[C::KC];
-#pragma unroll
-    for (int kc = 0; kc < C::KC; ++kc) {
-      sc[0] = Mfma<T>::run(ld_frag<T>(p.k, ko + kc * 8, true), qf[kc], sc[0]);
-      vrow[kc] = *(const u32x4*)((const char*)p.v + (vo + kc * 8) * 2);
-    }
+    own_tile(sc, nk);
     softmax(sc, s.ctx, nk);
-    // values that are not finite: a row that does not see them must not meet them as 0 inf, so they are added
-    // key by key then
-    float bad = 0.f;
-#pragma unroll
-    for (int kc = 0; kc < C::KC; ++kc) {
-      const v8 x = __builtin_bit_cast(v8, vrow[kc]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) bad = fmaf((float)x[e], 0.f, bad);
-    }
-    const bool careful = __builtin_amdgcn_ballot_w64(bad != bad) != 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int kc = 0; kc < C::KC; ++kc)
-        *(u32x4*)(vt + (i * 16 + l16) * (D * 2) + 16 * ((gq * C::KC + kc) ^ kv_swz<D>(l16))) =
-            i || careful ? u32x4{0u, 0u, 0u, 0u} : vrow[kc];
     values(0);
-    if (careful) {
-      for (int x = 0; x < 4; ++x)
+  }
+
+  // Values that are not finite in keys that a row does not see have reached it as 0 inf.  If there may be
+  // any, the wave walks its tiles once more and adds what a row sees key by key.
+  float bad = 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {  // key 4 x + r: its weight is in lane l16 + 16 x
-          const uint32_t pw = (uint32_t)__shfl((int)pf[0][r / 2], l16 + 16 * x);
-          const float wgt = (float)__builtin_bit_cast(T, (uint16_t)(r & 1 ? pw >> 16 : pw));
-          const int j = 4 * x + r;
-          if (j < nk && wgt != 0.f) {
-            const T* const val = (const T*)p.v + row_at(p.kv_layout, s.b, s.h, s.q0, j, p.v_sb, p.v_sh, p.v_sn) + 4 * gq;
+  for (int db = 0; db < C::NDB; ++db)
 #pragma unroll
-            for (int db = 0; db < C::NDB; ++db)
+    for (int r = 0; r < 4; ++r) bad = fmaf(o[db][r], 0.f, bad);
+  if (__builtin_amdgcn_ballot_w64(bad != bad)) {
+    m = -INFINITY;
+    lsum = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[db][e] = fmaf(wgt, (float)val[db * 16 + e], o[db][e]);
+    for (int db = 0; db < C::NDB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma clang loop unroll(disable)
+    for (int v = vb + wave; v < ve; v += kNW) {
+      const int t = wt.tile(v), nk = keys_in(t);
+      const bool own = t >= wt.nt0;
+      f32x4 sc[4];
+      if (own) {
+        own_tile(sc, nk);
+      } else {
+        page = page_of(v);
+        load(p.k_ctx, a.k_scales, page, nk - 1, kw, ks);
+        load(p.v_ctx, a.v_scales, page, nk - 1, vw, vs);
+        scores(sc);
+      }
+      softmax(sc, own ? s.ctx : t * kBK, nk);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (own && h > 0) break;
+        if (!own) put_values(h);
+        asm volatile("" ::: "memory");
+#pragma clang loop unroll(disable)
+        for (int x = 0; x < 8; ++x) {  // keys 4 x.. of these 32: their weights are in lane l16 + 16 (x % 4)
+          const uint32_t w0 = x < 4 ? pf[h][0] : pf[h][2], w1 = x < 4 ? pf[h][1] : pf[h][3];
+          const uint32_t w[2] = {(uint32_t)__shfl((int)w0, l16 + 16 * (x & 3)), (uint32_t)__shfl((int)w1, l16 + 16 * (x & 3))};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float wgt = (float)__builtin_bit_cast(T, (uint16_t)(r & 1 ? w[r / 2] >> 16 : w[r / 2]));
+            const int j = 4 * x + r;
+            if (wgt != 0.f) {
+#pragma unroll
+              for (int db = 0; db < C::NDB; ++db) {
+                const T* const val = (const T*)(vt + j * (D * 2) + 16 * ((2 * db + (gq >> 1)) ^ kv_swz<D>(j & 15)) + 8 * (gq & 1));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[db][e] = fmaf(wgt, (float)val[e], o[db][e]);
+              }
+            }
           }
         }
+        asm volatile("" ::: "memory");
+      }
     }
   }
 

@@ -571,6 +571,64 @@ def test_values_that_are_not_finite_under_long_windows(device, kind, D):
     assert not np.isfinite(got[:, dirty]).all(2).any()
 
 
+def _clean_rows(got, q, layer, k, v, first, clean, window, sinks, scale, dtype):
+    """The rows ``clean`` of one sequence against the oracle, as _check does; k and v None: the context holds them"""
+    for h in range(q.shape[1]):
+        kk, vv = layer.k[0][h], layer.v[0][h]
+        if k is not None:
+            kk, vv = (np.concatenate((x, _f64(y[0, h]))) for x, y in ((kk, k), (vv, v)))
+        seen = ref.visible(first, q.shape[2], len(kk), *window, sinks)[clean]
+        o, P = ref.attend(_f64(q[0, h])[clean], kk, vv, seen, scale)
+        size = P @ np.abs(np.where(np.isfinite(vv), vv, 0))
+        assert (np.abs(got[h, clean] - o) <= (3 * _half(dtype) + 1e-4) * size + 2.0**-24 * len(kk)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("appended", [False, True])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("n", [1, 5, 16, 17])
+def test_four_bit_values_that_are_not_finite_where_a_row_does_not_look(device, n, D, appended):
+    """Rows of a 4-bit context whose scales are no numbers, in tiles that the window and the sinks cut, and new
+    tokens that some rows do not see: calls of few rows (at most 16) and of more"""
+    dtype, H, ctx, window, sinks = "bf16", 2, 700, (40, 2), 3
+    g, q, k, v, meta = _inputs(device, dtype, [n], n, H, D, 15)
+    layer = _Layer("fp4", dtype, H, D, [ctx], device, g)
+    first = ctx - n if appended else ctx
+    kv = (None, None) if appended else (k, v)
+    run = lambda: flash_attn_mlm_window(q, *kv, H, meta, 0.1, window=window, sinks=sinks, inference_cache=layer.cache,  # noqa: E731
+                                        layer_id=0)
+    _check(run(), q, k, v, [n], [ctx], layer, window, sinks, 0.1, dtype, appended)
+    for late in (False, True):
+        # hidden from all rows: behind the sinks, in front of the band; then two that some rows see
+        spots = [3, 40, first - 41, first - 60] + ([first - 38, first + 10] if late else [])
+        for s in [s for s in spots if s < ctx]:
+            for name in ("k_scales", "v_scales"):
+                layer.pools[name].view(H, -1, D // 32)[:, layer.at[0][s]] = 255
+        for s in [s for s in spots if ctx <= s < first + n]:
+            k[0, :, s - first] = v[0, :, s - first] = float("nan")
+        dirty = [i for i in range(n) if any(first + i - 40 <= s <= first + i + 2 and s < first + n for s in spots)]
+        clean = [i for i in range(n) if i not in dirty]
+        assert len(clean) == n if not late else len(dirty) > 0
+        got = _f64(run()).reshape(H, n, D)
+        assert not np.isfinite(got[:, dirty]).any()
+        _clean_rows(got, q, layer, *kv, first, clean, window, sinks, 0.1, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("n", [5, 16])
+def test_new_values_that_are_not_finite_beside_few_rows_over_four_bits(device, n, bad):
+    """Only v of one new token, finite everywhere else: rows that see it get what it is"""
+    dtype, H, D, ctx, window = "fp16", 2, 64, 130, (100, 0)
+    g, q, k, v, meta = _inputs(device, dtype, [n], n, H, D, 16)
+    layer = _Layer("fp4", dtype, H, D, [ctx], device, g)
+    v[0, :, n - 2] = bad
+    out = flash_attn_mlm_window(q, k, v, H, meta, 0.1, window=window, inference_cache=layer.cache, layer_id=0)
+    got = _f64(out).reshape(H, n, D)
+    _clean_rows(got, q, layer, k, v, ctx, list(range(n - 2)), window, 0, 0.1, dtype)
+    assert (np.isnan(got[:, n - 2:]) if np.isnan(bad) else got[:, n - 2:] == bad).all()
+
+
 @pytest.mark.gpu
 def test_refusals_after_a_legal_call(device):
     """What equals a legal argument and is none is refused also when the legal one's call is kept"""
