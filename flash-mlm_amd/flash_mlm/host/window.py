@@ -232,6 +232,8 @@ def _backward(ctx, dout):
         raise RuntimeError("flash_attn_mlm_window: q_meta.cu_seqlens has been modified by an inplace operation since the forward")
     if dout.shape != out.shape:
         raise ValueError("gradient of the attention output has the wrong shape")
+    if call.params.total_q == 0:  # no token: padding rows alone
+        return None, torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
     p = _lib.AttnParams.from_buffer_copy(call.params)
     p.q, p.k, p.v = ptrs = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if (q.stride(), k.stride(), v.stride()) != call.strides or (ptrs[0] | ptrs[1] | ptrs[2]) & 15:
@@ -341,12 +343,9 @@ def flash_attn_mlm_window(
         if entry is not None:
             raise ValueError("flash_attn_mlm_window has no backward over a cached context; call it under torch.no_grad()")
         leaves = capture_leaves("flash_attn_mlm_window", q, k, v)
-        if call.params.total_q:
-            out = _Window.apply(call, q, k, v)
-            keep_leaves(leaves)
-            return out
+        out = _Window.apply(call, q, k, v)
+        keep_leaves(leaves)
+        return out
     if entry is not None and torch.is_grad_enabled() and entry.k_cache.requires_grad:
         raise ValueError("flash_attn_mlm_window has no gradient of a cached context; call it under torch.no_grad()")
-    if call.params.total_q == 0:
-        return torch.empty(call.out_shape, dtype=q.dtype, device=q.device)
     return call.run(*rows)

@@ -717,6 +717,23 @@ def test_no_tokens_and_empty_pools(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_batch_without_tokens_has_gradients(device, packed):
+    """Zeros, through the graph as those of any other batch"""
+    _, q, k, v, meta = _inputs(device, "bf16", [0, 0], 4, 2, 64, 14)
+    xs = [(x.view(-1, 64)[:0] if packed else x).clone().requires_grad_() for x in (q, k, v)]
+    for leaves in ((0, 1, 2), (1,)):
+        args = [x if i in leaves else x.detach() for i, x in enumerate(xs)]
+        for _ in range(2):  # the second call is the kept one
+            out = flash_attn_mlm_window(*args, 2, meta, 1.0, window=(3, 0), sinks=1)
+            assert out.shape == (0, 64) and out.requires_grad
+            grads = torch.autograd.grad(out.float().sum(), [xs[i] for i in leaves])
+            assert all(g.shape == xs[0].shape and not g.any() for g in grads)
+    with torch.no_grad():
+        assert not flash_attn_mlm_window(*xs, 2, meta, 1.0).requires_grad
+
+
+@pytest.mark.gpu
 def test_metadata_that_contradicts_itself_stays_in_bounds(device):
     _, q, k, v, meta = _inputs(device, "bf16", [3, 1], 4, 2, 64, 15)
     g = torch.Generator(device=device).manual_seed(0)
