@@ -93,11 +93,12 @@ def _context(entry, p, w, *, b: int, context_index, appended: bool, device):
     p.cu_seqlens_kv, p.ctx_batch, p.ctx_index = cu_kv.data_ptr(), cbs, _lib.ptr(index)
     p.ctx_rows, p.c_sh, p.c_sn = total, total * d, d
     k, v = entry.k_cache, entry.v_cache
-    if entry.block_table is not None:
-        p.ctx_block_table, p.ctx_pages_per_batch = entry.block_table.data_ptr(), int(entry.block_table.shape[1])
+    table = entry.block_table
+    if table is not None and (total == 0 or table.shape[1] == 0):
+        p.ctx_rows = 0  # no page to read, and no address of a table without columns
+    elif table is not None:
+        p.ctx_block_table, p.ctx_pages_per_batch = table.data_ptr(), int(table.shape[1])
         p.ctx_page_stride, p.ctx_rows = PAGE_ROWS * d, total // PAGE_ROWS
-        if total == 0:  # no page to read
-            p.ctx_pages_per_batch = 0
     elif k.numel():
         k, v = aligned16(k), aligned16(v)
     if k.numel():

@@ -125,6 +125,31 @@ def test_context_refusals():
         run("packed", 2, appended=True)
 
 
+@pytest.mark.parametrize("kind", ["paged", "fp4"])
+@pytest.mark.parametrize("pages,width", [(3, 0), (0, 2), (0, 0)])
+def test_contexts_without_a_page_to_read(kind, pages, width):
+    """A block table without columns (torch gives it no address) or a pool without pages: no context rows."""
+    from flash_mlm.host.window import _context
+
+    H, D, cache = 2, 64, InferenceCache()
+    index = dict(block_table=torch.zeros((2, width), dtype=torch.int32), context_lens=torch.zeros(2, dtype=torch.int32),
+                 num_heads=H, head_dim=D)
+    pool = lambda cols, dt: torch.zeros((H, pages, PAGE, cols), dtype=dt)  # noqa: E731
+    if kind == "fp4":
+        codes, scales = pool(D // 2, torch.uint8), pool(D // 32, torch.uint8)
+        cache.prefill_paged_fp4_cache(0, k_pages=codes, v_pages=codes, k_scales=scales, v_scales=scales,
+                                      dtype=torch.bfloat16, **index)
+    else:
+        rows = pool(D, torch.bfloat16)
+        cache.prefill_paged_kv_cache(0, k_pages=rows, v_pages=rows, is_mla=False, **index)
+    p, w = _lib.AttnParams(), _lib.Window()
+    p.dtype, p.B, p.H, p.D, p.N, p.total_q, p.cu_seqlens_q, p.q, p.o = 0, 2, H, D, 4, 8, 256, 256, 256
+    keep = _context(cache.layer_entry(0), p, w, b=2, context_index=None, appended=True, device=torch.device("cpu"))  # noqa: F841
+    w.flags |= _lib.WINDOW_APPENDED
+    assert p.ctx_rows == 0 and p.ctx_pages_per_batch == 0
+    assert _lib.load().fmlm_window_workspace_bytes(p, w) == 0
+
+
 def test_offsets_of_a_context_on_another_device_are_refused():
     """A packed entry keeps the offsets that it was given: their host address must not reach the kernel."""
     from flash_mlm.host.window import _context
@@ -714,6 +739,27 @@ def test_no_tokens_and_empty_pools(device):
         out = flash_attn_mlm_window(q, k, v, 2, meta, 1.0, window=(1, 0), inference_cache=layer.cache, layer_id=0)
         assert torch.equal(out, flash_attn_mlm_window(q, k, v, 2, meta, 1.0, window=(1, 0)))
         assert not flash_attn_mlm_window(q, None, None, 2, meta, 1.0, inference_cache=layer.cache, layer_id=0).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["paged", "fp4"])
+def test_block_tables_without_columns(device, kind):
+    """Contexts of no rows over a pool that has pages: before anyone's first token is stored"""
+    g, q, k, v, meta = _inputs(device, "bf16", [3, 1], 4, 2, 64, 14)
+    layer = _Layer(kind, "bf16", 2, 64, [70, 3], device, g)
+    index = dict(block_table=torch.zeros((2, 0), dtype=torch.int32, device=device),
+                 context_lens=torch.zeros(2, dtype=torch.int32, device=device), num_heads=2, head_dim=64)
+    if kind == "fp4":
+        layer.cache.prefill_paged_fp4_cache(0, **layer.pools, dtype=torch.bfloat16, **index)
+    else:
+        k_pages, v_pages = layer.cache.paged_kv_values(0)
+        layer.cache.prefill_paged_kv_cache(0, k_pages=k_pages, v_pages=v_pages, is_mla=False, **index)
+    run = lambda k, v, **kw: flash_attn_mlm_window(q, k, v, 2, meta, 1.0, window=(1, 0), **kw)  # noqa: E731
+    assert torch.equal(run(k, v, inference_cache=layer.cache, layer_id=0), run(k, v))
+    assert not run(None, None, inference_cache=layer.cache, layer_id=0).any()
+    got = fm.flash_attn_mlm_compressed(q, k, v, 2, meta, 1.0, layer.cache, 0)
+    want = flash_attn_mlm_window(q, k, v, 2, meta, 1.0)
+    assert (got.float() - want.float()).abs().max() <= 8 * 2.0**-8 * want.float().abs().max()
 
 
 @pytest.mark.gpu
