@@ -10,7 +10,7 @@ import torch
 
 from flash_mlm import _lib
 from flash_mlm.host.cache import PAGE_ROWS, InferenceCache, PackMetadata
-from flash_mlm.host.host import _context_index, _entry_of, _tkey, rows16
+from flash_mlm.host.host import _context_index, _entry_of, _tkey, _wants_grad, rows16
 from flash_mlm.host.host_utils import (
     _device_scope,
     aligned16,
@@ -304,7 +304,10 @@ def flash_attn_mlm_window(
     outputs of earlier calls on them are alive.
     """
     entry = _entry_of(inference_cache, layer_id)
-    refuse_tangents("flash_attn_mlm_window", q, k, v)
+    context = () if entry is None else (entry.k_cache, entry.v_cache)
+    refuse_tangents("flash_attn_mlm_window", q, k, v, *context)
+    if _wants_grad(*context):
+        raise ValueError("flash_attn_mlm_window has no gradient of a cached context; call it under torch.no_grad()")
     grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)
                                         or (v is not None and v.requires_grad))
     # (before the kept calls are asked: 1.0 and True equal 1 there)
@@ -328,10 +331,10 @@ def flash_attn_mlm_window(
     if call is None:
         validate_cache_request(prefill=False, inference_cache=inference_cache, layer_id=layer_id)
         call, rows = _build(q, k, v, num_heads, q_meta, scale, left, right, sinks, entry, context_index)
-        cu, context = call.keep
+        cu, kept = call.keep
         if (key is not None and rows[0] is q and rows[1] is k and rows[2] is v and cu is q_meta.cu_seqlens
-                and (context is None or (context[0] is entry.k_cache and context[1] is entry.v_cache
-                                         and context[2] is entry.cu_seqlens_kv))):
+                and (kept is None or (kept[0] is entry.k_cache and kept[1] is entry.v_cache
+                                      and kept[2] is entry.cu_seqlens_kv))):
             if len(q_meta.launch_memo) >= _MEMO_MAX:
                 q_meta.launch_memo.clear()
             # the entry's tensors are held by the entry alone, as in the other memos
@@ -347,6 +350,4 @@ def flash_attn_mlm_window(
         out = _Window.apply(call, q, k, v)
         keep_leaves(leaves)
         return out
-    if entry is not None and torch.is_grad_enabled() and entry.k_cache.requires_grad:
-        raise ValueError("flash_attn_mlm_window has no gradient of a cached context; call it under torch.no_grad()")
     return call.run(*rows)

@@ -150,6 +150,32 @@ def test_contexts_without_a_page_to_read(kind, pages, width):
     assert _lib.load().fmlm_window_workspace_bytes(p, w) == 0
 
 
+@pytest.mark.parametrize("which", [0, 1])
+def test_gradients_and_tangents_of_a_context_are_refused(which):
+    """Of keys or of values: the call would drop them without a word."""
+    import torch.autograd.forward_ad as fwd
+
+    q, meta = torch.zeros((2, 2, 2, 64), dtype=torch.bfloat16), _cpu_meta([2, 1], 2)
+    rows = [torch.zeros((2 * 6, 64), dtype=torch.bfloat16) for _ in range(2)]
+    cache = InferenceCache()
+
+    def run():
+        cache.prefill_kv_cache(0, k_cache=rows[0], v_cache=rows[1], total_context_len=6,
+                               cu_seqlens_kv=torch.tensor([0, 2, 6], dtype=torch.int32), context_batch_size=2,
+                               is_mla=False, num_heads=2, head_dim=64)
+        flash_attn_mlm_window(q, q, q, 2, meta, 1.0, inference_cache=cache, layer_id=0)
+
+    plain, rows[which] = rows[which], rows[which].clone().requires_grad_()
+    with pytest.raises(ValueError, match="no gradient of a cached context"):
+        run()
+    with torch.no_grad(), pytest.raises(ValueError, match="must be CUDA tensors"):
+        run()
+    with fwd.dual_level():
+        rows[which] = fwd.make_dual(plain, torch.ones_like(plain))
+        with pytest.raises(ValueError, match="no forward-mode"):
+            run()
+
+
 def test_offsets_of_a_context_on_another_device_are_refused():
     """A packed entry keeps the offsets that it was given: their host address must not reach the kernel."""
     from flash_mlm.host.window import _context
