@@ -65,14 +65,22 @@ class _Call:
         return out
 
 
+_MAX_PITCH = 1 << 22  # elements from row to row: a tile's byte offsets are 32 bits in the kernels
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    return rows16(t) if t.ndim == 4 else aligned16(t)
+    if t.ndim != 4:
+        return aligned16(t)
+    if t.stride(2) >= _MAX_PITCH and t.shape[2] > 1:
+        return t.clone(memory_format=torch.contiguous_format)
+    return rows16(t)
 
 
 def _strides(t: torch.Tensor, tokens: int):
     """Element strides (batch, head, position) of padded rows [B, H, N, D] or packed ones [H * T, D]."""
     if t.ndim == 4:
-        return t.stride()[:3]
+        sb, sh, sn, _ = t.stride()
+        return sb, sh, sn if t.shape[2] > 1 else t.shape[3]  # (of a single row: any)
     return 0, tokens * int(t.shape[1]), int(t.shape[1])
 
 

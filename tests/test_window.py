@@ -150,6 +150,17 @@ def test_contexts_without_a_page_to_read(kind, pages, width):
     assert _lib.load().fmlm_window_workspace_bytes(p, w) == 0
 
 
+def test_rows_far_apart_are_copied():
+    """Positions 2^22 elements apart and more are outside the kernels' tile offsets; a single row has no pitch."""
+    from flash_mlm.host.window import _rows, _strides
+
+    make = lambda n, pitch: torch.empty_strided((2, 3, n, 64), (192, 64, pitch, 1), dtype=torch.bfloat16, device="meta")  # noqa: E731
+    near, far, one = make(5, (1 << 22) - 8), make(5, 1 << 22), make(1, 1 << 40)
+    assert _rows(near) is near and _strides(near, 0) == (192, 64, (1 << 22) - 8)
+    assert _rows(far).is_contiguous() and _strides(_rows(far), 0) == (3 * 5 * 64, 5 * 64, 64)
+    assert _rows(one) is one and _strides(one, 0) == (192, 64, 64)
+
+
 @pytest.mark.parametrize("which", [0, 1])
 def test_gradients_and_tangents_of_a_context_are_refused(which):
     """Of keys or of values: the call would drop them without a word."""
@@ -520,6 +531,23 @@ def test_strides_and_packed_rows(device):
     assert torch.equal(run(*flat), want)
     one = [x[:, :1].expand(-1, H, -1, -1) for x in (q, k, v)]
     assert torch.equal(run(*one), run(*(x.contiguous() for x in one)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [1, 3])
+def test_positions_far_apart(device, N):
+    """Rows whose positions are 2^22 elements apart, as in a [N, B, H, D] batch of many sequences"""
+    lens, H, D = [N, 1], 2, 64
+    g, q, k, v, meta = _inputs(device, "bf16", lens, N, H, D, 18)
+    far = [torch.empty_strided(q.shape, (H * D, D, 1 << 22, 1), dtype=q.dtype, device=device).copy_(x) for x in (q, k, v)]
+    run = lambda a: flash_attn_mlm_window(*a, H, meta, 0.125, window=(9, 2), sinks=1)  # noqa: E731
+    assert torch.equal(run(far), run((q, k, v)))
+    do = _rand(g, (H * sum(lens), D), q.dtype)
+    grads = []
+    for xs in (far, (q, k, v)):
+        xs = [x.detach().requires_grad_() for x in xs]
+        grads.append(torch.autograd.grad(run(xs), xs, do))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
 
 
 @pytest.mark.gpu
