@@ -92,12 +92,15 @@ FMLM_DEV WinTiles win_tiles(const WinArgs& a, const WinSeq& s, int p0, int p1, i
 FMLM_DEV int win_parts(int n, int parts) { return max(1, min(parts, n / kMinPartTiles)); }
 
 // the work of a workgroup: part, (sequence, head) group, tile; groups vary fastest and keep to one
-// XCD (workgroup w runs on XCD w % 8), so that neighbouring tiles share its L2
-FMLM_DEV void win_unit(const WinArgs& a, int parts, int& g, int& part, int& tile) {
-  const uint32_t w = blockIdx.x, r = w / (uint32_t)a.groups;
+// XCD (workgroup w runs on XCD w % 8), so that neighbouring tiles share its L2.  Returns whether there is any.
+// (A launch has fewer than 2^32 threads in x: kGridX workgroups there, and z of them.)
+constexpr uint32_t kGridX = 1u << 23;
+FMLM_DEV bool win_unit(const fmlm_attn_params& p, const WinArgs& a, int parts, int& g, int& part, int& tile) {
+  const uint32_t w = blockIdx.x + blockIdx.z * kGridX, r = w / (uint32_t)a.groups;
   g = (int)(w - r * (uint32_t)a.groups);
   tile = (int)(r / (uint32_t)parts);
   part = (int)(r - (uint32_t)tile * (uint32_t)parts);
+  return g < p.B * p.H && tile < a.tiles;
 }
 
 // ---- which of a lane's elements are in view, as bits: element (block b, r) is bit 16 b + r, b < 4, r < 4.
@@ -240,8 +243,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
   auto vbuf = [&](int v) { return smem + (2 + v % C::NV) * C::TILEB; };
 
   int g, part, tile;
-  win_unit(a, a.parts, g, part, tile);
-  if (g >= p.B * p.H) return;
+  if (!win_unit(p, a, a.parts, g, part, tile)) return;
   tile = a.tiles - 1 - tile;  // the last rows see the most
   const WinSeq s = win_seq(p, a, g / p.H, g % p.H);
   const int row0 = tile * BQ, rows = min(BQ, s.len - row0);
@@ -791,8 +793,7 @@ __global__ __launch_bounds__(kNW * 64, FewCfg<D>::WPS) void window_fp4_few_kerne
   typedef typename Mfma<T>::v8 v8;
   extern __shared__ __align__(16) char smem[];
   int g, part, tile;
-  win_unit(a, a.parts, g, part, tile);
-  if (g >= p.B * p.H) return;
+  if (!win_unit(p, a, a.parts, g, part, tile)) return;
   const WinSeq s = win_seq(p, a, g / p.H, g % p.H);
   const int rows = min(kFewRows, s.len);
   if (rows <= 0) return;
@@ -1081,8 +1082,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const fmlm_attn_param
   __shared__ __align__(16) float sums[GG][RR][D];
   __shared__ float stat[GG][RR][2];
   int g, part, tile;
-  win_unit(a, 1, g, part, tile);
-  if (g >= p.B * p.H) return;
+  if (!win_unit(p, a, 1, g, part, tile)) return;
   tile = a.tiles - 1 - tile;
   const WinSeq s = win_seq(p, a, g / p.H, g % p.H);
   const int row0 = tile * bq, rows = min(bq, s.len - row0);
@@ -1202,8 +1202,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
   auto kbuf = [&](int i) { return smem + i * C::TILEB; };
   auto vbuf = [&](int i) { return smem + (2 + i) * C::TILEB; };
   int g, part, tile;
-  win_unit(a, 1, g, part, tile);
-  if (g >= p.B * p.H) return;
+  if (!win_unit(p, a, 1, g, part, tile)) return;
   tile = a.tiles - 1 - tile;
   const WinSeq s = win_seq(p, a, g / p.H, g % p.H);
   const int row0 = tile * C::BQ, rows = min(C::BQ, s.len - row0);
@@ -1380,8 +1379,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dkv_kernel(const fmlm_attn
   auto obuf = [&](int i) { return smem + i * C::SB + C::STEPB; };
   auto stat = [&](int i) { return (float*)(smem + i * C::SB + 2 * C::STEPB); };
   int g, part, tile;
-  win_unit(a, 1, g, part, tile);
-  if (g >= p.B * p.H) return;
+  if (!win_unit(p, a, 1, g, part, tile)) return;
   const WinSeq s = win_seq(p, a, g / p.H, g % p.H);
   const int j0 = tile * kBK;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1544,6 +1542,10 @@ int allow_lds(const void* fn, int bytes, std::atomic<uint64_t>& done) {
   if (e != hipSuccess) return (int)e;
   if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
   return 0;
+}
+
+dim3 grid_of(int64_t blocks, unsigned y = 1) {  // win_unit's
+  return dim3((unsigned)std::min<int64_t>(blocks, kGridX), y, (unsigned)((blocks + kGridX - 1) / kGridX));
 }
 
 int longest(const fmlm_attn_params& p) { return p.N > 0 && p.N < p.total_q ? p.N : p.total_q; }
@@ -1727,8 +1729,8 @@ int launch_bwd(const fmlm_attn_params& p, const fmlm_window& w, const fmlm_attn_
   int rc = allow_lds(dq, C::DQ_LDS, allowed[0]);
   if (!rc) rc = allow_lds(dkv, C::DKV_LDS, allowed[1]);
   if (rc) return rc;
-  hipLaunchKernelGGL((window_dq_kernel<T, D>), dim3((unsigned)(a.tiles * a.groups)), dim3(kNW * 64), C::DQ_LDS, s, p, a, g);
-  hipLaunchKernelGGL((window_dkv_kernel<T, D>), dim3((unsigned)(b.tiles * b.groups)), dim3(kNW * 64), C::DKV_LDS, s, p, b, g);
+  hipLaunchKernelGGL((window_dq_kernel<T, D>), grid_of((int64_t)a.tiles * a.groups), dim3(kNW * 64), C::DQ_LDS, s, p, a, g);
+  hipLaunchKernelGGL((window_dkv_kernel<T, D>), grid_of((int64_t)b.tiles * b.groups), dim3(kNW * 64), C::DKV_LDS, s, p, b, g);
   return launch_status();
 }
 template <typename T>
@@ -1778,7 +1780,7 @@ extern "C" int fmlm_window_fwd(const fmlm_attn_params* pp, const fmlm_window* ww
   if (rc) return rc;
   hipStream_t s = (hipStream_t)stream;
   void* args[2] = {&p, &a};
-  hipError_t e = hipLaunchKernel(f.fn, dim3((unsigned)blocks), dim3(kNW * 64), args, f.lds, s);
+  hipError_t e = hipLaunchKernel(f.fn, grid_of(blocks), dim3(kNW * 64), args, f.lds, s);
   if (e != hipSuccess) return (int)e;
   if (a.parts > 1) {
     int bq = f.bq;
@@ -1786,8 +1788,8 @@ extern "C" int fmlm_window_fwd(const fmlm_attn_params* pp, const fmlm_window* ww
     // few rows: a workgroup each, its threads share the parts
     const bool wide = a.rec_rows > 4;
     const int per = wide ? f.merge_rows : 1;
-    e = hipLaunchKernel(f.merge[wide], dim3((unsigned)(a.tiles * a.groups), (a.rec_rows + per - 1) / per), dim3(256), margs,
-                        0, s);
+    e = hipLaunchKernel(f.merge[wide], grid_of((int64_t)a.tiles * a.groups, (a.rec_rows + per - 1) / per), dim3(256), margs, 0,
+                        s);
     if (e != hipSuccess) return (int)e;
   }
   return launch_status();

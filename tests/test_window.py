@@ -534,6 +534,33 @@ def test_strides_and_packed_rows(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fp4", [False, True])
+def test_more_workgroups_than_a_grid_has_in_x(device, fp4):
+    """2^24 and more (sequence, head) pairs: 2^32 threads.  A single token sees itself alone: its output is its
+    value and dv the output's gradient, bit for bit."""
+    B, H, D = 65537, 256, 32
+    g = torch.Generator(device=device).manual_seed(19)
+    meta = build_pack_metadata(torch.ones(B, dtype=torch.int32, device=device), 1, 32)
+    q, k, v = (torch.randn((B, H, 1, D), generator=g, device=device, dtype=torch.bfloat16) for _ in range(3))
+    heads_first = lambda x: x[:, :, 0].transpose(0, 1).reshape(H * B, D)  # noqa: E731
+    if fp4:  # over an empty context
+        pool = lambda cols: torch.zeros((H, 1, PAGE, cols), dtype=torch.uint8, device=device)  # noqa: E731
+        cache = InferenceCache()
+        cache.prefill_paged_fp4_cache(0, k_pages=pool(16), v_pages=pool(16), k_scales=pool(1), v_scales=pool(1),
+                                      block_table=torch.zeros((1, 1), dtype=torch.int32), context_lens=torch.zeros(1, dtype=torch.int32),
+                                      num_heads=H, head_dim=D, dtype=q.dtype)
+        out = fm.flash_attn_mlm_compressed(q, k, v, H, meta, 0.3, cache, 0)
+        assert torch.equal(out, heads_first(v))
+        return
+    v.requires_grad_()
+    out = flash_attn_mlm_window(q, k, v, H, meta, 0.3, window=(3, 0))
+    assert torch.equal(out, heads_first(v))
+    do = torch.randn(out.shape, generator=g, device=device, dtype=out.dtype)
+    dv, = torch.autograd.grad(out, v, do)
+    assert torch.equal(heads_first(dv), do)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("N", [1, 3])
 def test_positions_far_apart(device, N):
     """Rows whose positions are 2^22 elements apart, as in a [N, B, H, D] batch of many sequences"""
