@@ -107,15 +107,17 @@ FMLM_DEV uint32_t fp4_encode(float (&x)[8], uint32_t& scale_byte) {
   return c;
 }
 
-// blockIdx.y: chunk of `heads` heads, z: q, k, v.  Rows: padded ones b * N + pos, or packed tokens
+// blockIdx.y: chunk of `heads` heads, z: q, k, v, and slices of kRaGridX workgroups (a launch has fewer than 2^32
+// threads in x).  Rows: padded ones b * N + pos, or packed tokens
+constexpr unsigned kRaGridX = 1u << 23;
 template <typename T, bool FP4>
 __global__ __launch_bounds__(kRaThreads) void rotate_append_kernel(const RaParams p, int lpr_log2, int heads) {
   constexpr int NH = FP4 ? kRaHeads4 : kRaHeads;
-  const int which = blockIdx.z;
+  const int which = blockIdx.z % 3;
   const fmlm_append_rows& a = which == 0 ? p.q : which == 1 ? p.k : p.v;
   if (!a.dst) return;
   const bool padded = p.layout == FMLM_LAYOUT_PADDED;
-  const int64_t at = (int64_t)blockIdx.x * kRaThreads + threadIdx.x;
+  const int64_t at = ((int64_t)(blockIdx.z / 3) * kRaGridX + blockIdx.x) * kRaThreads + threadIdx.x;
   const int64_t row = at >> lpr_log2;
   if (row >= (padded ? (int64_t)p.B * p.N : p.T)) return;
   const int d = (int)(at - (row << lpr_log2)) * 8;
@@ -297,7 +299,8 @@ extern "C" int fmlm_rotate_append(const fmlm_append_params* pp, void* stream) {
   // heads, D = 128: 130 us with 4 heads a thread, 116 with 16); few: all the threads there are (64
   // rows of 16 heads 5.1 us, with 16 heads a thread 8.5)
   const int heads = rows * lpr >= kRaManyThreads ? kRaMany : kRaHeads;
-  const dim3 grid((unsigned)blocks, (p.H + heads - 1) / heads, 3);
+  const dim3 grid((unsigned)std::min<int64_t>(blocks, kRaGridX), (p.H + heads - 1) / heads,
+                  3 * (unsigned)((blocks + kRaGridX - 1) / kRaGridX));
   hipStream_t s = (hipStream_t)stream;
   const bool fp4 = p.flags & FMLM_AP_FP4;
   if (p.dtype == FMLM_DTYPE_BF16) {

@@ -582,6 +582,36 @@ def test_metadata_that_contradicts_itself_stays_in_bounds(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fp4", [False, True])
+def test_more_threads_than_a_grid_has_in_x(device, fp4):
+    """A padded batch of 2^27 positions and more with 256 dims a row: 2^32 threads.  (Rows of one address; the only
+    tokens are the first and last ones.)"""
+    N, B, H, D = (1 << 16) + 8, 1 << 11, 1, 256
+    lens = [1] + [0] * (B - 2) + [N]
+    meta = build_pack_metadata(torch.tensor(lens, device=device), N, 32)
+    T, P = N + 1, (N + 1 + PAGE - 1) // PAGE
+    g = torch.Generator(device=device).manual_seed(4)
+    x = torch.randn((1, 1, 1, D), generator=g, device=device).bfloat16()
+    k = x.expand(B, H, N, D)
+    cache, table = InferenceCache(), torch.zeros((B, 1), dtype=torch.int32, device=device)
+    index = dict(block_table=table, context_lens=torch.zeros(B, dtype=torch.int32), num_heads=H, head_dim=D)
+    if fp4:
+        pools = _fp4_pools(H, P, D, device)
+        cache.prefill_paged_fp4_cache(0, **pools, dtype=x.dtype, **index)
+    else:
+        pools = {n: torch.zeros((H, P, PAGE, D), dtype=x.dtype, device=device) for n in ("k_pages", "v_pages")}
+        cache.prefill_paged_kv_cache(0, **pools, is_mla=False, **index)
+    plan = PagedMetadata(table, torch.arange(T, device=device), torch.zeros(T, dtype=torch.int32, device=device),
+                         torch.zeros(B, dtype=torch.int32, device=device), torch.zeros(B + 1, dtype=torch.int32, device=device))
+    cos = torch.ones((1, D // 2), device=device)  # (position 0: as they are)
+    cache.append_paged_kv_cache(0, k=k, v=k, q_meta=meta, plan=plan, cos=cos, sin=torch.zeros_like(cos))
+    want = torch.from_numpy(ref.fp4_values(*ref.fp4_encode(_f64(x), "bf16"))).to(device) if fp4 else x.double()
+    for pages in cache.paged_kv_values(0):
+        rows = pages.view(-1, D).double()
+        assert torch.equal(rows[:T], want.view(1, D).expand(T, D)) and not rows[T:].any()
+
+
+@pytest.mark.gpu
 def test_pools_past_32_bits(device):
     """Rows behind element 2^32 of a pool: stored, read back and attended to"""
     H, D, P = 2, 256, 135000  # 2 * 135000 * 64 * 256 = 4.4e9 elements
