@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "fmlm_fp4.h"
@@ -1652,6 +1653,7 @@ int check_window(const fmlm_attn_params& p, const fmlm_window& w) {
   if (p.B < 0 || p.H < 0 || p.N < 0 || p.total_q < 0 || p.total_q >= kNoLimit) return FMLM_E_ARG;
   if (p.B == 0 || p.H == 0 || p.total_q == 0) return 0;
   if (!p.cu_seqlens_q || (int64_t)p.B * p.H > 0x7fffff00) return FMLM_E_ARG;
+  if (!std::isfinite(p.scale)) return FMLM_E_ARG;  // (a mask is a score of -inf times it)
   const bool appended = w.flags & FMLM_WINDOW_APPENDED, fp4 = w.flags & FMLM_WINDOW_FP4;
   const bool ctx = p.cu_seqlens_kv || p.ctx_block_table || p.ctx_len > 0;
   if (!ctx && (appended || fp4)) return FMLM_E_ARG;

@@ -4,6 +4,7 @@ reference's queries see all keys."""
 
 from __future__ import annotations
 
+import math
 import weakref
 
 import torch
@@ -139,6 +140,8 @@ def _build(q, k, v, num_heads: int, q_meta: PackMetadata, scale, left, right, si
         raise ValueError("window attention needs bf16 or fp16 inputs")
     if d not in _HEAD_DIMS:
         raise ValueError("window attention needs head_dim 32, 64, 128 or 256")
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
     if k is not None and (k.dtype != q.dtype or v.dtype != q.dtype):
         raise ValueError("q, k and v must have the same dtype")
     if k is not None and (k.device != dev or v.device != dev):

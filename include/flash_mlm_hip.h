@@ -522,7 +522,7 @@ FMLM_API int fmlm_attn_tree_fwd(const fmlm_attn_params* p, const uint64_t* mask,
  *   j <= s + right  and  (j >= s - left  or  j < sinks).
  * left, right < 0: no limit.  A row that sees no key has output 0.
  *
- * p: bf16 or fp16, D = 32, 64, 128 or 256, flags 0, packed sequences (cu_seqlens_q); q, k and v
+ * p: bf16 or fp16, D = 32, 64, 128 or 256, a finite scale, flags 0, packed sequences (cu_seqlens_q); q, k and v
  * padded or packed, the output packed or padded; main keys linear; the context packed
  * (cu_seqlens_kv), paged, or none (cu_seqlens_kv NULL, ctx_len 0); ctx_index as there.  p->schedule
  * and tile_config are not used.

@@ -161,6 +161,20 @@ def test_rows_far_apart_are_copied():
     assert _rows(one) is one and _strides(one, 0) == (192, 64, 64)
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf")])
+def test_scales_that_are_not_finite_are_refused(scale):
+    """Masked scores are -inf times the scale."""
+    q = torch.zeros((2, 2, 2, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="scale must be finite"):
+        flash_attn_mlm_window(q, q, q, 2, _cpu_meta([2, 1], 2), scale)
+    p, w = _lib.AttnParams(), _lib.Window()
+    p.dtype, p.B, p.H, p.D, p.N, p.total_q, p.cu_seqlens_q = _lib.DTYPE_BF16, 1, 1, 64, 4, 4, 256
+    p.q = p.o = p.k = p.v = 256
+    assert _lib.load().fmlm_window_workspace_bytes(p, w) == 0
+    p.scale = scale
+    assert _lib.load().fmlm_window_workspace_bytes(p, w) == -1 and _lib.load().fmlm_window_fwd(p, w, None) == -1
+
+
 @pytest.mark.parametrize("which", [0, 1])
 def test_gradients_and_tangents_of_a_context_are_refused(which):
     """Of keys or of values: the call would drop them without a word."""
