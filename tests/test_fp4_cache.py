@@ -414,6 +414,50 @@ def test_rotated_append_into_sixteen_bits(device, shape, dtype, interleaved):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fp4", [False, True])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("H,packed,dtype", [(5, False, "bf16"), (17, False, "fp16"), (20, True, "bf16")])
+def test_appends_of_many_rows(device, H, packed, dtype, interleaved, fp4):
+    """Calls whose threads take 16 heads each: the bits of appends of a few hundred rows at a time, whose threads take
+    four (the tests above are of those), and a sample of them against the oracle"""
+    lens, N, D, R = [2900, 0, 2001, 700], 2900, 256, 96
+    meta, q, k, v, cache, pools, plan, slots = _case(device, dtype, lens, N, H, D, fp4, packed, spread=False)
+    T, B = sum(lens), len(lens)
+    assert (T if packed else B * N) * D // 8 >= 256 * 2048 // 3 > 600 * D // 8
+    cos, sin = _tables(D, R, device)
+    start = {n: x.clone() for n, x in pools.items()}
+    got_q = cache.append_paged_kv_cache(0, k=k, v=v, q_meta=meta, plan=plan, q=q, cos=cos, sin=sin, interleaved=interleaved)
+    got = {n: x.clone() for n, x in pools.items()}
+    for n, x in pools.items():
+        x.copy_(start[n])
+    flat = [x.view(H, T, D) if packed else torch.cat([x[b, :, :n] for b, n in enumerate(lens)], 1) for x in (q, k, v, got_q)]
+    zero = torch.zeros(1, dtype=torch.int32, device=device)
+    for at in range(0, T, 600):
+        n = min(600, T - at)
+        piece = PagedMetadata(plan.block_table[:1], plan.slot_mapping[at:at + n].contiguous(),
+                              plan.positions[at:at + n].contiguous(), zero, torch.zeros(2, dtype=torch.int32, device=device))
+        qq, kk, vv, want_q = (x[:, at:at + n].reshape(H * n, D) for x in flat)
+        out = cache.append_paged_kv_cache(0, k=kk, v=vv, q_meta=build_pack_metadata(torch.tensor([n], device=device), n, 32),
+                                          plan=piece, q=qq, cos=cos, sin=sin, interleaved=interleaved)
+        assert torch.equal(out, want_q)
+    assert all(torch.equal(x, got[n]) for n, x in pools.items())
+    if not packed:
+        for b, n in enumerate(lens):
+            assert not got_q[b, :, n:].any()
+    some = random.Random(1).sample([t for t in range(T) if 0 <= slots[t] < pools["k_pages"].shape[1] * PAGE], 200)
+    pos = plan.positions.cpu().numpy()[some]
+    kk = ref.rotate(_f64(flat[1][:, some]), _f64(cos)[pos], _f64(sin)[pos], interleaved)
+    for name, x in (("k", kk), ("v", _f64(flat[2][:, some]))):
+        rows = lambda n: got[name + n].view(H, -1, got[name + n].shape[-1])[:, [slots[t] for t in some]].cpu()  # noqa: B023,E731
+        if fp4:
+            codes, scales = ref.fp4_encode(x, dtype)
+            assert (rows("_pages").numpy() == codes).all() and (rows("_scales").numpy() == scales).all()
+        else:
+            tol = np.abs(x) * torch.finfo(TYPES[dtype]).eps / 2 + (np.abs(x).max() * 2.0**-21 + 2.0**-25 if name == "k" else 0)
+            assert (np.abs(_f64(rows("_pages")) - x) <= tol).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_values_that_are_not_finite(device, dtype):
     """Infinities as the largest value, NaN as 0, zeros, the smallest and the largest values"""

@@ -432,6 +432,81 @@ def test_contexts(device, kind, dtype, D, appended, window, sinks):
     _check(out, q, k, v, lens, ctx, layer, window, sinks, -0.15, dtype, appended)
 
 
+def _kept_bytes(meta):
+    """Bytes of the split's records of the one kept call of ``meta``"""
+    call, = meta.launch_memo.values()
+    return call.nbytes
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("appended", [False, True])
+@pytest.mark.parametrize("window,sinks", [((None, None), 0), ((1500, 0), 4)], ids=str)
+@pytest.mark.parametrize("N", [1, 4, 5, 16])
+@pytest.mark.parametrize("kind,dtype,D", [("fp4", "bf16", 32), ("fp4", "fp16", 64), ("fp4", "bf16", 128), ("fp4", "fp16", 256),
+                                          ("paged", "fp16", 64), ("packed", "bf16", 128), ("paged", "bf16", 256)])
+def test_few_rows_whose_key_ranges_are_split(device, kind, dtype, D, N, window, sinks, appended):
+    """Long contexts with partial last pages beside a short one, which stays whole in the same call"""
+    lens, H, ctx = [N, 1, max(N - 2, 1)], 2, [2500, 130, 2111]
+    g, q, k, v, meta = _inputs(device, dtype, lens, N, H, D, 41)
+    layer = _Layer(kind, dtype, H, D, ctx, device, g)
+    kv = (None, None) if appended else (k, v)
+    out = flash_attn_mlm_window(q, *kv, H, meta, 0.15, window=window, sinks=sinks, inference_cache=layer.cache, layer_id=0)
+    assert _kept_bytes(meta) > 0
+    _check(out, q, k, v, lens, ctx, layer, window, sinks, 0.15, dtype, appended)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp4", "paged"])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("N", [1, 6])
+def test_the_most_parts(device, kind, D, N):
+    """One sequence over 20 thousand keys: 32 parts, joined by one and by several rows a workgroup"""
+    lens, H, ctx = [N], 1, [20001]
+    g, q, k, v, meta = _inputs(device, "bf16", lens, N, H, D, 42)
+    layer = _Layer(kind, "bf16", H, D, ctx, device, g)
+    out = flash_attn_mlm_window(q, k, v, H, meta, 0.15, inference_cache=layer.cache, layer_id=0)
+    assert _kept_bytes(meta) == 32 * 8 * N * (D + 4) * 4  # (8: pairs are counted in eights)
+    _check(out, q, k, v, lens, ctx, layer, (None, None), 0, 0.15, "bf16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [1, 16])
+def test_few_rows_whose_key_ranges_stay_whole(device, N):
+    lens, H, D, ctx = [N, 1], 2, 64, [400, 3]
+    g, q, k, v, meta = _inputs(device, "bf16", lens, N, H, D, 43)
+    layer = _Layer("fp4", "bf16", H, D, ctx, device, g)
+    out = flash_attn_mlm_window(q, k, v, H, meta, 0.15, inference_cache=layer.cache, layer_id=0)
+    assert _kept_bytes(meta) == 0
+    _check(out, q, k, v, lens, ctx, layer, (None, None), 0, 0.15, "bf16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("appended", [False, True])
+@pytest.mark.parametrize("kind", ["packed", "paged", "fp4"])
+@pytest.mark.parametrize("lens", [[3, 1, 0, 5], [16, 2, 9, 16], [200, 40, 0, 1]], ids=str)
+@pytest.mark.parametrize("D", [64, 128])
+def test_layouts_beside_a_context(device, kind, lens, appended, D):
+    """Packed rows, rows of other strides and unaligned ones: the same bits as contiguous padded ones"""
+    N, H, ctx = max(lens), 3, [300, 64, 7, 129]
+    g, q, k, v, meta = _inputs(device, "fp16", lens, N, H, D, 44)
+    layer = _Layer(kind, "fp16", H, D, ctx, device, g)
+    run = lambda q, k, v: flash_attn_mlm_window(q, *((None, None) if appended else (k, v)), H, meta, 0.1, window=(120, 3),  # noqa: E731
+                                                sinks=5, inference_cache=layer.cache, layer_id=0)
+    want = run(q, k, v)
+    _check(want, q, k, v, lens, ctx, layer, (120, 3), 5, 0.1, "fp16", appended)
+    flat = [torch.cat([x[b, :, :n] for b, n in enumerate(lens)], 1).reshape(-1, D) for x in (q, k, v)]
+    assert torch.equal(run(*flat), want)
+    wide = torch.zeros((len(lens), N, 3, H, D + 8), dtype=q.dtype, device=device)
+    parts = [wide[:, :, i, :, :D].transpose(1, 2) for i in range(3)]
+    odd = [torch.zeros(q.numel() + 1, dtype=q.dtype, device=device)[1:].view(q.shape) for _ in range(3)]
+    for dst in (parts, odd):
+        for x, y in zip(dst, (q, k, v)):
+            x.copy_(y)
+        assert torch.equal(run(*dst), want)
+    one = [x[:, :1].expand(-1, H, -1, -1) for x in (q, k, v)]
+    assert torch.equal(run(*one), run(*(x.contiguous() for x in one)))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("window,sinks", WINDOWS[1:5], ids=str)
 @pytest.mark.parametrize("kind", ["packed", "paged", "fp4"])
@@ -777,6 +852,71 @@ def test_scores_of_infinite_size(device):
     # scores to 620: fp32 sums are off by at most 64 2^-24 of the sum of the products' sizes, about 620
     size = P @ np.abs(vv)
     assert (np.abs(_f64(out) - o) <= (3 * _half("bf16") + 2 * 64 * 2.0**-24 * 650) * size).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["paged", "fp4", None])
+def test_padded_outputs_and_whole_key_ranges(device, kind):
+    """The C entry point with what the Python one does not ask for: a padded output, whose padding rows stay as they
+    were, and key ranges that are not split"""
+    from flash_mlm.host.window import _build
+
+    lens, N, H, D = [3, 0, 5], 6, 2, 64
+    ctx = [2500, 0, 300] if kind else None
+    g, q, k, v, meta = _inputs(device, "bf16", lens, N, H, D, 45)
+    layer = _Layer(kind, "bf16", H, D, ctx, device, g) if kind else None
+    call, _rows = _build(q, k, v, H, meta, 0.15, 40, 2, 3, layer.cache.layer_entry(0) if kind else None, None)
+    assert call.nbytes == 0  # a short window
+    call, _rows = _build(q, k, v, H, meta, 0.15, -1, -1, 0, layer.cache.layer_entry(0) if kind else None, None)
+    assert (call.nbytes > 0) == (kind is not None)
+    p, lib = call.params, _lib.load()
+    out = torch.full((len(lens), H, N, D), 7.0, dtype=q.dtype, device=device)
+    p.q, p.k, p.v, p.o = (x.data_ptr() for x in (q, k, v, out))
+    p.o_layout, p.o_sb, p.o_sh, p.o_sn = _lib.LAYOUT_PADDED, H * N * D, N * D, D
+    ws = torch.empty(max(call.nbytes, 16), dtype=torch.uint8, device=device)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), call.nbytes
+    for flags in (0, _lib.FLAG_NOSPLIT):
+        p.flags = flags
+        if flags:
+            assert lib.fmlm_window_workspace_bytes(p, call.window) == 0
+            p.workspace = None
+        out.fill_(7)
+        assert lib.fmlm_window_fwd(p, call.window, _lib.stream_of(device)) == 0
+        _check(torch.cat([out[b, :, :n] for b, n in enumerate(lens)], 1).reshape(-1, D), q, k, v, lens, ctx, layer,
+               (None, None), 0, 0.15, "bf16")
+        for b, n in enumerate(lens):
+            assert (out[b, :, n:] == 7).all()
+
+
+@pytest.mark.gpu
+def test_gradients_with_a_padded_output(device):
+    """The C entry points of a training call with o, o_low and dout padded: the bits of the packed ones"""
+    from flash_mlm.host.window import _build
+
+    lens, N, H, D = [70, 0, 9], 71, 2, 64
+    g, q, k, v, meta = _inputs(device, "fp16", lens, N, H, D, 46)
+    xs = [x.requires_grad_() for x in (q, k, v)]
+    packed = flash_attn_mlm_window(*xs, H, meta, 0.15, window=(20, 1), sinks=2)
+    do = _rand(g, packed.shape, q.dtype)
+    want = torch.autograd.grad(packed, xs, do)
+    call, _rows = _build(*(x.detach() for x in xs), H, meta, 0.15, 20, 1, 2, None, None)
+    p, w, gr, lib, stream = call.params, call.window, call.grads, _lib.load(), _lib.stream_of(device)
+    out, low, dout = (torch.zeros_like(q) for _ in range(3))
+    at = 0
+    for b, n in enumerate(lens):
+        dout[b, :, :n] = do.view(H, -1, D)[:, at:at + n]
+        at += n
+    lse, ws = torch.empty(H * at, device=device), torch.empty(H * at, device=device)
+    p.q, p.k, p.v, p.o, p.lse, w.o_low = (x.data_ptr() for x in (q, k, v, out, lse, low))
+    p.o_layout, p.o_sb, p.o_sh, p.o_sn = _lib.LAYOUT_PADDED, H * N * D, N * D, D
+    assert lib.fmlm_window_fwd(p, w, stream) == 0
+    assert torch.equal(torch.cat([out[b, :, :n] for b, n in enumerate(lens)], 1).reshape(-1, D), packed)
+    grads = [torch.full_like(q, 7.0) for _ in range(3)]
+    gr.dout, gr.workspace = dout.data_ptr(), ws.data_ptr()
+    gr.dq, gr.dk, gr.dv = (x.data_ptr() for x in grads)
+    gr.do_sb, gr.do_sh, gr.do_sn = H * N * D, N * D, D
+    assert lib.fmlm_window_bwd(p, w, gr, stream) == 0
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
 
 
 @pytest.mark.gpu
