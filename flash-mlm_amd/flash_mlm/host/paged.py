@@ -256,9 +256,9 @@ def rotate_append(entry, q, k, v, *, q_meta: PackMetadata, slots, cos, sin, posi
     # all that the checks below and the block depend on, but addresses (the caller has checked k, v and slots)
     key = ("append", _layout(q), _layout(k), _layout(v), _layout(cos), _layout(sin), _layout(positions), interleaved,
            entry.dtype, dev, h, d, entry.total_context_len, entry.k_scales is None)
-    if q is not None:
-        refuse_tangents("append_paged_kv_cache", q)
-        if q.requires_grad and torch.is_grad_enabled():
+    if q is not None:  # (what is stored has no gradient in any case; the output must not drop one)
+        refuse_tangents("append_paged_kv_cache", q, cos, sin)
+        if (q.requires_grad or cos.requires_grad or (sin is not None and sin.requires_grad)) and torch.is_grad_enabled():
             raise ValueError("the rotated q has no gradient; use qk_norm_rope, or call under torch.no_grad()")
     memo = q_meta.launch_memo
     m = memo.get(key)

@@ -198,6 +198,22 @@ def test_append_refusals(fp4):
             cache.append_paged_kv_cache(0, **{**args, "cos": cos, "sin": cos, **kw})
 
 
+@pytest.mark.parametrize("fp4", [False, True])
+def test_gradients_and_tangents_of_the_rotated_q_are_refused(fp4):
+    """Those of q and of the tables it is rotated by: the returned q would drop them without a word."""
+    import torch.autograd.forward_ad as fwd
+
+    cache, args, cos = _append_args(fp4=fp4)
+    args.update(q=args["k"], cos=cos, sin=cos)
+    for name in ("q", "cos", "sin"):
+        with pytest.raises(ValueError, match="the rotated q has no gradient"):
+            cache.append_paged_kv_cache(0, **{**args, name: args[name].clone().requires_grad_()})
+        with torch.no_grad(), pytest.raises(ValueError, match="no CPU compute path"):
+            cache.append_paged_kv_cache(0, **{**args, name: args[name].clone().requires_grad_()})
+        with fwd.dual_level(), pytest.raises(ValueError, match="no forward-mode"):
+            cache.append_paged_kv_cache(0, **{**args, name: fwd.make_dual(args[name], torch.ones_like(args[name]))})
+
+
 def test_rotating_append_checks():
     """What paged._tables refuses, without a GPU."""
     from flash_mlm.host.paged import _tables
