@@ -1095,6 +1095,36 @@ def test_gradients(device, dtype, D, packed, window, sinks):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0**-10, 2.0**9])
+@pytest.mark.parametrize("D", [32, 128])
+def test_gradients_of_small_and_large_losses_in_fp16(device, D, size):
+    """dS is an fp16 operand: its normal range holds losses scaled by hundreds either way"""
+    lens, N, H = [90, 33], 90, 2
+    g, q, k, v, meta = _inputs(device, "fp16", lens, N, H, D, 35)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = flash_attn_mlm_window(*leaves, H, meta, D**-0.5, window=(20, 3), sinks=2)
+    do = _rand(g, out.shape, torch.float32).mul_(size).to(out.dtype)
+    got = [_by_sequence(x, lens, H, D) for x in torch.autograd.grad(out, leaves, do)]
+    _grad_check(got, q, k, v, _f64(do).reshape(H, -1, D), lens, (20, 3), 2, D**-0.5, "fp16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1.5])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_gradients_with_other_scales(device, D, scale):
+    """Negative scales turn the masks' infinities round, 0 leaves dv alone"""
+    lens, N, H = [70, 0, 33], 70, 2
+    g, q, k, v, meta = _inputs(device, "bf16", lens, N, H, D, 34)
+    leaves = [(x if scale < 1 else x * 0.3).requires_grad_() for x in (q, k, v)]
+    q, k, v = leaves
+    out = flash_attn_mlm_window(*leaves, H, meta, scale, window=(20, 3), sinks=2)
+    _check(out, q, k, v, lens, None, None, (20, 3), 2, scale, "bf16")
+    do = _rand(g, out.shape, out.dtype)
+    got = [_by_sequence(x, lens, H, D) for x in torch.autograd.grad(out, leaves, do)]
+    _grad_check(got, q, k, v, _f64(do).reshape(H, -1, D), lens, (20, 3), 2, scale, "bf16")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 def test_gradients_of_keys_are_as_exact_as_their_operands(device, dtype):
     """dK's root mean square error is that of dS rounded to the type, and of its own rounding: delta brings no
