@@ -1166,7 +1166,8 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const fmlm_attn_param
 // the input type as operands, off by half a step each; delta comes from o and o_low in 32 bits, or
 // o's rounding, the same for all of a row's keys, would be the largest error of dq and dk (1.55 times
 // the plain form's in fp16, with o_low 1.4).  What is left in it of the rounding of the forward's P goes
-// for dK: the dq kernel adds up what each row's dS, unrounded, lacks to a sum of 0.  dq by query tiles, then dK and dV by key tiles, which repeats S
+// for dK: the dq kernel adds up what each row's dS, unrounded, lacks to a sum of 0.  dq itself has the delta that is
+// not yet so exact; where that counts (TWO: rows of few keys) its dS goes in two terms.  dq by query tiles, then dK and dV by key tiles, which repeats S
 // and dP (2 of 7 products) and needs no atomics: the same bits every time.
 //
 // Bound (fp16, 4 x 16 sequences of 2000 to 4096 rows of 128, windows of 1024): dq 217 us, 37% of the matrix
@@ -1193,7 +1194,7 @@ FMLM_DEV void zero_row4(void* base, int64_t elem) {
   *(u32x2*)((char*)base + elem * 2) = u32x2{0u, 0u};
 }
 
-template <typename T, int D>
+template <typename T, int D, bool TWO>
 __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_params p, const WinArgs a,
                                                                              const fmlm_attn_grads gr) {
   typedef BwdCfg<D> C;
@@ -1278,7 +1279,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
     // kb's P and dS are made beside block kb + 1's dP, the last one's beside the first dq slots.
     constexpr int NSS = NKB * C::KC, NR = 2 * NSS, NS = NR + NKS * C::NDB, LEAD = 3;
     f32x4 sc[NKB][QB], dp[NKB][QB];
-    u32x4 ds[NKS][QB];
+    u32x4 ds[NKS][QB], ds2[TWO ? NKS : 1][TWO ? QB : 1];
     v8 fr[LEAD + 1];
     auto read = [&](int r) {
       if (r < NSS) fr[r % (LEAD + 1)] = tr.row(kt, r % NKB, r / NKB);
@@ -1295,6 +1296,11 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
       uint32_t w = pack2<T>(x, y);
       pin(w);
       ds[kb >> 1][qb][(kb & 1) * 2 + (r >> 1)] = w;
+      if constexpr (TWO) {
+        uint32_t w2 = pack2<T>(x - (float)__builtin_bit_cast(T, (uint16_t)w), y - (float)__builtin_bit_cast(T, (uint16_t)(w >> 16)));
+        pin(w2);
+        ds2[kb >> 1][qb][(kb & 1) * 2 + (r >> 1)] = w2;
+      }
     };
 #pragma unroll
     for (int r = 0; r < LEAD; ++r) read(r);
@@ -1347,7 +1353,10 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
         for (int e = NKS == 1 ? 0 : j * 2 * QB / C::NDB; e < (NKS == 1 ? 2 * QB : (j + 1) * 2 * QB / C::NDB); ++e) soft(NKB - 1, e);
       }
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) dq[db][qb] = Mfma<T>::run(x, __builtin_bit_cast(v8, ds[ks][qb]), dq[db][qb]);
+      for (int qb = 0; qb < QB; ++qb) {
+        dq[db][qb] = Mfma<T>::run(x, __builtin_bit_cast(v8, ds[ks][qb]), dq[db][qb]);
+        if constexpr (TWO) dq[db][qb] = Mfma<T>::run(x, __builtin_bit_cast(v8, ds2[ks][qb]), dq[db][qb]);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
@@ -1718,6 +1727,18 @@ int64_t record_bytes(const fmlm_attn_params& p, const WinArgs& a) {
   return a.parts > 1 ? (int64_t)a.tiles * a.groups * a.parts * a.rec_rows * (p.D + 4) * 4 : 0;
 }
 
+// dS of the dq kernel in two terms of the type where a row sees few keys.  Three roundings are dq's error: its own, dS's,
+// and that of the forward's P in delta, which grows with the weight of single keys (e^2 = sum P^2 of dS's).  With one term
+// the error is 1.44 times that of dq's own rounding over hundreds of keys, 1.48 over 64 and 1.50 to 1.53 below 16; two
+// leave 1.04 to 1.14.  They cost a third of the products: the whole backward of 4 x 16 x 4096 rows of 128 takes 223 us
+// for 219 with windows of 9 keys, 247 : 239 with 128, but 299 : 289 with 257, 609 : 576 with 1025; 8 x 8 x 1024 rows of
+// 256 169 : 166 with 201, 218 : 210 with 511.
+constexpr int kTwoTermKeys = 256;
+// keys that a row of a call without a context sees at most
+int64_t row_keys(const fmlm_attn_params& p, const fmlm_window& w) {
+  return std::min<int64_t>(longest(p), (int64_t)limit(w.left) + limit(w.right) + 1 + std::max(w.sinks, 0));
+}
+
 template <typename T, int D>
 int launch_bwd(const fmlm_attn_params& p, const fmlm_window& w, const fmlm_attn_grads& g, hipStream_t s) {
   typedef BwdCfg<D> C;
@@ -1726,12 +1747,15 @@ int launch_bwd(const fmlm_attn_params& p, const fmlm_window& w, const fmlm_attn_
   if (p.N > 0 && p.q_layout == FMLM_LAYOUT_PADDED) a.tiles = (p.N + C::BQ - 1) / C::BQ;
   if (p.N > 0 && p.kv_layout == FMLM_LAYOUT_PADDED) b.tiles = (p.N + kBK - 1) / kBK;
   if ((int64_t)a.tiles * a.groups > 0x7fffffff || (int64_t)b.tiles * b.groups > 0x7fffffff) return FMLM_E_ARG;
-  const void *dq = (const void*)window_dq_kernel<T, D>, *dkv = (const void*)window_dkv_kernel<T, D>;
-  static std::atomic<uint64_t> allowed[2];
-  int rc = allow_lds(dq, C::DQ_LDS, allowed[0]);
-  if (!rc) rc = allow_lds(dkv, C::DKV_LDS, allowed[1]);
+  const bool two = row_keys(p, w) <= kTwoTermKeys;
+  const void *dq = two ? (const void*)window_dq_kernel<T, D, true> : (const void*)window_dq_kernel<T, D, false>;
+  const void* const dkv = (const void*)window_dkv_kernel<T, D>;
+  static std::atomic<uint64_t> allowed[3];
+  int rc = allow_lds(dq, C::DQ_LDS, allowed[two]);
+  if (!rc) rc = allow_lds(dkv, C::DKV_LDS, allowed[2]);
   if (rc) return rc;
-  hipLaunchKernelGGL((window_dq_kernel<T, D>), grid_of((int64_t)a.tiles * a.groups), dim3(kNW * 64), C::DQ_LDS, s, p, a, g);
+  if (two) hipLaunchKernelGGL((window_dq_kernel<T, D, true>), grid_of((int64_t)a.tiles * a.groups), dim3(kNW * 64), C::DQ_LDS, s, p, a, g);
+  else hipLaunchKernelGGL((window_dq_kernel<T, D, false>), grid_of((int64_t)a.tiles * a.groups), dim3(kNW * 64), C::DQ_LDS, s, p, a, g);
   hipLaunchKernelGGL((window_dkv_kernel<T, D>), grid_of((int64_t)b.tiles * b.groups), dim3(kNW * 64), C::DKV_LDS, s, p, b, g);
   return launch_status();
 }
