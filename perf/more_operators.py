@@ -353,7 +353,7 @@ def _own_append(s):
 
 def _own_attn(s):
     c = s["case"]
-    if c["left"] < 0 and c["right"] < 0 and not c["appended"]:
+    if c["kind"] == "fp4" and c["left"] < 0 and c["right"] < 0 and not c["appended"]:
         return s["fm"].flash_attn_mlm_compressed(s["q"], s["k"], s["v"], c["H"], s["meta"], s["scale"], s["cache"], 0)
     return s["fm"].flash_attn_mlm_window(s["q"], s["k"], s["v"], c["H"], s["meta"], s["scale"], window=_window(c),
                                          sinks=c["sinks"], inference_cache=s["cache"], layer_id=0)
