@@ -1194,7 +1194,20 @@ FMLM_DEV void zero_row4(void* base, int64_t elem) {
   *(u32x2*)((char*)base + elem * 2) = u32x2{0u, 0u};
 }
 
-template <typename T, int D, bool TWO>
+// dS in two terms of the type for the rows of a workgroup of which one sees few keys.  Three roundings are dq's error:
+// its own, dS's, and that of the forward's P in delta, which grows with the weight of single keys (sum P^2 of dS's square).
+// With one term the error is 1.44 times that of dq's own rounding over hundreds of keys, 1.48 over 64 and 1.50 to
+// 1.53 below 16; two leave 1.04 to 1.14.  They cost a third of the products: the whole backward of 4 x 16 x 4096 rows of
+// 128 takes 223 us for 220 with windows of 9 keys, 247 : 241 with 128, and would take 299 : 289 with 257, 609 : 576 with
+// 1025; 8 x 8 x 1024 rows of 256 169 : 167 with 201, and 218 : 211 with 511.
+constexpr int kTwoTermKeys = 256;
+// keys that the row at position r sees, of a call without a context
+FMLM_DEV int row_keys(const WinArgs& a, const WinSeq& s, int r) {
+  const int lo = max(0, r - a.left);
+  return min(s.len, r + a.right + 1) - lo + min(a.sinks, lo);
+}
+
+template <typename T, int D>
 __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_params p, const WinArgs a,
                                                                              const fmlm_attn_grads gr) {
   typedef BwdCfg<D> C;
@@ -1266,6 +1279,9 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
   for (int db = 0; db < C::NDB; ++db)
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) dq[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // (a workgroup's own loop for each, not a branch in it)
+  auto walk = [&](auto two) {
+  constexpr bool TWO = decltype(two)::value;
   for (int v = 0; v < wt.n; ++v) {
     const int t = wt.tile(v), buf = v & 1, nk = keys_in(t);
     __builtin_amdgcn_s_waitcnt(0);
@@ -1361,6 +1377,9 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_dq_kernel(const fmlm_attn_
     }
     __builtin_amdgcn_s_setprio(0);
   }
+  };
+  if (min(row_keys(a, s, row0), row_keys(a, s, row0 + rows - 1)) <= kTwoTermKeys) walk(std::true_type{});
+  else walk(std::false_type{});
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int row = (wave * QB + qb) * 16 + l16;
@@ -1727,18 +1746,6 @@ int64_t record_bytes(const fmlm_attn_params& p, const WinArgs& a) {
   return a.parts > 1 ? (int64_t)a.tiles * a.groups * a.parts * a.rec_rows * (p.D + 4) * 4 : 0;
 }
 
-// dS of the dq kernel in two terms of the type where a row sees few keys.  Three roundings are dq's error: its own, dS's,
-// and that of the forward's P in delta, which grows with the weight of single keys (e^2 = sum P^2 of dS's).  With one term
-// the error is 1.44 times that of dq's own rounding over hundreds of keys, 1.48 over 64 and 1.50 to 1.53 below 16; two
-// leave 1.04 to 1.14.  They cost a third of the products: the whole backward of 4 x 16 x 4096 rows of 128 takes 223 us
-// for 219 with windows of 9 keys, 247 : 239 with 128, but 299 : 289 with 257, 609 : 576 with 1025; 8 x 8 x 1024 rows of
-// 256 169 : 166 with 201, 218 : 210 with 511.
-constexpr int kTwoTermKeys = 256;
-// keys that a row of a call without a context sees at most
-int64_t row_keys(const fmlm_attn_params& p, const fmlm_window& w) {
-  return std::min<int64_t>(longest(p), (int64_t)limit(w.left) + limit(w.right) + 1 + std::max(w.sinks, 0));
-}
-
 template <typename T, int D>
 int launch_bwd(const fmlm_attn_params& p, const fmlm_window& w, const fmlm_attn_grads& g, hipStream_t s) {
   typedef BwdCfg<D> C;
@@ -1747,15 +1754,12 @@ int launch_bwd(const fmlm_attn_params& p, const fmlm_window& w, const fmlm_attn_
   if (p.N > 0 && p.q_layout == FMLM_LAYOUT_PADDED) a.tiles = (p.N + C::BQ - 1) / C::BQ;
   if (p.N > 0 && p.kv_layout == FMLM_LAYOUT_PADDED) b.tiles = (p.N + kBK - 1) / kBK;
   if ((int64_t)a.tiles * a.groups > 0x7fffffff || (int64_t)b.tiles * b.groups > 0x7fffffff) return FMLM_E_ARG;
-  const bool two = row_keys(p, w) <= kTwoTermKeys;
-  const void *dq = two ? (const void*)window_dq_kernel<T, D, true> : (const void*)window_dq_kernel<T, D, false>;
-  const void* const dkv = (const void*)window_dkv_kernel<T, D>;
-  static std::atomic<uint64_t> allowed[3];
-  int rc = allow_lds(dq, C::DQ_LDS, allowed[two]);
-  if (!rc) rc = allow_lds(dkv, C::DKV_LDS, allowed[2]);
+  const void *dq = (const void*)window_dq_kernel<T, D>, *dkv = (const void*)window_dkv_kernel<T, D>;
+  static std::atomic<uint64_t> allowed[2];
+  int rc = allow_lds(dq, C::DQ_LDS, allowed[0]);
+  if (!rc) rc = allow_lds(dkv, C::DKV_LDS, allowed[1]);
   if (rc) return rc;
-  if (two) hipLaunchKernelGGL((window_dq_kernel<T, D, true>), grid_of((int64_t)a.tiles * a.groups), dim3(kNW * 64), C::DQ_LDS, s, p, a, g);
-  else hipLaunchKernelGGL((window_dq_kernel<T, D, false>), grid_of((int64_t)a.tiles * a.groups), dim3(kNW * 64), C::DQ_LDS, s, p, a, g);
+  hipLaunchKernelGGL((window_dq_kernel<T, D>), grid_of((int64_t)a.tiles * a.groups), dim3(kNW * 64), C::DQ_LDS, s, p, a, g);
   hipLaunchKernelGGL((window_dkv_kernel<T, D>), grid_of((int64_t)b.tiles * b.groups), dim3(kNW * 64), C::DKV_LDS, s, p, b, g);
   return launch_status();
 }

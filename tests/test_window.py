@@ -1096,20 +1096,20 @@ def test_gradients(device, dtype, D, packed, window, sinks):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("D", [32, 64, 128, 256])
-@pytest.mark.parametrize("left", [1, 8, 40])
+@pytest.mark.parametrize("left,right", [(1, 0), (8, 0), (40, 0), (None, 0), (2, None)])
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
-def test_gradients_of_queries_that_see_few_keys(device, dtype, left, D):
+def test_gradients_of_queries_that_see_few_keys(device, dtype, left, right, D):
     """dq's root mean square error is that of its own rounding and of the forward's rounded probabilities in delta,
     simulated here: dS brings no further one (rounded to the type it adds a third).  The roundings are of other
     mantissas than the simulation's and a quarter of the error comes from rows of few keys: 10%."""
-    n, H, scale = 200, 16, D**-0.5
+    n, H, scale = 300, 16, D**-0.5
     g, q, k, v, meta = _inputs(device, dtype, [n], n, H, D, 36)
     q.requires_grad_()
-    out = flash_attn_mlm_window(q, k, v, H, meta, scale, window=(left, 0))
+    out = flash_attn_mlm_window(q, k, v, H, meta, scale, window=(left, right))
     do = _rand(g, out.shape, out.dtype)
     got = _f64(torch.autograd.grad(out, q, do)[0][0])
     low = lambda x: _f64(torch.from_numpy(x).to(TYPES[dtype]))  # noqa: E731
-    seen, err, ideal = ref.visible(0, n, n, left, 0, 0), 0.0, 0.0
+    seen, err, ideal = ref.visible(0, n, n, left, right, 0), 0.0, 0.0
     for h, dd in enumerate(_f64(do).reshape(H, n, D)):
         qq, kk, vv = (_f64(x[0, h]) for x in (q, k, v))
         want = ref.attend_backward(qq, kk, vv, seen, scale, dd)[0]
