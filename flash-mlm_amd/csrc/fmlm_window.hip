@@ -222,7 +222,9 @@ struct FwdCfg {
 //
 // P goes to the input type as an operand of the matrix cores, off by half a step; l adds up the same
 // rounded values (a product with ones), so that what all of a row's probabilities share cancels.  Scores, maxima,
-// l and O stay in 32 bits.
+// l and O stay in 32 bits.  The statistics for a backward (LSE) are of the sum as it is: from the rounded one,
+// every probability of a row of few keys would be off alike by a quarter of a rounding's square (dv of 1993
+// rows over 4 keys with a sink 1.52 times the error of its own rounding, so 1.44).
 //
 // Bound: fp16, 4 x 16 causal sequences of 4096 rows of 128: a window of 64 takes 66 us (268 MB, 81% of a
 // large copy's rate), all keys 231 us (1190 TFLOP/s, a large matrix product's rate).  Between them
@@ -232,7 +234,7 @@ struct FwdCfg {
 // 4 bits: 93 us for the 46 GFLOP of four chunks of 300 to 512 rows over 2000 to 4000 keys, 21% of the matrix
 // cores and 26% of the VALU (the conversions among it) at 1.2 waves a SIMD: 512 workgroups, of unequal length.
 // ---------------------------------------------------------------------------
-template <typename T, int D, int QB, bool FP4>
+template <typename T, int D, int QB, bool FP4, bool LSE>
 __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn_params p, const WinArgs a) {
   typedef FwdCfg<D, FP4> C;
   typedef typename Mfma<T>::v8 v8;
@@ -387,7 +389,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
 
   v8 qf[QB][C::KC];
   f32x4 o[C::NDB][QB], lsum[QB];
-  float m[QB], mx[QB];
+  float m[QB], mx[QB], lx[QB];  // lx (LSE): the lane's part of the sum of the probabilities as they are
   f32x4 sa[NKB][QB], sb[NKB][QB];
   v8 ones;
 #pragma unroll
@@ -444,8 +446,10 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
     auto exp_pair = [&](int pi) {
       const int qb = pi / (2 * NKB), kb = (pi >> 1) % NKB, r = (pi & 1) * 2;
       if (r == 0) pin(sc[kb][qb]);
-      uint32_t w = pack2<T>(fast_exp2(fmaf(sc[kb][qb][r], c, ref[qb])), fast_exp2(fmaf(sc[kb][qb][r + 1], c, ref[qb])));
+      const float e0 = fast_exp2(fmaf(sc[kb][qb][r], c, ref[qb])), e1 = fast_exp2(fmaf(sc[kb][qb][r + 1], c, ref[qb]));
+      uint32_t w = pack2<T>(e0, e1);
       pin(w);
+      if constexpr (LSE) lx[qb] += e0 + e1;
       pf[kb >> 1][qb][(kb & 1) * 2 + (pi & 1)] = w;
     };
     auto max_step = [&](int k) {
@@ -538,6 +542,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
           const float alpha = mn == -INFINITY ? 1.f : fast_exp2(m[qb] - mn);
           m[qb] = mn;
           lsum[qb] *= alpha;
+          if constexpr (LSE) lx[qb] *= alpha;
 #pragma unroll
           for (int db = 0; db < C::NDB; ++db) o[db][qb] *= alpha;
         }
@@ -574,6 +579,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     m[qb] = -INFINITY;
+    lx[qb] = 0.f;
     lsum[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int db = 0; db < C::NDB; ++db) o[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -652,7 +658,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
 
   // a row's result: a part's record (O, m, l), or the output
   float* const rec = a.records + (((int64_t)(a.tiles - 1 - tile) * a.groups + g) * a.parts + part) * a.rec_rows * (D + 4);
-  auto put = [&](int qb, const f32x4 (&x)[C::NDB], float mrow, float l) {
+  auto put = [&](int qb, const f32x4 (&x)[C::NDB], float mrow, float l, float lrow) {
     const int row = (wave * QB + qb) * 16 + l16;
     if (row >= rows) return;
     if (parts > 1) {
@@ -666,7 +672,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     if (p.lse && gq == 0)
-      p.lse[(int64_t)s.h * p.total_q + s.q0 + row0 + row] = l > 0.f ? mrow + __log2f(l) : l != l ? l : INFINITY;
+      p.lse[(int64_t)s.h * p.total_q + s.q0 + row0 + row] = lrow > 0.f ? mrow + __log2f(lrow) : lrow != lrow ? lrow : INFINITY;
     const int64_t off = row_at(p.o_layout, s.b, s.h, s.q0, row0 + row, p.o_sb, p.o_sh, p.o_sn);
 #pragma unroll
     for (int db = 0; db < C::NDB; ++db) {
@@ -694,7 +700,11 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
 #pragma unroll
       for (int r = 0; r < 4; ++r) bad = fmaf(x[db][r], 0.f, bad);
     }
-    put(qb, x, m[qb], lsum[qb][0]);
+    if constexpr (LSE) {
+      lx[qb] += __shfl_xor(lx[qb], 16);
+      lx[qb] += __shfl_xor(lx[qb], 32);
+    }
+    put(qb, x, m[qb], lsum[qb][0], LSE ? lx[qb] : lsum[qb][0]);
   }
   // Values that are not finite in keys that a row does not see have reached it as 0 inf.  If there may
   // be any, the rows are computed again, a tile and a block of rows at a time, key by key.
@@ -762,7 +772,7 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
       }
       __syncthreads();
     }
-    put(qb, x, mr, l);
+    put(qb, x, mr, l, l);
   }
 }
 
@@ -1608,12 +1618,12 @@ void merge_of(FwdLaunch& f) {
   f.merge[0] = (const void*)window_merge_kernel<T, D, 1>;
   f.merge[1] = (const void*)window_merge_kernel<T, D, 256 / (D / 8)>;
 }
-template <typename T, int D, int QB, bool FP4>
+template <typename T, int D, int QB, bool FP4, bool LSE = false>
 FwdLaunch fwd_of() {
   static std::atomic<uint64_t> allowed;
   FwdLaunch f;
   f.allowed = &allowed;
-  f.fn = (const void*)window_fwd_kernel<T, D, QB, FP4>;
+  f.fn = (const void*)window_fwd_kernel<T, D, QB, FP4, LSE>;
   merge_of<T, D>(f);
   f.bq = kNW * QB * 16;
   f.lds = FwdCfg<D, FP4>::LDS;
@@ -1621,8 +1631,8 @@ FwdLaunch fwd_of() {
   return f;
 }
 template <typename T, int D, int QB>
-FwdLaunch fwd_of(bool fp4) {
-  return fp4 ? fwd_of<T, D, QB, true>() : fwd_of<T, D, QB, false>();
+FwdLaunch fwd_of(bool fp4, bool lse) {
+  return fp4 ? fwd_of<T, D, QB, true>() : lse ? fwd_of<T, D, QB, false, true>() : fwd_of<T, D, QB, false>();
 }
 template <typename T, int D>
 FwdLaunch few_of() {
@@ -1658,11 +1668,12 @@ FwdLaunch pick_fwd(const fmlm_attn_params& p, const fmlm_window& w) {
   // and end (4 x 16 x 512 rows over 4096 keys 84 : 77 at D = 64, 78 : 63 at 32, over 255 of 4000 16 : 18.6
   // and 13 : 14.8).
   const bool wide4 = fp4 && tall && tiles > kWideTiles;
+  const bool lse = p.lse;
   switch (p.D) {
-    case 32: return wide4 ? fwd_of<T, 32, 2, true>() : fwd_of<T, 32, 1>(fp4);
-    case 64: return wide4 ? fwd_of<T, 64, 2, true>() : fwd_of<T, 64, 1>(fp4);
-    case 128: return wide ? fwd_of<T, 128, 2, false>() : wide4 ? fwd_of<T, 128, 2, true>() : fwd_of<T, 128, 1>(fp4);
-    default: return fwd_of<T, 256, 1>(fp4);  // (two blocks of 16 rows spill)
+    case 32: return wide4 ? fwd_of<T, 32, 2, true>() : fwd_of<T, 32, 1>(fp4, lse);
+    case 64: return wide4 ? fwd_of<T, 64, 2, true>() : fwd_of<T, 64, 1>(fp4, lse);
+    case 128: return wide || wide4 ? fwd_of<T, 128, 2>(fp4, lse) : fwd_of<T, 128, 1>(fp4, lse);
+    default: return fwd_of<T, 256, 1>(fp4, lse);  // (two blocks of 16 rows spill)
   }
 }
 FwdLaunch pick_fwd(const fmlm_attn_params& p, const fmlm_window& w) {

@@ -1124,6 +1124,33 @@ def test_gradients_of_queries_that_see_few_keys(device, dtype, left, right, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_gradients_of_keys_and_values_that_few_share(device, dtype, D):
+    """dk's and dv's root mean square errors over windows of four keys are those of P and dS rounded to the type and
+    of their own rounding: the row statistics bring no further one (that of the forward's rounded P adds 7%).  The
+    roundings are the simulation's own but for fp32's part; 4% as for the keys above."""
+    n, H, scale, window, sinks = 600, 16, D**-0.5, (2, 0), 1
+    g, q, k, v, meta = _inputs(device, dtype, [n], n, H, D, 37)
+    k.requires_grad_()
+    v.requires_grad_()
+    out = flash_attn_mlm_window(q, k, v, H, meta, scale, window=window, sinks=sinks)
+    do = _rand(g, out.shape, out.dtype)
+    got = [_f64(x)[0] for x in torch.autograd.grad(out, (k, v), do)]
+    low = lambda x: _f64(torch.from_numpy(x).to(TYPES[dtype]))  # noqa: E731
+    seen, err, ideal = ref.visible(0, n, n, *window, sinks), np.zeros(2), np.zeros(2)
+    for h, dd in enumerate(_f64(do).reshape(H, n, D)):
+        qq, kk, vv = (_f64(x[0, h]) for x in (q, k, v))
+        _, dk, dv = ref.attend_backward(qq, kk, vv, seen, scale, dd)
+        o, P = ref.attend(qq, kk, vv, seen, scale)
+        dS = P * (dd @ vv.T - (dd * o).sum(1)[:, None])
+        for i, (want, best) in enumerate(((dk, low(low(dS).T @ qq * scale)), (dv, low(low(P).T @ dd)))):
+            err[i] += ((got[i][h] - want) ** 2).sum()
+            ideal[i] += ((best - want) ** 2).sum()
+    assert (err <= 1.04**2 * ideal).all(), (err / ideal) ** 0.5
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("size", [2.0**-10, 2.0**9])
 @pytest.mark.parametrize("D", [32, 128])
 def test_gradients_of_small_and_large_losses_in_fp16(device, D, size):
