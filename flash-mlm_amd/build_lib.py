@@ -36,7 +36,7 @@ COMMON_FLAGS = [
     "-Wno-unused-function",
     "-Wno-unused-variable",
     "-Wno-unused-but-set-variable",
-    # no packed fp32 instructions in device code (wrong results seen on this pool)
+    # no packed fp32 instructions in device code (some of their forms gave wrong results)
     "-Xclang",
     "-target-feature",
     "-Xclang",

@@ -17,7 +17,7 @@
 // lanes, 8 elements each, so that a block's maximum is a maximum of four lanes; a thread keeps its
 // row's angles over its heads.  The partner of a half-split pair comes from its lane, as read.
 // Measured: 589 MB of fp16 prompts 115 us, a large copy's rate; 20 thousand tokens with 12 heads
-// of 64 stored in 4 bits 47 us, their values made again 19 us (together at 82% of that rate); 64 tokens with 16
+// of 64 stored in 4 bits 47 us, their values made again 19 us (together at 83% of that rate); 64 tokens with 16
 // heads of 128 4.9 us.
 #include "fmlm_common.h"
 

@@ -222,17 +222,19 @@ struct FwdCfg {
 //
 // P goes to the input type as an operand of the matrix cores, off by half a step; l adds up the same
 // rounded values (a product with ones), so that what all of a row's probabilities share cancels.  Scores, maxima,
-// l and O stay in 32 bits.  The statistics for a backward (LSE) are of the sum as it is: from the rounded one,
-// every probability of a row of few keys would be off alike by a quarter of a rounding's square (dv of 1993
-// rows over 4 keys with a sink 1.52 times the error of its own rounding, so 1.44).
+// l and O stay in 32 bits.  The statistics for a backward (LSE) are of the sum as it is: with the rounded one
+// all of a row's probabilities would be off alike there by the mean rounding of its keys, which counts where they are
+// few (dv over 4 keys with a sink 1.52 times the error of its own rounding, so 1.44).
 //
-// Bound: fp16, 4 x 16 causal sequences of 4096 rows of 128: a window of 64 takes 66 us (268 MB, 81% of a
-// large copy's rate), all keys 231 us (1190 TFLOP/s, a large matrix product's rate).  Between them
-// the two add up (1024 keys: 150 us; 31% of the matrix cores, 37% of the VALU), as workgroups read their first
-// tiles and rows while few others compute; another order of the tiles, staggered starts or more fragments in
-// flight changed nothing.  Single rows over 1024 keys of a paged context (64 users) are at a copy's rate.
-// 4 bits: 93 us for the 46 GFLOP of four chunks of 300 to 512 rows over 2000 to 4000 keys, 21% of the matrix
+// Bound (times of a warm card, after 0.4 s of the same calls): fp16, 4 x 16 causal sequences of 4096 rows of 128:
+// a window of 64 takes 73 us (268 MB, 73% of a large copy's rate), all keys 283 us (970 TFLOP/s, 73% of a
+// large matrix product's rate).  Between them the two add up (1024 keys: 169 us; for a backward 30% of the matrix
+// cores, 39% of the VALU), as workgroups read their first tiles and rows while few others compute; another order of
+// the tiles, staggered starts or more fragments in flight changed nothing.  Single rows over 1024 keys of a paged
+// context (64 users) are at a copy's rate.
+// 4 bits: 87 us for the 44 GFLOP of four chunks of 300 to 512 rows over 2000 to 4000 keys, 21% of the matrix
 // cores and 26% of the VALU (the conversions among it) at 1.2 waves a SIMD: 512 workgroups, of unequal length.
+// (Pairs of figures below are of both forms side by side, some on a card that was not warm: up to 20% longer.)
 // ---------------------------------------------------------------------------
 template <typename T, int D, int QB, bool FP4, bool LSE>
 __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn_params p, const WinArgs a) {
@@ -784,8 +786,9 @@ __global__ __launch_bounds__(kNW * 64, 2) void window_fwd_kernel(const fmlm_attn
 // that order too.  V is converted the same way into a wave's own 32 rows of LDS and read back
 // transposed.  A tile's registers are loaded again as soon as they have been converted.  The four
 // waves' sums meet in LDS at the end.  Bound by memory: 64 users over 500 to 8192 keys of 16 heads, D = 128, 633 MB of
-// codes and scales in 128 us, 96% of a large copy's rate; the same through window_fwd_kernel's
+// codes and scales in 127 us, 97% of a large copy's rate; the same through window_fwd_kernel's
 // shared tiles 226 us with 4096 keys each, here 114 (16 rows a sequence: 73 and 35).
+// A wave whose rows come out not finite walks its tiles once more, key by key (see there).
 // ---------------------------------------------------------------------------
 constexpr int kFewRows = 16;
 
@@ -1177,13 +1180,16 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const fmlm_attn_param
 // o's rounding, the same for all of a row's keys, would be the largest error of dq and dk (1.55 times
 // the plain form's in fp16, with o_low 1.4).  What is left in it of the rounding of the forward's P goes
 // for dK: the dq kernel adds up what each row's dS, unrounded, lacks to a sum of 0.  dq itself has the delta that is
-// not yet so exact; where that counts (TWO: rows of few keys) its dS goes in two terms.  dq by query tiles, then dK and dV by key tiles, which repeats S
-// and dP (2 of 7 products) and needs no atomics: the same bits every time.
+// not yet so exact; where that counts (TWO: rows of few keys) its dS goes in two terms.  dS is held without its
+// scale: in fp16 P (do V^T - delta) ends at 65504, beyond which gradients are not finite, as beyond a loss scale's
+// range.  dq by query tiles, then dK and dV by key tiles, which repeats S and dP (2 of 7 products) and needs no
+// atomics: the same bits every time.
 //
-// Bound (fp16, 4 x 16 sequences of 2000 to 4096 rows of 128, windows of 1024): dq 217 us, 37% of the matrix
-// cores and 41% of the VALU; dK / dV 314 us, 33% and 40%, with 38% of LDS: its 16 keys a wave take a fragment
-// from LDS for each product.  32 keys a wave halve that and leave one wave a SIMD: 404 us.  At D = 256 dK
-// / dV spill 12 registers with two waves a SIMD, 107 us for 8 x 8 x 300 to 1024 rows with windows of 511 (one wave a SIMD and no spills: 5% more).
+// Bound (fp16, 4 x 16 sequences of 2000 to 4096 rows of 128, windows of 1024, a warm card): dq 184 us, 37% of the
+// matrix cores and 43% of the VALU; dK / dV 259 us, 33% and 39%, with 37% of LDS: its 16 keys a wave take a fragment
+// from LDS for each product.  32 keys a wave halve that and leave one wave a SIMD (404 us for 318 side by side).
+// At D = 256 dK / dV spill 12 registers with two waves a SIMD, 100 us for 8 x 8 x 300 to 1024 rows with windows of
+// 511 (one wave a SIMD and no spills: 5% more).
 // ---------------------------------------------------------------------------
 template <int D>
 struct BwdCfg {
@@ -1665,8 +1671,11 @@ FwdLaunch pick_fwd(const fmlm_attn_params& p, const fmlm_window& w) {
   // rows 12 : 17; 256 rows over 511 of 8192 keys 14 : 18, over 16384 keys 75 : 54).
   const bool wide = !fp4 && tall && units * (unsplit(p, w) ? 1 : std::max<int64_t>(tiles / kMinPartTiles, 1)) >= kFill;
   // In 4 bits they share its conversion too: at every D, but for short walks, whose workgroups are all start
-  // and end (4 x 16 x 512 rows over 4096 keys 84 : 77 at D = 64, 78 : 63 at 32, over 255 of 4000 16 : 18.6
-  // and 13 : 14.8).
+  // and end.  (us with 64 : 128 rows; 4 x 16 x 512 rows over 128, 512, 1024 and 4096 context keys: D = 128 26 : 34,
+  // 37 : 40, 50 : 49, 134 : 99; D = 64 19 : 23, 26 : 28, 37 : 35, 100 : 72; D = 32 17 : 21, 24 : 25, 33 : 30, 87 : 61.  2 x 16 x
+  // 2048 rows gain at all of them, D = 128 119 : 82 to 337 : 207, a few workgroups at none: 8 x 100 rows 13 : 16 to
+  // 21 : 24.  So the border of 10 tiles, a call's own keys counted, is about right for 512 rows between 500 and
+  // 1000 keys.)
   const bool wide4 = fp4 && tall && tiles > kWideTiles;
   const bool lse = p.lse;
   switch (p.D) {
@@ -1737,9 +1746,10 @@ WinArgs win_args(const fmlm_attn_params& p, const fmlm_window& w, int rows) {
 // single rows, D = 64, 66 / 52 / 53; 256 rows, D = 256, 88 / 68 / 97; the 512 against 256 and 1024 of
 // 128-row tiles: 85 : 116 : 111), each with kMinPartTiles tiles; of few rows in 4 bits, where the four waves
 // walk apart, with kFewTiles (16 rows, 8192 keys: 16.4 with 4, 13.8 with 8, 15.8 with 16).  Between 512 and 2048
-// units of those, parts of 32 tiles even out the last round (64 users with 4096 keys: 119 whole, 114 in
-// two, 121 in four; with 500 to 8192 keys, in two 131, in four 128); smaller ones cost more than that (32 x 4
-// rows, 1000 keys: 18.5 whole, 27 in two).
+// units of those, parts of 32 tiles even out sequences of different lengths and cost where all are as long, which
+// is not known here (single rows of 16 heads of 128, whole : as planned; 512 to 8192 keys: 32 users 81 : 70, 48 103 :
+// 99, 64 133 : 125, 96 178 : 178, 127 233 : 235; 8192 keys each 107 : 115, 157 : 161, 213 : 211, 295 : 306, 394 : 405; 4096
+// each 53 : 62, 84 : 89, 113 : 113, 156 : 162, 210 : 221); smaller parts cost more (1024 keys, 32 users: 19 whole, 26 in two).
 void plan_parts(const fmlm_attn_params& p, const fmlm_window& w, const FwdLaunch& f, WinArgs& a) {
   a.rec_rows = std::min(f.bq, longest(p));
   a.lg = f.lg;

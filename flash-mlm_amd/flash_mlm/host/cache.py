@@ -419,7 +419,7 @@ class InferenceCache:
     def paged_kv_values(self, layer_id: int | str) -> tuple[torch.Tensor, torch.Tensor | None]:
         """The pages of ``layer_id``'s paged context as values: (k, v) [H_kv, P, 64, D] of the entry's
         dtype (v None for MLA).  Of a 16-bit context the pools themselves, of a 4-bit one new
-        tensors, by one HIP launch each.  The block table says which pages are in use; the others hold
+        tensors, by one HIP launch for both.  The block table says which pages are in use; the others hold
         whatever their memory does."""
         entry = self._layer_kv.get(self._layer_key(layer_id))
         if entry is None:

@@ -308,8 +308,9 @@ def flash_attn_mlm_window(
 
     The context is the layer's packed, paged or 4-bit entry (none: no context), with
     ``context_index`` as in :func:`flash_attn_mlm_compressed`.  bf16 and fp16, D = 32, 64, 128 or 256,
-    no MLA.  Differentiable in q, k and v without a cached context, for finite inputs; gradients are
-    the same bits every time, those of padding rows zero.  With a context, inputs that
+    a finite scale, no MLA.  Differentiable in q, k and v without a cached context, for finite inputs (in
+    fp16 gradients are finite while |P (dO V^T - rowsum(dO O))| stays below 65504); gradients are
+    the same bits every time, those of padding rows zero.  With a context, inputs or cached rows that
     require grad raise ValueError (use ``torch.no_grad()``); with a forward-mode tangent always.  A
     call that is captured into a graph and takes leaves that require grad raises ValueError while
     outputs of earlier calls on them are alive.
