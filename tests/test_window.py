@@ -650,6 +650,77 @@ def test_more_workgroups_than_a_grid_has_in_x(device, fp4):
 
 
 @pytest.mark.gpu
+def test_calls_past_32_bits(device):
+    """Packed rows behind element 2^32 of q, k, v, the output and the gradients: the bits of the last sequence alone"""
+    H, D, n = 2, 256, 90
+    long = (1 << 32) // (H * D) + 1000
+    T = long + n
+    meta, alone = (build_pack_metadata(torch.tensor(x, device=device), max(x), 32) for x in ([long, n], [n]))
+    g = torch.Generator(device=device).manual_seed(20)
+    xs = [torch.randn((H * T, D), generator=g, device=device, dtype=torch.bfloat16).requires_grad_() for _ in range(3)]
+    do = torch.randn((H * T, D), generator=g, device=device, dtype=torch.bfloat16)
+    tail = lambda x: x.view(H, T, D)[:, long:].reshape(H * n, D).detach()  # noqa: E731
+    ys = [tail(x).requires_grad_() for x in xs]
+    a = flash_attn_mlm_window(*xs, H, meta, 0.07, window=(50, 3), sinks=2)
+    b = flash_attn_mlm_window(*ys, H, alone, 0.07, window=(50, 3), sinks=2)
+    assert torch.equal(tail(a), b)
+    want = torch.autograd.grad(b, ys, tail(do))
+    del b
+    assert all(torch.equal(tail(x), y) for x, y in zip(torch.autograd.grad(a, xs, do), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 90])
+@pytest.mark.parametrize("kind", ["paged", "packed"])
+def test_contexts_past_32_bits(device, kind, n):
+    """Context rows behind element 2^32: the bits of the same rows in a small context"""
+    H, D, P = 2, 256, 135000  # 2 * 135000 * 64 * 256 = 4.4e9 elements
+    lens, ctx = [n], [300]
+    g, q, k, v, meta = _inputs(device, "fp16", lens, n, H, D, 21)
+    small = _Layer(kind, "fp16", H, D, ctx, device, g)
+    run = lambda cache: flash_attn_mlm_window(q, k, v, H, meta, 0.07, window=(200, 3), sinks=2, inference_cache=cache, layer_id=0)  # noqa: E731
+    want = run(small.cache)
+    rows = [torch.zeros((H, P * PAGE, D), dtype=q.dtype, device=device) for _ in range(2)]
+    cache = InferenceCache()
+    if kind == "packed":
+        first = P * PAGE - 300
+        cache.prefill_kv_cache(0, k_cache=rows[0].view(-1, D), v_cache=rows[1].view(-1, D), total_context_len=P * PAGE,
+                               cu_seqlens_kv=torch.tensor([0, first, first + 300], dtype=torch.int32, device=device),
+                               context_batch_size=2, is_mla=False, num_heads=H, head_dim=D)
+        at = list(range(first, first + 300))
+        index = dict(context_index=torch.tensor([1], device=device))
+        run = lambda cache: flash_attn_mlm_window(q, k, v, H, meta, 0.07, window=(200, 3), sinks=2, inference_cache=cache,  # noqa: E731
+                                                  layer_id=0, **index)
+    else:
+        pages = [P - 1, P - 7, P - 2, P - 3, P - 5]
+        cache.prefill_paged_kv_cache(0, k_pages=rows[0].view(H, P, PAGE, D), v_pages=rows[1].view(H, P, PAGE, D),
+                                     block_table=torch.tensor([pages], device=device), context_lens=torch.tensor([300]),
+                                     is_mla=False, num_heads=H, head_dim=D)
+        at = [pages[j // PAGE] * PAGE + j % PAGE for j in range(300)]
+    for x, y in zip(rows, small.rows):
+        x[:, at] = y[:, small.at[0]]
+    # (key ranges may be cut otherwise: the larger context's rule knows its rows only)
+    got = run(cache)
+    _check(got, q, k, v, lens, ctx, small, (200, 3), 2, 0.07, "fp16")
+    assert (got.float() - want.float()).abs().max() <= 4 * 2.0**-11 * want.float().abs().max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_padding_rows_stay_out_of_gradients(device, D):
+    """Rows of a padded batch behind its sequences that are not finite"""
+    lens, N, H = [70, 0, 129, 1], 140, 2
+    g, q, k, v, meta = _inputs(device, "bf16", lens, N, H, D, 22)
+    do = _rand(g, (H * sum(lens), D), q.dtype)
+    run = lambda xs: torch.autograd.grad(flash_attn_mlm_window(*xs, H, meta, 0.1, window=(40, 9), sinks=3), xs, do)  # noqa: E731
+    want = run([x.clone().requires_grad_() for x in (q, k, v)])
+    for x in (q, k, v):
+        for b, n in enumerate(lens):
+            x[b, :, n:] = float("nan")
+    assert all(torch.equal(a, b) for a, b in zip(run([x.requires_grad_() for x in (q, k, v)]), want))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("N", [1, 3])
 def test_positions_far_apart(device, N):
     """Rows whose positions are 2^22 elements apart, as in a [N, B, H, D] batch of many sequences"""
@@ -1369,6 +1440,39 @@ def test_calls_in_a_graph(device, kind):
         got = [x.clone() for x in outs]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, run()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [1, 7])
+@pytest.mark.parametrize("kind", ["paged", "fp4"])
+def test_split_calls_in_two_graphs(device, kind, N):
+    """Two graphs of calls whose key ranges are split, replayed in turn on other rows and lengths: records of their own"""
+    lens, H, D = [N, 1], 2, 128
+    g, q, k, v, meta = _inputs(device, "bf16", lens, N, H, D, 27)
+    layer = _Layer(kind, "bf16", H, D, [3000, 2000], device, g)
+    q2 = _rand(g, q.shape, q.dtype)
+    run = lambda x: flash_attn_mlm_window(x, k, v, H, meta, 0.1, inference_cache=layer.cache, layer_id=0)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(q)
+    torch.cuda.current_stream().wait_stream(side)
+    assert _kept_bytes(meta) > 0
+    graphs, outs = [], []
+    for x in (q, q2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run(x))
+        graphs.append(graph)
+    for i in range(4):
+        for x in (q, q2, k, v):
+            x.normal_()
+        layer.cache.layer_entry(0).cu_seqlens_kv.copy_(torch.tensor([0, 900 * i, 900 * i + 600 * i], device=device))
+        for j in (i & 1, 1 - (i & 1)):
+            graphs[j].replay()
+        got = [x.clone() for x in outs]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, run(x)) for a, x in zip(got, (q, q2)))
 
 
 @pytest.mark.gpu
